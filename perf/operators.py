@@ -290,8 +290,10 @@ def _logsumexp(x):
 
 
 def _lse_plain(s):
+    """log sum exp of the logits over the temperature, and of the logits where labels need it (0 where not)."""
     z = s["logits"].float()
-    return torch.stack([_logsumexp(z / s["case"]["temperature"]), _logsumexp(z)], 1)
+    soft = _logsumexp(z / s["case"]["temperature"])
+    return torch.stack([soft, _logsumexp(z) if s["case"]["hard"] else torch.zeros_like(soft)], 1)
 
 
 def _teacher(s):
@@ -477,7 +479,7 @@ def _exact_distill(s, c):
     temperature, hard = c["temperature"], c["hard"]
     z = s["logits"].double()
     p = torch.softmax(s["teacher_logits"].double() / temperature, 1)
-    soft, plain = torch.log_softmax(z / temperature, 1), torch.log_softmax(z, 1)
+    soft, plain = torch.log_softmax(z / temperature, 1), torch.log_softmax(z, 1) if hard else None
     ids = s["teacher_ids"].long()
     r = {}
     if c["kind"] != "distill_backward":
@@ -485,7 +487,7 @@ def _exact_distill(s, c):
         if hard:
             losses = losses - hard * torch.take_along_dim(plain, s["labels"][:, None], 1).squeeze(1)
         r["losses"] = losses
-        r["lse"] = torch.stack([torch.logsumexp(z / temperature, 1), torch.logsumexp(z, 1)], 1)
+        r["lse"] = torch.stack([torch.logsumexp(z / temperature, 1), torch.logsumexp(z, 1) * (hard > 0)], 1)
     if c["kind"] != "distill_loss":
         wanted = torch.zeros_like(z).scatter_(1, ids, p)
         g = (1 - hard) * temperature * (soft.exp_() - wanted)
