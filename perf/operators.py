@@ -200,12 +200,12 @@ def prepare(case, seed):
     values, ids = teacher.topk(top, dim=1)
     s["teacher_logits"], s["teacher_ids"] = values.to(_TYPE[c["logits"]]), ids.to(torch.int32)
     s["labels"] = ids[:, 0].contiguous() if c["hard"] else None
-    s["losses"], s["lse"] = empty(rows), empty(rows, 2)
+    s["losses"], s["stats"] = empty(rows), empty(rows, 4)
     s["grad"] = empty(rows, vocab, dtype=_TYPE[c["logits"]])
     s["losses_grad"] = torch.rand(rows, generator=g, device="cuda").mul_(64.0)  # a loss scaled for F16
     s["losses_grad"][rows - rows // 16:] = 0.0                                   # rows of padding
     if c["kind"] == "distill_backward":
-        s["lse"] = _lse_plain(s)
+        s["stats"] = _stats_plain(s)
     return s
 
 
@@ -289,11 +289,14 @@ def _logsumexp(x):
     return top.squeeze(-1) + torch.log(torch.exp(x - top).sum(-1))
 
 
-def _lse_plain(s):
-    """log sum exp of the logits over the temperature, and of the logits where labels need it (0 where not)."""
-    z = s["logits"].float()
-    soft = _logsumexp(z / s["case"]["temperature"])
-    return torch.stack([soft, _logsumexp(z) if s["case"]["hard"] else torch.zeros_like(soft)], 1)
+def _stats_plain(s):
+    """A row's maximum, its log sum exp beside that over the temperature, and without the temperature where labels need it (0 where not)."""
+    z, c = s["logits"].float(), s["case"]
+    top = z.amax(-1, keepdim=True)
+    z = z - top
+    soft = torch.log(torch.exp(z / c["temperature"]).sum(-1))
+    hard = torch.log(torch.exp(z).sum(-1)) if c["hard"] else torch.zeros_like(soft)
+    return torch.stack([top.squeeze(-1), soft, hard, torch.zeros_like(soft)], 1)
 
 
 def _teacher(s):
@@ -305,21 +308,22 @@ def _teacher(s):
 def _distill_plain(s):
     c = s["case"]
     temperature, hard = c["temperature"], c["hard"]
-    z, ids = s["logits"].float(), s["teacher_ids"].long()
-    lse = s["lse"] if c["kind"] == "distill_backward" else _lse_plain(s)
+    ids = s["teacher_ids"].long()
+    stats = s["stats"] if c["kind"] == "distill_backward" else _stats_plain(s)
+    z = s["logits"].float() - stats[:, :1]
     p, log_p = _teacher(s)
     r = {}
     if c["kind"] != "distill_backward":
-        log_q = z.gather(1, ids) / temperature - lse[:, :1]
+        log_q = z.gather(1, ids) / temperature - stats[:, 1:2]
         losses = (1 - hard) * temperature ** 2 * (p * (log_p - log_q)).sum(1)
         if hard:
-            losses = losses + hard * (lse[:, 1] - z.gather(1, s["labels"][:, None])[:, 0])
-        r = {"losses": losses, "lse": lse}
+            losses = losses + hard * (stats[:, 2] - z.gather(1, s["labels"][:, None])[:, 0])
+        r = {"losses": losses, "stats": stats}
     if c["kind"] != "distill_loss":
         weight = s["losses_grad"][:, None]
-        g = torch.exp(z / temperature - lse[:, :1]).scatter_add_(1, ids, -p) * ((1 - hard) * temperature)
+        g = torch.exp(z / temperature - stats[:, 1:2]).scatter_add_(1, ids, -p) * ((1 - hard) * temperature)
         if hard:
-            q = torch.exp(z - lse[:, 1:])
+            q = torch.exp(z - stats[:, 2:3])
             g = g + hard * q.scatter_add_(1, s["labels"][:, None], torch.full_like(weight, -1.0))
         r["grad"] = (g * weight).to(s["grad"].dtype)
     return r
@@ -387,15 +391,15 @@ def _own(s):
         return r
     options = {"labels": v["labels"], "temperature": c["temperature"], "hard_weight": c["hard"]}
     if kind == "distill_backward":
-        gpu.distill_loss_backward(v["logits"], v["teacher_ids"], v["teacher_logits"], v["lse"], v["grad"],
+        gpu.distill_loss_backward(v["logits"], v["teacher_ids"], v["teacher_logits"], v["stats"], v["grad"],
                                   losses_grad=v["losses_grad"], **options)
         return {"grad": s["grad"]}
     if kind == "distill_loss":
-        gpu.distill_loss(v["logits"], v["teacher_ids"], v["teacher_logits"], v["losses"], lse=v["lse"], **options)
-        return {"losses": s["losses"], "lse": s["lse"]}
-    gpu.distill_loss(v["logits"], v["teacher_ids"], v["teacher_logits"], v["losses"], lse=v["lse"], grad=v["grad"],
+        gpu.distill_loss(v["logits"], v["teacher_ids"], v["teacher_logits"], v["losses"], stats=v["stats"], **options)
+        return {"losses": s["losses"], "stats": s["stats"]}
+    gpu.distill_loss(v["logits"], v["teacher_ids"], v["teacher_logits"], v["losses"], stats=v["stats"], grad=v["grad"],
                      losses_grad=v["losses_grad"], **options)
-    return {"losses": s["losses"], "lse": s["lse"], "grad": s["grad"]}
+    return {"losses": s["losses"], "stats": s["stats"], "grad": s["grad"]}
 
 
 def run(state):
@@ -487,7 +491,9 @@ def _exact_distill(s, c):
         if hard:
             losses = losses - hard * torch.take_along_dim(plain, s["labels"][:, None], 1).squeeze(1)
         r["losses"] = losses
-        r["lse"] = torch.stack([torch.logsumexp(z / temperature, 1), torch.logsumexp(z, 1) * (hard > 0)], 1)
+        top = z.amax(1)
+        r["stats"] = torch.stack([top, torch.logsumexp(z / temperature, 1) - top / temperature,
+                                  (torch.logsumexp(z, 1) - top) * (hard > 0), torch.zeros_like(top)], 1)
     if c["kind"] != "distill_loss":
         wanted = torch.zeros_like(z).scatter_(1, ids, p)
         g = (1 - hard) * temperature * (soft.exp_() - wanted)
