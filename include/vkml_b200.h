@@ -307,6 +307,125 @@ int b200_tape_enable_graphs(b200_tape* tape, int on);
 int b200_tape_stats(b200_tape* tape, uint64_t* steps, uint64_t* graph_launches, uint64_t* graph_captures);
 void b200_tape_destroy(b200_tape* tape);
 
+/* -- operators of language-model training (no counterpart in vkML, which composes them of many
+ *    nodes, each with a result of its own) --
+ *
+ * Each call queues its kernels on the context's stream, after everything submitted before it, and
+ * returns once they are ordered.  Sums, softmax statistics and norms are held in 32 bits whatever
+ * the tensors' types; a result is rounded once.  Repeated calls give identical bytes.
+ *
+ * Tensors are strided views.  A tensor of rows has rank 1, 2 or 3: the rows lie along its last
+ * axis, which has unit stride; the axes in front may have any strides (0 in an input: a row that
+ * stands for many).  Tensors that share rows have the same extents.  A result's elements are
+ * distinct, and a result overlaps no other tensor of the call unless its comment says so.  A tensor whose
+ * `data` is NULL is absent, where its comment allows that.  Up to 2^31 - 1 rows.  Whatever does
+ * not fit is refused before anything is queued.  Empty tensors are valid.
+ *
+ * Scratch: `workspace` is device memory of the caller, 256-byte aligned, of at least the bytes that the _workspace
+ * call of the same arguments tells; NULL takes the context's own, which every call shares: a caller that captures
+ * calls into CUDA graphs of its own, to be replayed beside other work, gives each graph a workspace
+ * (a call that would have to grow the context's own while its stream is captured is refused). */
+
+/* rows[t] = scale * table[ids[t]] -- and backward, table = scale * (the sum of the rows of each
+ * id), rows without a token zero, or, with B200_ACCUMULATE, added to what table holds, where rows without a token
+ * keep their bytes. */
+#define B200_ACCUMULATE 1u
+typedef struct b200_embedding_args {
+    b200_tensor table;   /* [V, D], F32 or F16: read by b200_embedding, written by its backward */
+    b200_tensor ids;     /* I64 or I32, any strides; an id outside [0, V) is an index error at the next
+                            synchronisation: its row reads as zeros, its gradient goes nowhere */
+    b200_tensor rows;    /* ids' extents and D, F32 or F16 whatever the table's type */
+    float scale;
+    uint32_t flags;      /* B200_ACCUMULATE (backward only) */
+    int64_t padding_id;  /* backward: tokens of this id have no gradient; negative: none */
+    void* workspace;     /* backward only */
+    size_t workspace_bytes;
+} b200_embedding_args;
+int b200_embedding(b200_ctx* ctx, const b200_embedding_args* args);
+int b200_embedding_backward(b200_ctx* ctx, const b200_embedding_args* args);
+int b200_embedding_backward_workspace(const b200_embedding_args* args, size_t* nbytes);
+
+/* What stands between two blocks of a residual network.  With N the norm of a row,
+ *     u      = N(branch) * post_weight + post_bias        (without B200_NORM_POST: u = branch)
+ *     out    = residual_scale * residual + branch_scale * gate * u
+ *     normed = N(out) * pre_weight + pre_bias
+ * RMS norm: N(x) = x / sqrt(mean(x^2) + eps); layer norm: N(x) = (x - mean) / sqrt(var + eps).
+ * `normed` is that of `out` before its rounding.  Widths up to 16384. */
+#define B200_NORM_RMS 0
+#define B200_NORM_LAYER 1
+#define B200_NORM_POST 1u
+typedef struct b200_block_norm_args {
+    b200_tensor residual;  /* rows; absent: the branch alone */
+    b200_tensor branch;    /* rows; absent: the residual alone */
+    b200_tensor out;       /* rows of the residual's type; may be absent; may lie exactly on residual or branch */
+    b200_tensor normed;    /* rows of the branch's type; may be absent; may lie exactly on residual or branch */
+    b200_tensor stats;     /* [number of rows, 4], F32, dense: mean and 1/sqrt of the branch's norm, mean and
+                              1/sqrt of out's (0 for what is not computed); backward needs it; may be absent */
+    b200_tensor post_weight, post_bias, pre_weight, pre_bias; /* [D] dense; absent: 1 and 0 */
+    b200_tensor gate;      /* [D], or [G, D] where row r has gate r / (rows / G); absent: 1.  Weights, biases and
+                              gate have one type, F32 or F16 */
+    float residual_scale, branch_scale, eps;
+    int32_t kind;          /* B200_NORM_RMS, B200_NORM_LAYER */
+    uint32_t flags;        /* B200_NORM_POST */
+} b200_block_norm_args;    /* (residual, branch): (F32, F32), (F16, F16) or (F32, F16); one absent: its type is that of the tensor beside it */
+int b200_block_norm(b200_ctx* ctx, const b200_block_norm_args* args);
+
+/* Gradients of b200_block_norm from those of its two results.  Every gradient may be absent. */
+typedef struct b200_block_norm_grad_args {
+    b200_tensor out, branch, stats;            /* as the forward call had and left them */
+    b200_tensor out_grad, normed_grad;         /* rows of out's and of the branch's type; either may be absent (zero) */
+    b200_tensor post_weight, post_bias, gate, pre_weight;
+    b200_tensor residual_grad;                 /* rows of out's type; may lie exactly on a tensor of rows that is read */
+    b200_tensor branch_grad;                   /* rows of the branch's type; the same */
+    b200_tensor post_weight_grad, post_bias_grad, pre_weight_grad, pre_bias_grad; /* [D] */
+    b200_tensor gate_grad;                     /* the gate's extents; these five have one type, F32 or F16, dense */
+    float residual_scale, branch_scale;
+    int32_t kind;
+    uint32_t flags;
+    void* workspace;
+    size_t workspace_bytes;
+} b200_block_norm_grad_args;
+int b200_block_norm_backward(b200_ctx* ctx, const b200_block_norm_grad_args* args);
+int b200_block_norm_backward_workspace(const b200_block_norm_grad_args* args, size_t* nbytes);
+
+/* Distillation from a teacher's top logits, with a share of cross-entropy.  For a row z of logits, the teacher's
+ * logits t at the columns k, temperature T and hard weight c,
+ *     p    = softmax(t / T),  q = softmax(z / T)
+ *     soft = T^2 * sum over k of p_k * (log p_k - log q_k)      (0 in a row without a teacher's entry)
+ *     hard = log sum exp z - z[label]                           (0 in a row without a label)
+ *     loss = (1 - c) * soft + c * hard
+ *     grad = grad_scale * losses_grad * d loss / d z            (zeros where that factor is 0, whatever z holds)
+ * A column that appears twice counts twice.  A part whose weight is 0 is not computed.  A teacher's id or a label
+ * below 0 is no entry; one at or above V is no entry either, and an index error at the next
+ * synchronisation.  A teacher's -inf has p = 0 and adds nothing; a row of logits that are all -inf has q = 0, and infinite losses. */
+typedef struct b200_distill_args {
+    b200_tensor logits;          /* rows [.., V], F32 or F16, V >= 1 */
+    b200_tensor teacher_ids;     /* rows [.., K], I32 or I64, K <= 1024 */
+    b200_tensor teacher_logits;  /* rows [.., K], F32 or F16 */
+    b200_tensor labels;          /* one for each row (the rows' extents), I32 or I64, any strides; absent: none */
+    b200_tensor losses;          /* F32, dense, one for each row; forward only, may be absent there */
+    b200_tensor stats;           /* [number of rows, 4], F32, dense: max z, log sum exp((z - max z) / T) (0 where c is 1),
+                                    log sum exp(z - max z) (0 where c is 0), 0; forward: a result, may be absent;
+                                    backward: as forward left it */
+    b200_tensor losses_grad;     /* F32, one for each row, any strides; absent: 1 */
+    b200_tensor grad;            /* rows like logits, of their type; may lie exactly on logits.  Forward: may be absent */
+    float temperature, hard_weight, grad_scale;
+} b200_distill_args;
+/* Losses and, where `grad` is given, the logits' gradient too, from one reading of the logits. */
+int b200_distill_loss(b200_ctx* ctx, const b200_distill_args* args);
+/* The gradient alone, for losses' gradients that are known only later. */
+int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
+
+/* The status that one of these calls would answer its arguments with, and the reason, without a context or a device:
+ * `args` is the call's struct.  What b200_supports is for nodes. */
+#define B200_CALL_EMBEDDING 0
+#define B200_CALL_EMBEDDING_BACKWARD 1
+#define B200_CALL_BLOCK_NORM 2
+#define B200_CALL_BLOCK_NORM_BACKWARD 3
+#define B200_CALL_DISTILL_LOSS 4
+#define B200_CALL_DISTILL_LOSS_BACKWARD 5
+int b200_check_operator(int which, const void* args, char* why, size_t why_len);
+
 /* -- an entry point that allocates nothing (no counterpart in vkML: its backends
  *    always own an allocator) --
  *

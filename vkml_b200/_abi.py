@@ -70,6 +70,38 @@ class ProfileRecord(C.Structure):
     _fields_ = [("label", C.c_char * 48), ("ms", C.c_float), ("op", C.c_uint32), ("submission", C.c_uint32)]
 
 
+class EmbeddingArgs(C.Structure):
+    """b200_embedding_args"""
+    _fields_ = [(n, Tensor) for n in ("table", "ids", "rows")] + [
+        ("scale", C.c_float), ("flags", C.c_uint32), ("padding_id", C.c_int64), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t)]
+
+
+class BlockNormArgs(C.Structure):
+    """b200_block_norm_args"""
+    _fields_ = [(n, Tensor) for n in (
+        "residual", "branch", "out", "normed", "stats", "post_weight", "post_bias", "pre_weight", "pre_bias", "gate")] + [
+        ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("eps", C.c_float), ("kind", C.c_int32),
+        ("flags", C.c_uint32)]
+
+
+class BlockNormGradArgs(C.Structure):
+    """b200_block_norm_grad_args"""
+    _fields_ = [(n, Tensor) for n in (
+        "out", "branch", "stats", "out_grad", "normed_grad", "post_weight", "post_bias", "gate", "pre_weight",
+        "residual_grad", "branch_grad", "post_weight_grad", "post_bias_grad", "pre_weight_grad", "pre_bias_grad",
+        "gate_grad")] + [
+        ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("kind", C.c_int32), ("flags", C.c_uint32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class DistillArgs(C.Structure):
+    """b200_distill_args"""
+    _fields_ = [(n, Tensor) for n in (
+        "logits", "teacher_ids", "teacher_logits", "labels", "losses", "stats", "losses_grad", "grad")] + [
+        ("temperature", C.c_float), ("hard_weight", C.c_float), ("grad_scale", C.c_float)]
+
+
 # Every symbol include/vkml_b200.h declares: name -> (restype, argtypes).
 _P = C.c_void_p
 SYMBOLS = {
@@ -116,6 +148,16 @@ SYMBOLS = {
     "b200_tape_enable_graphs": (C.c_int, [_P, C.c_int]),
     "b200_tape_stats": (C.c_int, [_P, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
     "b200_tape_destroy": (None, [_P]),
+    # (argument structs of operators: packed bytes, or a pointer to the structure)
+    "b200_embedding": (C.c_int, [_P, _P]),
+    "b200_embedding_backward": (C.c_int, [_P, _P]),
+    "b200_embedding_backward_workspace": (C.c_int, [_P, C.POINTER(C.c_size_t)]),
+    "b200_block_norm": (C.c_int, [_P, _P]),
+    "b200_block_norm_backward": (C.c_int, [_P, _P]),
+    "b200_block_norm_backward_workspace": (C.c_int, [_P, C.POINTER(C.c_size_t)]),
+    "b200_check_operator": (C.c_int, [C.c_int, _P, C.c_char_p, C.c_size_t]),
+    "b200_distill_loss": (C.c_int, [_P, _P]),
+    "b200_distill_loss_backward": (C.c_int, [_P, _P]),
     "b200_sum_columns_f32_noalloc": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, _P, _P, C.c_char_p, C.c_size_t]),
 }
 

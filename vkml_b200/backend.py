@@ -13,7 +13,7 @@ from typing import Sequence
 
 import numpy as np
 
-from . import _abi
+from . import _abi, graph
 from .graph import DType, NodeDesc, TensorDesc, pack_nodes
 
 
@@ -135,6 +135,98 @@ class Backend:
 
     def compute_packed(self, packed, n: int, flags: int = 0) -> None:
         self._check(self._lib.b200_compute(self._ctx, packed, n, flags), "compute")
+
+    # -- operators of language-model training ---------------------------------
+    # Tensors are DeviceTensor or TensorDesc; results are tensors that the caller made.  Every call is ordered on the
+    # backend's stream when it returns, like compute().  `workspace`: a Storage for calls that are captured into a
+    # graph of the caller's; without one the context's own scratch is used.
+    def embedding(self, table, ids, rows, scale: float = 1.0) -> None:
+        """rows[t] = scale * table[ids[t]].  table [V, D], ids of any extents up to rank 2 (I64 or I32), rows
+        ids' extents and D; F32 or F16 on either side.  An id outside [0, V) reads as zeros and is an IndexError at
+        the next synchronisation."""
+        self._check(self._lib.b200_embedding(self._ctx, graph.embedding_args(table, ids, rows, scale)), "embedding")
+
+    def embedding_backward(self, rows_grad, ids, table_grad, scale: float = 1.0, padding_id: int | None = None,
+                           accumulate: bool = False, workspace: Storage | None = None) -> None:
+        """table_grad[v] = scale * (the sum of rows_grad over the tokens of id v), zeros where there are none; with
+        `accumulate` added to what table_grad holds (a tied projection's gradient).  Tokens of `padding_id` are left
+        out.  Sums are held in F32, in an order that the ids alone decide."""
+        ws, nbytes = (workspace.data, workspace.nbytes) if workspace is not None else (0, 0)
+        self._check(self._lib.b200_embedding_backward(self._ctx, graph.embedding_args(
+            table_grad, ids, rows_grad, scale, graph.ACCUMULATE if accumulate else 0,
+            -1 if padding_id is None else padding_id, ws, nbytes)), "embedding_backward")
+
+    def embedding_backward_workspace(self, rows_grad, ids, table_grad) -> int:
+        """Bytes of a workspace for embedding_backward with these tensors."""
+        n = C.c_size_t(0)
+        self._check(self._lib.b200_embedding_backward_workspace(
+            graph.embedding_args(table_grad, ids, rows_grad, 1.0), C.byref(n)), "embedding_backward_workspace")
+        return n.value
+
+    def block_norm(self, residual, branch, *, out=None, normed=None, stats=None, post_weight=None, post_bias=None,
+                   gate=None, pre_weight=None, pre_bias=None, residual_scale: float = 1.0, branch_scale: float = 1.0,
+                   kind: str = "rms", eps: float = 1e-5, post_norm: bool = True) -> None:
+        """out = residual_scale * residual + branch_scale * gate * (N(branch) * post_weight + post_bias);
+        normed = N(out) * pre_weight + pre_bias: the norm behind a block, its gate, the sum with the residual
+        stream and the norm in front of the next block.  residual or branch may be None, and so may out or normed
+        (no norm in front).  `post_norm=False`: the branch as it is.  kind: "rms" or "layer".  stats [rows, 4] F32 is
+        what block_norm_backward needs."""
+        if branch is None:
+            post_norm = False
+        self._check(self._lib.b200_block_norm(self._ctx, graph.block_norm_args(
+            (residual, branch, out, normed, stats, post_weight, post_bias, pre_weight, pre_bias, gate),
+            residual_scale, branch_scale, eps, self._norm_kind(kind), graph.NORM_POST if post_norm else 0)), "block_norm")
+
+    @staticmethod
+    def _norm_kind(kind: str) -> int:
+        if kind not in graph.NORM_KINDS:
+            raise ValueError(f"block_norm: unknown kind of norm {kind!r}")
+        return graph.NORM_KINDS[kind]
+
+    def _block_norm_grad_args(self, out, branch, stats, *, out_grad=None, normed_grad=None, residual_grad=None,
+                              branch_grad=None, post_weight=None, post_bias=None, gate=None, pre_weight=None,
+                              post_weight_grad=None, post_bias_grad=None, gate_grad=None, pre_weight_grad=None,
+                              pre_bias_grad=None, residual_scale=1.0, branch_scale=1.0, kind="rms", post_norm=True,
+                              workspace=None) -> bytes:
+        ws, nbytes = (workspace.data, workspace.nbytes) if workspace is not None else (0, 0)
+        if branch is None:
+            post_norm = False
+        return graph.block_norm_grad_args(
+            (out, branch, stats, out_grad, normed_grad, post_weight, post_bias, gate, pre_weight, residual_grad, branch_grad,
+             post_weight_grad, post_bias_grad, pre_weight_grad, pre_bias_grad, gate_grad),
+            residual_scale, branch_scale, self._norm_kind(kind), graph.NORM_POST if post_norm else 0, ws, nbytes)
+
+    def block_norm_backward(self, out, branch, stats, **options) -> None:
+        """Gradients of block_norm from out_grad and normed_grad (either may be None: zero), with out and stats as the forward
+        call left them: residual_grad, branch_grad, post_weight_grad, post_bias_grad, gate_grad, pre_weight_grad and
+        pre_bias_grad, each where a tensor is given.  The other options are those of the forward call, and workspace."""
+        self._check(self._lib.b200_block_norm_backward(
+            self._ctx, self._block_norm_grad_args(out, branch, stats, **options)), "block_norm_backward")
+
+    def block_norm_backward_workspace(self, out, branch, stats, **options) -> int:
+        """Bytes of a workspace for block_norm_backward with these tensors and options."""
+        n = C.c_size_t(0)
+        self._check(self._lib.b200_block_norm_backward_workspace(
+            self._block_norm_grad_args(out, branch, stats, **options), C.byref(n)), "block_norm_backward_workspace")
+        return n.value
+
+    def distill_loss(self, logits, teacher_ids, teacher_logits, losses, *, labels=None, stats=None, grad=None,
+                     losses_grad=None, temperature: float = 1.0, hard_weight: float = 0.0,
+                     grad_scale: float = 1.0) -> None:
+        """losses = (1 - hard_weight) * T^2 * KL(softmax(teacher_logits / T) || softmax(logits / T) at teacher_ids)
+        + hard_weight * cross-entropy on labels, one F32 for each row.  Ids or labels below 0 are no entry.  With `grad`
+        the logits' gradient too, grad_scale * losses_grad * d loss / d logits, from the same reading of the logits (it
+        may lie on them).  stats [rows, 4] F32 is what distill_loss_backward needs."""
+        self._check(self._lib.b200_distill_loss(self._ctx, graph.distill_args(
+            (logits, teacher_ids, teacher_logits, labels, losses, stats, losses_grad, grad), temperature, hard_weight,
+            grad_scale)), "distill_loss")
+
+    def distill_loss_backward(self, logits, teacher_ids, teacher_logits, stats, grad, *, labels=None, losses_grad=None,
+                              temperature: float = 1.0, hard_weight: float = 0.0, grad_scale: float = 1.0) -> None:
+        """The logits' gradient alone, with stats as distill_loss left it; options as there."""
+        self._check(self._lib.b200_distill_loss_backward(self._ctx, graph.distill_args(
+            (logits, teacher_ids, teacher_logits, labels, None, stats, losses_grad, grad), temperature, hard_weight,
+            grad_scale)), "distill_loss_backward")
 
     # -- copies ---------------------------------------------------------------
     def copy_from_host(self, dst: Storage, dst_offset: int, src, nbytes: int | None = None) -> None:

@@ -1,0 +1,343 @@
+// What the operators of language-model training (embedding.cu, block_norm.cu, distill.cu) share: checks of their
+// arguments, rows of strided tensors, workspaces, and wide accesses.
+#pragma once
+
+#include "context.h"
+
+#include <cuda_fp16.h>
+
+#include <initializer_list>
+
+namespace b200 {
+
+// Runs the body of an entry point on its context's device and turns what it throws into a status and a message.
+template <typename Fn>
+int guarded_operator(b200_ctx* ctx, Fn&& fn) {
+    auto answer = [&](int status, const char* message) {
+        if (ctx != nullptr) {
+            std::lock_guard<std::mutex> lock(ctx->err_mu);
+            ctx->last_error = message;
+        }
+        return status;
+    };
+    try {
+        if (ctx != nullptr) B200_CUDA_CHECK(cudaSetDevice(ctx->device));
+        fn();
+        return B200_OK;
+    } catch (const Error& e) {
+        return answer(e.status, e.message.c_str());
+    } catch (const std::bad_alloc&) {
+        return answer(B200_OUT_OF_MEMORY, "host allocation failed");
+    } catch (const std::exception& e) {
+        return answer(B200_INTERNAL_ERROR, e.what());
+    }
+}
+
+// ---- arguments --------------------------------------------------------------
+
+inline bool is_float(int dtype) { return dtype == B200_F32 || dtype == B200_F16; }
+inline bool is_index(int dtype) { return dtype == B200_I32 || dtype == B200_I64; }
+
+inline int64_t numel_of(const b200_tensor& t) {
+    int64_t n = 1;
+    for (int d = 0; d < t.ndim; ++d) n *= t.dims[d];
+    return n;
+}
+
+// A tensor with a rank, extents and strides that can be: what every later check relies on.  The largest view reaches less than 2^62 bytes.
+inline void check_tensor(const b200_tensor& t, const char* name) {
+    const std::string who(name);
+    const int64_t size = static_cast<int64_t>(dtype_size(t.dtype));
+    if (size == 0) fail(B200_DTYPE_ERROR, who + ": unknown dtype " + std::to_string(t.dtype));
+    if (t.ndim < 0 || t.ndim > kMaxDims) fail(B200_SHAPE_ERROR, who + ": rank " + std::to_string(t.ndim) + " is outside 0..4");
+    double elements = 1, reach = 0;
+    for (int d = 0; d < t.ndim; ++d) {
+        if (t.dims[d] < 0) fail(B200_SHAPE_ERROR, who + ": negative extent");
+        if (t.strides[d] % size != 0) fail(B200_NOT_IMPLEMENTED, who + ": byte stride is not a multiple of the element size");
+        elements *= static_cast<double>(t.dims[d]);
+        reach += static_cast<double>(t.dims[d]) * (t.strides[d] < 0 ? -static_cast<double>(t.strides[d]) : static_cast<double>(t.strides[d]));
+    }
+    if (elements >= 9.0e18 || reach >= 4.0e18) fail(B200_SHAPE_ERROR, who + ": extents or strides are too large");
+    if (reinterpret_cast<uintptr_t>(t.data) % static_cast<uintptr_t>(size) != 0) fail(B200_INVALID_ARGUMENT, who + ": address is not aligned to its elements");
+}
+
+inline bool same_extents(const b200_tensor& a, const b200_tensor& b, int axes) {
+    for (int d = 0; d < axes; ++d) {
+        if (a.dims[d] != b.dims[d]) return false;
+    }
+    return true;
+}
+
+inline bool same_view(const b200_tensor& a, const b200_tensor& b) {
+    if (a.data != b.data || a.dtype != b.dtype || a.ndim != b.ndim) return false;
+    for (int d = 0; d < a.ndim; ++d) {
+        if (a.dims[d] != b.dims[d] || (a.dims[d] > 1 && a.strides[d] != b.strides[d])) return false;
+    }
+    return true;
+}
+
+inline bool is_dense(const b200_tensor& t) {
+    if (numel_of(t) == 0) return true;
+    int64_t expected = static_cast<int64_t>(dtype_size(t.dtype));
+    for (int d = t.ndim - 1; d >= 0; --d) {
+        if (t.dims[d] != 1 && t.strides[d] != expected) return false;
+        expected *= t.dims[d];
+    }
+    return true;
+}
+
+// Whether no element of a view lies on another: sorted by stride, each axis steps over everything below it.
+inline bool elements_distinct(const b200_tensor& t) {
+    if (numel_of(t) == 0) return true;
+    bool used[kMaxDims] = {};
+    int64_t end = static_cast<int64_t>(dtype_size(t.dtype));
+    for (int k = 0; k < t.ndim; ++k) {
+        int at = -1;
+        for (int d = 0; d < t.ndim; ++d) {
+            if (used[d] || t.dims[d] <= 1) continue;
+            if (at < 0 || std::abs(t.strides[d]) < std::abs(t.strides[at])) at = d;
+        }
+        if (at < 0) break;
+        used[at] = true;
+        const int64_t step = std::abs(t.strides[at]);
+        if (step < end) return false;
+        end += step * (t.dims[at] - 1);
+    }
+    return true;
+}
+
+// Rows of a tensor of rank 1 to 3: row r starts at base + (r / inner) * outer_stride + (r % inner) * inner_stride, in bytes.
+struct RowsArg {
+    char* base;
+    int64_t outer, step;
+};
+
+// The leading extents that every tensor of rows in a call shares.
+struct RowShape {
+    int64_t rows = 1, outer = 1, inner = 1;
+};
+
+inline RowShape row_shape(const b200_tensor& t, int axes) {
+    RowShape s;
+    if (axes >= 1) s.inner = t.dims[axes - 1];
+    if (axes >= 2) s.outer = t.dims[axes - 2];
+    s.rows = s.outer * s.inner;
+    return s;
+}
+
+// `axes`: how many of the tensor's axes stand in front of its rows.
+inline RowsArg rows_arg(const b200_tensor& t, int axes) {
+    RowsArg r;
+    r.base = static_cast<char*>(t.data);
+    r.step = axes >= 1 && t.dims[axes - 1] > 1 ? t.strides[axes - 1] : 0;
+    r.outer = axes >= 2 && t.dims[axes - 2] > 1 ? t.strides[axes - 2] : 0;
+    return r;
+}
+
+inline bool aligned_rows(const RowsArg& r, int64_t bytes) {
+    return r.base == nullptr || (reinterpret_cast<uintptr_t>(r.base) % static_cast<uintptr_t>(bytes) == 0 && r.outer % bytes == 0 && r.step % bytes == 0);
+}
+
+inline void check_rows(const b200_tensor& t, const char* name) {
+    check_tensor(t, name);
+    if (t.ndim < 1 || t.ndim > 3) fail(B200_SHAPE_ERROR, std::string(name) + ": rank " + std::to_string(t.ndim) + " is outside 1..3");
+    const int64_t width = t.dims[t.ndim - 1];
+    if (numel_of(t) != 0 && width > 1 && t.strides[t.ndim - 1] != static_cast<int64_t>(dtype_size(t.dtype))) {
+        fail(B200_NOT_IMPLEMENTED, std::string(name) + ": the last axis has no unit stride");
+    }
+    if (numel_of(t) != 0 && t.data == nullptr) fail(B200_INVALID_ARGUMENT, std::string(name) + " has no storage");
+    const RowShape s = row_shape(t, t.ndim - 1);
+    if (s.rows >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, std::string(name) + ": more than 2^31 - 1 rows");
+}
+
+// Whether two views may have an element in common.  Ranges of addresses that do not meet settle it; where they do (columns of one
+// buffer, say), every run of consecutive elements of a view starts at its address plus a multiple of g, the greatest common divisor of all strides
+// between runs: runs whose places modulo g do not meet never meet.
+inline bool may_share(const b200_tensor& x, const b200_tensor& y) {
+    if (!overlap(x, y)) return false;
+    auto gcd = [](int64_t a, int64_t b) {
+        a = std::abs(a), b = std::abs(b);
+        while (b != 0) {
+            const int64_t r = a % b;
+            a = b, b = r;
+        }
+        return a;
+    };
+    int64_t g = 0, run[2];
+    const b200_tensor* both[2] = {&x, &y};
+    for (int k = 0; k < 2; ++k) {
+        const b200_tensor& t = *both[k];
+        run[k] = static_cast<int64_t>(dtype_size(t.dtype));
+        for (int d = t.ndim - 1; d >= 0; --d) {
+            if (t.dims[d] <= 1) continue;
+            if (d == t.ndim - 1 && t.strides[d] == run[k]) run[k] *= t.dims[d];
+            else g = gcd(g, t.strides[d]);
+        }
+    }
+    if (g == 0) return true;
+    const int64_t apart = static_cast<const char*>(y.data) - static_cast<const char*>(x.data);
+    const int64_t place = ((apart % g) + g) % g;
+    return !(place >= run[0] && place + run[1] <= g);
+}
+
+// What a forward call leaves for its backward: four floats for each row.
+inline void check_stats(const b200_tensor& t, int64_t rows) {
+    check_tensor(t, "stats");
+    if (t.dtype != B200_F32) fail(B200_DTYPE_ERROR, "stats are F32");
+    if (t.ndim != 2 || t.dims[0] != rows || t.dims[1] != 4 || !is_dense(t) || reinterpret_cast<uintptr_t>(t.data) % 16 != 0) {
+        fail(B200_SHAPE_ERROR, "stats: not [rows, 4], dense and 16-byte aligned");
+    }
+}
+
+struct Named {
+    const b200_tensor* t;
+    const char* name;
+};
+
+// Every result's elements are its own, and lie on no other tensor's: on a tensor of `exact` only where the two are the same view.
+inline void check_results(std::initializer_list<Named> results, std::initializer_list<Named> inputs, std::initializer_list<Named> exact) {
+    for (const Named* r = results.begin(); r != results.end(); ++r) {
+        if (r->t->data == nullptr) continue;
+        const std::string who(r->name);
+        if (!elements_distinct(*r->t)) fail(B200_INVALID_ARGUMENT, who + ": a result's elements lie on one another");
+        for (const Named* o = results.begin(); o != r; ++o) {
+            if (may_share(*r->t, *o->t)) fail(B200_INVALID_ARGUMENT, who + " overlaps " + o->name);
+        }
+        for (const Named& i : inputs) {
+            if (may_share(*r->t, *i.t)) fail(B200_INVALID_ARGUMENT, who + " overlaps " + i.name);
+        }
+        for (const Named& i : exact) {
+            if (may_share(*r->t, *i.t) && !same_view(*r->t, *i.t)) fail(B200_INVALID_ARGUMENT, who + " overlaps " + i.name + " without being the same view");
+        }
+    }
+}
+
+// What b200_compute does before it queues a node: the tensors' pending all-reduces come first.
+inline void wait_for_tensors(b200_ctx* ctx, std::initializer_list<const b200_tensor*> tensors) {
+    if (!dist_has_pending(ctx)) return;
+    for (const b200_tensor* t : tensors) {
+        if (t->data == nullptr || numel_of(*t) == 0) continue;
+        const char* lo = static_cast<const char*>(t->data);
+        const char* hi = lo + dtype_size(t->dtype);
+        for (int d = 0; d < t->ndim; ++d) {
+            const int64_t reach = (t->dims[d] - 1) * t->strides[d];
+            (reach < 0 ? lo : hi) += reach;
+        }
+        dist_wait_range(ctx, lo, hi);
+    }
+}
+
+// The caller's workspace, or the context's own, grown where it has to be.
+inline char* operator_workspace(b200_ctx* ctx, void* workspace, size_t have, size_t need) {
+    if (need == 0) return nullptr;
+    if (workspace != nullptr) {
+        if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) fail(B200_INVALID_ARGUMENT, "workspace is not 256-byte aligned");
+        if (have < need) fail(B200_INVALID_ARGUMENT, "workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) + " are needed");
+        return static_cast<char*>(workspace);
+    }
+    if (need > ctx->workspace_bytes) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        B200_CUDA_CHECK(cudaStreamIsCapturing(ctx->stream, &status));
+        if (status != cudaStreamCaptureStatusNone) {
+            fail(B200_INVALID_ARGUMENT, "the context's workspace would have to grow while its stream is captured: pass a workspace, or make the call once before");
+        }
+    }
+    return static_cast<char*>(ctx->ensure_workspace(need));
+}
+
+// A caller's workspace as a tensor, so that results are checked against it too.
+inline b200_tensor workspace_tensor(void* workspace, size_t bytes) {
+    b200_tensor t{};
+    t.data = bytes != 0 ? workspace : nullptr;
+    t.ndim = 1;
+    t.dims[0] = static_cast<int64_t>(bytes);
+    t.strides[0] = 1;
+    t.dtype = B200_BOOL;
+    return t;
+}
+
+// What a call asks of its arguments, without a context: throws Error where it would be refused.
+void check_embedding_call(const b200_embedding_args& a, bool backward);
+void check_block_norm(const b200_block_norm_args& a);
+void check_block_norm_backward(const b200_block_norm_grad_args& a);
+void check_distill_loss(const b200_distill_args& a, bool forward);
+
+// ---- device side ------------------------------------------------------------
+
+#ifdef __CUDACC__
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// Eight elements of a row as they lie in memory: 16 bytes of F16 or 32 of F32, moved 16 bytes at a time.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<__half> {
+    uint4 a;
+};
+template <>
+struct Raw8<float> {
+    uint4 a, b;
+};
+
+__device__ __forceinline__ void load8(Raw8<__half>& r, const __half* p) { r.a = *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void load8(Raw8<float>& r, const float* p) {
+    r.a = reinterpret_cast<const uint4*>(p)[0];
+    r.b = reinterpret_cast<const uint4*>(p)[1];
+}
+
+__device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&x)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+}
+
+__device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// Where row r of a tensor lies.
+__device__ __forceinline__ char* row_at(const RowsArg& t, const FastDiv& inner, uint32_t r) {
+    uint32_t b, i;
+    inner.divmod(r, b, i);
+    return t.base + static_cast<int64_t>(b) * t.outer + static_cast<int64_t>(i) * t.step;
+}
+
+__device__ __forceinline__ int64_t load_index(const void* p, bool wide) {
+    return wide ? *static_cast<const int64_t*>(p) : static_cast<int64_t>(*static_cast<const int32_t*>(p));
+}
+
+#endif  // __CUDACC__
+
+}  // namespace b200

@@ -211,3 +211,45 @@ def pack_nodes(nodes: Sequence[NodeDesc]):
         parts.append(_NO_TENSORS[_abi.MAX_SRC - len(src)])
         parts.append(bytes(n.params[:_abi.PARAM_BYTES]).ljust(_abi.PARAM_BYTES, b"\0") if n.params else _NO_PARAMS)
     return (_abi.Node * len(nodes)).from_buffer_copy(b"".join(parts))
+
+
+# -- arguments of the operators of language-model training: the tensors' bytes, then the numbers, as the C structs lay them out --
+
+NORM_KINDS = {"rms": 0, "layer": 1}
+NORM_POST = 1
+ACCUMULATE = 1
+_EMBEDDING_TAIL = struct.Struct("<fIqQQ")
+_NORM_TAIL = struct.Struct("<fffiI4x")
+_NORM_GRAD_TAIL = struct.Struct("<ffiIQQ")
+_DISTILL_TAIL = struct.Struct("<fff4x")
+_ABSENT = bytes(_TENSOR_WORDS.size)
+for _tail, _tensors, _args in ((_EMBEDDING_TAIL, 3, _abi.EmbeddingArgs), (_NORM_TAIL, 10, _abi.BlockNormArgs),
+                               (_NORM_GRAD_TAIL, 16, _abi.BlockNormGradArgs), (_DISTILL_TAIL, 8, _abi.DistillArgs)):
+    assert _tensors * _TENSOR_WORDS.size + _tail.size == ctypes.sizeof(_args)
+
+
+def tensors_bytes(tensors: Sequence) -> bytes:
+    """Tensor descriptions (or tensors that have one, or None for an absent one) as consecutive b200_tensor structs."""
+    parts = []
+    for t in tensors:
+        if t is None:
+            parts.append(_ABSENT)
+        else:
+            parts.append(_tensor_bytes(t if type(t) is TensorDesc else t.desc))
+    return b"".join(parts)
+
+
+def embedding_args(table, ids, rows, scale, flags=0, padding_id=-1, workspace=0, workspace_bytes=0) -> bytes:
+    return tensors_bytes((table, ids, rows)) + _EMBEDDING_TAIL.pack(scale, flags, padding_id, workspace, workspace_bytes)
+
+
+def block_norm_args(tensors, residual_scale, branch_scale, eps, kind, flags) -> bytes:
+    return tensors_bytes(tensors) + _NORM_TAIL.pack(residual_scale, branch_scale, eps, kind, flags)
+
+
+def block_norm_grad_args(tensors, residual_scale, branch_scale, kind, flags, workspace=0, workspace_bytes=0) -> bytes:
+    return tensors_bytes(tensors) + _NORM_GRAD_TAIL.pack(residual_scale, branch_scale, kind, flags, workspace, workspace_bytes)
+
+
+def distill_args(tensors, temperature, hard_weight, grad_scale) -> bytes:
+    return tensors_bytes(tensors) + _DISTILL_TAIL.pack(temperature, hard_weight, grad_scale)
