@@ -493,7 +493,7 @@ void with_types(const Shape& p, Fn&& fn) {
     else fn(float{}, float{});
 }
 
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned_columns(const void* p) { return reinterpret_cast<uintptr_t>(p) % 32 == 0; }
 
 Shape check_forward(const b200_block_norm_args& a, int& columns) {
     Shape p = check_sides({{&a.residual, "residual"}, {&a.out, "out"}}, {{&a.branch, "branch"}, {&a.normed, "normed"}}, a.kind, a.flags);
@@ -539,8 +539,8 @@ void launch_forward(b200_ctx* ctx, const b200_block_norm_args& a) {
     k.share = 1.f / static_cast<float>(p.width);
     k.layer = a.kind == B200_NORM_LAYER;
     k.post = (a.flags & B200_NORM_POST) != 0;
-    const bool wide = p.width % 8 == 0 && aligned_rows(k.residual, 16) && aligned_rows(k.branch, 16) && aligned_rows(k.out, 16) && aligned_rows(k.normed, 16) &&
-                      aligned16(k.post_weight) && aligned16(k.post_bias) && aligned16(k.pre_weight) && aligned16(k.pre_bias) && aligned16(k.gate);
+    const bool wide = p.width % 8 == 0 && aligned_rows(k.residual, p.residual_type) && aligned_rows(k.branch, p.branch_type) && aligned_rows(k.out, p.residual_type) && aligned_rows(k.normed, p.branch_type) &&
+                      aligned_columns(k.post_weight) && aligned_columns(k.post_bias) && aligned_columns(k.pre_weight) && aligned_columns(k.pre_bias) && aligned_columns(k.gate);
     // narrow rows are a warp's, eight of them to a block; wider ones a block's with one piece to a thread, two above 2048 columns
     const bool warp = p.width <= 256;
     const int pieces = p.width <= 2048 ? 1 : 2;
@@ -684,9 +684,9 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     k.share = 1.f / static_cast<float>(p.width);
     k.layer = a.kind == B200_NORM_LAYER;
     k.post = (a.flags & B200_NORM_POST) != 0;
-    const bool wide = p.width % 8 == 0 && aligned_rows(k.out, 16) && aligned_rows(k.branch, 16) && aligned_rows(k.out_grad, 16) && aligned_rows(k.normed_grad, 16) &&
-                      aligned_rows(k.residual_grad, 16) && aligned_rows(k.branch_grad, 16) && aligned16(k.post_weight) && aligned16(k.post_bias) &&
-                      aligned16(k.pre_weight) && aligned16(k.gate);
+    const bool wide = p.width % 8 == 0 && aligned_rows(k.out, p.residual_type) && aligned_rows(k.branch, p.branch_type) && aligned_rows(k.out_grad, p.residual_type) && aligned_rows(k.normed_grad, p.branch_type) &&
+                      aligned_rows(k.residual_grad, p.residual_type) && aligned_rows(k.branch_grad, p.branch_type) && aligned_columns(k.post_weight) && aligned_columns(k.post_bias) &&
+                      aligned_columns(k.pre_weight) && aligned_columns(k.gate);
     ProfScope scope(ctx, "block_norm_backward");
     with_types(p, [&](auto th, auto ty) {
         using TH = decltype(th);

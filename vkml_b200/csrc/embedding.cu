@@ -177,161 +177,254 @@ owned_rows_kernel(char* table, int64_t pitch, RowsArg grad, Ids ids, uint32_t co
 
 // ---- gradient: sorted tokens --------------------------------------------------
 
-// The tokens are sorted by id, those of one id in their own order, by one cluster of blocks: radix passes over 8 bits of the id, each of which counts
-// the digits of every warp's stretch of the tokens, adds the counts up over warps (shared memory) and blocks (the cluster's shared memory), and
-// moves each token to its place.  Tokens that have no gradient sort behind all others, as id V.  The blocks outside of the first cluster write zeros
-// over the table meanwhile: sorting leaves the memory idle.  16 blocks of 1024 threads sort 131072 tokens in the time that writing 130 MB takes.
+// The tokens are sorted by id, those of one id in their own order: radix passes over up to 8 bits of the id, of two kernels each.  A block has a tile of
+// the tokens, a warp a stretch of the tile.  count_kernel leaves the counts of the tile's digits; move_kernel ranks every token among those of
+// its digit in its stretch, adds the counts of the warps, the tiles and the digits before, and moves each token to its place.  Tokens that have no gradient
+// sort behind all others, as id V.  The memory is idle meanwhile, so
+// blocks behind those that sort write zeros over the table's last rows; the rest of the rows without a token is written beside the sums.
+// (One cluster of 16 blocks that counts through its shared memory was 14 us for any number of tokens and 50 us for 131072 of them.)
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kMostHeld = 8;        // tokens of a thread
+constexpr int kScannedTiles = 64;   // up to here move_kernel adds up the tiles' counts itself; above, scan_kernel does beforehand
+
+// Rows of the table that are to be zeros.
+struct Zeros {
+    char* table;  // null: none
+    int64_t pitch;
+    uint32_t row0, rows;
+    FastDiv pieces;  // of a row: of 16 bytes where `wide`, else of 2
+    bool wide;
+};
 
 struct SortArgs {
     Ids ids;
-    uint2* buffer[2];  // (id, token)
-    uint32_t count;
-    uint32_t vocab;
+    const uint2* from;   // (id, token); null: the ids
+    uint2* to;
+    uint32_t* counts;    // [tiles][256]; from scan_kernel, the counts of the tiles before
+    uint32_t* totals;    // [256], from scan_kernel
+    uint32_t* touched;   // a bit for each row, or null
+    uint32_t count, vocab, tiles, tile;  // tile: tokens of one
     int64_t padding;
-    int passes, digit_bits;
-    char* table;       // to be filled with zeros: null where not
-    int64_t pitch, row_bytes;
+    int shift, bits;
+    bool scanned;
+    Zeros zeros;
     uint32_t* status;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_blocks() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-// A word of shared memory of block `rank` of the cluster, at the address that `mine` has here.
-__device__ __forceinline__ uint32_t cluster_load(const uint32_t* mine, uint32_t rank) {
-    uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(mine)), there, x;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(there) : "memory");
-    return x;
-}
-
-__device__ void fill_zeros(const SortArgs& k, uint32_t block, uint32_t blocks) {
-    const uint32_t warp = block * kSortWarps + threadIdx.x / 32, warps = blocks * kSortWarps, lane = threadIdx.x % 32;
-    const bool wide = ((reinterpret_cast<uintptr_t>(k.table) | k.pitch | k.row_bytes) & 15) == 0;
-    if (wide) {
-        // dense rows are one stretch, cut into pieces of 4 KB; others are taken one by one
-        const bool dense = k.pitch == k.row_bytes;
-        const int64_t piece = dense ? 256 : k.row_bytes / 16, all = dense ? int64_t(k.vocab) * k.row_bytes / 16 : 0;
-        const int64_t pieces = dense ? (all + piece - 1) / piece : k.vocab;
-        for (int64_t p = warp; p < pieces; p += warps) {
-            uint4* to = reinterpret_cast<uint4*>(k.table + (dense ? p * piece * 16 : p * k.pitch));
-            const int64_t n = dense ? min(piece, all - p * piece) : piece;
-            for (int64_t i = lane; i < n; i += 32) to[i] = make_uint4(0, 0, 0, 0);
-        }
-    } else {
-        for (int64_t r = warp; r < k.vocab; r += warps) {
-            uint16_t* to = reinterpret_cast<uint16_t*>(k.table + r * k.pitch);
-            for (int64_t i = lane; i < k.row_bytes / 2; i += 32) to[i] = 0;
-        }
+// Thread `tid` of `threads` writes its share of the zeros of 32 rows; `skip`: the rows that have a token.
+__device__ __forceinline__ void zero_rows(const Zeros& z, uint32_t row0, uint32_t rows, uint32_t skip, uint32_t tid, uint32_t threads) {
+    const uint32_t n = rows * z.pieces.d;  // (32 rows of less than 2^26 pieces)
+    for (uint32_t i = tid; i < n; i += threads) {
+        uint32_t r, c;
+        z.pieces.divmod(i, r, c);
+        if ((skip >> r) & 1) continue;
+        char* to = z.table + int64_t(row0 + r) * z.pitch;
+        if (z.wide) reinterpret_cast<uint4*>(to)[c] = make_uint4(0, 0, 0, 0);
+        else reinterpret_cast<uint16_t*>(to)[c] = 0;
     }
 }
+// The blocks behind the tiles'.
+__device__ __forceinline__ bool zeros_block(const SortArgs& k) {
+    if (blockIdx.x < k.tiles) return false;
+    for (uint32_t r = (blockIdx.x - k.tiles) * 32; r < k.zeros.rows; r += (gridDim.x - k.tiles) * 32) {
+        zero_rows(k.zeros, k.zeros.row0 + r, min(32u, k.zeros.rows - r), 0, threadIdx.x, blockDim.x);
+    }
+    return true;
+}
 
-__global__ void __launch_bounds__(kSortThreads) sort_tokens_kernel(const SortArgs k) {
-    __shared__ uint32_t place[kSortWarps][256];  // counts of each warp's digits; then where its next token of a digit goes
-    __shared__ uint32_t total[256];              // this block's counts, read by the others
-    __shared__ uint32_t upto[8];
+// Token i of a tile's thread, as (id, token).
+__device__ __forceinline__ uint2 sort_token(const SortArgs& k, uint32_t i, bool report) {
+    if (k.from != nullptr) return k.from[i];
+    const int64_t id = k.ids[i];
+    const bool in = id >= 0 && id < int64_t(k.vocab);
+    if (report && !in && id != k.padding) atomicOr(k.status, kStatusIndexOutOfRange);
+    return make_uint2(in && id != k.padding ? static_cast<uint32_t>(id) : k.vocab, i);
+}
+
+// HELD tokens of each thread, all under way at once: warp w has the 32 * HELD tokens from w * 32 * HELD on, 32 neighbours at a time.
+template <int HELD>
+__device__ __forceinline__ uint32_t held_index(const SortArgs& k, int h) {
+    return blockIdx.x * k.tile + (threadIdx.x / 32 * HELD + h) * 32 + threadIdx.x % 32;
+}
+
+template <int HELD>
+__global__ void __launch_bounds__(kSortThreads) count_kernel(const SortArgs k) {
+    __shared__ uint32_t counts[256];
     pdl_prologue();
-    const uint32_t blocks = cluster_blocks(), rank = cluster_rank();
-    if (blockIdx.x >= blocks) {
-        if (k.table != nullptr) fill_zeros(k, blockIdx.x - blocks, gridDim.x - blocks);
-        return;  // (whole clusters)
+    if (zeros_block(k)) return;
+    if (k.touched != nullptr && k.from == nullptr) {
+        for (uint32_t i = blockIdx.x * kSortThreads + threadIdx.x; i < (k.vocab + 31) / 32; i += k.tiles * kSortThreads) k.touched[i] = 0;
     }
-    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    // each warp's stretch: whole groups of 32 tokens
-    const uint32_t groups = (k.count + 31) / 32, warps = blocks * kSortWarps, per = (groups + warps - 1) / warps;
-    const uint32_t first = min(groups, (rank * kSortWarps + warp) * per), last = min(groups, first + per);
-    for (int pass = 0; pass < k.passes; ++pass) {
-        const uint2* from = k.buffer[(pass + 1) & 1];
-        uint2* to = k.buffer[pass & 1];
-        const int shift = pass * k.digit_bits;
-        const uint32_t mask = (1u << k.digit_bits) - 1;
-        auto token = [&](uint32_t i, bool report) {
-            if (pass > 0) return __ldcg(&from[i]);
-            const int64_t id = k.ids[i];
-            const bool in = id >= 0 && id < int64_t(k.vocab);
-            if (report && !in && id != k.padding) atomicOr(k.status, kStatusIndexOutOfRange);
-            return make_uint2(in && id != k.padding ? static_cast<uint32_t>(id) : k.vocab, i);
-        };
-        for (int i = tid; i < kSortWarps * 256; i += kSortThreads) (&place[0][0])[i] = 0;
-        __syncthreads();
-        for (uint32_t g = first; g < last; ++g) {
-            const uint32_t i = g * 32 + lane;
-            const uint32_t d = i < k.count ? (token(i, true).x >> shift) & mask : 256u;
-            const uint32_t peers = __match_any_sync(0xffffffffu, d);
-            if (d < 256 && lane == __ffs(peers) - 1) place[warp][d] += __popc(peers);
-            __syncwarp();
-        }
-        __syncthreads();
-        if (tid < 256) {  // exclusive over the warps
-            uint32_t sum = 0;
-#pragma unroll 8
-            for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t n = place[w][tid];
-                place[w][tid] = sum;
-                sum += n;
-            }
-            total[tid] = sum;
-        }
-        cluster_sync();
-        if (tid < 256) {  // over the blocks, and over the digits below
-            uint32_t all = 0, before = 0;
-            for (uint32_t b = 0; b < blocks; ++b) {
-                const uint32_t n = cluster_load(&total[tid], b);
-                if (b < rank) before += n;
-                all += n;
-            }
-            uint32_t scan = all;
+    uint2 x[HELD];
 #pragma unroll
-            for (int s = 1; s < 32; s *= 2) {
-                const uint32_t other = __shfl_up_sync(0xffffffffu, scan, s);
-                if (lane >= s) scan += other;
-            }
-            if (lane == 31) upto[warp] = scan;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            for (int w = 0; w < warp; ++w) scan += upto[w];
-            const uint32_t base = scan - all + before;
-#pragma unroll 8
-            for (int w = 0; w < kSortWarps; ++w) place[w][tid] += base;
+    for (int h = 0; h < HELD; ++h) {
+        const uint32_t i = held_index<HELD>(k, h);
+        if (i < k.count) x[h] = sort_token(k, i, true);
+    }
+    if (threadIdx.x < 256) counts[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const bool in = held_index<HELD>(k, h) < k.count;
+        const uint32_t d = in ? (x[h].x >> k.shift) & ((1u << k.bits) - 1) : 256u;
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);  // (frequent tokens would queue up at one counter)
+        if (in && threadIdx.x % 32 == __ffs(peers) - 1) atomicAdd(&counts[d], __popc(peers));
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) k.counts[blockIdx.x * 256 + threadIdx.x] = counts[threadIdx.x];
+}
+
+// A block to a digit: the tiles' counts become those of the tiles before, and their total.
+__global__ void __launch_bounds__(kSortThreads) scan_kernel(const SortArgs k) {
+    __shared__ uint32_t upto[kSortWarps];
+    pdl_prologue();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < k.tiles; base += kSortThreads) {
+        const uint32_t i = base + threadIdx.x;
+        const uint32_t n = i < k.tiles ? k.counts[int64_t(i) * 256 + blockIdx.x] : 0;
+        uint32_t scan = n;
+#pragma unroll
+        for (int s = 1; s < 32; s *= 2) {
+            const uint32_t other = __shfl_up_sync(0xffffffffu, scan, s);
+            if (lane >= s) scan += other;
         }
+        if (lane == 31) upto[warp] = scan;
         __syncthreads();
-        for (uint32_t g = first; g < last; ++g) {
-            const uint32_t i = g * 32 + lane;
-            const uint2 x = i < k.count ? token(i, false) : make_uint2(0, 0);
-            const uint32_t d = i < k.count ? (x.x >> shift) & mask : 256u;
-            const uint32_t peers = __match_any_sync(0xffffffffu, d);
-            if (d < 256) to[place[warp][d] + __popc(peers & ((1u << lane) - 1))] = x;
-            __syncwarp();
-            if (d < 256 && lane == __ffs(peers) - 1) place[warp][d] += __popc(peers);
-            __syncwarp();
+        uint32_t below = lane < warp ? upto[lane] : 0, all = upto[lane];
+#pragma unroll
+        for (int s = 16; s > 0; s /= 2) {
+            below += __shfl_xor_sync(0xffffffffu, below, s);
+            all += __shfl_xor_sync(0xffffffffu, all, s);
         }
-        cluster_sync();  // the moved tokens are there, and no block reads another's counts any more
+        if (i < k.tiles) k.counts[int64_t(i) * 256 + blockIdx.x] = before + below + scan - n;
+        before += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) k.totals[blockIdx.x] = before;
+}
+
+template <int HELD>
+__global__ void __launch_bounds__(kSortThreads) move_kernel(const SortArgs k) {
+    __shared__ uint32_t place[kSortWarps][257];  // counts of each warp's digits, then of the warps before; a row of odd length keeps columns off one bank
+    __shared__ uint32_t base[256];               // where this tile's tokens of a digit go
+    __shared__ uint32_t upto[kSortWarps];
+    pdl_prologue();
+    if (zeros_block(k)) return;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, d4 = tid / 4, q = tid % 4;
+    uint2 x[HELD];
+    uint32_t order[HELD];  // a token's rank among those of its digit in the stretch
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const uint32_t i = held_index<HELD>(k, h);
+        if (i < k.count) x[h] = sort_token(k, i, false);
+    }
+    // the tiles before, and all: four threads to a digit
+    uint32_t all = 0, before = 0;
+    if (k.scanned) {
+        all = q == 0 ? k.totals[d4] : 0;
+        before = q == 0 ? k.counts[int64_t(blockIdx.x) * 256 + d4] : 0;
+    } else {
+        uint32_t n[kScannedTiles / 4];
+#pragma unroll
+        for (int i = 0; i < kScannedTiles / 4; ++i) n[i] = i * 4 + q < k.tiles ? k.counts[(i * 4 + q) * 256 + d4] : 0;
+#pragma unroll
+        for (int i = 0; i < kScannedTiles / 4; ++i) {
+            all += n[i];
+            if (i * 4 + q < blockIdx.x) before += n[i];
+        }
+    }
+#pragma unroll
+    for (int s = 1; s < 4; s *= 2) {
+        all += __shfl_xor_sync(0xffffffffu, all, s);
+        before += __shfl_xor_sync(0xffffffffu, before, s);
+    }
+    uint32_t scan = all;  // of the warp's 8 digits
+#pragma unroll
+    for (int s = 4; s < 32; s *= 2) {
+        const uint32_t other = __shfl_up_sync(0xffffffffu, scan, s);
+        if (lane >= s) scan += other;
+    }
+    if (lane == 31) upto[warp] = scan;
+    for (int i = lane; i < 257; i += 32) place[warp][i] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const bool in = held_index<HELD>(k, h) < k.count;
+        const uint32_t d = in ? (x[h].x >> k.shift) & ((1u << k.bits) - 1) : 256u;
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        const uint32_t sofar = place[warp][d];
+        order[h] = sofar + __popc(peers & ((1u << lane) - 1));
+        __syncwarp();
+        if (lane == __ffs(peers) - 1) place[warp][d] = sofar + __popc(peers);
+        __syncwarp();
+    }
+    __syncthreads();
+    uint32_t below = lane < warp ? upto[lane] : 0;
+#pragma unroll
+    for (int s = 16; s > 0; s /= 2) below += __shfl_xor_sync(0xffffffffu, below, s);
+    if (q == 0) base[d4] = below + scan - all + before;
+    {  // exclusive over the warps: eight warps to a thread
+        uint32_t n[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            n[i] = place[q * 8 + i][d4];
+            sum += n[i];
+        }
+        uint32_t upper = sum;
+#pragma unroll
+        for (int s = 1; s < 4; s *= 2) {
+            const uint32_t other = __shfl_up_sync(0xffffffffu, upper, s, 4);
+            if (q >= s) upper += other;
+        }
+        upper -= sum;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            place[q * 8 + i][d4] = upper;
+            upper += n[i];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        if (held_index<HELD>(k, h) >= k.count) continue;
+        const uint32_t d = (x[h].x >> k.shift) & ((1u << k.bits) - 1);
+        k.to[base[d] + place[warp][d] + order[h]] = x[h];
     }
 }
 
-// The sorted tokens are cut into chunks of equal length.  Threads that share a row walk a chunk with a sum for each of their columns; where the id
-// changes, the sum is that row of the table, unless the id's tokens reach over an end of the chunk: such a sum is left in `partial`, [chunk][0]
-// where they began in an earlier chunk, [chunk][1] where they begin here, and join_kernel adds them up in order.
-constexpr int kSumThreads = 128;
+// A bit for each row of the table that has a token: from the sorted tokens, where each id comes up once.  (Marked by the first pass of the sort, frequent
+// ids' words took 20 us of queued atomics.)
+__global__ void __launch_bounds__(kSortThreads) mark_kernel(const SortArgs k) {
+    pdl_prologue();
+    if (zeros_block(k)) return;
+    const uint32_t i = blockIdx.x * kSortThreads + threadIdx.x;
+    if (i >= k.count) return;
+    const uint32_t id = k.from[i].x;
+    if (id < k.vocab && (i == 0 || k.from[i - 1].x != id)) atomicOr(&k.touched[id / 32], 1u << (id % 32));
+}
+
+// The sorted tokens are cut into chunks of equal length, one to each group of threads that share a row.  A thread walks its chunk with a sum for each
+// of its eight columns; where the id changes, the sum is that row of the table, unless the id's tokens reach over an end of the chunk.  Such sums meet in
+// shared memory: the group where they begin adds up those of the groups behind it.  What reaches over an end of the block is left in `partial`,
+// [block][0] where it began in an earlier block, [block][1] where it begins here, and join_kernel adds those up.  Always in the tokens' order.
+// Behind the blocks that sum come blocks that write zeros over rows without a token.
+constexpr int kSumThreads = 256;
 
 struct SumArgs {
     const uint2* tokens;
+    const uint32_t* touched;
     RowsArg rows;
     FastDiv inner;
     char* table;
     int64_t pitch;
-    float* partial;  // [chunks][2][width]
-    uint32_t count, vocab, chunk, chunks;
-    int width, threads;  // threads that share a row, a power of two
+    float* partial;  // [blocks][2][width]
+    uint32_t count, vocab, chunk, chunks, blocks;  // blocks: along the tokens
+    int width, threads, tiles;  // threads that share a row, a power of two up to 128; tiles of threads * 8 columns
     float scale;
     int accumulate;
+    uint32_t sum_blocks, zero_words;  // zero_words: groups of 32 rows to a block
+    Zeros zeros;
 };
 
 template <bool WIDE>
@@ -388,115 +481,158 @@ __device__ __forceinline__ void write_row(const SumArgs& k, uint32_t id, const f
 }
 
 template <typename TG, typename TO, bool WIDE>
-__global__ void __launch_bounds__(kSumThreads) sum_tokens_kernel(const SumArgs k) {
+__global__ void __launch_bounds__(kSumThreads, 2) sum_tokens_kernel(const SumArgs k) {
+    __shared__ float meet[2][8][kSumThreads];  // sums that reach over a chunk's end: [began earlier, begins here][column][thread]
+    // of each group: the id of its first and last token (V: none), and which sums it left: 1: began earlier, 2: begins here, 4: the first goes on behind the chunk
+    __shared__ uint32_t left[kSumThreads], first_id[kSumThreads], last_id[kSumThreads];
     pdl_prologue();
-    const int t = threadIdx.x % k.threads;
-    const uint32_t chunk = blockIdx.x * (kSumThreads / k.threads) + threadIdx.x / k.threads;
-    if (chunk >= k.chunks) return;
-    const int first = blockIdx.y * (k.threads * 8);
-    const uint32_t i0 = chunk * k.chunk, i1 = min(k.count, i0 + k.chunk);
-    uint32_t id = __ldg(&k.tokens[i0]).x;
-    if (id >= k.vocab) return;
-    bool open = i0 > 0 && __ldg(&k.tokens[i0 - 1]).x == id;  // its tokens began in an earlier chunk
-    const uint32_t next = i1 < k.count ? __ldg(&k.tokens[i1]).x : k.vocab;
-    float sum[8] = {};
-    auto leave = [&](int which) {
-        float* to = k.partial + (int64_t(chunk) * 2 + which) * k.width + first;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = sum_column<WIDE>(e, t, k.threads);
-            if (first + c < k.width) to[c] = sum[e];
+    if (blockIdx.x >= k.sum_blocks) {
+        const uint32_t word0 = (blockIdx.x - k.sum_blocks) * k.zero_words;
+        for (uint32_t w = word0; w < word0 + k.zero_words && w * 32 < k.zeros.rows; ++w) {
+            zero_rows(k.zeros, w * 32, min(32u, k.zeros.rows - w * 32), __ldg(&k.touched[w]), threadIdx.x, kSumThreads);
         }
-    };
-    constexpr int U = 4;  // rows under way
-    for (uint32_t i = i0; i < i1; i += U) {
-        uint2 token[U];
-        Piece<TG, WIDE> piece[U];
+        return;
+    }
+    const uint32_t block = blockIdx.x / k.tiles;
+    const int first = static_cast<int>(blockIdx.x % k.tiles) * (k.threads * 8);
+    const int groups = kSumThreads / k.threads, group = threadIdx.x / k.threads, t = threadIdx.x % k.threads;
+    const uint32_t chunk = block * groups + group;
+    const uint32_t i0 = min(k.count, chunk * k.chunk), i1 = min(k.count, i0 + k.chunk);
+    uint32_t id = k.vocab, marks = 0, start = k.vocab;
+    if (i0 < i1) {
+        start = id = __ldg(&k.tokens[i0]).x;
+        const uint32_t before = i0 > 0 ? __ldg(&k.tokens[i0 - 1]).x : k.vocab, next = i1 < k.count ? __ldg(&k.tokens[i1]).x : k.vocab;
+        bool open = id < k.vocab && before == id;  // its tokens began in an earlier chunk
+        float sum[8] = {};
+        auto leave = [&](int which) {
+            marks |= 1u << which;
 #pragma unroll
-        for (int u = 0; u < U; ++u) token[u] = i + u < i1 ? __ldg(&k.tokens[i + u]) : make_uint2(k.vocab, 0);
+            for (int e = 0; e < 8; ++e) meet[which][e][threadIdx.x] = sum[e];
+        };
+        constexpr int U = WIDE ? 8 : 4;  // rows under way, and the tokens behind them
+        uint2 token[U], next_token[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (token[u].x < k.vocab) piece[u].load(row_at(k.rows, k.inner, token[u].y), first, t, k.threads, k.width);
-        }
+        for (int u = 0; u < U; ++u) next_token[u] = i0 + u < i1 ? __ldg(&k.tokens[i0 + u]) : make_uint2(k.vocab, 0);
+        for (uint32_t i = i0; i < i1 && id < k.vocab; i += U) {
+            Piece<TG, WIDE> piece[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (token[u].x != id) {
-                if (id < k.vocab) {
-                    if (open) leave(0);
-                    else write_row<TO, WIDE>(k, id, sum, first, t);
-                }
-                open = false;
-                id = token[u].x;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+            for (int u = 0; u < U; ++u) {
+                token[u] = next_token[u];
+                if (token[u].x < k.vocab) piece[u].load(row_at(k.rows, k.inner, token[u].y), first, t, k.threads, k.width);
             }
-            if (id < k.vocab) {
-                float x[8];
-                piece[u].get(x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] += x[e];
+            for (int u = 0; u < U; ++u) next_token[u] = i + U + u < i1 ? __ldg(&k.tokens[i + U + u]) : make_uint2(k.vocab, 0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u >= i1) break;
+                if (token[u].x != id) {
+                    if (id < k.vocab) {
+                        if (open) leave(0);
+                        else write_row<TO, WIDE>(k, id, sum, first, t);
+                    }
+                    open = false;
+                    id = token[u].x;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+                }
+                if (id < k.vocab) {
+                    float x[8];
+                    piece[u].get(x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum[e] += x[e];
+                }
+            }
+        }
+        if (id < k.vocab) {
+            if (open) {
+                leave(0);
+                if (next == id) marks |= 4;
+            } else if (next == id) {
+                leave(1);
+            } else {
+                write_row<TO, WIDE>(k, id, sum, first, t);
             }
         }
     }
-    if (id < k.vocab) {
-        if (open) leave(0);
-        else if (next == id) leave(1);
-        else write_row<TO, WIDE>(k, id, sum, first, t);
+    if (t == 0) left[group] = marks, first_id[group] = start, last_id[group] = id;
+    __syncthreads();
+    // Sums that begin in this block, and the one that the block's first group continues from the block before.
+    for (int which = 1; which >= 0; --which) {
+        const bool mine = which == 1 ? (left[group] & 2) != 0 : group == 0 && (left[0] & 1) != 0;
+        if (!mine) continue;
+        float sum[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = meet[which][e][threadIdx.x];
+        bool on = which == 1 || (left[0] & 4) != 0;  // goes on into the next group
+        int g = group + 1;
+        for (; on && g < groups; ++g) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += meet[0][e][g * k.threads + t];
+            on = (left[g] & 4) != 0;
+        }
+        const uint32_t of = which == 1 ? last_id[group] : first_id[0];
+        if (which == 0 || on) {  // over an end of the block
+            float* to = k.partial + (int64_t(block) * 2 + which) * k.width + first;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = sum_column<WIDE>(e, t, k.threads);
+                if (first + c < k.width) to[c] = sum[e];
+            }
+        } else {
+            write_row<TO, WIDE>(k, of, sum, first, t);
+        }
     }
 }
 
-// One block for each chunk's end over which an id's tokens reach, where they begin in that chunk: 8 groups of threads take an eighth each of the chunks
-// that follow, in order, and the eighths are added in order.
-constexpr int kJoinGroups = 8;
+// One block for each end of a block of sums that an id's tokens reach over, where they begin in that block, and each kJoinColumns columns: four groups of
+// threads take a quarter each of the partial sums, in order, and the quarters are added in order.
+constexpr int kJoinColumns = 256, kJoinThreads = kJoinColumns / 4, kJoinGroups = 4;
 
-template <typename TO, bool WIDE>
-__global__ void __launch_bounds__(kSumThreads * kJoinGroups) join_kernel(const SumArgs k) {
-    __shared__ float part[kJoinGroups][kSumThreads * 8];
+template <typename TO>
+__global__ void __launch_bounds__(kJoinThreads * kJoinGroups) join_kernel(const SumArgs k) {
+    __shared__ float part[kJoinGroups][kJoinColumns];
     __shared__ uint32_t end;
     pdl_prologue();
-    const uint32_t chunk = blockIdx.x;
-    const uint32_t i1 = (chunk + 1) * k.chunk;  // (not the last chunk: the tokens go on)
-    const uint32_t id = __ldg(&k.tokens[i1]).x;
-    if (id >= k.vocab || __ldg(&k.tokens[i1 - 1]).x != id) return;
-    const uint32_t i0 = chunk * k.chunk;
-    if (i0 > 0 && __ldg(&k.tokens[i0]).x == id && __ldg(&k.tokens[i0 - 1]).x == id) return;  // they began earlier
-    // the first chunk from the next one on that does not begin with the id
-    if (threadIdx.x == 0) end = k.chunks;
+    const uint32_t span = k.chunk * (kSumThreads / k.threads);  // tokens of a block
+    const uint32_t block = blockIdx.x, i0 = block * span, i1 = i0 + span;  // (not the last block: the tokens go on)
+    const uint32_t before = i0 > 0 ? __ldg(&k.tokens[i0 - 1]).x : k.vocab, begin = __ldg(&k.tokens[i0]).x, last = __ldg(&k.tokens[i1 - 1]).x, id = __ldg(&k.tokens[i1]).x;
+    if (threadIdx.x == 0) end = k.blocks;
+    if (id >= k.vocab || last != id || (begin == id && before == id)) return;  // nothing over the end, or it began earlier
     __syncthreads();
-    for (uint32_t base = chunk + 1; base < k.chunks; base += blockDim.x) {
-        const uint32_t c = base + threadIdx.x;
-        if (c < k.chunks && __ldg(&k.tokens[c * k.chunk]).x != id) atomicMin(&end, c);
+    // the first block from the next one on that does not begin with the id
+    for (uint32_t from = block + 1; from < k.blocks; from += blockDim.x) {
+        const uint32_t c = from + threadIdx.x;
+        if (c < k.blocks && __ldg(&k.tokens[c * span]).x != id) atomicMin(&end, c);
         __syncthreads();
-        const bool found = end < k.chunks;
+        const bool found = end < k.blocks;
         __syncthreads();  // (before the next round's writes)
         if (found) break;
     }
-    const uint32_t parts = end - chunk;  // [chunk][1], then [chunk + 1 ..][0]
-    const int g = threadIdx.x / kSumThreads, t = threadIdx.x % kSumThreads;
+    const uint32_t parts = end - block;  // [block][1], then [block + 1 ..][0]
+    const int g = threadIdx.x / kJoinThreads, t = threadIdx.x % kJoinThreads;
     const uint32_t p0 = static_cast<uint32_t>(uint64_t(parts) * g / kJoinGroups), p1 = static_cast<uint32_t>(uint64_t(parts) * (g + 1) / kJoinGroups);
-    for (int first = 0; first < k.width; first += kSumThreads * 8) {
-        float sum[8] = {};
-#pragma unroll 4
-        for (uint32_t p = p0; p < p1; ++p) {
-            const float* from = k.partial + (int64_t(chunk + p) * 2 + (p == 0 ? 1 : 0)) * k.width + first;
+    const int first = blockIdx.y * kJoinColumns;
+    float sum[4] = {};
+#pragma unroll 8
+    for (uint32_t p = p0; p < p1; ++p) {
+        const float* from = k.partial + (int64_t(block + p) * 2 + (p == 0 ? 1 : 0)) * k.width + first;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = e * kSumThreads + t;
-                if (first + c < k.width) sum[e] += from[c];
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int c = e * kJoinThreads + t;
+            if (first + c < k.width) sum[e] += from[c];
         }
-        __syncthreads();
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part[g][e * kSumThreads + t] = sum[e];
-        __syncthreads();
-        for (int c = threadIdx.x; c < kSumThreads * 8 && first + c < k.width; c += blockDim.x) {
-            float total = part[0][c];
+    for (int e = 0; e < 4; ++e) part[g][e * kJoinThreads + t] = sum[e];
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (first + c < k.width) {
+        float total = part[0][c];
 #pragma unroll
-            for (int i = 1; i < kJoinGroups; ++i) total += part[i][c];
-            TO* to = reinterpret_cast<TO*>(k.table + int64_t(id) * k.pitch) + first + c;
-            const float x = total * k.scale + (k.accumulate ? to_float(*to) : 0.f);
-            *to = from_float<TO>(x);
-        }
+        for (int i = 1; i < kJoinGroups; ++i) total += part[i][c];
+        TO* to = reinterpret_cast<TO*>(k.table + int64_t(id) * k.pitch) + first + c;
+        const float x = total * k.scale + (k.accumulate ? to_float(*to) : 0.f);
+        *to = from_float<TO>(x);
     }
 }
 
@@ -549,7 +685,7 @@ void launch_lookup(b200_ctx* ctx, const b200_embedding_args& a) {
     const Problem p = check_embedding(a, false);
     if (p.count == 0 || p.width == 0) return;
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
-    const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, 16) && reinterpret_cast<uintptr_t>(a.table.data) % 16 == 0 && p.pitch % 16 == 0;
+    const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
     const int64_t pieces = wide ? p.width / 8 : p.width, total = p.count * pieces;
     const int64_t blocks = ceil_div(total, kThreads * kItems);
     if (blocks >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "embedding: too many elements");
@@ -566,9 +702,11 @@ void launch_lookup(b200_ctx* ctx, const b200_embedding_args& a) {
 
 // How a gradient of many tokens is divided, and where its scratch lies.
 struct Division {
-    uint32_t chunk, chunks;
+    uint32_t chunk, chunks, blocks;
     int threads, tiles;
-    int64_t token_bytes, partial_bytes;
+    int held;             // tokens of a thread that sorts
+    uint32_t sort_tiles;
+    int64_t token_bytes, touched_bytes, partial_bytes, count_bytes;
     size_t bytes;
 };
 
@@ -579,15 +717,24 @@ Division divide(const Problem& p) {
     Division d{};
     if (p.count <= kOwnedTokens || p.vocab == 0 || p.width == 0) return d;
     d.threads = 1;
-    while (d.threads < kSumThreads && d.threads * 8 < p.width) d.threads *= 2;
+    while (d.threads < 128 && d.threads * 8 < p.width) d.threads *= 2;
     d.tiles = static_cast<int>(ceil_div(p.width, int64_t(d.threads) * 8));
-    // chunks of 16 to 128 tokens: short ones where there are few tokens, so that each SM has eight chunks of whole rows; long ones leave fewer partial sums
-    d.chunk = 16;
-    while (d.chunk < 128 && p.count / d.chunk > int64_t(sm_count()) * 16) d.chunk *= 2;
+    const int groups = kSumThreads / d.threads;
+    // two waves of blocks, two to an SM, of chunks that are no longer than 256 tokens
+    const int64_t wave = std::max<int64_t>(1, int64_t(sm_count()) * 4 / d.tiles);
+    d.chunk = static_cast<uint32_t>(std::min<int64_t>(256, std::max<int64_t>(4, ceil_div(ceil_div(p.count, wave * groups), 4) * 4)));
     d.chunks = static_cast<uint32_t>(ceil_div(p.count, int64_t(d.chunk)));
-    d.token_bytes = (p.count * 8 + 255) / 256 * 256;
-    d.partial_bytes = (int64_t(d.chunks) * 2 * p.width * 4 + 255) / 256 * 256;
-    d.bytes = static_cast<size_t>(2 * d.token_bytes + d.partial_bytes);
+    d.blocks = static_cast<uint32_t>(ceil_div(int64_t(d.chunks), groups));
+    auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    d.token_bytes = whole(p.count * 8);
+    d.touched_bytes = whole(ceil_div(p.vocab, 32) * 4);
+    d.partial_bytes = whole(int64_t(d.blocks) * 2 * p.width * 4);
+    // few tiles, as every block adds up the counts of all; but a thread holds eight tokens at most
+    d.held = 1;
+    while (d.held < kMostHeld && ceil_div(p.count, int64_t(kSortThreads) * d.held) > kScannedTiles) d.held *= 2;
+    d.sort_tiles = static_cast<uint32_t>(ceil_div(p.count, int64_t(kSortThreads) * d.held));
+    d.count_bytes = int64_t(d.sort_tiles) * 1024 + 1024;
+    d.bytes = static_cast<size_t>(2 * d.token_bytes + d.touched_bytes + d.partial_bytes + d.count_bytes);
     return d;
 }
 
@@ -609,87 +756,112 @@ void launch_owned_rows(b200_ctx* ctx, const b200_embedding_args& a, const Proble
     ctx->count_launch();
 }
 
-// The blocks of the sorting cluster: 16, where the device takes clusters that large, else 8.
-int sort_cluster() {
-    static int known[64] = {};
-    int dev = 0;
-    B200_CUDA_CHECK(cudaGetDevice(&dev));
-    int& n = known[dev & 63];
-    if (n == 0) {
-        n = 8;
-        if (cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = 16;
-            cfg.blockDim = kSortThreads;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 16;
-            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            int fit = 0;
-            if (cudaOccupancyMaxActiveClusters(&fit, sort_tokens_kernel, &cfg) == cudaSuccess && fit > 0) n = 16;
-        }
-        cudaGetLastError();
-    }
-    return n;
-}
+// Zeros written beside each of the sort's kernels: what the memory takes in the two microseconds or so of one.
+constexpr int64_t kZerosBesideSort = int64_t(10) << 20;
 
 void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p, const Division& d) {
     char* scratch = operator_workspace(ctx, a.workspace, a.workspace_bytes, d.bytes);
+    const bool accumulate = (a.flags & B200_ACCUMULATE) != 0;
+    const int64_t size = static_cast<int64_t>(dtype_size(a.table.dtype)), row_bytes = p.width * size;
+    uint2* buffer[2] = {reinterpret_cast<uint2*>(scratch), reinterpret_cast<uint2*>(scratch + d.token_bytes)};
+    scratch += 2 * d.token_bytes;
     SortArgs s{};
     s.ids = p.ids;
-    s.buffer[0] = reinterpret_cast<uint2*>(scratch);
-    s.buffer[1] = reinterpret_cast<uint2*>(scratch + d.token_bytes);
+    s.touched = accumulate ? nullptr : reinterpret_cast<uint32_t*>(scratch);
+    scratch += d.touched_bytes;
+    float* partial = reinterpret_cast<float*>(scratch);
+    scratch += d.partial_bytes;
+    s.totals = reinterpret_cast<uint32_t*>(scratch);
+    s.counts = s.totals + 256;
     s.count = static_cast<uint32_t>(p.count);
     s.vocab = static_cast<uint32_t>(p.vocab);
     s.padding = a.padding_id < 0 ? INT64_MIN : a.padding_id;
+    s.tiles = d.sort_tiles;
+    s.tile = static_cast<uint32_t>(kSortThreads * d.held);
+    s.scanned = d.sort_tiles > kScannedTiles;
+    s.status = ctx->d_status;
     int bits = 1;
     while ((int64_t(1) << bits) <= p.vocab) ++bits;
-    s.passes = (bits + 7) / 8;
-    s.digit_bits = (bits + s.passes - 1) / s.passes;
-    const bool accumulate = (a.flags & B200_ACCUMULATE) != 0;
-    s.table = accumulate ? nullptr : static_cast<char*>(a.table.data);
-    s.pitch = p.vocab > 1 ? p.pitch : p.width * static_cast<int64_t>(dtype_size(a.table.dtype));
-    s.row_bytes = p.width * static_cast<int64_t>(dtype_size(a.table.dtype));
-    s.status = ctx->d_status;
-    const int cluster = sort_cluster();
-    const unsigned clusters = accumulate ? 1u : static_cast<unsigned>(std::max(2, sm_count() * 2 / cluster));
-    launch_kernel_clustered(ctx, sort_tokens_kernel, dim3(clusters * cluster), dim3(kSortThreads), 0, cluster, true, s);
-    check_last_launch("embedding_backward");
+    const int passes = (bits + 7) / 8;
+    s.bits = (bits + passes - 1) / passes;
+    Zeros zeros{};
+    uint32_t zeros_left = 0;  // rows, from the first on, whose zeros are not written yet
+    int64_t early = 0;        // rows beside each kernel of the sort
+    if (!accumulate) {
+        zeros.table = static_cast<char*>(a.table.data);
+        zeros.pitch = p.pitch;
+        zeros.wide = ((reinterpret_cast<uintptr_t>(zeros.table) | static_cast<uintptr_t>(p.pitch) | static_cast<uintptr_t>(row_bytes)) & 15) == 0;
+        zeros.pieces = FastDiv(static_cast<uint32_t>(row_bytes / (zeros.wide ? 16 : 2)));
+        zeros_left = s.vocab;
+        early = kZerosBesideSort / row_bytes / 32 * 32;
+    }
+    auto sort = [&](auto kernel) {
+        s.zeros = zeros;
+        s.zeros.row0 = static_cast<uint32_t>(zeros_left > early ? (zeros_left - early + 31) / 32 * 32 : 0);
+        s.zeros.rows = zeros_left > s.zeros.row0 ? zeros_left - s.zeros.row0 : 0;
+        zeros_left -= s.zeros.rows;
+        const int64_t beside = std::min<int64_t>(sm_count() * 2, ceil_div(int64_t(s.zeros.rows), 32));
+        launch_kernel(ctx, kernel, dim3(s.tiles + static_cast<unsigned>(beside)), kSortThreads, 0, s);
+        check_last_launch("embedding_backward");
+        ctx->count_launch();
+    };
+    for (int pass = 0; pass < passes; ++pass) {
+        s.from = pass == 0 ? nullptr : buffer[(pass + 1) & 1];
+        s.to = buffer[pass & 1];
+        s.shift = pass * s.bits;
+        sort(d.held == 1 ? count_kernel<1> : d.held == 2 ? count_kernel<2> : d.held == 4 ? count_kernel<4> : count_kernel<8>);
+        if (s.scanned) {
+            launch_kernel(ctx, scan_kernel, dim3(256), kSortThreads, 0, s);
+            check_last_launch("embedding_backward");
+            ctx->count_launch();
+        }
+        sort(d.held == 1 ? move_kernel<1> : d.held == 2 ? move_kernel<2> : d.held == 4 ? move_kernel<4> : move_kernel<8>);
+    }
+    if (!accumulate) {
+        s.from = s.to;
+        s.tiles = static_cast<uint32_t>(ceil_div(p.count, kSortThreads));
+        sort(mark_kernel);
+    }
 
     SumArgs k{};
-    k.tokens = s.buffer[(s.passes + 1) & 1];
+    k.tokens = s.to;
+    k.touched = s.touched;
     k.rows = p.rows;
     k.inner = p.ids.inner;
     k.table = static_cast<char*>(a.table.data);
     k.pitch = p.pitch;
-    k.partial = reinterpret_cast<float*>(scratch + 2 * d.token_bytes);
+    k.partial = partial;
     k.count = s.count;
     k.vocab = s.vocab;
     k.chunk = d.chunk;
     k.chunks = d.chunks;
+    k.blocks = d.blocks;
     k.width = static_cast<int>(p.width);
     k.threads = d.threads;
+    k.tiles = d.tiles;
     k.scale = a.scale;
     k.accumulate = accumulate;
-    const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, 16) && reinterpret_cast<uintptr_t>(a.table.data) % 16 == 0 && p.pitch % 16 == 0;
-    const dim3 grid(static_cast<unsigned>(ceil_div(int64_t(d.chunks) * d.threads, kSumThreads)), static_cast<unsigned>(d.tiles));
+    k.sum_blocks = d.blocks * static_cast<uint32_t>(d.tiles);
+    k.zeros = zeros;
+    k.zeros.rows = zeros_left;
+    k.zero_words = static_cast<uint32_t>(std::max<int64_t>(1, (128 << 10) / (32 * row_bytes)));
+    const uint32_t zero_blocks = static_cast<uint32_t>(ceil_div(ceil_div(int64_t(zeros_left), 32), int64_t(k.zero_words)));
+    const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
     with_types(a.table.dtype, a.rows.dtype, [&](auto to, auto tg) {
         using TO = decltype(to);
         using TG = decltype(tg);
-        launch_kernel(ctx, wide ? sum_tokens_kernel<TG, TO, true> : sum_tokens_kernel<TG, TO, false>, grid, kSumThreads, 0, k);
+        launch_kernel(ctx, wide ? sum_tokens_kernel<TG, TO, true> : sum_tokens_kernel<TG, TO, false>, dim3(k.sum_blocks + zero_blocks), kSumThreads, 0, k);
         check_last_launch("embedding_backward");
-        if (d.chunks > 1) launch_kernel(ctx, wide ? join_kernel<TO, true> : join_kernel<TO, false>, dim3(d.chunks - 1), kSumThreads * kJoinGroups, 0, k);
+        if (d.blocks > 1) launch_kernel(ctx, join_kernel<TO>, dim3(d.blocks - 1, static_cast<unsigned>(ceil_div(p.width, kJoinColumns))), kJoinThreads * kJoinGroups, 0, k);
     });
     check_last_launch("embedding_backward");
-    ctx->count_launch(d.chunks > 1 ? 3 : 2);
+    ctx->count_launch(d.blocks > 1 ? 3 : 2);
 }
 
 void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
     const Problem p = check_embedding(a, true);
     if (p.vocab == 0 || p.width == 0) return;
-    if (p.width > int64_t(65535) * 1024) fail(B200_SHAPE_ERROR, "embedding_backward: a row of more than 65535 * 1024 elements");
+    if (p.width >= int64_t(1) << 24) fail(B200_SHAPE_ERROR, "embedding_backward: a row of 2^24 elements or more");
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
     ProfScope scope(ctx, "embedding_backward");
     const Division d = divide(p);

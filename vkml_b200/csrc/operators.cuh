@@ -134,7 +134,9 @@ inline RowsArg rows_arg(const b200_tensor& t, int axes) {
     return r;
 }
 
-inline bool aligned_rows(const RowsArg& r, int64_t bytes) {
+// Whether rows can be read and written eight elements at a time (load8, store8), given that their width is a multiple of eight.
+inline bool aligned_rows(const RowsArg& r, int dtype) {
+    const int64_t bytes = 8 * static_cast<int64_t>(dtype_size(dtype));
     return r.base == nullptr || (reinterpret_cast<uintptr_t>(r.base) % static_cast<uintptr_t>(bytes) == 0 && r.outer % bytes == 0 && r.step % bytes == 0);
 }
 
@@ -280,7 +282,7 @@ __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
-// Eight elements of a row as they lie in memory: 16 bytes of F16 or 32 of F32, moved 16 bytes at a time.
+// Eight elements of a row as they lie in memory: 16 bytes of F16 or 32 of F32, moved in one access of that width and alignment.
 template <typename T>
 struct Raw8;
 template <>
@@ -289,13 +291,15 @@ struct Raw8<__half> {
 };
 template <>
 struct Raw8<float> {
-    uint4 a, b;
+    float a[8];
 };
 
 __device__ __forceinline__ void load8(Raw8<__half>& r, const __half* p) { r.a = *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ void load8(Raw8<float>& r, const float* p) {
-    r.a = reinterpret_cast<const uint4*>(p)[0];
-    r.b = reinterpret_cast<const uint4*>(p)[1];
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(r.a[0]), "=f"(r.a[1]), "=f"(r.a[2]), "=f"(r.a[3]), "=f"(r.a[4]), "=f"(r.a[5]), "=f"(r.a[6]), "=f"(r.a[7])
+                 : "l"(__cvta_generic_to_global(p))
+                 : "memory");
 }
 
 __device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&x)[8]) {
@@ -308,9 +312,8 @@ __device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&x)[8]) {
     }
 }
 __device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&x)[8]) {
-    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+    for (int i = 0; i < 8; ++i) x[i] = r.a[i];
 }
 
 __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
@@ -323,8 +326,9 @@ __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+                 "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
 }
 
 // Where row r of a tensor lies.
