@@ -84,7 +84,26 @@ def test_gradient(backend, row_type, table_type, shape, vocab, width, layout, ac
     backend.synchronize()
 
 
-@pytest.mark.parametrize("count,vocab", [(3000, 4), (30000, 50000)])
+@pytest.mark.parametrize("count,vocab,width", [(1024, 255, 8), (1025, 256, 8), (16384, 65535, 4), (16385, 65536, 4), (70001, 300, 3), (131072, 70000, 8), (131073, 900, 8),
+                                               (600000, 66000, 5), (1200000, 130, 8)])
+@pytest.mark.parametrize("skew", [False, True])
+def test_gradient_of_many_tokens(backend, count, vocab, width, skew):
+    """Counts at which the sort changes over, and ids of one, two and three digits."""
+    rng = np.random.default_rng(count)
+    ids = ids_of(rng, (count,), vocab, np.int32 if skew else np.int64, skew)
+    grad = rng.standard_normal((count, width)).astype(np.float32)
+    table = np.full((vocab, width), np.nan, np.float32)
+    space = Space(backend)
+    g, i, t = space.put(grad), space.put(ids), space.put(table)
+    backend.embedding_backward(g, i, t)
+    got = space.get(table)[0]
+    want, bound, touched = embedding_backward(ids, grad, vocab, 1.0, None, None)
+    check(got, want, bound, np.float32, "table gradient")
+    assert not got[~touched].any()
+    backend.synchronize()
+
+
+@pytest.mark.parametrize("count,vocab", [(3000, 4), (30000, 50000), (200000, 9)])
 def test_gradient_of_one_token(backend, count, vocab):
     """Every token the same: one list, as long as there are tokens."""
     rng = np.random.default_rng(5)

@@ -181,10 +181,11 @@ owned_rows_kernel(char* table, int64_t pitch, RowsArg grad, Ids ids, uint32_t co
 // the tokens, a warp a stretch of the tile.  count_kernel leaves the counts of the tile's digits; move_kernel ranks every token among those of
 // its digit in its stretch, adds the counts of the warps, the tiles and the digits before, and moves each token to its place.  Tokens that have no gradient
 // sort behind all others, as id V.  The memory is idle meanwhile, so
-// blocks behind those that sort write zeros over the table's last rows; the rest of the rows without a token is written beside the sums.
-// (One cluster of 16 blocks that counts through its shared memory was 14 us for any number of tokens and 50 us for 131072 of them.)
+// blocks behind those that sort write zeros over the table's last rows; the sums leave a bit for each row that has a token, and the rest of the
+// rows without one is written at the end.  Up to 32768 tokens one cluster of blocks sorts in one launch (sort_cluster_kernel).
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kMostHeld = 8;        // tokens of a thread
+constexpr int kMostHeld = 8;        // tokens of a thread of many blocks
+constexpr int kMostClusterHeld = 2; // ... and of a cluster's: 131072 tokens by 16 blocks of 8 to a thread took 40 us, by 64 blocks 27
 constexpr int kScannedTiles = 64;   // up to here move_kernel adds up the tiles' counts itself; above, scan_kernel does beforehand
 
 // Rows of the table that are to be zeros.
@@ -202,7 +203,7 @@ struct SortArgs {
     uint2* to;
     uint32_t* counts;    // [tiles][256]; from scan_kernel, the counts of the tiles before
     uint32_t* totals;    // [256], from scan_kernel
-    uint32_t* touched;   // a bit for each row, or null
+    uint32_t* touched;   // a bit for each row, cleared here; or null
     uint32_t count, vocab, tiles, tile;  // tile: tokens of one
     int64_t padding;
     int shift, bits;
@@ -241,6 +242,18 @@ __device__ __forceinline__ uint2 sort_token(const SortArgs& k, uint32_t i, bool 
     return make_uint2(in && id != k.padding ? static_cast<uint32_t>(id) : k.vocab, i);
 }
 
+// The lanes that have the same digit (none: 256 and above), in nine votes.
+__device__ __forceinline__ uint32_t same_digit(uint32_t d) {
+    const uint32_t in = __ballot_sync(0xffffffffu, d < 256);
+    uint32_t peers = d < 256 ? in : ~in;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const uint32_t ones = __ballot_sync(0xffffffffu, (d >> b) & 1);
+        peers &= (d >> b) & 1 ? ones : ~ones;
+    }
+    return peers;
+}
+
 // HELD tokens of each thread, all under way at once: warp w has the 32 * HELD tokens from w * 32 * HELD on, 32 neighbours at a time.
 template <int HELD>
 __device__ __forceinline__ uint32_t held_index(const SortArgs& k, int h) {
@@ -267,7 +280,7 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const SortArgs k) {
     for (int h = 0; h < HELD; ++h) {
         const bool in = held_index<HELD>(k, h) < k.count;
         const uint32_t d = in ? (x[h].x >> k.shift) & ((1u << k.bits) - 1) : 256u;
-        const uint32_t peers = __match_any_sync(0xffffffffu, d);  // (frequent tokens would queue up at one counter)
+        const uint32_t peers = same_digit(d);  // (frequent tokens would queue up at one counter)
         if (in && threadIdx.x % 32 == __ffs(peers) - 1) atomicAdd(&counts[d], __popc(peers));
     }
     __syncthreads();
@@ -352,7 +365,7 @@ __global__ void __launch_bounds__(kSortThreads) move_kernel(const SortArgs k) {
     for (int h = 0; h < HELD; ++h) {
         const bool in = held_index<HELD>(k, h) < k.count;
         const uint32_t d = in ? (x[h].x >> k.shift) & ((1u << k.bits) - 1) : 256u;
-        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        const uint32_t peers = same_digit(d);
         const uint32_t sofar = place[warp][d];
         order[h] = sofar + __popc(peers & ((1u << lane) - 1));
         __syncwarp();
@@ -393,27 +406,165 @@ __global__ void __launch_bounds__(kSortThreads) move_kernel(const SortArgs k) {
     }
 }
 
-// A bit for each row of the table that has a token: from the sorted tokens, where each id comes up once.  (Marked by the first pass of the sort, frequent
-// ids' words took 20 us of queued atomics.)
-__global__ void __launch_bounds__(kSortThreads) mark_kernel(const SortArgs k) {
+// The same sort by the blocks of one cluster, which hold all tokens: a pass reads the counts of the other blocks and moves the tokens through the cluster's
+// shared memory.  One launch where the kernels above are four.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_blocks() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+// Where the shared memory at `mine` lies in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_address(const void* mine, uint32_t rank) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ uint32_t cluster_load(uint32_t at) {
+    uint32_t x;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return x;
+}
+__device__ __forceinline__ void cluster_store(uint32_t at, uint2 x) {
+    asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(x.x), "r"(x.y) : "memory");
+}
+constexpr int kMostCluster = 16;
+
+template <int HELD>
+__global__ void __launch_bounds__(kSortThreads) sort_cluster_kernel(SortArgs k) {
+    extern __shared__ uint2 held[];              // [kSortThreads * HELD]: this block's tokens between passes
+    __shared__ uint32_t place[kSortWarps][257];  // (as in move_kernel)
+    __shared__ uint32_t total[256], local[256], base[256], upto[kSortWarps];
     pdl_prologue();
-    if (zeros_block(k)) return;
-    const uint32_t i = blockIdx.x * kSortThreads + threadIdx.x;
-    if (i >= k.count) return;
-    const uint32_t id = k.from[i].x;
-    if (id < k.vocab && (i == 0 || k.from[i - 1].x != id)) atomicOr(&k.touched[id / 32], 1u << (id % 32));
+    const uint32_t blocks = cluster_blocks(), rank = cluster_rank();
+    k.tiles = blocks;  // (the first cluster's blocks are the tiles)
+    if (zeros_block(k)) return;  // (whole clusters)
+    constexpr uint32_t kTile = kSortThreads * HELD;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, d4 = tid / 4, q = tid % 4;
+    if (k.touched != nullptr) {
+        for (uint32_t i = rank * kSortThreads + tid; i < (k.vocab + 31) / 32; i += blocks * kSortThreads) k.touched[i] = 0;
+    }
+    uint2 x[HELD];
+    uint32_t order[HELD];
+    for (k.shift = 0; k.shift < 32 && (k.vocab >> k.shift) != 0; k.shift += k.bits) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const uint32_t i = held_index<HELD>(k, h);
+            if (i < k.count) x[h] = k.shift == 0 ? sort_token(k, i, true) : held[i - rank * kTile];
+        }
+        for (int i = lane; i < 257; i += 32) place[warp][i] = 0;
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const bool in = held_index<HELD>(k, h) < k.count;
+            const uint32_t d = in ? (x[h].x >> k.shift) & ((1u << k.bits) - 1) : 256u;
+            const uint32_t peers = same_digit(d);
+            const uint32_t sofar = place[warp][d];
+            order[h] = sofar + __popc(peers & ((1u << lane) - 1));
+            __syncwarp();
+            if (lane == __ffs(peers) - 1) place[warp][d] = sofar + __popc(peers);
+            __syncwarp();
+        }
+        __syncthreads();
+        uint32_t mine = 0;  // this block's tokens of digit d4
+        {  // exclusive over the warps
+            uint32_t n[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                n[i] = place[q * 8 + i][d4];
+                sum += n[i];
+            }
+            uint32_t upper = sum;
+#pragma unroll
+            for (int s = 1; s < 4; s *= 2) {
+                const uint32_t other = __shfl_up_sync(0xffffffffu, upper, s, 4);
+                if (q >= s) upper += other;
+            }
+            mine = __shfl_sync(0xffffffffu, upper, 3, 4);
+            if (q == 0) total[d4] = mine;
+            upper -= sum;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                place[q * 8 + i][d4] = upper;
+                upper += n[i];
+            }
+        }
+        // The digits before, among this block's tokens: these are put in order here first, so that neighbours move to the other blocks together.
+        auto digits_before = [&](uint32_t n) {
+            uint32_t scan = n;  // of the warp's 8 digits
+#pragma unroll
+            for (int s = 4; s < 32; s *= 2) {
+                const uint32_t other = __shfl_up_sync(0xffffffffu, scan, s);
+                if (lane >= s) scan += other;
+            }
+            if (lane == 31) upto[warp] = scan;
+            __syncthreads();
+            uint32_t below = lane < warp ? upto[lane] : 0;
+#pragma unroll
+            for (int s = 16; s > 0; s /= 2) below += __shfl_xor_sync(0xffffffffu, below, s);
+            return below + scan - n;
+        };
+        const uint32_t here = digits_before(mine);
+        if (q == 0) local[d4] = here;
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (held_index<HELD>(k, h) >= k.count) continue;
+            const uint32_t d = (x[h].x >> k.shift) & ((1u << k.bits) - 1);
+            held[local[d] + place[warp][d] + order[h]] = x[h];
+        }
+        __syncthreads();
+        const uint32_t tokens = min(k.count, (rank + 1) * kTile) - min(k.count, rank * kTile);
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            if (h * kSortThreads + tid < tokens) x[h] = held[h * kSortThreads + tid];
+        }
+        cluster_sync();  // the counts are there, and every block's tokens are in registers
+        uint32_t n[kMostCluster / 4], all = 0, before = 0;
+#pragma unroll
+        for (int i = 0; i < kMostCluster / 4; ++i) n[i] = i * 4 + q < blocks ? cluster_load(cluster_address(&total[d4], i * 4 + q)) : 0;
+#pragma unroll
+        for (int i = 0; i < kMostCluster / 4; ++i) {
+            all += n[i];
+            if (i * 4 + q < rank) before += n[i];
+        }
+#pragma unroll
+        for (int s = 1; s < 4; s *= 2) {
+            all += __shfl_xor_sync(0xffffffffu, all, s);
+            before += __shfl_xor_sync(0xffffffffu, before, s);
+        }
+        const uint32_t everywhere = digits_before(all);
+        if (q == 0) base[d4] = everywhere + before - here;  // a token's place from its place in this block
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const uint32_t slot = h * kSortThreads + tid;
+            if (slot >= tokens) continue;
+            const uint32_t at = base[(x[h].x >> k.shift) & ((1u << k.bits) - 1)] + slot;
+            cluster_store(cluster_address(&held[at % kTile], at / kTile), x[h]);
+        }
+        cluster_sync();  // the moved tokens are there, and no block reads another's counts any more
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const uint32_t slot = h * kSortThreads + tid, i = rank * kTile + slot;
+        if (i < k.count) k.to[i] = held[slot];
+    }
 }
 
 // The sorted tokens are cut into chunks of equal length, one to each group of threads that share a row.  A thread walks its chunk with a sum for each
 // of its eight columns; where the id changes, the sum is that row of the table, unless the id's tokens reach over an end of the chunk.  Such sums meet in
 // shared memory: the group where they begin adds up those of the groups behind it.  What reaches over an end of the block is left in `partial`,
 // [block][0] where it began in an earlier block, [block][1] where it begins here, and join_kernel adds those up.  Always in the tokens' order.
-// Behind the blocks that sum come blocks that write zeros over rows without a token.
 constexpr int kSumThreads = 256;
 
 struct SumArgs {
     const uint2* tokens;
-    const uint32_t* touched;
+    uint32_t* touched;   // a bit for each row that has a token; null: not wanted
     RowsArg rows;
     FastDiv inner;
     char* table;
@@ -423,7 +574,7 @@ struct SumArgs {
     int width, threads, tiles;  // threads that share a row, a power of two up to 128; tiles of threads * 8 columns
     float scale;
     int accumulate;
-    uint32_t sum_blocks, zero_words;  // zero_words: groups of 32 rows to a block
+    uint32_t join_blocks, zero_words;  // join_kernel's blocks; groups of 32 rows to each of its blocks behind those
     Zeros zeros;
 };
 
@@ -458,9 +609,15 @@ struct Piece<T, false> {
     }
 };
 
+// Once for each row that has a token.
+__device__ __forceinline__ void mark_row(const SumArgs& k, uint32_t id, int first, int t) {
+    if (k.touched != nullptr && first == 0 && t == 0) atomicOr(&k.touched[id / 32], 1u << (id % 32));
+}
+
 template <typename TO, bool WIDE>
 __device__ __forceinline__ void write_row(const SumArgs& k, uint32_t id, const float (&sum)[8], int first, int t) {
     char* row = k.table + int64_t(id) * k.pitch;
+    mark_row(k, id, first, t);
     float x[8] = {};
     if (k.accumulate) {
         Piece<TO, WIDE> old;
@@ -486,13 +643,6 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_tokens_kernel(const SumArg
     // of each group: the id of its first and last token (V: none), and which sums it left: 1: began earlier, 2: begins here, 4: the first goes on behind the chunk
     __shared__ uint32_t left[kSumThreads], first_id[kSumThreads], last_id[kSumThreads];
     pdl_prologue();
-    if (blockIdx.x >= k.sum_blocks) {
-        const uint32_t word0 = (blockIdx.x - k.sum_blocks) * k.zero_words;
-        for (uint32_t w = word0; w < word0 + k.zero_words && w * 32 < k.zeros.rows; ++w) {
-            zero_rows(k.zeros, w * 32, min(32u, k.zeros.rows - w * 32), __ldg(&k.touched[w]), threadIdx.x, kSumThreads);
-        }
-        return;
-    }
     const uint32_t block = blockIdx.x / k.tiles;
     const int first = static_cast<int>(blockIdx.x % k.tiles) * (k.threads * 8);
     const int groups = kSumThreads / k.threads, group = threadIdx.x / k.threads, t = threadIdx.x % k.threads;
@@ -572,6 +722,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_tokens_kernel(const SumArg
         }
         const uint32_t of = which == 1 ? last_id[group] : first_id[0];
         if (which == 0 || on) {  // over an end of the block
+            if (which == 1) mark_row(k, of, first, t);
             float* to = k.partial + (int64_t(block) * 2 + which) * k.width + first;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -585,7 +736,8 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_tokens_kernel(const SumArg
 }
 
 // One block for each end of a block of sums that an id's tokens reach over, where they begin in that block, and each kJoinColumns columns: four groups of
-// threads take a quarter each of the partial sums, in order, and the quarters are added in order.
+// threads take a quarter each of the partial sums, in order, and the quarters are added in order.  Few of these blocks have something to do, and that
+// waits more than it moves; so the zeros of rows without a token are written by blocks behind them.
 constexpr int kJoinColumns = 256, kJoinThreads = kJoinColumns / 4, kJoinGroups = 4;
 
 template <typename TO>
@@ -593,8 +745,16 @@ __global__ void __launch_bounds__(kJoinThreads * kJoinGroups) join_kernel(const 
     __shared__ float part[kJoinGroups][kJoinColumns];
     __shared__ uint32_t end;
     pdl_prologue();
+    if (blockIdx.x >= k.join_blocks) {
+        const uint32_t word0 = (blockIdx.x - k.join_blocks) * k.zero_words;
+        for (uint32_t w = word0; w < word0 + k.zero_words && w * 32 < k.zeros.rows; ++w) {
+            zero_rows(k.zeros, w * 32, min(32u, k.zeros.rows - w * 32), __ldg(&k.touched[w]), threadIdx.x, kJoinThreads * kJoinGroups);
+        }
+        return;
+    }
     const uint32_t span = k.chunk * (kSumThreads / k.threads);  // tokens of a block
-    const uint32_t block = blockIdx.x, i0 = block * span, i1 = i0 + span;  // (not the last block: the tokens go on)
+    const int column_blocks = (k.width + kJoinColumns - 1) / kJoinColumns;
+    const uint32_t block = blockIdx.x / column_blocks, i0 = block * span, i1 = i0 + span;  // (not the last block: the tokens go on)
     const uint32_t before = i0 > 0 ? __ldg(&k.tokens[i0 - 1]).x : k.vocab, begin = __ldg(&k.tokens[i0]).x, last = __ldg(&k.tokens[i1 - 1]).x, id = __ldg(&k.tokens[i1]).x;
     if (threadIdx.x == 0) end = k.blocks;
     if (id >= k.vocab || last != id || (begin == id && before == id)) return;  // nothing over the end, or it began earlier
@@ -611,7 +771,7 @@ __global__ void __launch_bounds__(kJoinThreads * kJoinGroups) join_kernel(const 
     const uint32_t parts = end - block;  // [block][1], then [block + 1 ..][0]
     const int g = threadIdx.x / kJoinThreads, t = threadIdx.x % kJoinThreads;
     const uint32_t p0 = static_cast<uint32_t>(uint64_t(parts) * g / kJoinGroups), p1 = static_cast<uint32_t>(uint64_t(parts) * (g + 1) / kJoinGroups);
-    const int first = blockIdx.y * kJoinColumns;
+    const int first = static_cast<int>(blockIdx.x % column_blocks) * kJoinColumns;
     float sum[4] = {};
 #pragma unroll 8
     for (uint32_t p = p0; p < p1; ++p) {
@@ -700,11 +860,55 @@ void launch_lookup(b200_ctx* ctx, const b200_embedding_args& a) {
     ctx->count_launch();
 }
 
+using SortCluster = void (*)(SortArgs);
+SortCluster sort_cluster(int held) {
+    return held == 1 ? sort_cluster_kernel<1> : sort_cluster_kernel<2>;
+}
+
+// How many clusters of `blocks` blocks the current device holds at once; 0 where it takes none of them.
+int clusters_at_once(int held, int blocks) {
+    static int known[64][2][5] = {};  // device, held, blocks: one more than the answer
+    int dev = 0, h = 0, b = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return blocks <= 8 ? 1 : 0;
+    }
+    while ((1 << h) < held) ++h;
+    while ((1 << b) < blocks) ++b;
+    int& n = known[dev & 63][h][b];
+    if (n == 0) {
+        const size_t shared = static_cast<size_t>(kSortThreads) * held * sizeof(uint2);
+        int fit = 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = static_cast<unsigned>(blocks);
+        cfg.blockDim = kSortThreads;
+        cfg.dynamicSmemBytes = shared;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const SortCluster kernel = sort_cluster(held);
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess ||
+            (blocks > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+            cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess) {
+            fit = 0;
+        }
+        cudaGetLastError();
+        n = fit + 1;
+    }
+    return n - 1;
+}
+// (Where there is no device to ask, for the size of a workspace: the larger answer of the two is the smaller cluster's.)
+int largest_cluster() { return clusters_at_once(kMostClusterHeld, kMostCluster) > 0 ? kMostCluster : 8; }
+
 // How a gradient of many tokens is divided, and where its scratch lies.
 struct Division {
     uint32_t chunk, chunks, blocks;
     int threads, tiles;
     int held;             // tokens of a thread that sorts
+    int cluster;          // blocks of the cluster that sorts; 0: many blocks
     uint32_t sort_tiles;
     int64_t token_bytes, touched_bytes, partial_bytes, count_bytes;
     size_t bytes;
@@ -729,9 +933,17 @@ Division divide(const Problem& p) {
     d.token_bytes = whole(p.count * 8);
     d.touched_bytes = whole(ceil_div(p.vocab, 32) * 4);
     d.partial_bytes = whole(int64_t(d.blocks) * 2 * p.width * 4);
-    // few tiles, as every block adds up the counts of all; but a thread holds eight tokens at most
     d.held = 1;
-    while (d.held < kMostHeld && ceil_div(p.count, int64_t(kSortThreads) * d.held) > kScannedTiles) d.held *= 2;
+    const int most = largest_cluster();
+    if (p.count <= int64_t(kSortThreads) * kMostClusterHeld * most) {
+        // as few tokens to a thread as the cluster allows; a smaller cluster where one token is enough
+        while (int64_t(kSortThreads) * d.held * most < p.count) d.held *= 2;
+        d.cluster = 1;
+        while (int64_t(kSortThreads) * d.held * d.cluster < p.count) d.cluster *= 2;
+    } else {
+        // few tiles, as every block adds up the counts of all; but a thread holds eight tokens at most
+        while (d.held < kMostHeld && ceil_div(p.count, int64_t(kSortThreads) * d.held) > kScannedTiles) d.held *= 2;
+    }
     d.sort_tiles = static_cast<uint32_t>(ceil_div(p.count, int64_t(kSortThreads) * d.held));
     d.count_bytes = int64_t(d.sort_tiles) * 1024 + 1024;
     d.bytes = static_cast<size_t>(2 * d.token_bytes + d.touched_bytes + d.partial_bytes + d.count_bytes);
@@ -756,8 +968,8 @@ void launch_owned_rows(b200_ctx* ctx, const b200_embedding_args& a, const Proble
     ctx->count_launch();
 }
 
-// Zeros written beside each of the sort's kernels: what the memory takes in the two microseconds or so of one.
-constexpr int64_t kZerosBesideSort = int64_t(10) << 20;
+// Zeros written beside the sort: what the memory takes meanwhile, of one kernel of the many and of the cluster's.
+constexpr int64_t kZerosBesideKernel = int64_t(20) << 20, kZerosBesideCluster = int64_t(48) << 20;
 
 void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p, const Division& d) {
     char* scratch = operator_workspace(ctx, a.workspace, a.workspace_bytes, d.bytes);
@@ -793,19 +1005,32 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
         zeros.wide = ((reinterpret_cast<uintptr_t>(zeros.table) | static_cast<uintptr_t>(p.pitch) | static_cast<uintptr_t>(row_bytes)) & 15) == 0;
         zeros.pieces = FastDiv(static_cast<uint32_t>(row_bytes / (zeros.wide ? 16 : 2)));
         zeros_left = s.vocab;
-        early = kZerosBesideSort / row_bytes / 32 * 32;
+        early = (d.cluster > 0 ? kZerosBesideCluster : kZerosBesideKernel) / row_bytes / 32 * 32;
     }
-    auto sort = [&](auto kernel) {
+    auto take_zeros = [&] {
         s.zeros = zeros;
         s.zeros.row0 = static_cast<uint32_t>(zeros_left > early ? (zeros_left - early + 31) / 32 * 32 : 0);
         s.zeros.rows = zeros_left > s.zeros.row0 ? zeros_left - s.zeros.row0 : 0;
         zeros_left -= s.zeros.rows;
-        const int64_t beside = std::min<int64_t>(sm_count() * 2, ceil_div(int64_t(s.zeros.rows), 32));
-        launch_kernel(ctx, kernel, dim3(s.tiles + static_cast<unsigned>(beside)), kSortThreads, 0, s);
+        return static_cast<unsigned>(std::min<int64_t>(sm_count() * 2, ceil_div(int64_t(s.zeros.rows), 32)));
+    };
+    auto sort = [&](auto kernel) {
+        const unsigned beside = take_zeros();
+        launch_kernel(ctx, kernel, dim3(s.tiles + beside), kSortThreads, 0, s);
         check_last_launch("embedding_backward");
         ctx->count_launch();
     };
-    for (int pass = 0; pass < passes; ++pass) {
+    if (d.cluster > 0) {
+        s.to = buffer[0];
+        const int at_once = clusters_at_once(d.held, d.cluster);
+        if (at_once < 1) fail(B200_DEVICE_ERROR, "embedding_backward: the device takes no cluster of " + std::to_string(d.cluster) + " blocks");
+        const unsigned beside = static_cast<unsigned>(std::min<int64_t>(std::max(1, at_once - 1), ceil_div(int64_t(take_zeros()), d.cluster)));
+        launch_kernel_clustered(ctx, sort_cluster(d.held), dim3((1 + beside) * d.cluster), dim3(kSortThreads), static_cast<size_t>(kSortThreads) * d.held * sizeof(uint2), d.cluster,
+                                true, s);
+        check_last_launch("embedding_backward");
+        ctx->count_launch();
+    }
+    for (int pass = 0; pass < passes && d.cluster == 0; ++pass) {
         s.from = pass == 0 ? nullptr : buffer[(pass + 1) & 1];
         s.to = buffer[pass & 1];
         s.shift = pass * s.bits;
@@ -817,12 +1042,6 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
         }
         sort(d.held == 1 ? move_kernel<1> : d.held == 2 ? move_kernel<2> : d.held == 4 ? move_kernel<4> : move_kernel<8>);
     }
-    if (!accumulate) {
-        s.from = s.to;
-        s.tiles = static_cast<uint32_t>(ceil_div(p.count, kSortThreads));
-        sort(mark_kernel);
-    }
-
     SumArgs k{};
     k.tokens = s.to;
     k.touched = s.touched;
@@ -841,21 +1060,21 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
     k.tiles = d.tiles;
     k.scale = a.scale;
     k.accumulate = accumulate;
-    k.sum_blocks = d.blocks * static_cast<uint32_t>(d.tiles);
     k.zeros = zeros;
     k.zeros.rows = zeros_left;
     k.zero_words = static_cast<uint32_t>(std::max<int64_t>(1, (128 << 10) / (32 * row_bytes)));
-    const uint32_t zero_blocks = static_cast<uint32_t>(ceil_div(ceil_div(int64_t(zeros_left), 32), int64_t(k.zero_words)));
+    k.join_blocks = static_cast<uint32_t>((d.blocks - 1) * ceil_div(p.width, kJoinColumns));
+    const uint32_t last_blocks = k.join_blocks + static_cast<uint32_t>(ceil_div(ceil_div(int64_t(zeros_left), 32), int64_t(k.zero_words)));
     const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
     with_types(a.table.dtype, a.rows.dtype, [&](auto to, auto tg) {
         using TO = decltype(to);
         using TG = decltype(tg);
-        launch_kernel(ctx, wide ? sum_tokens_kernel<TG, TO, true> : sum_tokens_kernel<TG, TO, false>, dim3(k.sum_blocks + zero_blocks), kSumThreads, 0, k);
+        launch_kernel(ctx, wide ? sum_tokens_kernel<TG, TO, true> : sum_tokens_kernel<TG, TO, false>, dim3(d.blocks * static_cast<uint32_t>(d.tiles)), kSumThreads, 0, k);
         check_last_launch("embedding_backward");
-        if (d.blocks > 1) launch_kernel(ctx, join_kernel<TO>, dim3(d.blocks - 1, static_cast<unsigned>(ceil_div(p.width, kJoinColumns))), kJoinThreads * kJoinGroups, 0, k);
+        if (last_blocks > 0) launch_kernel(ctx, join_kernel<TO>, dim3(last_blocks), kJoinThreads * kJoinGroups, 0, k);
     });
     check_last_launch("embedding_backward");
-    ctx->count_launch(d.blocks > 1 ? 3 : 2);
+    ctx->count_launch(last_blocks > 0 ? 2 : 1);
 }
 
 void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
