@@ -10,97 +10,89 @@
 //   dy  = r2 * (q - mean(q) - y^ * mean(q * y^))  with q = du * w2
 //
 // Bound by memory: forward reads h and y and writes s and n, backward reads dout, dn, s and y and writes dh and dy.  A row is read once: it stays
-// in the registers of the threads that share it, 8 elements of each tensor to a thread for each of its NV pieces, and what is summed over the
-// row goes through shuffles and shared memory.
+// in the registers of the threads that share it, 8 elements of each tensor to a thread for each of its NV pieces.  Blocks stay on their SM and take
+// one row after another, with the next row's loads under way while they work on one: a block that waits for its row, for the row's sums and then for
+// the next block's start left the memory idle for a third (forward) and three quarters (backward) of the time.  What is summed over the row goes
+// through shuffles and shared memory.
 #include "operators.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200 {
 namespace {
 
 constexpr int64_t kMostWidth = 16384;
-constexpr int kWarpRows = 8;  // rows to a block where a row is a warp's
+constexpr int kWarpRows = 8;  // warps of a block where a row is a warp's
 
-// A vector over the columns (a weight, a bias, the gate), F32 or F16.
-struct Columns {
-    const void* p;
-    int64_t pitch;  // of the gate's rows, in elements
-};
-
-// Element e of piece v of thread t of `threads` that share a row: pieces of 8 neighbours where WIDE, else neighbours to neighbouring threads.
-template <bool WIDE>
-__device__ __forceinline__ int column_of(int v, int e, int t, int threads) {
-    return WIDE ? (v * threads + t) * 8 + e : (v * 8 + e) * threads + t;
-}
-
-template <typename T, bool WIDE>
-__device__ __forceinline__ void read_piece(float (&x)[8], const char* row, int v, int t, int threads, int width) {
-    const T* p = reinterpret_cast<const T*>(row);
-    if constexpr (WIDE) {
-        const int c = column_of<true>(v, 0, t, threads);
-        Raw8<T> raw = {};
-        if (c < width) load8(raw, p + c);
-        unpack8(raw, x);
-    } else {
+// Sums of N values over the threads of a row, the same bits in each of them.  `slot` alternates between calls, so that one barrier is enough.
+template <bool WARP, int N>
+__device__ __forceinline__ void row_sums(float (&x)[N], float* part, int& slot) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = column_of<false>(v, e, t, threads);
-            x[e] = c < width ? to_float(p[c]) : 0.f;
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
+    }
+    if constexpr (!WARP) {
+        const int lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        float* const here = part + slot * (N * 32);
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) here[i * 32 + threadIdx.x / 32] = x[i];
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = lane < warps ? here[i * 32 + lane] : 0.f;
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
+        }
+        slot ^= 1;
     }
 }
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void write_piece(char* row, const float (&x)[8], int v, int t, int threads, int width) {
-    T* p = reinterpret_cast<T*>(row);
-    if constexpr (WIDE) {
-        const int c = column_of<true>(v, 0, t, threads);
-        if (c < width) store8(p + c, x);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = column_of<false>(v, e, t, threads);
-            if (c < width) p[c] = from_float<T>(x[e]);
-        }
-    }
+// Eight values to a thread in memory that no other thread touches: 16 bytes of the block's threads side by side.
+__device__ __forceinline__ void own_store(float* p, int which, const float (&x)[8]) {
+    float4* to = reinterpret_cast<float4*>(p) + (which * 2) * blockDim.x + threadIdx.x;
+    to[0] = make_float4(x[0], x[1], x[2], x[3]);
+    to[blockDim.x] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void own_load(const float* p, int which, float (&x)[8]) {
+    const float4* from = reinterpret_cast<const float4*>(p) + (which * 2) * blockDim.x + threadIdx.x;
+    const float4 a = from[0], b = from[blockDim.x];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 
-// The piece of a vector over the columns; `absent` where there is none.
+// A piece of a vector over the columns (a weight, a bias, the gate), F32 or F16; `absent` where there is none.
 template <bool WIDE>
-__device__ __forceinline__ void read_columns(float (&x)[8], const void* p, bool half, float absent, int v, int t, int threads, int width) {
+__device__ __forceinline__ void read_columns(float (&x)[8], const void* p, bool half, float absent, int first, int t, int threads, int width) {
     if (p == nullptr) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = absent;
     } else if (half) {
-        read_piece<__half, WIDE>(x, static_cast<const char*>(p), v, t, threads, width);
+        Piece<__half, WIDE> piece;
+        piece.load(static_cast<const char*>(p), first, t, threads, width);
+        piece.get(x);
     } else {
-        read_piece<float, WIDE>(x, static_cast<const char*>(p), v, t, threads, width);
+        Piece<float, WIDE> piece;
+        piece.load(static_cast<const char*>(p), first, t, threads, width);
+        piece.get(x);
     }
 }
 
-// Sums of two values over the threads of a row, the same bits in each of them.  `slot` alternates between calls, so that one barrier is enough.
-template <bool WARP>
-__device__ __forceinline__ float2 row_sum(float2 x, float2 (&part)[2][32], int& slot) {
+// A piece of sums over rows, in a row that may start anywhere.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_columns(T* row, const float (&x)[8], int first, int t, int threads, int width) {
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) {
-        x.x += __shfl_xor_sync(0xffffffffu, x.x, d);
-        x.y += __shfl_xor_sync(0xffffffffu, x.y, d);
+    for (int e = 0; e < 8; ++e) {
+        const int c = first + piece_column<WIDE>(e, t, threads);
+        if (c < width) row[c] = from_float<T>(x[e]);
     }
-    if constexpr (!WARP) {
-        const int lane = threadIdx.x % 32, warps = blockDim.x / 32;
-        if (lane == 0) part[slot][threadIdx.x / 32] = x;
-        __syncthreads();
-        x = lane < warps ? part[slot][lane] : make_float2(0.f, 0.f);
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            x.x += __shfl_xor_sync(0xffffffffu, x.x, d);
-            x.y += __shfl_xor_sync(0xffffffffu, x.y, d);
-        }
-        slot ^= 1;
-    }
-    return x;
 }
+
+// The rows of worker w of n: a stretch of them.
+__device__ __forceinline__ uint32_t stretch(uint32_t rows, uint32_t w, uint32_t n) { return static_cast<uint32_t>(uint64_t(rows) * w / n); }
 
 struct ForwardArgs {
     RowsArg residual, branch, out, normed;
@@ -116,84 +108,152 @@ struct ForwardArgs {
 
 // Mean and 1 / sqrt of a row's norm.  The variance is that of the differences to the mean, which the registers still hold: no cancellation.
 template <bool WARP, bool WIDE, int NV>
-__device__ __forceinline__ float2 norm_of(const float (&x)[NV][8], bool layer, float eps, float share, int t, int threads, int width,
-                                          float2 (&part)[2][32], int& slot) {
-    float mean = 0.f;
+__device__ __forceinline__ float2 norm_of(const float (&x)[NV][8], bool layer, float eps, float share, int t, int threads, int width, float* part, int& slot) {
+    float mean[1] = {0.f}, square[1] = {0.f};
     if (layer) {
-        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s.x += x[v][e];
-        mean = row_sum<WARP>(s, part, slot).x * share;
+            for (int e = 0; e < 8; ++e) mean[0] += x[v][e];
+        row_sums<WARP, 1>(mean, part, slot);
+        mean[0] *= share;
     }
-    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float d = column_of<WIDE>(v, e, t, threads) < width ? x[v][e] - mean : 0.f;
-            s.x += d * d;
+            const float d = v * threads * 8 + piece_column<WIDE>(e, t, threads) < width ? x[v][e] - mean[0] : 0.f;
+            square[0] += d * d;
         }
-    return make_float2(mean, 1.f / sqrtf(row_sum<WARP>(s, part, slot).x * share + eps));
+    row_sums<WARP, 1>(square, part, slot);
+    return make_float2(mean[0], 1.f / sqrtf(square[0] * share + eps));
 }
 
-template <typename TH, typename TY, int NV, bool WIDE, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : 1024)
+// AHEAD: the next row's loads are under way while a row is worked on (which takes registers that blocks of 1024 threads do not have).
+template <typename TH, typename TY, int NV, bool WIDE, bool WARP, bool AHEAD>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : AHEAD ? 512 : 1024)
 norm_kernel(const ForwardArgs k) {
-    __shared__ float2 part[2][32];
+    extern __shared__ __align__(16) float own[];  // the columns' factors: of the branch, of the norm in front; and their biases
+    __shared__ float part[2 * 32];
     pdl_prologue();
     int slot = 0;
     const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x % 32 : threadIdx.x;
-    const uint32_t r = WARP ? blockIdx.x * kWarpRows + threadIdx.x / 32 : blockIdx.x;
-    if (r >= k.rows) return;  // (a whole warp, or a whole block)
-    float h[NV][8], y[NV][8];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[v][e] = y[v][e] = 0.f;
-        if (k.residual.base != nullptr) read_piece<TH, WIDE>(h[v], row_at(k.residual, k.inner, r), v, t, threads, k.width);
-        if (k.branch.base != nullptr) read_piece<TY, WIDE>(y[v], row_at(k.branch, k.inner, r), v, t, threads, k.width);
-    }
-    float2 post = make_float2(0.f, 0.f), pre = make_float2(0.f, 0.f);
-    if (k.post) post = norm_of<WARP, WIDE, NV>(y, k.layer, k.eps, k.share, t, threads, k.width, part, slot);
-    const char* gate = static_cast<const char*>(k.gate);
-    if (gate != nullptr) gate += int64_t(k.gate_rows.div(r)) * k.gate_pitch;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (k.branch.base != nullptr) {
-            float w[8], b[8], g[8];
-            read_columns<WIDE>(g, gate, k.half_columns, 1.f, v, t, threads, k.width);
-            if (k.post) {
-                read_columns<WIDE>(w, k.post_weight, k.half_columns, 1.f, v, t, threads, k.width);
-                read_columns<WIDE>(b, k.post_bias, k.half_columns, 0.f, v, t, threads, k.width);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[v][e] = (y[v][e] - post.x) * post.y * w[e] + b[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                h[v][e] = k.a * h[v][e] + k.b * (g[e] * y[v][e]);
-                if (column_of<WIDE>(v, e, t, threads) >= k.width) h[v][e] = 0.f;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[v][e] *= k.a;
-        }
-        if (k.out.base != nullptr) write_piece<TH, WIDE>(row_at(k.out, k.inner, r), h[v], v, t, threads, k.width);
-    }
-    if (k.normed.base != nullptr) {
-        pre = norm_of<WARP, WIDE, NV>(h, k.layer, k.eps, k.share, t, threads, k.width, part, slot);
+    const uint32_t workers = WARP ? gridDim.x * kWarpRows : gridDim.x, worker = WARP ? blockIdx.x * kWarpRows + threadIdx.x / 32 : blockIdx.x;
+    const uint32_t r0 = stretch(k.rows, worker, workers), r1 = stretch(k.rows, worker + 1, workers);
+    const bool has_residual = k.residual.base != nullptr, has_branch = k.branch.base != nullptr;
+    const bool post_bias = k.post_bias != nullptr, pre_bias = k.pre_bias != nullptr;
+    Piece<TH, WIDE> h_piece[NV];
+    Piece<TY, WIDE> y_piece[NV];
+    auto load = [&](uint32_t r) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            float w[8], b[8];
-            read_columns<WIDE>(w, k.pre_weight, k.half_columns, 1.f, v, t, threads, k.width);
-            read_columns<WIDE>(b, k.pre_bias, k.half_columns, 0.f, v, t, threads, k.width);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[v][e] = (h[v][e] - pre.x) * pre.y * w[e] + b[e];
-            write_piece<TY, WIDE>(row_at(k.normed, k.inner, r), h[v], v, t, threads, k.width);
+            if (has_residual) h_piece[v].load(row_at(k.residual, k.inner, r), v * threads * 8, t, threads, k.width);
+            else h_piece[v].clear();
+            if (has_branch) y_piece[v].load(row_at(k.branch, k.inner, r), v * threads * 8, t, threads, k.width);
+            else y_piece[v].clear();
         }
+    };
+    // The columns' factors and biases: b gate w2, w1, b gate b2, b1.  Kept in the thread's own shared memory (AHEAD; not for 1024 threads of 16 columns), else made
+    // where they are needed.
+    enum { kW2, kW1, kB2, kB1 };
+    const char* gate = nullptr;
+    auto read_factor = [&](int which, int v, float (&x)[8]) {
+        const void* from = which == kW2 ? k.post_weight : which == kW1 ? k.pre_weight : which == kB2 ? k.post_bias : k.pre_bias;
+        read_columns<WIDE>(x, from, k.half_columns, which == kW2 || which == kW1 ? 1.f : 0.f, v * threads * 8, t, threads, k.width);
+        if (which == kW2 || which == kB2) {
+            float g[8];
+            read_columns<WIDE>(g, gate, k.half_columns, 1.f, v * threads * 8, t, threads, k.width);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= g[e] * k.b;
+        }
+    };
+    auto place = [&](int which) { return which == kB1 && !post_bias ? 2 : which; };
+    auto factor = [&](int which, int v, float (&x)[8]) {
+        if constexpr (AHEAD) own_load(own, place(which) * NV + v, x);
+        else read_factor(which, v, x);
+    };
+    auto keep_factor = [&](int which) {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                float x[8];
+                read_factor(which, v, x);
+                own_store(own, place(which) * NV + v, x);
+            }
+        }
+    };
+    auto set_branch = [&](uint32_t group) {
+        gate = static_cast<const char*>(k.gate);
+        if (gate != nullptr) gate += int64_t(group) * k.gate_pitch;
+        keep_factor(kW2);
+        if (post_bias) keep_factor(kB2);
+    };
+    if (r0 < r1) load(r0);
+    uint32_t group = r0 < r1 ? k.gate_rows.div(r0) : 0;
+    if (r0 < r1 && has_branch) set_branch(group);
+    if (r0 < r1 && k.normed.base != nullptr) {
+        keep_factor(kW1);
+        if (pre_bias) keep_factor(kB1);
     }
-    if (k.stats != nullptr && t == 0) k.stats[r] = make_float4(post.x, post.y, pre.x, pre.y);
+    for (uint32_t r = r0; r < r1; ++r) {
+        float h[NV][8], y[NV][8];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            h_piece[v].get(h[v]);
+            y_piece[v].get(y[v]);
+        }
+        if (AHEAD && r + 1 < r1) load(r + 1);
+        float2 post = make_float2(0.f, 0.f), pre = make_float2(0.f, 0.f);
+        if (k.post) post = norm_of<WARP, WIDE, NV>(y, k.layer, k.eps, k.share, t, threads, k.width, part, slot);
+        const uint32_t now = k.gate_rows.div(r);
+        if (now != group) {
+            group = now;
+            if (k.gate != nullptr) set_branch(group);
+        }
+        const float scale = k.post ? post.y : 1.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (has_branch) {
+                float w[8];
+                factor(kW2, v, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[v][e] = k.a * h[v][e] + (y[v][e] - post.x) * scale * w[e];
+                if (post_bias) {
+                    factor(kB2, v, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) h[v][e] += w[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[v][e] *= k.a;
+            }
+            if (k.out.base != nullptr) store_piece<TH, WIDE>(row_at(k.out, k.inner, r), h[v], v * threads * 8, t, threads, k.width);
+            if (k.layer) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (v * threads * 8 + piece_column<WIDE>(e, t, threads) >= k.width) h[v][e] = 0.f;
+                }
+            }
+        }
+        if (k.normed.base != nullptr) {
+            pre = norm_of<WARP, WIDE, NV>(h, k.layer, k.eps, k.share, t, threads, k.width, part, slot);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                float w[8];
+                factor(kW1, v, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[v][e] = (h[v][e] - pre.x) * pre.y * w[e];
+                if (pre_bias) {
+                    factor(kB1, v, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) h[v][e] += w[e];
+                }
+                store_piece<TY, WIDE>(row_at(k.normed, k.inner, r), h[v], v * threads * 8, t, threads, k.width);
+            }
+        }
+        if (k.stats != nullptr && t == 0) k.stats[r] = make_float4(post.x, post.y, pre.x, pre.y);
+        if (!AHEAD && r + 1 < r1) load(r + 1);
+    }
 }
 
 // ---- backward ---------------------------------------------------------------
@@ -207,170 +267,329 @@ struct BackwardArgs {
     const void *post_weight, *post_bias, *pre_weight, *gate;
     int64_t gate_pitch;          // bytes
     float* partial[kSums];       // [blocks][width], the gate's [items][width]; null: not wanted
+    void* gate_grad;             // where a gate's rows are one item: its gradient itself, in place of partial[kGate]
+    float* own;                  // the sums where registers do not hold them: [blocks][kOwnSums * NV * 8 * threads]; null: in shared memory
     FastDiv inner;
     uint32_t group_rows, pieces;  // rows to a gate, and how many items they are divided into
     uint32_t items;
     int width;
     float a, b, share;
-    bool layer, post, half_columns;
+    bool layer, post, half_columns, half_gate_grad;
+    bool warp_items;  // WARP: an item is a warp's; else a block's, whose warps take its rows in turn
 };
 
-// A block takes items one after another: item i is piece i % pieces of the rows of gate i / pieces.  The gate's sums are left behind after each
-// item, the others once, in the block's own row of the partial sums; fold_kernel adds those up in order, so that no result depends on timing.
-// REGS: the sums stay in the threads' registers; else in the partial sums themselves (each thread its own columns).
-template <typename TH, typename TY, int NV, bool WIDE, bool WARP, bool REGS>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : REGS ? 512 : 1024)
+// In a gate's rows the gate and the weights are the same, so that two sums hold the gradients of three vectors: E = sum ds * y^ and F = sum ds, with
+// dgate = b (w2 E + b2 F), dw2 += b gate E, db2 += b gate F at the end of the rows.  Both row sums of the two norms come from one reduction: with c = b gate w2
+// and t = dout + r1 g, where ds = t - r1 (m0 + s^ m1),
+//   mean(c y^ ds) = mean(c y^ t) - r1 (m0 mean(c y^) + m1 mean(c y^ s^))      mean(c ds) = mean(c t) - r1 (m0 mean(c) + m1 mean(c s^))
+// A block takes items one after another: item i is piece i % pieces of the rows of gate i / pieces.  The gate's sums are left behind after each item, the others
+// once, in the block's row of the partial sums; fold_kernel adds those up in order, so that no result depends on timing.
+// FULL: layer norms and biases too; without it RMS norms alone.  REGS: the sums over rows stay in registers, else in the thread's own memory.
+// HOLD: a row stays in registers between the reduction and the results, else it is read again.  AHEAD: the next row's loads are under way meanwhile.
+enum OwnSum { kE, kPreW, kF, kPreB, kPostW, kPostB, kOwnSums };
+constexpr int kOwnRms = 3;  // without FULL: kE, kPreW and kPostW, which come first in memory
+__host__ __device__ constexpr int own_place(int which) { return which == kE ? 0 : which == kPreW ? 1 : which == kPostW ? 2 : which == kF ? 3 : which == kPreB ? 4 : 5; }
+
+template <typename TH, typename TY, int NV, bool WIDE, bool WARP, bool FULL, bool REGS, bool HOLD, bool AHEAD>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : HOLD ? 512 : 1024, WARP ? 2 : 1)
 norm_backward_kernel(const BackwardArgs k) {
-    __shared__ float2 part[2][32];
+    constexpr int N = FULL ? 8 : 3;
+    extern __shared__ __align__(16) float shared_own[];
+    __shared__ float part[2 * N * 32];
+    __shared__ float meet[WARP ? kWarpRows : 1][WARP ? 256 : 1];
     pdl_prologue();
     int slot = 0;
-    const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x % 32 : threadIdx.x;
-    const int own = WARP ? blockIdx.x * kWarpRows + threadIdx.x / 32 : blockIdx.x;  // whose partial sums
-    const int owners = WARP ? gridDim.x * kWarpRows : gridDim.x;
-    float sum[REGS ? kSums : 1][REGS ? NV : 1][8];
+    const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x % 32 : threadIdx.x, warp = threadIdx.x / 32;
+    float* const own = k.own != nullptr ? k.own + int64_t(blockIdx.x) * ((FULL ? kOwnSums : kOwnRms) * NV * 8) * blockDim.x : shared_own;
+    float* const factors = shared_own + (REGS ? 2 : 0) * NV * 8 * blockDim.x;  // REGS: kPostW and kPostB lie in front
+    const bool pre = k.normed_grad.base != nullptr, branch = k.branch.base != nullptr || k.branch_grad.base != nullptr;
+    // running sums: in registers, or in `own`
+    float sum[REGS ? 4 : 1][REGS ? NV : 1][8];
     auto clear = [&](int which) {
-        if constexpr (REGS) {
+        const float zero[8] = {};
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (REGS) {
+                if (which < 4) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[which][v][e] = 0.f;
-        }
-    };
-    auto each_column = [&](float* to, auto&& f) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = column_of<WIDE>(v, e, t, threads);
-                if (c < k.width) f(to[c], v, e);
+                    for (int e = 0; e < 8; ++e) sum[which][v][e] = 0.f;
+                } else {
+                    own_store(shared_own, (which - kPostW) * NV + v, zero);
+                }
+            } else {
+                own_store(own, own_place(which) * NV + v, zero);
             }
-    };
-    auto row_of = [&](int which, uint32_t item) { return k.partial[which] + int64_t(which == kGate ? item : uint32_t(own)) * k.width; };
-    auto begin = [&](int which, uint32_t item) {
-        if constexpr (REGS) clear(which);
-        else if (k.partial[which] != nullptr) each_column(row_of(which, item), [](float& x, int, int) { x = 0.f; });
-    };
-    auto end = [&](int which, uint32_t item) {
-        if constexpr (REGS) {
-            if (k.partial[which] != nullptr) each_column(row_of(which, item), [&](float& x, int v, int e) { x = sum[which][v][e]; });
         }
     };
+    auto get_sum = [&](int which, int v, float (&x)[8]) {
+        if constexpr (REGS) {
+            if (which < 4) {
 #pragma unroll
-    for (int s = kPostWeight; s < kSums; ++s) begin(s, 0);
-    for (uint32_t item = own; item < k.items; item += owners) {
-        const uint32_t group = item / k.pieces, piece = item % k.pieces;
-        const uint32_t r0 = group * k.group_rows + static_cast<uint32_t>(uint64_t(k.group_rows) * piece / k.pieces);
-        const uint32_t r1 = group * k.group_rows + static_cast<uint32_t>(uint64_t(k.group_rows) * (piece + 1) / k.pieces);
-        const char* gate = static_cast<const char*>(k.gate);
-        if (gate != nullptr) gate += int64_t(group) * k.gate_pitch;
-        begin(kGate, item);
-        for (uint32_t r = r0; r < r1; ++r) {
-            float s[NV][8], dn[NV][8], ds[NV][8], y[NV][8];
-            const bool pre = k.normed_grad.base != nullptr;
+                for (int e = 0; e < 8; ++e) x[e] = sum[which][v][e];
+            } else {
+                own_load(shared_own, (which - kPostW) * NV + v, x);
+            }
+        } else {
+            own_load(own, own_place(which) * NV + v, x);
+        }
+    };
+    auto add = [&](int which, int v, const float (&x)[8]) {
+        if constexpr (REGS) {
+            if (which < 4) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[which][v][e] += x[e];
+                return;
+            }
+        }
+        float y[8];
+        get_sum(which, v, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] += x[e];
+        if constexpr (REGS) own_store(shared_own, (which - kPostW) * NV + v, y);
+        else own_store(own, own_place(which) * NV + v, y);
+    };
+    // WARP: a value summed over the block's warps, in the first one
+    auto over_warps = [&](float (&x)[8]) {
+        if constexpr (WARP) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) meet[warp][e * 32 + t] = x[e];
+            __syncthreads();
+            if (warp == 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    for (int w = 1; w < kWarpRows; ++w) x[e] += meet[w][e * 32 + t];
+                }
+            }
+        }
+    };
+    // the columns' factors: w1, w2, b gate and b2; from the thread's own memory where that is (REGS), else read where they are needed
+    enum { kW1, kW2, kG, kB2 };
+    const char* gate = nullptr;
+    auto read_factor = [&](int which, int v, float (&x)[8]) {
+        const void* from = which == kW1 ? k.pre_weight : which == kW2 ? k.post_weight : which == kG ? static_cast<const void*>(gate) : k.post_bias;
+        read_columns<WIDE>(x, from, k.half_columns, which == kB2 ? 0.f : 1.f, v * threads * 8, t, threads, k.width);
+        if (which == kG) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= k.b;
+        }
+    };
+    auto factor = [&](int which, int v, float (&x)[8]) {
+        if constexpr (REGS) own_load(factors, which * NV + v, x);
+        else read_factor(which, v, x);
+    };
+    auto keep_factor = [&](int which) {
+        if constexpr (REGS) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[v][e] = dn[v][e] = ds[v][e] = y[v][e] = 0.f;
-                if (pre) {
-                    read_piece<TH, WIDE>(s[v], row_at(k.out, k.inner, r), v, t, threads, k.width);
-                    read_piece<TY, WIDE>(dn[v], row_at(k.normed_grad, k.inner, r), v, t, threads, k.width);
-                }
-                if (k.out_grad.base != nullptr) read_piece<TH, WIDE>(ds[v], row_at(k.out_grad, k.inner, r), v, t, threads, k.width);
-                if (k.branch.base != nullptr) read_piece<TY, WIDE>(y[v], row_at(k.branch, k.inner, r), v, t, threads, k.width);
+                float x[8];
+                read_factor(which, v, x);
+                own_store(factors, which * NV + v, x);
             }
-            const float4 st = k.stats != nullptr ? k.stats[r] : make_float4(0.f, 1.f, 0.f, 1.f);
-            auto add = [&](int which, int v, const float (&x)[8]) {
-                if constexpr (REGS) {
+        }
+    };
+    Piece<TH, WIDE> s_piece[NV], o_piece[NV], s_next[AHEAD ? NV : 1], o_next[AHEAD ? NV : 1];
+    Piece<TY, WIDE> n_piece[NV], y_piece[NV], n_next[AHEAD ? NV : 1], y_next[AHEAD ? NV : 1];
+    float4 st = make_float4(0.f, 1.f, 0.f, 1.f), st_next = st;
+    auto load_piece = [&](uint32_t r, int v, Piece<TH, WIDE>& s, Piece<TY, WIDE>& n, Piece<TH, WIDE>& o, Piece<TY, WIDE>& y) {
+        const int first = v * threads * 8;
+        if (pre) s.load(row_at(k.out, k.inner, r), first, t, threads, k.width);
+        else s.clear();
+        if (pre) n.load(row_at(k.normed_grad, k.inner, r), first, t, threads, k.width);
+        else n.clear();
+        if (k.out_grad.base != nullptr) o.load(row_at(k.out_grad, k.inner, r), first, t, threads, k.width);
+        else o.clear();
+        if (k.branch.base != nullptr) y.load(row_at(k.branch, k.inner, r), first, t, threads, k.width);
+        else y.clear();
+    };
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum[which][v][e] += x[e];
-                } else if (k.partial[which] != nullptr) {
-                    float* to = row_of(which, item);
+    for (int s = 0; s < kOwnSums; ++s) {
+        if (FULL || own_place(s) < kOwnRms) clear(s);
+    }
+    keep_factor(kW1);
+    keep_factor(kW2);
+    if (FULL) keep_factor(kB2);
+    const bool by_warp = WARP && k.warp_items;
+    const uint32_t step = WARP && !by_warp ? kWarpRows : 1, workers = by_warp ? gridDim.x * kWarpRows : gridDim.x;
+    for (uint32_t item = by_warp ? blockIdx.x * kWarpRows + warp : blockIdx.x; item < k.items; item += workers) {
+        const uint32_t group = item / k.pieces, piece = item % k.pieces;
+        const uint32_t r0 = group * k.group_rows + stretch(k.group_rows, piece, k.pieces) + (step > 1 ? warp : 0);
+        const uint32_t r1 = group * k.group_rows + stretch(k.group_rows, piece + 1, k.pieces);
+        gate = static_cast<const char*>(k.gate);
+        if (gate != nullptr) gate += int64_t(group) * k.gate_pitch;
+        keep_factor(kG);
+        auto load_ahead = [&](uint32_t r) {
+            if constexpr (AHEAD) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int c = column_of<WIDE>(v, e, t, threads);
-                        if (c < k.width) to[c] += x[e];
-                    }
+                for (int v = 0; v < NV; ++v) load_piece(r, v, s_next[v], n_next[v], o_next[v], y_next[v]);
+                if (k.stats != nullptr) st_next = k.stats[r];
+            }
+        };
+        if (r0 < r1) load_ahead(r0);
+        float mean_c = 0.f;  // FULL: of c
+        if (FULL && k.layer && k.post) {
+            float x[1] = {0.f};
+            if (!WARP) __syncthreads();  // (the reductions before and after lay their values out otherwise)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                float w[8], g[8];
+                factor(kW2, v, w);
+                factor(kG, v, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[0] += v * threads * 8 + piece_column<WIDE>(e, t, threads) < k.width ? w[e] * g[e] : 0.f;
+            }
+            row_sums<WARP, 1>(x, part, slot);
+            if (!WARP) __syncthreads();
+            mean_c = x[0] * k.share;
+        }
+        for (uint32_t r = r0; r < r1; r += step) {
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v) s_piece[v] = s_next[v], n_piece[v] = n_next[v], o_piece[v] = o_next[v], y_piece[v] = y_next[v];
+                st = st_next;
+                if (r + step < r1) load_ahead(r + step);
+            } else {
+                if constexpr (HOLD) {
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) load_piece(r, v, s_piece[v], n_piece[v], o_piece[v], y_piece[v]);
+                }
+                if (k.stats != nullptr) st = k.stats[r];
+            }
+            const float y_mean = k.post ? st.x : 0.f, y_scale = k.post ? st.y : 1.f;
+            // s^, g, t and y^ of a piece
+            auto terms = [&](int v, float (&s)[8], float (&n)[8], float (&g)[8], float (&o)[8], float (&y)[8]) {
+                if constexpr (!HOLD) load_piece(r, v, s_piece[0], n_piece[0], o_piece[0], y_piece[0]);
+                s_piece[HOLD ? v : 0].get(s);
+                n_piece[HOLD ? v : 0].get(n);
+                o_piece[HOLD ? v : 0].get(o);
+                y_piece[HOLD ? v : 0].get(y);
+                float w[8];
+                factor(kW1, v, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    s[e] = pre ? (s[e] - st.z) * st.w : 0.f;
+                    g[e] = n[e] * w[e];
+                    y[e] = (y[e] - y_mean) * y_scale;
+                    o[e] = pre ? fmaf(st.w, g[e], o[e]) : o[e];
                 }
             };
-            if (pre) {
-                float2 m = make_float2(0.f, 0.f);
+            float x[N] = {};  // g s^; c y^ t, c y^ s^; FULL: g; c t, c s^, c y^
 #pragma unroll
-                for (int v = 0; v < NV; ++v) {
-                    float w[8], x[8];
-                    read_columns<WIDE>(w, k.pre_weight, k.half_columns, 1.f, v, t, threads, k.width);
-                    add(kPreBias, v, dn[v]);
+            for (int v = 0; v < NV; ++v) {
+                float s[8], n[8], g[8], o[8], y[8], c[8], w[8];
+                terms(v, s, n, g, o, y);
+                factor(kW2, v, c);
+                factor(kG, v, w);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        s[v][e] = (s[v][e] - st.z) * st.w;
-                        x[e] = dn[v][e] * s[v][e];
-                        dn[v][e] *= w[e];
-                        m.x += dn[v][e] * s[v][e];
-                        m.y += dn[v][e];
+                for (int e = 0; e < 8; ++e) {
+                    if (!WIDE || FULL) {  // (columns behind the row's end: y^ is not 0 there)
+                        if (v * threads * 8 + piece_column<WIDE>(e, t, threads) >= k.width) continue;
                     }
-                    add(kPreWeight, v, x);
-                }
-                m = row_sum<WARP>(m, part, slot);
-                m.x *= k.share;
-                m.y = k.layer ? m.y * k.share : 0.f;
-#pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ds[v][e] += st.w * (dn[v][e] - m.y - s[v][e] * m.x);
-            }
-            if (k.residual_grad.base != nullptr) {
-#pragma unroll
-                for (int v = 0; v < NV; ++v) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = k.a * ds[v][e];
-                    write_piece<TH, WIDE>(row_at(k.residual_grad, k.inner, r), x, v, t, threads, k.width);
+                    c[e] *= w[e];
+                    const float cy = c[e] * y[e];
+                    x[0] = fmaf(g[e], s[e], x[0]);
+                    x[1] = fmaf(cy, o[e], x[1]);
+                    x[2] = fmaf(cy, s[e], x[2]);
+                    if constexpr (FULL) {
+                        x[3] += g[e];
+                        x[4] = fmaf(c[e], o[e], x[4]);
+                        x[5] = fmaf(c[e], s[e], x[5]);
+                        x[6] += cy;
+                    }
                 }
             }
-            if (k.branch.base == nullptr && k.branch_grad.base == nullptr) continue;
-            float2 m = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                float w[8], b[8], g[8], x[8];
-                read_columns<WIDE>(g, gate, k.half_columns, 1.f, v, t, threads, k.width);
-                read_columns<WIDE>(w, k.post_weight, k.half_columns, 1.f, v, t, threads, k.width);
-                read_columns<WIDE>(b, k.post_bias, k.half_columns, 0.f, v, t, threads, k.width);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (k.post) y[v][e] = (y[v][e] - st.x) * st.y;
-                    ds[v][e] *= k.b;
-                    x[e] = ds[v][e] * (y[v][e] * w[e] + b[e]);
-                    ds[v][e] *= g[e];  // du
-                }
-                add(kGate, v, x);
-                add(kPostBias, v, ds[v]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = ds[v][e] * y[v][e];
-                    ds[v][e] *= w[e];
-                    m.x += ds[v][e] * y[v][e];
-                    m.y += ds[v][e];
-                }
-                add(kPostWeight, v, x);
-            }
-            if (k.branch_grad.base == nullptr) continue;
+            row_sums<WARP, N>(x, part, slot);
+            const float m1 = x[0] * k.share * st.w;  // r1 m1, r1 m0
+            const float m0 = FULL && k.layer ? x[FULL ? 3 : 0] * k.share * st.w : 0.f;
+            float k1 = 0.f, k0 = 0.f;
             if (k.post) {
-                m = row_sum<WARP>(m, part, slot);
-                m.x *= k.share;
-                m.y = k.layer ? m.y * k.share : 0.f;
+                k1 = x[1] * k.share - m1 * (x[2] * k.share);
+                if constexpr (FULL) {
+                    if (k.layer) {
+                        k1 -= m0 * (x[6] * k.share);
+                        k0 = x[4] * k.share - m0 * mean_c - m1 * (x[5] * k.share);
+                    }
+                }
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                if (k.post) {
+                float s[8], n[8], g[8], o[8], y[8];
+                terms(v, s, n, g, o, y);
+                if (pre) {
+                    float q[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) ds[v][e] = st.y * (ds[v][e] - m.y - y[v][e] * m.x);
+                    for (int e = 0; e < 8; ++e) q[e] = n[e] * s[e];
+                    add(kPreW, v, q);
+                    if (FULL) add(kPreB, v, n);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = o[e] - m0 - s[e] * m1;  // ds
                 }
-                write_piece<TY, WIDE>(row_at(k.branch_grad, k.inner, r), ds[v], v, t, threads, k.width);
+                if (k.residual_grad.base != nullptr) {
+                    float q[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) q[e] = k.a * o[e];
+                    store_piece<TH, WIDE>(row_at(k.residual_grad, k.inner, r), q, v * threads * 8, t, threads, k.width);
+                }
+                if (branch) {
+                    float q[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) q[e] = o[e] * y[e];
+                    add(kE, v, q);
+                    if (FULL) add(kF, v, o);
+                    if (k.branch_grad.base != nullptr) {
+                        float w[8];
+                        factor(kG, v, q);
+                        factor(kW2, v, w);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) q[e] = y_scale * (q[e] * w[e] * o[e] - k0 - y[e] * k1);
+                        store_piece<TY, WIDE>(row_at(k.branch_grad, k.inner, r), q, v * threads * 8, t, threads, k.width);
+                    }
+                }
             }
         }
-        end(kGate, item);
-    }
+        // the item's sums
 #pragma unroll
-    for (int s = kPostWeight; s < kSums; ++s) end(s, 0);
+        for (int v = 0; v < NV; ++v) {
+            float e_sum[8], f_sum[8] = {}, w[8], b[8] = {}, q[8];
+            get_sum(kE, v, e_sum);
+            if (FULL) get_sum(kF, v, f_sum);
+            if (WARP && !by_warp) {
+                over_warps(e_sum);
+                if (FULL) over_warps(f_sum);
+            }
+            if (WARP && !by_warp && warp != 0) continue;
+            if (k.partial[kGate] != nullptr || k.gate_grad != nullptr) {
+                factor(kW2, v, w);
+                if (FULL) factor(kB2, v, b);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[e] = k.b * (w[e] * e_sum[e] + b[e] * f_sum[e]);
+                // (the partial sums and a gate's gradient are dense, and may start anywhere)
+                const int64_t at = int64_t(k.gate_grad != nullptr ? group : item) * k.width;
+                if (k.gate_grad != nullptr && k.half_gate_grad) store_columns<__half, WIDE>(static_cast<__half*>(k.gate_grad) + at, q, v * threads * 8, t, threads, k.width);
+                else store_columns<float, WIDE>((k.gate_grad != nullptr ? static_cast<float*>(k.gate_grad) : k.partial[kGate]) + at, q, v * threads * 8, t, threads, k.width);
+            }
+            factor(kG, v, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) e_sum[e] *= w[e], f_sum[e] *= w[e];
+            add(kPostW, v, e_sum);
+            if (FULL) add(kPostB, v, f_sum);
+        }
+        clear(kE);
+        if (FULL) clear(kF);
+    }
+    const int own_of[kSums] = {kE, kPostW, kPostB, kPreW, kPreB};
+#pragma unroll
+    for (int s = kPostWeight; s < kSums; ++s) {
+        if (k.partial[s] == nullptr || (!FULL && own_place(own_of[s]) >= kOwnRms)) continue;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float x[8];
+            get_sum(own_of[s], v, x);
+            over_warps(x);
+            if (WARP && warp != 0) continue;
+            store_columns<float, WIDE>(k.partial[s] + int64_t(blockIdx.x) * k.width, x, v * threads * 8, t, threads, k.width);
+        }
+    }
 }
 
 struct Fold {
@@ -545,54 +764,83 @@ void launch_forward(b200_ctx* ctx, const b200_block_norm_args& a) {
     const bool warp = p.width <= 256;
     const int pieces = p.width <= 2048 ? 1 : 2;
     const int threads = warp ? kWarpRows * 32 : static_cast<int>(ceil_div(p.width, int64_t(8) * pieces * 32)) * 32;
-    const unsigned blocks = static_cast<unsigned>(warp ? ceil_div(p.s.rows, kWarpRows) : p.s.rows);
+    const size_t shared = threads > 512 ? 0 : static_cast<size_t>(2 + (k.post_bias != nullptr) + (k.pre_bias != nullptr)) * pieces * 32 * threads;
     ProfScope scope(ctx, "block_norm");
     with_types(p, [&](auto th, auto ty) {
         using TH = decltype(th);
         using TY = decltype(ty);
-        auto go = [&](auto kernel) { launch_kernel(ctx, kernel, blocks, threads, 0, k); };
-        if (wide) go(warp ? norm_kernel<TH, TY, 1, true, true> : pieces == 1 ? norm_kernel<TH, TY, 1, true, false> : norm_kernel<TH, TY, 2, true, false>);
-        else go(warp ? norm_kernel<TH, TY, 1, false, true> : pieces == 1 ? norm_kernel<TH, TY, 1, false, false> : norm_kernel<TH, TY, 2, false, false>);
+        auto go = [&](auto kernel) {
+            const int64_t most = int64_t(sm_count()) * blocks_at_once(reinterpret_cast<const void*>(kernel), threads, shared);
+            const int64_t blocks = std::min<int64_t>(most, warp ? ceil_div(p.s.rows, kWarpRows) : p.s.rows);
+            launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), shared, k);
+        };
+        auto of_width = [&](auto is_wide) {
+            constexpr bool W = decltype(is_wide)::value;
+            if (warp) go(norm_kernel<TH, TY, 1, W, true, true>);
+            else if (pieces == 1) go(norm_kernel<TH, TY, 1, W, false, true>);
+            else if (threads <= 512) go(norm_kernel<TH, TY, 2, W, false, true>);
+            else go(norm_kernel<TH, TY, 2, W, false, false>);
+        };
+        if (wide) of_width(std::true_type{});
+        else of_width(std::false_type{});
     });
     check_last_launch("block_norm");
     ctx->count_launch();
 }
 
-// How a backward call is divided.
+// How a backward call is divided.  Rows of up to 256 elements are a warp's; up to 4096 a block's of up to 512 threads that keep the sums over rows in
+// registers; up to 8192 the same with the sums in shared memory; wider ones are read twice by 1024 threads.
 struct Division {
-    uint32_t blocks, threads, owners, pieces, items;
-    bool warp, regs;
+    uint32_t blocks, threads, pieces, items;
+    bool warp, regs, hold, full, warp_items, direct_gate;
     int nv;
-    int64_t partial_floats[kSums];
+    size_t shared;
+    int64_t partial_floats[kSums], own_floats;
     size_t bytes;
 };
+
+constexpr size_t kMostShared = 220 << 10;
 
 Division divide(const b200_block_norm_grad_args& a, const Shape& p, int sms) {
     Division d{};
     d.warp = p.width <= 256;
-    d.nv = p.width <= 4096 ? 1 : 2;
-    d.regs = d.nv == 1;
+    d.regs = p.width <= 4096;
+    d.hold = p.width <= 8192;
+    d.nv = d.regs ? 1 : 2;
     d.threads = d.warp ? kWarpRows * 32 : static_cast<uint32_t>(ceil_div(p.width, int64_t(8) * d.nv * 32)) * 32;
+    d.full = a.kind == B200_NORM_LAYER || present(a.post_bias) || present(a.post_bias_grad) || present(a.pre_bias_grad);
+    const size_t own = static_cast<size_t>(d.nv) * 32 * d.threads;  // bytes of one vector of the threads' columns
+    d.shared = d.regs ? own * (2 + (d.full ? 4 : 3)) : own * (d.full ? kOwnSums : kOwnRms);
+    const bool own_shared = d.shared <= kMostShared;
+    if (!own_shared) d.shared = 0;
     const int64_t group_rows = p.s.rows / p.gates;
     // as many blocks as the registers of an SM hold at once
-    const int64_t resident = int64_t(sms) * std::max<int64_t>(1, (d.regs ? 512 : 1024) / d.threads);
-    const int64_t workers = d.warp ? resident * kWarpRows : resident;
+    const int64_t resident = int64_t(sms) * std::max<int64_t>(1, std::min<int64_t>((d.hold ? 512 : 1024) / d.threads, static_cast<int64_t>(kMostShared / (d.shared + 4096))));
+    // warps share a block's rows, unless a gate has too few of them
+    d.warp_items = d.warp && p.gates > 1 && group_rows < 8 * kWarpRows;
+    const int64_t workers = d.warp_items ? resident * kWarpRows : resident;
+    const int64_t unit = d.warp && !d.warp_items ? kWarpRows : 1;  // rows that a worker takes at once
     // a gate's rows in as many pieces as leave the longest worker the least to do
     int64_t best = INT64_MAX;
     d.pieces = 1;
-    for (int64_t n = 1; n <= std::min(group_rows, workers) && (n == 1 || p.gates * n < 2 * workers + p.gates); ++n) {
-        const int64_t longest = ceil_div(p.gates * n, workers) * ceil_div(group_rows, n);
+    for (int64_t n = 1; n <= std::min(ceil_div(group_rows, unit), workers) && (n == 1 || p.gates * n < 2 * workers + p.gates); ++n) {
+        const int64_t longest = ceil_div(p.gates * n, workers) * ceil_div(ceil_div(group_rows, n), unit);
         if (longest < best) best = longest, d.pieces = static_cast<uint32_t>(n);
     }
     d.items = static_cast<uint32_t>(p.gates * d.pieces);
     const int64_t needed = std::min<int64_t>(workers, d.items);
-    d.blocks = static_cast<uint32_t>(d.warp ? ceil_div(needed, kWarpRows) : needed);
-    d.owners = d.warp ? d.blocks * kWarpRows : d.blocks;
+    d.blocks = static_cast<uint32_t>(d.warp_items ? ceil_div(needed, kWarpRows) : needed);
+    d.direct_gate = d.pieces == 1;
     const b200_tensor* wanted[kSums] = {&a.gate_grad, &a.post_weight_grad, &a.post_bias_grad, &a.pre_weight_grad, &a.pre_bias_grad};
+    auto whole = [](int64_t floats) { return (static_cast<size_t>(floats) * sizeof(float) + 255) / 256 * 256; };
     for (int s = 0; s < kSums; ++s) {
-        if (!present(*wanted[s])) continue;
-        d.partial_floats[s] = (s == kGate ? int64_t(d.items) : int64_t(d.owners)) * p.width;
-        d.bytes += (static_cast<size_t>(d.partial_floats[s]) * sizeof(float) + 255) / 256 * 256;
+        if (!present(*wanted[s]) || (s == kGate && d.direct_gate)) continue;
+        d.partial_floats[s] = int64_t(s == kGate ? d.items : d.blocks) * p.width;
+        d.bytes += whole(d.partial_floats[s]);
+    }
+    if (!own_shared) {
+        d.own_floats = int64_t(d.blocks) * (d.full ? kOwnSums : kOwnRms) * d.nv * 8 * d.threads;
+        d.bytes += whole(d.own_floats);
     }
     return d;
 }
@@ -666,11 +914,21 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     FoldArgs fold{};
     fold.width = static_cast<int>(p.width);
     unsigned folds = 0, groups = 1;
+    auto take = [&](int64_t floats) {
+        float* at = reinterpret_cast<float*>(scratch);
+        scratch += (static_cast<size_t>(floats) * sizeof(float) + 255) / 256 * 256;
+        return at;
+    };
+    if (d.own_floats > 0) k.own = take(d.own_floats);
     for (int s = 0; s < kSums; ++s) {
         if (!present(*vectors[s])) continue;
-        k.partial[s] = reinterpret_cast<float*>(scratch);
-        scratch += (static_cast<size_t>(d.partial_floats[s]) * sizeof(float) + 255) / 256 * 256;
-        fold.f[folds++] = Fold{k.partial[s], vectors[s]->data, static_cast<uint32_t>(s == kGate ? p.gates : 1), s == kGate ? d.pieces : d.owners};
+        if (s == kGate && d.direct_gate) {
+            k.gate_grad = vectors[s]->data;
+            k.half_gate_grad = vectors[s]->dtype == B200_F16;
+            continue;
+        }
+        k.partial[s] = take(d.partial_floats[s]);
+        fold.f[folds++] = Fold{k.partial[s], vectors[s]->data, static_cast<uint32_t>(s == kGate ? p.gates : 1), s == kGate ? d.pieces : d.blocks};
         if (s == kGate) groups = static_cast<unsigned>(std::min<int64_t>(p.gates, 4096));
         fold.half = vectors[s]->dtype == B200_F16;
     }
@@ -678,6 +936,7 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     k.group_rows = static_cast<uint32_t>(p.s.rows / p.gates);
     k.pieces = d.pieces;
     k.items = d.items;
+    k.warp_items = d.warp_items;
     k.width = static_cast<int>(p.width);
     k.a = a.residual_scale;
     k.b = a.branch_scale;
@@ -691,11 +950,22 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     with_types(p, [&](auto th, auto ty) {
         using TH = decltype(th);
         using TY = decltype(ty);
-        auto go = [&](auto kernel) { launch_kernel(ctx, kernel, d.blocks, d.threads, 0, k); };
-        if (wide) go(d.warp ? norm_backward_kernel<TH, TY, 1, true, true, true> : d.regs ? norm_backward_kernel<TH, TY, 1, true, false, true>
-                                                                                         : norm_backward_kernel<TH, TY, 2, true, false, false>);
-        else go(d.warp ? norm_backward_kernel<TH, TY, 1, false, true, true> : d.regs ? norm_backward_kernel<TH, TY, 1, false, false, true>
-                                                                                     : norm_backward_kernel<TH, TY, 2, false, false, false>);
+        constexpr bool kBothHalf = sizeof(TH) == 2;
+        auto go = [&](auto kernel) {
+            (void)blocks_at_once(reinterpret_cast<const void*>(kernel), static_cast<int>(d.threads), d.shared);  // (allows that much shared memory)
+            launch_kernel(ctx, kernel, dim3(d.blocks), dim3(d.threads), d.shared, k);
+        };
+        auto of_kind = [&](auto is_wide, auto is_full) {
+            constexpr bool W = decltype(is_wide)::value, F = decltype(is_full)::value;
+            if (d.warp) go(norm_backward_kernel<TH, TY, 1, W, true, F, true, true, true>);
+            else if (d.regs) go(norm_backward_kernel<TH, TY, 1, W, false, F, true, true, true>);
+            else if (d.hold) go(norm_backward_kernel<TH, TY, 2, W, false, F, false, true, kBothHalf && W>);
+            else go(norm_backward_kernel<TH, TY, 2, W, false, F, false, false, false>);
+        };
+        if (wide && d.full) of_kind(std::true_type{}, std::true_type{});
+        else if (wide) of_kind(std::true_type{}, std::false_type{});
+        else if (d.full) of_kind(std::false_type{}, std::true_type{});
+        else of_kind(std::false_type{}, std::false_type{});
     });
     check_last_launch("block_norm_backward");
     if (folds > 0) {

@@ -578,37 +578,6 @@ struct SumArgs {
     Zeros zeros;
 };
 
-template <bool WIDE>
-__device__ __forceinline__ int sum_column(int e, int t, int threads) {
-    return WIDE ? t * 8 + e : e * threads + t;
-}
-
-// Eight columns of a row, from `first` on.
-template <typename T, bool WIDE>
-struct Piece {
-    Raw8<T> raw;
-    __device__ __forceinline__ void load(const char* row, int first, int t, int threads, int width) {
-        raw = {};
-        if (first + t * 8 < width) load8(raw, reinterpret_cast<const T*>(row) + first + t * 8);
-    }
-    __device__ __forceinline__ void get(float (&x)[8]) const { unpack8(raw, x); }
-};
-template <typename T>
-struct Piece<T, false> {
-    T raw[8];
-    __device__ __forceinline__ void load(const char* row, int first, int t, int threads, int width) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = first + sum_column<false>(e, t, threads);
-            raw[e] = c < width ? reinterpret_cast<const T*>(row)[c] : from_float<T>(0.f);
-        }
-    }
-    __device__ __forceinline__ void get(float (&x)[8]) const {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
-    }
-};
-
 // Once for each row that has a token.
 __device__ __forceinline__ void mark_row(const SumArgs& k, uint32_t id, int first, int t) {
     if (k.touched != nullptr && first == 0 && t == 0) atomicOr(&k.touched[id / 32], 1u << (id % 32));
@@ -626,15 +595,7 @@ __device__ __forceinline__ void write_row(const SumArgs& k, uint32_t id, const f
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] += sum[e] * k.scale;
-    if constexpr (WIDE) {
-        if (first + t * 8 < k.width) store8(reinterpret_cast<TO*>(row) + first + t * 8, x);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = first + sum_column<false>(e, t, k.threads);
-            if (c < k.width) reinterpret_cast<TO*>(row)[c] = from_float<TO>(x[e]);
-        }
-    }
+    store_piece<TO, WIDE>(row, x, first, t, k.threads, k.width);
 }
 
 template <typename TG, typename TO, bool WIDE>
@@ -726,7 +687,7 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_tokens_kernel(const SumArg
             float* to = k.partial + (int64_t(block) * 2 + which) * k.width + first;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int c = sum_column<WIDE>(e, t, k.threads);
+                const int c = piece_column<WIDE>(e, t, k.threads);
                 if (first + c < k.width) to[c] = sum[e];
             }
         } else {

@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 
 #include <initializer_list>
+#include <tuple>
 
 namespace b200 {
 
@@ -264,6 +265,31 @@ void check_block_norm(const b200_block_norm_args& a);
 void check_block_norm_backward(const b200_block_norm_grad_args& a);
 void check_distill_loss(const b200_distill_args& a, bool forward);
 
+// How many blocks of a kernel an SM of the current device holds at once.
+inline int blocks_at_once(const void* kernel, int threads, size_t shared) {
+    struct Key {
+        const void* kernel;
+        int threads;
+        size_t shared;
+        int device;
+        bool operator<(const Key& o) const { return std::tie(kernel, threads, shared, device) < std::tie(o.kernel, o.threads, o.shared, o.device); }
+    };
+    static std::mutex mutex;
+    static std::map<Key, int> known;
+    int dev = 0;
+    B200_CUDA_CHECK(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mutex);
+    int& n = known[Key{kernel, threads, shared, dev}];
+    if (n == 0) {
+        if (shared > 0) B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
+        int found = 0;
+        B200_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&found, kernel, threads, shared));
+        if (found < 1) fail(B200_INTERNAL_ERROR, "a kernel does not fit on an SM");
+        n = found;
+    }
+    return n;
+}
+
 // ---- device side ------------------------------------------------------------
 
 #ifdef __CUDACC__
@@ -329,6 +355,57 @@ __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
     asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
                  "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
                  : "memory");
+}
+
+// Eight columns of a row, from `first` on, for thread t of `threads` that share the row: eight neighbours where WIDE (rows of whole pieces, aligned),
+// else one of each eight stretches of `threads` neighbours.
+template <bool WIDE>
+__device__ __forceinline__ int piece_column(int e, int t, int threads) {
+    return WIDE ? t * 8 + e : e * threads + t;
+}
+
+template <typename T, bool WIDE>
+struct Piece {
+    Raw8<T> raw;
+    __device__ __forceinline__ void load(const char* row, int first, int t, int threads, int width) {
+        raw = {};
+        if (first + t * 8 < width) load8(raw, reinterpret_cast<const T*>(row) + first + t * 8);
+    }
+    __device__ __forceinline__ void clear() { raw = {}; }
+    __device__ __forceinline__ void get(float (&x)[8]) const { unpack8(raw, x); }
+};
+template <typename T>
+struct Piece<T, false> {
+    T raw[8];
+    __device__ __forceinline__ void load(const char* row, int first, int t, int threads, int width) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = first + piece_column<false>(e, t, threads);
+            raw[e] = c < width ? reinterpret_cast<const T*>(row)[c] : from_float<T>(0.f);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = from_float<T>(0.f);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = to_float(raw[e]);
+    }
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_piece(char* row, const float (&x)[8], int first, int t, int threads, int width) {
+    T* p = reinterpret_cast<T*>(row) + first;
+    if constexpr (WIDE) {
+        if (first + t * 8 < width) store8(p + t * 8, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = piece_column<false>(e, t, threads);
+            if (first + c < width) p[c] = from_float<T>(x[e]);
+        }
+    }
 }
 
 // Where row r of a tensor lies.
