@@ -25,30 +25,44 @@ namespace {
 constexpr int64_t kMostWidth = 16384;
 constexpr int kWarpRows = 8;  // warps of a block where a row is a warp's
 
-// Sums of N values over the threads of a row, the same bits in each of them.  `slot` alternates between calls, so that one barrier is enough.
+// Sums of N values (1, 4 or 8) over the threads of a row, the same bits in each of them.  Lanes halve the values among each other before they halve the
+// lanes: 6 shuffles for 4 values and 9 for 8, where one value after another takes 20 and 40.  `slot` alternates between calls, so that one
+// barrier is enough.
 template <bool WARP, int N>
 __device__ __forceinline__ void row_sums(float (&x)[N], float* part, int& slot) {
+    const int lane = threadIdx.x % 32;
+    int d = 16;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int half = N / 2; half >= 1; half /= 2, d /= 2) {
+        const bool upper = (lane & d) != 0;
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
+        for (int i = 0; i < half; ++i) {
+            const float give = upper ? x[i] : x[i + half];
+            x[i] = (upper ? x[i + half] : x[i]) + __shfl_xor_sync(0xffffffffu, give, d);
+        }
     }
+#pragma unroll
+    for (; d > 0; d /= 2) x[0] += __shfl_xor_sync(0xffffffffu, x[0], d);
+    constexpr int kLanes = 32 / N;  // lane v * kLanes has value v
+    float total = x[0];
+    int from = kLanes;
     if constexpr (!WARP) {
-        const int lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        const int values = blockDim.x / 32 * N;
         float* const here = part + slot * (N * 32);
-        if (lane == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) here[i * 32 + threadIdx.x / 32] = x[i];
-        }
+        if (lane % kLanes == 0) here[threadIdx.x / 32 * N + lane / kLanes] = total;
         __syncthreads();
+        total = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            x[i] = lane < warps ? here[i * 32 + lane] : 0.f;
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) x[i] += __shfl_xor_sync(0xffffffffu, x[i], d);
+        for (int i = 0; i < N; ++i) {  // lane l has values l % N of some warps
+            if (i * 32 < values && i * 32 + lane < values) total += here[i * 32 + lane];
         }
+#pragma unroll
+        for (int e = N; e < 32; e *= 2) total += __shfl_xor_sync(0xffffffffu, total, e);
         slot ^= 1;
+        from = 1;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = N == 1 ? total : __shfl_sync(0xffffffffu, total, i * from);
 }
 
 // Eight values to a thread in memory that no other thread touches: 16 bytes of the block's threads side by side.
@@ -293,7 +307,7 @@ __host__ __device__ constexpr int own_place(int which) { return which == kE ? 0 
 template <typename TH, typename TY, int NV, bool WIDE, bool WARP, bool FULL, bool REGS, bool HOLD, bool AHEAD>
 __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : HOLD ? 512 : 1024, WARP ? 2 : 1)
 norm_backward_kernel(const BackwardArgs k) {
-    constexpr int N = FULL ? 8 : 3;
+    constexpr int N = FULL ? 8 : 4;
     extern __shared__ __align__(16) float shared_own[];
     __shared__ float part[2 * N * 32];
     __shared__ float meet[WARP ? kWarpRows : 1][WARP ? 256 : 1];
@@ -336,17 +350,25 @@ norm_backward_kernel(const BackwardArgs k) {
     auto add = [&](int which, int v, const float (&x)[8]) {
         if constexpr (REGS) {
             if (which < 4) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum[which][v][e] += x[e];
+                add8(sum[which][v], sum[which][v], x);
                 return;
             }
         }
         float y[8];
         get_sum(which, v, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += x[e];
+        add8(y, y, x);
         if constexpr (REGS) own_store(shared_own, (which - kPostW) * NV + v, y);
         else own_store(own, own_place(which) * NV + v, y);
+    };
+    auto add_product = [&](int which, int v, const float (&a)[8], const float (&b)[8]) {
+        if constexpr (REGS) {
+            fma8(sum[which][v], a, b, sum[which][v]);
+        } else {
+            float y[8];
+            get_sum(which, v, y);
+            fma8(y, a, b, y);
+            own_store(own, own_place(which) * NV + v, y);
+        }
     };
     // WARP: a value summed over the block's warps, in the first one
     auto over_warps = [&](float (&x)[8]) {
@@ -363,15 +385,25 @@ norm_backward_kernel(const BackwardArgs k) {
             }
         }
     };
-    // the columns' factors: w1, w2, b gate and b2; from the thread's own memory where that is (REGS), else read where they are needed
-    enum { kW1, kW2, kG, kB2 };
+    // the columns' factors: w1 and c = b gate w2 in every row, b gate, w2 and b2 at an item's end; w1 and c from the thread's own memory where that is (REGS)
+    enum { kW1, kC, kW2, kG, kB2 };
     const char* gate = nullptr;
     auto read_factor = [&](int which, int v, float (&x)[8]) {
-        const void* from = which == kW1 ? k.pre_weight : which == kW2 ? k.post_weight : which == kG ? static_cast<const void*>(gate) : k.post_bias;
-        read_columns<WIDE>(x, from, k.half_columns, which == kB2 ? 0.f : 1.f, v * threads * 8, t, threads, k.width);
-        if (which == kG) {
+        const int first = v * threads * 8;
+        const void* from = which == kW1 ? k.pre_weight : which == kB2 ? k.post_bias : which == kG ? static_cast<const void*>(gate) : k.post_weight;
+        read_columns<WIDE>(x, from, k.half_columns, which == kB2 ? 0.f : 1.f, first, t, threads, k.width);
+        if (which == kG) mul8(x, x, k.b);
+        if (which == kC) {
+            float g[8];
+            read_columns<WIDE>(g, gate, k.half_columns, 1.f, first, t, threads, k.width);
+            mul8(g, g, k.b);
+            mul8(x, x, g);
+            if constexpr (!WIDE || FULL) {  // y^ is not 0 behind the row's end
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= k.b;
+                for (int e = 0; e < 8; ++e) {
+                    if (first + piece_column<WIDE>(e, t, threads) >= k.width) x[e] = 0.f;
+                }
+            }
         }
     };
     auto factor = [&](int which, int v, float (&x)[8]) {
@@ -407,8 +439,6 @@ norm_backward_kernel(const BackwardArgs k) {
         if (FULL || own_place(s) < kOwnRms) clear(s);
     }
     keep_factor(kW1);
-    keep_factor(kW2);
-    if (FULL) keep_factor(kB2);
     const bool by_warp = WARP && k.warp_items;
     const uint32_t step = WARP && !by_warp ? kWarpRows : 1, workers = by_warp ? gridDim.x * kWarpRows : gridDim.x;
     for (uint32_t item = by_warp ? blockIdx.x * kWarpRows + warp : blockIdx.x; item < k.items; item += workers) {
@@ -417,7 +447,7 @@ norm_backward_kernel(const BackwardArgs k) {
         const uint32_t r1 = group * k.group_rows + stretch(k.group_rows, piece + 1, k.pieces);
         gate = static_cast<const char*>(k.gate);
         if (gate != nullptr) gate += int64_t(group) * k.gate_pitch;
-        keep_factor(kG);
+        keep_factor(kC);
         auto load_ahead = [&](uint32_t r) {
             if constexpr (AHEAD) {
 #pragma unroll
@@ -432,11 +462,10 @@ norm_backward_kernel(const BackwardArgs k) {
             if (!WARP) __syncthreads();  // (the reductions before and after lay their values out otherwise)
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                float w[8], g[8];
-                factor(kW2, v, w);
-                factor(kG, v, g);
+                float c[8];
+                factor(kC, v, c);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[0] += v * threads * 8 + piece_column<WIDE>(e, t, threads) < k.width ? w[e] * g[e] : 0.f;
+                for (int e = 0; e < 8; ++e) x[0] += c[e];
             }
             row_sums<WARP, 1>(x, part, slot);
             if (!WARP) __syncthreads();
@@ -455,52 +484,61 @@ norm_backward_kernel(const BackwardArgs k) {
                 }
                 if (k.stats != nullptr) st = k.stats[r];
             }
-            const float y_mean = k.post ? st.x : 0.f, y_scale = k.post ? st.y : 1.f;
-            // s^, g, t and y^ of a piece
-            auto terms = [&](int v, float (&s)[8], float (&n)[8], float (&g)[8], float (&o)[8], float (&y)[8]) {
+            const float y_scale = k.post ? st.y : 1.f, y_shift = FULL && k.post ? -st.x : 0.f;
+            const float s_scale = pre ? st.w : 0.f, s_shift = FULL && pre ? -st.z : 0.f;
+            float s[HOLD ? NV : 1][8], n[HOLD ? NV : 1][8], o[HOLD ? NV : 1][8], y[HOLD ? NV : 1][8];
+            // s^, dn, t and y^ of a piece; adds g s^ and g
+            float2 sum_gs = {}, sum_g = {};
+            auto terms = [&](int v, bool sums) {
+                const int h = HOLD ? v : 0;
                 if constexpr (!HOLD) load_piece(r, v, s_piece[0], n_piece[0], o_piece[0], y_piece[0]);
-                s_piece[HOLD ? v : 0].get(s);
-                n_piece[HOLD ? v : 0].get(n);
-                o_piece[HOLD ? v : 0].get(o);
-                y_piece[HOLD ? v : 0].get(y);
-                float w[8];
-                factor(kW1, v, w);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    s[e] = pre ? (s[e] - st.z) * st.w : 0.f;
-                    g[e] = n[e] * w[e];
-                    y[e] = (y[e] - y_mean) * y_scale;
-                    o[e] = pre ? fmaf(st.w, g[e], o[e]) : o[e];
+                s_piece[h].get(s[h]);
+                n_piece[h].get(n[h]);
+                o_piece[h].get(o[h]);
+                y_piece[h].get(y[h]);
+                if constexpr (FULL) {  // (the difference first: what lies near the mean keeps its digits)
+                    add8(s[h], s[h], s_shift);
+                    add8(y[h], y[h], y_shift);
+                }
+                mul8(s[h], s[h], s_scale);
+                mul8(y[h], y[h], y_scale);
+                if (pre) {
+                    float g[8];
+                    factor(kW1, v, g);
+                    mul8(g, g, n[h]);
+                    fma8(o[h], g, st.w, o[h]);
+                    if (sums) {
+                        dot8(sum_gs, g, s[h]);
+                        if (FULL) sum8(sum_g, g);
+                    }
                 }
             };
-            float x[N] = {};  // g s^; c y^ t, c y^ s^; FULL: g; c t, c s^, c y^
+            float2 sum_cyt = {}, sum_cys = {}, sum_ct = {}, sum_cs = {}, sum_cy = {};
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                float s[8], n[8], g[8], o[8], y[8], c[8], w[8];
-                terms(v, s, n, g, o, y);
-                factor(kW2, v, c);
-                factor(kG, v, w);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (!WIDE || FULL) {  // (columns behind the row's end: y^ is not 0 there)
-                        if (v * threads * 8 + piece_column<WIDE>(e, t, threads) >= k.width) continue;
-                    }
-                    c[e] *= w[e];
-                    const float cy = c[e] * y[e];
-                    x[0] = fmaf(g[e], s[e], x[0]);
-                    x[1] = fmaf(cy, o[e], x[1]);
-                    x[2] = fmaf(cy, s[e], x[2]);
-                    if constexpr (FULL) {
-                        x[3] += g[e];
-                        x[4] = fmaf(c[e], o[e], x[4]);
-                        x[5] = fmaf(c[e], s[e], x[5]);
-                        x[6] += cy;
+                const int h = HOLD ? v : 0;
+                terms(v, true);
+                if (k.post) {
+                    float c[8], cy[8];
+                    factor(kC, v, c);
+                    mul8(cy, c, y[h]);
+                    dot8(sum_cyt, cy, o[h]);
+                    dot8(sum_cys, cy, s[h]);
+                    if (FULL && k.layer) {
+                        dot8(sum_ct, c, o[h]);
+                        dot8(sum_cs, c, s[h]);
+                        sum8(sum_cy, cy);
                     }
                 }
             }
+            float x[N] = {};
+            x[0] = sum_gs.x + sum_gs.y, x[1] = sum_cyt.x + sum_cyt.y, x[2] = sum_cys.x + sum_cys.y;
+            if constexpr (FULL) {
+                x[3] = sum_g.x + sum_g.y, x[4] = sum_ct.x + sum_ct.y, x[5] = sum_cs.x + sum_cs.y, x[6] = sum_cy.x + sum_cy.y;
+            }
             row_sums<WARP, N>(x, part, slot);
-            const float m1 = x[0] * k.share * st.w;  // r1 m1, r1 m0
-            const float m0 = FULL && k.layer ? x[FULL ? 3 : 0] * k.share * st.w : 0.f;
+            const float m1 = x[0] * k.share * s_scale;  // r1 m1, r1 m0
+            const float m0 = FULL && k.layer ? x[3] * k.share * s_scale : 0.f;
             float k1 = 0.f, k0 = 0.f;
             if (k.post) {
                 k1 = x[1] * k.share - m1 * (x[2] * k.share);
@@ -513,35 +551,31 @@ norm_backward_kernel(const BackwardArgs k) {
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                float s[8], n[8], g[8], o[8], y[8];
-                terms(v, s, n, g, o, y);
+                const int h = HOLD ? v : 0;
+                if constexpr (!HOLD) terms(v, false);
                 if (pre) {
-                    float q[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[e] = n[e] * s[e];
-                    add(kPreW, v, q);
-                    if (FULL) add(kPreB, v, n);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = o[e] - m0 - s[e] * m1;  // ds
+                    add_product(kPreW, v, n[h], s[h]);
+                    if (FULL) add(kPreB, v, n[h]);
+                    fma8(o[h], s[h], -m1, o[h]);  // ds
+                    if constexpr (FULL) {
+                        add8(o[h], o[h], -m0);
+                    }
                 }
                 if (k.residual_grad.base != nullptr) {
                     float q[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[e] = k.a * o[e];
+                    mul8(q, o[h], k.a);
                     store_piece<TH, WIDE>(row_at(k.residual_grad, k.inner, r), q, v * threads * 8, t, threads, k.width);
                 }
                 if (branch) {
-                    float q[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[e] = o[e] * y[e];
-                    add(kE, v, q);
-                    if (FULL) add(kF, v, o);
+                    add_product(kE, v, o[h], y[h]);
+                    if (FULL) add(kF, v, o[h]);
                     if (k.branch_grad.base != nullptr) {
-                        float w[8];
-                        factor(kG, v, q);
-                        factor(kW2, v, w);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) q[e] = y_scale * (q[e] * w[e] * o[e] - k0 - y[e] * k1);
+                        float q[8];
+                        factor(kC, v, q);
+                        mul8(q, q, o[h]);
+                        fma8(q, y[h], -k1, q);
+                        if constexpr (FULL) fma8(q, q, y_scale, -k0 * y_scale);
+                        else mul8(q, q, y_scale);
                         store_piece<TY, WIDE>(row_at(k.branch_grad, k.inner, r), q, v * threads * 8, t, threads, k.width);
                     }
                 }
@@ -559,8 +593,8 @@ norm_backward_kernel(const BackwardArgs k) {
             }
             if (WARP && !by_warp && warp != 0) continue;
             if (k.partial[kGate] != nullptr || k.gate_grad != nullptr) {
-                factor(kW2, v, w);
-                if (FULL) factor(kB2, v, b);
+                read_factor(kW2, v, w);
+                if (FULL) read_factor(kB2, v, b);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) q[e] = k.b * (w[e] * e_sum[e] + b[e] * f_sum[e]);
                 // (the partial sums and a gate's gradient are dense, and may start anywhere)
@@ -568,9 +602,9 @@ norm_backward_kernel(const BackwardArgs k) {
                 if (k.gate_grad != nullptr && k.half_gate_grad) store_columns<__half, WIDE>(static_cast<__half*>(k.gate_grad) + at, q, v * threads * 8, t, threads, k.width);
                 else store_columns<float, WIDE>((k.gate_grad != nullptr ? static_cast<float*>(k.gate_grad) : k.partial[kGate]) + at, q, v * threads * 8, t, threads, k.width);
             }
-            factor(kG, v, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) e_sum[e] *= w[e], f_sum[e] *= w[e];
+            read_factor(kG, v, w);
+            mul8(e_sum, e_sum, w);
+            if (FULL) mul8(f_sum, f_sum, w);
             add(kPostW, v, e_sum);
             if (FULL) add(kPostB, v, f_sum);
         }
@@ -810,7 +844,7 @@ Division divide(const b200_block_norm_grad_args& a, const Shape& p, int sms) {
     d.threads = d.warp ? kWarpRows * 32 : static_cast<uint32_t>(ceil_div(p.width, int64_t(8) * d.nv * 32)) * 32;
     d.full = a.kind == B200_NORM_LAYER || present(a.post_bias) || present(a.post_bias_grad) || present(a.pre_bias_grad);
     const size_t own = static_cast<size_t>(d.nv) * 32 * d.threads;  // bytes of one vector of the threads' columns
-    d.shared = d.regs ? own * (2 + (d.full ? 4 : 3)) : own * (d.full ? kOwnSums : kOwnRms);
+    d.shared = d.regs ? own * 4 : own * (d.full ? kOwnSums : kOwnRms);
     const bool own_shared = d.shared <= kMostShared;
     if (!own_shared) d.shared = 0;
     const int64_t group_rows = p.s.rows / p.gates;

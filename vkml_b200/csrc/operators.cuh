@@ -357,6 +357,67 @@ __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
                  : "memory");
 }
 
+// Arithmetic on eight values, two to an instruction.
+__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul_pair(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add_pair(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+// d = a * b + c, of eight; of one b; of one b and one c
+__device__ __forceinline__ void fma8(float (&d)[8], const float (&a)[8], const float (&b)[8], const float (&c)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) fma_pair(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+}
+__device__ __forceinline__ void fma8(float (&d)[8], const float (&a)[8], float b, const float (&c)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) fma_pair(d[i], d[i + 1], a[i], a[i + 1], b, b, c[i], c[i + 1]);
+}
+__device__ __forceinline__ void fma8(float (&d)[8], const float (&a)[8], float b, float c) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) fma_pair(d[i], d[i + 1], a[i], a[i + 1], b, b, c, c);
+}
+__device__ __forceinline__ void mul8(float (&d)[8], const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) mul_pair(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+}
+__device__ __forceinline__ void mul8(float (&d)[8], const float (&a)[8], float b) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) mul_pair(d[i], d[i + 1], a[i], a[i + 1], b, b);
+}
+__device__ __forceinline__ void add8(float (&d)[8], const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) add_pair(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+}
+__device__ __forceinline__ void add8(float (&d)[8], const float (&a)[8], float b) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) add_pair(d[i], d[i + 1], a[i], a[i + 1], b, b);
+}
+// s += a * b, and s += a, in two sums
+__device__ __forceinline__ void dot8(float2& s, const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) fma_pair(s.x, s.y, a[i], a[i + 1], b[i], b[i + 1], s.x, s.y);
+}
+__device__ __forceinline__ void sum8(float2& s, const float (&a)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) add_pair(s.x, s.y, s.x, s.y, a[i], a[i + 1]);
+}
+
 // Eight columns of a row, from `first` on, for thread t of `threads` that share the row: eight neighbours where WIDE (rows of whole pieces, aligned),
 // else one of each eight stretches of `threads` neighbours.
 template <bool WIDE>
