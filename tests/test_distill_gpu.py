@@ -73,7 +73,24 @@ def test_losses_and_gradient(backend, dtype, shape, top, layout, temperature, ha
     run(backend, placed(z, layout), placed(k, layout), placed(t, layout), labels, weights, temperature, hard, 4.0, layout)
 
 
-@pytest.mark.parametrize("shape", [(4, 100), (2, 40000), (2, 130001)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("shape,top,layout,temperature,hard", [
+    ((300, 16384), 8, "dense", 1.0, 0.5), ((150, 2, 17001), 33, "odd", 2.0, 0.0), ((297, 32768), 64, "dense", 1.0, 0.0), ((301, 40003), 5, "offset", 2.0, 0.3),
+    ((2, 150, 52000), 100, "swapped", 1.5, 1.0), ((320, 98304), 3, "dense", 1.0, 0.1), ((299, 99001), 40, "pitch", 2.0, 0.5)])
+def test_many_rows(backend, dtype, shape, top, layout, temperature, hard):
+    """More rows than blocks: every row's sums, loss and columns are its own."""
+    rng = np.random.default_rng(shape[-1])
+    rows, vocab = int(np.prod(shape[:-1])), shape[-1]
+    z = rng.standard_normal(shape, dtype=np.float32).astype(dtype) * dtype(2)
+    k = rng.integers(-1, vocab, shape[:-1] + (top,)).astype(np.int32)
+    t = rng.standard_normal(shape[:-1] + (top,)).astype(dtype)
+    labels = rng.integers(-1, vocab, shape[:-1]) if hard else None
+    weights = (rng.random(shape[:-1]) * 8).astype(F32)
+    weights.reshape(-1)[::7] = 0
+    run(backend, placed(z, layout), placed(k, "dense"), placed(t, layout), labels, weights, temperature, hard, 4.0, layout)
+
+
+@pytest.mark.parametrize("shape", [(4, 100), (2, 40000), (2, 130001), (300, 17000), (300, 100003)])
 @pytest.mark.parametrize("dtype", [F32, F16])
 def test_gradient_over_the_logits(backend, shape, dtype):
     rng = np.random.default_rng(2)

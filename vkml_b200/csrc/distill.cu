@@ -6,9 +6,12 @@
 //   loss = (1 - c) T^2 sum_j p_j (log p_j - log q_{k_j}) + c (log sum exp z - z_label)
 //   grad = w [ (1 - c) T (q - p at k) + c (h - 1 at the label) ]
 //
-// Bound by memory: z read once and, with a gradient, as much written.  A block takes a row.  One pass over it keeps the running maximum and the
-// running sums of exp((z - max) / T) and exp(z - max); the gradient's pass writes q and h in every column, and the K + 1 columns that
-// the teacher or the label adds to are written again afterwards.
+// Bound by memory: z read once and, with a gradient, as much written.  A row is a block's, or a cluster's whose blocks take a stretch of it each: up to
+// kVectors vectors of 16 bytes to a thread, all under way at once and held in registers from the reading to the gradient, so that z is read once.  (Rows
+// too long for a cluster of 8 are taken in batches and read again for the gradient.)  A thread finds the maximum of what it holds and the sums of
+// exp((z - max) / T) and exp(z - max) beside it; the block, and then the cluster, joins these threes in one round.  The gradient's pass writes q and h in every
+// column, and the K + 1 columns that the teacher or the label adds to are written again afterwards.
+// Where both parts have a weight and T is not 1, an element takes two exponentials in each pass.
 #include "operators.cuh"
 
 #include <algorithm>
@@ -17,7 +20,8 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kMostThreads = 512;
+constexpr int kVectors = 8;
 constexpr int kMostTop = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -29,6 +33,7 @@ struct Args {
     uint32_t* status;
     int64_t vocab;
     int top;
+    int blocks;           // of a row's cluster
     bool wide_ids, wide_labels, half_teacher;
     bool soft, hard;      // which parts have a weight
     float temperature, inverse, hard_weight, grad_scale;
@@ -40,12 +45,33 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
-// Running maximum and sums of a part of a row.  A maximum of -inf (nothing but -inf so far) has sums of 0.
-struct Running {
+// A maximum of -inf (nothing but -inf so far) has sums of 0: differences to 0 keep them so.
+__device__ __forceinline__ float shift_of(float top) { return top == -INFINITY ? 0.f : top; }
+
+// Maximum, and the sums of exp((z - max) / T) and exp(z - max), of a part of a row.
+struct Part {
     float top, soft, hard;
 };
 
-__device__ __forceinline__ float shift_of(float top) { return top == -INFINITY ? 0.f : top; }
+// Over the lanes of a warp, in each of them.
+__device__ __forceinline__ Part warp_part(Part x, float c_soft, bool soft, bool hard) {
+    float top = x.top;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float apart = x.top - shift_of(top);
+    x.top = top;
+    if (soft) {
+        x.soft *= fast_exp2(apart * c_soft);
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) x.soft += __shfl_xor_sync(0xffffffffu, x.soft, d);
+    }
+    if (hard) {
+        x.hard *= fast_exp2(apart * kLog2e);
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) x.hard += __shfl_xor_sync(0xffffffffu, x.hard, d);
+    }
+    return x;
+}
 
 template <typename F>
 __device__ __forceinline__ float block_reduce(float x, float* part, F&& join, float empty) {
@@ -54,18 +80,21 @@ __device__ __forceinline__ float block_reduce(float x, float* part, F&& join, fl
     __syncthreads();
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = x;
     __syncthreads();
-    x = threadIdx.x % 32 < kThreads / 32 ? part[threadIdx.x % 32] : empty;
+    x = threadIdx.x % 32 < blockDim.x / 32 ? part[threadIdx.x % 32] : empty;
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) x = join(x, __shfl_xor_sync(0xffffffffu, x, d));
     return x;
 }
 
-// Elements of a row that lie before its first 16-byte boundary, and how many vectors of 16 bytes follow.
+// Elements of a row that lie before its first 16-byte boundary.
 template <typename T>
 __device__ __forceinline__ int64_t head_of(const T* row, int64_t n) {
     const int64_t head = (16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / int64_t(sizeof(T));
     return head < n ? head : n;
 }
+
+template <typename T>
+constexpr uint32_t kNothing = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u;  // -inf
 
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& raw, float (&x)[16 / sizeof(T)]) {
@@ -97,26 +126,168 @@ __device__ __forceinline__ uint4 pack(const float (&x)[16 / sizeof(T)]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The largest element of a vector (halves compare as halves, two at a time).
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& raw) {
+    if constexpr (sizeof(T) == 2) {
+        const __half2* h = reinterpret_cast<const __half2*>(&raw);
+        const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    } else {
+        return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+    }
+}
+
+// Adds the elements of kVectors vectors to a part of a row.
+template <typename T>
+__device__ __forceinline__ void take_vectors(Part& run, const uint4 (&raw)[kVectors], float c_soft, bool with_soft, bool with_hard) {
+    constexpr int E = 16 / sizeof(T);
+    float top = run.top;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) top = fmaxf(top, largest<T>(raw[i]));
+    const float shift = shift_of(top);
+    if (top > run.top) {
+        run.soft *= fast_exp2((run.top - shift) * c_soft);
+        run.hard *= fast_exp2((run.top - shift) * kLog2e);
+        run.top = top;
+    }
+    float2 soft = {}, hard = {};
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        float x[E], y[E];
+        unpack<T>(raw[i], x);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) add_pair(x[e], x[e + 1], x[e], x[e + 1], -shift, -shift);
+        if (with_soft) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                mul_pair(y[e], y[e + 1], x[e], x[e + 1], c_soft, c_soft);
+                add_pair(soft.x, soft.y, soft.x, soft.y, fast_exp2(y[e]), fast_exp2(y[e + 1]));
+            }
+        }
+        if (with_hard) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                mul_pair(y[e], y[e + 1], x[e], x[e + 1], kLog2e, kLog2e);
+                add_pair(hard.x, hard.y, hard.x, hard.y, fast_exp2(y[e]), fast_exp2(y[e + 1]));
+            }
+        }
+    }
+    run.soft += soft.x + soft.y;
+    run.hard += hard.x + hard.y;
+}
+
+// What a row's gradient is made of: ws q + wh h, q = exp2((z - at) c_soft + soft2), h = exp2((z - at) log2 e + hard2).
+struct RowGrad {
+    float ws, wh, at, soft2, hard2;
+};
+__device__ __forceinline__ float grad_value(const RowGrad& g, float c_soft, float x) {
+    float y = 0.f;
+    if (g.ws != 0.f) y += g.ws * fast_exp2(fmaf(x - g.at, c_soft, g.soft2));
+    if (g.wh != 0.f) y += g.wh * fast_exp2(fmaf(x - g.at, kLog2e, g.hard2));
+    return y;
+}
+template <typename T>
+__device__ __forceinline__ void grad_vector(const RowGrad& g, float c_soft, const uint4& raw, T* to, bool aligned) {
+    constexpr int E = 16 / sizeof(T);
+    float x[E], y[E];
+    unpack<T>(raw, x);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) add_pair(x[e], x[e + 1], x[e], x[e + 1], -g.at, -g.at);
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = 0.f;
+    if (g.ws != 0.f) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            fma_pair(y[e], y[e + 1], x[e], x[e + 1], c_soft, c_soft, g.soft2, g.soft2);
+            mul_pair(y[e], y[e + 1], fast_exp2(y[e]), fast_exp2(y[e + 1]), g.ws, g.ws);
+        }
+    }
+    if (g.wh != 0.f) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            fma_pair(x[e], x[e + 1], x[e], x[e + 1], kLog2e, kLog2e, g.hard2, g.hard2);
+            fma_pair(y[e], y[e + 1], fast_exp2(x[e]), fast_exp2(x[e + 1]), g.wh, g.wh, y[e], y[e + 1]);
+        }
+    }
+    if (aligned) {
+        *reinterpret_cast<uint4*>(to) = pack<T>(y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) to[e] = from_float<T>(y[e]);
+    }
+}
+
+// What p and the label take off the gradient's column col[j], if entry j is the first that names it.  The columns lie on a 16-byte boundary, `top` + 1 of
+// them and none (-1) up to the next multiple of four.  Almost always an entry is alone, which a comparison with four at a time shows.
+__device__ __forceinline__ bool entry_takes(const RowGrad& row, const int* col, const float* p, int top, bool soft, int j, float& minus) {
+    const int c = col[j];
+    int equal = 0;
+#pragma unroll 4
+    for (int m = 0; m <= top; m += 4) {
+        const int4 four = *reinterpret_cast<const int4*>(col + m);
+        equal += (four.x == c) + (four.y == c) + (four.z == c) + (four.w == c);
+    }
+    minus = 0.f;
+    if (equal == 1) {
+        if (j == top) minus = row.wh;
+        else if (row.ws != 0.f) minus = row.ws * p[j];
+        return true;
+    }
+    for (int m = 0; m < top && soft; ++m) {
+        if (col[m] != c) continue;
+        if (m < j) return false;
+        if (row.ws != 0.f) minus += row.ws * p[m];
+    }
+    if (col[top] == c) minus += row.wh;
+    return true;
+}
+// Arrays of a row's entries in shared memory: the columns [top + 1 and up to 3 of none], probabilities [top], logits there [top + 1].
+__host__ __device__ __forceinline__ int entry_words(int top) { return (top / 4 + 1) * 4 + (top + 3) / 4 * 4 + (top / 4 + 1) * 4; }
+
+// Few rows, or short ones: a block or a cluster to a row.
 template <typename T, bool FORWARD, bool GRAD>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kMostThreads, 2)
 distill_kernel(const Args k) {
     constexpr int E = 16 / sizeof(T);
-    extern __shared__ char shared[];
-    float* const p = reinterpret_cast<float*>(shared);        // [top]: the teacher's probabilities
-    float* const zk = p + k.top;                              // [top + 1]: the logits at its columns, and at the label's
-    int* const col = reinterpret_cast<int*>(zk + k.top + 1);  // [top + 1]: the columns, -1: none
+    extern __shared__ __align__(16) char shared[];
+    int* const col = reinterpret_cast<int*>(shared);                         // the columns, -1: none
+    float* const p = reinterpret_cast<float*>(col + (k.top / 4 + 1) * 4);    // the teacher's probabilities
+    float* const zk = p + (k.top + 3) / 4 * 4;                               // the logits at the teacher's columns, and at the label's
     __shared__ float part[32];
+    __shared__ Part parts[32];
+    __shared__ Part block_part;  // read by the other blocks of the cluster
     pdl_prologue();
-    const int tid = threadIdx.x;
-    const uint32_t r = blockIdx.x;
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const uint32_t r = blockIdx.x / k.blocks, rank = blockIdx.x % k.blocks;
     const T* const z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
+    T* const g = GRAD ? reinterpret_cast<T*>(row_at(k.grad, k.inner, r)) : nullptr;
+
+    // This block's vectors, kVectors * threads at a time; and an element of the row's ends for some threads of the first and the last block.
+    const int64_t head = head_of(z, k.vocab), all_vectors = (k.vocab - head) / E, tail = head + all_vectors * E;
+    const int64_t v0 = all_vectors * rank / k.blocks, v1 = all_vectors * (rank + 1) / k.blocks;
+    int64_t end = -1;
+    if (rank == 0 && tid < head) end = tid;
+    if (rank + 1 == k.blocks && tid >= 8 && tail + (tid - 8) < k.vocab) end = tail + (tid - 8);
+    const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
+    uint4 raw[kVectors];
+    float end_z = -INFINITY;
+    auto load = [&](int64_t from) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int64_t v = from + i * threads + tid;
+            raw[i] = v < v1 ? zv[v] : make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+        }
+    };
+    load(v0);
+    if (end >= 0) end_z = to_float(z[end]);
 
     // the teacher's distribution and the logits at its columns
     float top_t = -INFINITY;
     if (k.soft) {
         const char* ids = row_at(k.ids, k.inner, r);
         const char* t = row_at(k.teacher, k.inner, r);
-        for (int j = tid; j < k.top; j += kThreads) {
+        for (int j = tid; j < k.top; j += threads) {
             const int64_t id = load_index(ids + int64_t(j) * (k.wide_ids ? 8 : 4), k.wide_ids);
             const bool in = id >= 0 && id < k.vocab;
             if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
@@ -126,6 +297,10 @@ distill_kernel(const Args k) {
             top_t = fmaxf(top_t, p[j]);
         }
     }
+    if (!k.soft) {
+        for (int j = tid; j < k.top; j += threads) col[j] = -1;
+    }
+    if (tid > 0 && tid < 4 && k.top + tid < (k.top / 4 + 1) * 4) col[k.top + tid] = -1;
     if (tid == 0) {
         int64_t id = -1;
         if (k.hard) id = load_index(row_at(k.labels, k.inner, r), k.wide_labels);
@@ -141,74 +316,64 @@ distill_kernel(const Args k) {
     if (k.soft) {
         top_t = block_reduce(top_t, part, [](float a, float b) { return fmaxf(a, b); }, -INFINITY);
         float sum = 0.f;
-        for (int j = tid; j < k.top; j += kThreads) sum += col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse) : 0.f;
+        for (int j = tid; j < k.top; j += threads) sum += col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse) : 0.f;
         sum = block_reduce(sum, part, [](float a, float b) { return a + b; }, 0.f);
         taught = !(sum == 0.f);
         log_sum = logf(sum);
         if constexpr (!FORWARD) {
-            for (int j = tid; j < k.top; j += kThreads) p[j] = taught && col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse - log_sum) : 0.f;
+            for (int j = tid; j < k.top; j += threads) p[j] = taught && col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse - log_sum) : 0.f;
         }
     }
 
-    // the row's log sums of exponentials
+    // The row's maximum and log sums of exponentials: q = exp((z - at) / T - log_soft), h = exp(z - at - log_hard).  The maximum and the logarithms stay
+    // apart: their sum would lose the logarithm in a row whose logits are all the type's lowest value.
     const float c_soft = k.inverse * kLog2e;
-    const int64_t head = head_of(z, k.vocab), vectors = (k.vocab - head) / E, tail = head + vectors * E;
-    // q = exp((z - at) / T - log_soft), h = exp(z - at - log_hard).  The maximum and the logarithms stay apart: their sum would lose the
-    // logarithm in a row whose logits are all the type's lowest value.
     float at = 0.f, log_soft = 0.f, log_hard = 0.f;
     if constexpr (FORWARD) {
-        Running run = {-INFINITY, 0.f, 0.f};
-        auto take = [&](const float* x, int n) {
-            float top = x[0];
-            for (int e = 1; e < n; ++e) top = fmaxf(top, x[e]);
-            if (top > run.top) {
-                const float at = shift_of(top);
-                run.soft *= fast_exp2((run.top - at) * c_soft);
-                run.hard *= fast_exp2((run.top - at) * kLog2e);
-                run.top = top;
-            }
-            const float at = shift_of(run.top);
-            if (k.soft) {
-                for (int e = 0; e < n; ++e) run.soft += fast_exp2((x[e] - at) * c_soft);
-            }
-            if (k.hard) {
-                for (int e = 0; e < n; ++e) run.hard += fast_exp2((x[e] - at) * kLog2e);
-            }
-        };
-        for (int64_t i = tid; i < head; i += kThreads) {
-            const float x = to_float(z[i]);
-            take(&x, 1);
+        const float one = end_z == -INFINITY ? 0.f : 1.f + (end_z - end_z);  // (not a number where z is none or +inf, as it is in a vector)
+        Part run = {end_z, one, one};
+        for (int64_t from = v0;;) {
+            take_vectors<T>(run, raw, c_soft, k.soft, k.hard);
+            from += kVectors * threads;
+            if (from >= v1) break;
+            load(from);
         }
-        for (int64_t i = tail + tid; i < k.vocab; i += kThreads) {
-            const float x = to_float(z[i]);
-            take(&x, 1);
+        run = warp_part(run, c_soft, k.soft, k.hard);
+        if (tid % 32 == 0) parts[tid / 32] = run;
+        __syncthreads();
+        run = tid % 32 < threads / 32 ? parts[tid % 32] : Part{-INFINITY, 0.f, 0.f};
+        run = warp_part(run, c_soft, k.soft, k.hard);
+        if (k.blocks > 1) {
+            if (tid == 0) block_part = run;
+            cluster_sync();
+            run = Part{-INFINITY, 0.f, 0.f};
+            if (tid % 32 < k.blocks) {
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&block_part))), "r"(tid % 32));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(run.top) : "r"(there) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(run.soft) : "r"(there + 4) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(run.hard) : "r"(there + 8) : "memory");
+            }
+            run = warp_part(run, c_soft, k.soft, k.hard);
+            asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // this block has read the others' parts
         }
-        const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
-#pragma unroll 4
-        for (int64_t i = tid; i < vectors; i += kThreads) {
-            float x[E];
-            unpack<T>(zv[i], x);
-            take(x, E);
-        }
-        const float top = block_reduce(run.top, part, [](float a, float b) { return fmaxf(a, b); }, -INFINITY);
-        at = shift_of(top);
-        auto add = [](float a, float b) { return a + b; };
-        if (k.soft) log_soft = logf(block_reduce(run.soft * fast_exp2((run.top - at) * c_soft), part, add, 0.f));
-        if (k.hard) log_hard = logf(block_reduce(run.hard * fast_exp2((run.top - at) * kLog2e), part, add, 0.f));
-        if (tid == 0 && k.stats != nullptr) k.stats[r] = make_float4(top, log_soft, log_hard, 0.f);
+        at = shift_of(run.top);
+        if (k.soft) log_soft = logf(run.soft);
+        if (k.hard) log_hard = logf(run.hard);
+        if (rank == 0 && tid == 0 && k.stats != nullptr) k.stats[r] = make_float4(run.top, log_soft, log_hard, 0.f);
         // a row of nothing but -inf: the sums are 0 and their logarithms -inf, which stay out of the differences so that q = 0, log q = -inf
         log_soft = shift_of(log_soft), log_hard = shift_of(log_hard);
         float kl = 0.f;
-        if (k.soft) {
-            for (int j = tid; j < k.top; j += kThreads) {
+        if (k.soft && (GRAD || rank == 0)) {
+            for (int j = tid; j < k.top; j += threads) {
                 const float lp = (p[j] - shift_of(top_t)) * k.inverse - log_sum;
                 const float pj = taught && col[j] >= 0 ? expf(lp) : 0.f;
                 p[j] = pj;
                 if (pj != 0.f) kl += pj * (lp - ((zk[j] - at) * k.inverse - log_soft));
             }
-            kl = block_reduce(kl, part, add, 0.f);
+            if (rank == 0 && k.losses != nullptr) kl = block_reduce(kl, part, [](float a, float b) { return a + b; }, 0.f);
         }
-        if (tid == 0 && k.losses != nullptr) {
+        if (rank == 0 && tid == 0 && k.losses != nullptr) {
             float loss = 0.f;
             if (taught) loss += (1.f - k.hard_weight) * k.temperature * k.temperature * kl;
             if (k.hard && col[k.top] >= 0) loss += k.hard_weight * (log_hard - (zk[k.top] - at));
@@ -220,53 +385,346 @@ distill_kernel(const Args k) {
     }
 
     if constexpr (GRAD) {
-        __syncthreads();  // (p, zk and col of the other threads; and z is written from here on where the gradient lies on it)
-        T* const g = reinterpret_cast<T*>(row_at(k.grad, k.inner, r));
+        // The other threads' p, zk and col; and where the gradient lies on the logits, the other blocks' reading of them.
+        __syncthreads();
+        if (FORWARD && k.blocks > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         const float w = k.grad_scale * (k.weights.base != nullptr ? *reinterpret_cast<const float*>(row_at(k.weights, k.inner, r)) : 1.f);
-        const bool hard_there = k.hard && col[k.top] >= 0;
-        const float ws = taught ? w * (1.f - k.hard_weight) * k.temperature : 0.f;
-        const float wh = hard_there ? w * k.hard_weight : 0.f;
-        const float soft2 = log_soft * kLog2e, hard2 = log_hard * kLog2e;
-        auto value = [&](float x) {
-            float y = 0.f;
-            if (ws != 0.f) y += ws * fast_exp2(fmaf(x - at, c_soft, -soft2));
-            if (wh != 0.f) y += wh * fast_exp2(fmaf(x - at, kLog2e, -hard2));
-            return y;
-        };
-        for (int64_t i = tid; i < head; i += kThreads) g[i] = from_float<T>(value(to_float(z[i])));
-        for (int64_t i = tail + tid; i < k.vocab; i += kThreads) g[i] = from_float<T>(value(to_float(z[i])));
-        const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
-        if ((reinterpret_cast<uintptr_t>(g + head) & 15) == 0) {
-#pragma unroll 4
-            for (int64_t i = tid; i < vectors; i += kThreads) {
-                float x[E];
-                unpack<T>(zv[i], x);
+        const bool labelled = k.hard && col[k.top] >= 0;
+        RowGrad row;
+        row.ws = taught ? w * (1.f - k.hard_weight) * k.temperature : 0.f;
+        row.wh = labelled ? w * k.hard_weight : 0.f;
+        row.at = at, row.soft2 = -log_soft * kLog2e, row.hard2 = -log_hard * kLog2e;
+        if (end >= 0) g[end] = from_float<T>(grad_value(row, c_soft, end_z));
+        const bool aligned = (reinterpret_cast<uintptr_t>(g + head) & 15) == 0;
+        const bool again = v1 - v0 > int64_t(kVectors) * threads && FORWARD;  // not held any more
+        for (int64_t from = v0; from < v1; from += kVectors * threads) {
+            if (again || from != v0) load(from);
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = value(x[e]);
-                reinterpret_cast<uint4*>(g + head)[i] = pack<T>(x);
+            for (int i = 0; i < kVectors; ++i) {
+                const int64_t v = from + i * threads + tid;
+                if (v >= v1) break;
+                grad_vector<T>(row, c_soft, raw[i], g + head + v * E, aligned);
             }
-        } else {
-            for (int64_t i = head + tid; i < tail; i += kThreads) g[i] = from_float<T>(value(to_float(z[i])));
         }
         __syncthreads();
-        // the columns that p or the label adds to, each by the first entry that names it
-        for (int j = tid; j <= k.top; j += kThreads) {
-            const int c = j < k.top && !k.soft ? -1 : col[j];
-            if (c < 0) continue;
-            bool first = true;
-            float minus = 0.f;
+        // the columns of this block that p or the label adds to, each by the first entry that names it
+        const int64_t c0 = rank == 0 ? 0 : head + v0 * E, c1 = rank + 1 == k.blocks ? k.vocab : head + v1 * E;
+        for (int j = tid; j <= k.top; j += threads) {
+            const int c = col[j];
+            float minus;
+            if (c < 0 || c < c0 || c >= c1 || !entry_takes(row, col, p, k.top, k.soft, j, minus)) continue;
+            g[c] = from_float<T>(grad_value(row, c_soft, zk[j]) - minus);
+        }
+    } else {
+        if (FORWARD && k.blocks > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // (no block leaves before its part is read)
+    }
+}
+
+// ---- many rows ----------------------------------------------------------------
+
+// Two blocks to an SM take one row after another each, so that one computes while the other meets.  kRowWarps warps work on the logits, which come through shared memory: each thread copies its own vectors
+// (cp.async, 16 bytes) some visits ahead, and copies the next one into a place as soon as it has used what lay there, so that the memory is never idle.
+// A visit is a chunk of a row, or, where the losses and the gradient are computed at once and the row fits, the whole row, which then stays until its
+// gradient is written.  Two more warps do what the teacher and the label ask for, one the even and one the odd rows, up to two rows ahead: ids, the
+// logits at them, softmax, the loss once the row's sums are there, and the columns written again once the gradient is.  They meet by named barriers
+// at which neither side waits for what it does not need: told (the teacher's part of row i is there), summed (the warps' sums are) and written.
+// (A block or a cluster to each row waited for ids, logits, sums and its successor's start one after another: 4096 x 32000 took 157 us and 189 us.)
+constexpr int kRowWarps = 8, kRowThreads = kRowWarps * 32, kTeachers = 2, kRowBlocks = 2;
+constexpr int kRowShared = 112 << 10;  // of a block: the ring and the teachers' arrays
+
+template <int ID>
+__device__ __forceinline__ void barrier_sync(int parity, int threads) {
+    asm volatile("barrier.sync %0, %1;" ::"r"(ID + parity), "r"(threads) : "memory");
+}
+template <int ID>
+__device__ __forceinline__ void barrier_arrive(int parity, int threads) {
+    asm volatile("barrier.arrive %0, %1;" ::"r"(ID + parity), "r"(threads) : "memory");
+}
+constexpr int kRowBarrier = 1, kTold = 2, kSummed = 4, kWritten = 6;
+constexpr int kMeeting = kRowThreads + 32;
+
+struct TeacherRow {
+    RowGrad grad;  // (forward: at, soft2 and hard2 are not known yet)
+    float top_t, log_sum;
+    bool taught;
+};
+
+struct RingArgs {
+    int chunk;   // vectors of a thread in a visit
+    int slots;   // visits in shared memory: 1 to 3
+    int chunks;  // of a row
+    bool held;   // the row stays for its gradient: one chunk
+};
+
+__device__ __forceinline__ void copy_vector(uint32_t to, const uint4* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(__cvta_generic_to_global(from)) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest slots - 1 groups of this thread's copies are there.
+__device__ __forceinline__ void copies_wait(int slots) {
+    if (slots == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (slots == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T, bool FORWARD, bool GRAD>
+__global__ void __launch_bounds__(kRowThreads + kTeachers * 32, kRowBlocks)
+distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
+    constexpr int E = 16 / sizeof(T);
+    extern __shared__ __align__(16) char shared[];
+    uint4* const held = reinterpret_cast<uint4*>(shared);  // [slots][chunk][kRowThreads]
+    int* const entries = reinterpret_cast<int*>(held + ring.slots * ring.chunk * kRowThreads);
+    __shared__ Part parts[kTeachers][kRowWarps];
+    __shared__ TeacherRow told[kTeachers];
+    pdl_prologue();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const uint32_t n = (rows - blockIdx.x + gridDim.x - 1) / gridDim.x;  // rows of this block: blockIdx.x + i * gridDim.x
+    const float c_soft = k.inverse * kLog2e;
+    auto logits_of = [&](uint32_t i) { return reinterpret_cast<const T*>(row_at(k.logits, k.inner, blockIdx.x + i * gridDim.x)); };
+    auto grad_of = [&](uint32_t i) { return reinterpret_cast<T*>(row_at(k.grad, k.inner, blockIdx.x + i * gridDim.x)); };
+
+    if (warp >= kRowWarps) {
+        const int parity = warp - kRowWarps;
+        int* const col = entries + parity * entry_words(k.top);
+        float* const p = reinterpret_cast<float*>(col + (k.top / 4 + 1) * 4);
+        float* const zk = p + (k.top + 3) / 4 * 4;
+        if (!k.soft) {
+            for (int j = lane; j < k.top; j += 32) col[j] = -1;
+        }
+        if (lane > 0 && lane < 4 && k.top + lane < (k.top / 4 + 1) * 4) col[k.top + lane] = -1;
+        for (uint32_t i = parity; i < n; i += kTeachers) {
+            const uint32_t r = blockIdx.x + i * gridDim.x;
+            const T* const z = logits_of(i);
+            float top_t = -INFINITY, sum = 0.f;
             if (k.soft) {
-                for (int i = 0; i < k.top; ++i) {
-                    if (col[i] != c) continue;
-                    if (i < j) first = false;
-                    if (ws != 0.f) minus += ws * p[i];
+                const char* ids = row_at(k.ids, k.inner, r);
+                const char* t = row_at(k.teacher, k.inner, r);
+#pragma unroll 4
+                for (int j = lane; j < k.top; j += 32) {
+                    const int64_t id = load_index(ids + int64_t(j) * (k.wide_ids ? 8 : 4), k.wide_ids);
+                    const bool in = id >= 0 && id < k.vocab;
+                    if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
+                    const float tj = in ? (k.half_teacher ? __half2float(reinterpret_cast<const __half*>(t)[j]) : reinterpret_cast<const float*>(t)[j]) : -INFINITY;
+                    col[j] = in ? static_cast<int>(id) : -1;
+                    p[j] = tj;
+                    zk[j] = in ? to_float(z[id]) : 0.f;
+                    top_t = fmaxf(top_t, tj);
+                }
+#pragma unroll
+                for (int d = 16; d > 0; d /= 2) top_t = fmaxf(top_t, __shfl_xor_sync(0xffffffffu, top_t, d));
+                for (int j = lane; j < k.top; j += 32) sum += col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse) : 0.f;
+#pragma unroll
+                for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            }
+            const bool taught = k.soft && !(sum == 0.f);
+            const float log_sum = logf(sum);
+            int label = -1;
+            float label_z = 0.f;
+            if (k.hard) {
+                const int64_t id = load_index(row_at(k.labels, k.inner, r), k.wide_labels);
+                if (id >= k.vocab && lane == 0) atomicOr(k.status, kStatusIndexOutOfRange);
+                if (id >= 0 && id < k.vocab) {
+                    label = static_cast<int>(id);
+                    label_z = to_float(z[id]);
                 }
             }
-            if (!first) continue;
-            if (col[k.top] == c) minus += wh;
-            g[c] = from_float<T>(value(zk[j]) - minus);
+            if (lane == 0) col[k.top] = label, zk[k.top] = label_z;
+            RowGrad row = {};
+            if constexpr (GRAD) {
+                const float w = k.grad_scale * (k.weights.base != nullptr ? *reinterpret_cast<const float*>(row_at(k.weights, k.inner, r)) : 1.f);
+                row.ws = taught ? w * (1.f - k.hard_weight) * k.temperature : 0.f;
+                row.wh = label >= 0 ? w * k.hard_weight : 0.f;
+            }
+            if constexpr (!FORWARD) {
+                const float4 s = k.stats[r];
+                row.at = shift_of(s.x), row.soft2 = -shift_of(s.y) * kLog2e, row.hard2 = -shift_of(s.z) * kLog2e;
+            }
+            if (lane == 0) told[parity].grad = row;
+            __syncwarp();
+            barrier_arrive<kTold>(parity, kMeeting);
+            if constexpr (FORWARD) {
+                barrier_sync<kSummed>(parity, kMeeting);
+                Part run = lane < kRowWarps ? parts[parity][lane] : Part{-INFINITY, 0.f, 0.f};
+                run = warp_part(run, c_soft, k.soft, k.hard);
+                const float at = shift_of(run.top);
+                float log_soft = k.soft ? logf(run.soft) : 0.f, log_hard = k.hard ? logf(run.hard) : 0.f;
+                if (lane == 0 && k.stats != nullptr) k.stats[r] = make_float4(run.top, log_soft, log_hard, 0.f);
+                log_soft = shift_of(log_soft), log_hard = shift_of(log_hard);
+                row.at = at, row.soft2 = -log_soft * kLog2e, row.hard2 = -log_hard * kLog2e;
+                float kl = 0.f;
+                for (int j = lane; j < k.top && k.soft; j += 32) {
+                    const float lp = (p[j] - shift_of(top_t)) * k.inverse - log_sum;
+                    const float pj = taught && col[j] >= 0 ? expf(lp) : 0.f;
+                    p[j] = pj;
+                    if (pj != 0.f) kl += pj * (lp - ((zk[j] - at) * k.inverse - log_soft));
+                }
+#pragma unroll
+                for (int d = 16; d > 0; d /= 2) kl += __shfl_xor_sync(0xffffffffu, kl, d);
+                if (lane == 0 && k.losses != nullptr) {
+                    float loss = 0.f;
+                    if (taught) loss += (1.f - k.hard_weight) * k.temperature * k.temperature * kl;
+                    if (label >= 0) loss += k.hard_weight * (log_hard - (label_z - at));
+                    k.losses[r] = loss;
+                }
+            } else {
+                for (int j = lane; j < k.top && k.soft; j += 32) p[j] = taught && col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse - log_sum) : 0.f;
+            }
+            __syncwarp();
+            if constexpr (GRAD) {
+                barrier_sync<kWritten>(parity, kMeeting);
+                T* const g = grad_of(i);
+                for (int j = lane; j <= k.top; j += 32) {
+                    float minus;
+                    if (col[j] < 0 || !entry_takes(row, col, p, k.top, k.soft, j, minus)) continue;
+                    g[col[j]] = from_float<T>(grad_value(row, c_soft, zk[j]) - minus);
+                }
+                __syncwarp();
+            }
         }
+        return;
     }
+
+    // the rows' warps
+    const int tid = threadIdx.x;
+    const bool reread = GRAD && !(FORWARD && ring.held);               // the gradient has visits of its own
+    const uint32_t visits = ((FORWARD ? 1u : 0u) + (reread ? 1u : 0u)) * ring.chunks;  // of a row
+    const uint32_t my_place = static_cast<uint32_t>(__cvta_generic_to_shared(held)) + tid * 16;
+    // The visit whose copies are issued next: row, chunk within a sweep, sweep; its vectors from `source` on, `limit` of them for this thread.
+    uint32_t next_row = 0, next_visit = 0;
+    const uint4* source = nullptr;
+    int limit = 0;
+    // how many of `vectors` from place `first` on, kRowThreads apart, belong to a visit
+    auto count_of = [&](int64_t vectors, int64_t first) {
+        return static_cast<int>(max(int64_t(0), min(int64_t(ring.chunk), (vectors - first + kRowThreads - 1) / kRowThreads)));
+    };
+    auto aim = [&] {
+        limit = 0;
+        if (next_row >= n) return;
+        const T* const z = logits_of(next_row);
+        const int64_t head = head_of(z, k.vocab), first = int64_t(next_visit % ring.chunks) * ring.chunk * kRowThreads + tid;
+        source = reinterpret_cast<const uint4*>(z + head) + first;
+        limit = count_of((k.vocab - head) / E, first);
+        if (++next_visit == visits) next_visit = 0, ++next_row;
+    };
+    int slot = 0, next_slot = 0;
+    constexpr uint32_t kApart = kRowThreads * 16;  // bytes from a thread's vector to its next
+    auto place = [&](int s, int v) { return my_place + static_cast<uint32_t>(s * ring.chunk + v) * kApart; };
+    // kVectors copies of the next visit, from its vector v on
+    auto copy = [&](int v) {
+        const uint32_t to = place(next_slot, v);
+        const uint4* const from = source + int64_t(v) * kRowThreads;
+        if (v + kVectors <= limit) {
+#pragma unroll
+            for (int h = 0; h < kVectors; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
+        } else {
+            for (int h = 0; v + h < limit; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
+        }
+    };
+    for (int s = 0; s < ring.slots; ++s) {
+        next_slot = s;
+        aim();
+        for (int v = 0; v < ring.chunk; v += kVectors) copy(v);
+        copies_commit();
+    }
+    // an element of a row's ends for some threads: behind the last vector for those from 8 on
+    auto end_of = [&](const T* z) {
+        const int64_t head = head_of(z, k.vocab), tail = head + (k.vocab - head) / E * E;
+        return tid < head ? int64_t(tid) : tid >= 8 && tail + (tid - 8) < k.vocab ? tail + (tid - 8) : int64_t(-1);
+    };
+    int64_t end = end_of(logits_of(0));
+    float end_z = end >= 0 ? to_float(logits_of(0)[end]) : -INFINITY;
+    uint4 raw[kVectors];
+    for (uint32_t i = 0; i < n; ++i) {
+        const int parity = i % kTeachers;
+        const T* const z = logits_of(i);
+        const int64_t head = head_of(z, k.vocab), all_vectors = (k.vocab - head) / E;
+        int64_t next_end = -1;
+        float next_end_z = -INFINITY;
+        if (i + 1 < n) {
+            const T* const after = logits_of(i + 1);
+            next_end = end_of(after);
+            if (next_end >= 0) next_end_z = to_float(after[next_end]);
+        }
+        // kVectors of a visit's vectors from v on; `count`: how many there are in the visit for this thread
+        auto fetch = [&](int v, int count) {
+            const uint32_t from = place(slot, v);
+            auto get = [&](uint4& x, uint32_t at) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory"); };
+            if (v + kVectors <= count) {
+#pragma unroll
+                for (int h = 0; h < kVectors; ++h) get(raw[h], from + h * kApart);
+            } else {
+#pragma unroll
+                for (int h = 0; h < kVectors; ++h) {
+                    raw[h] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+                    if (v + h < count) get(raw[h], from + h * kApart);
+                }
+            }
+        };
+        auto done = [&] {
+            copies_commit();
+            slot = slot + 1 == ring.slots ? 0 : slot + 1;
+        };
+        if constexpr (FORWARD) {
+            const float one = end_z == -INFINITY ? 0.f : 1.f + (end_z - end_z);
+            Part run = {end_z, one, one};
+            const bool keep = GRAD && ring.held;
+            for (int c = 0; c < ring.chunks; ++c) {
+                copies_wait(ring.slots);
+                const int count = count_of(all_vectors, int64_t(c) * ring.chunk * kRowThreads + tid);
+                if (!keep) {
+                    aim();
+                    next_slot = slot;
+                }
+                for (int v = 0; v < ring.chunk; v += kVectors) {
+                    fetch(v, count);
+                    take_vectors<T>(run, raw, c_soft, k.soft, k.hard);
+                    if (!keep) copy(v);
+                }
+                if (!keep) done();
+            }
+            run = warp_part(run, c_soft, k.soft, k.hard);
+            barrier_sync<kTold>(parity, kMeeting);  // (so the teacher is done with the sums of two rows ago, too)
+            if (lane == 0) parts[parity][warp] = run;
+            __syncwarp();
+            if constexpr (GRAD) barrier_sync<kRowBarrier>(0, kRowThreads);
+            barrier_arrive<kSummed>(parity, kMeeting);
+        } else {
+            barrier_sync<kTold>(parity, kMeeting);
+        }
+        if constexpr (GRAD) {
+            RowGrad row = told[parity].grad;
+            if constexpr (FORWARD) {
+                Part run = lane < kRowWarps ? parts[parity][lane] : Part{-INFINITY, 0.f, 0.f};
+                run = warp_part(run, c_soft, k.soft, k.hard);
+                row.at = shift_of(run.top);
+                row.soft2 = k.soft ? -shift_of(logf(run.soft)) * kLog2e : 0.f;
+                row.hard2 = k.hard ? -shift_of(logf(run.hard)) * kLog2e : 0.f;
+            }
+            T* const g = grad_of(i);
+            const bool aligned = (reinterpret_cast<uintptr_t>(g + head) & 15) == 0;
+            if (end >= 0) g[end] = from_float<T>(grad_value(row, c_soft, end_z));
+            for (int c = 0; c < ring.chunks; ++c) {
+                if (reread) copies_wait(ring.slots);
+                const int count = count_of(all_vectors, int64_t(c) * ring.chunk * kRowThreads + tid);
+                aim();
+                next_slot = slot;
+                for (int v = 0; v < ring.chunk; v += kVectors) {
+                    fetch(v, count);
+                    T* const to = g + head + ((int64_t(c) * ring.chunk + v) * kRowThreads + tid) * E;
+#pragma unroll
+                    for (int h = 0; h < kVectors; ++h) {
+                        if (v + h >= count) break;
+                        grad_vector<T>(row, c_soft, raw[h], to + h * kRowThreads * E, aligned);
+                    }
+                    copy(v);  // (the places have been read: their values are used)
+                }
+                done();
+            }
+            __syncwarp();
+            barrier_arrive<kWritten>(parity, kMeeting);
+        }
+        end = next_end;
+        end_z = next_end_z;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- arguments --------------------------------------------------------------
@@ -344,7 +802,10 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
 
 void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
     const Plan plan = check_distill(a, forward);
-    const auto& [axes, vocab, top, s, labelled] = plan;
+    const int axes = plan.axes;
+    const int64_t vocab = plan.vocab, top = plan.top;
+    const RowShape s = plan.s;
+    const bool labelled = plan.labelled;
     if (s.rows == 0) return;
     wait_for_tensors(ctx, {&a.logits, &a.teacher_ids, &a.teacher_logits, &a.labels, &a.losses, &a.stats, &a.losses_grad, &a.grad});
     Args k{};
@@ -370,10 +831,46 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
     k.hard_weight = a.hard_weight;
     k.grad_scale = a.grad_scale;
     ProfScope scope(ctx, forward ? "distill_loss" : "distill_loss_backward");
-    const size_t shared = (3 * static_cast<size_t>(top) + 2) * 4;
-    const unsigned blocks = static_cast<unsigned>(s.rows);
-    auto go = [&](auto kernel) { launch_kernel(ctx, kernel, blocks, kThreads, shared, k); };
+    const size_t shared = static_cast<size_t>(entry_words(static_cast<int>(top))) * 4;
     const bool half = a.logits.dtype == B200_F16;
+    // Many rows of at least 16 KB each: blocks that stay take one row after another.  (Below, a block's warps have little to do between a row's meetings.)
+    const int64_t row_vectors = ceil_div(vocab, half ? 8 : 4);
+    if (s.rows >= int64_t(sm_count()) * kRowBlocks && row_vectors >= kRowThreads * 4) {
+        RingArgs ring{};
+        const int64_t whole = ceil_div(ceil_div(row_vectors, kRowThreads), kVectors) * kVectors;
+        const int most = static_cast<int>((kRowShared - kTeachers * shared) / (kRowThreads * 16));  // vectors of a thread
+        ring.held = forward && present(a.grad) && whole <= most;
+        ring.chunk = ring.held ? static_cast<int>(whole) : kVectors;
+        ring.slots = std::min(3, most / ring.chunk);
+        ring.chunks = static_cast<int>(ceil_div(whole, ring.chunk));
+        const size_t bytes = static_cast<size_t>(ring.slots) * ring.chunk * kRowThreads * 16 + kTeachers * shared;
+        auto go = [&](auto kernel) {
+            (void)blocks_at_once(reinterpret_cast<const void*>(kernel), kRowThreads + kTeachers * 32, bytes);  // (allows that much shared memory)
+            launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(sm_count() * kRowBlocks)), dim3(kRowThreads + kTeachers * 32), bytes, k, ring, static_cast<uint32_t>(s.rows));
+        };
+        if (!forward) go(half ? distill_rows_kernel<__half, false, true> : distill_rows_kernel<float, false, true>);
+        else if (present(a.grad)) go(half ? distill_rows_kernel<__half, true, true> : distill_rows_kernel<float, true, true>);
+        else go(half ? distill_rows_kernel<__half, true, false> : distill_rows_kernel<float, true, false>);
+        check_last_launch("distill_loss");
+        ctx->count_launch();
+        return;
+    }
+    // 256 threads and a cluster of up to 4, so that an SM has four blocks in different states; longer rows 512 threads and a cluster of up to 8.  Where there
+    // are fewer rows than SMs, a cluster as large as leaves a thread a vector.
+    const int64_t vectors = row_vectors;
+    int threads = 256, blocks = 1;
+    while (blocks < 4 && vectors > int64_t(blocks) * threads * kVectors) blocks *= 2;
+    if (vectors > int64_t(blocks) * threads * kVectors) threads = kMostThreads;
+    while (blocks < 8 && vectors > int64_t(blocks) * threads * kVectors) blocks *= 2;
+    while (blocks < 8 && s.rows * blocks * 2 <= sm_count() && vectors > int64_t(blocks) * threads) blocks *= 2;
+    while (threads > 64 && s.rows * blocks > sm_count() && int64_t(blocks) * (threads / 2) * 4 >= vectors) threads /= 2;
+    k.blocks = blocks;
+    const int64_t grid = s.rows * blocks;
+    if (grid >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "distill_loss: too many rows of this length");
+    auto go = [&](auto kernel) {
+        if (blocks == 1 || !forward) launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, k);
+        else launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, blocks, true, k);
+    };
     if (!forward) go(half ? distill_kernel<__half, false, true> : distill_kernel<float, false, true>);
     else if (present(a.grad)) go(half ? distill_kernel<__half, true, true> : distill_kernel<float, true, true>);
     else go(half ? distill_kernel<__half, true, false> : distill_kernel<float, true, false>);
