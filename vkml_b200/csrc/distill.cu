@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace b200 {
 namespace {
@@ -96,6 +97,7 @@ __device__ __forceinline__ int64_t head_of(const T* row, int64_t n) {
 template <typename T>
 constexpr uint32_t kNothing = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u;  // -inf
 
+// The elements of a vector.  (Plain arithmetic on them: pairs in 64-bit registers, two to an instruction, cost more moves than they saved here.)
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& raw, float (&x)[16 / sizeof(T)]) {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -112,110 +114,174 @@ __device__ __forceinline__ void unpack(const uint4& raw, float (&x)[16 / sizeof(
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 pack(const float (&x)[16 / sizeof(T)]) {
-    uint32_t w[4];
+__device__ __forceinline__ void store_vector(T* to, const float (&x)[16 / sizeof(T)], bool aligned) {
+    if (aligned) {
+        uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2) {
-            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-            w[i] = __float_as_uint(x[i]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                w[i] = __float_as_uint(x[i]);
+            }
         }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// The largest element of a vector (halves compare as halves, two at a time).
-template <typename T>
-__device__ __forceinline__ float largest(const uint4& raw) {
-    if constexpr (sizeof(T) == 2) {
-        const __half2* h = reinterpret_cast<const __half2*>(&raw);
-        const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-        return fmaxf(__low2float(m), __high2float(m));
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-        return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+#pragma unroll
+        for (int e = 0; e < 16 / int(sizeof(T)); ++e) to[e] = from_float<T>(x[e]);
     }
 }
 
-// Adds the elements of kVectors vectors to a part of a row.
-template <typename T>
-__device__ __forceinline__ void take_vectors(Part& run, const uint4 (&raw)[kVectors], float c_soft, bool with_soft, bool with_hard) {
-    constexpr int E = 16 / sizeof(T);
-    float top = run.top;
+// The largest element of NV vectors (halves compare as halves, two at a time).
+template <typename T, int NV>
+__device__ __forceinline__ float largest(const uint4 (&raw)[NV]) {
+    if constexpr (sizeof(T) == 2) {
+        const __half2* h = reinterpret_cast<const __half2*>(&raw[0]);
+        __half2 m[2] = {__hmax2(h[0], h[1]), __hmax2(h[2], h[3])};
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) top = fmaxf(top, largest<T>(raw[i]));
-    const float shift = shift_of(top);
-    if (top > run.top) {
-        run.soft *= fast_exp2((run.top - shift) * c_soft);
-        run.hard *= fast_exp2((run.top - shift) * kLog2e);
-        run.top = top;
-    }
-    float2 soft = {}, hard = {};
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-        float x[E], y[E];
-        unpack<T>(raw[i], x);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) add_pair(x[e], x[e + 1], x[e], x[e + 1], -shift, -shift);
-        if (with_soft) {
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                mul_pair(y[e], y[e + 1], x[e], x[e + 1], c_soft, c_soft);
-                add_pair(soft.x, soft.y, soft.x, soft.y, fast_exp2(y[e]), fast_exp2(y[e + 1]));
-            }
+        for (int i = 1; i < NV; ++i) {
+            const __half2* g = reinterpret_cast<const __half2*>(&raw[i]);
+            m[0] = __hmax2(m[0], __hmax2(g[0], g[1]));
+            m[1] = __hmax2(m[1], __hmax2(g[2], g[3]));
         }
-        if (with_hard) {
+        m[0] = __hmax2(m[0], m[1]);
+        return fmaxf(__low2float(m[0]), __high2float(m[0]));
+    } else {
+        float m = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                mul_pair(y[e], y[e + 1], x[e], x[e + 1], kLog2e, kLog2e);
-                add_pair(hard.x, hard.y, hard.x, hard.y, fast_exp2(y[e]), fast_exp2(y[e + 1]));
-            }
+        for (int i = 0; i < NV; ++i) {
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y)), fmaxf(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w))));
         }
+        return m;
     }
-    run.soft += soft.x + soft.y;
-    run.hard += hard.x + hard.y;
 }
+
+// Powers of two of (x - at) * c + plus as one multiply-add each, x * c + offset, where at * c is of a size that leaves the offset its digits: what its rounding
+// took away is given back by the factor.  Where it is not (logits of the type's lowest value), the difference comes first.
+struct Exponent {
+    float c, at, offset, factor;
+    bool direct;
+};
+__device__ __forceinline__ Exponent exponent_of(float at, float c, float plus) {
+    Exponent x;
+    const float p = at * c;
+    x.c = c, x.at = at;
+    x.direct = fabsf(p) < 4096.f;
+    x.offset = x.direct ? plus - p : plus;
+    x.factor = 1.f;
+    if (x.direct) {  // plus - at c, without the offset that stands for it: the difference's rounding and the product's
+        const float b = plus - x.offset, a = x.offset + b;
+        const float lost = ((plus - a) + (b - p)) - fmaf(at, c, -p);
+        x.factor = fmaf(lost, 0.6931471805599453f, 1.f);
+    }
+    return x;
+}
+// Without the factor.
+template <bool DIRECT>
+__device__ __forceinline__ float power(const Exponent& x, float z) {
+    if constexpr (!DIRECT) z -= x.at;
+    return fast_exp2(fmaf(z, x.c, x.offset));
+}
+
+// Adds the elements of NV vectors to a part of a row.
+template <typename T, bool DIRECT, int NV>
+__device__ __forceinline__ float sum_powers(const Exponent& x, const uint4 (&raw)[NV]) {
+    constexpr int E = 16 / sizeof(T);
+    float sum[4] = {};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float z[E];
+        unpack<T>(raw[i], z);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e % 4] += power<DIRECT>(x, z[e]);
+    }
+    return ((sum[0] + sum[1]) + (sum[2] + sum[3])) * x.factor;
+}
+// A part of a row while its vectors come by: the maximum so far, the sums beside it, and what they are computed by.
+struct Running {
+    Part part;
+    Exponent soft, hard;
+    float c_soft;
+    bool with_soft, with_hard;
+
+    __device__ __forceinline__ void begin(float z, float c, bool use_soft, bool use_hard) {  // with one element, or -inf for none
+        const float one = z == -INFINITY ? 0.f : 1.f + (z - z);  // (not a number where z is none or +inf, as it is in a vector)
+        part = Part{z, one, one};
+        c_soft = c, with_soft = use_soft, with_hard = use_hard;
+        aim();
+    }
+    __device__ __forceinline__ void aim() {
+        soft = exponent_of(shift_of(part.top), c_soft, 0.f);
+        hard = exponent_of(shift_of(part.top), kLog2e, 0.f);
+    }
+    template <typename T, int NV>
+    __device__ __forceinline__ void take(const uint4 (&raw)[NV]) {
+        const float top = largest<T, NV>(raw);
+        if (top > part.top) {
+            part.soft *= fast_exp2((part.top - top) * c_soft);
+            part.hard *= fast_exp2((part.top - top) * kLog2e);
+            part.top = top;
+            aim();
+        }
+        if (with_soft) part.soft += soft.direct ? sum_powers<T, true>(soft, raw) : sum_powers<T, false>(soft, raw);
+        if (with_hard) part.hard += hard.direct ? sum_powers<T, true>(hard, raw) : sum_powers<T, false>(hard, raw);
+    }
+};
 
 // What a row's gradient is made of: ws q + wh h, q = exp2((z - at) c_soft + soft2), h = exp2((z - at) log2 e + hard2).
 struct RowGrad {
     float ws, wh, at, soft2, hard2;
 };
-__device__ __forceinline__ float grad_value(const RowGrad& g, float c_soft, float x) {
+struct GradPowers {
+    Exponent soft, hard;
+    float ws, wh;  // the exponents' factors included
+};
+__device__ __forceinline__ GradPowers grad_powers(const RowGrad& g, float c_soft) {
+    GradPowers x;
+    x.soft = exponent_of(g.at, c_soft, g.soft2);
+    x.hard = exponent_of(g.at, kLog2e, g.hard2);
+    x.ws = g.ws != 0.f ? g.ws * x.soft.factor : 0.f;  // (a row that does not count may hold anything)
+    x.wh = g.wh != 0.f ? g.wh * x.hard.factor : 0.f;
+    return x;
+}
+__device__ __forceinline__ float grad_value(const RowGrad& g, float c_soft, float z) {
+    const GradPowers x = grad_powers(g, c_soft);
     float y = 0.f;
-    if (g.ws != 0.f) y += g.ws * fast_exp2(fmaf(x - g.at, c_soft, g.soft2));
-    if (g.wh != 0.f) y += g.wh * fast_exp2(fmaf(x - g.at, kLog2e, g.hard2));
+    if (g.ws != 0.f) y += x.ws * (x.soft.direct ? power<true>(x.soft, z) : power<false>(x.soft, z));
+    if (g.wh != 0.f) y += x.wh * (x.hard.direct ? power<true>(x.hard, z) : power<false>(x.hard, z));
     return y;
 }
-template <typename T>
-__device__ __forceinline__ void grad_vector(const RowGrad& g, float c_soft, const uint4& raw, T* to, bool aligned) {
+template <typename T, bool DIRECT, int NV>
+__device__ __forceinline__ void grad_vectors(const GradPowers& g, const uint4 (&raw)[NV], T* to, int apart_by, int count, bool aligned) {
     constexpr int E = 16 / sizeof(T);
-    float x[E], y[E];
-    unpack<T>(raw, x);
 #pragma unroll
-    for (int e = 0; e < E; e += 2) add_pair(x[e], x[e + 1], x[e], x[e + 1], -g.at, -g.at);
+    for (int i = 0; i < NV; ++i) {
+        if (i >= count) break;
+        float z[E], y[E];
+        unpack<T>(raw[i], z);
+        if (g.ws != 0.f) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = 0.f;
-    if (g.ws != 0.f) {
+            for (int e = 0; e < E; ++e) y[e] = power<DIRECT>(g.soft, z[e]) * g.ws;
+            if (g.wh != 0.f) {
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            fma_pair(y[e], y[e + 1], x[e], x[e + 1], c_soft, c_soft, g.soft2, g.soft2);
-            mul_pair(y[e], y[e + 1], fast_exp2(y[e]), fast_exp2(y[e + 1]), g.ws, g.ws);
+                for (int e = 0; e < E; ++e) y[e] = fmaf(power<DIRECT>(g.hard, z[e]), g.wh, y[e]);
+            }
+        } else if (g.wh != 0.f) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = power<DIRECT>(g.hard, z[e]) * g.wh;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = 0.f;
         }
+        store_vector<T>(to + i * apart_by, y, aligned);
     }
-    if (g.wh != 0.f) {
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            fma_pair(x[e], x[e + 1], x[e], x[e + 1], kLog2e, kLog2e, g.hard2, g.hard2);
-            fma_pair(y[e], y[e + 1], fast_exp2(x[e]), fast_exp2(x[e + 1]), g.wh, g.wh, y[e], y[e + 1]);
-        }
-    }
-    if (aligned) {
-        *reinterpret_cast<uint4*>(to) = pack<T>(y);
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) to[e] = from_float<T>(y[e]);
-    }
+}
+// The gradient in `count` vectors of a thread, `apart_by` elements from one to the next.
+template <typename T, int NV>
+__device__ __forceinline__ void put_grad(const GradPowers& g, const uint4 (&raw)[NV], T* to, int apart_by, int count, bool aligned) {
+    if (g.soft.direct && g.hard.direct) grad_vectors<T, true>(g, raw, to, apart_by, count, aligned);
+    else grad_vectors<T, false>(g, raw, to, apart_by, count, aligned);
 }
 
 // What p and the label take off the gradient's column col[j], if entry j is the first that names it.  The columns lie on a 16-byte boundary, `top` + 1 of
@@ -330,15 +396,15 @@ distill_kernel(const Args k) {
     const float c_soft = k.inverse * kLog2e;
     float at = 0.f, log_soft = 0.f, log_hard = 0.f;
     if constexpr (FORWARD) {
-        const float one = end_z == -INFINITY ? 0.f : 1.f + (end_z - end_z);  // (not a number where z is none or +inf, as it is in a vector)
-        Part run = {end_z, one, one};
+        Running running;
+        running.begin(end_z, c_soft, k.soft, k.hard);
         for (int64_t from = v0;;) {
-            take_vectors<T>(run, raw, c_soft, k.soft, k.hard);
+            running.take<T>(raw);
             from += kVectors * threads;
             if (from >= v1) break;
             load(from);
         }
-        run = warp_part(run, c_soft, k.soft, k.hard);
+        Part run = warp_part(running.part, c_soft, k.soft, k.hard);
         if (tid % 32 == 0) parts[tid / 32] = run;
         __syncthreads();
         run = tid % 32 < threads / 32 ? parts[tid % 32] : Part{-INFINITY, 0.f, 0.f};
@@ -397,14 +463,11 @@ distill_kernel(const Args k) {
         if (end >= 0) g[end] = from_float<T>(grad_value(row, c_soft, end_z));
         const bool aligned = (reinterpret_cast<uintptr_t>(g + head) & 15) == 0;
         const bool again = v1 - v0 > int64_t(kVectors) * threads && FORWARD;  // not held any more
+        const GradPowers powers = grad_powers(row, c_soft);
         for (int64_t from = v0; from < v1; from += kVectors * threads) {
             if (again || from != v0) load(from);
-#pragma unroll
-            for (int i = 0; i < kVectors; ++i) {
-                const int64_t v = from + i * threads + tid;
-                if (v >= v1) break;
-                grad_vector<T>(row, c_soft, raw[i], g + head + v * E, aligned);
-            }
+            const int64_t v = from + tid;
+            put_grad<T>(powers, raw, g + head + v * E, threads * E, static_cast<int>(min(int64_t(kVectors), (v1 - v + threads - 1) / threads)), aligned);
         }
         __syncthreads();
         // the columns of this block that p or the label adds to, each by the first entry that names it
@@ -429,7 +492,8 @@ distill_kernel(const Args k) {
 // logits at them, softmax, the loss once the row's sums are there, and the columns written again once the gradient is.  They meet by named barriers
 // at which neither side waits for what it does not need: told (the teacher's part of row i is there), summed (the warps' sums are) and written.
 // (A block or a cluster to each row waited for ids, logits, sums and its successor's start one after another: 4096 x 32000 took 157 us and 189 us.)
-constexpr int kRowWarps = 8, kRowThreads = kRowWarps * 32, kTeachers = 2, kRowBlocks = 2;
+constexpr int kRowWarps = 12, kRowThreads = kRowWarps * 32, kTeachers = 2, kRowBlocks = 2;
+constexpr int kBatch = 4;            // vectors that a thread works on at once
 constexpr int kRowShared = 112 << 10;  // of a block: the ring and the teachers' arrays
 
 template <int ID>
@@ -584,103 +648,119 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
 
     // the rows' warps
     const int tid = threadIdx.x;
-    const bool reread = GRAD && !(FORWARD && ring.held);               // the gradient has visits of its own
-    const uint32_t visits = ((FORWARD ? 1u : 0u) + (reread ? 1u : 0u)) * ring.chunks;  // of a row
-    const uint32_t my_place = static_cast<uint32_t>(__cvta_generic_to_shared(held)) + tid * 16;
-    // The visit whose copies are issued next: row, chunk within a sweep, sweep; its vectors from `source` on, `limit` of them for this thread.
-    uint32_t next_row = 0, next_visit = 0;
-    const uint4* source = nullptr;
-    int limit = 0;
-    // how many of `vectors` from place `first` on, kRowThreads apart, belong to a visit
-    auto count_of = [&](int64_t vectors, int64_t first) {
-        return static_cast<int>(max(int64_t(0), min(int64_t(ring.chunk), (vectors - first + kRowThreads - 1) / kRowThreads)));
+    const int chunks = ring.chunks, chunk = ring.chunk, slots = ring.slots;
+    const bool keep = FORWARD && GRAD && ring.held;               // the row stays
+    const int sweeps = FORWARD && GRAD && !keep ? 2 : 1;          // visits of a chunk of a row
+    constexpr uint32_t kApart = kRowThreads * 16;                 // bytes from a thread's vector to its next
+    const uint32_t my_place = static_cast<uint32_t>(__cvta_generic_to_shared(held)) + tid * 16, slot_bytes = chunk * kApart;
+    // A row: where its vectors begin, how many they are, and the element at its ends that is this thread's (behind the last vector for those from 8 on; -1: none).
+    struct Row {
+        const T* z;
+        int head, vectors;
     };
+    auto row_of = [&](uint32_t i) {
+        Row row;
+        row.z = logits_of(i);
+        row.head = static_cast<int>(head_of(row.z, k.vocab));
+        row.vectors = (static_cast<int>(k.vocab) - row.head) / E;
+        return row;
+    };
+    auto end_of = [&](const Row& row) {
+        const int behind = row.head + row.vectors * E + tid - 8;
+        return tid < row.head ? tid : tid >= 8 && tid < 16 && behind < static_cast<int>(k.vocab) ? behind : -1;
+    };
+    // how many of this thread's vectors of a row lie in the chunk that begins with its vector v
+    auto count_of = [&](int vectors, int v) { return max(0, min(chunk, (vectors - tid + kRowThreads - 1) / kRowThreads - v)); };
+    // the visit whose copies are issued next
+    Row ahead = row_of(0);
+    uint32_t ahead_row = 0;
+    int ahead_chunk = 0, ahead_sweep = 0, limit = 0;
+    const uint4* source = nullptr;
     auto aim = [&] {
         limit = 0;
-        if (next_row >= n) return;
-        const T* const z = logits_of(next_row);
-        const int64_t head = head_of(z, k.vocab), first = int64_t(next_visit % ring.chunks) * ring.chunk * kRowThreads + tid;
-        source = reinterpret_cast<const uint4*>(z + head) + first;
-        limit = count_of((k.vocab - head) / E, first);
-        if (++next_visit == visits) next_visit = 0, ++next_row;
+        if (ahead_row >= n) return;
+        source = reinterpret_cast<const uint4*>(ahead.z + ahead.head) + ahead_chunk * chunk * kRowThreads + tid;
+        limit = count_of(ahead.vectors, ahead_chunk * chunk);
+        if (++ahead_chunk == chunks) {
+            ahead_chunk = 0;
+            if (++ahead_sweep == sweeps) {
+                ahead_sweep = 0;
+                if (++ahead_row < n) ahead = row_of(ahead_row);
+            }
+        }
     };
-    int slot = 0, next_slot = 0;
-    constexpr uint32_t kApart = kRowThreads * 16;  // bytes from a thread's vector to its next
-    auto place = [&](int s, int v) { return my_place + static_cast<uint32_t>(s * ring.chunk + v) * kApart; };
-    // kVectors copies of the next visit, from its vector v on
-    auto copy = [&](int v) {
-        const uint32_t to = place(next_slot, v);
-        const uint4* const from = source + int64_t(v) * kRowThreads;
-        if (v + kVectors <= limit) {
+    uint32_t slot = 0;  // in bytes
+    // `many` copies of the next visit into this one's places, from its vector v on
+    auto copy = [&](int v, auto many) {
+        constexpr int M = decltype(many)::value;
+        const uint32_t to = my_place + slot + v * kApart;
+        const uint4* const from = source + v * kRowThreads;
+        if (v + M <= limit) {
 #pragma unroll
-            for (int h = 0; h < kVectors; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
+            for (int h = 0; h < M; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
         } else {
             for (int h = 0; v + h < limit; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
         }
     };
-    for (int s = 0; s < ring.slots; ++s) {
-        next_slot = s;
-        aim();
-        for (int v = 0; v < ring.chunk; v += kVectors) copy(v);
-        copies_commit();
-    }
-    // an element of a row's ends for some threads: behind the last vector for those from 8 on
-    auto end_of = [&](const T* z) {
-        const int64_t head = head_of(z, k.vocab), tail = head + (k.vocab - head) / E * E;
-        return tid < head ? int64_t(tid) : tid >= 8 && tail + (tid - 8) < k.vocab ? tail + (tid - 8) : int64_t(-1);
+    using Batch = std::integral_constant<int, kBatch>;
+    using One = std::integral_constant<int, 1>;
+    // f of the `count` vectors of a visit, kBatch at a time as far as that goes, and then of the places that hold none: f(vectors, the first one's number, how many)
+    auto each = [&](int count, auto&& f) {
+        auto get = [&](uint4& x, uint32_t at) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory"); };
+        int v = 0;
+        uint32_t from = my_place + slot;
+        for (; v + kBatch <= count; v += kBatch, from += kBatch * kApart) {
+            uint4 raw[kBatch];
+#pragma unroll
+            for (int h = 0; h < kBatch; ++h) get(raw[h], from + h * kApart);
+            f(raw, v, Batch{});
+        }
+        for (; v < count; ++v, from += kApart) {
+            uint4 raw[1];
+            get(raw[0], from);
+            f(raw, v, One{});
+        }
+        return v;
     };
-    int64_t end = end_of(logits_of(0));
-    float end_z = end >= 0 ? to_float(logits_of(0)[end]) : -INFINITY;
-    uint4 raw[kVectors];
+    auto done = [&](int v) {  // with a visit, of which v places have been copied into
+        for (; v < limit; ++v) copy(v, One{});
+        copies_commit();
+        slot = slot + slot_bytes == slots * slot_bytes ? 0 : slot + slot_bytes;
+    };
+    for (int s = 0; s < slots; ++s) {
+        aim();
+        done(0);
+    }
+    Row row = row_of(0);
+    int end = end_of(row);
+    float end_z = end >= 0 ? to_float(row.z[end]) : -INFINITY;
     for (uint32_t i = 0; i < n; ++i) {
         const int parity = i % kTeachers;
-        const T* const z = logits_of(i);
-        const int64_t head = head_of(z, k.vocab), all_vectors = (k.vocab - head) / E;
-        int64_t next_end = -1;
+        Row next_row = row;
+        int next_end = -1;
         float next_end_z = -INFINITY;
         if (i + 1 < n) {
-            const T* const after = logits_of(i + 1);
-            next_end = end_of(after);
-            if (next_end >= 0) next_end_z = to_float(after[next_end]);
+            next_row = row_of(i + 1);
+            next_end = end_of(next_row);
+            if (next_end >= 0) next_end_z = to_float(next_row.z[next_end]);
         }
-        // kVectors of a visit's vectors from v on; `count`: how many there are in the visit for this thread
-        auto fetch = [&](int v, int count) {
-            const uint32_t from = place(slot, v);
-            auto get = [&](uint4& x, uint32_t at) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory"); };
-            if (v + kVectors <= count) {
-#pragma unroll
-                for (int h = 0; h < kVectors; ++h) get(raw[h], from + h * kApart);
-            } else {
-#pragma unroll
-                for (int h = 0; h < kVectors; ++h) {
-                    raw[h] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
-                    if (v + h < count) get(raw[h], from + h * kApart);
-                }
-            }
-        };
-        auto done = [&] {
-            copies_commit();
-            slot = slot + 1 == ring.slots ? 0 : slot + 1;
-        };
         if constexpr (FORWARD) {
-            const float one = end_z == -INFINITY ? 0.f : 1.f + (end_z - end_z);
-            Part run = {end_z, one, one};
-            const bool keep = GRAD && ring.held;
-            for (int c = 0; c < ring.chunks; ++c) {
-                copies_wait(ring.slots);
-                const int count = count_of(all_vectors, int64_t(c) * ring.chunk * kRowThreads + tid);
-                if (!keep) {
+            Running running;
+            running.begin(end_z, c_soft, k.soft, k.hard);
+            for (int c = 0; c < chunks; ++c) {
+                copies_wait(slots);
+                const int count = count_of(row.vectors, c * chunk);
+                if (keep) {
+                    each(count, [&](const auto& raw, int, auto) { running.take<T>(raw); });
+                } else {
                     aim();
-                    next_slot = slot;
+                    done(each(count, [&](const auto& raw, int v, auto many) {
+                        running.take<T>(raw);
+                        copy(v, many);
+                    }));
                 }
-                for (int v = 0; v < ring.chunk; v += kVectors) {
-                    fetch(v, count);
-                    take_vectors<T>(run, raw, c_soft, k.soft, k.hard);
-                    if (!keep) copy(v);
-                }
-                if (!keep) done();
             }
-            run = warp_part(run, c_soft, k.soft, k.hard);
+            Part run = warp_part(running.part, c_soft, k.soft, k.hard);
             barrier_sync<kTold>(parity, kMeeting);  // (so the teacher is done with the sums of two rows ago, too)
             if (lane == 0) parts[parity][warp] = run;
             __syncwarp();
@@ -690,37 +770,31 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
             barrier_sync<kTold>(parity, kMeeting);
         }
         if constexpr (GRAD) {
-            RowGrad row = told[parity].grad;
+            RowGrad grad = told[parity].grad;
             if constexpr (FORWARD) {
                 Part run = lane < kRowWarps ? parts[parity][lane] : Part{-INFINITY, 0.f, 0.f};
                 run = warp_part(run, c_soft, k.soft, k.hard);
-                row.at = shift_of(run.top);
-                row.soft2 = k.soft ? -shift_of(logf(run.soft)) * kLog2e : 0.f;
-                row.hard2 = k.hard ? -shift_of(logf(run.hard)) * kLog2e : 0.f;
+                grad.at = shift_of(run.top);
+                grad.soft2 = k.soft ? -shift_of(logf(run.soft)) * kLog2e : 0.f;
+                grad.hard2 = k.hard ? -shift_of(logf(run.hard)) * kLog2e : 0.f;
             }
+            const GradPowers powers = grad_powers(grad, c_soft);
             T* const g = grad_of(i);
-            const bool aligned = (reinterpret_cast<uintptr_t>(g + head) & 15) == 0;
-            if (end >= 0) g[end] = from_float<T>(grad_value(row, c_soft, end_z));
-            for (int c = 0; c < ring.chunks; ++c) {
-                if (reread) copies_wait(ring.slots);
-                const int count = count_of(all_vectors, int64_t(c) * ring.chunk * kRowThreads + tid);
+            const bool aligned = (reinterpret_cast<uintptr_t>(g + row.head) & 15) == 0;
+            if (end >= 0) g[end] = from_float<T>(grad_value(grad, c_soft, end_z));
+            T* to = g + row.head + tid * E;
+            for (int c = 0; c < chunks; ++c, to += chunk * kRowThreads * E) {
+                if (!keep) copies_wait(slots);
                 aim();
-                next_slot = slot;
-                for (int v = 0; v < ring.chunk; v += kVectors) {
-                    fetch(v, count);
-                    T* const to = g + head + ((int64_t(c) * ring.chunk + v) * kRowThreads + tid) * E;
-#pragma unroll
-                    for (int h = 0; h < kVectors; ++h) {
-                        if (v + h >= count) break;
-                        grad_vector<T>(row, c_soft, raw[h], to + h * kRowThreads * E, aligned);
-                    }
-                    copy(v);  // (the places have been read: their values are used)
-                }
-                done();
+                done(each(count_of(row.vectors, c * chunk), [&](const auto& raw, int v, auto many) {
+                    put_grad<T, decltype(many)::value>(powers, raw, to + v * kRowThreads * E, kRowThreads * E, decltype(many)::value, aligned);
+                    copy(v, many);  // (the places have been read: their values are used)
+                }));
             }
             __syncwarp();
             barrier_arrive<kWritten>(parity, kMeeting);
         }
+        row = next_row;
         end = next_end;
         end_z = next_end_z;
     }
@@ -837,12 +911,12 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
     const int64_t row_vectors = ceil_div(vocab, half ? 8 : 4);
     if (s.rows >= int64_t(sm_count()) * kRowBlocks && row_vectors >= kRowThreads * 4) {
         RingArgs ring{};
-        const int64_t whole = ceil_div(ceil_div(row_vectors, kRowThreads), kVectors) * kVectors;
+        const int64_t whole = ceil_div(row_vectors, kRowThreads);
         const int most = static_cast<int>((kRowShared - kTeachers * shared) / (kRowThreads * 16));  // vectors of a thread
         ring.held = forward && present(a.grad) && whole <= most;
-        ring.chunk = ring.held ? static_cast<int>(whole) : kVectors;
-        ring.slots = std::min(3, most / ring.chunk);
+        ring.chunk = ring.held ? static_cast<int>(whole) : 2 * kBatch;
         ring.chunks = static_cast<int>(ceil_div(whole, ring.chunk));
+        ring.slots = std::min(3, most / ring.chunk);
         const size_t bytes = static_cast<size_t>(ring.slots) * ring.chunk * kRowThreads * 16 + kTeachers * shared;
         auto go = [&](auto kernel) {
             (void)blocks_at_once(reinterpret_cast<const void*>(kernel), kRowThreads + kTeachers * 32, bytes);  // (allows that much shared memory)
