@@ -245,11 +245,10 @@ __device__ __forceinline__ GradPowers grad_powers(const RowGrad& g, float c_soft
     x.wh = g.wh != 0.f ? g.wh * x.hard.factor : 0.f;
     return x;
 }
-__device__ __forceinline__ float grad_value(const RowGrad& g, float c_soft, float z) {
-    const GradPowers x = grad_powers(g, c_soft);
+__device__ __forceinline__ float grad_value(const GradPowers& x, float z) {
     float y = 0.f;
-    if (g.ws != 0.f) y += x.ws * (x.soft.direct ? power<true>(x.soft, z) : power<false>(x.soft, z));
-    if (g.wh != 0.f) y += x.wh * (x.hard.direct ? power<true>(x.hard, z) : power<false>(x.hard, z));
+    if (x.ws != 0.f) y += x.ws * (x.soft.direct ? power<true>(x.soft, z) : power<false>(x.soft, z));
+    if (x.wh != 0.f) y += x.wh * (x.hard.direct ? power<true>(x.hard, z) : power<false>(x.hard, z));
     return y;
 }
 template <typename T, bool DIRECT, int NV>
@@ -460,10 +459,10 @@ distill_kernel(const Args k) {
         row.ws = taught ? w * (1.f - k.hard_weight) * k.temperature : 0.f;
         row.wh = labelled ? w * k.hard_weight : 0.f;
         row.at = at, row.soft2 = -log_soft * kLog2e, row.hard2 = -log_hard * kLog2e;
-        if (end >= 0) g[end] = from_float<T>(grad_value(row, c_soft, end_z));
+        const GradPowers powers = grad_powers(row, c_soft);
+        if (end >= 0) g[end] = from_float<T>(grad_value(powers, end_z));
         const bool aligned = (reinterpret_cast<uintptr_t>(g + head) & 15) == 0;
         const bool again = v1 - v0 > int64_t(kVectors) * threads && FORWARD;  // not held any more
-        const GradPowers powers = grad_powers(row, c_soft);
         for (int64_t from = v0; from < v1; from += kVectors * threads) {
             if (again || from != v0) load(from);
             const int64_t v = from + tid;
@@ -476,7 +475,7 @@ distill_kernel(const Args k) {
             const int c = col[j];
             float minus;
             if (c < 0 || c < c0 || c >= c1 || !entry_takes(row, col, p, k.top, k.soft, j, minus)) continue;
-            g[c] = from_float<T>(grad_value(row, c_soft, zk[j]) - minus);
+            g[c] = from_float<T>(grad_value(powers, zk[j]) - minus);
         }
     } else {
         if (FORWARD && k.blocks > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // (no block leaves before its part is read)
@@ -488,11 +487,11 @@ distill_kernel(const Args k) {
 // Two blocks to an SM take one row after another each, so that one computes while the other meets.  kRowWarps warps work on the logits, which come through shared memory: each thread copies its own vectors
 // (cp.async, 16 bytes) some visits ahead, and copies the next one into a place as soon as it has used what lay there, so that the memory is never idle.
 // A visit is a chunk of a row, or, where the losses and the gradient are computed at once and the row fits, the whole row, which then stays until its
-// gradient is written.  Two more warps do what the teacher and the label ask for, one the even and one the odd rows, up to two rows ahead: ids, the
+// gradient is written.  Three more warps do what the teacher and the label ask for, each for every third row, up to two rows ahead: ids, the
 // logits at them, softmax, the loss once the row's sums are there, and the columns written again once the gradient is.  They meet by named barriers
 // at which neither side waits for what it does not need: told (the teacher's part of row i is there), summed (the warps' sums are) and written.
 // (A block or a cluster to each row waited for ids, logits, sums and its successor's start one after another: 4096 x 32000 took 157 us and 189 us.)
-constexpr int kRowWarps = 12, kRowThreads = kRowWarps * 32, kTeachers = 2, kRowBlocks = 2;
+constexpr int kRowWarps = 8, kRowThreads = kRowWarps * 32, kTeachers = 3, kRowBlocks = 2;
 constexpr int kBatch = 4;            // vectors that a thread works on at once
 constexpr int kRowShared = 112 << 10;  // of a block: the ring and the teachers' arrays
 
@@ -504,7 +503,7 @@ template <int ID>
 __device__ __forceinline__ void barrier_arrive(int parity, int threads) {
     asm volatile("barrier.arrive %0, %1;" ::"r"(ID + parity), "r"(threads) : "memory");
 }
-constexpr int kRowBarrier = 1, kTold = 2, kSummed = 4, kWritten = 6;
+constexpr int kRowBarrier = 1, kTold = 2, kSummed = kTold + kTeachers, kWritten = kSummed + kTeachers;
 constexpr int kMeeting = kRowThreads + 32;
 
 struct TeacherRow {
@@ -557,50 +556,62 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
         for (uint32_t i = parity; i < n; i += kTeachers) {
             const uint32_t r = blockIdx.x + i * gridDim.x;
             const T* const z = logits_of(i);
+            // what hangs on nothing else is asked for first
+            const int64_t label_id = k.hard ? load_index(row_at(k.labels, k.inner, r), k.wide_labels) : -1;
+            const float weight = GRAD && k.weights.base != nullptr ? *reinterpret_cast<const float*>(row_at(k.weights, k.inner, r)) : 1.f;
+            const float4 stats = FORWARD ? make_float4(0.f, 0.f, 0.f, 0.f) : k.stats[r];
+            const int label = label_id >= 0 && label_id < k.vocab ? static_cast<int>(label_id) : -1;
+            if (label_id >= k.vocab && lane == 0) atomicOr(k.status, kStatusIndexOutOfRange);
             float top_t = -INFINITY, sum = 0.f;
             if (k.soft) {
                 const char* ids = row_at(k.ids, k.inner, r);
                 const char* t = row_at(k.teacher, k.inner, r);
-#pragma unroll 4
-                for (int j = lane; j < k.top; j += 32) {
-                    const int64_t id = load_index(ids + int64_t(j) * (k.wide_ids ? 8 : 4), k.wide_ids);
-                    const bool in = id >= 0 && id < k.vocab;
-                    if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
-                    const float tj = in ? (k.half_teacher ? __half2float(reinterpret_cast<const __half*>(t)[j]) : reinterpret_cast<const float*>(t)[j]) : -INFINITY;
-                    col[j] = in ? static_cast<int>(id) : -1;
-                    p[j] = tj;
-                    zk[j] = in ? to_float(z[id]) : 0.f;
-                    top_t = fmaxf(top_t, tj);
+                bool outside = false;
+                for (int j0 = lane; j0 < k.top; j0 += 128) {  // four entries of a lane at once: their ids, then the logits there
+                    int c[4];
+                    float tj[4], zj[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int j = j0 + u * 32;
+                        c[u] = -1, tj[u] = -INFINITY;
+                        if (j < k.top) {
+                            const int64_t id = load_index(ids + int64_t(j) * (k.wide_ids ? 8 : 4), k.wide_ids);
+                            tj[u] = k.half_teacher ? __half2float(reinterpret_cast<const __half*>(t)[j]) : reinterpret_cast<const float*>(t)[j];
+                            outside |= id >= k.vocab;
+                            if (id >= 0 && id < k.vocab) c[u] = static_cast<int>(id);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) zj[u] = c[u] >= 0 ? to_float(z[c[u]]) : 0.f;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int j = j0 + u * 32;
+                        if (c[u] < 0) tj[u] = -INFINITY;
+                        if (j < k.top) col[j] = c[u], p[j] = tj[u], zk[j] = zj[u];
+                        top_t = fmaxf(top_t, tj[u]);
+                    }
                 }
+                if (outside) atomicOr(k.status, kStatusIndexOutOfRange);
+            }
+            const float label_z = label >= 0 ? to_float(z[label]) : 0.f;
+            if (lane == 0) col[k.top] = label, zk[k.top] = label_z;
+            if (k.soft) {
 #pragma unroll
                 for (int d = 16; d > 0; d /= 2) top_t = fmaxf(top_t, __shfl_xor_sync(0xffffffffu, top_t, d));
-                for (int j = lane; j < k.top; j += 32) sum += col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse) : 0.f;
+#pragma unroll 4
+                for (int j = lane; j < k.top; j += 32) sum += fast_exp2((p[j] - shift_of(top_t)) * c_soft);  // (no entry: -inf)
 #pragma unroll
                 for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             }
             const bool taught = k.soft && !(sum == 0.f);
             const float log_sum = logf(sum);
-            int label = -1;
-            float label_z = 0.f;
-            if (k.hard) {
-                const int64_t id = load_index(row_at(k.labels, k.inner, r), k.wide_labels);
-                if (id >= k.vocab && lane == 0) atomicOr(k.status, kStatusIndexOutOfRange);
-                if (id >= 0 && id < k.vocab) {
-                    label = static_cast<int>(id);
-                    label_z = to_float(z[id]);
-                }
-            }
-            if (lane == 0) col[k.top] = label, zk[k.top] = label_z;
             RowGrad row = {};
             if constexpr (GRAD) {
-                const float w = k.grad_scale * (k.weights.base != nullptr ? *reinterpret_cast<const float*>(row_at(k.weights, k.inner, r)) : 1.f);
+                const float w = k.grad_scale * weight;
                 row.ws = taught ? w * (1.f - k.hard_weight) * k.temperature : 0.f;
                 row.wh = label >= 0 ? w * k.hard_weight : 0.f;
             }
-            if constexpr (!FORWARD) {
-                const float4 s = k.stats[r];
-                row.at = shift_of(s.x), row.soft2 = -shift_of(s.y) * kLog2e, row.hard2 = -shift_of(s.z) * kLog2e;
-            }
+            if constexpr (!FORWARD) row.at = shift_of(stats.x), row.soft2 = -shift_of(stats.y) * kLog2e, row.hard2 = -shift_of(stats.z) * kLog2e;
             if (lane == 0) told[parity].grad = row;
             __syncwarp();
             barrier_arrive<kTold>(parity, kMeeting);
@@ -614,9 +625,10 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
                 log_soft = shift_of(log_soft), log_hard = shift_of(log_hard);
                 row.at = at, row.soft2 = -log_soft * kLog2e, row.hard2 = -log_hard * kLog2e;
                 float kl = 0.f;
-                for (int j = lane; j < k.top && k.soft; j += 32) {
+#pragma unroll 4
+                for (int j = lane; j < (k.soft ? k.top : 0); j += 32) {
                     const float lp = (p[j] - shift_of(top_t)) * k.inverse - log_sum;
-                    const float pj = taught && col[j] >= 0 ? expf(lp) : 0.f;
+                    const float pj = taught ? fast_exp2(lp * kLog2e) : 0.f;  // (no entry: exp of -inf)
                     p[j] = pj;
                     if (pj != 0.f) kl += pj * (lp - ((zk[j] - at) * k.inverse - log_soft));
                 }
@@ -629,16 +641,18 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
                     k.losses[r] = loss;
                 }
             } else {
-                for (int j = lane; j < k.top && k.soft; j += 32) p[j] = taught && col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse - log_sum) : 0.f;
+#pragma unroll 4
+                for (int j = lane; j < (k.soft ? k.top : 0); j += 32) p[j] = taught ? fast_exp2(((p[j] - shift_of(top_t)) * k.inverse - log_sum) * kLog2e) : 0.f;
             }
             __syncwarp();
             if constexpr (GRAD) {
                 barrier_sync<kWritten>(parity, kMeeting);
                 T* const g = grad_of(i);
+                const GradPowers powers = grad_powers(row, c_soft);
                 for (int j = lane; j <= k.top; j += 32) {
                     float minus;
                     if (col[j] < 0 || !entry_takes(row, col, p, k.top, k.soft, j, minus)) continue;
-                    g[col[j]] = from_float<T>(grad_value(row, c_soft, zk[j]) - minus);
+                    g[col[j]] = from_float<T>(grad_value(powers, zk[j]) - minus);
                 }
                 __syncwarp();
             }
@@ -761,7 +775,7 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
                 }
             }
             Part run = warp_part(running.part, c_soft, k.soft, k.hard);
-            barrier_sync<kTold>(parity, kMeeting);  // (so the teacher is done with the sums of two rows ago, too)
+            barrier_sync<kTold>(parity, kMeeting);  // (so the teacher is done with the sums of its last row, too)
             if (lane == 0) parts[parity][warp] = run;
             __syncwarp();
             if constexpr (GRAD) barrier_sync<kRowBarrier>(0, kRowThreads);
@@ -781,7 +795,7 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
             const GradPowers powers = grad_powers(grad, c_soft);
             T* const g = grad_of(i);
             const bool aligned = (reinterpret_cast<uintptr_t>(g + row.head) & 15) == 0;
-            if (end >= 0) g[end] = from_float<T>(grad_value(grad, c_soft, end_z));
+            if (end >= 0) g[end] = from_float<T>(grad_value(powers, end_z));
             T* to = g + row.head + tid * E;
             for (int c = 0; c < chunks; ++c, to += chunk * kRowThreads * E) {
                 if (!keep) copies_wait(slots);
