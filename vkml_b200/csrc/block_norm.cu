@@ -637,14 +637,15 @@ struct FoldArgs {
     bool half;
 };
 
-// to[g][c] = sum over p of from[g * parts + p][c]: 32 columns to a block, 8 threads to a column, each with an eighth of the parts in order.
-__global__ void __launch_bounds__(256) fold_kernel(const FoldArgs k) {
-    __shared__ float part[8][33];
+// to[g][c] = sum over p of from[g * parts + p][c]: 32 columns to a block, kFoldShares threads to a column, each with its share of the parts in order.
+constexpr int kFoldShares = 8;
+__global__ void __launch_bounds__(32 * kFoldShares) fold_kernel(const FoldArgs k) {
+    __shared__ float part[kFoldShares][33];
     pdl_prologue();
     const Fold& f = k.f[blockIdx.y];
     const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = blockIdx.x * 32 + x;
     for (uint32_t g = blockIdx.z; g < f.groups; g += gridDim.z) {
-        const uint32_t p0 = f.parts * y / 8, p1 = f.parts * (y + 1) / 8;
+        const uint32_t p0 = stretch(f.parts, y, kFoldShares), p1 = stretch(f.parts, y + 1, kFoldShares);
         float sum = 0.f;
         if (c < k.width) {
             const float* from = f.from + (int64_t(g) * f.parts) * k.width + c;
@@ -656,6 +657,7 @@ __global__ void __launch_bounds__(256) fold_kernel(const FoldArgs k) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum += v[i];
             }
+#pragma unroll 4
             for (; p < p1; ++p) sum += from[int64_t(p) * k.width];
         }
         part[y][x] = sum;
@@ -663,7 +665,7 @@ __global__ void __launch_bounds__(256) fold_kernel(const FoldArgs k) {
         if (y == 0 && c < k.width) {
             float total = part[0][x];
 #pragma unroll
-            for (int i = 1; i < 8; ++i) total += part[i][x];
+            for (int i = 1; i < kFoldShares; ++i) total += part[i][x];
             const int64_t at = int64_t(g) * k.width + c;
             if (k.half) static_cast<__half*>(f.to)[at] = __float2half_rn(total);
             else static_cast<float*>(f.to)[at] = total;
@@ -1003,7 +1005,7 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     });
     check_last_launch("block_norm_backward");
     if (folds > 0) {
-        launch_kernel(ctx, fold_kernel, dim3(static_cast<unsigned>(ceil_div(p.width, 32)), folds, groups), 256, 0, fold);
+        launch_kernel(ctx, fold_kernel, dim3(static_cast<unsigned>(ceil_div(p.width, 32)), folds, groups), 32 * kFoldShares, 0, fold);
         check_last_launch("block_norm_backward");
     }
     ctx->count_launch(folds > 0 ? 2 : 1);

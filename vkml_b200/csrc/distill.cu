@@ -521,11 +521,16 @@ struct RingArgs {
 
 __device__ __forceinline__ void copy_vector(uint32_t to, const uint4* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(__cvta_generic_to_global(from)) : "memory"); }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the newest slots - 1 groups of this thread's copies are there.
-__device__ __forceinline__ void copies_wait(int slots) {
-    if (slots == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (slots == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+// All but the newest `pending` groups of this thread's copies are there.
+__device__ __forceinline__ void copies_wait(int pending) {
+    switch (pending) {
+        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;  // (more are waited for than need be)
+    }
 }
 
 template <typename T, bool FORWARD, bool GRAD>
@@ -704,46 +709,62 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
         }
     };
     uint32_t slot = 0;  // in bytes
-    // `many` copies of the next visit into this one's places, from its vector v on
-    auto copy = [&](int v, auto many) {
-        constexpr int M = decltype(many)::value;
+    // kBatch copies of the next visit into this one's places, from its vector v on
+    auto copy = [&](int v) {
         const uint32_t to = my_place + slot + v * kApart;
         const uint4* const from = source + v * kRowThreads;
-        if (v + M <= limit) {
+        if (v + kBatch <= limit) {
 #pragma unroll
-            for (int h = 0; h < M; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
+            for (int h = 0; h < kBatch; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
         } else {
             for (int h = 0; v + h < limit; ++h) copy_vector(to + h * kApart, from + h * kRowThreads);
         }
+        if (keep) copies_commit();  // (a group to each batch, so that a row can be begun before its end is there)
     };
-    using Batch = std::integral_constant<int, kBatch>;
-    using One = std::integral_constant<int, 1>;
-    // f of the `count` vectors of a visit, kBatch at a time as far as that goes, and then of the places that hold none: f(vectors, the first one's number, how many)
-    auto each = [&](int count, auto&& f) {
-        auto get = [&](uint4& x, uint32_t at) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory"); };
-        int v = 0;
-        uint32_t from = my_place + slot;
-        for (; v + kBatch <= count; v += kBatch, from += kBatch * kApart) {
-            uint4 raw[kBatch];
-#pragma unroll
-            for (int h = 0; h < kBatch; ++h) get(raw[h], from + h * kApart);
-            f(raw, v, Batch{});
-        }
-        for (; v < count; ++v, from += kApart) {
-            uint4 raw[1];
-            get(raw[0], from);
-            f(raw, v, One{});
-        }
-        return v;
-    };
-    auto done = [&](int v) {  // with a visit, of which v places have been copied into
-        for (; v < limit; ++v) copy(v, One{});
-        copies_commit();
+    auto next = [&] {
+        if (!keep) copies_commit();
         slot = slot + slot_bytes == slots * slot_bytes ? 0 : slot + slot_bytes;
     };
+    const int batches = (chunk + kBatch - 1) / kBatch, newest = keep ? slots * batches - 1 : slots - 1;
+    // A visit with `count` vectors for this thread: f(vectors, the first one's number), kBatch at a time as far as that goes.  WAIT: the copies are waited for; FREE: the next
+    // visit's take their places, which have been read: their values are used.
+    auto visit = [&](int count, auto wait, auto free, auto&& f) {
+        auto get = [&](uint4& x, uint32_t at) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory"); };
+        if (decltype(free)::value) aim();
+        if (decltype(wait)::value && !keep) copies_wait(newest);
+        uint32_t from = my_place + slot;
+        for (int v = 0, batch = 0; v < chunk; v += kBatch, ++batch, from += kBatch * kApart) {
+            if (decltype(wait)::value && keep) copies_wait(newest - batch);
+            if (v + kBatch <= count) {
+                uint4 raw[kBatch];
+#pragma unroll
+                for (int h = 0; h < kBatch; ++h) get(raw[h], from + h * kApart);
+                f(raw, v);
+            } else {
+                int h = 0;
+                if (v + 2 <= count) {
+                    uint4 raw[2];
+                    get(raw[0], from);
+                    get(raw[1], from + kApart);
+                    f(raw, v);
+                    h = 2;
+                }
+                if (v + h < count) {
+                    uint4 raw[1];
+                    get(raw[0], from + h * kApart);
+                    f(raw, v + h);
+                }
+            }
+            if (decltype(free)::value) copy(v);
+        }
+        if (decltype(free)::value) next();
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
     for (int s = 0; s < slots; ++s) {
         aim();
-        done(0);
+        for (int v = 0; v < chunk; v += kBatch) copy(v);
+        next();
     }
     Row row = row_of(0);
     int end = end_of(row);
@@ -761,18 +782,11 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
         if constexpr (FORWARD) {
             Running running;
             running.begin(end_z, c_soft, k.soft, k.hard);
-            for (int c = 0; c < chunks; ++c) {
-                copies_wait(slots);
-                const int count = count_of(row.vectors, c * chunk);
-                if (keep) {
-                    each(count, [&](const auto& raw, int, auto) { running.take<T>(raw); });
-                } else {
-                    aim();
-                    done(each(count, [&](const auto& raw, int v, auto many) {
-                        running.take<T>(raw);
-                        copy(v, many);
-                    }));
-                }
+            auto take = [&](const auto& raw, int) { running.take<T>(raw); };
+            if (keep) {
+                visit(count_of(row.vectors, 0), Yes{}, No{}, take);
+            } else {
+                for (int c = 0; c < chunks; ++c) visit(count_of(row.vectors, c * chunk), Yes{}, Yes{}, take);
             }
             Part run = warp_part(running.part, c_soft, k.soft, k.hard);
             barrier_sync<kTold>(parity, kMeeting);  // (so the teacher is done with the sums of its last row, too)
@@ -797,13 +811,14 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
             const bool aligned = (reinterpret_cast<uintptr_t>(g + row.head) & 15) == 0;
             if (end >= 0) g[end] = from_float<T>(grad_value(powers, end_z));
             T* to = g + row.head + tid * E;
-            for (int c = 0; c < chunks; ++c, to += chunk * kRowThreads * E) {
-                if (!keep) copies_wait(slots);
-                aim();
-                done(each(count_of(row.vectors, c * chunk), [&](const auto& raw, int v, auto many) {
-                    put_grad<T, decltype(many)::value>(powers, raw, to + v * kRowThreads * E, kRowThreads * E, decltype(many)::value, aligned);
-                    copy(v, many);  // (the places have been read: their values are used)
-                }));
+            auto put = [&](const auto& raw, int v) {
+                constexpr int M = std::extent<std::remove_reference_t<decltype(raw)>>::value;
+                put_grad<T, M>(powers, raw, to + v * kRowThreads * E, kRowThreads * E, M, aligned);
+            };
+            if (keep) {
+                visit(count_of(row.vectors, 0), No{}, Yes{}, put);
+            } else {
+                for (int c = 0; c < chunks; ++c, to += chunk * kRowThreads * E) visit(count_of(row.vectors, c * chunk), Yes{}, Yes{}, put);
             }
             __syncwarp();
             barrier_arrive<kWritten>(parity, kMeeting);

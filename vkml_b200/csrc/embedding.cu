@@ -25,11 +25,12 @@ struct Ids {
 
 // ---- lookup -----------------------------------------------------------------
 
-// A thread moves kItems pieces of a row, kThreads pieces apart, so that their ids and then their elements are all under way together.
-// A piece is 8 elements where rows of both sides start on 16 bytes and hold whole pieces, one element otherwise.
-constexpr int kItems = 4;
+// Rows that start on a boundary of eight elements and hold whole eights: a thread moves kItems such pieces, kThreads pieces apart, so that their ids and then
+// their elements are under way together.  (16384 rows of 1024, F32 to F16: 14.4 us with four pieces to a thread, 12.2 with two, 13.6 with one: four leave an SM
+// half as many threads.)
+constexpr int kItems = 2;
 
-template <typename TI, typename TO, bool WIDE>
+template <typename TI, typename TO>
 __global__ void __launch_bounds__(kThreads)
 lookup_kernel(RowsArg out, const char* table, int64_t pitch, Ids ids, int64_t vocab, FastDiv pieces, int64_t total, float scale, uint32_t* status) {
     pdl_prologue();
@@ -54,34 +55,55 @@ lookup_kernel(RowsArg out, const char* table, int64_t pitch, Ids ids, int64_t vo
             }
         }
     }
-    if constexpr (WIDE) {
-        Raw8<TI> raw[kItems];
+    Raw8<TI> raw[kItems];
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            if (id[k] >= 0) load8(raw[k], reinterpret_cast<const TI*>(table + id[k] * pitch) + int64_t(piece[k]) * 8);
+    for (int k = 0; k < kItems; ++k) {
+        if (id[k] >= 0) load8(raw[k], reinterpret_cast<const TI*>(table + id[k] * pitch) + int64_t(piece[k]) * 8);
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        if (id[k] == -2) continue;
+        float x[8] = {};
+        if (id[k] >= 0) {
+            unpack8(raw[k], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= scale;
         }
-#pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            if (id[k] == -2) continue;
-            float x[8] = {};
-            if (id[k] >= 0) {
-                unpack8(raw[k], x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= scale;
-            }
-            store8(reinterpret_cast<TO*>(row_at(out, ids.inner, token[k])) + int64_t(piece[k]) * 8, x);
-        }
+        store8(reinterpret_cast<TO*>(row_at(out, ids.inner, token[k])) + int64_t(piece[k]) * 8, x);
+    }
+}
+
+// Other rows: a warp moves up to kStretch columns of a row, neighbours to neighbouring lanes.
+constexpr int kStretch = 256;
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(kThreads)
+lookup_any_kernel(RowsArg out, const char* table, int64_t pitch, Ids ids, int64_t vocab, int64_t width, FastDiv stretches, int64_t total, float scale, uint32_t* status) {
+    pdl_prologue();
+    const int64_t task = int64_t(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32;
+    if (task >= total) return;
+    const int lane = threadIdx.x % 32;
+    uint32_t token, part;
+    if (total < (int64_t(1) << 31)) {
+        stretches.divmod(static_cast<uint32_t>(task), token, part);
     } else {
-        TI raw[kItems];
+        token = static_cast<uint32_t>(task / stretches.d);
+        part = static_cast<uint32_t>(task - int64_t(token) * stretches.d);
+    }
+    const int64_t id = ids[token];
+    const bool in = id >= 0 && id < vocab;
+    if (!in && lane == 0 && part == 0) atomicOr(status, kStatusIndexOutOfRange);
+    const int64_t first = int64_t(part) * kStretch + lane;
+    const TI* const from = reinterpret_cast<const TI*>(table + (in ? id : 0) * pitch) + first;
+    TO* const to = reinterpret_cast<TO*>(row_at(out, ids.inner, token)) + first;
+    TI raw[kStretch / 32];
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            if (id[k] >= 0) raw[k] = reinterpret_cast<const TI*>(table + id[k] * pitch)[piece[k]];
-        }
+    for (int k = 0; k < kStretch / 32; ++k) {
+        if (in && first + k * 32 < width) raw[k] = from[k * 32];
+    }
 #pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-            if (id[k] == -2) continue;
-            reinterpret_cast<TO*>(row_at(out, ids.inner, token[k]))[piece[k]] = from_float<TO>(id[k] >= 0 ? to_float(raw[k]) * scale : 0.f);
-        }
+    for (int k = 0; k < kStretch / 32; ++k) {
+        if (first + k * 32 < width) to[k * 32] = from_float<TO>(in ? to_float(raw[k]) * scale : 0.f);
     }
 }
 
@@ -807,15 +829,18 @@ void launch_lookup(b200_ctx* ctx, const b200_embedding_args& a) {
     if (p.count == 0 || p.width == 0) return;
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
     const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
-    const int64_t pieces = wide ? p.width / 8 : p.width, total = p.count * pieces;
-    const int64_t blocks = ceil_div(total, kThreads * kItems);
+    const int64_t pieces = wide ? p.width / 8 : ceil_div(p.width, kStretch), total = p.count * pieces;
+    const int64_t blocks = ceil_div(total, wide ? kThreads * kItems : kThreads / 32);
     if (blocks >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "embedding: too many elements");
     ProfScope scope(ctx, "embedding");
+    const char* table = static_cast<const char*>(a.table.data);
+    const FastDiv by(static_cast<uint32_t>(pieces));
     with_types(a.table.dtype, a.rows.dtype, [&](auto ti, auto to) {
         using TI = decltype(ti);
         using TO = decltype(to);
-        launch_kernel(ctx, wide ? lookup_kernel<TI, TO, true> : lookup_kernel<TI, TO, false>, static_cast<unsigned>(blocks), kThreads, 0, p.rows,
-                      static_cast<const char*>(a.table.data), p.pitch, p.ids, p.vocab, FastDiv(static_cast<uint32_t>(pieces)), total, a.scale, ctx->d_status);
+        const dim3 grid(static_cast<unsigned>(blocks));
+        if (wide) launch_kernel(ctx, lookup_kernel<TI, TO>, grid, kThreads, 0, p.rows, table, p.pitch, p.ids, p.vocab, by, total, a.scale, ctx->d_status);
+        else launch_kernel(ctx, lookup_any_kernel<TI, TO>, grid, kThreads, 0, p.rows, table, p.pitch, p.ids, p.vocab, p.width, by, total, a.scale, ctx->d_status);
     });
     check_last_launch("embedding");
     ctx->count_launch();
