@@ -305,7 +305,7 @@ constexpr int kOwnRms = 3;  // without FULL: kE, kPreW and kPostW, which come fi
 __host__ __device__ constexpr int own_place(int which) { return which == kE ? 0 : which == kPreW ? 1 : which == kPostW ? 2 : which == kF ? 3 : which == kPreB ? 4 : 5; }
 
 template <typename TH, typename TY, int NV, bool WIDE, bool WARP, bool FULL, bool REGS, bool HOLD, bool AHEAD>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : HOLD ? 512 : 1024, WARP ? 2 : 1)
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : AHEAD ? 512 : 1024, WARP ? 2 : 1)
 norm_backward_kernel(const BackwardArgs k) {
     constexpr int N = FULL ? 8 : 4;
     extern __shared__ __align__(16) float shared_own[];
@@ -315,7 +315,8 @@ norm_backward_kernel(const BackwardArgs k) {
     int slot = 0;
     const int threads = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x % 32 : threadIdx.x, warp = threadIdx.x / 32;
     float* const own = k.own != nullptr ? k.own + int64_t(blockIdx.x) * ((FULL ? kOwnSums : kOwnRms) * NV * 8) * blockDim.x : shared_own;
-    float* const factors = shared_own + (REGS ? 2 : 0) * NV * 8 * blockDim.x;  // REGS: kPostW and kPostB lie in front
+    constexpr bool KEEP = REGS || (HOLD && !FULL);                          // the columns' factors in shared memory, behind the sums there
+    float* const factors = shared_own + (REGS ? 2 : kOwnRms) * NV * 8 * blockDim.x;  // (REGS: kPostW and kPostB lie in front)
     const bool pre = k.normed_grad.base != nullptr, branch = k.branch.base != nullptr || k.branch_grad.base != nullptr;
     // running sums: in registers, or in `own`
     float sum[REGS ? 4 : 1][REGS ? NV : 1][8];
@@ -385,7 +386,7 @@ norm_backward_kernel(const BackwardArgs k) {
             }
         }
     };
-    // the columns' factors: w1 and c = b gate w2 in every row, b gate, w2 and b2 at an item's end; w1 and c from the thread's own memory where that is (REGS)
+    // the columns' factors: w1 and c = b gate w2 in every row, b gate, w2 and b2 at an item's end; w1 and c from the thread's own memory where there is room (KEEP)
     enum { kW1, kC, kW2, kG, kB2 };
     const char* gate = nullptr;
     auto read_factor = [&](int which, int v, float (&x)[8]) {
@@ -407,11 +408,11 @@ norm_backward_kernel(const BackwardArgs k) {
         }
     };
     auto factor = [&](int which, int v, float (&x)[8]) {
-        if constexpr (REGS) own_load(factors, which * NV + v, x);
+        if constexpr (KEEP) own_load(factors, which * NV + v, x);
         else read_factor(which, v, x);
     };
     auto keep_factor = [&](int which) {
-        if constexpr (REGS) {
+        if constexpr (KEEP) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 float x[8];
@@ -637,8 +638,9 @@ struct FoldArgs {
     bool half;
 };
 
-// to[g][c] = sum over p of from[g * parts + p][c]: 32 columns to a block, kFoldShares threads to a column, each with its share of the parts in order.
-constexpr int kFoldShares = 8;
+// to[g][c] = sum over p of from[g * parts + p][c]: 32 columns to a block, kFoldShares threads to a column, each with its share of the parts in order, kFoldAtOnce of
+// them under way.  (Eight threads to a column, eight parts under way: 10 us for 592 blocks' sums of 1024 columns, as long as their rows' reading waits.)
+constexpr int kFoldShares = 16, kFoldAtOnce = 20;
 __global__ void __launch_bounds__(32 * kFoldShares) fold_kernel(const FoldArgs k) {
     __shared__ float part[kFoldShares][33];
     pdl_prologue();
@@ -646,19 +648,14 @@ __global__ void __launch_bounds__(32 * kFoldShares) fold_kernel(const FoldArgs k
     const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = blockIdx.x * 32 + x;
     for (uint32_t g = blockIdx.z; g < f.groups; g += gridDim.z) {
         const uint32_t p0 = stretch(f.parts, y, kFoldShares), p1 = stretch(f.parts, y + 1, kFoldShares);
+        const float* from = f.from + (int64_t(g) * f.parts + p0) * k.width + c;
         float sum = 0.f;
-        if (c < k.width) {
-            const float* from = f.from + (int64_t(g) * f.parts) * k.width + c;
-            uint32_t p = p0;
-            for (; p + 8 <= p1; p += 8) {
-                float v[8];
+        for (uint32_t p = p0; p < p1; p += kFoldAtOnce, from += int64_t(kFoldAtOnce) * k.width) {
+            float v[kFoldAtOnce];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = from[int64_t(p + i) * k.width];
+            for (int i = 0; i < kFoldAtOnce; ++i) v[i] = p + i < p1 && c < k.width ? from[int64_t(i) * k.width] : 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += v[i];
-            }
-#pragma unroll 4
-            for (; p < p1; ++p) sum += from[int64_t(p) * k.width];
+            for (int i = 0; i < kFoldAtOnce; ++i) sum += v[i];
         }
         part[y][x] = sum;
         __syncthreads();
@@ -825,7 +822,7 @@ void launch_forward(b200_ctx* ctx, const b200_block_norm_args& a) {
 }
 
 // How a backward call is divided.  Rows of up to 256 elements are a warp's; up to 4096 a block's of up to 512 threads that keep the sums over rows in
-// registers; up to 8192 the same with the sums in shared memory; wider ones are read twice by 1024 threads.
+// registers; up to 8192 a block's of up to 1024 threads that keep them in shared memory; wider ones are read twice by 1024 threads.
 struct Division {
     uint32_t blocks, threads, pieces, items;
     bool warp, regs, hold, full, warp_items, direct_gate;
@@ -842,16 +839,16 @@ Division divide(const b200_block_norm_grad_args& a, const Shape& p, int sms) {
     d.warp = p.width <= 256;
     d.regs = p.width <= 4096;
     d.hold = p.width <= 8192;
-    d.nv = d.regs ? 1 : 2;
+    d.nv = d.hold ? 1 : 2;
     d.threads = d.warp ? kWarpRows * 32 : static_cast<uint32_t>(ceil_div(p.width, int64_t(8) * d.nv * 32)) * 32;
     d.full = a.kind == B200_NORM_LAYER || present(a.post_bias) || present(a.post_bias_grad) || present(a.pre_bias_grad);
     const size_t own = static_cast<size_t>(d.nv) * 32 * d.threads;  // bytes of one vector of the threads' columns
-    d.shared = d.regs ? own * 4 : own * (d.full ? kOwnSums : kOwnRms);
+    d.shared = d.regs ? own * 4 : d.full ? own * kOwnSums : own * (kOwnRms + (d.hold ? 2 : 0));
     const bool own_shared = d.shared <= kMostShared;
     if (!own_shared) d.shared = 0;
     const int64_t group_rows = p.s.rows / p.gates;
     // as many blocks as the registers of an SM hold at once
-    const int64_t resident = int64_t(sms) * std::max<int64_t>(1, std::min<int64_t>((d.hold ? 512 : 1024) / d.threads, static_cast<int64_t>(kMostShared / (d.shared + 4096))));
+    const int64_t resident = int64_t(sms) * std::max<int64_t>(1, std::min<int64_t>((d.regs ? 512 : 1024) / d.threads, static_cast<int64_t>(kMostShared / (d.shared + 4096))));
     // warps share a block's rows, unless a gate has too few of them
     d.warp_items = d.warp && p.gates > 1 && group_rows < 8 * kWarpRows;
     const int64_t workers = d.warp_items ? resident * kWarpRows : resident;
@@ -986,7 +983,6 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     with_types(p, [&](auto th, auto ty) {
         using TH = decltype(th);
         using TY = decltype(ty);
-        constexpr bool kBothHalf = sizeof(TH) == 2;
         auto go = [&](auto kernel) {
             (void)blocks_at_once(reinterpret_cast<const void*>(kernel), static_cast<int>(d.threads), d.shared);  // (allows that much shared memory)
             launch_kernel(ctx, kernel, dim3(d.blocks), dim3(d.threads), d.shared, k);
@@ -995,7 +991,7 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
             constexpr bool W = decltype(is_wide)::value, F = decltype(is_full)::value;
             if (d.warp) go(norm_backward_kernel<TH, TY, 1, W, true, F, true, true, true>);
             else if (d.regs) go(norm_backward_kernel<TH, TY, 1, W, false, F, true, true, true>);
-            else if (d.hold) go(norm_backward_kernel<TH, TY, 2, W, false, F, false, true, kBothHalf && W>);
+            else if (d.hold) go(norm_backward_kernel<TH, TY, 1, W, false, F, false, true, false>);
             else go(norm_backward_kernel<TH, TY, 2, W, false, F, false, false, false>);
         };
         if (wide && d.full) of_kind(std::true_type{}, std::true_type{});
