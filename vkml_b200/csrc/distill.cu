@@ -972,7 +972,7 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
     if (grid >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "distill_loss: too many rows of this length");
     auto go = [&](auto kernel) {
         if (blocks == 1 || !forward) launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, k);
-        else launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, blocks, true, k);
+        else launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, blocks, false, k);
     };
     if (!forward) go(half ? distill_kernel<__half, false, true> : distill_kernel<float, false, true>);
     else if (present(a.grad)) go(half ? distill_kernel<__half, true, true> : distill_kernel<float, true, true>);

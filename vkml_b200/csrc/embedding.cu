@@ -1011,8 +1011,7 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
         const int at_once = clusters_at_once(d.held, d.cluster);
         if (at_once < 1) fail(B200_DEVICE_ERROR, "embedding_backward: the device takes no cluster of " + std::to_string(d.cluster) + " blocks");
         const unsigned beside = static_cast<unsigned>(std::min<int64_t>(std::max(1, at_once - 1), ceil_div(int64_t(take_zeros()), d.cluster)));
-        launch_kernel_clustered(ctx, sort_cluster(d.held), dim3((1 + beside) * d.cluster), dim3(kSortThreads), static_cast<size_t>(kSortThreads) * d.held * sizeof(uint2), d.cluster,
-                                true, s);
+        launch_kernel_clustered(ctx, sort_cluster(d.held), dim3((1 + beside) * d.cluster), dim3(kSortThreads), static_cast<size_t>(kSortThreads) * d.held * sizeof(uint2), d.cluster, false, s);  // (not early: clusters of 16 wait for a GPC's SMs, which a kernel before may hold)
         check_last_launch("embedding_backward");
         ctx->count_launch();
     }
