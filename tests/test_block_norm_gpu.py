@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 F32, F16 = np.float32, np.float16
 SIDES = [(F32, F32), (F16, F16), (F32, F16)]
 WEIGHTS = ("post_weight", "post_bias", "pre_weight", "pre_bias")
-SHAPES = [((1, 1), "dense"), ((4, 1, 512), "dense"), ((3, 5, 33), "odd"), ((2, 7, 256), "pitch"), ((6, 3, 264), "swapped"), ((37, 1000), "dense"),
+SHAPES = [((1, 1), "dense"), ((40,), "dense"), ((4, 1, 512), "dense"), ((3, 5, 33), "odd"), ((2, 7, 256), "pitch"), ((6, 3, 264), "swapped"), ((37, 1000), "dense"),
           ((5, 1024), "offset"), ((3, 2, 2048), "backwards"), ((3, 2056), "dense"), ((2, 3, 4096), "pitch"), ((7, 4104), "dense"), ((2, 5001), "odd"),
           ((3, 8192), "dense"), ((2, 2, 16384), "dense"), ((1, 16383), "dense")]
 
@@ -38,7 +38,7 @@ def test_forward_and_backward(backend, th, ty, shape, layout, kind):
     rng = np.random.default_rng(shape[-1] + 3 * len(shape))
     layer, width, rows = kind == "layer", shape[-1], int(np.prod(shape[:-1]))
     wt = ty if layout in ("dense", "odd") else F32
-    gates = {"dense": 1, "odd": shape[0], "pitch": rows, "swapped": shape[0], "offset": 0, "backwards": shape[0]}[layout]
+    gates = {"dense": min(1, len(shape) - 1), "odd": shape[0], "pitch": rows, "swapped": shape[0], "offset": 0, "backwards": shape[0]}[layout]
     p = parameters(rng, width, wt, rows, gates, layer)
     h = placed((rng.standard_normal(shape) * 2 + 0.5).astype(th), layout)
     y = placed((rng.standard_normal(shape) + 0.25).astype(ty), layout)

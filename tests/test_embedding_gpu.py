@@ -139,6 +139,27 @@ def test_gradient_leaves_bad_ids_out(backend, count):
     backend.synchronize()  # nothing but padding was left out
 
 
+@pytest.mark.parametrize("count", [0, 3, 600, 40000])
+def test_rows_without_a_token_are_zeros_whatever_the_scale(backend, count):
+    ids, grad = np.full(count, 3, np.int64), np.ones((count, 16), np.float32)
+    table = np.full((9, 16), np.nan, np.float32)
+    space = Space(backend)
+    backend.embedding_backward(space.put(grad), space.put(ids), space.put(table), scale=float("inf"))
+    got = space.get(table)[0]
+    assert not np.delete(got, 3, 0).any() and (count == 0 or np.isinf(got[3]).all())
+
+
+def test_one_token(backend):
+    """An id without extents: one row."""
+    table, ids, row = np.arange(12, dtype=np.float32).reshape(3, 4), np.array(2, np.int32), np.empty(4, np.float32)
+    space = Space(backend)
+    backend.embedding(space.put(table), space.put(ids), space.put(row))
+    assert np.array_equal(space.get(row)[0], table[2])
+    grad = np.full((3, 4), np.nan, np.float32)
+    backend.embedding_backward(space.put(row + 1), space.put(ids), space.put(grad))
+    assert not space.get(grad)[0][:2].any()
+
+
 def test_repeated_row_of_gradients(backend):
     """A gradient that is one row for all tokens (stride 0), as that of a sum is."""
     ids = np.arange(5000, dtype=np.int64).reshape(50, 100) % 7

@@ -789,12 +789,14 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
                 for (int c = 0; c < chunks; ++c) visit(count_of(row.vectors, c * chunk), Yes{}, Yes{}, take);
             }
             Part run = warp_part(running.part, c_soft, k.soft, k.hard);
+            __syncwarp();
             barrier_sync<kTold>(parity, kMeeting);  // (so the teacher is done with the sums of its last row, too)
             if (lane == 0) parts[parity][warp] = run;
             __syncwarp();
             if constexpr (GRAD) barrier_sync<kRowBarrier>(0, kRowThreads);
             barrier_arrive<kSummed>(parity, kMeeting);
         } else {
+            __syncwarp();
             barrier_sync<kTold>(parity, kMeeting);
         }
         if constexpr (GRAD) {
@@ -862,7 +864,9 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
     if (top > kMostTop) fail(B200_NOT_IMPLEMENTED, "distill_loss: more than 1024 of the teacher's logits");
     if (vocab < 1 || vocab >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "logits: rows of no element, or of 2^31 or more");
     const RowShape s = row_shape(a.logits, axes);
-    if (!(a.temperature > 0.f) || std::isinf(a.temperature)) fail(B200_INVALID_ARGUMENT, "distill_loss: the temperature is not above 0 and finite");
+    if (!(a.temperature > 0.f) || std::isinf(a.temperature) || std::isinf(1.f / a.temperature)) {
+        fail(B200_INVALID_ARGUMENT, "distill_loss: the temperature is not above 0 and finite, or its inverse is not");
+    }
     if (!(a.hard_weight >= 0.f && a.hard_weight <= 1.f)) fail(B200_INVALID_ARGUMENT, "distill_loss: the hard weight is not in 0..1");
     const bool labelled = a.labels.data != nullptr || a.labels.ndim != 0;
     if (labelled) {

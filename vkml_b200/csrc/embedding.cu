@@ -190,7 +190,7 @@ owned_rows_kernel(char* table, int64_t pitch, RowsArg grad, Ids ids, uint32_t co
         if (accumulate && !any) continue;
         TO* to = reinterpret_cast<TO*>(table + (row0 + r) * pitch) + col0;
         for (int c = tid; c < cols; c += kThreads) {
-            float x = sums[r * columns + c] * scale;
+            float x = any ? sums[r * columns + c] * scale : 0.f;  // (zeros whatever the scale)
             if (accumulate) x += to_float(to[c]);
             to[c] = from_float<TO>(x);
         }
@@ -202,9 +202,8 @@ owned_rows_kernel(char* table, int64_t pitch, RowsArg grad, Ids ids, uint32_t co
 // The tokens are sorted by id, those of one id in their own order: radix passes over up to 8 bits of the id, of two kernels each.  A block has a tile of
 // the tokens, a warp a stretch of the tile.  count_kernel leaves the counts of the tile's digits; move_kernel ranks every token among those of
 // its digit in its stretch, adds the counts of the warps, the tiles and the digits before, and moves each token to its place.  Tokens that have no gradient
-// sort behind all others, as id V.  The memory is idle meanwhile, so
-// blocks behind those that sort write zeros over the table's last rows; the sums leave a bit for each row that has a token, and the rest of the
-// rows without one is written at the end.  Up to 32768 tokens one cluster of blocks sorts in one launch (sort_cluster_kernel).
+// sort behind all others, as id V.  The memory is idle meanwhile, so blocks behind those that sort write zeros over the table's last rows; the sums leave a
+// bit for each row that has a token, and the rest of the rows without one is written at the end.  Up to 32768 tokens one cluster of blocks sorts in one launch (sort_cluster_kernel).
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMostHeld = 8;        // tokens of a thread of many blocks
 constexpr int kMostClusterHeld = 2; // ... and of a cluster's: 131072 tokens by 16 blocks of 8 to a thread took 40 us, by 64 blocks 27

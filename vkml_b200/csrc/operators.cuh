@@ -22,7 +22,10 @@ int guarded_operator(b200_ctx* ctx, Fn&& fn) {
         return status;
     };
     try {
-        if (ctx != nullptr) B200_CUDA_CHECK(cudaSetDevice(ctx->device));
+        if (ctx != nullptr) {
+            B200_CUDA_CHECK(cudaSetDevice(ctx->device));
+            ctx->current_op = B200_OP_COUNT;  // (a profile's records of these launches belong to no node)
+        }
         fn();
         return B200_OK;
     } catch (const Error& e) {
