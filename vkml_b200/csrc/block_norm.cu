@@ -439,7 +439,7 @@ norm_backward_kernel(const BackwardArgs k) {
     for (int s = 0; s < kOwnSums; ++s) {
         if (FULL || own_place(s) < kOwnRms) clear(s);
     }
-    keep_factor(kW1);
+    bool first_item = true;
     const bool by_warp = WARP && k.warp_items;
     const uint32_t step = WARP && !by_warp ? kWarpRows : 1, workers = by_warp ? gridDim.x * kWarpRows : gridDim.x;
     for (uint32_t item = by_warp ? blockIdx.x * kWarpRows + warp : blockIdx.x; item < k.items; item += workers) {
@@ -448,7 +448,6 @@ norm_backward_kernel(const BackwardArgs k) {
         const uint32_t r1 = group * k.group_rows + stretch(k.group_rows, piece + 1, k.pieces);
         gate = static_cast<const char*>(k.gate);
         if (gate != nullptr) gate += int64_t(group) * k.gate_pitch;
-        keep_factor(kC);
         auto load_ahead = [&](uint32_t r) {
             if constexpr (AHEAD) {
 #pragma unroll
@@ -456,7 +455,11 @@ norm_backward_kernel(const BackwardArgs k) {
                 if (k.stats != nullptr) st_next = k.stats[r];
             }
         };
-        if (r0 < r1) load_ahead(r0);
+        if (WIDE && r0 < r1) load_ahead(r0);  // (element by element it costs: 4096 x 3000 F16 took 75 us, 62 this way)
+        if (first_item) keep_factor(kW1);
+        first_item = false;
+        keep_factor(kC);
+        if (!WIDE && r0 < r1) load_ahead(r0);
         float mean_c = 0.f;  // FULL: of c
         if (FULL && k.layer && k.post) {
             float x[1] = {0.f};
@@ -634,6 +637,7 @@ struct Fold {
 };
 struct FoldArgs {
     Fold f[kSums];
+    uint32_t vectors;  // folds of one group; one of several, the gate's, comes behind them
     int width;
     bool half;
 };
@@ -644,9 +648,11 @@ constexpr int kFoldShares = 16, kFoldAtOnce = 20;
 __global__ void __launch_bounds__(32 * kFoldShares) fold_kernel(const FoldArgs k) {
     __shared__ float part[kFoldShares][33];
     pdl_prologue();
-    const Fold& f = k.f[blockIdx.y];
+    const bool one = blockIdx.y < k.vectors;
+    const Fold& f = k.f[one ? blockIdx.y : k.vectors];
     const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = blockIdx.x * 32 + x;
-    for (uint32_t g = blockIdx.z; g < f.groups; g += gridDim.z) {
+    const uint32_t step = one ? 1 : gridDim.y - k.vectors;  // (at least 1: this block is one of them)
+    for (uint32_t g = one ? 0 : blockIdx.y - k.vectors; g < f.groups; g += step) {
         const uint32_t p0 = stretch(f.parts, y, kFoldShares), p1 = stretch(f.parts, y + 1, kFoldShares);
         const float* from = f.from + (int64_t(g) * f.parts + p0) * k.width + c;
         float sum = 0.f;
@@ -946,14 +952,14 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     k.gate_pitch = p.width * (k.half_columns ? 2 : 4);
     FoldArgs fold{};
     fold.width = static_cast<int>(p.width);
-    unsigned folds = 0, groups = 1;
+    unsigned folds = 0, groups = 0;
     auto take = [&](int64_t floats) {
         float* at = reinterpret_cast<float*>(scratch);
         scratch += (static_cast<size_t>(floats) * sizeof(float) + 255) / 256 * 256;
         return at;
     };
     if (d.own_floats > 0) k.own = take(d.own_floats);
-    for (int s = 0; s < kSums; ++s) {
+    for (int s : {kPostWeight, kPostBias, kPreWeight, kPreBias, kGate}) {
         if (!present(*vectors[s])) continue;
         if (s == kGate && d.direct_gate) {
             k.gate_grad = vectors[s]->data;
@@ -961,8 +967,10 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
             continue;
         }
         k.partial[s] = take(d.partial_floats[s]);
-        fold.f[folds++] = Fold{k.partial[s], vectors[s]->data, static_cast<uint32_t>(s == kGate ? p.gates : 1), s == kGate ? d.pieces : d.blocks};
-        if (s == kGate) groups = static_cast<unsigned>(std::min<int64_t>(p.gates, 4096));
+        const bool several = s == kGate && p.gates > 1;
+        fold.f[folds++] = Fold{k.partial[s], vectors[s]->data, static_cast<uint32_t>(several ? p.gates : 1), s == kGate ? d.pieces : d.blocks};
+        if (several) groups = static_cast<unsigned>(std::min<int64_t>(p.gates, 4096));
+        else ++fold.vectors;
         fold.half = vectors[s]->dtype == B200_F16;
     }
     k.inner = FastDiv(static_cast<uint32_t>(p.s.inner));
@@ -1001,7 +1009,7 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     });
     check_last_launch("block_norm_backward");
     if (folds > 0) {
-        launch_kernel(ctx, fold_kernel, dim3(static_cast<unsigned>(ceil_div(p.width, 32)), folds, groups), 32 * kFoldShares, 0, fold);
+        launch_kernel(ctx, fold_kernel, dim3(static_cast<unsigned>(ceil_div(p.width, 32)), fold.vectors + groups), 32 * kFoldShares, 0, fold);
         check_last_launch("block_norm_backward");
     }
     ctx->count_launch(folds > 0 ? 2 : 1);
