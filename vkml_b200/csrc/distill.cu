@@ -74,19 +74,6 @@ __device__ __forceinline__ Part warp_part(Part x, float c_soft, bool soft, bool 
     return x;
 }
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float x, float* part, F&& join, float empty) {
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) x = join(x, __shfl_xor_sync(0xffffffffu, x, d));
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = x;
-    __syncthreads();
-    x = threadIdx.x % 32 < blockDim.x / 32 ? part[threadIdx.x % 32] : empty;
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) x = join(x, __shfl_xor_sync(0xffffffffu, x, d));
-    return x;
-}
-
 // Elements of a row that lie before its first 16-byte boundary.
 template <typename T>
 __device__ __forceinline__ int64_t head_of(const T* row, int64_t n) {
@@ -310,7 +297,8 @@ __device__ __forceinline__ bool entry_takes(const RowGrad& row, const int* col, 
 // Arrays of a row's entries in shared memory: the columns [top + 1 and up to 3 of none], probabilities [top], logits there [top + 1].
 __host__ __device__ __forceinline__ int entry_words(int top) { return (top / 4 + 1) * 4 + (top + 3) / 4 * 4 + (top / 4 + 1) * 4; }
 
-// Few rows, or short ones: a block or a cluster to a row.
+// Few rows, or short ones: a block or a cluster to a row.  Its warps meet as seldom as can be, since that is what a row of few vectors takes its time for: when
+// the teacher's entries are there, when the warps' sums are, and before the entries' columns are written.  Each warp finds the teacher's maximum and sum by itself.
 template <typename T, bool FORWARD, bool GRAD>
 __global__ void __launch_bounds__(kMostThreads, 2)
 distill_kernel(const Args k) {
@@ -319,7 +307,6 @@ distill_kernel(const Args k) {
     int* const col = reinterpret_cast<int*>(shared);                         // the columns, -1: none
     float* const p = reinterpret_cast<float*>(col + (k.top / 4 + 1) * 4);    // the teacher's probabilities
     float* const zk = p + (k.top + 3) / 4 * 4;                               // the logits at the teacher's columns, and at the label's
-    __shared__ float part[32];
     __shared__ Part parts[32];
     __shared__ Part block_part;  // read by the other blocks of the cluster
     pdl_prologue();
@@ -348,7 +335,6 @@ distill_kernel(const Args k) {
     if (end >= 0) end_z = to_float(z[end]);
 
     // the teacher's distribution and the logits at its columns
-    float top_t = -INFINITY;
     if (k.soft) {
         const char* ids = row_at(k.ids, k.inner, r);
         const char* t = row_at(k.teacher, k.inner, r);
@@ -359,10 +345,8 @@ distill_kernel(const Args k) {
             col[j] = in ? static_cast<int>(id) : -1;
             p[j] = in ? (k.half_teacher ? __half2float(reinterpret_cast<const __half*>(t)[j]) : reinterpret_cast<const float*>(t)[j]) : -INFINITY;
             zk[j] = in ? to_float(z[id]) : 0.f;
-            top_t = fmaxf(top_t, p[j]);
         }
-    }
-    if (!k.soft) {
+    } else {
         for (int j = tid; j < k.top; j += threads) col[j] = -1;
     }
     if (tid > 0 && tid < 4 && k.top + tid < (k.top / 4 + 1) * 4) col[k.top + tid] = -1;
@@ -376,29 +360,38 @@ distill_kernel(const Args k) {
         col[k.top] = static_cast<int>(id < 0 ? -1 : id);
         zk[k.top] = id < 0 ? 0.f : to_float(z[id]);
     }
+    __syncthreads();
+    const float c_soft = k.inverse * kLog2e;
     bool taught = false;  // whether the row has a teacher's entry
-    float log_sum = 0.f;
+    float top_t = -INFINITY, log_sum = 0.f;
     if (k.soft) {
-        top_t = block_reduce(top_t, part, [](float a, float b) { return fmaxf(a, b); }, -INFINITY);
         float sum = 0.f;
-        for (int j = tid; j < k.top; j += threads) sum += col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse) : 0.f;
-        sum = block_reduce(sum, part, [](float a, float b) { return a + b; }, 0.f);
+        for (int j = tid % 32; j < k.top; j += 32) top_t = fmaxf(top_t, p[j]);
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) top_t = fmaxf(top_t, __shfl_xor_sync(0xffffffffu, top_t, d));
+        for (int j = tid % 32; j < k.top; j += 32) sum += fast_exp2((p[j] - shift_of(top_t)) * c_soft);  // (no entry: -inf)
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         taught = !(sum == 0.f);
         log_sum = logf(sum);
         if constexpr (!FORWARD) {
+            __syncthreads();  // (every warp has read what the teacher says)
             for (int j = tid; j < k.top; j += threads) p[j] = taught && col[j] >= 0 ? expf((p[j] - shift_of(top_t)) * k.inverse - log_sum) : 0.f;
         }
     }
 
     // The row's maximum and log sums of exponentials: q = exp((z - at) / T - log_soft), h = exp(z - at - log_hard).  The maximum and the logarithms stay
     // apart: their sum would lose the logarithm in a row whose logits are all the type's lowest value.
-    const float c_soft = k.inverse * kLog2e;
     float at = 0.f, log_soft = 0.f, log_hard = 0.f;
     if constexpr (FORWARD) {
         Running running;
         running.begin(end_z, c_soft, k.soft, k.hard);
         for (int64_t from = v0;;) {
-            running.take<T>(raw);
+            const int64_t left = v1 - from;  // (what lies behind the end costs exponentials too)
+            if (left <= threads) running.take<T>(reinterpret_cast<const uint4 (&)[1]>(raw));
+            else if (left <= 2 * threads) running.take<T>(reinterpret_cast<const uint4 (&)[2]>(raw));
+            else if (left <= 4 * threads) running.take<T>(reinterpret_cast<const uint4 (&)[4]>(raw));
+            else running.take<T>(raw);
             from += kVectors * threads;
             if (from >= v1) break;
             load(from);
@@ -429,14 +422,15 @@ distill_kernel(const Args k) {
         // a row of nothing but -inf: the sums are 0 and their logarithms -inf, which stay out of the differences so that q = 0, log q = -inf
         log_soft = shift_of(log_soft), log_hard = shift_of(log_hard);
         float kl = 0.f;
-        if (k.soft && (GRAD || rank == 0)) {
-            for (int j = tid; j < k.top; j += threads) {
+        if (k.soft && tid < 32 && (GRAD || rank == 0)) {  // the first warp's, while the others go on
+            for (int j = tid; j < k.top; j += 32) {
                 const float lp = (p[j] - shift_of(top_t)) * k.inverse - log_sum;
                 const float pj = taught && col[j] >= 0 ? expf(lp) : 0.f;
                 p[j] = pj;
                 if (pj != 0.f) kl += pj * (lp - ((zk[j] - at) * k.inverse - log_soft));
             }
-            if (rank == 0 && k.losses != nullptr) kl = block_reduce(kl, part, [](float a, float b) { return a + b; }, 0.f);
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) kl += __shfl_xor_sync(0xffffffffu, kl, d);
         }
         if (rank == 0 && tid == 0 && k.losses != nullptr) {
             float loss = 0.f;
@@ -450,8 +444,7 @@ distill_kernel(const Args k) {
     }
 
     if constexpr (GRAD) {
-        // The other threads' p, zk and col; and where the gradient lies on the logits, the other blocks' reading of them.
-        __syncthreads();
+        // Where the gradient lies on the logits: the other blocks' reading of them.  (This block's ended before its warps met.)
         if (FORWARD && k.blocks > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         const float w = k.grad_scale * (k.weights.base != nullptr ? *reinterpret_cast<const float*>(row_at(k.weights, k.inner, r)) : 1.f);
         const bool labelled = k.hard && col[k.top] >= 0;
