@@ -138,6 +138,38 @@ def test_the_same_bits_again_and_between_other_work(backend):
         assert np.array_equal(x, first[k]), k
 
 
+@pytest.mark.parametrize("large,small", [(1000, 320), (4096, 264), (8192, 4104), (16384, 8200)])
+def test_a_size_again_after_a_smaller_one(backend, large, small):
+    """The widths, and the numbers of a teacher's entries, in turn: what a kernel was allowed for a size holds when the size comes back."""
+    rng = np.random.default_rng(large)
+
+    def norms(width, kind):
+        a = {k: rng0.standard_normal((5, width)).astype(F32) for k in ("h", "y", "dout", "dn")}
+        t = {k: tensor(backend, x) for k, x in a.items()}
+        t.update({k: DeviceTensor.empty(backend, (5, width)) for k in ("out", "normed", "dh", "dy")}, stats=DeviceTensor.empty(backend, (5, 4)), dw=DeviceTensor.empty(backend, (width,)))
+        backend.block_norm(t["h"], t["y"], out=t["out"], normed=t["normed"], stats=t["stats"], kind=kind)
+        backend.block_norm_backward(t["out"], t["y"], t["stats"], out_grad=t["dout"], normed_grad=t["dn"], residual_grad=t["dh"], branch_grad=t["dy"], pre_weight_grad=t["dw"],
+                                    kind=kind)
+        return [t[k].numpy() for k in ("out", "normed", "dh", "dy", "dw")]
+
+    logits = tensor(backend, rng.standard_normal((300, 16384)).astype(F16))
+
+    def distilled(top):
+        ids, teacher = tensor(backend, rng0.integers(0, 16384, (300, top))), tensor(backend, rng0.standard_normal((300, top)).astype(F32))
+        losses, stats, grad, again = (DeviceTensor.empty(backend, s, d) for s, d in (((300,), DType.F32), ((300, 4), DType.F32), ((300, 16384), DType.F16), ((300, 16384), DType.F16)))
+        backend.distill_loss(logits, ids, teacher, losses, stats=stats, temperature=2.0)
+        backend.distill_loss(logits, ids, teacher, losses, stats=stats, grad=grad, temperature=2.0)
+        backend.distill_loss_backward(logits, ids, teacher, stats, again, temperature=2.0)
+        return [x.numpy() for x in (losses, stats, grad, again)]
+
+    results = []
+    for width in (large, small, large):
+        rng0 = np.random.default_rng(width)
+        results.append(norms(width, "rms") + norms(width, "layer") + distilled(min(1024, width // 16)))
+    for x, y in zip(results[0], results[2]):
+        assert np.array_equal(x, y)
+
+
 class Runtime:
     """The few calls of the CUDA runtime that capture and launch a graph."""
 

@@ -268,7 +268,7 @@ void check_block_norm(const b200_block_norm_args& a);
 void check_block_norm_backward(const b200_block_norm_grad_args& a);
 void check_distill_loss(const b200_distill_args& a, bool forward);
 
-// How many blocks of a kernel an SM of the current device holds at once.
+// How many blocks of a kernel an SM of the current device holds at once; allows the kernel that much shared memory.
 inline int blocks_at_once(const void* kernel, int threads, size_t shared) {
     struct Key {
         const void* kernel;
@@ -279,12 +279,17 @@ inline int blocks_at_once(const void* kernel, int threads, size_t shared) {
     };
     static std::mutex mutex;
     static std::map<Key, int> known;
+    static std::map<std::pair<const void*, int>, size_t> allowed;
     int dev = 0;
     B200_CUDA_CHECK(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mutex);
     int& n = known[Key{kernel, threads, shared, dev}];
     if (n == 0) {
-        if (shared > 0) B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
+        size_t& most = allowed[{kernel, dev}];  // (never lowered: a call of the larger size may come again, and finds its answer here)
+        if (shared > most) {
+            B200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)));
+            most = shared;
+        }
         int found = 0;
         B200_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&found, kernel, threads, shared));
         if (found < 1) fail(B200_INTERNAL_ERROR, "a kernel does not fit on an SM");
