@@ -118,6 +118,23 @@ def test_a_view_of_longer_sequences(backend):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rows,vocab,top", [(3, 40, 64), (5, 200, 65), (300, 333, 100), (2, 90001, 1024), (298, 9001, 70), (297, 33001, 120), (299, 18000, 300)])
+def test_many_entries_that_repeat(backend, dtype, rows, vocab, top):
+    """More entries than there are different columns: each column is written once, with all that its entries take off."""
+    rng = np.random.default_rng(top)
+    z = rng.standard_normal((rows, vocab), dtype=np.float32).astype(dtype)
+    columns = rng.choice(vocab, max(2, min(vocab, top * 2 // 3)), replace=False)
+    columns[:2] = 0, vocab - 1
+    k = rng.choice(columns, (rows, top)).astype(np.int32)
+    k[rng.random(k.shape) < 0.1] = -1
+    t = rng.standard_normal((rows, top)).astype(dtype)
+    labels = rng.choice(columns, rows)
+    labels[::5] = -1
+    some = np.unique([0, 1, rows // 2, rows - 1])
+    run(backend, z, k, t, labels, None, 2.0, 0.25, 4.0, some=some)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("vocab", [50, 70000])
 def test_entries_that_are_none_and_entries_that_repeat(backend, dtype, vocab):
     """Ids below 0, rows without any, a column named several times, -inf of the teacher; labels below 0; a label on a teacher's column."""

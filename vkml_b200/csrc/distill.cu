@@ -34,6 +34,7 @@ struct Args {
     uint32_t* status;
     int64_t vocab;
     int top;
+    int slots;            // of a row's table of columns; 0: none
     int blocks;           // of a row's cluster
     bool wide_ids, wide_labels, half_teacher;
     bool soft, hard;      // which parts have a weight
@@ -270,31 +271,71 @@ __device__ __forceinline__ void put_grad(const GradPowers& g, const uint4 (&raw)
     else grad_vectors<T, false>(g, raw, to, apart_by, count, aligned);
 }
 
+// A table of a row's columns in shared memory, which shows whether an entry is the only one of its column: open addressing, the sign of a slot set where
+// more than one entry came.  At most a third of it is taken.  Rows of few entries compare each with all instead, which is as fast for 64 of them and takes twice as
+// long for 256 (33554 x 1000 F32 with gradient: 706 us, 313 with the table).
+constexpr int kMostCompared = 64;
+constexpr int kEmptySlot = 0x7fffffff;  // (no column: rows have fewer than 2^31)
+int table_slots(int top) {
+    int slots = 256;
+    while (slots < top * 3) slots *= 2;
+    return top <= kMostCompared ? 0 : slots;
+}
+__device__ __forceinline__ void clear_table(int* table, int slots, int t, int threads) {
+    for (int i = t * 4; i < slots; i += threads * 4) *reinterpret_cast<int4*>(table + i) = make_int4(kEmptySlot, kEmptySlot, kEmptySlot, kEmptySlot);
+}
+__device__ __forceinline__ uint32_t first_slot(int c, int slots) { return (static_cast<uint32_t>(c) * 0x9e3779b1u) >> 16 & (slots - 1); }
+__device__ __forceinline__ void enter_column(int* table, int slots, int c) {
+    for (uint32_t at = first_slot(c, slots);; at = (at + 1) & (slots - 1)) {
+        const int seen = atomicCAS(&table[at], kEmptySlot, c);
+        if (seen == kEmptySlot) return;
+        if ((seen & 0x7fffffff) == c) {
+            atomicOr(&table[at], static_cast<int>(0x80000000u));
+            return;
+        }
+    }
+}
+__device__ __forceinline__ bool column_alone(const int* table, int slots, int c) {
+    for (uint32_t at = first_slot(c, slots);; at = (at + 1) & (slots - 1)) {
+        if ((table[at] & 0x7fffffff) == c) return table[at] >= 0;
+    }
+}
+
 // What p and the label take off the gradient's column col[j], if entry j is the first that names it.  The columns lie on a 16-byte boundary, `top` + 1 of
-// them and none (-1) up to the next multiple of four.  Almost always an entry is alone, which a comparison with four at a time shows.
-__device__ __forceinline__ bool entry_takes(const RowGrad& row, const int* col, const float* p, int top, bool soft, int j, float& minus) {
+// them and none (-1) up to the next multiple of four.  Almost always an entry is alone.
+__device__ __forceinline__ bool entry_takes(const RowGrad& row, const int* col, const float* p, const int* table, int slots, int top, bool soft, int j, float& minus) {
     const int c = col[j];
-    int equal = 0;
+    bool alone;
+    if (slots > 0) {
+        alone = column_alone(table, slots, c);
+    } else {
+        int equal = 0;
 #pragma unroll 4
-    for (int m = 0; m <= top; m += 4) {
-        const int4 four = *reinterpret_cast<const int4*>(col + m);
-        equal += (four.x == c) + (four.y == c) + (four.z == c) + (four.w == c);
+        for (int m = 0; m <= top; m += 4) {
+            const int4 four = *reinterpret_cast<const int4*>(col + m);
+            equal += (four.x == c) + (four.y == c) + (four.z == c) + (four.w == c);
+        }
+        alone = equal == 1;
     }
     minus = 0.f;
-    if (equal == 1) {
+    if (alone) {
         if (j == top) minus = row.wh;
         else if (row.ws != 0.f) minus = row.ws * p[j];
         return true;
     }
-    for (int m = 0; m < top && soft; ++m) {
-        if (col[m] != c) continue;
-        if (m < j) return false;
-        if (row.ws != 0.f) minus += row.ws * p[m];
+    for (int m = 0; m < top && soft; m += 4) {
+        const int4 four = *reinterpret_cast<const int4*>(col + m);
+        if (four.x != c && four.y != c && four.z != c && four.w != c) continue;
+        for (int e = m; e < m + 4 && e < top; ++e) {
+            if (col[e] != c) continue;
+            if (e < j) return false;
+            if (row.ws != 0.f) minus += row.ws * p[e];
+        }
     }
     if (col[top] == c) minus += row.wh;
     return true;
 }
-// Arrays of a row's entries in shared memory: the columns [top + 1 and up to 3 of none], probabilities [top], logits there [top + 1].
+// Arrays of a row's entries in shared memory: the columns [top + 1 and up to 3 of none], probabilities [top], logits there [top + 1]; the table comes behind.
 __host__ __device__ __forceinline__ int entry_words(int top) { return (top / 4 + 1) * 4 + (top + 3) / 4 * 4 + (top / 4 + 1) * 4; }
 
 // Few rows, or short ones: a block or a cluster to a row.  Its warps meet as seldom as can be, since that is what a row of few vectors takes its time for: when
@@ -307,6 +348,7 @@ distill_kernel(const Args k) {
     int* const col = reinterpret_cast<int*>(shared);                         // the columns, -1: none
     float* const p = reinterpret_cast<float*>(col + (k.top / 4 + 1) * 4);    // the teacher's probabilities
     float* const zk = p + (k.top + 3) / 4 * 4;                               // the logits at the teacher's columns, and at the label's
+    int* const table = col + entry_words(k.top);
     __shared__ Part parts[32];
     __shared__ Part block_part;  // read by the other blocks of the cluster
     pdl_prologue();
@@ -332,6 +374,7 @@ distill_kernel(const Args k) {
         }
     };
     load(v0);
+    if (GRAD) clear_table(table, k.slots, tid, threads);
     if (end >= 0) end_z = to_float(z[end]);
 
     // the teacher's distribution and the logits at its columns
@@ -361,6 +404,11 @@ distill_kernel(const Args k) {
         zk[k.top] = id < 0 ? 0.f : to_float(z[id]);
     }
     __syncthreads();
+    if (GRAD && k.slots > 0) {
+        for (int j = tid; j <= k.top; j += threads) {
+            if (col[j] >= 0) enter_column(table, k.slots, col[j]);
+        }
+    }
     const float c_soft = k.inverse * kLog2e;
     bool taught = false;  // whether the row has a teacher's entry
     float top_t = -INFINITY, log_sum = 0.f;
@@ -467,7 +515,7 @@ distill_kernel(const Args k) {
         for (int j = tid; j <= k.top; j += threads) {
             const int c = col[j];
             float minus;
-            if (c < 0 || c < c0 || c >= c1 || !entry_takes(row, col, p, k.top, k.soft, j, minus)) continue;
+            if (c < 0 || c < c0 || c >= c1 || !entry_takes(row, col, p, table, k.slots, k.top, k.soft, j, minus)) continue;
             g[c] = from_float<T>(grad_value(powers, zk[j]) - minus);
         }
     } else {
@@ -544,9 +592,10 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
 
     if (warp >= kRowWarps) {
         const int parity = warp - kRowWarps;
-        int* const col = entries + parity * entry_words(k.top);
+        int* const col = entries + parity * (entry_words(k.top) + k.slots);
         float* const p = reinterpret_cast<float*>(col + (k.top / 4 + 1) * 4);
         float* const zk = p + (k.top + 3) / 4 * 4;
+        int* const table = col + entry_words(k.top);
         if (!k.soft) {
             for (int j = lane; j < k.top; j += 32) col[j] = -1;
         }
@@ -642,6 +691,13 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
 #pragma unroll 4
                 for (int j = lane; j < (k.soft ? k.top : 0); j += 32) p[j] = taught ? fast_exp2(((p[j] - shift_of(top_t)) * k.inverse - log_sum) * kLog2e) : 0.f;
             }
+            if (GRAD && k.slots > 0) {
+                clear_table(table, k.slots, lane, 32);
+                __syncwarp();
+                for (int j = lane; j <= k.top; j += 32) {
+                    if (col[j] >= 0) enter_column(table, k.slots, col[j]);
+                }
+            }
             __syncwarp();
             if constexpr (GRAD) {
                 barrier_sync<kWritten>(parity, kMeeting);
@@ -649,7 +705,7 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
                 const GradPowers powers = grad_powers(row, c_soft);
                 for (int j = lane; j <= k.top; j += 32) {
                     float minus;
-                    if (col[j] < 0 || !entry_takes(row, col, p, k.top, k.soft, j, minus)) continue;
+                    if (col[j] < 0 || !entry_takes(row, col, p, table, k.slots, k.top, k.soft, j, minus)) continue;
                     g[col[j]] = from_float<T>(grad_value(powers, zk[j]) - minus);
                 }
                 __syncwarp();
@@ -931,16 +987,19 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
     k.hard_weight = a.hard_weight;
     k.grad_scale = a.grad_scale;
     ProfScope scope(ctx, forward ? "distill_loss" : "distill_loss_backward");
-    const size_t shared = static_cast<size_t>(entry_words(static_cast<int>(top))) * 4;
+    k.slots = present(a.grad) ? table_slots(static_cast<int>(top)) : 0;
+    const size_t shared = static_cast<size_t>(entry_words(static_cast<int>(top)) + k.slots) * 4;
     const bool half = a.logits.dtype == B200_F16;
-    // Many rows of at least 16 KB each: blocks that stay take one row after another.  (Below, a block's warps have little to do between a row's meetings.)
+    // Many rows of at least 16 KB each: blocks that stay take one row after another.  (Below, a block's warps have little to do between a row's meetings.)  Not where
+    // a row's entries take a teacher's warp longer than its logits take the others: 2048 x 16384 F16, gradient: 64 entries 39 us and 45 by a block to a row, 256
+    // entries 86 and 61; losses and gradient: 256 entries 94 and 88, 1000 276 and 174; losses alone: 256 entries 36 and 36, 1000 92 and 61.
     const int64_t row_vectors = ceil_div(vocab, half ? 8 : 4);
-    if (s.rows >= int64_t(sm_count()) * kRowBlocks && row_vectors >= kRowThreads * 4) {
+    if (s.rows >= int64_t(sm_count()) * kRowBlocks && row_vectors >= std::max<int64_t>(kRowThreads * 4, top * (!forward ? 16 : present(a.grad) ? 6 : 4))) {
         RingArgs ring{};
         const int64_t whole = ceil_div(row_vectors, kRowThreads);
         const int most = static_cast<int>((kRowShared - kTeachers * shared) / (kRowThreads * 16));  // vectors of a thread
         ring.held = forward && present(a.grad) && whole <= most;
-        ring.chunk = ring.held ? static_cast<int>(whole) : 2 * kBatch;
+        ring.chunk = ring.held ? static_cast<int>(whole) : most >= 4 * kBatch ? 2 * kBatch : kBatch;
         ring.chunks = static_cast<int>(ceil_div(whole, ring.chunk));
         ring.slots = std::min(3, most / ring.chunk);
         const size_t bytes = static_cast<size_t>(ring.slots) * ring.chunk * kRowThreads * 16 + kTeachers * shared;
