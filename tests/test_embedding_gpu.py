@@ -103,6 +103,22 @@ def test_gradient_of_many_tokens(backend, count, vocab, width, skew):
     backend.synchronize()
 
 
+@pytest.mark.parametrize("count,vocab,width", [(0, 70000, 64), (1, 70000, 64), (3, 1100000, 4), (128, 5000, 838), (128, 5000, 840), (128, 60, 1000), (129, 60, 1000), (129, 1, 1), (512, 1024, 128), (513, 1024, 128), (512, 1025, 128)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient_of_few_tokens(backend, count, vocab, width, accumulate):
+    """The counts and tables at which the rows are no longer owned by blocks."""
+    rng = np.random.default_rng(count + width)
+    ids, grad = ids_of(rng, (count,), vocab, np.int64, True), rng.standard_normal((count, width)).astype(np.float16)
+    table = rng.standard_normal((vocab, width)).astype(np.float32) if accumulate else np.full((vocab, width), np.nan, np.float32)
+    space = Space(backend)
+    g, i, t = space.put(grad), space.put(ids), space.put(table)
+    backend.embedding_backward(g, i, t, accumulate=accumulate)
+    got = space.get(table)[0]
+    want, bound, touched = embedding_backward(ids, grad, vocab, 1.0, None, table if accumulate else None)
+    check(got, want, bound, np.float32, "table gradient")
+    assert np.array_equal(got[~touched], table[~touched]) if accumulate else not got[~touched].any()
+
+
 @pytest.mark.parametrize("count,vocab", [(3000, 4), (30000, 50000), (200000, 9)])
 def test_gradient_of_one_token(backend, count, vocab):
     """Every token the same: one list, as long as there are tokens."""

@@ -173,26 +173,40 @@ owned_rows_kernel(char* table, int64_t pitch, RowsArg grad, Ids ids, uint32_t co
         __syncthreads();
         const int n = warp_count[kChunk / 32 - 1];
         for (int c = tid; c < cols; c += kThreads) {
-            int j = 0;
-            for (; j + 4 <= n; j += 4) {  // four rows under way
-                float g[4];
+            constexpr int kAtOnce = 16;  // rows under way: the most frequent ids' block has a good part of the tokens
+            for (int j = 0; j < n; j += kAtOnce) {
+                TG g[kAtOnce];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) g[k] = to_float(reinterpret_cast<const TG*>(row_at(grad, ids.inner, list_token[j + k]))[col0 + c]);
+                for (int k = 0; k < kAtOnce; ++k) {
+                    if (j + k < n) g[k] = reinterpret_cast<const TG*>(row_at(grad, ids.inner, list_token[j + k]))[col0 + c];
+                }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sums[int(list_row[j + k]) * columns + c] += g[k];
+                for (int k = 0; k < kAtOnce; ++k) {
+                    if (j + k < n) sums[int(list_row[j + k]) * columns + c] += to_float(g[k]);
+                }
             }
-            for (; j < n; ++j) sums[int(list_row[j]) * columns + c] += to_float(reinterpret_cast<const TG*>(row_at(grad, ids.inner, list_token[j]))[col0 + c]);
         }
     }
     __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-        const bool any = (touched[r / 32] >> (r % 32)) & 1;
-        if (accumulate && !any) continue;
-        TO* to = reinterpret_cast<TO*>(table + (row0 + r) * pitch) + col0;
-        for (int c = tid; c < cols; c += kThreads) {
-            float x = any ? sums[r * columns + c] * scale : 0.f;  // (zeros whatever the scale)
-            if (accumulate) x += to_float(to[c]);
-            to[c] = from_float<TO>(x);
+    // The rows side by side, each rounded up to a power of two of columns, so that narrow ones have all threads too.
+    const int shift = cols > 1 ? 32 - __clz(cols - 1) : 0, cells = rows << shift;
+    constexpr int kCells = 4;  // under way
+    for (int first = tid; first < cells; first += kThreads * kCells) {
+        float x[kCells] = {};
+        if (accumulate) {
+#pragma unroll
+            for (int k = 0; k < kCells; ++k) {
+                const int cell = first + k * kThreads, r = cell >> shift, c = cell & ((1 << shift) - 1);
+                if (cell < cells && c < cols && (touched[r / 32] >> (r % 32) & 1)) x[k] = to_float(reinterpret_cast<const TO*>(table + (row0 + r) * pitch)[col0 + c]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kCells; ++k) {
+            const int cell = first + k * kThreads, r = cell >> shift, c = cell & ((1 << shift) - 1);
+            if (cell >= cells || c >= cols) continue;
+            const bool any = touched[r / 32] >> (r % 32) & 1;
+            if (any) x[k] += sums[r * columns + c] * scale;  // (else zeros whatever the scale)
+            if (any || !accumulate) reinterpret_cast<TO*>(table + (row0 + r) * pitch)[col0 + c] = from_float<TO>(x[k]);
         }
     }
 }
@@ -899,12 +913,14 @@ struct Division {
     size_t bytes;
 };
 
-// Few tokens: rows owned by blocks, each of which reads all ids.  Many: sorted tokens.
-constexpr int64_t kOwnedTokens = 512;
+// Few tokens and no large table, or a small one: rows owned by blocks, each of which reads all ids.  Else sorted tokens, whose launches take 12 to 14 us together, beside which
+// zeros are written.  (F32, owned and sorted: 128 tokens of 1000 x 64 5.5 us and 12.3, 512 tokens 13.5 and 13.7; of 1000 x 512 9.7 and 14.4, 27.6 and 14.4; 8 tokens
+// of 50000 x 128 13.9 and 12.3, of 50000 x 1024 77.8 and 41.2.)
+bool is_owned(int64_t count, int64_t elements) { return (count <= 128 && elements <= 1 << 22) || (count <= 512 && elements <= 1 << 17); }
 
 Division divide(const Problem& p) {
     Division d{};
-    if (p.count <= kOwnedTokens || p.vocab == 0 || p.width == 0) return d;
+    if (p.vocab == 0 || p.width == 0 || p.count == 0 || is_owned(p.count, p.vocab * p.width)) return d;
     d.threads = 1;
     while (d.threads < 128 && d.threads * 8 < p.width) d.threads *= 2;
     d.tiles = static_cast<int>(ceil_div(p.width, int64_t(d.threads) * 8));
