@@ -146,21 +146,22 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[NV]) {
 }
 
 // Powers of two of (x - at) * c + plus as one multiply-add each, x * c + offset, where at * c is of a size that leaves the offset its digits: what its rounding
-// took away is given back by the factor.  Where it is not (logits of the type's lowest value), the difference comes first.
+// took away is given back by the factor.  Where it is not (logits of the type's lowest value), the difference comes first.  The factor's terms are rounded one by
+// one, as written: joined into multiply-adds they count the product's rounding twice (1e-4 of a row's sums at a maximum of 1400).
 struct Exponent {
     float c, at, offset, factor;
     bool direct;
 };
 __device__ __forceinline__ Exponent exponent_of(float at, float c, float plus) {
     Exponent x;
-    const float p = at * c;
+    const float p = __fmul_rn(at, c);
     x.c = c, x.at = at;
     x.direct = fabsf(p) < 4096.f;
-    x.offset = x.direct ? plus - p : plus;
+    x.offset = x.direct ? __fsub_rn(plus, p) : plus;
     x.factor = 1.f;
     if (x.direct) {  // plus - at c, without the offset that stands for it: the difference's rounding and the product's
-        const float b = plus - x.offset, a = x.offset + b;
-        const float lost = ((plus - a) + (b - p)) - fmaf(at, c, -p);
+        const float b = __fsub_rn(plus, x.offset), a = __fadd_rn(x.offset, b);
+        const float lost = __fsub_rn(__fadd_rn(__fsub_rn(plus, a), __fsub_rn(b, p)), fmaf(at, c, -p));
         x.factor = fmaf(lost, 0.6931471805599453f, 1.f);
     }
     return x;
