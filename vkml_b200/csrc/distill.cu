@@ -152,11 +152,12 @@ struct Exponent {
     float c, at, offset, factor;
     bool direct;
 };
-__device__ __forceinline__ Exponent exponent_of(float at, float c, float plus) {
+__device__ __forceinline__ bool is_direct(float at, float c) { return fabsf(at * c) < 4096.f; }
+__device__ __forceinline__ Exponent exponent_of(float at, float c, float plus, bool direct) {
     Exponent x;
     const float p = __fmul_rn(at, c);
     x.c = c, x.at = at;
-    x.direct = fabsf(p) < 4096.f;
+    x.direct = direct;
     x.offset = x.direct ? __fsub_rn(plus, p) : plus;
     x.factor = 1.f;
     if (x.direct) {  // plus - at c, without the offset that stands for it: the difference's rounding and the product's
@@ -201,8 +202,9 @@ struct Running {
         aim();
     }
     __device__ __forceinline__ void aim() {
-        soft = exponent_of(shift_of(part.top), c_soft, 0.f);
-        hard = exponent_of(shift_of(part.top), kLog2e, 0.f);
+        const float at = shift_of(part.top);
+        soft = exponent_of(at, c_soft, 0.f, is_direct(at, c_soft));
+        hard = exponent_of(at, kLog2e, 0.f, is_direct(at, kLog2e));
     }
     template <typename T, int NV>
     __device__ __forceinline__ void take(const uint4 (&raw)[NV]) {
@@ -225,19 +227,21 @@ struct RowGrad {
 struct GradPowers {
     Exponent soft, hard;
     float ws, wh;  // the exponents' factors included
+    bool direct;   // both of them: a vector's elements take one form.  One whose weight is 0 is not asked
 };
 __device__ __forceinline__ GradPowers grad_powers(const RowGrad& g, float c_soft) {
     GradPowers x;
-    x.soft = exponent_of(g.at, c_soft, g.soft2);
-    x.hard = exponent_of(g.at, kLog2e, g.hard2);
+    x.direct = (g.ws == 0.f || is_direct(g.at, c_soft)) && (g.wh == 0.f || is_direct(g.at, kLog2e));
+    x.soft = exponent_of(g.at, c_soft, g.soft2, x.direct);
+    x.hard = exponent_of(g.at, kLog2e, g.hard2, x.direct);
     x.ws = g.ws != 0.f ? g.ws * x.soft.factor : 0.f;  // (a row that does not count may hold anything)
     x.wh = g.wh != 0.f ? g.wh * x.hard.factor : 0.f;
     return x;
 }
 __device__ __forceinline__ float grad_value(const GradPowers& x, float z) {
     float y = 0.f;
-    if (x.ws != 0.f) y += x.ws * (x.soft.direct ? power<true>(x.soft, z) : power<false>(x.soft, z));
-    if (x.wh != 0.f) y += x.wh * (x.hard.direct ? power<true>(x.hard, z) : power<false>(x.hard, z));
+    if (x.ws != 0.f) y += x.ws * (x.direct ? power<true>(x.soft, z) : power<false>(x.soft, z));
+    if (x.wh != 0.f) y += x.wh * (x.direct ? power<true>(x.hard, z) : power<false>(x.hard, z));
     return y;
 }
 template <typename T, bool DIRECT, int NV>
@@ -268,7 +272,7 @@ __device__ __forceinline__ void grad_vectors(const GradPowers& g, const uint4 (&
 // The gradient in `count` vectors of a thread, `apart_by` elements from one to the next.
 template <typename T, int NV>
 __device__ __forceinline__ void put_grad(const GradPowers& g, const uint4 (&raw)[NV], T* to, int apart_by, int count, bool aligned) {
-    if (g.soft.direct && g.hard.direct) grad_vectors<T, true>(g, raw, to, apart_by, count, aligned);
+    if (g.direct) grad_vectors<T, true>(g, raw, to, apart_by, count, aligned);
     else grad_vectors<T, false>(g, raw, to, apart_by, count, aligned);
 }
 
