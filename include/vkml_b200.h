@@ -322,9 +322,9 @@ void b200_tape_destroy(b200_tape* tape);
  * not fit is refused before anything is queued.  Empty tensors are valid.
  *
  * Scratch: `workspace` is device memory of the caller, 256-byte aligned, of at least the bytes that the _workspace
- * call of the same arguments tells; NULL takes the context's own, which every call shares: a caller that captures
- * calls into CUDA graphs of its own, to be replayed beside other work, gives each graph a workspace
- * (a call that would have to grow the context's own while its stream is captured is refused). */
+ * call of the same arguments tells; NULL takes the context's own, which every call shares and a later call may move.
+ * While the context's stream is captured into a CUDA graph of the caller's, a call that needs scratch is refused
+ * without a workspace; graphs that may be replayed beside each other have one each. */
 
 /* rows[t] = scale * table[ids[t]] -- and backward, table = scale * (the sum of the rows of each
  * id), rows without a token zero, or, with B200_ACCUMULATE, added to what table holds, where rows without a token

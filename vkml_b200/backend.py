@@ -139,7 +139,7 @@ class Backend:
     # -- operators of language-model training ---------------------------------
     # Tensors are DeviceTensor or TensorDesc; results are tensors that the caller made.  Every call is ordered on the
     # backend's stream when it returns, like compute().  `workspace`: a Storage for calls that are captured into a
-    # graph of the caller's; without one the context's own scratch is used.
+    # graph of the caller's, which are refused without one; else the context's own scratch is used.
     def embedding(self, table, ids, rows, scale: float = 1.0) -> None:
         """rows[t] = scale * table[ids[t]].  table [V, D], ids of any extents up to rank 2 (I64 or I32), rows
         ids' extents and D; F32 or F16 on either side.  An id outside [0, V) reads as zeros and is an IndexError at

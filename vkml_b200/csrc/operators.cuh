@@ -233,7 +233,8 @@ inline void wait_for_tensors(b200_ctx* ctx, std::initializer_list<const b200_ten
     }
 }
 
-// The caller's workspace, or the context's own, grown where it has to be.
+// The caller's workspace, or the context's own, grown where it has to be.  A graph of the caller's would go on writing to the context's after a later call had
+// moved it, and beside whatever else uses it: a call that is captured brings its own.
 inline char* operator_workspace(b200_ctx* ctx, void* workspace, size_t have, size_t need) {
     if (need == 0) return nullptr;
     if (workspace != nullptr) {
@@ -241,13 +242,9 @@ inline char* operator_workspace(b200_ctx* ctx, void* workspace, size_t have, siz
         if (have < need) fail(B200_INVALID_ARGUMENT, "workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) + " are needed");
         return static_cast<char*>(workspace);
     }
-    if (need > ctx->workspace_bytes) {
-        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-        B200_CUDA_CHECK(cudaStreamIsCapturing(ctx->stream, &status));
-        if (status != cudaStreamCaptureStatusNone) {
-            fail(B200_INVALID_ARGUMENT, "the context's workspace would have to grow while its stream is captured: pass a workspace, or make the call once before");
-        }
-    }
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    B200_CUDA_CHECK(cudaStreamIsCapturing(ctx->stream, &status));
+    if (status != cudaStreamCaptureStatusNone) fail(B200_INVALID_ARGUMENT, "a call that is captured into a graph needs a workspace of the caller's");
     return static_cast<char*>(ctx->ensure_workspace(need));
 }
 
