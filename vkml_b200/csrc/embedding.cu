@@ -899,7 +899,6 @@ int clusters_at_once(int held, int blocks) {
     }
     return n - 1;
 }
-// (Where there is no device to ask, for the size of a workspace: the larger answer of the two is the smaller cluster's.)
 int largest_cluster() { return clusters_at_once(kMostClusterHeld, kMostCluster) > 0 ? kMostCluster : 8; }
 
 // How a gradient of many tokens is divided, and where its scratch lies.
@@ -946,7 +945,9 @@ Division divide(const Problem& p) {
         while (d.held < kMostHeld && ceil_div(p.count, int64_t(kSortThreads) * d.held) > kScannedTiles) d.held *= 2;
     }
     d.sort_tiles = static_cast<uint32_t>(ceil_div(p.count, int64_t(kSortThreads) * d.held));
-    d.count_bytes = int64_t(d.sort_tiles) * 1024 + 1024;
+    // As many as any cluster's limit asks for: what is told where there is no device, or of another one, is enough.
+    const int64_t most_tiles = p.count <= int64_t(kSortThreads) * kMostClusterHeld * kMostCluster ? ceil_div(p.count, kSortThreads) : d.sort_tiles;
+    d.count_bytes = most_tiles * 1024 + 1024;
     d.bytes = static_cast<size_t>(2 * d.token_bytes + d.touched_bytes + d.partial_bytes + d.count_bytes);
     return d;
 }
