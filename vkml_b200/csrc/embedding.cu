@@ -866,6 +866,7 @@ SortCluster sort_cluster(int held) {
 
 // How many clusters of `blocks` blocks the current device holds at once; 0 where it takes none of them.
 int clusters_at_once(int held, int blocks) {
+    static std::mutex mutex;
     static int known[64][2][5] = {};  // device, held, blocks: one more than the answer
     int dev = 0, h = 0, b = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -874,6 +875,7 @@ int clusters_at_once(int held, int blocks) {
     }
     while ((1 << h) < held) ++h;
     while ((1 << b) < blocks) ++b;
+    std::lock_guard<std::mutex> lock(mutex);
     int& n = known[dev & 63][h][b];
     if (n == 0) {
         const size_t shared = static_cast<size_t>(kSortThreads) * held * sizeof(uint2);
@@ -892,9 +894,9 @@ int clusters_at_once(int held, int blocks) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared)) != cudaSuccess ||
             (blocks > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
             cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess) {
-            fit = 0;
+            cudaGetLastError();
+            return 0;  // (not kept: the question failed, not the device)
         }
-        cudaGetLastError();
         n = fit + 1;
     }
     return n - 1;
