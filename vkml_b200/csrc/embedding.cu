@@ -143,7 +143,7 @@ owned_rows_kernel(char* table, int64_t pitch, RowsArg grad, Ids ids, uint32_t co
                 const int64_t id = ids[t];
                 if (id >= row0 && id < row0 + rows && id != padding) {
                     row[k] = id - row0;
-                } else if ((id < 0 || id >= vocab) && id != padding && blockIdx.x == 0 && blockIdx.y == 0) {
+                } else if ((id < 0 || (id >= vocab && id != padding)) && blockIdx.x == 0 && blockIdx.y == 0) {
                     atomicOr(status, kStatusIndexOutOfRange);
                 }
             }
@@ -240,7 +240,7 @@ struct SortArgs {
     uint32_t* totals;    // [256], from scan_kernel
     uint32_t* touched;   // a bit for each row, cleared here; or null
     uint32_t count, vocab, tiles, tile;  // tile: tokens of one
-    int64_t padding;
+    int64_t padding;  // below 0: none, and no id is equal to it
     int shift, bits;
     bool scanned;
     Zeros zeros;
@@ -273,7 +273,7 @@ __device__ __forceinline__ uint2 sort_token(const SortArgs& k, uint32_t i, bool 
     if (k.from != nullptr) return k.from[i];
     const int64_t id = k.ids[i];
     const bool in = id >= 0 && id < int64_t(k.vocab);
-    if (report && !in && id != k.padding) atomicOr(k.status, kStatusIndexOutOfRange);
+    if (report && !in && (id < 0 || id != k.padding)) atomicOr(k.status, kStatusIndexOutOfRange);
     return make_uint2(in && id != k.padding ? static_cast<uint32_t>(id) : k.vocab, i);
 }
 
@@ -965,7 +965,7 @@ void launch_owned_rows(b200_ctx* ctx, const b200_embedding_args& a, const Proble
         using TO = decltype(to);
         using TG = decltype(tg);
         launch_kernel(ctx, owned_rows_kernel<TG, TO>, grid, kThreads, sizeof(float) * owned * columns, static_cast<char*>(a.table.data), p.pitch, p.rows, p.ids,
-                      static_cast<uint32_t>(p.count), p.vocab, p.width, owned, columns, a.padding_id < 0 ? INT64_MIN : a.padding_id, a.scale,
+                      static_cast<uint32_t>(p.count), p.vocab, p.width, owned, columns, a.padding_id, a.scale,
                       static_cast<int>(a.flags & B200_ACCUMULATE), ctx->d_status);
     });
     check_last_launch("embedding_backward");
@@ -991,7 +991,7 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
     s.counts = s.totals + 256;
     s.count = static_cast<uint32_t>(p.count);
     s.vocab = static_cast<uint32_t>(p.vocab);
-    s.padding = a.padding_id < 0 ? INT64_MIN : a.padding_id;
+    s.padding = a.padding_id;
     s.tiles = d.sort_tiles;
     s.tile = static_cast<uint32_t>(kSortThreads * d.held);
     s.scanned = d.sort_tiles > kScannedTiles;
