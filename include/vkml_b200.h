@@ -331,7 +331,7 @@ void b200_tape_destroy(b200_tape* tape);
  * keep their bytes. */
 #define B200_ACCUMULATE 1u
 typedef struct b200_embedding_args {
-    b200_tensor table;   /* [V, D], F32 or F16: read by b200_embedding, written by its backward */
+    b200_tensor table;   /* [V, D], F32 or F16: read by b200_embedding, written by its backward (D below 2^24 there) */
     b200_tensor ids;     /* I64 or I32, any strides; an id outside [0, V) is an index error at the next
                             synchronisation: its row reads as zeros, its gradient goes nowhere */
     b200_tensor rows;    /* ids' extents and D, F32 or F16 whatever the table's type */
@@ -417,7 +417,8 @@ int b200_distill_loss(b200_ctx* ctx, const b200_distill_args* args);
 int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
 
 /* The status that one of these calls would answer its arguments with, and the reason, without a context or a device:
- * `args` is the call's struct.  What b200_supports is for nodes. */
+ * `args` is the call's struct, its workspace included.  What b200_supports is for nodes.  (What only a context knows --
+ * memory that is full, a stream that is captured -- is not told.) */
 #define B200_CALL_EMBEDDING 0
 #define B200_CALL_EMBEDDING_BACKWARD 1
 #define B200_CALL_BLOCK_NORM 2

@@ -1,0 +1,83 @@
+"""b200_check_operator tells what the call would answer: limits of extents and the workspace too, without a device."""
+import ctypes as C
+
+from test_language_refusals import DISTILL, EMBEDDING, EMBEDDING_BACKWARD, F16, F32, I32, I64, INVALID, NORM_BACKWARD, OK, SHAPE, At, answer, distill_args, grad_args
+from vkml_b200 import _abi, graph
+
+
+def size(name, args):
+    n = C.c_size_t(0)
+    status = getattr(_abi.load(), f"b200_{name}_workspace")(args, C.byref(n))
+    return n.value if status == OK else -status
+
+
+def test_rows_of_a_table():
+    at = At()
+
+    def args(width, table=F32, **k):
+        return graph.embedding_args(at((4, width), table), at((3,), I64), at((3, width), F16), 1.0, **k)
+
+    assert answer(EMBEDDING, args(1 << 24)) == OK
+    for which, width, says in ((EMBEDDING_BACKWARD, (1 << 24) - 1, OK), (EMBEDDING_BACKWARD, 1 << 24, SHAPE)):
+        assert answer(which, args(width)) == says
+        assert (size("embedding_backward", args(width)) >= 0) == (says == OK)
+
+
+def test_lookups_of_many_pieces():
+    """Blocks of 8 rows of one to 256 odd columns each."""
+    at = At()
+    says = lambda n, width: answer(EMBEDDING, graph.embedding_args(at((4, width), F32), at((n,), I64, (0,)), at((n, width), F16), 1.0))  # noqa: E731
+    assert says((1 << 31) - 1, 255) == OK
+    assert says((1 << 31) - 1, 256 * 10 - 1) == SHAPE
+
+
+def test_an_embeddings_workspace():
+    at = At()
+    tensors = at((5000, 64)), at((3000,), I64), at((3000, 64), F16)
+    need = size("embedding_backward", graph.embedding_args(*tensors, 1.0))
+    assert need > 0
+    base = 1 << 20
+
+    def says(address, nbytes):
+        return answer(EMBEDDING_BACKWARD, graph.embedding_args(*tensors, 1.0, workspace=address, workspace_bytes=nbytes))
+
+    assert says(base, need) == OK and says(base, need + 1) == OK
+    assert says(base, need - 1) == INVALID and says(base, 0) == INVALID
+    assert says(base + 128, need) == INVALID
+    assert says(0, 0) == OK and says(0, need) == OK  # the context's own
+    few = at((50, 8)), at((3,), I64), at((3, 8), F16)
+    assert size("embedding_backward", graph.embedding_args(*few, 1.0)) == 0
+    assert answer(EMBEDDING_BACKWARD, graph.embedding_args(*few, 1.0, workspace=base + 8, workspace_bytes=1)) == OK  # nothing is needed
+
+
+def test_a_norms_workspace():
+    at = At()
+    tensors = dict(zip(("out", "branch", "stats", "out_grad", "normed_grad", "residual_grad", "branch_grad"),
+                       (at((2, 3, 8)), at((2, 3, 8), F16), at((6, 4)), at((2, 3, 8)), at((2, 3, 8), F16), at((2, 3, 8)), at((2, 3, 8), F16))))
+    need = size("block_norm_backward", grad_args(at, **tensors))
+    assert need > 0
+    base = 1 << 20
+
+    def says(address, nbytes, **more):
+        return answer(NORM_BACKWARD, grad_args(at, **tensors, workspace=address, workspace_bytes=nbytes, **more))
+
+    assert says(base, need) == OK
+    assert says(base, need - 1) == INVALID and says(base, 0) == INVALID and says(base + 64, need) == INVALID
+    assert size("block_norm_backward", grad_args(at, **tensors, workspace=base, workspace_bytes=1)) == need  # the question does not ask for the answer
+    none = dict.fromkeys(("post_weight_grad", "post_bias_grad", "pre_weight_grad", "pre_bias_grad", "gate_grad"))
+    assert size("block_norm_backward", grad_args(at, **tensors, **none)) == 0
+    assert says(base + 64, 1, **none) == OK
+
+
+def test_many_long_rows_of_logits():
+    """Rows that take two blocks each, as their entries ask for: 2^30 of them are as many blocks as a launch has no room for."""
+    at = At()
+
+    def losses_alone(n, vocab, top):
+        rows = lambda width, dtype, nbytes: at((n, width), dtype, (0, nbytes))  # noqa: E731
+        return answer(DISTILL, distill_args(at, logits=rows(vocab, F16, 2), teacher_ids=rows(top, I32, 4), teacher_logits=rows(top, F32, 4), labels=None, stats=None,
+                                            losses=at((n,)), losses_grad=None, grad=None, hard_weight=0.0))
+
+    assert losses_alone(1 << 20, 20000, 1000) == OK
+    assert losses_alone(1 << 30, 20000, 1000) == SHAPE
+    assert losses_alone(1 << 30, 20000, 10) == OK  # blocks that stay take these

@@ -98,3 +98,29 @@ def test_calls_without_scratch_are_captured_without_a_workspace():
         assert np.array_equal(s[k].numpy(), want[k]), k
     rt("cudaGraphExecDestroy", execution)
     close(backend, s)
+
+
+def test_workspaces_that_are_too_small_or_not_aligned(backend):
+    """Refused before anything is queued: the results keep their bytes."""
+    s = scratch_problem(backend, 14)
+    before = {k: s[k].numpy() for k in RESULTS}
+    need = backend.embedding_backward_workspace(s["rows"], s["ids"], s["table"])
+    workspace = backend.allocate(max(need, 1 << 24))
+
+    class At:
+        def __init__(self, offset, nbytes):
+            self.data, self.nbytes = workspace.data + offset, nbytes
+
+    for bad in (At(0, 255), At(128, workspace.nbytes - 128), At(8, workspace.nbytes - 8), At(256, 0)):
+        with pytest.raises(ValueError, match="workspace"):
+            backend.embedding_backward(s["rows"], s["ids"], s["table"], workspace=bad)
+        with pytest.raises(ValueError, match="workspace"):
+            backend.block_norm_backward(s["out"], s["branch"], s["stats"], out_grad=s["rows"], residual_grad=s["dh"], post_weight_grad=s["dw"], workspace=bad)
+    backend.synchronize()
+    for k, x in before.items():
+        assert np.array_equal(s[k].numpy(), x, equal_nan=True), k
+    operators(backend, s, At(256, workspace.nbytes - 256))
+    backend.embedding_backward(s["rows"], s["ids"], s["table"], workspace=At(256, need))  # exactly enough
+    got = s["table"].numpy()
+    backend.embedding_backward(s["rows"], s["ids"], s["table"])
+    assert np.array_equal(s["table"].numpy(), got)

@@ -917,8 +917,18 @@ Shape check_backward(const b200_block_norm_grad_args& a) {
     return p;
 }
 
-void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
+// What a backward call asks of its arguments, its workspace included.
+Shape check_division(const b200_block_norm_grad_args& a, Division& d) {
     const Shape p = check_backward(a);
+    if (p.s.rows == 0 || p.width == 0) return p;
+    d = divide(a, p, sm_count());
+    check_workspace(a.workspace, a.workspace_bytes, d.bytes);
+    return p;
+}
+
+void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
+    Division d{};
+    const Shape p = check_division(a, d);
     const b200_tensor* vectors[kSums] = {&a.gate_grad, &a.post_weight_grad, &a.post_bias_grad, &a.pre_weight_grad, &a.pre_bias_grad};
     if (p.width == 0) return;
     wait_for_tensors(ctx, {&a.out, &a.branch, &a.stats, &a.out_grad, &a.normed_grad, &a.post_weight, &a.post_bias, &a.gate, &a.pre_weight, &a.residual_grad, &a.branch_grad,
@@ -929,8 +939,7 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
         }
         return;
     }
-    const Division d = divide(a, p, sm_count());
-    char* scratch = operator_workspace(ctx, a.workspace, a.workspace_bytes, d.bytes);
+    char* scratch = operator_workspace(ctx, a.workspace, d.bytes);
     BackwardArgs k{};
     auto rows = [&](const b200_tensor& t) { return rows_arg(t, present(t) ? p.axes : 0); };
     k.out = rows(a.out);
@@ -1021,7 +1030,10 @@ void check_block_norm(const b200_block_norm_args& a) {
     int columns = -1;
     (void)check_forward(a, columns);
 }
-void check_block_norm_backward(const b200_block_norm_grad_args& a) { (void)check_backward(a); }
+void check_block_norm_backward(const b200_block_norm_grad_args& a) {
+    Division d{};
+    (void)check_division(a, d);
+}
 
 }  // namespace b200
 

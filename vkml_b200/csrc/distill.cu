@@ -900,7 +900,31 @@ struct Plan {
     int64_t vocab, top;
     RowShape s;
     bool labelled;
+    int64_t row_vectors;
+    bool many_rows;       // blocks that stay take one row after another
+    int threads, blocks;  // else: of a block, and blocks to a row
 };
+
+// How a call's rows are divided.
+void divide(Plan& plan, bool forward, bool grad, bool half) {
+    // Many rows of at least 16 KB each: blocks that stay take one row after another.  (Below, a block's warps have little to do between a row's meetings.)  Not where
+    // a row's entries take a teacher's warp longer than its logits take the others: 2048 x 16384 F16, gradient: 64 entries 39 us and 45 by a block to a row, 256
+    // entries 86 and 61; losses and gradient: 256 entries 94 and 88, 1000 276 and 174; losses alone: 256 entries 36 and 36, 1000 92 and 61.
+    const int64_t vectors = plan.row_vectors = ceil_div(plan.vocab, half ? 8 : 4);
+    plan.many_rows = plan.s.rows >= int64_t(sm_count()) * kRowBlocks && vectors >= std::max<int64_t>(kRowThreads * 4, plan.top * (!forward ? 16 : grad ? 6 : 4));
+    if (plan.many_rows) return;
+    // 256 threads and a cluster of up to 4, so that an SM has four blocks in different states; longer rows 512 threads and a cluster of up to 8.  Where there
+    // are fewer rows than SMs, a cluster as large as leaves a thread a vector.
+    int threads = 256, blocks = 1;
+    while (blocks < 4 && vectors > int64_t(blocks) * threads * kVectors) blocks *= 2;
+    if (vectors > int64_t(blocks) * threads * kVectors) threads = kMostThreads;
+    while (blocks < 8 && vectors > int64_t(blocks) * threads * kVectors) blocks *= 2;
+    while (blocks < 8 && plan.s.rows * blocks * 2 <= sm_count() && vectors > int64_t(blocks) * threads) blocks *= 2;
+    while (threads > 64 && plan.s.rows * blocks > sm_count() && int64_t(blocks) * (threads / 2) * 4 >= vectors) threads /= 2;
+    plan.threads = threads;
+    plan.blocks = blocks;
+    if (plan.s.rows * blocks >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "distill_loss: too many rows of this length");
+}
 
 Plan check_distill(const b200_distill_args& a, bool forward) {
     check_rows(a.logits, "logits");
@@ -952,12 +976,13 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
         check_results({{&a.grad, "grad"}}, {{&a.teacher_ids, "teacher_ids"}, {&a.teacher_logits, "teacher_logits"}, {&a.labels, "labels"}, {&a.losses_grad, "losses_grad"},
                                             {&a.stats, "stats"}}, {{&a.logits, "logits"}});
     }
-    const Plan plan{axes, vocab, top, s, labelled};
+    Plan plan{axes, vocab, top, s, labelled, 0, false, 0, 0};
     if (s.rows == 0) return plan;
     if (labelled && !present(a.labels)) fail(B200_INVALID_ARGUMENT, "labels have no storage");
     if (forward && !present(a.losses) && !present(a.stats) && !present(a.grad)) fail(B200_INVALID_ARGUMENT, "distill_loss: no result is asked for");
     if (!forward && (!present(a.grad) || !present(a.stats))) fail(B200_INVALID_ARGUMENT, "distill_loss_backward: grad and the forward call's stats are needed");
     if (a.hard_weight > 0.f && !labelled) fail(B200_INVALID_ARGUMENT, "distill_loss: a hard weight without labels");
+    divide(plan, forward, present(a.grad), a.logits.dtype == B200_F16);
     return plan;
 }
 
@@ -995,13 +1020,9 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
     k.slots = present(a.grad) ? table_slots(static_cast<int>(top)) : 0;
     const size_t shared = static_cast<size_t>(entry_words(static_cast<int>(top)) + k.slots) * 4;
     const bool half = a.logits.dtype == B200_F16;
-    // Many rows of at least 16 KB each: blocks that stay take one row after another.  (Below, a block's warps have little to do between a row's meetings.)  Not where
-    // a row's entries take a teacher's warp longer than its logits take the others: 2048 x 16384 F16, gradient: 64 entries 39 us and 45 by a block to a row, 256
-    // entries 86 and 61; losses and gradient: 256 entries 94 and 88, 1000 276 and 174; losses alone: 256 entries 36 and 36, 1000 92 and 61.
-    const int64_t row_vectors = ceil_div(vocab, half ? 8 : 4);
-    if (s.rows >= int64_t(sm_count()) * kRowBlocks && row_vectors >= std::max<int64_t>(kRowThreads * 4, top * (!forward ? 16 : present(a.grad) ? 6 : 4))) {
+    if (plan.many_rows) {
         RingArgs ring{};
-        const int64_t whole = ceil_div(row_vectors, kRowThreads);
+        const int64_t whole = ceil_div(plan.row_vectors, kRowThreads);
         const int most = static_cast<int>((kRowShared - kTeachers * shared) / (kRowThreads * 16));  // vectors of a thread
         ring.held = forward && present(a.grad) && whole <= most;
         ring.chunk = ring.held ? static_cast<int>(whole) : most >= 4 * kBatch ? 2 * kBatch : kBatch;
@@ -1019,18 +1040,8 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
         ctx->count_launch();
         return;
     }
-    // 256 threads and a cluster of up to 4, so that an SM has four blocks in different states; longer rows 512 threads and a cluster of up to 8.  Where there
-    // are fewer rows than SMs, a cluster as large as leaves a thread a vector.
-    const int64_t vectors = row_vectors;
-    int threads = 256, blocks = 1;
-    while (blocks < 4 && vectors > int64_t(blocks) * threads * kVectors) blocks *= 2;
-    if (vectors > int64_t(blocks) * threads * kVectors) threads = kMostThreads;
-    while (blocks < 8 && vectors > int64_t(blocks) * threads * kVectors) blocks *= 2;
-    while (blocks < 8 && s.rows * blocks * 2 <= sm_count() && vectors > int64_t(blocks) * threads) blocks *= 2;
-    while (threads > 64 && s.rows * blocks > sm_count() && int64_t(blocks) * (threads / 2) * 4 >= vectors) threads /= 2;
-    k.blocks = blocks;
+    const int blocks = k.blocks = plan.blocks, threads = plan.threads;
     const int64_t grid = s.rows * blocks;
-    if (grid >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "distill_loss: too many rows of this length");
     auto go = [&](auto kernel) {
         if (blocks == 1 || !forward) launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, k);
         else launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(grid)), dim3(threads), shared, blocks, false, k);

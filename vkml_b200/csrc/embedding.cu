@@ -796,6 +796,8 @@ struct Problem {
     int64_t count, vocab, width, pitch;
     Ids ids;
     RowsArg rows;
+    bool wide;               // rows and table hold whole eights on their boundaries
+    int64_t pieces, blocks;  // of a lookup: pieces of a row, and blocks of all of them
 };
 
 // What both directions ask of their arguments.
@@ -826,6 +828,11 @@ Problem check_embedding(const b200_embedding_args& a, bool backward) {
     const b200_tensor none{}, scratch = backward ? workspace_tensor(a.workspace, a.workspace_bytes) : none;
     if (backward) check_results({{&a.table, "table"}, {&scratch, "workspace"}}, {{&a.ids, "ids"}, {&a.rows, "rows"}}, {});
     else check_results({{&a.rows, "rows"}}, {{&a.ids, "ids"}, {&a.table, "table"}}, {});
+    p.wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
+    p.pieces = p.wide ? p.width / 8 : ceil_div(p.width, kStretch);
+    p.blocks = ceil_div(p.count * p.pieces, p.wide ? kThreads * kItems : kThreads / 32);
+    if (!backward && p.blocks >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "embedding: too many elements");
+    if (backward && p.vocab != 0 && p.width >= int64_t(1) << 24) fail(B200_SHAPE_ERROR, "embedding_backward: a row of 2^24 elements or more");
     return p;
 }
 
@@ -841,18 +848,15 @@ void launch_lookup(b200_ctx* ctx, const b200_embedding_args& a) {
     const Problem p = check_embedding(a, false);
     if (p.count == 0 || p.width == 0) return;
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
-    const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
-    const int64_t pieces = wide ? p.width / 8 : ceil_div(p.width, kStretch), total = p.count * pieces;
-    const int64_t blocks = ceil_div(total, wide ? kThreads * kItems : kThreads / 32);
-    if (blocks >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "embedding: too many elements");
     ProfScope scope(ctx, "embedding");
     const char* table = static_cast<const char*>(a.table.data);
-    const FastDiv by(static_cast<uint32_t>(pieces));
+    const FastDiv by(static_cast<uint32_t>(p.pieces));
+    const int64_t total = p.count * p.pieces;
     with_types(a.table.dtype, a.rows.dtype, [&](auto ti, auto to) {
         using TI = decltype(ti);
         using TO = decltype(to);
-        const dim3 grid(static_cast<unsigned>(blocks));
-        if (wide) launch_kernel(ctx, lookup_kernel<TI, TO>, grid, kThreads, 0, p.rows, table, p.pitch, p.ids, p.vocab, by, total, a.scale, ctx->d_status);
+        const dim3 grid(static_cast<unsigned>(p.blocks));
+        if (p.wide) launch_kernel(ctx, lookup_kernel<TI, TO>, grid, kThreads, 0, p.rows, table, p.pitch, p.ids, p.vocab, by, total, a.scale, ctx->d_status);
         else launch_kernel(ctx, lookup_any_kernel<TI, TO>, grid, kThreads, 0, p.rows, table, p.pitch, p.ids, p.vocab, p.width, by, total, a.scale, ctx->d_status);
     });
     check_last_launch("embedding");
@@ -976,7 +980,7 @@ void launch_owned_rows(b200_ctx* ctx, const b200_embedding_args& a, const Proble
 constexpr int64_t kZerosBesideKernel = int64_t(20) << 20, kZerosBesideCluster = int64_t(48) << 20;
 
 void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p, const Division& d) {
-    char* scratch = operator_workspace(ctx, a.workspace, a.workspace_bytes, d.bytes);
+    char* scratch = operator_workspace(ctx, a.workspace, d.bytes);
     const bool accumulate = (a.flags & B200_ACCUMULATE) != 0;
     const int64_t size = static_cast<int64_t>(dtype_size(a.table.dtype)), row_bytes = p.width * size;
     uint2* buffer[2] = {reinterpret_cast<uint2*>(scratch), reinterpret_cast<uint2*>(scratch + d.token_bytes)};
@@ -1068,11 +1072,10 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
     k.zero_words = static_cast<uint32_t>(std::max<int64_t>(1, (128 << 10) / (32 * row_bytes)));
     k.join_blocks = static_cast<uint32_t>((d.blocks - 1) * ceil_div(p.width, kJoinColumns));
     const uint32_t last_blocks = k.join_blocks + static_cast<uint32_t>(ceil_div(ceil_div(int64_t(zeros_left), 32), int64_t(k.zero_words)));
-    const bool wide = p.width % 8 == 0 && aligned_rows(p.rows, a.rows.dtype) && aligned_rows(RowsArg{static_cast<char*>(a.table.data), 0, p.pitch}, a.table.dtype);
     with_types(a.table.dtype, a.rows.dtype, [&](auto to, auto tg) {
         using TO = decltype(to);
         using TG = decltype(tg);
-        launch_kernel(ctx, wide ? sum_tokens_kernel<TG, TO, true> : sum_tokens_kernel<TG, TO, false>, dim3(d.blocks * static_cast<uint32_t>(d.tiles)), kSumThreads, 0, k);
+        launch_kernel(ctx, p.wide ? sum_tokens_kernel<TG, TO, true> : sum_tokens_kernel<TG, TO, false>, dim3(d.blocks * static_cast<uint32_t>(d.tiles)), kSumThreads, 0, k);
         check_last_launch("embedding_backward");
         if (last_blocks > 0) launch_kernel(ctx, join_kernel<TO>, dim3(last_blocks), kJoinThreads * kJoinGroups, 0, k);
     });
@@ -1080,20 +1083,31 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
     ctx->count_launch(last_blocks > 0 ? 2 : 1);
 }
 
-void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
+// What a gradient's call asks of its arguments, its workspace included.
+Problem check_gradient(const b200_embedding_args& a, Division& d) {
     const Problem p = check_embedding(a, true);
+    d = divide(p);
+    check_workspace(a.workspace, a.workspace_bytes, d.bytes);
+    return p;
+}
+
+void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
+    Division d;
+    const Problem p = check_gradient(a, d);
     if (p.vocab == 0 || p.width == 0) return;
-    if (p.width >= int64_t(1) << 24) fail(B200_SHAPE_ERROR, "embedding_backward: a row of 2^24 elements or more");
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
     ProfScope scope(ctx, "embedding_backward");
-    const Division d = divide(p);
     if (d.bytes == 0) launch_owned_rows(ctx, a, p);
     else launch_sorted(ctx, a, p, d);
 }
 
 }  // namespace
 
-void check_embedding_call(const b200_embedding_args& a, bool backward) { (void)check_embedding(a, backward); }
+void check_embedding_call(const b200_embedding_args& a, bool backward) {
+    Division d;
+    if (backward) (void)check_gradient(a, d);
+    else (void)check_embedding(a, false);
+}
 
 }  // namespace b200
 

@@ -233,15 +233,18 @@ inline void wait_for_tensors(b200_ctx* ctx, std::initializer_list<const b200_ten
     }
 }
 
-// The caller's workspace, or the context's own, grown where it has to be.  A graph of the caller's would go on writing to the context's after a later call had
+// A caller's workspace, where a call needs one of `need` bytes.
+inline void check_workspace(const void* workspace, size_t have, size_t need) {
+    if (need == 0 || workspace == nullptr) return;
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) fail(B200_INVALID_ARGUMENT, "workspace is not 256-byte aligned");
+    if (have < need) fail(B200_INVALID_ARGUMENT, "workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) + " are needed");
+}
+
+// The caller's workspace (checked), or the context's own, grown where it has to be.  A graph of the caller's would go on writing to the context's after a later call had
 // moved it, and beside whatever else uses it: a call that is captured brings its own.
-inline char* operator_workspace(b200_ctx* ctx, void* workspace, size_t have, size_t need) {
+inline char* operator_workspace(b200_ctx* ctx, void* workspace, size_t need) {
     if (need == 0) return nullptr;
-    if (workspace != nullptr) {
-        if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) fail(B200_INVALID_ARGUMENT, "workspace is not 256-byte aligned");
-        if (have < need) fail(B200_INVALID_ARGUMENT, "workspace has " + std::to_string(have) + " bytes, " + std::to_string(need) + " are needed");
-        return static_cast<char*>(workspace);
-    }
+    if (workspace != nullptr) return static_cast<char*>(workspace);
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     B200_CUDA_CHECK(cudaStreamIsCapturing(ctx->stream, &status));
     if (status != cudaStreamCaptureStatusNone) fail(B200_INVALID_ARGUMENT, "a call that is captured into a graph needs a workspace of the caller's");
