@@ -1,8 +1,9 @@
 """b200_check_operator tells what the call would answer: limits of extents and the workspace too, without a device."""
 import ctypes as C
 
-from test_language_refusals import DISTILL, EMBEDDING, EMBEDDING_BACKWARD, F16, F32, I32, I64, INVALID, NORM_BACKWARD, OK, SHAPE, At, answer, distill_args, grad_args
-from vkml_b200 import _abi, graph
+from test_language_refusals import (DISTILL, DISTILL_BACKWARD, EMBEDDING, EMBEDDING_BACKWARD, F16, F32, I32, I64, INVALID, NORM, NORM_BACKWARD, OK, SHAPE, At, answer,
+                                    distill_args, grad_args, norm_args)
+from vkml_b200 import TensorDesc, _abi, graph
 
 
 def size(name, args):
@@ -81,3 +82,19 @@ def test_many_long_rows_of_logits():
     assert losses_alone(1 << 20, 20000, 1000) == OK
     assert losses_alone(1 << 30, 20000, 1000) == SHAPE
     assert losses_alone(1 << 30, 20000, 10) == OK  # blocks that stay take these
+
+
+def without_storage(t):
+    return TensorDesc(0, t.dims, t.strides, t.dtype)
+
+
+def test_rows_of_no_element_need_no_storage():
+    """Weights of their norms are as welcome as with rows, and gradients of sums of nothing."""
+    at = At()
+    h, y = (without_storage(at((0, 8), dtype)) for dtype in (F32, F16))
+    assert answer(NORM, norm_args(at, residual=h, branch=y, out=h, normed=y, stats=None, gate=at((8,)))) == OK
+    assert answer(NORM, norm_args(at, residual=h, branch=None, out=h, normed=y, stats=None, gate=None, flags=0, post_weight=None, post_bias=None)) == OK
+    assert answer(NORM_BACKWARD, grad_args(at, out=h, branch=y, out_grad=h, normed_grad=y, residual_grad=h, branch_grad=y, stats=None, gate=at((8,)), gate_grad=at((8,)))) == OK
+    assert answer(NORM, norm_args(at, residual=without_storage(at((0, 9))))) == SHAPE
+    no_width = {k: without_storage(at((2, 3, 0), F16 if k in ("branch", "normed") else F32)) for k in ("residual", "branch", "out", "normed")}
+    assert answer(NORM, norm_args(at, **no_width, **{k: without_storage(at((0,))) for k in ("post_weight", "post_bias", "pre_weight", "pre_bias", "gate")})) == OK

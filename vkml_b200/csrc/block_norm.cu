@@ -719,6 +719,8 @@ Shape check_sides(std::initializer_list<Named> residual_side, std::initializer_l
 }
 
 bool present(const b200_tensor& t) { return t.data != nullptr; }
+// Rows of no element have no storage, and are there all the same.  (For tensors that check_sides has looked at.)
+bool given(const b200_tensor& t) { return present(t) || (t.ndim != 0 && numel_of(t) == 0); }
 
 // Weights, biases and gate, or their gradients: one type, dense, of the rows' width.  The gate has a row for each of its groups.
 int check_columns(std::initializer_list<Named> vectors, const Named& gate, Shape& p) {
@@ -756,9 +758,9 @@ bool aligned_columns(const void* p) { return reinterpret_cast<uintptr_t>(p) % 32
 Shape check_forward(const b200_block_norm_args& a, int& columns) {
     Shape p = check_sides({{&a.residual, "residual"}, {&a.out, "out"}}, {{&a.branch, "branch"}, {&a.normed, "normed"}}, a.kind, a.flags);
     columns = check_columns({{&a.post_weight, "post_weight"}, {&a.post_bias, "post_bias"}, {&a.pre_weight, "pre_weight"}, {&a.pre_bias, "pre_bias"}}, {&a.gate, "gate"}, p);
-    if (!present(a.branch) && (present(a.gate) || (a.flags & B200_NORM_POST) != 0)) fail(B200_INVALID_ARGUMENT, "block_norm: a gate or a norm of an absent branch");
+    if (!given(a.branch) && (present(a.gate) || (a.flags & B200_NORM_POST) != 0)) fail(B200_INVALID_ARGUMENT, "block_norm: a gate or a norm of an absent branch");
     if ((a.flags & B200_NORM_POST) == 0 && (present(a.post_weight) || present(a.post_bias))) fail(B200_INVALID_ARGUMENT, "block_norm: weights of a norm that is not applied");
-    if (!present(a.normed) && (present(a.pre_weight) || present(a.pre_bias))) fail(B200_INVALID_ARGUMENT, "block_norm: weights of a norm that is not applied");
+    if (!given(a.normed) && (present(a.pre_weight) || present(a.pre_bias))) fail(B200_INVALID_ARGUMENT, "block_norm: weights of a norm that is not applied");
     if (present(a.stats)) check_stats(a.stats, p.s.rows);
     check_results({{&a.out, "out"}, {&a.normed, "normed"}, {&a.stats, "stats"}},
                   {{&a.post_weight, "post_weight"}, {&a.post_bias, "post_bias"}, {&a.pre_weight, "pre_weight"}, {&a.pre_bias, "pre_bias"}, {&a.gate, "gate"}},
@@ -893,7 +895,7 @@ Shape check_backward(const b200_block_norm_grad_args& a) {
                    {&a.pre_bias_grad, "pre_bias_grad"}}, {&a.gate_grad, "gate_grad"}, p);
     if (present(a.gate) && present(a.gate_grad) && gates != p.gates) fail(B200_SHAPE_ERROR, "gate_grad has not the gate's extents");
     if (present(a.gate)) p.gates = gates;
-    const bool post = (a.flags & B200_NORM_POST) != 0, pre = present(a.normed_grad);
+    const bool post = (a.flags & B200_NORM_POST) != 0, pre = given(a.normed_grad);
     if (!post && (present(a.post_weight) || present(a.post_bias) || present(a.post_weight_grad) || present(a.post_bias_grad))) {
         fail(B200_INVALID_ARGUMENT, "block_norm_backward: weights of a norm that is not applied");
     }
