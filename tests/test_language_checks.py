@@ -98,3 +98,24 @@ def test_rows_of_no_element_need_no_storage():
     assert answer(NORM, norm_args(at, residual=without_storage(at((0, 9))))) == SHAPE
     no_width = {k: without_storage(at((2, 3, 0), F16 if k in ("branch", "normed") else F32)) for k in ("residual", "branch", "out", "normed")}
     assert answer(NORM, norm_args(at, **no_width, **{k: without_storage(at((0,))) for k in ("post_weight", "post_bias", "pre_weight", "pre_bias", "gate")})) == OK
+
+
+def test_a_tensor_without_storage_is_absent_whatever_its_extents():
+    """Where a call can do without it: its extents are then those of nothing."""
+    at = At()
+    for name in ("residual", "stats", "out", "post_weight", "post_bias", "pre_weight", "pre_bias", "gate"):
+        for dims in ((2, 3, 8), (7,), (3, 5, 9, 2)):
+            assert answer(NORM, norm_args(at, **{name: without_storage(at(dims))})) == OK, (name, dims)
+    none = without_storage(at((2, 3, 8), F16))
+    assert answer(NORM, norm_args(at, branch=none)) == INVALID  # a gate of nothing
+    assert answer(NORM, norm_args(at, branch=none, gate=none, flags=0, post_weight=none, post_bias=none)) == OK
+    assert answer(NORM, norm_args(at, branch=none, residual=none, gate=none, flags=0, post_weight=none, post_bias=none)) == INVALID
+    for name in ("out_grad", "residual_grad", "branch_grad", "gate_grad", "post_bias", "pre_bias_grad"):
+        assert answer(NORM_BACKWARD, grad_args(at, **{name: without_storage(at((2, 3, 8)))})) == OK, name
+    for which, losses in ((DISTILL, at((2, 3))), (DISTILL_BACKWARD, without_storage(at((2, 3))))):
+        for name in ("labels", "losses_grad"):
+            absent = {name: without_storage(at((2, 3), I64 if name == "labels" else F32))}
+            assert answer(which, distill_args(at, losses=losses, **absent, hard_weight=0.0)) == OK, name
+        assert answer(which, distill_args(at, losses=losses, labels=without_storage(at((2, 3), I64)))) == INVALID  # a weight of nothing
+    # what a call cannot do without
+    assert answer(DISTILL, distill_args(at, logits=without_storage(at((2, 3, 50), F16)))) == INVALID

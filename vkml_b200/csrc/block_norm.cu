@@ -694,7 +694,7 @@ Shape check_sides(std::initializer_list<Named> residual_side, std::initializer_l
     int side = 0;
     for (const auto& list : {residual_side, branch_side}) {
         for (const Named& n : list) {
-            if (n.t->data == nullptr && n.t->ndim == 0) continue;
+            if (is_absent(*n.t, n.name)) continue;
             check_rows(*n.t, n.name);
             if (like == nullptr) like = n.t;
             if (n.t->ndim != like->ndim || !same_extents(*n.t, *like, like->ndim)) fail(B200_SHAPE_ERROR, std::string(n.name) + ": rows of other extents");

@@ -946,7 +946,7 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
         fail(B200_INVALID_ARGUMENT, "distill_loss: the temperature is not above 0 and finite, or its inverse is not");
     }
     if (!(a.hard_weight >= 0.f && a.hard_weight <= 1.f)) fail(B200_INVALID_ARGUMENT, "distill_loss: the hard weight is not in 0..1");
-    const bool labelled = a.labels.data != nullptr || a.labels.ndim != 0;
+    const bool labelled = !is_absent(a.labels, "labels");
     if (labelled) {
         check_scalar_rows(a.labels, "labels", a.logits);
         if (!is_index(a.labels.dtype)) fail(B200_DTYPE_ERROR, "labels are I32 or I64");
@@ -978,7 +978,6 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
     }
     Plan plan{axes, vocab, top, s, labelled, 0, false, 0, 0};
     if (s.rows == 0) return plan;
-    if (labelled && !present(a.labels)) fail(B200_INVALID_ARGUMENT, "labels have no storage");
     if (forward && !present(a.losses) && !present(a.stats) && !present(a.grad)) fail(B200_INVALID_ARGUMENT, "distill_loss: no result is asked for");
     if (!forward && (!present(a.grad) || !present(a.stats))) fail(B200_INVALID_ARGUMENT, "distill_loss_backward: grad and the forward call's stats are needed");
     if (a.hard_weight > 0.f && !labelled) fail(B200_INVALID_ARGUMENT, "distill_loss: a hard weight without labels");

@@ -156,6 +156,14 @@ inline void check_rows(const b200_tensor& t, const char* name) {
     if (s.rows >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, std::string(name) + ": more than 2^31 - 1 rows");
 }
 
+// Whether a tensor that a call can do without is not there: no storage.  (One of no elements has none either, and still says what its extents are.)
+inline bool is_absent(const b200_tensor& t, const char* name) {
+    if (t.data != nullptr) return false;
+    if (t.ndim == 0) return true;
+    check_tensor(t, name);
+    return numel_of(t) != 0;
+}
+
 // Whether two views may have an element in common.  Ranges of addresses that do not meet settle it; where they do (columns of one
 // buffer, say), every run of consecutive elements of a view starts at its address plus a multiple of g, the greatest common divisor of all strides
 // between runs: runs whose places modulo g do not meet never meet.
