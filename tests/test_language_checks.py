@@ -119,3 +119,11 @@ def test_a_tensor_without_storage_is_absent_whatever_its_extents():
         assert answer(which, distill_args(at, losses=losses, labels=without_storage(at((2, 3), I64)))) == INVALID  # a weight of nothing
     # what a call cannot do without
     assert answer(DISTILL, distill_args(at, logits=without_storage(at((2, 3, 50), F16)))) == INVALID
+
+
+def test_temperatures_whose_inverse_times_log2_e_is_not_finite():
+    """The smallest temperature is log2(e) / the largest float, 4.24e-39: a logit's exponent is taken by that product."""
+    at = At()
+    for which, losses in ((DISTILL, at((2, 3))), (DISTILL_BACKWARD, None)):
+        for temperature, says in ((2.95e-39, INVALID), (4.2e-39, INVALID), (4.3e-39, OK), (1e-30, OK), (3e38, OK)):
+            assert answer(which, distill_args(at, losses=losses, temperature=temperature)) == says, temperature

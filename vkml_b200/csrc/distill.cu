@@ -942,8 +942,8 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
     if (top > kMostTop) fail(B200_NOT_IMPLEMENTED, "distill_loss: more than 1024 of the teacher's logits");
     if (vocab < 1 || vocab >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "logits: rows of no element, or of 2^31 or more");
     const RowShape s = row_shape(a.logits, axes);
-    if (!(a.temperature > 0.f) || std::isinf(a.temperature) || std::isinf(1.f / a.temperature)) {
-        fail(B200_INVALID_ARGUMENT, "distill_loss: the temperature is not above 0 and finite, or its inverse is not");
+    if (!(a.temperature > 0.f) || std::isinf(a.temperature) || std::isinf(1.f / a.temperature * kLog2e)) {
+        fail(B200_INVALID_ARGUMENT, "distill_loss: the temperature is not above 0 and finite, or its inverse times log2 e is not");
     }
     if (!(a.hard_weight >= 0.f && a.hard_weight <= 1.f)) fail(B200_INVALID_ARGUMENT, "distill_loss: the hard weight is not in 0..1");
     const bool labelled = !is_absent(a.labels, "labels");
