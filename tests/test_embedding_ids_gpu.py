@@ -27,3 +27,15 @@ def test_the_types_ends_are_out_of_range(backend, count, dtype, end, padding):
     backend.embedding_backward(g, i, t, padding_id=-int(2 ** 63))  # the type's lowest value as a padding id: none
     with pytest.raises(IndexError):
         backend.synchronize()
+
+
+def test_one_token_of_its_own(backend):
+    """An id without extents: its row of the gradient is the token's, the others are zeros; added to what is there, theirs stay."""
+    row, ids = np.array([1.5, -2.0, 0.25, 3.0], np.float32), np.array(2, np.int32)
+    for before in (None, np.arange(12, dtype=np.float32).reshape(3, 4)):
+        table = np.full((3, 4), np.nan, np.float32) if before is None else before.copy()
+        space = Space(backend)
+        backend.embedding_backward(space.put(row), space.put(ids), space.put(table), scale=2.0, accumulate=before is not None)
+        want = np.zeros((3, 4), np.float32) if before is None else before.copy()
+        want[2] += 2 * row
+        assert np.array_equal(space.get(table)[0], want)
