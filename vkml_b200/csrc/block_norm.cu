@@ -919,18 +919,10 @@ Shape check_backward(const b200_block_norm_grad_args& a) {
     return p;
 }
 
-// What a backward call asks of its arguments, its workspace included.
-Shape check_division(const b200_block_norm_grad_args& a, Division& d) {
-    const Shape p = check_backward(a);
-    if (p.s.rows == 0 || p.width == 0) return p;
-    d = divide(a, p, sm_count());
-    check_workspace(a.workspace, a.workspace_bytes, d.bytes);
-    return p;
-}
-
 void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
-    Division d{};
-    const Shape p = check_division(a, d);
+    const Shape p = check_backward(a);
+    const Division d = p.s.rows != 0 && p.width != 0 ? divide(a, p, sm_count()) : Division{};
+    check_workspace(a.workspace, a.workspace_bytes, d.bytes);
     const b200_tensor* vectors[kSums] = {&a.gate_grad, &a.post_weight_grad, &a.post_bias_grad, &a.pre_weight_grad, &a.pre_bias_grad};
     if (p.width == 0) return;
     wait_for_tensors(ctx, {&a.out, &a.branch, &a.stats, &a.out_grad, &a.normed_grad, &a.post_weight, &a.post_bias, &a.gate, &a.pre_weight, &a.residual_grad, &a.branch_grad,
@@ -1033,8 +1025,8 @@ void check_block_norm(const b200_block_norm_args& a) {
     (void)check_forward(a, columns);
 }
 void check_block_norm_backward(const b200_block_norm_grad_args& a) {
-    Division d{};
-    (void)check_division(a, d);
+    const Shape p = check_backward(a);
+    if (a.workspace != nullptr && p.s.rows != 0 && p.width != 0) check_workspace(a.workspace, a.workspace_bytes, divide(a, p, sm_count()).bytes);
 }
 
 }  // namespace b200

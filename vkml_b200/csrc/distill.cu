@@ -976,17 +976,17 @@ Plan check_distill(const b200_distill_args& a, bool forward) {
         check_results({{&a.grad, "grad"}}, {{&a.teacher_ids, "teacher_ids"}, {&a.teacher_logits, "teacher_logits"}, {&a.labels, "labels"}, {&a.losses_grad, "losses_grad"},
                                             {&a.stats, "stats"}}, {{&a.logits, "logits"}});
     }
-    Plan plan{axes, vocab, top, s, labelled, 0, false, 0, 0};
+    const Plan plan{axes, vocab, top, s, labelled, 0, false, 0, 0};
     if (s.rows == 0) return plan;
     if (forward && !present(a.losses) && !present(a.stats) && !present(a.grad)) fail(B200_INVALID_ARGUMENT, "distill_loss: no result is asked for");
     if (!forward && (!present(a.grad) || !present(a.stats))) fail(B200_INVALID_ARGUMENT, "distill_loss_backward: grad and the forward call's stats are needed");
     if (a.hard_weight > 0.f && !labelled) fail(B200_INVALID_ARGUMENT, "distill_loss: a hard weight without labels");
-    divide(plan, forward, present(a.grad), a.logits.dtype == B200_F16);
     return plan;
 }
 
 void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
-    const Plan plan = check_distill(a, forward);
+    Plan plan = check_distill(a, forward);
+    divide(plan, forward, present(a.grad), a.logits.dtype == B200_F16);
     const int axes = plan.axes;
     const int64_t vocab = plan.vocab, top = plan.top;
     const RowShape s = plan.s;
@@ -1054,7 +1054,10 @@ void launch_distill(b200_ctx* ctx, const b200_distill_args& a, bool forward) {
 
 }  // namespace
 
-void check_distill_loss(const b200_distill_args& a, bool forward) { (void)check_distill(a, forward); }
+void check_distill_loss(const b200_distill_args& a, bool forward) {
+    Plan plan = check_distill(a, forward);
+    if (plan.s.rows >= int64_t(1) << 28) divide(plan, forward, present(a.grad), a.logits.dtype == B200_F16);  // (fewer rows, of up to 8 blocks each, always fit)
+}
 
 }  // namespace b200
 

@@ -911,7 +911,7 @@ int largest_cluster() { return clusters_at_once(kMostClusterHeld, kMostCluster) 
 struct Division {
     uint32_t chunk, chunks, blocks;
     int threads, tiles;
-    int held;             // tokens of a thread that sorts
+    int held;             // (from choose_sort) tokens of a thread that sorts
     int cluster;          // blocks of the cluster that sorts; 0: many blocks
     uint32_t sort_tiles;
     int64_t token_bytes, touched_bytes, partial_bytes, count_bytes;
@@ -922,6 +922,15 @@ struct Division {
 // zeros are written.  (F32, owned and sorted: 128 tokens of 1000 x 64 5.5 us and 12.3, 512 tokens 13.5 and 13.7; of 1000 x 512 9.7 and 14.4, 27.6 and 14.4; 8 tokens
 // of 50000 x 128 13.9 and 12.3, of 50000 x 1024 77.8 and 41.2.)
 bool is_owned(int64_t count, int64_t elements) { return (count <= 128 && elements <= 1 << 22) || (count <= 512 && elements <= 1 << 17); }
+
+constexpr int64_t kMostClusterTokens = int64_t(kSortThreads) * kMostClusterHeld * kMostCluster;
+
+// Tokens of a thread where many blocks sort: few tiles, as every block adds up the counts of all; but eight at most.
+int tokens_held(int64_t count) {
+    int held = 1;
+    while (held < kMostHeld && ceil_div(count, int64_t(kSortThreads) * held) > kScannedTiles) held *= 2;
+    return held;
+}
 
 Division divide(const Problem& p) {
     Division d{};
@@ -939,23 +948,27 @@ Division divide(const Problem& p) {
     d.token_bytes = whole(p.count * 8);
     d.touched_bytes = whole(ceil_div(p.vocab, 32) * 4);
     d.partial_bytes = whole(int64_t(d.blocks) * 2 * p.width * 4);
+    // As many tiles as any way to sort asks for, whatever clusters the device takes.
+    const int64_t most_tiles = p.count <= kMostClusterTokens ? ceil_div(p.count, kSortThreads) : ceil_div(p.count, int64_t(kSortThreads) * tokens_held(p.count));
+    d.count_bytes = most_tiles * 1024 + 1024;
+    d.bytes = static_cast<size_t>(2 * d.token_bytes + d.touched_bytes + d.partial_bytes + d.count_bytes);
+    return d;
+}
+
+// Who sorts: asks the device for its clusters.
+void choose_sort(Division& d, const Problem& p) {
+    if (d.bytes == 0) return;
     d.held = 1;
-    const int most = largest_cluster();
+    const int most = p.count <= kMostClusterTokens ? largest_cluster() : 0;
     if (p.count <= int64_t(kSortThreads) * kMostClusterHeld * most) {
         // as few tokens to a thread as the cluster allows; a smaller cluster where one token is enough
         while (int64_t(kSortThreads) * d.held * most < p.count) d.held *= 2;
         d.cluster = 1;
         while (int64_t(kSortThreads) * d.held * d.cluster < p.count) d.cluster *= 2;
     } else {
-        // few tiles, as every block adds up the counts of all; but a thread holds eight tokens at most
-        while (d.held < kMostHeld && ceil_div(p.count, int64_t(kSortThreads) * d.held) > kScannedTiles) d.held *= 2;
+        d.held = tokens_held(p.count);
     }
     d.sort_tiles = static_cast<uint32_t>(ceil_div(p.count, int64_t(kSortThreads) * d.held));
-    // As many as any cluster's limit asks for: what is told where there is no device, or of another one, is enough.
-    const int64_t most_tiles = p.count <= int64_t(kSortThreads) * kMostClusterHeld * kMostCluster ? ceil_div(p.count, kSortThreads) : d.sort_tiles;
-    d.count_bytes = most_tiles * 1024 + 1024;
-    d.bytes = static_cast<size_t>(2 * d.token_bytes + d.touched_bytes + d.partial_bytes + d.count_bytes);
-    return d;
 }
 
 void launch_owned_rows(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p) {
@@ -1083,18 +1096,12 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
     ctx->count_launch(last_blocks > 0 ? 2 : 1);
 }
 
-// What a gradient's call asks of its arguments, its workspace included.
-Problem check_gradient(const b200_embedding_args& a, Division& d) {
-    const Problem p = check_embedding(a, true);
-    d = divide(p);
-    check_workspace(a.workspace, a.workspace_bytes, d.bytes);
-    return p;
-}
-
 void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
-    Division d;
-    const Problem p = check_gradient(a, d);
+    const Problem p = check_embedding(a, true);
     if (p.vocab == 0 || p.width == 0) return;
+    Division d = divide(p);
+    check_workspace(a.workspace, a.workspace_bytes, d.bytes);
+    choose_sort(d, p);
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
     ProfScope scope(ctx, "embedding_backward");
     if (d.bytes == 0) launch_owned_rows(ctx, a, p);
@@ -1104,9 +1111,8 @@ void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
 }  // namespace
 
 void check_embedding_call(const b200_embedding_args& a, bool backward) {
-    Division d;
-    if (backward) (void)check_gradient(a, d);
-    else (void)check_embedding(a, false);
+    const Problem p = check_embedding(a, backward);
+    if (backward && a.workspace != nullptr) check_workspace(a.workspace, a.workspace_bytes, divide(p).bytes);
 }
 
 }  // namespace b200

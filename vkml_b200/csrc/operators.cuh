@@ -270,7 +270,8 @@ inline b200_tensor workspace_tensor(void* workspace, size_t bytes) {
     return t;
 }
 
-// What a call asks of its arguments, without a context: throws Error where it would be refused.
+// What a call asks of its arguments, without a context: throws Error where it would be refused.  Nothing is asked of the device, which may not be there, or not be
+// begun with yet, unless an argument that comes from one needs it: a workspace, or rows beyond 2^28.
 void check_embedding_call(const b200_embedding_args& a, bool backward);
 void check_block_norm(const b200_block_norm_args& a);
 void check_block_norm_backward(const b200_block_norm_grad_args& a);
