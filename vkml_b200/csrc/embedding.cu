@@ -605,7 +605,7 @@ struct SumArgs {
     char* table;
     int64_t pitch;
     float* partial;  // [blocks][2][width]
-    uint32_t count, vocab, chunk, chunks, blocks;  // blocks: along the tokens
+    uint32_t count, vocab, chunk, blocks;  // blocks: along the tokens
     int width, threads, tiles;  // threads that share a row, a power of two up to 128; tiles of threads * 8 columns
     float scale;
     int accumulate;
@@ -909,7 +909,7 @@ int largest_cluster() { return clusters_at_once(kMostClusterHeld, kMostCluster) 
 
 // How a gradient of many tokens is divided, and where its scratch lies.
 struct Division {
-    uint32_t chunk, chunks, blocks;
+    uint32_t chunk, blocks;
     int threads, tiles;
     int held;             // (from choose_sort) tokens of a thread that sorts
     int cluster;          // blocks of the cluster that sorts; 0: many blocks
@@ -942,8 +942,7 @@ Division divide(const Problem& p) {
     // two waves of blocks, two to an SM, of chunks that are no longer than 256 tokens
     const int64_t wave = std::max<int64_t>(1, int64_t(sm_count()) * 4 / d.tiles);
     d.chunk = static_cast<uint32_t>(std::min<int64_t>(256, std::max<int64_t>(4, ceil_div(ceil_div(p.count, wave * groups), 4) * 4)));
-    d.chunks = static_cast<uint32_t>(ceil_div(p.count, int64_t(d.chunk)));
-    d.blocks = static_cast<uint32_t>(ceil_div(int64_t(d.chunks), groups));
+    d.blocks = static_cast<uint32_t>(ceil_div(ceil_div(p.count, int64_t(d.chunk)), groups));
     auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
     d.token_bytes = whole(p.count * 8);
     d.touched_bytes = whole(ceil_div(p.vocab, 32) * 4);
@@ -1073,7 +1072,6 @@ void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p
     k.count = s.count;
     k.vocab = s.vocab;
     k.chunk = d.chunk;
-    k.chunks = d.chunks;
     k.blocks = d.blocks;
     k.width = static_cast<int>(p.width);
     k.threads = d.threads;
