@@ -925,6 +925,7 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
     check_workspace(a.workspace, a.workspace_bytes, d.bytes);
     const b200_tensor* vectors[kSums] = {&a.gate_grad, &a.post_weight_grad, &a.post_bias_grad, &a.pre_weight_grad, &a.pre_bias_grad};
     if (p.width == 0) return;
+    char* scratch = operator_workspace(ctx, a.workspace, d.bytes);  // (refuses, too, before anything is queued)
     wait_for_tensors(ctx, {&a.out, &a.branch, &a.stats, &a.out_grad, &a.normed_grad, &a.post_weight, &a.post_bias, &a.gate, &a.pre_weight, &a.residual_grad, &a.branch_grad,
                            &a.post_weight_grad, &a.post_bias_grad, &a.pre_weight_grad, &a.pre_bias_grad, &a.gate_grad});
     if (p.s.rows == 0) {  // sums of nothing
@@ -933,7 +934,6 @@ void launch_backward(b200_ctx* ctx, const b200_block_norm_grad_args& a) {
         }
         return;
     }
-    char* scratch = operator_workspace(ctx, a.workspace, d.bytes);
     BackwardArgs k{};
     auto rows = [&](const b200_tensor& t) { return rows_arg(t, present(t) ? p.axes : 0); };
     k.out = rows(a.out);

@@ -991,8 +991,7 @@ void launch_owned_rows(b200_ctx* ctx, const b200_embedding_args& a, const Proble
 // Zeros written beside the sort: what the memory takes meanwhile, of one kernel of the many and of the cluster's.
 constexpr int64_t kZerosBesideKernel = int64_t(20) << 20, kZerosBesideCluster = int64_t(48) << 20;
 
-void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p, const Division& d) {
-    char* scratch = operator_workspace(ctx, a.workspace, d.bytes);
+void launch_sorted(b200_ctx* ctx, const b200_embedding_args& a, const Problem& p, const Division& d, char* scratch) {
     const bool accumulate = (a.flags & B200_ACCUMULATE) != 0;
     const int64_t size = static_cast<int64_t>(dtype_size(a.table.dtype)), row_bytes = p.width * size;
     uint2* buffer[2] = {reinterpret_cast<uint2*>(scratch), reinterpret_cast<uint2*>(scratch + d.token_bytes)};
@@ -1100,10 +1099,11 @@ void launch_gradient(b200_ctx* ctx, const b200_embedding_args& a) {
     Division d = divide(p);
     check_workspace(a.workspace, a.workspace_bytes, d.bytes);
     choose_sort(d, p);
+    char* const scratch = operator_workspace(ctx, a.workspace, d.bytes);  // (refuses, too, before anything is queued)
     wait_for_tensors(ctx, {&a.table, &a.ids, &a.rows});
     ProfScope scope(ctx, "embedding_backward");
     if (d.bytes == 0) launch_owned_rows(ctx, a, p);
-    else launch_sorted(ctx, a, p, d);
+    else launch_sorted(ctx, a, p, d, scratch);
 }
 
 }  // namespace
