@@ -552,6 +552,12 @@ __device__ __forceinline__ void barrier_arrive(int parity, int threads) {
 constexpr int kRowBarrier = 1, kTold = 2, kSummed = kTold + kTeachers, kWritten = kSummed + kTeachers;
 constexpr int kMeeting = kRowThreads + 32;
 
+// What a teacher's warp says of its row (forward: at, soft2 and hard2 are not known yet).  On 32 bytes, which the rows' warps read in wide accesses (4096 x 32000 F16,
+// losses and gradient: 130.3 us, 133.5 without).
+struct __align__(32) Told {
+    RowGrad grad;
+};
+
 struct RingArgs {
     int chunk;   // vectors of a thread in a visit
     int slots;   // visits in shared memory: 1 to 3
@@ -581,7 +587,7 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
     uint4* const held = reinterpret_cast<uint4*>(shared);  // [slots][chunk][kRowThreads]
     int* const entries = reinterpret_cast<int*>(held + ring.slots * ring.chunk * kRowThreads);
     __shared__ Part parts[kTeachers][kRowWarps];
-    __shared__ RowGrad told[kTeachers];  // what a teacher's warp says of its row (forward: at, soft2 and hard2 are not known yet)
+    __shared__ Told told[kTeachers];
     pdl_prologue();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const uint32_t n = (rows - blockIdx.x + gridDim.x - 1) / gridDim.x;  // rows of this block: blockIdx.x + i * gridDim.x
@@ -658,7 +664,7 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
                 row.wh = label >= 0 ? w * k.hard_weight : 0.f;
             }
             if constexpr (!FORWARD) row.at = shift_of(stats.x), row.soft2 = -shift_of(stats.y) * kLog2e, row.hard2 = -shift_of(stats.z) * kLog2e;
-            if (lane == 0) told[parity] = row;
+            if (lane == 0) told[parity].grad = row;
             __syncwarp();
             barrier_arrive<kTold>(parity, kMeeting);
             if constexpr (FORWARD) {
@@ -848,7 +854,7 @@ distill_rows_kernel(const Args k, const RingArgs ring, uint32_t rows) {
             barrier_sync<kTold>(parity, kMeeting);
         }
         if constexpr (GRAD) {
-            RowGrad grad = told[parity];
+            RowGrad grad = told[parity].grad;
             if constexpr (FORWARD) {
                 Part run = lane < kRowWarps ? parts[parity][lane] : Part{-INFINITY, 0.f, 0.f};
                 run = warp_part(run, c_soft, k.soft, k.hard);
