@@ -416,6 +416,96 @@ int b200_distill_loss(b200_ctx* ctx, const b200_distill_args* args);
 /* The gradient alone, for losses' gradients that are known only later. */
 int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
 
+/* A gated linear recurrence along a sequence, each channel by itself: h_t = a_t h_{t-1} + b_t, out_t = h_t, with
+ *     B200_GATES_SIGMOID: a = sigmoid(gate), b = (1 - a) x        B200_GATES_EXP: a = exp(gate), b = x
+ * A gate of -inf begins anew (a = 0).  Products of decays just below 1 keep their digits: 1 - a is carried where a is above a half. */
+#define B200_GATES_SIGMOID 0
+#define B200_GATES_EXP 1
+#define B200_RECURRENCE_CHUNK 16
+typedef struct b200_recurrence_args {
+    b200_tensor x;         /* rows [L, D] or [B, L, D]: the axis in front of the rows' own is time */
+    b200_tensor gate;      /* x's extents.  (x, gate): (F32, F32), (F16, F16) or (F16, F32) */
+    b200_tensor initial;   /* h in front of the first step, rows [D] or [B, D], F32; absent: zeros */
+    b200_tensor lengths;   /* steps of each sequence: [B], or one without an axis; I32 or I64, any stride; absent: L.  Steps behind a sequence's end are
+                              not read, and zeros in out.  One outside 0..L is an index error at the next synchronisation, and taken as the nearer end */
+    b200_tensor out;       /* x's extents and type; may lie exactly on x or gate */
+    b200_tensor final_state; /* h behind the last step, extents like initial, F32; may be absent; may lie exactly on initial */
+    b200_tensor states;    /* [C, D] or [B, C, D], C = ceil(L / B200_RECURRENCE_CHUNK), F32, dense: h in front of steps 0, 16, 32 .. (behind a
+                              sequence's end: its final one); backward needs it; may be absent */
+    int32_t kind;          /* B200_GATES_SIGMOID, B200_GATES_EXP */
+    uint32_t flags;        /* 0 */
+} b200_recurrence_args;
+int b200_gated_recurrence(b200_ctx* ctx, const b200_recurrence_args* args);
+
+/* Gradients of b200_gated_recurrence from those of out and of the final state.  Every gradient may be absent; one of them at least is there. */
+typedef struct b200_recurrence_grad_args {
+    b200_tensor x, gate, lengths, states;   /* as the forward call had and left them */
+    b200_tensor out_grad;                   /* x's extents and type; absent: zeros */
+    b200_tensor final_grad;                 /* extents like initial, F32; absent: zeros */
+    b200_tensor x_grad, gate_grad;          /* x's extents, types of x and gate; zeros behind a sequence's end; may lie exactly on x, gate or out_grad */
+    b200_tensor initial_grad;               /* extents like initial, F32; may lie exactly on final_grad */
+    int32_t kind;
+    uint32_t flags;
+} b200_recurrence_grad_args;
+int b200_gated_recurrence_backward(b200_ctx* ctx, const b200_recurrence_grad_args* args);
+
+/* Log probabilities of given tokens, the entropy of their distribution, and its likeliest tokens.  For a row z of logits and temperature T, q = softmax(z / T):
+ *     logprob = log q[token]      (0 in a row without a token)          entropy = - sum of q log q
+ *     top     = the K largest logits: their columns, the largest first, of equal ones the lowest column first; and log q there
+ * and backward, for a row's gradients u of logprob (0 where it has no token) and w of entropy,
+ *     grad    = grad_scale * (u * (one at token - q) - w * q * (log q + entropy)) / T      (zeros where u and w are 0, whatever z holds)
+ * A token below 0 is none; one at or above V is none either, and an index error at the next synchronisation.  A logit of -inf has q = 0; a row of nothing else
+ * has log q = -inf everywhere and entropy 0, and no gradient.  A row that holds +inf or no number has results that are no numbers; its top counts what is no number as
+ * the largest. */
+#define B200_MOST_TOP 128
+typedef struct b200_token_logprobs_args {
+    b200_tensor logits;          /* rows [.., V], F32 or F16, V >= 1 */
+    b200_tensor tokens;          /* one for each row (the rows' extents), I32 or I64, any strides; absent: none */
+    b200_tensor logprobs;        /* F32, dense, one for each row; forward only, may be absent */
+    b200_tensor entropies;       /* the same */
+    b200_tensor stats;           /* [number of rows, 4], F32, dense: max z, log sum exp((z - max z) / T), entropy, 0; forward: a result, may be absent;
+                                    backward: as forward left it */
+    b200_tensor top_ids;         /* rows [.., K], I32 or I64, K <= B200_MOST_TOP and <= V; forward only, may be absent */
+    b200_tensor top_logprobs;    /* rows [.., K], F32; forward only, may be absent */
+    b200_tensor logprobs_grad;   /* F32, one for each row, any strides; absent: zeros; backward only */
+    b200_tensor entropies_grad;  /* the same */
+    b200_tensor grad;            /* rows like logits, of their type; may lie exactly on logits; backward only */
+    float temperature, grad_scale;
+} b200_token_logprobs_args;
+int b200_token_logprobs(b200_ctx* ctx, const b200_token_logprobs_args* args);
+int b200_token_logprobs_backward(b200_ctx* ctx, const b200_token_logprobs_args* args);
+
+/* One AdamW step over many tensors.  With g = grad_scale * grad, t the step (from 1 on) and lr the rate of a tensor (lr * its lr_scale),
+ *     m = beta1 m + (1 - beta1) g          v = beta2 v + (1 - beta2) g^2
+ *     param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * States of 8 bits: m and sqrt(v) lie as bytes of a sign, 4 bits of exponent and 3 of mantissa (bias 7, subnormal below 2^-6, 448 the largest), in units of a
+ * scale that 256 elements share (the largest of their sizes / 448; a block that holds nothing of 2^-100 is zero).  A value between two bytes goes up or down by 16 random
+ * bits of seed, step, the tensor's number and the element's, so that changes smaller than a byte's step are kept on average; a root that is not 0 keeps at least
+ * the least byte.  The update goes by m and v before they are rounded.  A block that holds a value that is not finite has scales and bytes that are no numbers.
+ * With mix(x) = (x ^= x >> 16, x *= 0x6a09e667, x ^= x >> 15, x *= 0x3c6ef373, x ^ x >> 16) on 32 bits, the bits of element i of tensor k are
+ * mix(mix(mix(mix(seed) + step) + k) + i * 0x9e3779b9): the lower 16 for m, the upper for the root; r of them add (16 r + 8) / 2^20 of a step before the rest is cut off. */
+typedef struct b200_adamw_tensor {
+    b200_tensor param;    /* F32, dense, written in place */
+    b200_tensor grad;     /* param's extents, F32 or F16, dense */
+    b200_tensor first;    /* m: F32 of param's extents, dense; or, in 8 bits, I32 [ceil(n / 4)] for n elements, four to a word, the lowest byte first */
+    b200_tensor second;   /* v: the same; in 8 bits its root.  Bytes behind the last element stay as they are */
+    b200_tensor scales;   /* 8 bits: [ceil(n / 256), 2], F32, dense: of first and second.  Else absent */
+    b200_tensor copy;     /* F16, param's extents, dense: takes the new param, rounded; may be absent */
+    float weight_decay, lr_scale;
+} b200_adamw_tensor;
+typedef struct b200_adamw_args {
+    const b200_adamw_tensor* tensors; /* host memory, read before the call returns */
+    int64_t count;
+    b200_tensor lr_on_device;         /* one F32: takes the place of lr (a schedule in a captured step); absent: lr */
+    b200_tensor step_on_device;       /* one I64: takes the place of step; absent: step.  Where it is below 1 nothing changes */
+    b200_tensor scale_on_device;      /* one F32, times grad_scale (clipping; an unscaled loss); absent: 1.  Where the product is not finite nothing changes */
+    int64_t step;                     /* from 1 on */
+    double beta1, beta2;              /* in [0, 1) */
+    float lr, eps, grad_scale;        /* eps above 0 */
+    uint32_t seed;                    /* 8 bits only */
+} b200_adamw_args;
+int b200_adamw(b200_ctx* ctx, const b200_adamw_args* args);
+
 /* The status that one of these calls would answer its arguments with, and the reason, without a context or a device:
  * `args` is the call's struct, its workspace included.  What b200_supports is for nodes.  (What only a context knows --
  * memory that is full, a stream that is captured -- is not told.) */
@@ -425,6 +515,11 @@ int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
 #define B200_CALL_BLOCK_NORM_BACKWARD 3
 #define B200_CALL_DISTILL_LOSS 4
 #define B200_CALL_DISTILL_LOSS_BACKWARD 5
+#define B200_CALL_GATED_RECURRENCE 16
+#define B200_CALL_GATED_RECURRENCE_BACKWARD 17
+#define B200_CALL_TOKEN_LOGPROBS 18
+#define B200_CALL_TOKEN_LOGPROBS_BACKWARD 19
+#define B200_CALL_ADAMW 20
 int b200_check_operator(int which, const void* args, char* why, size_t why_len);
 
 /* -- an entry point that allocates nothing (no counterpart in vkML: its backends

@@ -8,9 +8,9 @@ interface for tests, benchmarks and scripting.
 from .backend import (Backend, DeviceTensor, Storage, Error, ShapeError, DTypeError, DeviceError,
                       OutOfMemoryError, InternalError, COMPUTE_SYNC, COMPUTE_GRAD_SYNC, GEMM_3XTF32,
                       GEMM_TF32, GEMM_FP32)
-from .graph import DType, Op, NodeDesc, TensorDesc, op_name
+from .graph import AdamWTable, AdamWTensor, DType, Op, NodeDesc, TensorDesc, adamw_table, op_name
 from . import graph
 
-__all__ = ["Backend", "DeviceTensor", "Storage", "DType", "Op", "NodeDesc", "TensorDesc", "graph",
+__all__ = ["AdamWTable", "AdamWTensor", "adamw_table", "Backend", "DeviceTensor", "Storage", "DType", "Op", "NodeDesc", "TensorDesc", "graph",
            "op_name", "Error", "ShapeError", "DTypeError", "DeviceError", "OutOfMemoryError",
            "InternalError", "COMPUTE_SYNC", "COMPUTE_GRAD_SYNC", "GEMM_3XTF32", "GEMM_TF32", "GEMM_FP32"]

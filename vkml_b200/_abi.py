@@ -102,6 +102,40 @@ class DistillArgs(C.Structure):
         ("temperature", C.c_float), ("hard_weight", C.c_float), ("grad_scale", C.c_float)]
 
 
+class RecurrenceArgs(C.Structure):
+    """b200_recurrence_args"""
+    _fields_ = [(n, Tensor) for n in ("x", "gate", "initial", "lengths", "out", "final_state", "states")] + [
+        ("kind", C.c_int32), ("flags", C.c_uint32)]
+
+
+class RecurrenceGradArgs(C.Structure):
+    """b200_recurrence_grad_args"""
+    _fields_ = [(n, Tensor) for n in (
+        "x", "gate", "lengths", "states", "out_grad", "final_grad", "x_grad", "gate_grad", "initial_grad")] + [
+        ("kind", C.c_int32), ("flags", C.c_uint32)]
+
+
+class TokenLogprobsArgs(C.Structure):
+    """b200_token_logprobs_args"""
+    _fields_ = [(n, Tensor) for n in (
+        "logits", "tokens", "logprobs", "entropies", "stats", "top_ids", "top_logprobs", "logprobs_grad", "entropies_grad",
+        "grad")] + [("temperature", C.c_float), ("grad_scale", C.c_float)]
+
+
+class AdamWTensor(C.Structure):
+    """b200_adamw_tensor"""
+    _fields_ = [(n, Tensor) for n in ("param", "grad", "first", "second", "scales", "copy")] + [
+        ("weight_decay", C.c_float), ("lr_scale", C.c_float)]
+
+
+class AdamWArgs(C.Structure):
+    """b200_adamw_args"""
+    _fields_ = [("tensors", C.c_void_p), ("count", C.c_int64)] + [
+        (n, Tensor) for n in ("lr_on_device", "step_on_device", "scale_on_device")] + [
+        ("step", C.c_int64), ("beta1", C.c_double), ("beta2", C.c_double), ("lr", C.c_float), ("eps", C.c_float),
+        ("grad_scale", C.c_float), ("seed", C.c_uint32)]
+
+
 # Every symbol include/vkml_b200.h declares: name -> (restype, argtypes).
 _P = C.c_void_p
 SYMBOLS = {
@@ -158,6 +192,11 @@ SYMBOLS = {
     "b200_check_operator": (C.c_int, [C.c_int, _P, C.c_char_p, C.c_size_t]),
     "b200_distill_loss": (C.c_int, [_P, _P]),
     "b200_distill_loss_backward": (C.c_int, [_P, _P]),
+    "b200_gated_recurrence": (C.c_int, [_P, _P]),
+    "b200_gated_recurrence_backward": (C.c_int, [_P, _P]),
+    "b200_token_logprobs": (C.c_int, [_P, _P]),
+    "b200_token_logprobs_backward": (C.c_int, [_P, _P]),
+    "b200_adamw": (C.c_int, [_P, _P]),
     "b200_sum_columns_f32_noalloc": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, _P, _P, C.c_char_p, C.c_size_t]),
 }
 

@@ -228,6 +228,57 @@ class Backend:
             (logits, teacher_ids, teacher_logits, labels, None, stats, losses_grad, grad), temperature, hard_weight,
             grad_scale)), "distill_loss_backward")
 
+    def gated_recurrence(self, x, gate, out, *, initial=None, final=None, states=None, lengths=None, kind: str = "sigmoid") -> None:
+        """out[t] = h = a[t] * h + b[t] along the axis in front of the last, each channel by itself.  kind "sigmoid":
+        a = sigmoid(gate), b = (1 - a) * x; "exp": a = exp(gate), b = x.  x, gate and out [L, D] or [B, L, D]; `initial`
+        and `final` [D] or [B, D] F32 are h in front of the first step (None: zeros) and behind the last, and may be one
+        tensor: that is how a sequence is continued token by token.  `lengths` [B]: steps of each sequence; behind them out is zeros.  `states`
+        [.., ceil(L / 16), D] F32 is what gated_recurrence_backward needs."""
+        self._check(self._lib.b200_gated_recurrence(self._ctx, graph.recurrence_args(
+            (x, gate, initial, lengths, out, final, states), self._gate_kind(kind))), "gated_recurrence")
+
+    @staticmethod
+    def _gate_kind(kind: str) -> int:
+        if kind not in graph.GATE_KINDS:
+            raise ValueError(f"gated_recurrence: unknown kind of gates {kind!r}")
+        return graph.GATE_KINDS[kind]
+
+    def gated_recurrence_backward(self, x, gate, states, *, out_grad=None, final_grad=None, x_grad=None, gate_grad=None,
+                                  initial_grad=None, lengths=None, kind: str = "sigmoid") -> None:
+        """Gradients of gated_recurrence from out_grad and final_grad (either may be None: zero), with states as the forward call left
+        them: x_grad, gate_grad and initial_grad, each where a tensor is given."""
+        self._check(self._lib.b200_gated_recurrence_backward(self._ctx, graph.recurrence_args(
+            (x, gate, lengths, states, out_grad, final_grad, x_grad, gate_grad, initial_grad), self._gate_kind(kind))),
+            "gated_recurrence_backward")
+
+    def token_logprobs(self, logits, tokens=None, logprobs=None, *, entropies=None, stats=None, top_ids=None, top_logprobs=None,
+                       temperature: float = 1.0) -> None:
+        """logprobs = log softmax(logits / T) at tokens, one F32 for each row (0 where the token is below 0); entropies of the same
+        distributions; top_ids [.., K] (I32 or I64) the columns of the K <= 128 largest logits, the largest first (equal ones: the lowest
+        column), and top_logprobs [.., K] F32 their log probabilities -- what distill_loss reads as a teacher's.  Each where a tensor is given.
+        stats [rows, 4] F32 is what token_logprobs_backward needs."""
+        self._check(self._lib.b200_token_logprobs(self._ctx, graph.logprobs_args(
+            (logits, tokens, logprobs, entropies, stats, top_ids, top_logprobs, None, None, None), temperature, 1.0)), "token_logprobs")
+
+    def token_logprobs_backward(self, logits, tokens, stats, grad, *, logprobs_grad=None, entropies_grad=None,
+                                temperature: float = 1.0, grad_scale: float = 1.0) -> None:
+        """The logits' gradient from those of logprobs and entropies (either may be None: zero), times grad_scale, with stats as
+        token_logprobs left them; grad may lie on logits."""
+        self._check(self._lib.b200_token_logprobs_backward(self._ctx, graph.logprobs_args(
+            (logits, tokens, None, None, stats, None, None, logprobs_grad, entropies_grad, grad), temperature, grad_scale)),
+            "token_logprobs_backward")
+
+    def adamw(self, tensors, *, lr, step, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale=1.0,
+              seed: int = 0) -> None:
+        """One AdamW step over all tensors: a sequence of AdamWTensor, or what adamw_table() made of one, once for all steps.  States in
+        F32, or in 8 bits with a scale to 256 elements, rounded up or down by bits of seed and step.  lr, step (from 1 on) and grad_scale are
+        numbers, or one-element tensors on the device (F32, I64, F32) for a step that is captured once: where grad_scale is not finite there,
+        or step below 1, nothing changes."""
+        table = tensors if isinstance(tensors, graph.AdamWTable) else graph.adamw_table(tensors)
+        args, keep = graph.adamw_args(table, lr, step, beta1, beta2, eps, grad_scale, seed)
+        self._check(self._lib.b200_adamw(self._ctx, args), "adamw")
+        del keep
+
     # -- copies ---------------------------------------------------------------
     def copy_from_host(self, dst: Storage, dst_offset: int, src, nbytes: int | None = None) -> None:
         buf = np.ascontiguousarray(src) if not isinstance(src, int) else None

@@ -1,0 +1,445 @@
+// One AdamW step over many tensors, states in F32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g        v = b2 v + (1 - b2) g^2        p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound by memory: 28 bytes to an element with everything in F32, 14 to 18 with 8-bit states.  The tensors' addresses travel in the launch's parameters, some
+// hundreds at a time, so that a step over all of a model's tensors is one launch and uploads nothing.  A warp takes 256 elements, which are a block of 8-bit
+// states: their largest is a reduction in the warp, and a state is read, updated, scaled and written without leaving its registers.
+//
+// An 8-bit state's change in a step is mostly smaller than half a step of its byte (v moves by a thousandth, a byte's step is 6 to 12 %): rounded to the nearest,
+// it would stay where it is.  Each is rounded up or down by random bits instead, whose mean is what was computed.  The root of v is what is kept: it has half
+// of v's range in powers of two, and a byte covers 2^17 of them, as for m.
+// (This file is compiled without joining multiplications and additions: the bytes are what the formulas give, operation by operation.)
+#include "operators.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+namespace b200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;                // elements that share a scale: a warp's
+constexpr int kRounds = 4;                 // blocks of 256 that a warp takes one after another
+constexpr int kItem = kThreads / 32 * kRounds * kBlock;  // elements of a block of threads
+constexpr int kMostTensors = 384;          // of a launch: 32,764 bytes of parameters
+
+struct Tensor {
+    float* param;
+    const void* grad;
+    void* first;
+    void* second;
+    float2* scales;  // null: F32 states
+    __half* copy;
+    int64_t n;
+    float decay, lr_scale;
+    uint32_t item;    // its first of the launch
+    uint32_t number;  // in the caller's list
+    uint32_t half_grad, wide;
+};
+
+struct Numbers {
+    const float* lr_at;
+    const int64_t* step_at;
+    const float* scale_at;
+    int64_t step;
+    float lr, b1, rest1, b2, rest2, eps, scale;
+    float log_b1, log_b2;                  // natural logarithms
+    float inverse1, root_inverse2;         // 1 / (1 - b1^step), 1 / sqrt(1 - b2^step)
+    uint32_t seed;
+};
+
+template <int N>
+struct Table {
+    Numbers numbers;
+    int count;
+    Tensor t[N];
+};
+
+// ---- 8-bit states -----------------------------------------------------------
+
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x6a09e667u;
+    x = (x ^ (x >> 15)) * 0x3c6ef373u;
+    return x ^ (x >> 16);
+}
+
+// The values of two bytes.
+__device__ __forceinline__ float2 byte_values(uint32_t pair) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 p;\n\tcvt.u16.u32 p, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\t}" : "=r"(h) : "r"(pair));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// The byte of a size that is at most 448, up or down by 16 random bits.  Times 2^-120 a float's exponent field is the byte's, and so are the leading bits of its
+// fraction, subnormal ones too: adding below them carries into them.
+__device__ __forceinline__ uint32_t byte_of(float x, uint32_t bits) {
+    const uint32_t whole = __float_as_uint(x * 0x1p-120f);
+    return min((whole + (bits << 4 | 8u)) >> 20, 126u);
+}
+
+// What a block's sizes are divided by, and its inverse; of a block that is zero, or not finite.
+struct Scale {
+    float scale, inverse;
+    bool broken;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t most_bits) {
+    const float most = __uint_as_float(most_bits);
+    Scale s;
+    s.broken = most_bits >= 0x7f800000u;
+    const bool some = most >= 0x1p-100f;
+    s.scale = s.broken ? __uint_as_float(0x7fffffffu) : some ? most * (1.f / 448.f) : 0.f;
+    s.inverse = some ? 1.f / most * 448.f : 0.f;
+    return s;
+}
+
+// ---- the step ---------------------------------------------------------------
+
+struct Step {
+    float b1, rest1, b2, rest2, eps, scale, root_inverse2, keep, rate;
+    __device__ __forceinline__ void moments(float g, float& m, float& v) const {
+        g = g * scale;
+        m = m * b1 + g * rest1;
+        v = v * b2 + g * g * rest2;
+    }
+    __device__ __forceinline__ float param(float p, float m, float root) const { return p * keep - __fdividef(m, root * root_inverse2 + eps) * rate; }
+};
+
+// Eight elements of a lane: neighbours where the tensor's addresses allow it, else 32 apart.
+template <bool WIDE, typename T>
+__device__ __forceinline__ void load_values(float (&x)[8], const T* from, int64_t left, int lane) {
+    if constexpr (WIDE) {
+        Raw8<T> raw;
+        load8(raw, from + lane * 8);
+        unpack8(raw, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = e * 32 + lane < left ? to_float(from[e * 32 + lane]) : 0.f;
+    }
+}
+template <bool WIDE, typename T>
+__device__ __forceinline__ void store_values(T* to, const float (&x)[8], int64_t left, int lane) {
+    if constexpr (WIDE) {
+        store8(to + lane * 8, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e * 32 + lane < left) to[e * 32 + lane] = from_float<T>(x[e]);
+        }
+    }
+}
+template <bool WIDE>
+__device__ __forceinline__ void load_bytes(uint32_t (&c)[2], const uint8_t* from, int64_t left, int lane) {
+    if constexpr (WIDE) {
+        const uint2 w = *reinterpret_cast<const uint2*>(from + lane * 8);
+        c[0] = w.x, c[1] = w.y;
+    } else {
+        c[0] = c[1] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e * 32 + lane < left) c[e / 4] |= static_cast<uint32_t>(from[e * 32 + lane]) << (e % 4 * 8);
+        }
+    }
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_bytes(uint8_t* to, const uint32_t (&c)[2], int64_t left, int lane) {
+    if constexpr (WIDE) {
+        *reinterpret_cast<uint2*>(to + lane * 8) = make_uint2(c[0], c[1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e * 32 + lane < left) to[e * 32 + lane] = static_cast<uint8_t>(c[e / 4] >> (e % 4 * 8));
+        }
+    }
+}
+__device__ __forceinline__ void bytes_values(float (&x)[8], const uint32_t (&c)[2], float scale) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = byte_values(c[i / 2] >> (i % 2 * 16));
+        x[2 * i] = f.x * scale;
+        x[2 * i + 1] = f.y * scale;
+    }
+}
+
+// 256 elements from element `from` on, or what is left of them.
+template <bool WIDE>
+__device__ __forceinline__ void step_block(const Tensor& t, const Step& s, uint32_t key, int64_t from, int lane) {
+    const int64_t left = t.n - from;
+    float p[8], g[8], m[8], v[8];
+    uint32_t a[2], b[2];
+    float2 scales = make_float2(0.f, 0.f);
+    load_values<WIDE>(p, t.param + from, left, lane);
+    if (t.half_grad) load_values<WIDE>(g, static_cast<const __half*>(t.grad) + from, left, lane);
+    else load_values<WIDE>(g, static_cast<const float*>(t.grad) + from, left, lane);
+    const bool bytes = t.scales != nullptr;
+    if (bytes) {
+        load_bytes<WIDE>(a, static_cast<const uint8_t*>(t.first) + from, left, lane);
+        load_bytes<WIDE>(b, static_cast<const uint8_t*>(t.second) + from, left, lane);
+        scales = t.scales[from / kBlock];
+        bytes_values(m, a, scales.x);
+        bytes_values(v, b, scales.y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * v[e];
+    } else {
+        load_values<WIDE>(m, static_cast<const float*>(t.first) + from, left, lane);
+        load_values<WIDE>(v, static_cast<const float*>(t.second) + from, left, lane);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s.moments(g[e], m[e], v[e]);
+    if (!bytes) {
+        store_values<WIDE>(static_cast<float*>(t.first) + from, m, left, lane);
+        store_values<WIDE>(static_cast<float*>(t.second) + from, v, left, lane);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sqrtf(v[e]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = s.param(p[e], m[e], v[e]);
+    store_values<WIDE>(t.param + from, p, left, lane);
+    if (t.copy != nullptr) store_values<WIDE>(t.copy + from, p, left, lane);
+    if (!bytes) return;
+    uint32_t most_m = 0, most_v = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        most_m = max(most_m, __float_as_uint(m[e]) & 0x7fffffffu);
+        most_v = max(most_v, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    const Scale sm = scale_of(__reduce_max_sync(0xffffffffu, most_m)), sv = scale_of(__reduce_max_sync(0xffffffffu, most_v));
+    a[0] = a[1] = b[0] = b[1] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t i = static_cast<uint32_t>(from) + static_cast<uint32_t>(WIDE ? lane * 8 + e : e * 32 + lane);
+        const uint32_t bits = mix(key + i * 0x9e3779b9u);
+        uint32_t first = byte_of(fabsf(m[e]) * sm.inverse, bits & 0xffffu) | (__float_as_uint(m[e]) >> 31 << 7);
+        uint32_t second = byte_of(v[e] * sv.inverse, bits >> 16);
+        if (v[e] > 0.f && sv.inverse > 0.f) second = max(second, 1u);
+        if (sm.broken) first = 127u;
+        if (sv.broken) second = 127u;
+        a[e / 4] |= first << (e % 4 * 8);
+        b[e / 4] |= second << (e % 4 * 8);
+    }
+    store_bytes<WIDE>(static_cast<uint8_t*>(t.first) + from, a, left, lane);
+    store_bytes<WIDE>(static_cast<uint8_t*>(t.second) + from, b, left, lane);
+    if (lane == 0) t.scales[from / kBlock] = make_float2(sm.scale, sv.scale);
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> k) {
+    pdl_prologue();
+    int lo = 0, hi = k.count;  // the tensor whose items this block's is one of
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (k.t[mid].item <= blockIdx.x) lo = mid;
+        else hi = mid;
+    }
+    const Tensor& t = k.t[lo];
+    const Numbers& n = k.numbers;
+    Step s;
+    s.b1 = n.b1, s.rest1 = n.rest1, s.b2 = n.b2, s.rest2 = n.rest2, s.eps = n.eps, s.scale = n.scale;
+    float inverse1 = n.inverse1, lr = n.lr;
+    int64_t step = n.step;
+    s.root_inverse2 = n.root_inverse2;
+    if (n.step_at != nullptr) {
+        step = *n.step_at;
+        if (step < 1) return;
+        inverse1 = -1.f / expm1f(static_cast<float>(step) * n.log_b1);
+        s.root_inverse2 = 1.f / sqrtf(-expm1f(static_cast<float>(step) * n.log_b2));
+    }
+    if (n.lr_at != nullptr) lr = *n.lr_at;
+    if (n.scale_at != nullptr) {
+        s.scale = s.scale * *n.scale_at;
+        if (!isfinite(s.scale)) return;
+    }
+    lr = lr * t.lr_scale;
+    s.keep = 1.f - lr * t.decay;
+    s.rate = lr * inverse1;
+    const uint32_t key = t.scales != nullptr ? mix(mix(mix(n.seed) + static_cast<uint32_t>(step)) + t.number) : 0u;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t base = int64_t(blockIdx.x - t.item) * kItem;
+#pragma unroll 1
+    for (int r = 0; r < kRounds; ++r) {
+        const int64_t from = base + (r * (kThreads / 32) + warp) * kBlock;
+        if (from >= t.n) return;
+        if (t.wide && t.n - from >= kBlock) step_block<true>(t, s, key, from, lane);
+        else step_block<false>(t, s, key, from, lane);
+    }
+}
+
+// ---- arguments --------------------------------------------------------------
+
+bool present(const b200_tensor& t) { return t.data != nullptr; }
+
+void check_one(const b200_tensor& t, const char* name, int dtype) {
+    if (!present(t)) return;
+    check_tensor(t, name);
+    if (t.dtype != dtype) fail(B200_DTYPE_ERROR, std::string(name) + " has another type");
+    if (numel_of(t) != 1) fail(B200_SHAPE_ERROR, std::string(name) + ": not one element");
+}
+
+struct Range {
+    const char *lo, *hi;
+    bool written;
+    bool operator<(const Range& o) const { return lo < o.lo; }
+};
+
+void check_numbers(const b200_adamw_args& a) {
+    if (a.count < 0 || a.count >= (int64_t(1) << 31)) fail(B200_INVALID_ARGUMENT, "adamw: the number of tensors is below 0 or too large");
+    if (a.count > 0 && a.tensors == nullptr) fail(B200_INVALID_ARGUMENT, "adamw: no tensors");
+    check_one(a.lr_on_device, "lr_on_device", B200_F32);
+    check_one(a.step_on_device, "step_on_device", B200_I64);
+    check_one(a.scale_on_device, "scale_on_device", B200_F32);
+    if (!(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1)) fail(B200_INVALID_ARGUMENT, "adamw: a beta is not in [0, 1)");
+    if (!(a.eps > 0.f) || std::isinf(a.eps)) fail(B200_INVALID_ARGUMENT, "adamw: eps is not above 0 and finite");
+    if (!std::isfinite(a.lr) || !std::isfinite(a.grad_scale)) fail(B200_INVALID_ARGUMENT, "adamw: lr or grad_scale is not finite");
+    if (a.step < 1) fail(B200_INVALID_ARGUMENT, "adamw: the step is below 1");
+}
+
+// The tensors' checks; what is written lies on nothing else of the call (sorted addresses: a neighbour shows it).
+void check_tensors(const b200_adamw_args& a) {
+    std::vector<Range> ranges;
+    ranges.reserve(static_cast<size_t>(a.count) * 6 + 3);
+    auto add = [&](const b200_tensor& t, bool written) {
+        const int64_t bytes = numel_of(t) * static_cast<int64_t>(dtype_size(t.dtype));
+        if (present(t) && bytes != 0) ranges.push_back({static_cast<const char*>(t.data), static_cast<const char*>(t.data) + bytes, written});
+    };
+    for (int64_t i = 0; i < a.count; ++i) {
+        const b200_adamw_tensor& t = a.tensors[i];
+        auto refuse = [&](int status, const char* why) { fail(status, "adamw: tensor " + std::to_string(i) + ": " + why); };
+        check_tensor(t.param, "param");
+        check_tensor(t.grad, "grad");
+        check_tensor(t.first, "first");
+        check_tensor(t.second, "second");
+        const int64_t n = numel_of(t.param);
+        const bool bytes = t.first.dtype == B200_I32;
+        if (t.param.dtype != B200_F32) refuse(B200_DTYPE_ERROR, "param is F32");
+        if (!is_float(t.grad.dtype)) refuse(B200_DTYPE_ERROR, "grad is F32 or F16");
+        if (t.first.dtype != t.second.dtype || (!bytes && t.first.dtype != B200_F32)) refuse(B200_DTYPE_ERROR, "first and second are both F32, or both I32 words of bytes");
+        if (t.grad.ndim != t.param.ndim || !same_extents(t.grad, t.param, t.param.ndim)) refuse(B200_SHAPE_ERROR, "grad has not param's extents");
+        for (const b200_tensor* s : {&t.first, &t.second}) {
+            if (bytes ? s->ndim != 1 || s->dims[0] != ceil_div(n, 4) : s->ndim != t.param.ndim || !same_extents(*s, t.param, t.param.ndim)) {
+                refuse(B200_SHAPE_ERROR, "a state has not param's extents, or its number of bytes");
+            }
+        }
+        if (bytes ? n != 0 && !present(t.scales) : present(t.scales)) refuse(B200_INVALID_ARGUMENT, "scales go with 8-bit states, and only with them");
+        if (present(t.scales)) {
+            check_tensor(t.scales, "scales");
+            if (t.scales.dtype != B200_F32) refuse(B200_DTYPE_ERROR, "scales are F32");
+            if (t.scales.ndim != 2 || t.scales.dims[0] != ceil_div(n, kBlock) || t.scales.dims[1] != 2 || !is_dense(t.scales) || reinterpret_cast<uintptr_t>(t.scales.data) % 8 != 0) {
+                refuse(B200_SHAPE_ERROR, "scales: not two for every 256 elements, dense and 8-byte aligned");
+            }
+        }
+        if (present(t.copy)) {
+            check_tensor(t.copy, "copy");
+            if (t.copy.dtype != B200_F16) refuse(B200_DTYPE_ERROR, "copy is F16");
+            if (t.copy.ndim != t.param.ndim || !same_extents(t.copy, t.param, t.param.ndim)) refuse(B200_SHAPE_ERROR, "copy has not param's extents");
+            if (!is_dense(t.copy)) refuse(B200_NOT_IMPLEMENTED, "copy is not dense");
+        }
+        for (const b200_tensor* s : {&t.param, &t.grad, &t.first, &t.second}) {
+            if (!is_dense(*s)) refuse(B200_NOT_IMPLEMENTED, "a tensor is not dense");
+            if (n != 0 && !present(*s)) refuse(B200_INVALID_ARGUMENT, "a tensor has no storage");
+        }
+        if (!(t.weight_decay >= 0.f) || std::isinf(t.weight_decay) || !std::isfinite(t.lr_scale)) refuse(B200_INVALID_ARGUMENT, "weight_decay or lr_scale is not finite, or weight_decay below 0");
+        add(t.param, true);
+        add(t.grad, false);
+        add(t.first, true);
+        add(t.second, true);
+        if (present(t.scales)) add(t.scales, true);
+        if (present(t.copy)) add(t.copy, true);
+    }
+    add(a.lr_on_device, false);
+    add(a.step_on_device, false);
+    add(a.scale_on_device, false);
+    std::sort(ranges.begin(), ranges.end());
+    const char* reach[2] = {nullptr, nullptr};  // the farthest end so far, of what is read and of what is written
+    for (const Range& r : ranges) {
+        if (r.lo < reach[1] || (r.written && r.lo < reach[0])) fail(B200_INVALID_ARGUMENT, "adamw: a tensor that is written overlaps another");
+        reach[r.written] = std::max(reach[r.written], r.hi);
+    }
+}
+
+template <int N>
+void launch_table(b200_ctx* ctx, const Numbers& numbers, const std::vector<Tensor>& tensors, size_t first, size_t count, uint32_t items) {
+    static_assert(sizeof(Table<N>) <= 32764, "the launch's parameters");
+    Table<N> table;
+    table.numbers = numbers;
+    table.count = static_cast<int>(count);
+    std::copy_n(tensors.begin() + static_cast<std::ptrdiff_t>(first), count, table.t);
+    launch_kernel(ctx, adamw_kernel<N>, dim3(items), dim3(kThreads), 0, table);
+    check_last_launch("adamw");
+    ctx->count_launch();
+}
+
+void launch_adamw(b200_ctx* ctx, const b200_adamw_args& a) {
+    check_numbers(a);
+    check_tensors(a);
+    Numbers k{};
+    k.lr_at = static_cast<const float*>(a.lr_on_device.data);
+    k.step_at = static_cast<const int64_t*>(a.step_on_device.data);
+    k.scale_at = static_cast<const float*>(a.scale_on_device.data);
+    k.step = a.step;
+    k.lr = a.lr, k.eps = a.eps, k.scale = a.grad_scale, k.seed = a.seed;
+    k.b1 = static_cast<float>(a.beta1), k.rest1 = static_cast<float>(1 - a.beta1), k.log_b1 = static_cast<float>(std::log(a.beta1));
+    k.b2 = static_cast<float>(a.beta2), k.rest2 = static_cast<float>(1 - a.beta2), k.log_b2 = static_cast<float>(std::log(a.beta2));
+    k.inverse1 = static_cast<float>(1 / (1 - std::pow(a.beta1, static_cast<double>(a.step))));
+    k.root_inverse2 = static_cast<float>(1 / std::sqrt(1 - std::pow(a.beta2, static_cast<double>(a.step))));
+    std::vector<Tensor> tensors;
+    tensors.reserve(static_cast<size_t>(a.count));
+    for (int64_t i = 0; i < a.count; ++i) {
+        const b200_adamw_tensor& s = a.tensors[i];
+        if (numel_of(s.param) == 0) continue;
+        if (dist_has_pending(ctx)) wait_for_tensors(ctx, {&s.param, &s.grad, &s.first, &s.second, &s.scales, &s.copy});
+        Tensor t{};
+        t.param = static_cast<float*>(s.param.data);
+        t.grad = s.grad.data;
+        t.first = s.first.data;
+        t.second = s.second.data;
+        t.scales = static_cast<float2*>(s.scales.data);
+        t.copy = static_cast<__half*>(s.copy.data);
+        t.n = numel_of(s.param);
+        t.decay = s.weight_decay;
+        t.lr_scale = s.lr_scale;
+        t.number = static_cast<uint32_t>(i);
+        t.half_grad = s.grad.dtype == B200_F16;
+        auto on = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+        const uintptr_t state = t.scales != nullptr ? 8 : 32;
+        t.wide = on(t.param, 32) && on(t.grad, t.half_grad ? 16 : 32) && on(t.first, state) && on(t.second, state) && on(t.copy, 16);
+        tensors.push_back(t);
+    }
+    wait_for_tensors(ctx, {&a.lr_on_device, &a.step_on_device, &a.scale_on_device});
+    ProfScope scope(ctx, "adamw");
+    size_t done = 0;
+    while (done < tensors.size()) {
+        size_t count = 0;
+        int64_t items = 0;
+        while (done + count < tensors.size() && count < kMostTensors) {
+            const int64_t more = ceil_div(tensors[done + count].n, kItem);
+            if (items + more >= (int64_t(1) << 31)) break;
+            tensors[done + count].item = static_cast<uint32_t>(items);
+            items += more;
+            ++count;
+        }
+        if (count == 0) fail(B200_SHAPE_ERROR, "adamw: a tensor is too large");
+        launch_table<kMostTensors>(ctx, k, tensors, done, count, static_cast<uint32_t>(items));
+        done += count;
+    }
+}
+
+}  // namespace
+
+void check_adamw(const b200_adamw_args& a) {
+    check_numbers(a);
+    check_tensors(a);
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_adamw(b200_ctx* ctx, const b200_adamw_args* args) {
+    if (ctx == nullptr || args == nullptr) return B200_INVALID_ARGUMENT;
+    return guarded_operator(ctx, [&] { launch_adamw(ctx, *args); });
+}
+
+}  // extern "C"

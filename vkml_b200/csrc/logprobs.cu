@@ -1,0 +1,566 @@
+// Log probabilities of given tokens, the entropy of their distribution and its likeliest tokens, and the gradient of the first two.
+//
+// For a row z of V logits and temperature T, with u = (z - max) / T, s = sum e^u and q = e^u / s:
+//
+//   log q_j = u_j - log s        H = log s - (sum e^u u) / s
+//   grad = k [ a (one at token - q) - w q (log q + H) ] / T,  a and w the gradients of the token's log q and of H
+//
+// Bound by memory: z read once, and backward as much written.  A block takes a row: each thread keeps the maximum of what it has read and the sums of e^u and
+// e^u u beside it, and the block joins these threes.
+//
+// The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least
+// reach; it is found by halving the range between the maxima.  Only threads whose maximum reaches it (about K of them) read what they had again and put what reaches the
+// bound into shared memory, little more than K entries, where an entry's rank is the number of larger ones.  Where more entries reach it than there is room for (a
+// row of few different values: most of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in the order of
+// their columns.
+#include "operators.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace b200 {
+namespace {
+
+constexpr int kMostTop = B200_MOST_TOP;
+constexpr int kMostThreads = 512;
+constexpr int kRoom = 1280;  // entries: where fewer threads have elements than are wanted, all of a row's are (8 to each of 127, and the ends)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Args {
+    RowsArg logits, tokens, ids, tops, logprobs_grad, entropies_grad, grad;
+    float* logprobs;
+    float* entropies;
+    float4* stats;
+    FastDiv inner;
+    uint32_t* status;
+    int64_t vocab;
+    uint32_t rows;
+    int top;
+    bool wide_tokens, wide_ids;
+    float inverse, scale;  // 1 / T; backward: grad_scale / T
+};
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The larger one; no number where one of them is none.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float shift_of(float top) { return top == -INFINITY ? 0.f : top; }
+
+// Elements of a row that lie before its first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ int head_of(const T* row, int64_t n) {
+    const int64_t head = (16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / int64_t(sizeof(T));
+    return static_cast<int>(head < n ? head : n);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& raw, float (&x)[16 / sizeof(T)]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    }
+}
+
+// Whole numbers in the order of the logits: equal ones (0 and -0) alike, what is no number above all.
+__device__ __forceinline__ uint32_t order_of(float z) {
+    if (z != z) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(z + 0.f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order >> 31 ? order & 0x7fffffffu : ~order); }
+
+// The maximum, and beside it the sums of e^u and of e^u u in powers of two: 2^v and 2^v v, v = (z - max) log2 e / T.
+struct Part {
+    float top, sum, turned;
+};
+
+__device__ __forceinline__ void shift_part(Part& x, float top, float c) {
+    const float apart = (x.top - shift_of(top)) * c;
+    if (x.sum != 0.f) {  // (nothing so far: a maximum of -inf)
+        const float f = fast_exp2(apart);
+        x.turned = f * fmaf(apart, x.sum, x.turned);
+        x.sum *= f;
+        if (f == 0.f) x.turned = 0.f;  // (far below: no infinity times zero)
+    }
+    x.top = top;
+}
+
+__device__ __forceinline__ Part warp_part(Part x, float c) {
+    float top = x.top;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+    shift_part(x, top, c);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) {
+        x.sum += __shfl_xor_sync(0xffffffffu, x.sum, d);
+        x.turned += __shfl_xor_sync(0xffffffffu, x.turned, d);
+    }
+    return x;
+}
+
+// Adds elements to a part; those of -inf count as far below (a power of two of -150 is 0).
+template <int N>
+__device__ __forceinline__ void take(Part& part, const float (&z)[N], float c) {
+    float top = z[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = max_nan(top, z[e]);
+    top = max_nan(top, part.top);
+    if (!(top == part.top)) shift_part(part, top, c);
+    const float at = shift_of(top);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float v = max_nan((z[e] - at) * c, -150.f), p = fast_exp2(v);
+        part.sum += p;
+        part.turned = fmaf(p, v, part.turned);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMostThreads) logprobs_kernel(const Args k) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ Part parts[kMostThreads / 32];
+    __shared__ uint64_t entries[kRoom];
+    __shared__ int count;
+    __shared__ int before[kMostThreads / 32 + 1];
+    pdl_prologue();
+    const int tid = threadIdx.x, threads = blockDim.x, warps = threads / 32;
+    const uint32_t r = blockIdx.x;
+    const T* const z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
+    const int head = head_of(z, k.vocab);
+    const int vectors = static_cast<int>((k.vocab - head) / E), tail = head + vectors * E;
+    const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
+    const float c = k.inverse * kLog2e;
+
+    // an element of the row's ends for some threads
+    int end = -1;
+    if (tid < head) end = tid;
+    else if (tid >= 8 && tail + (tid - 8) < k.vocab) end = tail + (tid - 8);
+    Part part{-INFINITY, 0.f, 0.f};
+    if (end >= 0) {
+        const float one[1] = {to_float(z[end])};
+        take(part, one, c);
+    }
+    float token_z = 0.f;
+    bool token = false;
+    if (tid == 0 && k.tokens.base != nullptr) {
+        const int64_t id = load_index(row_at(k.tokens, k.inner, r), k.wide_tokens);
+        if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
+        token = id >= 0 && id < k.vocab;
+        if (token) token_z = to_float(z[id]);
+    }
+    int v = tid;
+    for (; v + 3 * threads < vectors; v += 4 * threads) {
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = zv[v + i * threads];
+        float x[4 * E];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float y[E];
+            unpack<T>(raw[i], y);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[i * E + e] = y[e];
+        }
+        take(part, x, c);
+    }
+    for (; v < vectors; v += threads) {
+        float x[E];
+        unpack<T>(zv[v], x);
+        take(part, x, c);
+    }
+    const float own_top = part.top;
+    const Part mine = warp_part(part, c);
+    if (tid % 32 == 0) parts[tid / 32] = mine;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    Part all = tid % 32 < warps ? parts[tid % 32] : Part{-INFINITY, 0.f, 0.f};
+    all = warp_part(all, c);
+    const bool some = all.sum != 0.f;  // (or no number)
+    const float at = shift_of(all.top);
+    const float log_sum = some ? logf(all.sum) : 0.f;
+    const float entropy = some ? log_sum - all.turned / all.sum * kLn2 : 0.f;
+    if (tid == 0) {
+        if (k.logprobs != nullptr) k.logprobs[r] = token ? (token_z - at) * k.inverse - log_sum : 0.f;
+        if (k.entropies != nullptr) k.entropies[r] = entropy;
+        if (k.stats != nullptr) k.stats[r] = make_float4(all.top, log_sum, entropy, 0.f);
+    }
+    if (k.top == 0) return;
+
+    // a bound that at least `top` elements reach
+    const bool owner = end >= 0 || tid < vectors;
+    const uint32_t own = owner ? order_of(own_top) : 0u;
+    uint32_t lo = 0, hi = order_of(all.top);
+    if (__syncthreads_count(own >= hi) >= k.top) lo = hi;
+    else {
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int n = __syncthreads_count(own >= mid);
+            if (n >= k.top) lo = mid;
+            else hi = mid;
+            if (n == k.top) break;
+        }
+    }
+    auto each = [&](auto&& visit) {  // of this thread's elements: (order, column)
+        if (end >= 0) visit(order_of(to_float(z[end])), static_cast<uint32_t>(end));
+        for (int i = tid; i < vectors; i += threads) {
+            float x[E];
+            unpack<T>(zv[i], x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) visit(order_of(x[e]), static_cast<uint32_t>(head + i * E + e));
+        }
+    };
+    auto counted = [&](uint32_t bound) {  // how many of the row's elements reach a bound
+        int n = 0;
+        if (own >= bound) each([&](uint32_t o, uint32_t) { n += o >= bound; });
+        n = __reduce_add_sync(0xffffffffu, n);
+        __syncthreads();
+        if (tid % 32 == 0) before[tid / 32] = n;
+        __syncthreads();
+        n = tid % 32 < warps ? before[tid % 32] : 0;
+        return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+    };
+    auto collect = [&](uint32_t bound) {
+        if (own >= bound && owner) {
+            each([&](uint32_t o, uint32_t column) {
+                if (o < bound) return;
+                const int i = atomicAdd(&count, 1);
+                if (i < kRoom) entries[i] = uint64_t(o) << 32 | (0xffffffffu - column);
+            });
+        }
+        __syncthreads();
+    };
+    collect(lo);
+    int n = count;
+    if (n > kRoom) {
+        uint32_t top = 0xffffffffu;  // the largest number that K elements reach, or one whose entries there is room for
+        if (counted(0xffffffffu) >= k.top) lo = 0xffffffffu;
+        else {
+            while (top - lo > 1) {
+                const uint32_t mid = lo + (top - lo) / 2;
+                const int reach = counted(mid);
+                if (reach >= k.top) {
+                    lo = mid;
+                    if (reach <= kRoom) break;
+                } else {
+                    top = mid;
+                }
+            }
+        }
+        const int equal_too = counted(lo);
+        __syncthreads();
+        if (tid == 0) count = 0;
+        __syncthreads();
+        if (equal_too <= kRoom) {
+            collect(lo);
+        } else {
+            // fewer than K are larger; of the equal ones those of the lowest columns
+            if (lo != 0xffffffffu) collect(lo + 1);
+            int have = count;
+            for (int64_t from = 0; from < k.vocab && have < k.top; from += threads) {
+                const int64_t column = from + tid;
+                const bool hit = column < k.vocab && order_of(to_float(z[column])) == lo;
+                const uint32_t ballot = __ballot_sync(0xffffffffu, hit);
+                __syncthreads();
+                if (tid % 32 == 0) before[tid / 32] = __popc(ballot);
+                __syncthreads();
+                int at_most = have, in_front = have;
+                for (int w = 0; w < warps; ++w) {
+                    if (w < tid / 32) in_front += before[w];
+                    at_most += before[w];
+                }
+                const int i = in_front + __popc(ballot & ((1u << tid % 32) - 1));
+                if (hit && i < k.top) entries[i] = uint64_t(lo) << 32 | (0xffffffffu - static_cast<uint32_t>(column));
+                have = min(at_most, k.top);
+            }
+            __syncthreads();
+            if (tid == 0) count = have;
+            __syncthreads();
+        }
+        n = count;
+    }
+    char* const ids = k.ids.base != nullptr ? row_at(k.ids, k.inner, r) : nullptr;
+    float* const tops = k.tops.base != nullptr ? reinterpret_cast<float*>(row_at(k.tops, k.inner, r)) : nullptr;
+    for (int i = tid; i < n; i += threads) {
+        const uint64_t entry = entries[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += entries[j] > entry;
+        if (rank >= k.top) continue;
+        const uint32_t column = 0xffffffffu - static_cast<uint32_t>(entry);
+        if (ids != nullptr) {
+            if (k.wide_ids) reinterpret_cast<int64_t*>(ids)[rank] = column;
+            else reinterpret_cast<int32_t*>(ids)[rank] = static_cast<int32_t>(column);
+        }
+        if (tops != nullptr) tops[rank] = (value_of(static_cast<uint32_t>(entry >> 32)) - at) * k.inverse - log_sum;
+    }
+}
+
+// ---- the gradient -----------------------------------------------------------
+
+constexpr int kGradThreads = 256;
+constexpr int kGradVectors = 4;
+
+// What a row's gradient is made of: q (plain + turned log q), and `given` at the token.
+struct RowGrad {
+    float at, log_sum, plain, turned, given;
+    int64_t token;
+};
+
+__device__ __forceinline__ float grad_of(const RowGrad& g, float inverse, float z) {
+    const float log_q = max_nan(fmaf(z - g.at, inverse, -g.log_sum), -200.f);
+    return fast_exp2(log_q * kLog2e) * fmaf(g.turned, log_q, g.plain);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const Args k, uint32_t pieces) {
+    constexpr int E = 16 / sizeof(T);
+    pdl_prologue();
+    const int tid = threadIdx.x;
+    const uint32_t r = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+    const T* const z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
+    T* const to = reinterpret_cast<T*>(row_at(k.grad, k.inner, r));
+    const int head = head_of(z, k.vocab);
+    const int64_t vectors = (k.vocab - head) / E;
+    const int64_t tail = head + vectors * E;
+    RowGrad g{};
+    g.token = -1;
+    if (k.tokens.base != nullptr) {
+        g.token = load_index(row_at(k.tokens, k.inner, r), k.wide_tokens);
+        if (g.token >= k.vocab) {
+            if (tid == 0) atomicOr(k.status, kStatusIndexOutOfRange);
+            g.token = -1;
+        }
+    }
+    const float4 stats = k.stats[r];
+    const float a = k.logprobs_grad.base != nullptr && g.token >= 0 ? *reinterpret_cast<const float*>(row_at(k.logprobs_grad, k.inner, r)) : 0.f;
+    const float w = k.entropies_grad.base != nullptr ? *reinterpret_cast<const float*>(row_at(k.entropies_grad, k.inner, r)) : 0.f;
+    const bool zero = (a == 0.f && w == 0.f) || stats.x == -INFINITY;
+    g.at = stats.x;
+    g.log_sum = stats.y;
+    g.given = a * k.scale;
+    g.turned = -w * k.scale;
+    g.plain = -(a + w * stats.z) * k.scale;
+    if (zero) g.given = 0.f;
+    const bool aligned = reinterpret_cast<uintptr_t>(to + head) % 16 == 0;
+    auto value = [&](float x, int64_t column) { return (zero ? 0.f : grad_of(g, k.inverse, x)) + (column == g.token ? g.given : 0.f); };
+    if (piece == 0) {
+        if (tid < head) to[tid] = from_float<T>(value(zero ? 0.f : to_float(z[tid]), tid));
+        const int64_t column = tail + (tid - 8);
+        if (tid >= 8 && column < k.vocab) to[column] = from_float<T>(value(zero ? 0.f : to_float(z[column]), column));
+    }
+    const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
+    const int64_t first = int64_t(piece) * (kGradThreads * kGradVectors) + tid;
+    uint4 raw[kGradVectors];
+#pragma unroll
+    for (int i = 0; i < kGradVectors; ++i) {
+        const int64_t v = first + i * kGradThreads;
+        raw[i] = !zero && v < vectors ? zv[v] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kGradVectors; ++i) {
+        const int64_t v = first + i * kGradThreads;
+        if (v >= vectors) break;
+        float x[E];
+        unpack<T>(raw[i], x);
+        const int64_t column = head + v * E;
+        if (zero) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = 0.f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = grad_of(g, k.inverse, x[e]);
+            if (g.token >= column && g.token < column + E) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] += g.token == column + e ? g.given : 0.f;
+            }
+        }
+        T* const p = to + column;
+        if (aligned) {
+            uint32_t out[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 2) {
+                    const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                    out[j] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    out[j] = __float_as_uint(x[j]);
+                }
+            }
+            *reinterpret_cast<uint4*>(p) = make_uint4(out[0], out[1], out[2], out[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) p[e] = from_float<T>(x[e]);
+        }
+    }
+}
+
+// ---- arguments --------------------------------------------------------------
+
+bool present(const b200_tensor& t) { return t.data != nullptr; }
+
+struct Plan {
+    int axes;
+    int64_t vocab, top;
+    RowShape s;
+    bool told;  // tokens are given
+};
+
+void check_one_each(const b200_tensor& t, const char* name, const b200_tensor& logits, bool dense) {
+    check_tensor(t, name);
+    if (t.ndim != logits.ndim - 1 || !same_extents(t, logits, t.ndim)) fail(B200_SHAPE_ERROR, std::string(name) + ": not one for each row of logits");
+    if (t.dtype != B200_F32) fail(B200_DTYPE_ERROR, std::string(name) + " is F32");
+    if (dense && !is_dense(t)) fail(B200_NOT_IMPLEMENTED, std::string(name) + " is not dense");
+}
+
+Plan check_logprobs(const b200_token_logprobs_args& a, bool forward) {
+    check_rows(a.logits, "logits");
+    if (!is_float(a.logits.dtype)) fail(B200_DTYPE_ERROR, "logits are F32 or F16");
+    const int axes = a.logits.ndim - 1;
+    Plan plan{axes, a.logits.dims[axes], 0, row_shape(a.logits, axes), false};
+    if (plan.vocab < 1 || plan.vocab >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "logits: rows of no element, or of 2^31 or more");
+    if (!(a.temperature > 0.f) || std::isinf(a.temperature) || std::isinf(1.f / a.temperature * kLog2e)) {
+        fail(B200_INVALID_ARGUMENT, "token_logprobs: the temperature is not above 0 and finite, or its inverse times log2 e is not");
+    }
+    plan.told = !is_absent(a.tokens, "tokens");
+    if (plan.told) {
+        check_tensor(a.tokens, "tokens");
+        if (a.tokens.ndim != axes || !same_extents(a.tokens, a.logits, axes)) fail(B200_SHAPE_ERROR, "tokens: not one for each row of logits");
+        if (!is_index(a.tokens.dtype)) fail(B200_DTYPE_ERROR, "tokens are I32 or I64");
+    }
+    for (const Named& t : {Named{&a.logprobs, "logprobs"}, Named{&a.entropies, "entropies"}}) {
+        if (present(*t.t)) check_one_each(*t.t, t.name, a.logits, true);
+    }
+    for (const Named& t : {Named{&a.logprobs_grad, "logprobs_grad"}, Named{&a.entropies_grad, "entropies_grad"}}) {
+        if (present(*t.t)) check_one_each(*t.t, t.name, a.logits, false);
+    }
+    if (present(a.stats)) check_stats(a.stats, plan.s.rows);
+    for (const Named& t : {Named{&a.top_ids, "top_ids"}, Named{&a.top_logprobs, "top_logprobs"}}) {
+        if (!present(*t.t)) continue;
+        check_rows(*t.t, t.name);
+        if (t.t->ndim != a.logits.ndim || !same_extents(*t.t, a.logits, axes)) fail(B200_SHAPE_ERROR, std::string(t.name) + ": rows of other extents than logits");
+        plan.top = t.t->dims[axes];
+    }
+    if (present(a.top_ids) && !is_index(a.top_ids.dtype)) fail(B200_DTYPE_ERROR, "top_ids are I32 or I64");
+    if (present(a.top_logprobs) && a.top_logprobs.dtype != B200_F32) fail(B200_DTYPE_ERROR, "top_logprobs are F32");
+    if (present(a.top_ids) && present(a.top_logprobs) && a.top_ids.dims[axes] != a.top_logprobs.dims[axes]) fail(B200_SHAPE_ERROR, "top_ids and top_logprobs have different widths");
+    if (plan.top > plan.vocab) fail(B200_SHAPE_ERROR, "token_logprobs: more of the largest logits than a row has");
+    if (plan.top > kMostTop) fail(B200_NOT_IMPLEMENTED, "token_logprobs: more than 128 of the largest logits");
+    if (present(a.grad)) {
+        check_rows(a.grad, "grad");
+        if (a.grad.ndim != a.logits.ndim || !same_extents(a.grad, a.logits, a.logits.ndim)) fail(B200_SHAPE_ERROR, "grad has not the logits' extents");
+        if (a.grad.dtype != a.logits.dtype) fail(B200_DTYPE_ERROR, "grad has not the logits' type");
+    }
+    if (forward) {
+        if (present(a.grad) || present(a.logprobs_grad) || present(a.entropies_grad)) fail(B200_INVALID_ARGUMENT, "token_logprobs computes no gradient");
+        check_results({{&a.logprobs, "logprobs"}, {&a.entropies, "entropies"}, {&a.stats, "stats"}, {&a.top_ids, "top_ids"}, {&a.top_logprobs, "top_logprobs"}},
+                      {{&a.logits, "logits"}, {&a.tokens, "tokens"}}, {});
+    } else {
+        if (present(a.logprobs) || present(a.entropies) || present(a.top_ids) || present(a.top_logprobs)) fail(B200_INVALID_ARGUMENT, "token_logprobs_backward computes the gradient alone");
+        check_results({{&a.grad, "grad"}}, {{&a.tokens, "tokens"}, {&a.logprobs_grad, "logprobs_grad"}, {&a.entropies_grad, "entropies_grad"}, {&a.stats, "stats"}}, {{&a.logits, "logits"}});
+    }
+    if (plan.s.rows == 0) return plan;
+    if (forward) {
+        if (!present(a.logprobs) && !present(a.entropies) && !present(a.stats) && plan.top == 0) fail(B200_INVALID_ARGUMENT, "token_logprobs: no result is asked for");
+        if (present(a.logprobs) && !plan.told) fail(B200_INVALID_ARGUMENT, "token_logprobs: log probabilities of no tokens");
+    } else {
+        if (!present(a.grad) || !present(a.stats)) fail(B200_INVALID_ARGUMENT, "token_logprobs_backward: grad and the forward call's stats are needed");
+        if (present(a.logprobs_grad) && !plan.told) fail(B200_INVALID_ARGUMENT, "token_logprobs_backward: gradients of no tokens");
+    }
+    return plan;
+}
+
+// Blocks that a row's gradient takes.
+int64_t grad_pieces(int64_t vocab, bool half) {
+    const int64_t vectors = vocab / (half ? 8 : 4);
+    return std::max<int64_t>(1, ceil_div(vectors, kGradThreads * kGradVectors));
+}
+
+Args common_args(b200_ctx* ctx, const b200_token_logprobs_args& a, const Plan& plan) {
+    Args k{};
+    k.logits = rows_arg(a.logits, plan.axes);
+    if (plan.told) k.tokens = rows_arg(a.tokens, plan.axes);
+    k.stats = static_cast<float4*>(a.stats.data);
+    k.inner = FastDiv(static_cast<uint32_t>(plan.s.inner));
+    k.status = ctx->d_status;
+    k.vocab = plan.vocab;
+    k.rows = static_cast<uint32_t>(plan.s.rows);
+    k.wide_tokens = a.tokens.dtype == B200_I64;
+    k.inverse = 1.f / a.temperature;
+    return k;
+}
+
+void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
+    const Plan plan = check_logprobs(a, true);
+    if (plan.s.rows == 0) return;
+    wait_for_tensors(ctx, {&a.logits, &a.tokens, &a.logprobs, &a.entropies, &a.stats, &a.top_ids, &a.top_logprobs});
+    Args k = common_args(ctx, a, plan);
+    k.logprobs = static_cast<float*>(a.logprobs.data);
+    k.entropies = static_cast<float*>(a.entropies.data);
+    if (present(a.top_ids)) k.ids = rows_arg(a.top_ids, plan.axes);
+    if (present(a.top_logprobs)) k.tops = rows_arg(a.top_logprobs, plan.axes);
+    k.top = static_cast<int>(plan.top);
+    k.wide_ids = a.top_ids.dtype == B200_I64;
+    ProfScope scope(ctx, "token_logprobs");
+    const bool half = a.logits.dtype == B200_F16;
+    const int threads = plan.vocab * (half ? 2 : 4) > 16384 ? kMostThreads : 128;
+    launch_kernel(ctx, half ? logprobs_kernel<__half> : logprobs_kernel<float>, dim3(k.rows), dim3(threads), 0, k);
+    check_last_launch("token_logprobs");
+    ctx->count_launch();
+}
+
+void launch_logprobs_backward(b200_ctx* ctx, const b200_token_logprobs_args& a) {
+    const Plan plan = check_logprobs(a, false);
+    if (plan.s.rows == 0) return;
+    const bool half = a.logits.dtype == B200_F16;
+    const int64_t pieces = grad_pieces(plan.vocab, half);
+    if (plan.s.rows * pieces >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "token_logprobs_backward: too many rows of this length");
+    wait_for_tensors(ctx, {&a.logits, &a.tokens, &a.stats, &a.logprobs_grad, &a.entropies_grad, &a.grad});
+    Args k = common_args(ctx, a, plan);
+    if (present(a.logprobs_grad)) k.logprobs_grad = rows_arg(a.logprobs_grad, plan.axes);
+    if (present(a.entropies_grad)) k.entropies_grad = rows_arg(a.entropies_grad, plan.axes);
+    k.grad = rows_arg(a.grad, plan.axes);
+    k.scale = a.grad_scale / a.temperature;
+    ProfScope scope(ctx, "token_logprobs_backward");
+    launch_kernel(ctx, half ? logprobs_grad_kernel<__half> : logprobs_grad_kernel<float>, dim3(static_cast<unsigned>(plan.s.rows * pieces)), dim3(kGradThreads), 0, k, static_cast<uint32_t>(pieces));
+    check_last_launch("token_logprobs_backward");
+    ctx->count_launch();
+}
+
+}  // namespace
+
+void check_token_logprobs(const b200_token_logprobs_args& a, bool forward) {
+    const Plan plan = check_logprobs(a, forward);
+    if (!forward && plan.s.rows * grad_pieces(plan.vocab, a.logits.dtype == B200_F16) >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "token_logprobs_backward: too many rows of this length");
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_token_logprobs(b200_ctx* ctx, const b200_token_logprobs_args* args) {
+    if (ctx == nullptr || args == nullptr) return B200_INVALID_ARGUMENT;
+    return guarded_operator(ctx, [&] { launch_logprobs(ctx, *args); });
+}
+
+int b200_token_logprobs_backward(b200_ctx* ctx, const b200_token_logprobs_args* args) {
+    if (ctx == nullptr || args == nullptr) return B200_INVALID_ARGUMENT;
+    return guarded_operator(ctx, [&] { launch_logprobs_backward(ctx, *args); });
+}
+
+}  // extern "C"

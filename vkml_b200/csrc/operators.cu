@@ -21,6 +21,13 @@ int b200_check_operator(int which, const void* args, char* why, size_t why_len) 
             case B200_CALL_DISTILL_LOSS_BACKWARD:
                 check_distill_loss(*static_cast<const b200_distill_args*>(args), which == B200_CALL_DISTILL_LOSS);
                 break;
+            case B200_CALL_GATED_RECURRENCE: check_gated_recurrence(*static_cast<const b200_recurrence_args*>(args)); break;
+            case B200_CALL_GATED_RECURRENCE_BACKWARD: check_gated_recurrence_backward(*static_cast<const b200_recurrence_grad_args*>(args)); break;
+            case B200_CALL_TOKEN_LOGPROBS:
+            case B200_CALL_TOKEN_LOGPROBS_BACKWARD:
+                check_token_logprobs(*static_cast<const b200_token_logprobs_args*>(args), which == B200_CALL_TOKEN_LOGPROBS);
+                break;
+            case B200_CALL_ADAMW: check_adamw(*static_cast<const b200_adamw_args*>(args)); break;
             default: status = B200_INVALID_ARGUMENT; message = "unknown operator";
         }
     } catch (const Error& e) {

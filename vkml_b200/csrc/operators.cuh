@@ -1,4 +1,4 @@
-// What the operators of language-model training (embedding.cu, block_norm.cu, distill.cu) share: checks of their
+// What the operators of language-model training (embedding.cu, block_norm.cu, distill.cu, recurrence.cu, logprobs.cu, adamw.cu) share: checks of their
 // arguments, rows of strided tensors, workspaces, and wide accesses.
 #pragma once
 
@@ -276,6 +276,10 @@ void check_embedding_call(const b200_embedding_args& a, bool backward);
 void check_block_norm(const b200_block_norm_args& a);
 void check_block_norm_backward(const b200_block_norm_grad_args& a);
 void check_distill_loss(const b200_distill_args& a, bool forward);
+void check_gated_recurrence(const b200_recurrence_args& a);
+void check_gated_recurrence_backward(const b200_recurrence_grad_args& a);
+void check_token_logprobs(const b200_token_logprobs_args& a, bool forward);
+void check_adamw(const b200_adamw_args& a);
 
 // How many blocks of a kernel an SM of the current device holds at once; allows the kernel that much shared memory.
 inline int blocks_at_once(const void* kernel, int threads, size_t shared) {

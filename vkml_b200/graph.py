@@ -222,10 +222,21 @@ _EMBEDDING_TAIL = struct.Struct("<fIqQQ")
 _NORM_TAIL = struct.Struct("<fffiI4x")
 _NORM_GRAD_TAIL = struct.Struct("<ffiIQQ")
 _DISTILL_TAIL = struct.Struct("<fff4x")
+GATE_KINDS = {"sigmoid": 0, "exp": 1}
+RECURRENCE_CHUNK = 16
+ADAMW_BLOCK = 256
+_RECURRENCE_TAIL = struct.Struct("<iI")
+_LOGPROBS_TAIL = struct.Struct("<ff")
+_ADAMW_ENTRY_TAIL = struct.Struct("<ff")
+_ADAMW_HEAD = struct.Struct("<Qq")
+_ADAMW_TAIL = struct.Struct("<q2d3fI")
 _ABSENT = bytes(_TENSOR_WORDS.size)
 for _tail, _tensors, _args in ((_EMBEDDING_TAIL, 3, _abi.EmbeddingArgs), (_NORM_TAIL, 10, _abi.BlockNormArgs),
-                               (_NORM_GRAD_TAIL, 16, _abi.BlockNormGradArgs), (_DISTILL_TAIL, 8, _abi.DistillArgs)):
+                               (_NORM_GRAD_TAIL, 16, _abi.BlockNormGradArgs), (_DISTILL_TAIL, 8, _abi.DistillArgs),
+                               (_RECURRENCE_TAIL, 7, _abi.RecurrenceArgs), (_RECURRENCE_TAIL, 9, _abi.RecurrenceGradArgs),
+                               (_LOGPROBS_TAIL, 10, _abi.TokenLogprobsArgs), (_ADAMW_ENTRY_TAIL, 6, _abi.AdamWTensor)):
     assert _tensors * _TENSOR_WORDS.size + _tail.size == ctypes.sizeof(_args)
+assert _ADAMW_HEAD.size + 3 * _TENSOR_WORDS.size + _ADAMW_TAIL.size == ctypes.sizeof(_abi.AdamWArgs)
 
 
 def tensors_bytes(tensors: Sequence) -> bytes:
@@ -253,3 +264,58 @@ def block_norm_grad_args(tensors, residual_scale, branch_scale, kind, flags, wor
 
 def distill_args(tensors, temperature, hard_weight, grad_scale) -> bytes:
     return tensors_bytes(tensors) + _DISTILL_TAIL.pack(temperature, hard_weight, grad_scale)
+
+
+def recurrence_args(tensors, kind) -> bytes:
+    """x, gate, initial, lengths, out, final, states; or x, gate, lengths, states, out_grad, final_grad, x_grad, gate_grad, initial_grad."""
+    return tensors_bytes(tensors) + _RECURRENCE_TAIL.pack(kind, 0)
+
+
+def logprobs_args(tensors, temperature, grad_scale) -> bytes:
+    return tensors_bytes(tensors) + _LOGPROBS_TAIL.pack(temperature, grad_scale)
+
+
+@dataclass
+class AdamWTensor:
+    """A tensor of an optimiser's step: what it is, its gradient and its states (F32 like it; or 8-bit ones, I32 words of four bytes, with
+    their scales), and where its new value goes in F16 besides."""
+    param: object
+    grad: object
+    first: object
+    second: object
+    scales: object = None
+    copy: object = None
+    weight_decay: float = 0.0
+    lr_scale: float = 1.0
+
+    @staticmethod
+    def state_dims(count: int) -> tuple:
+        """((words of 8-bit states), (rows of scales, 2)) for a tensor of `count` elements."""
+        return (-(-count // 4),), (-(-count // ADAMW_BLOCK), 2)
+
+
+@dataclass
+class AdamWTable:
+    """An optimiser's tensors as the library reads them, described once for all steps."""
+    data: bytes
+    count: int
+    tensors: tuple  # (kept: the storages must live as long as the table)
+
+
+def adamw_table(tensors: Sequence[AdamWTensor]) -> AdamWTable:
+    parts = [tensors_bytes((t.param, t.grad, t.first, t.second, t.scales, t.copy)) + _ADAMW_ENTRY_TAIL.pack(t.weight_decay, t.lr_scale)
+             for t in tensors]
+    return AdamWTable(b"".join(parts), len(parts), tuple(tensors))
+
+
+_one = (int, float, np.integer, np.floating)
+
+
+def adamw_args(table: AdamWTable, lr, step, beta1, beta2, eps, grad_scale, seed) -> tuple:
+    """(the arguments' bytes, what they point to): lr, step and grad_scale are numbers, or one-element tensors on the device."""
+    on_device = [None if isinstance(v, _one) else v for v in (lr, step, grad_scale)]
+    buffer = ctypes.c_char_p(table.data)
+    head = _ADAMW_HEAD.pack(ctypes.cast(buffer, ctypes.c_void_p).value or 0, table.count)
+    return head + tensors_bytes(on_device) + _ADAMW_TAIL.pack(
+        1 if on_device[1] is not None else step, beta1, beta2, 0.0 if on_device[0] is not None else lr, eps,
+        1.0 if on_device[2] is not None else grad_scale, seed & 0xFFFFFFFF), buffer
