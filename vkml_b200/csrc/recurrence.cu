@@ -189,6 +189,324 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
     if (k.initial.base != nullptr) reinterpret_cast<float*>(k.initial.base + b * k.initial.step)[ch] = e;
 }
 
+// ---- blocks that walk along a sequence --------------------------------------
+//
+// A block, or a cluster of blocks, has 32 lanes' channels of a sequence and walks along it window by window; a warp has 16 steps of a window.  A thread computes what
+// its steps do to a state that comes in (a decay and a sum: a step like any other), the warps tell each other by shared memory, the cluster's blocks by each
+// other's, and every thread goes through its steps again from the state that does come in.  All of it stays in registers: gates and inputs are read once, and the
+// next window's are under way while this one is computed.
+
+constexpr int kMostWarps = 8;
+constexpr int kMostCluster = 8;
+
+// VEC neighbouring channels of a lane as they lie in memory, and as floats.
+template <typename T, int VEC>
+struct Raw {
+    T a;
+    __device__ __forceinline__ void load(const char* p) { a = *reinterpret_cast<const T*>(p); }
+    __device__ __forceinline__ void clear() { a = from_float<T>(0.f); }
+    __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = to_float(a); }
+    static __device__ __forceinline__ void store(char* p, const float (&x)[1]) { *reinterpret_cast<T*>(p) = from_float<T>(x[0]); }
+};
+template <>
+struct Raw<__half, 2> {
+    uint32_t a;
+    __device__ __forceinline__ void load(const char* p) { a = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ __forceinline__ void clear() { a = 0; }
+    __device__ __forceinline__ void get(float (&x)[2]) const {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+        x[0] = f.x, x[1] = f.y;
+    }
+    static __device__ __forceinline__ void store(char* p, const float (&x)[2]) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x[0], x[1]); }
+};
+template <>
+struct Raw<float, 2> {
+    float2 a;
+    __device__ __forceinline__ void load(const char* p) { a = *reinterpret_cast<const float2*>(p); }
+    __device__ __forceinline__ void clear() { a = make_float2(0.f, 0.f); }
+    __device__ __forceinline__ void get(float (&x)[2]) const { x[0] = a.x, x[1] = a.y; }
+    static __device__ __forceinline__ void store(char* p, const float (&x)[2]) { *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]); }
+};
+
+// What a run of steps does to the state in front of it: their decays' product, as such and less 1 (either keeps digits that the other loses).
+struct Product {
+    float a = 1.f, less = 0.f;
+    __device__ __forceinline__ void then(float c) {
+        const float a1 = keeps(c) ? 1.f + c : c, less1 = keeps(c) ? c : c - 1.f;
+        a *= a1;
+        less = fmaf(less, less1, less) + less1;
+    }
+    __device__ __forceinline__ float decay() const { return less <= 0.f && less > -0.5f ? -fabsf(less) : a; }
+};
+// The decay of two runs, one behind the other.
+__device__ __forceinline__ float both(float c, float d) {
+    const float less = fmaf(c, d, c) + d;
+    const float product = (keeps(c) ? 1.f + c : c) * (keeps(d) ? 1.f + d : d);
+    return keeps(c) && keeps(d) ? (less > -0.5f ? -fabsf(less) : 1.f + less) : product;
+}
+
+// What the segments of a block, and the blocks of a cluster, do to a state: decay and sum, for every channel.  Two of each: a window's are read while the next one's
+// are written.
+template <int VEC>
+struct Told {
+    float2 segments[2][kMostWarps][32 * VEC];
+    float2 blocks[2][kMostCluster][32 * VEC];
+};
+
+__device__ __forceinline__ void tell(float2* mine, uint32_t rank, float2 value) {
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(value.x), "f"(value.y) : "memory");
+}
+
+// The state that comes into this warp's steps, from `carry` in front of the window (which becomes that behind it), by every segment's decay and sum.  Segments
+// come one after another, in the order of their warps and blocks, or (BACK) the other way round.
+template <int VEC, bool BACK>
+__device__ __forceinline__ void join(Told<VEC>& told, int parity, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, const float2 (&own)[VEC], float (&carry)[VEC], float (&in)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) told.segments[parity][warp][e * 32 + lane] = own[e];
+    __syncthreads();
+    float begin[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) begin[e] = carry[e];
+    if (cluster > 1) {
+        float2 block[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) block[e] = make_float2(kHold, 0.f);
+        for (int i = 0; i < warps; ++i) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float2 s = told.segments[parity][BACK ? warps - 1 - i : i][e * 32 + lane];
+                block[e] = make_float2(both(block[e].x, s.x), apply(s.x, block[e].y, s.y));
+            }
+        }
+        for (uint32_t to = warp; to < cluster; to += warps) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) tell(&told.blocks[parity][rank][e * 32 + lane], to, block[e]);
+        }
+        cluster_sync();
+        for (uint32_t i = 0; i < cluster; ++i) {
+            const uint32_t of = BACK ? cluster - 1 - i : i;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (of == rank) begin[e] = carry[e];
+                const float2 s = told.blocks[parity][of][e * 32 + lane];
+                carry[e] = apply(s.x, carry[e], s.y);
+            }
+        }
+    }
+    for (int i = 0; i < warps; ++i) {
+        const int of = BACK ? warps - 1 - i : i;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if (of == warp) in[e] = begin[e];
+            const float2 s = told.segments[parity][of][e * 32 + lane];
+            begin[e] = apply(s.x, begin[e], s.y);
+        }
+    }
+    if (cluster == 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) carry[e] = begin[e];
+    }
+}
+
+// Where a thread works: its sequence, channels, and place in a window.
+template <int VEC>
+struct Place {
+    int b, ch, warp, lane, warps;
+    uint32_t rank, cluster;
+    bool in;
+    __device__ __forceinline__ Place(const Args& k, uint32_t strips, uint32_t blocks) {
+        cluster = blocks;
+        rank = blockIdx.x % blocks;
+        const uint32_t i = blockIdx.x / blocks;
+        b = static_cast<int>(i / strips);
+        warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        ch = static_cast<int>(i % strips) * (32 * VEC) + lane * VEC;
+        in = ch < k.width;
+    }
+    __device__ __forceinline__ int64_t span() const { return int64_t(warps) * kSteps * cluster; }
+    __device__ __forceinline__ int64_t first() const { return int64_t(rank * warps + warp) * kSteps; }
+    template <typename T>
+    __device__ __forceinline__ char* base(const Stream& s) const { return s.base != nullptr ? s.base + b * s.batch + int64_t(ch) * int64_t(sizeof(T)) : nullptr; }
+};
+
+// Sixteen steps of a stream, from step t on, where they are before n.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_steps(Raw<T, VEC> (&r)[kSteps], const char* base, int64_t step, int64_t t, int64_t n, bool in) {
+    const char* p = base + t * step;
+    if (in && t + kSteps <= n) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) r[j].load(p + j * step);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            r[j].clear();
+            if (in && t + j < n) r[j].load(p + j * step);
+        }
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, int b, int ch, bool in) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] = end.base != nullptr && in ? reinterpret_cast<const float*>(end.base + b * end.step)[ch + e] : 0.f;
+}
+
+template <typename T, typename G, int KIND, int VEC>
+__global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    __shared__ Told<VEC> told;
+    pdl_prologue();
+    if (cluster > 1) cluster_sync();  // (every block is there before another writes to it)
+    const Place<VEC> at(k, strips, cluster);
+    const int64_t n = steps_of(k, at.b), span = at.span();
+    const char *const x = at.template base<T>(k.x), *const gate = at.template base<G>(k.gate);
+    char* const out = at.template base<T>(k.out);
+    Raw<T, VEC> rx[kSteps];
+    Raw<G, VEC> rg[kSteps];
+    int64_t t = at.first();
+    load_steps(rx, x, k.x.step, t, n, at.in);
+    load_steps(rg, gate, k.gate.step, t, n, at.in);
+    float carry[VEC];
+    load_end<VEC>(carry, k.initial, at.b, at.ch, at.in);
+    int parity = 0;
+    for (int64_t begin = 0; begin < k.length; begin += span, t += span, parity ^= 1) {
+        float c[kSteps][VEC], b[kSteps][VEC];
+        Product product[VEC];
+        float sum[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            float xs[VEC], gs[VEC];
+            rx[j].get(xs);
+            rg[j].get(gs);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float input;
+                c[j][e] = decay<KIND>(gs[e], input);
+                b[j][e] = input * xs[e];
+                if (t + j >= n) c[j][e] = kHold, b[j][e] = 0.f;
+                product[e].then(c[j][e]);
+                sum[e] = apply(c[j][e], sum[e], b[j][e]);
+            }
+        }
+        if (begin + span < k.length) {
+            load_steps(rx, x, k.x.step, t + span, n, at.in);
+            load_steps(rg, gate, k.gate.step, t + span, n, at.in);
+        }
+        float2 own[VEC];
+        float h[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) own[e] = make_float2(product[e].decay(), sum[e]);
+        join<VEC, false>(told, parity, at.warp, at.lane, at.warps, at.rank, at.cluster, own, carry, h);
+        if (!at.in || t >= k.length) continue;
+        if (k.states != nullptr) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
+        char* p = out + t * k.out.step;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            float y[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                h[e] = apply(c[j][e], h[e], b[j][e]);
+                y[e] = t + j < n ? h[e] : 0.f;
+            }
+            if (t + j < k.length) Raw<T, VEC>::store(p + j * k.out.step, y);
+        }
+    }
+    if (k.final_state.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(k.final_state.base + at.b * k.final_state.step)[at.ch + e] = carry[e];
+    }
+}
+
+constexpr int kBackWarps = 4;
+
+template <typename T, typename G, int KIND, int VEC>
+__global__ void __launch_bounds__(32 * kBackWarps, 3) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    __shared__ Told<VEC> told;
+    pdl_prologue();
+    if (cluster > 1) cluster_sync();  // (every block is there before another writes to it)
+    const Place<VEC> at(k, strips, cluster);
+    const int64_t n = steps_of(k, at.b), span = at.span();
+    const char *const x = at.template base<T>(k.x), *const gate = at.template base<G>(k.gate), *const dout = at.template base<T>(k.dout);
+    char *const dx = at.template base<T>(k.dx), *const dgate = at.template base<G>(k.dgate);
+    const float* const states = k.states + int64_t(at.b) * k.chunks * k.width + at.ch;
+    Raw<T, VEC> rx[kSteps], rd[kSteps];
+    Raw<G, VEC> rg[kSteps];
+    Raw<float, VEC> rh;
+    const int64_t windows = (k.length + span - 1) / span;
+    int64_t t = (windows - 1) * span + at.first();
+    auto load = [&](int64_t t) {
+        load_steps(rx, x, k.x.step, t, n, at.in);
+        load_steps(rg, gate, k.gate.step, t, n, at.in);
+        load_steps(rd, dout, k.dout.step, t, dout != nullptr ? n : 0, at.in);
+        rh.clear();
+        if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + t / kSteps * k.width));
+    };
+    load(t);
+    float carry[VEC];
+    load_end<VEC>(carry, k.final_state, at.b, at.ch, at.in);
+    int parity = 0;
+    for (int64_t w = windows - 1; w >= 0; --w, t -= span, parity ^= 1) {
+        float c[kSteps][VEC], u[kSteps][VEC], d[kSteps][VEC], h[VEC];
+        rh.get(h);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            float xs[VEC], gs[VEC];
+            rx[j].get(xs);
+            rg[j].get(gs);
+            rd[j].get(d[j]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float input;
+                c[j][e] = decay<KIND>(gs[e], input);
+                u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
+                h[e] = apply(c[j][e], h[e], input * xs[e]);
+                if (t + j >= n) c[j][e] = kHold;
+            }
+        }
+        if (w > 0) load(t - span);
+        Product product[VEC];
+        float2 own[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float sum = 0.f;
+#pragma unroll
+            for (int j = kSteps - 1; j >= 0; --j) {
+                product[e].then(c[j][e]);
+                sum = apply(c[j][e], d[j][e] + sum, 0.f);
+            }
+            own[e] = make_float2(product[e].decay(), sum);
+        }
+        float later[VEC];
+        join<VEC, true>(told, parity, at.warp, at.lane, at.warps, at.rank, at.cluster, own, carry, later);
+        if (!at.in || t >= k.length) continue;
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            float px[VEC], pg[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float D = d[j][e] + later[e];
+                later[e] = apply(c[j][e], D, 0.f);
+                float slope, input;
+                slopes<KIND>(c[j][e], slope, input);
+                const bool on = t + j < n;
+                px[e] = on ? input * D : 0.f;
+                pg[e] = on ? slope * u[j][e] * D : 0.f;
+            }
+            if (t + j < k.length) {
+                if (dx != nullptr) Raw<T, VEC>::store(dx + (t + j) * k.dx.step, px);
+                if (dgate != nullptr) Raw<G, VEC>::store(dgate + (t + j) * k.dgate.step, pg);
+            }
+        }
+    }
+    if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(k.initial.base + at.b * k.initial.step)[at.ch + e] = carry[e];
+    }
+}
+
 // ---- arguments --------------------------------------------------------------
 
 bool present(const b200_tensor& t) { return t.data != nullptr; }
@@ -314,6 +632,42 @@ void by_type(const b200_tensor& x, const b200_tensor& gate, int kind, Fn&& go) {
     else with(__half{}, __half{});
 }
 
+// How a call's blocks walk.
+struct Walk {
+    int warps = 0;  // of a block; 0: a thread to a channel
+    int vec = 1, cluster = 1;
+    int64_t strips = 0, blocks = 0;
+};
+struct Typed {
+    Stream s;
+    int dtype;
+};
+Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams, int most_warps, int blocks_at_once) {
+    Walk w;
+    if (s.length <= kSteps) return w;
+    // two channels to a lane where every row of halves has them side by side on an address for both
+    bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
+    for (const Typed& t : streams) {
+        if (t.s.base == nullptr) continue;
+        const int64_t bytes = 2 * static_cast<int64_t>(dtype_size(t.dtype));
+        halves |= t.dtype == B200_F16;
+        pairs = pairs && reinterpret_cast<uintptr_t>(t.s.base) % static_cast<uintptr_t>(bytes) == 0 && t.s.step % bytes == 0 && t.s.batch % bytes == 0;
+    }
+    w.vec = pairs && halves ? 2 : 1;
+    w.strips = ceil_div(s.width, 32 * w.vec);
+    w.warps = static_cast<int>(std::min<int64_t>(most_warps, ceil_div(s.length, kSteps)));
+    while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster < int64_t(sm_count()) * blocks_at_once && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
+    w.blocks = s.batch * w.strips * w.cluster;
+    return w;
+}
+
+template <typename Kernel>
+void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, const Args& k) {
+    const dim3 grid(static_cast<unsigned>(w.blocks)), threads(static_cast<unsigned>(32 * w.warps));
+    if (w.cluster == 1) launch_kernel(ctx, kernel, grid, threads, 0, k, static_cast<uint32_t>(w.strips), 1u);
+    else launch_kernel_clustered(ctx, kernel, grid, threads, 0, w.cluster, false, k, static_cast<uint32_t>(w.strips), static_cast<uint32_t>(w.cluster));
+}
+
 void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
     const Shape s = check_forward(a);
     if (s.batch * s.width == 0 || (s.length == 0 && !present(a.final_state))) return;
@@ -323,8 +677,18 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
     k.initial = end_of(a.initial);
     k.final_state = end_of(a.final_state);
     ProfScope scope(ctx, "gated_recurrence");
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}}, kMostWarps, 2);
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
-        launch_kernel(ctx, serial_kernel<decltype(t), decltype(g), decltype(kind)::value>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
+        using T = decltype(t);
+        using G = decltype(g);
+        constexpr int KIND = decltype(kind)::value;
+        if (w.warps == 0) {
+            launch_kernel(ctx, serial_kernel<T, G, KIND>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
+        } else if (w.vec == 1) {
+            launch_walk(ctx, walk_kernel<T, G, KIND, 1>, w, k);
+        } else if constexpr (sizeof(T) == 2) {
+            launch_walk(ctx, walk_kernel<T, G, KIND, 2>, w, k);
+        }
     });
     check_last_launch("gated_recurrence");
     ctx->count_launch();
@@ -341,8 +705,18 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
     k.initial = end_of(a.initial_grad);
     k.final_state = end_of(a.final_grad);
     ProfScope scope(ctx, "gated_recurrence_backward");
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}}, kBackWarps, 3);
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
-        launch_kernel(ctx, serial_backward_kernel<decltype(t), decltype(g), decltype(kind)::value>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
+        using T = decltype(t);
+        using G = decltype(g);
+        constexpr int KIND = decltype(kind)::value;
+        if (w.warps == 0) {
+            launch_kernel(ctx, serial_backward_kernel<T, G, KIND>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
+        } else if (w.vec == 1) {
+            launch_walk(ctx, walk_backward_kernel<T, G, KIND, 1>, w, k);
+        } else if constexpr (sizeof(T) == 2) {
+            launch_walk(ctx, walk_backward_kernel<T, G, KIND, 2>, w, k);
+        }
     });
     check_last_launch("gated_recurrence_backward");
     ctx->count_launch();
