@@ -31,25 +31,57 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
     return y;
 }
 
-// A step's decay: -d where a = 1 - d is above a half (the sign bit says so, also of zero), else a.
-__device__ __forceinline__ bool keeps(float c) { return __float_as_int(c) < 0; }
+// A step's decay: -d where a = 1 - d is above a half (never 0: the sign tells), else a.
+constexpr float kHold = -0x1p-126f;  // h stays
+__device__ __forceinline__ bool keeps(float c) { return c < 0.f; }
+__device__ __forceinline__ float kept(float less) { return fminf(less, kHold); }  // of a product less 1
 __device__ __forceinline__ float apply(float c, float h, float b) {
     const float t = fmaf(c, h, b);
     return keeps(c) ? h + t : t;
 }
-constexpr float kHold = -0.f;  // h stays
 
-// c, and b / x, of a gate.
+// Arithmetic on a lane's channels, two to an instruction.
+template <int V>
+__device__ __forceinline__ void fma_v(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+    if constexpr (V == 2) fma_pair(d[0], d[1], a[0], a[1], b[0], b[1], c[0], c[1]);
+    else d[0] = fmaf(a[0], b[0], c[0]);
+}
+template <int V>
+__device__ __forceinline__ void mul_v(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+    if constexpr (V == 2) mul_pair(d[0], d[1], a[0], a[1], b[0], b[1]);
+    else d[0] = a[0] * b[0];
+}
+template <int V>
+__device__ __forceinline__ void add_v(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+    if constexpr (V == 2) add_pair(d[0], d[1], a[0], a[1], b[0], b[1]);
+    else d[0] = a[0] + b[0];
+}
+template <int V>
+__device__ __forceinline__ void apply_v(float (&h)[V], const float (&c)[V], const float (&b)[V]) {
+    float t[V], same[V];
+    fma_v(t, c, h, b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) same[e] = keeps(c[e]) ? 1.f : 0.f;
+    fma_v(h, same, h, t);
+}
+
+// What a gate does to a step: its decay c (as above), a itself, 1 - a, and b / x.
+struct Gate {
+    float c, a, less, input;  // less: a - 1
+};
 template <int KIND>
-__device__ __forceinline__ float decay(float gate, float& input) {
+__device__ __forceinline__ Gate gate_of(float gate) {
+    Gate r;
     if constexpr (KIND == B200_GATES_SIGMOID) {
         const float z = fast_exp2(fabsf(gate) * -kLog2e);
-        const float r = fast_reciprocal(1.f + z), s = z * r;  // s(|gate|) and s(-|gate|)
+        const float large = fast_reciprocal(1.f + z), small = z * large;  // s(|gate|) and s(-|gate|)
         const bool keep = gate > 0.f;
-        input = keep ? s : r;
-        return keep ? -s : s;
+        r.input = keep ? small : large;
+        r.a = keep ? large : small;
+        r.less = -r.input;
+        r.c = keep ? kept(-small) : small;
     } else {
-        input = 1.f;
+        r.input = 1.f;
         // e^x - 1 by its series (the term left out is 2e-8 of it at |x| = 0.69), e^x itself beyond
         float e = fmaf(gate, 1.f / 362880.f, 1.f / 40320.f);
         e = fmaf(gate, e, 1.f / 5040.f);
@@ -60,9 +92,11 @@ __device__ __forceinline__ float decay(float gate, float& input) {
         e = fmaf(gate, e, 0.5f);
         e = fmaf(gate * gate, e, gate);
         const bool near = fabsf(gate) < 0.6931f;
-        // (a growing state keeps its digits in the same form, with a positive e: the sign bit tells the forms apart, so such a decay is given as a)
-        return near && gate <= 0.f ? -fabsf(e) : near ? 1.f + e : fast_exp2(gate * kLog2e);
+        r.a = near ? 1.f + e : fast_exp2(gate * kLog2e);
+        r.less = e;
+        r.c = near && gate <= 0.f ? kept(e) : r.a;  // (a growing state: a itself, as below a half)
     }
+    return r;
 }
 // What dgate is (h_{t-1} - x) D times, or h_{t-1} D times; and dx is D times.
 template <int KIND>
@@ -75,6 +109,36 @@ __device__ __forceinline__ void slopes(float c, float& gate, float& input) {
         gate = keeps(c) ? 1.f + c : c;
         input = 1.f;
     }
+}
+
+// What a run of steps does to the state in front of it.  By gates of the kind exp it is a step itself, whose gate is the sum of theirs; else the product of
+// the a's, as such and less 1 (either keeps digits that the other loses).
+template <int KIND, int V>
+struct Product {
+    float a[V], less[V];
+    __device__ __forceinline__ Product() {
+#pragma unroll
+        for (int e = 0; e < V; ++e) a[e] = KIND == B200_GATES_SIGMOID ? 1.f : 0.f, less[e] = 0.f;
+    }
+    __device__ __forceinline__ void then(const float (&gate)[V], const float (&a1)[V], const float (&less1)[V]) {
+        if constexpr (KIND == B200_GATES_SIGMOID) {
+            mul_v(a, a, a1);
+            fma_v(less, less, less1, less);
+            add_v(less, less, less1);
+        } else {
+            add_v(a, a, gate);
+        }
+    }
+    __device__ __forceinline__ float decay(int e) const {
+        if constexpr (KIND == B200_GATES_SIGMOID) return less[e] > -0.5f ? kept(less[e]) : a[e];
+        else return gate_of<KIND>(a[e]).c;
+    }
+};
+// The decay of two runs, one behind the other.
+__device__ __forceinline__ float both(float c, float d) {
+    const float less = fmaf(c, d, c) + d;
+    const float product = (keeps(c) ? 1.f + c : c) * (keeps(d) ? 1.f + d : d);
+    return keeps(c) && keeps(d) ? (less > -0.5f ? kept(less) : 1.f + less) : product;
 }
 
 struct Stream {
@@ -134,10 +198,9 @@ __global__ void __launch_bounds__(kThreads) serial_kernel(const Args k) {
         }
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-            float input;
-            const float c = decay<KIND>(g[j], input);
+            const Gate s = gate_of<KIND>(g[j]);
             const bool in = t0 + j < n;
-            if (in) h = apply(c, h, input * x[j]);
+            if (in) h = apply(s.c, h, s.input * x[j]);
             if (t0 + j < k.length) *at<T>(k.out, b, t0 + j, ch) = from_float<T>(in ? h : 0.f);
         }
     }
@@ -167,11 +230,10 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
         for (int j = 0; j < kSteps; ++j) {
             const bool in = t0 + j < n;
             const float x = w[j];
-            float input;
-            c[j] = decay<KIND>(c[j], input);
+            const Gate s = gate_of<KIND>(c[j]);
+            c[j] = in ? s.c : kHold;
             w[j] = KIND == B200_GATES_SIGMOID ? h - x : h;
-            if (in) h = apply(c[j], h, input * x);
-            else c[j] = kHold;
+            if (in) h = apply(s.c, h, s.input * x);
         }
 #pragma unroll
         for (int j = kSteps - 1; j >= 0; --j) {
@@ -228,41 +290,68 @@ struct Raw<float, 2> {
     static __device__ __forceinline__ void store(char* p, const float (&x)[2]) { *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]); }
 };
 
-// What a run of steps does to the state in front of it: their decays' product, as such and less 1 (either keeps digits that the other loses).
-struct Product {
-    float a = 1.f, less = 0.f;
-    __device__ __forceinline__ void then(float c) {
-        const float a1 = keeps(c) ? 1.f + c : c, less1 = keeps(c) ? c : c - 1.f;
-        a *= a1;
-        less = fmaf(less, less1, less) + less1;
-    }
-    __device__ __forceinline__ float decay() const { return less <= 0.f && less > -0.5f ? -fabsf(less) : a; }
-};
-// The decay of two runs, one behind the other.
-__device__ __forceinline__ float both(float c, float d) {
-    const float less = fmaf(c, d, c) + d;
-    const float product = (keeps(c) ? 1.f + c : c) * (keeps(d) ? 1.f + d : d);
-    return keeps(c) && keeps(d) ? (less > -0.5f ? -fabsf(less) : 1.f + less) : product;
-}
-
 // What the segments of a block, and the blocks of a cluster, do to a state: decay and sum, for every channel.  Two of each: a window's are read while the next one's
-// are written.
+// are written.  (A block that is told of the window after next has told the next one itself, behind its reading of this one.)
 template <int VEC>
 struct Told {
     float2 segments[2][kMostWarps][32 * VEC];
     float2 blocks[2][kMostCluster][32 * VEC];
+    uint64_t bars[2];  // count the bytes that the cluster's blocks tell this one
+    int given_up;
 };
 
-__device__ __forceinline__ void tell(float2* mine, uint32_t rank, float2 value) {
+// Stores to another block of the cluster that its barrier counts.  (A cluster barrier would order them too, but waits for every store of the block before it.)
+__device__ __forceinline__ void tell(uint32_t to, uint32_t bar, float2 value) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(value.x), "f"(value.y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t address, uint32_t rank) {
     uint32_t to;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(value.x), "f"(value.y) : "memory");
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(address), "r"(rank));
+    return to;
+}
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Waits for a phase of a barrier, four seconds at most; whoever gives up says so, and goes on with what is there.
+__device__ __noinline__ void wait_for(uint32_t bar, uint32_t phase, int* given_up, uint32_t* status) {
+    uint64_t start = 0;
+    for (uint32_t spins = 0;; ++spins) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 2000;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(phase) : "memory");
+        if (done || *static_cast<volatile int*>(given_up) != 0) return;
+        if (spins % 64 == 63) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+            if (start == 0) start = now;
+            else if (now - start > 4000000000ull) {
+                *static_cast<volatile int*>(given_up) = 1;
+                atomicOr(status, kStatusWaitTimedOut);
+                return;
+            }
+        }
+    }
+}
+
+// Before a cluster's blocks tell each other anything, and before one of them ends.
+template <int VEC>
+__device__ __forceinline__ void begin_cluster(Told<VEC>& told) {
+    if (threadIdx.x == 0) {
+        told.given_up = 0;
+        for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&told.bars[i])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    cluster_sync();
+}
+__device__ __forceinline__ void end_cluster() {
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
 // The state that comes into this warp's steps, from `carry` in front of the window (which becomes that behind it), by every segment's decay and sum.  Segments
-// come one after another, in the order of their warps and blocks, or (BACK) the other way round.
+// come one after another, in the order of their warps and blocks, or (BACK) the other way round.  `window` counts from 0.
 template <int VEC, bool BACK>
-__device__ __forceinline__ void join(Told<VEC>& told, int parity, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, const float2 (&own)[VEC], float (&carry)[VEC], float (&in)[VEC]) {
+__device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, uint32_t* status, const float2 (&own)[VEC],
+                                     float (&carry)[VEC], float (&in)[VEC]) {
+    const uint32_t parity = window & 1;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) told.segments[parity][warp][e * 32 + lane] = own[e];
     __syncthreads();
@@ -270,21 +359,25 @@ __device__ __forceinline__ void join(Told<VEC>& told, int parity, int warp, int 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) begin[e] = carry[e];
     if (cluster > 1) {
-        float2 block[VEC];
+        const uint32_t bar = shared_address(&told.bars[parity]);
+        if (warp == 0 && lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
+        if (static_cast<uint32_t>(warp) < cluster) {
+            float2 block[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) block[e] = make_float2(kHold, 0.f);
-        for (int i = 0; i < warps; ++i) {
+            for (int e = 0; e < VEC; ++e) block[e] = make_float2(kHold, 0.f);
+            for (int i = 0; i < warps; ++i) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float2 s = told.segments[parity][BACK ? warps - 1 - i : i][e * 32 + lane];
-                block[e] = make_float2(both(block[e].x, s.x), apply(s.x, block[e].y, s.y));
+                for (int e = 0; e < VEC; ++e) {
+                    const float2 s = told.segments[parity][BACK ? warps - 1 - i : i][e * 32 + lane];
+                    block[e] = make_float2(both(block[e].x, s.x), apply(s.x, block[e].y, s.y));
+                }
+            }
+            for (uint32_t to = warp; to < cluster; to += warps) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) tell(in_block(shared_address(&told.blocks[parity][rank][e * 32 + lane]), to), in_block(bar, to), block[e]);
             }
         }
-        for (uint32_t to = warp; to < cluster; to += warps) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) tell(&told.blocks[parity][rank][e * 32 + lane], to, block[e]);
-        }
-        cluster_sync();
+        wait_for(bar, window >> 1 & 1, &told.given_up, status);
         for (uint32_t i = 0; i < cluster; ++i) {
             const uint32_t of = BACK ? cluster - 1 - i : i;
 #pragma unroll
@@ -327,25 +420,62 @@ struct Place {
     }
     __device__ __forceinline__ int64_t span() const { return int64_t(warps) * kSteps * cluster; }
     __device__ __forceinline__ int64_t first() const { return int64_t(rank * warps + warp) * kSteps; }
+    // Bytes of the warp's channels that there are, from its first on; and where that, or this lane's first, lies at step 0.
+    __device__ __forceinline__ int valid(int width, size_t size) const { return (width - (ch - lane * VEC)) * static_cast<int>(size); }
+    template <typename T>
+    __device__ __forceinline__ const char* strip(const Stream& s) const { return s.base != nullptr ? s.base + b * s.batch + int64_t(ch - lane * VEC) * int64_t(sizeof(T)) : nullptr; }
     template <typename T>
     __device__ __forceinline__ char* base(const Stream& s) const { return s.base != nullptr ? s.base + b * s.batch + int64_t(ch) * int64_t(sizeof(T)) : nullptr; }
 };
 
-// Sixteen steps of a stream, from step t on, where they are before n.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_steps(Raw<T, VEC> (&r)[kSteps], const char* base, int64_t step, int64_t t, int64_t n, bool in) {
-    const char* p = base + t * step;
-    if (in && t + kSteps <= n) {
+// A warp's steps of `STREAMS` streams on their way.  Where rows lie on 16 (or 4) bytes: through shared memory, by asynchronous copies of that size some windows
+// ahead, into places of the warp's own, so that no warp waits for another one's.  Else (rows of halves at odd addresses) an element at a time through registers.
+template <int CHUNK, int BYTES>
+__device__ __forceinline__ void copy_steps(uint32_t to, const char* from, int64_t step, int64_t t, int64_t n, int valid, int lane) {
+    constexpr int kPieces = BYTES / CHUNK;  // of a row
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) r[j].load(p + j * step);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            r[j].clear();
-            if (in && t + j < n) r[j].load(p + j * step);
+    for (int i = 0; i < kSteps * kPieces / 32; ++i) {
+        const int at = i * 32 + lane, row = at / kPieces, off = at % kPieces * CHUNK;
+        const bool in = t + row < n && off < valid;
+        const char* p = in ? from + (t + row) * step + off : from;
+        if constexpr (CHUNK == 16) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at * CHUNK), "l"(__cvta_generic_to_global(p)), "r"(in ? CHUNK : 0) : "memory");
+        } else {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + at * CHUNK), "l"(__cvta_generic_to_global(p)), "r"(in ? CHUNK : 0) : "memory");
         }
     }
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+template <typename T, int VEC, int CHUNK>
+struct Steps {  // of one stream
+    static constexpr int kBytes = 32 * VEC * int(sizeof(T)), kPlace = kSteps * kBytes;
+    Raw<T, VEC> r[CHUNK == 0 ? kSteps : 1];
+    const char* place;
+    // `base`: of the warp's first channel; `valid`: bytes of the channels that there are
+    __device__ __forceinline__ void load(char* at, const char* base, int64_t step, int64_t t, int64_t n, int valid, int lane) {
+        if constexpr (CHUNK != 0) {
+            copy_steps<CHUNK, kBytes>(shared_address(at), base, step, t, n, valid, lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                r[j].clear();
+                if (lane * VEC * int(sizeof(T)) < valid && t + j < n) r[j].load(base + (t + j) * step + lane * VEC * int(sizeof(T)));
+            }
+        }
+    }
+    __device__ __forceinline__ Raw<T, VEC> get(int j, int lane) const {
+        if constexpr (CHUNK != 0) {
+            Raw<T, VEC> x;
+            x.load(place + j * kBytes + lane * VEC * int(sizeof(T)));
+            return x;
+        } else {
+            return r[j];
+        }
+    }
+};
 
 template <int VEC>
 __device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, int b, int ch, bool in) {
@@ -353,158 +483,235 @@ __device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, in
     for (int e = 0; e < VEC; ++e) h[e] = end.base != nullptr && in ? reinterpret_cast<const float*>(end.base + b * end.step)[ch + e] : 0.f;
 }
 
-template <typename T, typename G, int KIND, int VEC>
+constexpr int kStages = 3, kBackStages = 2;  // windows in shared memory, forward and backward
+
+template <typename T, typename G, int KIND, int VEC, int CHUNK>
 __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    using X = Steps<T, VEC, CHUNK>;
+    using Y = Steps<G, VEC, CHUNK>;
+    extern __shared__ __align__(16) char ring[];
     __shared__ Told<VEC> told;
     pdl_prologue();
-    if (cluster > 1) cluster_sync();  // (every block is there before another writes to it)
+    if (cluster > 1) begin_cluster(told);
     const Place<VEC> at(k, strips, cluster);
     const int64_t n = steps_of(k, at.b), span = at.span();
-    const char *const x = at.template base<T>(k.x), *const gate = at.template base<G>(k.gate);
+    const char *const x = at.template strip<T>(k.x), *const gate = at.template strip<G>(k.gate);
     char* const out = at.template base<T>(k.out);
-    Raw<T, VEC> rx[kSteps];
-    Raw<G, VEC> rg[kSteps];
-    int64_t t = at.first();
-    load_steps(rx, x, k.x.step, t, n, at.in);
-    load_steps(rg, gate, k.gate.step, t, n, at.in);
+    X rx;
+    Y rg;
+    auto stage = [&](uint32_t w) { return ring + (w % kStages * at.warps + at.warp) * (X::kPlace + Y::kPlace); };
+    auto load = [&](uint32_t w) {
+        const int64_t t = int64_t(w) * span + at.first();
+        if (t < k.length) {
+            char* const to = stage(w);
+            rx.load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
+            rg.load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
+        }
+        if constexpr (CHUNK != 0) copies_commit();
+    };
+    const uint32_t windows = static_cast<uint32_t>((k.length + span - 1) / span);
+    for (uint32_t w = 0; w < (CHUNK != 0 ? kStages - 1 : 1); ++w) load(w);
     float carry[VEC];
     load_end<VEC>(carry, k.initial, at.b, at.ch, at.in);
-    int parity = 0;
-    for (int64_t begin = 0; begin < k.length; begin += span, t += span, parity ^= 1) {
+    int64_t t = at.first();
+    for (uint32_t w = 0; w < windows; ++w, t += span) {
+        if constexpr (CHUNK != 0) {
+            copies_wait<kStages - 2>();
+            __syncwarp();
+            rx.place = stage(w), rg.place = rx.place + X::kPlace;
+            load(w + kStages - 1);  // (where the window before lay)
+        }
         float c[kSteps][VEC], b[kSteps][VEC];
-        Product product[VEC];
+        Product<KIND, VEC> product;
         float sum[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
+        const int left = static_cast<int>(n - t < kSteps ? (n - t < 0 ? 0 : n - t) : kSteps);  // steps of the sequence
+        auto take = [&](auto whole) {
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            float xs[VEC], gs[VEC];
-            rx[j].get(xs);
-            rg[j].get(gs);
+            for (int j = 0; j < kSteps; ++j) {
+                float xs[VEC], gs[VEC], a[VEC], less[VEC], input[VEC];
+                rx.get(j, at.lane).get(xs);
+                rg.get(j, at.lane).get(gs);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float input;
-                c[j][e] = decay<KIND>(gs[e], input);
-                b[j][e] = input * xs[e];
-                if (t + j >= n) c[j][e] = kHold, b[j][e] = 0.f;
-                product[e].then(c[j][e]);
-                sum[e] = apply(c[j][e], sum[e], b[j][e]);
+                for (int e = 0; e < VEC; ++e) {
+                    if (!whole.value && j >= left) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;  // the state stays
+                    const Gate s = gate_of<KIND>(gs[e]);
+                    c[j][e] = s.c, a[e] = s.a, less[e] = s.less, input[e] = s.input;
+                }
+                mul_v(b[j], input, xs);
+                product.then(gs, a, less);
+                fma_v(sum, a, sum, b[j]);  // (a's rounding counts within these steps only)
             }
-        }
-        if (begin + span < k.length) {
-            load_steps(rx, x, k.x.step, t + span, n, at.in);
-            load_steps(rg, gate, k.gate.step, t + span, n, at.in);
-        }
+        };
+        if (left == kSteps) take(std::true_type{});
+        else take(std::false_type{});
+        if constexpr (CHUNK == 0) load(w + 1);
         float2 own[VEC];
         float h[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) own[e] = make_float2(product[e].decay(), sum[e]);
-        join<VEC, false>(told, parity, at.warp, at.lane, at.warps, at.rank, at.cluster, own, carry, h);
+        for (int e = 0; e < VEC; ++e) own[e] = make_float2(product.decay(e), sum[e]);
+        join<VEC, false>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, h);
         if (!at.in || t >= k.length) continue;
         if (k.states != nullptr) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
-        char* p = out + t * k.out.step;
+        char* const p = out + t * k.out.step;
+        const int rows = static_cast<int>(k.length - t < kSteps ? k.length - t : kSteps);
+        auto put = [&](auto whole) {
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            float y[VEC];
+            for (int j = 0; j < kSteps; ++j) {
+                apply_v(h, c[j], b[j]);
+                float y[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                h[e] = apply(c[j][e], h[e], b[j][e]);
-                y[e] = t + j < n ? h[e] : 0.f;
+                for (int e = 0; e < VEC; ++e) y[e] = whole.value || j < left ? h[e] : 0.f;
+                if (whole.value || j < rows) Raw<T, VEC>::store(p + j * k.out.step, y);
             }
-            if (t + j < k.length) Raw<T, VEC>::store(p + j * k.out.step, y);
-        }
+        };
+        if (left == kSteps) put(std::true_type{});
+        else put(std::false_type{});
     }
     if (k.final_state.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(k.final_state.base + at.b * k.final_state.step)[at.ch + e] = carry[e];
     }
+    if (cluster > 1) end_cluster();
 }
 
-constexpr int kBackWarps = 4;
-
-template <typename T, typename G, int KIND, int VEC>
-__global__ void __launch_bounds__(32 * kBackWarps, 3) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+template <typename T, typename G, int KIND, int VEC, int CHUNK>
+__global__ void __launch_bounds__(32 * kMostWarps, CHUNK != 0 ? 2 : 1) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    using X = Steps<T, VEC, CHUNK>;
+    using Y = Steps<G, VEC, CHUNK>;
+    extern __shared__ __align__(16) char ring[];
     __shared__ Told<VEC> told;
     pdl_prologue();
-    if (cluster > 1) cluster_sync();  // (every block is there before another writes to it)
+    if (cluster > 1) begin_cluster(told);
     const Place<VEC> at(k, strips, cluster);
     const int64_t n = steps_of(k, at.b), span = at.span();
-    const char *const x = at.template base<T>(k.x), *const gate = at.template base<G>(k.gate), *const dout = at.template base<T>(k.dout);
+    const char *const x = at.template strip<T>(k.x), *const gate = at.template strip<G>(k.gate), *const dout = at.template strip<T>(k.dout);
     char *const dx = at.template base<T>(k.dx), *const dgate = at.template base<G>(k.dgate);
     const float* const states = k.states + int64_t(at.b) * k.chunks * k.width + at.ch;
-    Raw<T, VEC> rx[kSteps], rd[kSteps];
-    Raw<G, VEC> rg[kSteps];
+    const uint32_t windows = static_cast<uint32_t>((k.length + span - 1) / span);
+    X rx, rd;
+    Y rg;
     Raw<float, VEC> rh;
-    const int64_t windows = (k.length + span - 1) / span;
-    int64_t t = (windows - 1) * span + at.first();
-    auto load = [&](int64_t t) {
-        load_steps(rx, x, k.x.step, t, n, at.in);
-        load_steps(rg, gate, k.gate.step, t, n, at.in);
-        load_steps(rd, dout, k.dout.step, t, dout != nullptr ? n : 0, at.in);
-        rh.clear();
-        if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + t / kSteps * k.width));
+    auto stage = [&](uint32_t w) { return ring + (w % kBackStages * at.warps + at.warp) * (2 * X::kPlace + Y::kPlace); };
+    auto load = [&](uint32_t w) {  // window w from the end
+        const int64_t t = int64_t(windows - 1 - w) * span + at.first();
+        if (w < windows && (CHUNK == 0 || t < k.length)) {
+            char* const to = stage(w);
+            rx.load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
+            rg.load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
+            if (dout != nullptr) rd.load(to + X::kPlace + Y::kPlace, dout, k.dout.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
+            rh.clear();
+            if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + t / kSteps * k.width));
+        }
+        if constexpr (CHUNK != 0) copies_commit();
     };
-    load(t);
+    load(0);
     float carry[VEC];
     load_end<VEC>(carry, k.final_state, at.b, at.ch, at.in);
-    int parity = 0;
-    for (int64_t w = windows - 1; w >= 0; --w, t -= span, parity ^= 1) {
-        float c[kSteps][VEC], u[kSteps][VEC], d[kSteps][VEC], h[VEC];
+    int64_t t = int64_t(windows - 1) * span + at.first();
+    for (uint32_t w = 0; w < windows; ++w, t -= span) {
+        float c[kSteps][VEC], u[kSteps][VEC], h[VEC];
+        Raw<T, VEC> kept_d[CHUNK != 0 ? 1 : kSteps];
         rh.get(h);
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            float xs[VEC], gs[VEC];
-            rx[j].get(xs);
-            rg[j].get(gs);
-            rd[j].get(d[j]);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float input;
-                c[j][e] = decay<KIND>(gs[e], input);
-                u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
-                h[e] = apply(c[j][e], h[e], input * xs[e]);
-                if (t + j >= n) c[j][e] = kHold;
-            }
+        if constexpr (CHUNK != 0) {
+            copies_wait<0>();
+            __syncwarp();
+            rx.place = stage(w), rg.place = rx.place + X::kPlace, rd.place = rg.place + Y::kPlace;
+            load(w + 1);  // (where the window before lay)
         }
-        if (w > 0) load(t - span);
-        Product product[VEC];
+        Product<KIND, VEC> product;
+        const int left = static_cast<int>(n - t < kSteps ? (n - t < 0 ? 0 : n - t) : kSteps);  // steps of the sequence
+        auto take = [&](auto whole) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                float xs[VEC], gs[VEC], a[VEC], less[VEC], input[VEC], b[VEC];
+                rx.get(j, at.lane).get(xs);
+                rg.get(j, at.lane).get(gs);
+                if constexpr (CHUNK == 0) {
+                    if (dout != nullptr) kept_d[j] = rd.r[j];
+                    else kept_d[j].clear();
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (!whole.value && j >= left) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
+                    const Gate s = gate_of<KIND>(gs[e]);
+                    c[j][e] = s.c, a[e] = s.a, less[e] = s.less, input[e] = s.input;
+                    u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
+                }
+                mul_v(b, input, xs);
+                product.then(gs, a, less);
+                apply_v(h, c[j], b);
+            }
+        };
+        if (left == kSteps) take(std::true_type{});
+        else take(std::false_type{});
+        if constexpr (CHUNK == 0) load(w + 1);
+        auto gradient = [&](int j, float (&d)[VEC]) {
+            if constexpr (CHUNK != 0) {
+                if (dout != nullptr && j < left) {
+                    rd.get(j, at.lane).get(d);
+                    return;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) d[e] = 0.f;
+            } else {
+                kept_d[j].get(d);
+            }
+        };
         float2 own[VEC];
+        float sum[VEC], zero[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float sum = 0.f;
-#pragma unroll
-            for (int j = kSteps - 1; j >= 0; --j) {
-                product[e].then(c[j][e]);
-                sum = apply(c[j][e], d[j][e] + sum, 0.f);
-            }
-            own[e] = make_float2(product[e].decay(), sum);
-        }
-        float later[VEC];
-        join<VEC, true>(told, parity, at.warp, at.lane, at.warps, at.rank, at.cluster, own, carry, later);
-        if (!at.in || t >= k.length) continue;
+        for (int e = 0; e < VEC; ++e) sum[e] = zero[e] = 0.f;
 #pragma unroll
         for (int j = kSteps - 1; j >= 0; --j) {
-            float px[VEC], pg[VEC];
+            float d[VEC], a[VEC];
+            gradient(j, d);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float D = d[j][e] + later[e];
-                later[e] = apply(c[j][e], D, 0.f);
-                float slope, input;
-                slopes<KIND>(c[j][e], slope, input);
-                const bool on = t + j < n;
-                px[e] = on ? input * D : 0.f;
-                pg[e] = on ? slope * u[j][e] * D : 0.f;
-            }
-            if (t + j < k.length) {
-                if (dx != nullptr) Raw<T, VEC>::store(dx + (t + j) * k.dx.step, px);
-                if (dgate != nullptr) Raw<G, VEC>::store(dgate + (t + j) * k.dgate.step, pg);
-            }
+            for (int e = 0; e < VEC; ++e) a[e] = keeps(c[j][e]) ? 1.f + c[j][e] : c[j][e];
+            add_v(d, d, sum);
+            mul_v(sum, a, d);  // (a's rounding counts within these steps only)
         }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) own[e] = make_float2(product.decay(e), sum[e]);
+        float later[VEC];
+        join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, later);
+        if (!at.in || t >= k.length) continue;
+        char *const to_x = dx != nullptr ? dx + t * k.dx.step : nullptr, *const to_gate = dgate != nullptr ? dgate + t * k.dgate.step : nullptr;
+        const int rows = static_cast<int>(k.length - t < kSteps ? k.length - t : kSteps);
+        auto put = [&](auto whole) {
+#pragma unroll
+            for (int j = kSteps - 1; j >= 0; --j) {
+                float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC];
+                gradient(j, D);
+                add_v(D, D, later);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    later[e] = D[e];
+                    slopes<KIND>(c[j][e], slope[e], input[e]);
+                }
+                apply_v(later, c[j], zero);
+                mul_v(px, input, D);
+                mul_v(pg, slope, u[j]);
+                mul_v(pg, pg, D);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (!whole.value && j >= left) px[e] = pg[e] = 0.f;
+                }
+                if (whole.value || j < rows) {
+                    if (to_x != nullptr) Raw<T, VEC>::store(to_x + j * k.dx.step, px);
+                    if (to_gate != nullptr) Raw<G, VEC>::store(to_gate + j * k.dgate.step, pg);
+                }
+            }
+        };
+        if (left == kSteps) put(std::true_type{});
+        else put(std::false_type{});
     }
     if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(k.initial.base + at.b * k.initial.step)[at.ch + e] = carry[e];
     }
+    if (cluster > 1) end_cluster();
 }
 
 // ---- arguments --------------------------------------------------------------
@@ -634,38 +841,63 @@ void by_type(const b200_tensor& x, const b200_tensor& gate, int kind, Fn&& go) {
 
 // How a call's blocks walk.
 struct Walk {
-    int warps = 0;  // of a block; 0: a thread to a channel
-    int vec = 1, cluster = 1;
+    int warps = 0;   // of a block; 0: a thread to a channel
+    int vec = 1;     // channels of a lane
+    int chunk = 0;   // bytes of an asynchronous copy; 0: through registers
+    int cluster = 1;
     int64_t strips = 0, blocks = 0;
 };
 struct Typed {
     Stream s;
     int dtype;
+    bool read;
 };
-Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams, int most_warps, int blocks_at_once) {
+Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams) {
     Walk w;
     if (s.length <= kSteps) return w;
-    // two channels to a lane where every row of halves has them side by side on an address for both
+    // Copies of 16 or of 4 bytes where every row that is read lies on so many; two channels to a lane where every row of halves has them side by side on an address
+    // for both.
     bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
+    int chunk = 16;
     for (const Typed& t : streams) {
         if (t.s.base == nullptr) continue;
-        const int64_t bytes = 2 * static_cast<int64_t>(dtype_size(t.dtype));
+        const int64_t size = static_cast<int64_t>(dtype_size(t.dtype));
+        auto on = [&](int64_t bytes) { return reinterpret_cast<uintptr_t>(t.s.base) % static_cast<uintptr_t>(bytes) == 0 && t.s.step % bytes == 0 && t.s.batch % bytes == 0; };
         halves |= t.dtype == B200_F16;
-        pairs = pairs && reinterpret_cast<uintptr_t>(t.s.base) % static_cast<uintptr_t>(bytes) == 0 && t.s.step % bytes == 0 && t.s.batch % bytes == 0;
+        pairs = pairs && on(2 * size);
+        if (t.read && chunk == 16 && !(on(16) && s.width * size % 16 == 0)) chunk = 4;
+        if (t.read && chunk == 4 && !(on(4) && s.width * size % 4 == 0)) chunk = 0;
     }
     w.vec = pairs && halves ? 2 : 1;
+    w.chunk = halves && !pairs ? 0 : chunk;
     w.strips = ceil_div(s.width, 32 * w.vec);
-    w.warps = static_cast<int>(std::min<int64_t>(most_warps, ceil_div(s.length, kSteps)));
-    while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster < int64_t(sm_count()) * blocks_at_once && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
+    w.warps = static_cast<int>(std::min<int64_t>(kMostWarps, ceil_div(s.length, kSteps)));
+    while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
     w.blocks = s.batch * w.strips * w.cluster;
     return w;
 }
 
+// Calls go(VEC, CHUNK) with what a walk has.
+template <typename T, typename Fn>
+void by_walk(const Walk& w, Fn&& go) {
+    using One = std::integral_constant<int, 1>;
+    if constexpr (sizeof(T) == 2) {
+        using Two = std::integral_constant<int, 2>;
+        if (w.chunk == 16) go(Two{}, std::integral_constant<int, 16>{});
+        else if (w.chunk == 4) go(Two{}, std::integral_constant<int, 4>{});
+        else go(One{}, std::integral_constant<int, 0>{});
+    } else {
+        if (w.chunk == 16) go(One{}, std::integral_constant<int, 16>{});
+        else go(One{}, std::integral_constant<int, 4>{});
+    }
+}
+
 template <typename Kernel>
-void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, const Args& k) {
+void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, size_t shared, const Args& k) {
     const dim3 grid(static_cast<unsigned>(w.blocks)), threads(static_cast<unsigned>(32 * w.warps));
-    if (w.cluster == 1) launch_kernel(ctx, kernel, grid, threads, 0, k, static_cast<uint32_t>(w.strips), 1u);
-    else launch_kernel_clustered(ctx, kernel, grid, threads, 0, w.cluster, false, k, static_cast<uint32_t>(w.strips), static_cast<uint32_t>(w.cluster));
+    (void)blocks_at_once(reinterpret_cast<const void*>(kernel), 32 * w.warps, shared);  // (allows that much shared memory)
+    if (w.cluster == 1) launch_kernel(ctx, kernel, grid, threads, shared, k, static_cast<uint32_t>(w.strips), 1u);
+    else launch_kernel_clustered(ctx, kernel, grid, threads, shared, w.cluster, false, k, static_cast<uint32_t>(w.strips), static_cast<uint32_t>(w.cluster));
 }
 
 void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
@@ -677,17 +909,20 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
     k.initial = end_of(a.initial);
     k.final_state = end_of(a.final_state);
     ProfScope scope(ctx, "gated_recurrence");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}}, kMostWarps, 2);
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype, true}, {k.gate, a.gate.dtype, true}, {k.out, a.out.dtype, false}});
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
         constexpr int KIND = decltype(kind)::value;
         if (w.warps == 0) {
             launch_kernel(ctx, serial_kernel<T, G, KIND>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
-        } else if (w.vec == 1) {
-            launch_walk(ctx, walk_kernel<T, G, KIND, 1>, w, k);
-        } else if constexpr (sizeof(T) == 2) {
-            launch_walk(ctx, walk_kernel<T, G, KIND, 2>, w, k);
+        } else {
+            by_walk<T>(w, [&](auto vec, auto chunk) {
+                constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
+                using X = Steps<T, VEC, CHUNK>;
+                using Y = Steps<G, VEC, CHUNK>;
+                launch_walk(ctx, walk_kernel<T, G, KIND, VEC, CHUNK>, w, CHUNK != 0 ? static_cast<size_t>(w.warps) * kStages * (X::kPlace + Y::kPlace) : 0, k);
+            });
         }
     });
     check_last_launch("gated_recurrence");
@@ -705,17 +940,20 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
     k.initial = end_of(a.initial_grad);
     k.final_state = end_of(a.final_grad);
     ProfScope scope(ctx, "gated_recurrence_backward");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}}, kBackWarps, 3);
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype, true}, {k.gate, a.gate.dtype, true}, {k.dout, a.x.dtype, true}, {k.dx, a.x.dtype, false}, {k.dgate, a.gate.dtype, false}});
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
         constexpr int KIND = decltype(kind)::value;
         if (w.warps == 0) {
             launch_kernel(ctx, serial_backward_kernel<T, G, KIND>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
-        } else if (w.vec == 1) {
-            launch_walk(ctx, walk_backward_kernel<T, G, KIND, 1>, w, k);
-        } else if constexpr (sizeof(T) == 2) {
-            launch_walk(ctx, walk_backward_kernel<T, G, KIND, 2>, w, k);
+        } else {
+            by_walk<T>(w, [&](auto vec, auto chunk) {
+                constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
+                using X = Steps<T, VEC, CHUNK>;
+                using Y = Steps<G, VEC, CHUNK>;
+                launch_walk(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK>, w, CHUNK != 0 ? static_cast<size_t>(w.warps) * kBackStages * (2 * X::kPlace + Y::kPlace) : 0, k);
+            });
         }
     });
     check_last_launch("gated_recurrence_backward");
