@@ -428,54 +428,54 @@ struct Place {
     __device__ __forceinline__ char* base(const Stream& s) const { return s.base != nullptr ? s.base + b * s.batch + int64_t(ch) * int64_t(sizeof(T)) : nullptr; }
 };
 
-// A warp's steps of `STREAMS` streams on their way.  Where rows lie on 16 (or 4) bytes: through shared memory, by asynchronous copies of that size some windows
-// ahead, into places of the warp's own, so that no warp waits for another one's.  Else (rows of halves at odd addresses) an element at a time through registers.
-template <int CHUNK, int BYTES>
-__device__ __forceinline__ void copy_steps(uint32_t to, const char* from, int64_t step, int64_t t, int64_t n, int valid, int lane) {
-    constexpr int kPieces = BYTES / CHUNK;  // of a row
-#pragma unroll
-    for (int i = 0; i < kSteps * kPieces / 32; ++i) {
-        const int at = i * 32 + lane, row = at / kPieces, off = at % kPieces * CHUNK;
-        const bool in = t + row < n && off < valid;
-        const char* p = in ? from + (t + row) * step + off : from;
-        if constexpr (CHUNK == 16) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + at * CHUNK), "l"(__cvta_generic_to_global(p)), "r"(in ? CHUNK : 0) : "memory");
-        } else {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + at * CHUNK), "l"(__cvta_generic_to_global(p)), "r"(in ? CHUNK : 0) : "memory");
-        }
-    }
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-
+// A warp's steps of a stream come through shared memory, by asynchronous copies some windows ahead, into places of the warp's own, so that no warp waits for
+// another one's.  CHUNK: bytes of a copy, where every row's part lies on so many; 2: rows of halves at odd addresses, by the words of four bytes that hold them.
 template <typename T, int VEC, int CHUNK>
-struct Steps {  // of one stream
-    static constexpr int kBytes = 32 * VEC * int(sizeof(T)), kPlace = kSteps * kBytes;
-    Raw<T, VEC> r[CHUNK == 0 ? kSteps : 1];
+struct Steps {
+    static constexpr bool kAround = CHUNK == 2 && sizeof(T) == 2;
+    static constexpr int kCopy = CHUNK == 2 ? 4 : CHUNK;
+    static constexpr int kBytes = 32 * VEC * int(sizeof(T)) + (kAround ? 4 : 0), kPlace = kSteps * kBytes;
+    static constexpr int kPieces = kBytes / kCopy;  // of a row
     const char* place;
+    uint32_t low, low_step;  // of step 0's address and of a step
+
     // `base`: of the warp's first channel; `valid`: bytes of the channels that there are
-    __device__ __forceinline__ void load(char* at, const char* base, int64_t step, int64_t t, int64_t n, int valid, int lane) {
-        if constexpr (CHUNK != 0) {
-            copy_steps<CHUNK, kBytes>(shared_address(at), base, step, t, n, valid, lane);
-        } else {
+    static __device__ __forceinline__ void load(char* to, const char* base, int64_t step, int64_t t, int64_t n, int valid, int lane) {
+        const uint32_t place = shared_address(to);
+        const char* const from = base + t * step;
+        const int rows = static_cast<int>(n - t < kSteps ? n - t : kSteps);
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                r[j].clear();
-                if (lane * VEC * int(sizeof(T)) < valid && t + j < n) r[j].load(base + (t + j) * step + lane * VEC * int(sizeof(T)));
+        for (int i = 0; i < (kSteps * kPieces + 31) / 32; ++i) {
+            const int at = i * 32 + lane, row = at / kPieces, off = at % kPieces * kCopy;
+            if (kSteps * kPieces % 32 != 0 && row >= kSteps) break;
+            const char* p = from + row * step;
+            int behind = 0;  // bytes in front of the row's in its first word
+            if constexpr (kAround) behind = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 2);
+            const bool in = row < rows && off < valid + behind;
+            p = in ? p - behind + off : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(base) & ~uintptr_t(3));
+            if constexpr (kCopy == 16) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place + at * kCopy), "l"(__cvta_generic_to_global(p)), "r"(in ? kCopy : 0) : "memory");
+            } else {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(place + at * kCopy), "l"(__cvta_generic_to_global(p)), "r"(in ? kCopy : 0) : "memory");
             }
         }
     }
+    // The window from step t on lies at `to`.
+    __device__ __forceinline__ void look(const char* to, const char* base, int64_t step, int64_t t) {
+        place = to;
+        if constexpr (kAround) low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + t * step)), low_step = static_cast<uint32_t>(step);
+    }
     __device__ __forceinline__ Raw<T, VEC> get(int j, int lane) const {
-        if constexpr (CHUNK != 0) {
-            Raw<T, VEC> x;
-            x.load(place + j * kBytes + lane * VEC * int(sizeof(T)));
-            return x;
-        } else {
-            return r[j];
-        }
+        Raw<T, VEC> x;
+        const char* p = place + j * kBytes + lane * VEC * int(sizeof(T));
+        if constexpr (kAround) p += (low + j * low_step) & 2;
+        x.load(p);
+        return x;
     }
 };
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
 template <int VEC>
 __device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, int b, int ch, bool in) {
@@ -504,23 +504,22 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, 
         const int64_t t = int64_t(w) * span + at.first();
         if (t < k.length) {
             char* const to = stage(w);
-            rx.load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
-            rg.load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
+            X::load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
+            Y::load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
         }
-        if constexpr (CHUNK != 0) copies_commit();
+        copies_commit();
     };
     const uint32_t windows = static_cast<uint32_t>((k.length + span - 1) / span);
-    for (uint32_t w = 0; w < (CHUNK != 0 ? kStages - 1 : 1); ++w) load(w);
+    for (uint32_t w = 0; w < kStages - 1; ++w) load(w);
     float carry[VEC];
     load_end<VEC>(carry, k.initial, at.b, at.ch, at.in);
     int64_t t = at.first();
     for (uint32_t w = 0; w < windows; ++w, t += span) {
-        if constexpr (CHUNK != 0) {
-            copies_wait<kStages - 2>();
-            __syncwarp();
-            rx.place = stage(w), rg.place = rx.place + X::kPlace;
-            load(w + kStages - 1);  // (where the window before lay)
-        }
+        copies_wait<kStages - 2>();
+        __syncwarp();
+        rx.look(stage(w), x, k.x.step, t);
+        rg.look(stage(w) + X::kPlace, gate, k.gate.step, t);
+        load(w + kStages - 1);  // (where the window before lay)
         float c[kSteps][VEC], b[kSteps][VEC];
         Product<KIND, VEC> product;
         float sum[VEC];
@@ -546,7 +545,6 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, 
         };
         if (left == kSteps) take(std::true_type{});
         else take(std::false_type{});
-        if constexpr (CHUNK == 0) load(w + 1);
         float2 own[VEC];
         float h[VEC];
 #pragma unroll
@@ -577,7 +575,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, 
 }
 
 template <typename T, typename G, int KIND, int VEC, int CHUNK>
-__global__ void __launch_bounds__(32 * kMostWarps, CHUNK != 0 ? 2 : 1) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+__global__ void __launch_bounds__(32 * kMostWarps, 2) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
     using X = Steps<T, VEC, CHUNK>;
     using Y = Steps<G, VEC, CHUNK>;
     extern __shared__ __align__(16) char ring[];
@@ -596,15 +594,15 @@ __global__ void __launch_bounds__(32 * kMostWarps, CHUNK != 0 ? 2 : 1) walk_back
     auto stage = [&](uint32_t w) { return ring + (w % kBackStages * at.warps + at.warp) * (2 * X::kPlace + Y::kPlace); };
     auto load = [&](uint32_t w) {  // window w from the end
         const int64_t t = int64_t(windows - 1 - w) * span + at.first();
-        if (w < windows && (CHUNK == 0 || t < k.length)) {
+        if (w < windows && t < k.length) {
             char* const to = stage(w);
-            rx.load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
-            rg.load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
-            if (dout != nullptr) rd.load(to + X::kPlace + Y::kPlace, dout, k.dout.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
+            X::load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
+            Y::load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
+            if (dout != nullptr) X::load(to + X::kPlace + Y::kPlace, dout, k.dout.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
             rh.clear();
             if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + t / kSteps * k.width));
         }
-        if constexpr (CHUNK != 0) copies_commit();
+        copies_commit();
     };
     load(0);
     float carry[VEC];
@@ -612,14 +610,13 @@ __global__ void __launch_bounds__(32 * kMostWarps, CHUNK != 0 ? 2 : 1) walk_back
     int64_t t = int64_t(windows - 1) * span + at.first();
     for (uint32_t w = 0; w < windows; ++w, t -= span) {
         float c[kSteps][VEC], u[kSteps][VEC], h[VEC];
-        Raw<T, VEC> kept_d[CHUNK != 0 ? 1 : kSteps];
         rh.get(h);
-        if constexpr (CHUNK != 0) {
-            copies_wait<0>();
-            __syncwarp();
-            rx.place = stage(w), rg.place = rx.place + X::kPlace, rd.place = rg.place + Y::kPlace;
-            load(w + 1);  // (where the window before lay)
-        }
+        copies_wait<0>();
+        __syncwarp();
+        rx.look(stage(w), x, k.x.step, t);
+        rg.look(stage(w) + X::kPlace, gate, k.gate.step, t);
+        rd.look(stage(w) + X::kPlace + Y::kPlace, dout, k.dout.step, t);
+        load(w + 1);  // (where the window before lay)
         Product<KIND, VEC> product;
         const int left = static_cast<int>(n - t < kSteps ? (n - t < 0 ? 0 : n - t) : kSteps);  // steps of the sequence
         auto take = [&](auto whole) {
@@ -628,10 +625,6 @@ __global__ void __launch_bounds__(32 * kMostWarps, CHUNK != 0 ? 2 : 1) walk_back
                 float xs[VEC], gs[VEC], a[VEC], less[VEC], input[VEC], b[VEC];
                 rx.get(j, at.lane).get(xs);
                 rg.get(j, at.lane).get(gs);
-                if constexpr (CHUNK == 0) {
-                    if (dout != nullptr) kept_d[j] = rd.r[j];
-                    else kept_d[j].clear();
-                }
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     if (!whole.value && j >= left) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
@@ -646,18 +639,13 @@ __global__ void __launch_bounds__(32 * kMostWarps, CHUNK != 0 ? 2 : 1) walk_back
         };
         if (left == kSteps) take(std::true_type{});
         else take(std::false_type{});
-        if constexpr (CHUNK == 0) load(w + 1);
         auto gradient = [&](int j, float (&d)[VEC]) {
-            if constexpr (CHUNK != 0) {
-                if (dout != nullptr && j < left) {
-                    rd.get(j, at.lane).get(d);
-                    return;
-                }
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) d[e] = 0.f;
-            } else {
-                kept_d[j].get(d);
+            if (dout != nullptr && j < left) {
+                rd.get(j, at.lane).get(d);
+                return;
             }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) d[e] = 0.f;
         };
         float2 own[VEC];
         float sum[VEC], zero[VEC];
@@ -843,7 +831,7 @@ void by_type(const b200_tensor& x, const b200_tensor& gate, int kind, Fn&& go) {
 struct Walk {
     int warps = 0;   // of a block; 0: a thread to a channel
     int vec = 1;     // channels of a lane
-    int chunk = 0;   // bytes of an asynchronous copy; 0: through registers
+    int chunk = 2;   // of Steps
     int cluster = 1;
     int64_t strips = 0, blocks = 0;
 };
@@ -866,10 +854,10 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
         halves |= t.dtype == B200_F16;
         pairs = pairs && on(2 * size);
         if (t.read && chunk == 16 && !(on(16) && s.width * size % 16 == 0)) chunk = 4;
-        if (t.read && chunk == 4 && !(on(4) && s.width * size % 4 == 0)) chunk = 0;
+        if (t.read && chunk == 4 && !(on(4) && s.width * size % 4 == 0)) chunk = 2;
     }
     w.vec = pairs && halves ? 2 : 1;
-    w.chunk = halves && !pairs ? 0 : chunk;
+    w.chunk = halves && !pairs ? 2 : chunk;
     w.strips = ceil_div(s.width, 32 * w.vec);
     w.warps = static_cast<int>(std::min<int64_t>(kMostWarps, ceil_div(s.length, kSteps)));
     while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
@@ -885,7 +873,7 @@ void by_walk(const Walk& w, Fn&& go) {
         using Two = std::integral_constant<int, 2>;
         if (w.chunk == 16) go(Two{}, std::integral_constant<int, 16>{});
         else if (w.chunk == 4) go(Two{}, std::integral_constant<int, 4>{});
-        else go(One{}, std::integral_constant<int, 0>{});
+        else go(One{}, std::integral_constant<int, 2>{});
     } else {
         if (w.chunk == 16) go(One{}, std::integral_constant<int, 16>{});
         else go(One{}, std::integral_constant<int, 4>{});
@@ -921,7 +909,7 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
                 using X = Steps<T, VEC, CHUNK>;
                 using Y = Steps<G, VEC, CHUNK>;
-                launch_walk(ctx, walk_kernel<T, G, KIND, VEC, CHUNK>, w, CHUNK != 0 ? static_cast<size_t>(w.warps) * kStages * (X::kPlace + Y::kPlace) : 0, k);
+                launch_walk(ctx, walk_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * kStages * (X::kPlace + Y::kPlace), k);
             });
         }
     });
@@ -952,7 +940,7 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
                 using X = Steps<T, VEC, CHUNK>;
                 using Y = Steps<G, VEC, CHUNK>;
-                launch_walk(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK>, w, CHUNK != 0 ? static_cast<size_t>(w.warps) * kBackStages * (2 * X::kPlace + Y::kPlace) : 0, k);
+                launch_walk(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * kBackStages * (2 * X::kPlace + Y::kPlace), k);
             });
         }
     });
