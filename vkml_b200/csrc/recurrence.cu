@@ -34,7 +34,6 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 // A step's decay: -d where a = 1 - d is above a half (never 0: the sign tells), else a.
 constexpr float kHold = -0x1p-126f;  // h stays
 __device__ __forceinline__ bool keeps(float c) { return c < 0.f; }
-__device__ __forceinline__ float kept(float less) { return fminf(less, kHold); }  // of a product less 1
 __device__ __forceinline__ float apply(float c, float h, float b) {
     const float t = fmaf(c, h, b);
     return keeps(c) ? h + t : t;
@@ -65,38 +64,70 @@ __device__ __forceinline__ void apply_v(float (&h)[V], const float (&c)[V], cons
     fma_v(h, same, h, t);
 }
 
-// What a gate does to a step: its decay c (as above), a itself, 1 - a, and b / x.
-struct Gate {
-    float c, a, less, input;  // less: a - 1
-};
-template <int KIND>
-__device__ __forceinline__ Gate gate_of(float gate) {
-    Gate r;
+// What gates do to a step: its decay c (as above), a, d = 1 - a, and b / x.
+template <int KIND, int V>
+__device__ __forceinline__ void gates_of(const float (&gate)[V], float (&c)[V], float (&a)[V], float (&d)[V], float (&input)[V]) {
     if constexpr (KIND == B200_GATES_SIGMOID) {
-        const float z = fast_exp2(fabsf(gate) * -kLog2e);
-        const float large = fast_reciprocal(1.f + z), small = z * large;  // s(|gate|) and s(-|gate|)
-        const bool keep = gate > 0.f;
-        r.input = keep ? small : large;
-        r.a = keep ? large : small;
-        r.less = -r.input;
-        r.c = keep ? kept(-small) : small;
+        // a = 1 / (1 + z), 1 - a = z a, z = e^-gate up to 2^126, where a is 2^-126: that is taken off, so that a gate of -inf has a = 0 (and added to the
+        // other, so that it is never 0).  Nothing else is as small.
+        float z[V], one[V], tiny[V], least[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            asm("min.NaN.f32 %0, %1, %2;" : "=f"(z[e]) : "f"(gate[e] * -kLog2e), "f"(126.f));
+            z[e] = fast_exp2(z[e]);
+            one[e] = 1.f, tiny[e] = 0x1p-126f, least[e] = -0x1p-126f;
+        }
+        add_v(one, one, z);
+#pragma unroll
+        for (int e = 0; e < V; ++e) a[e] = fast_reciprocal(one[e]);
+        fma_v(d, z, a, tiny);
+        add_v(a, a, least);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            c[e] = gate[e] > 0.f ? -d[e] : a[e];
+            input[e] = d[e];
+        }
     } else {
-        r.input = 1.f;
-        // e^x - 1 by its series (the term left out is 2e-8 of it at |x| = 0.69), e^x itself beyond
-        float e = fmaf(gate, 1.f / 362880.f, 1.f / 40320.f);
-        e = fmaf(gate, e, 1.f / 5040.f);
-        e = fmaf(gate, e, 1.f / 720.f);
-        e = fmaf(gate, e, 1.f / 120.f);
-        e = fmaf(gate, e, 1.f / 24.f);
-        e = fmaf(gate, e, 1.f / 6.f);
-        e = fmaf(gate, e, 0.5f);
-        e = fmaf(gate * gate, e, gate);
-        const bool near = fabsf(gate) < 0.6931f;
-        r.a = near ? 1.f + e : fast_exp2(gate * kLog2e);
-        r.less = e;
-        r.c = near && gate <= 0.f ? kept(e) : r.a;  // (a growing state: a itself, as below a half)
+        // e^x - 1 by its series down to -0.69 (the term left out is 2e-8 of it there), e^x itself beyond
+        float s[V], q[V], k[V];
+        auto constant = [&](float value) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) k[e] = value;
+        };
+        auto next = [&](float value) {
+            constant(value);
+            fma_v(s, gate, s, k);
+        };
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] = 1.f / 362880.f;
+        next(1.f / 40320.f);
+        next(1.f / 5040.f);
+        next(1.f / 720.f);
+        next(1.f / 120.f);
+        next(1.f / 24.f);
+        next(1.f / 6.f);
+        next(0.5f);
+        mul_v(q, gate, gate);
+        constant(-0x1p-126f);
+        add_v(k, gate, k);  // (never 0)
+        fma_v(s, q, s, k);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const bool near = gate[e] <= 0.f && gate[e] > -0.6931f;
+            const float far = fast_exp2(gate[e] * kLog2e);
+            c[e] = near ? s[e] : far;  // (a growing state: a itself, as below a half)
+            a[e] = near ? 1.f + s[e] : far;
+            d[e] = near ? -s[e] : 1.f - far;
+            input[e] = 1.f;
+        }
     }
-    return r;
+}
+template <int KIND>
+__device__ __forceinline__ float gate_of(float gate, float& input) {
+    float g[1] = {gate}, c[1], a[1], d[1], i[1];
+    gates_of<KIND>(g, c, a, d, i);
+    input = i[0];
+    return c[0];
 }
 // What dgate is (h_{t-1} - x) D times, or h_{t-1} D times; and dx is D times.
 template <int KIND>
@@ -111,35 +142,33 @@ __device__ __forceinline__ void slopes(float c, float& gate, float& input) {
     }
 }
 
-// What a run of steps does to the state in front of it.  By gates of the kind exp it is a step itself, whose gate is the sum of theirs; else the product of
-// the a's, as such and less 1 (either keeps digits that the other loses).
-template <int KIND, int V>
-struct Product {
-    float a[V], less[V];
-    __device__ __forceinline__ Product() {
+// What a run of steps does to the state in front of it: h becomes a h + sum, as h + (sum - d h) where a is above a half.  The product of the a's is kept as such and as
+// d = 1 - a: either has digits that the other loses.
+template <int V>
+struct Run {
+    float a[V], d[V], sum[V];
+    __device__ __forceinline__ void begin() {
 #pragma unroll
-        for (int e = 0; e < V; ++e) a[e] = KIND == B200_GATES_SIGMOID ? 1.f : 0.f, less[e] = 0.f;
+        for (int e = 0; e < V; ++e) a[e] = 1.f, d[e] = 0.f, sum[e] = 0.f;
     }
-    __device__ __forceinline__ void then(const float (&gate)[V], const float (&a1)[V], const float (&less1)[V]) {
-        if constexpr (KIND == B200_GATES_SIGMOID) {
-            mul_v(a, a, a1);
-            fma_v(less, less, less1, less);
-            add_v(less, less, less1);
-        } else {
-            add_v(a, a, gate);
-        }
+    // A step, or another run, behind this one.  (a's rounding counts within the run only.)
+    __device__ __forceinline__ void decays(const float (&a1)[V], const float (&d1)[V]) {
+        mul_v(a, a, a1);
+        fma_v(d, a1, d, d1);
     }
-    __device__ __forceinline__ float decay(int e) const {
-        if constexpr (KIND == B200_GATES_SIGMOID) return less[e] > -0.5f ? kept(less[e]) : a[e];
-        else return gate_of<KIND>(a[e]).c;
+    __device__ __forceinline__ void adds(const float (&a1)[V], const float (&b)[V]) { fma_v(sum, a1, sum, b); }
+    __device__ __forceinline__ void then(const Run& r) {
+        adds(r.a, r.sum);
+        decays(r.a, r.d);
+    }
+    __device__ __forceinline__ float decay(int e) const { return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : a[e]; }
+    __device__ __forceinline__ void apply_to(float (&h)[V]) const {
+        float c[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) c[e] = decay(e);
+        apply_v(h, c, sum);
     }
 };
-// The decay of two runs, one behind the other.
-__device__ __forceinline__ float both(float c, float d) {
-    const float less = fmaf(c, d, c) + d;
-    const float product = (keeps(c) ? 1.f + c : c) * (keeps(d) ? 1.f + d : d);
-    return keeps(c) && keeps(d) ? (less > -0.5f ? kept(less) : 1.f + less) : product;
-}
 
 struct Stream {
     char* base;
@@ -198,9 +227,10 @@ __global__ void __launch_bounds__(kThreads) serial_kernel(const Args k) {
         }
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-            const Gate s = gate_of<KIND>(g[j]);
+            float input;
+            const float c = gate_of<KIND>(g[j], input);
             const bool in = t0 + j < n;
-            if (in) h = apply(s.c, h, s.input * x[j]);
+            if (in) h = apply(c, h, input * x[j]);
             if (t0 + j < k.length) *at<T>(k.out, b, t0 + j, ch) = from_float<T>(in ? h : 0.f);
         }
     }
@@ -230,10 +260,11 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
         for (int j = 0; j < kSteps; ++j) {
             const bool in = t0 + j < n;
             const float x = w[j];
-            const Gate s = gate_of<KIND>(c[j]);
-            c[j] = in ? s.c : kHold;
+            float input;
+            const float decay = gate_of<KIND>(c[j], input);
+            c[j] = in ? decay : kHold;
             w[j] = KIND == B200_GATES_SIGMOID ? h - x : h;
-            if (in) h = apply(s.c, h, s.input * x);
+            if (in) h = apply(decay, h, input * x);
         }
 #pragma unroll
         for (int j = kSteps - 1; j >= 0; --j) {
@@ -290,19 +321,42 @@ struct Raw<float, 2> {
     static __device__ __forceinline__ void store(char* p, const float (&x)[2]) { *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]); }
 };
 
-// What the segments of a block, and the blocks of a cluster, do to a state: decay and sum, for every channel.  Two of each: a window's are read while the next one's
-// are written.  (A block that is told of the window after next has told the next one itself, behind its reading of this one.)
+// What the segments of a block, and the blocks of a cluster (as a decay and a sum), do to a state.  Two of the latter: a window's are read while the next one's are
+// written.  (A block that is told of the window after next has told the next one itself, behind its reading of this one.)
 template <int VEC>
 struct Told {
-    float2 segments[2][kMostWarps][32 * VEC];
-    float2 blocks[2][kMostCluster][32 * VEC];
+    float segments[kMostWarps][3][32 * VEC];
+    float blocks[2][kMostCluster][2][32 * VEC];
     uint64_t bars[2];  // count the bytes that the cluster's blocks tell this one
     int given_up;
 };
+template <int VEC>
+__device__ __forceinline__ Run<VEC> read_run(const float (&from)[3][32 * VEC], int lane) {
+    Run<VEC> r;
+    Raw<float, VEC> x;
+    x.load(reinterpret_cast<const char*>(&from[0][lane * VEC]));
+    x.get(r.a);
+    x.load(reinterpret_cast<const char*>(&from[1][lane * VEC]));
+    x.get(r.d);
+    x.load(reinterpret_cast<const char*>(&from[2][lane * VEC]));
+    x.get(r.sum);
+    return r;
+}
+template <int VEC>
+__device__ __forceinline__ void write_run(float (&to)[3][32 * VEC], int lane, const Run<VEC>& r) {
+    Raw<float, VEC>::store(reinterpret_cast<char*>(&to[0][lane * VEC]), r.a);
+    Raw<float, VEC>::store(reinterpret_cast<char*>(&to[1][lane * VEC]), r.d);
+    Raw<float, VEC>::store(reinterpret_cast<char*>(&to[2][lane * VEC]), r.sum);
+}
 
 // Stores to another block of the cluster that its barrier counts.  (A cluster barrier would order them too, but waits for every store of the block before it.)
-__device__ __forceinline__ void tell(uint32_t to, uint32_t bar, float2 value) {
-    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(value.x), "f"(value.y), "r"(bar) : "memory");
+template <int VEC>
+__device__ __forceinline__ void tell(uint32_t to, uint32_t bar, const float (&x)[VEC]) {
+    if constexpr (VEC == 2) {
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(x[0]), "f"(x[1]), "r"(bar) : "memory");
+    } else {
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(x[0]), "r"(bar) : "memory");
+    }
 }
 __device__ __forceinline__ uint32_t in_block(uint32_t address, uint32_t rank) {
     uint32_t to;
@@ -346,61 +400,58 @@ __device__ __forceinline__ void end_cluster() {
     asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
-// The state that comes into this warp's steps, from `carry` in front of the window (which becomes that behind it), by every segment's decay and sum.  Segments
+// The state that comes into this warp's steps, from `carry` in front of the window (which becomes that behind it), by what every segment does.  Segments
 // come one after another, in the order of their warps and blocks, or (BACK) the other way round.  `window` counts from 0.
 template <int VEC, bool BACK>
-__device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, uint32_t* status, const float2 (&own)[VEC],
+__device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<VEC>& own,
                                      float (&carry)[VEC], float (&in)[VEC]) {
     const uint32_t parity = window & 1;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) told.segments[parity][warp][e * 32 + lane] = own[e];
+    write_run<VEC>(told.segments[warp], lane, own);
     __syncthreads();
-    float begin[VEC];
+    Run<VEC> before, all;
+    before.begin();
+    all.begin();
+    const int mine = BACK ? warps - 1 - warp : warp;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) begin[e] = carry[e];
+    for (int i = 0; i < kMostWarps; ++i) {
+        if (i == mine) before = all;
+        if (i < warps) all.then(read_run<VEC>(told.segments[BACK ? warps - 1 - i : i], lane));
+    }
+    __syncthreads();  // (the next window's are written where these lie)
     if (cluster > 1) {
         const uint32_t bar = shared_address(&told.bars[parity]);
         if (warp == 0 && lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
-        if (static_cast<uint32_t>(warp) < cluster) {
-            float2 block[VEC];
+        float decay[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) block[e] = make_float2(kHold, 0.f);
-            for (int i = 0; i < warps; ++i) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float2 s = told.segments[parity][BACK ? warps - 1 - i : i][e * 32 + lane];
-                    block[e] = make_float2(both(block[e].x, s.x), apply(s.x, block[e].y, s.y));
-                }
-            }
-            for (uint32_t to = warp; to < cluster; to += warps) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) tell(in_block(shared_address(&told.blocks[parity][rank][e * 32 + lane]), to), in_block(bar, to), block[e]);
-            }
+        for (int e = 0; e < VEC; ++e) decay[e] = all.decay(e);
+        for (uint32_t to = warp; to < cluster; to += warps) {
+            const uint32_t there = in_block(shared_address(&told.blocks[parity][rank][0][lane * VEC]), to), bar_there = in_block(bar, to);
+            tell<VEC>(there, bar_there, decay);
+            tell<VEC>(there + 128 * VEC, bar_there, all.sum);
         }
         wait_for(bar, window >> 1 & 1, &told.given_up, status);
-        for (uint32_t i = 0; i < cluster; ++i) {
-            const uint32_t of = BACK ? cluster - 1 - i : i;
+        const uint32_t ahead = BACK ? cluster - 1 - rank : rank;
+        auto pass = [&](uint32_t j) {
+            const auto& block = told.blocks[parity][BACK ? cluster - 1 - j : j];
+            float c[VEC], sum[VEC];
+            Raw<float, VEC> x;
+            x.load(reinterpret_cast<const char*>(&block[0][lane * VEC]));
+            x.get(c);
+            x.load(reinterpret_cast<const char*>(&block[1][lane * VEC]));
+            x.get(sum);
+            apply_v(carry, c, sum);
+        };
+        uint32_t j = 0;
+        for (; j < ahead; ++j) pass(j);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (of == rank) begin[e] = carry[e];
-                const float2 s = told.blocks[parity][of][e * 32 + lane];
-                carry[e] = apply(s.x, carry[e], s.y);
-            }
-        }
-    }
-    for (int i = 0; i < warps; ++i) {
-        const int of = BACK ? warps - 1 - i : i;
+        for (int e = 0; e < VEC; ++e) in[e] = carry[e];
+        for (; j < cluster; ++j) pass(j);
+    } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            if (of == warp) in[e] = begin[e];
-            const float2 s = told.segments[parity][of][e * 32 + lane];
-            begin[e] = apply(s.x, begin[e], s.y);
-        }
+        for (int e = 0; e < VEC; ++e) in[e] = carry[e];
+        all.apply_to(carry);
     }
-    if (cluster == 1) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) carry[e] = begin[e];
-    }
+    before.apply_to(in);
 }
 
 // Where a thread works: its sequence, channels, and place in a window.
@@ -418,10 +469,10 @@ struct Place {
         ch = static_cast<int>(i % strips) * (32 * VEC) + lane * VEC;
         in = ch < k.width;
     }
-    __device__ __forceinline__ int64_t span() const { return int64_t(warps) * kSteps * cluster; }
-    __device__ __forceinline__ int64_t first() const { return int64_t(rank * warps + warp) * kSteps; }
+    __device__ __forceinline__ uint32_t span() const { return warps * kSteps * cluster; }
+    __device__ __forceinline__ uint32_t first() const { return (rank * warps + warp) * kSteps; }
     // Bytes of the warp's channels that there are, from its first on; and where that, or this lane's first, lies at step 0.
-    __device__ __forceinline__ int valid(int width, size_t size) const { return (width - (ch - lane * VEC)) * static_cast<int>(size); }
+    __device__ __forceinline__ int valid(int width, size_t size) const { return min(width - (ch - lane * VEC), 32 * VEC) * static_cast<int>(size); }
     template <typename T>
     __device__ __forceinline__ const char* strip(const Stream& s) const { return s.base != nullptr ? s.base + b * s.batch + int64_t(ch - lane * VEC) * int64_t(sizeof(T)) : nullptr; }
     template <typename T>
@@ -436,43 +487,89 @@ struct Steps {
     static constexpr int kCopy = CHUNK == 2 ? 4 : CHUNK;
     static constexpr int kBytes = 32 * VEC * int(sizeof(T)) + (kAround ? 4 : 0), kPlace = kSteps * kBytes;
     static constexpr int kPieces = kBytes / kCopy;  // of a row
-    const char* place;
-    uint32_t low, low_step;  // of step 0's address and of a step
+    const char* from;     // this lane's first piece of the window that is copied next (kAround: the warp's row)
+    int64_t step, jump;   // bytes to the next step's, to the next window's
+    int valid;            // bytes of the row that there are
+    const char* place;    // the window that is looked at
+    uint32_t low;         // (kAround) of its first address
 
-    // `base`: of the warp's first channel; `valid`: bytes of the channels that there are
-    static __device__ __forceinline__ void load(char* to, const char* base, int64_t step, int64_t t, int64_t n, int valid, int lane) {
+    // `base`: of the warp's first channel at step 0; windows from step t on, `span` steps apart (or back).
+    __device__ __forceinline__ void begin(const char* base, int64_t bytes, uint32_t t, int64_t span, int row_bytes, int lane) {
+        step = bytes, jump = span * bytes, valid = row_bytes;
+        from = base + t * bytes;
+        if constexpr (!kAround) {
+            if constexpr (kPieces <= 32) from += lane / kPieces * bytes + lane % kPieces * kCopy;
+            else from += lane * kCopy;
+        }
+    }
+    static __device__ __forceinline__ void copy(uint32_t to, const char* p, int size) {
+        if constexpr (kCopy == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(__cvta_generic_to_global(p)), "r"(size) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(__cvta_generic_to_global(p)), "r"(size) : "memory");
+    }
+    // The window's first `rows` steps to `to`, zeros behind them.  (Where nothing is read the address is one that could be.)
+    __device__ __forceinline__ void load(char* to, int rows, int lane) {
         const uint32_t place = shared_address(to);
-        const char* const from = base + t * step;
-        const int rows = static_cast<int>(n - t < kSteps ? n - t : kSteps);
+        if constexpr (kAround) {
 #pragma unroll
-        for (int i = 0; i < (kSteps * kPieces + 31) / 32; ++i) {
-            const int at = i * 32 + lane, row = at / kPieces, off = at % kPieces * kCopy;
-            if (kSteps * kPieces % 32 != 0 && row >= kSteps) break;
-            const char* p = from + row * step;
-            int behind = 0;  // bytes in front of the row's in its first word
-            if constexpr (kAround) behind = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 2);
-            const bool in = row < rows && off < valid + behind;
-            p = in ? p - behind + off : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(base) & ~uintptr_t(3));
-            if constexpr (kCopy == 16) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place + at * kCopy), "l"(__cvta_generic_to_global(p)), "r"(in ? kCopy : 0) : "memory");
+            for (int i = 0; i < (kSteps * kPieces + 31) / 32; ++i) {
+                const int at = i * 32 + lane, row = at / kPieces, off = at % kPieces * kCopy;
+                if (row >= kSteps) break;
+                const char* p = from + row * step;
+                const int behind = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 2);  // bytes in front of the row's in its first word
+                const bool in = row < rows && off < valid + behind;
+                copy(place + at * kCopy, in ? p - behind + off : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3)), in ? kCopy : 0);
+            }
+        } else if constexpr (kPieces <= 32) {
+            constexpr int kRows = 32 / kPieces;  // of one copy of the warp's
+            const int row = lane / kPieces;
+            const bool in = lane % kPieces * kCopy < valid;
+            const uint32_t mine = place + lane * kCopy;
+            const char* p = in ? from : from - lane % kPieces * kCopy;
+            const int64_t more = step * kRows;
+            if (rows == kSteps) {
+#pragma unroll
+                for (int i = 0; i < kSteps / kRows; ++i, p += more) copy(mine + i * 32 * kCopy, p, in ? kCopy : 0);
             } else {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(place + at * kCopy), "l"(__cvta_generic_to_global(p)), "r"(in ? kCopy : 0) : "memory");
+                const char* const first = p - row * step;
+#pragma unroll
+                for (int i = 0; i < kSteps / kRows; ++i, p += more) {
+                    const bool here = i * kRows + row < rows;
+                    copy(mine + i * 32 * kCopy, here ? p : first, in && here ? kCopy : 0);
+                }
+            }
+        } else {
+            constexpr int kTimes = kPieces / 32;
+            const char* p = from;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i, p += step) {
+#pragma unroll
+                for (int m = 0; m < kTimes; ++m) {
+                    const bool in = (m * 32 + lane) * kCopy < valid && i < rows;
+                    copy(place + ((i * kTimes + m) * 32 + lane) * kCopy, in ? p + m * 32 * kCopy : from - lane * kCopy, in ? kCopy : 0);
+                }
             }
         }
     }
-    // The window from step t on lies at `to`.
-    __device__ __forceinline__ void look(const char* to, const char* base, int64_t step, int64_t t) {
-        place = to;
-        if constexpr (kAround) low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base + t * step)), low_step = static_cast<uint32_t>(step);
+    __device__ __forceinline__ void next() { from += jump; }
+    // The window that begins at `base` lies at `at`.
+    __device__ __forceinline__ void look(const char* at, const char* base) {
+        place = at;
+        if constexpr (kAround) low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base));
     }
     __device__ __forceinline__ Raw<T, VEC> get(int j, int lane) const {
         Raw<T, VEC> x;
         const char* p = place + j * kBytes + lane * VEC * int(sizeof(T));
-        if constexpr (kAround) p += (low + j * low_step) & 2;
+        if constexpr (kAround) p += (low + j * static_cast<uint32_t>(step)) & 2;
         x.load(p);
         return x;
     }
 };
+// Windows in shared memory of a warp's `bytes` each: two or three, and two blocks on an SM where they fit.
+constexpr int kFewBytes = 98304;
+__host__ __device__ constexpr int stages_of(int bytes) { return kMostWarps * bytes * 3 <= kFewBytes ? 3 : kMostWarps * bytes * 2 <= kFewBytes ? 2 : kMostWarps * bytes * 3 <= 2 * kFewBytes ? 3 : 2; }
+__host__ __device__ constexpr int blocks_of(int bytes) { return kMostWarps * bytes * stages_of(bytes) <= kFewBytes ? 2 : 1; }
+template <typename T, typename G, int VEC, int CHUNK, bool BACK>
+constexpr int kWindowBytes = (BACK ? 2 : 1) * Steps<T, VEC, CHUNK>::kPlace + Steps<G, VEC, CHUNK>::kPlace;
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
@@ -483,10 +580,9 @@ __device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, in
     for (int e = 0; e < VEC; ++e) h[e] = end.base != nullptr && in ? reinterpret_cast<const float*>(end.base + b * end.step)[ch + e] : 0.f;
 }
 
-constexpr int kStages = 3, kBackStages = 2;  // windows in shared memory, forward and backward
-
 template <typename T, typename G, int KIND, int VEC, int CHUNK>
-__global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+__global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, VEC, CHUNK, false>)) walk_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>, kStages = stages_of(kBytes);
     using X = Steps<T, VEC, CHUNK>;
     using Y = Steps<G, VEC, CHUNK>;
     extern __shared__ __align__(16) char ring[];
@@ -494,74 +590,88 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, 
     pdl_prologue();
     if (cluster > 1) begin_cluster(told);
     const Place<VEC> at(k, strips, cluster);
-    const int64_t n = steps_of(k, at.b), span = at.span();
-    const char *const x = at.template strip<T>(k.x), *const gate = at.template strip<G>(k.gate);
-    char* const out = at.template base<T>(k.out);
-    X rx;
-    Y rg;
-    auto stage = [&](uint32_t w) { return ring + (w % kStages * at.warps + at.warp) * (X::kPlace + Y::kPlace); };
-    auto load = [&](uint32_t w) {
-        const int64_t t = int64_t(w) * span + at.first();
-        if (t < k.length) {
-            char* const to = stage(w);
-            X::load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
-            Y::load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
+    const uint32_t length = static_cast<uint32_t>(k.length), n = static_cast<uint32_t>(steps_of(k, at.b)), span = at.span();
+    const uint32_t windows = (length + span - 1) / span;
+    X x;
+    Y gate;
+    x.begin(at.template strip<T>(k.x), k.x.step, at.first(), span, at.valid(k.width, sizeof(T)), at.lane);
+    gate.begin(at.template strip<G>(k.gate), k.gate.step, at.first(), span, at.valid(k.width, sizeof(G)), at.lane);
+    char* out = at.template base<T>(k.out) + at.first() * k.out.step;
+    const int64_t out_jump = span * k.out.step;
+    const char* x_at = at.template strip<T>(k.x) + at.first() * k.x.step;  // (of the window that is computed: X::kAround asks)
+    const char* gate_at = at.template strip<G>(k.gate) + at.first() * k.gate.step;
+    char *const places = ring + at.warp * kBytes, *const end = places + kStages * at.warps * kBytes, *read = places, *write = places;
+    const int apart = at.warps * kBytes;
+    uint32_t t = at.first(), t_load = t, w_load = 0;
+    auto load = [&]() {
+        if (w_load < windows && t_load < length) {
+            const int rows = t_load < n ? static_cast<int>(min(n - t_load, uint32_t(kSteps))) : 0;
+            x.load(write, rows, at.lane);
+            gate.load(write + X::kPlace, rows, at.lane);
         }
         copies_commit();
+        x.next(), gate.next();
+        ++w_load, t_load += span;
+        write += apart;
+        if (write == end) write = places;
     };
-    const uint32_t windows = static_cast<uint32_t>((k.length + span - 1) / span);
-    for (uint32_t w = 0; w < kStages - 1; ++w) load(w);
+    for (int i = 0; i < kStages - 1; ++i) load();
     float carry[VEC];
     load_end<VEC>(carry, k.initial, at.b, at.ch, at.in);
-    int64_t t = at.first();
-    for (uint32_t w = 0; w < windows; ++w, t += span) {
+    for (uint32_t w = 0; w < windows; ++w, t += span, out += out_jump) {
         copies_wait<kStages - 2>();
         __syncwarp();
-        rx.look(stage(w), x, k.x.step, t);
-        rg.look(stage(w) + X::kPlace, gate, k.gate.step, t);
-        load(w + kStages - 1);  // (where the window before lay)
+        x.look(read, x_at);
+        gate.look(read + X::kPlace, gate_at);
+        if constexpr (X::kAround) x_at += x.jump;
+        if constexpr (Y::kAround) gate_at += gate.jump;
+        read += apart;
+        if (read == end) read = places;
+        load();  // (where the window before lay)
         float c[kSteps][VEC], b[kSteps][VEC];
-        Product<KIND, VEC> product;
-        float sum[VEC];
+        Run<VEC> own;
+        own.begin();
+        float gate_sum[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
-        const int left = static_cast<int>(n - t < kSteps ? (n - t < 0 ? 0 : n - t) : kSteps);  // steps of the sequence
+        for (int e = 0; e < VEC; ++e) gate_sum[e] = 0.f;
+        const int left = t < n ? static_cast<int>(min(n - t, uint32_t(kSteps))) : 0;  // steps of the sequence
         auto take = [&](auto whole) {
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
-                float xs[VEC], gs[VEC], a[VEC], less[VEC], input[VEC];
-                rx.get(j, at.lane).get(xs);
-                rg.get(j, at.lane).get(gs);
+                float xs[VEC], gs[VEC], a[VEC], d[VEC], input[VEC];
+                x.get(j, at.lane).get(xs);
+                gate.get(j, at.lane).get(gs);
+                if (!whole.value && j >= left) {  // the state stays
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (!whole.value && j >= left) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;  // the state stays
-                    const Gate s = gate_of<KIND>(gs[e]);
-                    c[j][e] = s.c, a[e] = s.a, less[e] = s.less, input[e] = s.input;
+                    for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
                 }
+                gates_of<KIND>(gs, c[j], a, d, input);
                 mul_v(b[j], input, xs);
-                product.then(gs, a, less);
-                fma_v(sum, a, sum, b[j]);  // (a's rounding counts within these steps only)
+                if constexpr (KIND == B200_GATES_SIGMOID) own.decays(a, d);
+                else add_v(gate_sum, gate_sum, gs);
+                own.adds(a, b[j]);
             }
         };
         if (left == kSteps) take(std::true_type{});
         else take(std::false_type{});
-        float2 own[VEC];
+        if constexpr (KIND == B200_GATES_EXP) {  // the product of the a's is that of one step whose gate is the sum
+            float unused[2][VEC];
+            gates_of<KIND>(gate_sum, unused[0], own.a, own.d, unused[1]);
+        }
         float h[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) own[e] = make_float2(product.decay(e), sum[e]);
         join<VEC, false>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, h);
-        if (!at.in || t >= k.length) continue;
+        if (!at.in || t >= length) continue;
         if (k.states != nullptr) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
-        char* const p = out + t * k.out.step;
-        const int rows = static_cast<int>(k.length - t < kSteps ? k.length - t : kSteps);
+        const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
         auto put = [&](auto whole) {
+            char* p = out;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
+            for (int j = 0; j < kSteps; ++j, p += k.out.step) {
                 apply_v(h, c[j], b[j]);
                 float y[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) y[e] = whole.value || j < left ? h[e] : 0.f;
-                if (whole.value || j < rows) Raw<T, VEC>::store(p + j * k.out.step, y);
+                if (whole.value || j < rows) Raw<T, VEC>::store(p, y);
             }
         };
         if (left == kSteps) put(std::true_type{});
@@ -575,7 +685,8 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_kernel(const Args k, 
 }
 
 template <typename T, typename G, int KIND, int VEC, int CHUNK>
-__global__ void __launch_bounds__(32 * kMostWarps, 2) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+__global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, VEC, CHUNK, true>)) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, true>, kStages = stages_of(kBytes);
     using X = Steps<T, VEC, CHUNK>;
     using Y = Steps<G, VEC, CHUNK>;
     extern __shared__ __align__(16) char ring[];
@@ -583,117 +694,134 @@ __global__ void __launch_bounds__(32 * kMostWarps, 2) walk_backward_kernel(const
     pdl_prologue();
     if (cluster > 1) begin_cluster(told);
     const Place<VEC> at(k, strips, cluster);
-    const int64_t n = steps_of(k, at.b), span = at.span();
-    const char *const x = at.template strip<T>(k.x), *const gate = at.template strip<G>(k.gate), *const dout = at.template strip<T>(k.dout);
-    char *const dx = at.template base<T>(k.dx), *const dgate = at.template base<G>(k.dgate);
-    const float* const states = k.states + int64_t(at.b) * k.chunks * k.width + at.ch;
-    const uint32_t windows = static_cast<uint32_t>((k.length + span - 1) / span);
-    X rx, rd;
-    Y rg;
-    Raw<float, VEC> rh;
-    auto stage = [&](uint32_t w) { return ring + (w % kBackStages * at.warps + at.warp) * (2 * X::kPlace + Y::kPlace); };
-    auto load = [&](uint32_t w) {  // window w from the end
-        const int64_t t = int64_t(windows - 1 - w) * span + at.first();
-        if (w < windows && t < k.length) {
-            char* const to = stage(w);
-            X::load(to, x, k.x.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
-            Y::load(to + X::kPlace, gate, k.gate.step, t, n, at.valid(k.width, sizeof(G)), at.lane);
-            if (dout != nullptr) X::load(to + X::kPlace + Y::kPlace, dout, k.dout.step, t, n, at.valid(k.width, sizeof(T)), at.lane);
-            rh.clear();
-            if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + t / kSteps * k.width));
+    const uint32_t length = static_cast<uint32_t>(k.length), n = static_cast<uint32_t>(steps_of(k, at.b)), span = at.span();
+    const uint32_t windows = (length + span - 1) / span;
+    // windows from the last on
+    uint32_t t = (windows - 1) * span + at.first(), t_load = t, w_load = 0;
+    X x, dout;
+    Y gate;
+    const bool with_dout = k.dout.base != nullptr;
+    x.begin(at.template strip<T>(k.x), k.x.step, t, -int64_t(span), at.valid(k.width, sizeof(T)), at.lane);
+    gate.begin(at.template strip<G>(k.gate), k.gate.step, t, -int64_t(span), at.valid(k.width, sizeof(G)), at.lane);
+    if (with_dout) dout.begin(at.template strip<T>(k.dout), k.dout.step, t, -int64_t(span), at.valid(k.width, sizeof(T)), at.lane);
+    char *dx = at.template base<T>(k.dx), *dgate = at.template base<G>(k.dgate);
+    const bool with_dx = dx != nullptr, with_dgate = dgate != nullptr;
+    if (with_dx) dx += t * k.dx.step;
+    if (with_dgate) dgate += t * k.dgate.step;
+    const char *x_at = at.template strip<T>(k.x) + t * k.x.step, *gate_at = at.template strip<G>(k.gate) + t * k.gate.step, *dout_at = nullptr;
+    if (with_dout) dout_at = at.template strip<T>(k.dout) + t * k.dout.step;
+    char *const places = ring + at.warp * kBytes, *const end = places + kStages * at.warps * kBytes, *read = places, *write = places;
+    const int apart = at.warps * kBytes;
+    auto load = [&]() {
+        if (w_load < windows && t_load < length) {
+            const int rows = t_load < n ? static_cast<int>(min(n - t_load, uint32_t(kSteps))) : 0;
+            x.load(write, rows, at.lane);
+            gate.load(write + X::kPlace, rows, at.lane);
+            if (with_dout) dout.load(write + X::kPlace + Y::kPlace, rows, at.lane);
         }
         copies_commit();
+        x.next(), gate.next();
+        if (with_dout) dout.next();
+        ++w_load, t_load -= span;
+        write += apart;
+        if (write == end) write = places;
     };
-    load(0);
+    for (int i = 0; i < kStages - 1; ++i) load();
+    const float* const states = k.states + int64_t(at.b) * k.chunks * k.width + at.ch;
+    Raw<float, VEC> rh;  // the state in front of the next window's steps
+    auto load_state = [&](uint32_t t) {
+        rh.clear();
+        if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + int64_t(t / kSteps) * k.width));
+    };
+    load_state(t);
     float carry[VEC];
     load_end<VEC>(carry, k.final_state, at.b, at.ch, at.in);
-    int64_t t = int64_t(windows - 1) * span + at.first();
     for (uint32_t w = 0; w < windows; ++w, t -= span) {
         float c[kSteps][VEC], u[kSteps][VEC], h[VEC];
         rh.get(h);
-        copies_wait<0>();
+        copies_wait<kStages - 2>();
         __syncwarp();
-        rx.look(stage(w), x, k.x.step, t);
-        rg.look(stage(w) + X::kPlace, gate, k.gate.step, t);
-        rd.look(stage(w) + X::kPlace + Y::kPlace, dout, k.dout.step, t);
-        load(w + 1);  // (where the window before lay)
-        Product<KIND, VEC> product;
-        const int left = static_cast<int>(n - t < kSteps ? (n - t < 0 ? 0 : n - t) : kSteps);  // steps of the sequence
-        auto take = [&](auto whole) {
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                float xs[VEC], gs[VEC], a[VEC], less[VEC], input[VEC], b[VEC];
-                rx.get(j, at.lane).get(xs);
-                rg.get(j, at.lane).get(gs);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (!whole.value && j >= left) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
-                    const Gate s = gate_of<KIND>(gs[e]);
-                    c[j][e] = s.c, a[e] = s.a, less[e] = s.less, input[e] = s.input;
-                    u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
-                }
-                mul_v(b, input, xs);
-                product.then(gs, a, less);
-                apply_v(h, c[j], b);
-            }
-        };
-        if (left == kSteps) take(std::true_type{});
-        else take(std::false_type{});
+        x.look(read, x_at);
+        gate.look(read + X::kPlace, gate_at);
+        dout.look(read + X::kPlace + Y::kPlace, dout_at);
+        if constexpr (X::kAround) {
+            x_at += x.jump;
+            if (with_dout) dout_at += dout.jump;
+        }
+        if constexpr (Y::kAround) gate_at += gate.jump;
+        read += apart;
+        if (read == end) read = places;
+        load();  // (where the window before lay)
+        if (w + 1 < windows) load_state(t - span);
+        Run<VEC> own;
+        own.begin();
+        const int left = t < n ? static_cast<int>(min(n - t, uint32_t(kSteps))) : 0;  // steps of the sequence
         auto gradient = [&](int j, float (&d)[VEC]) {
-            if (dout != nullptr && j < left) {
-                rd.get(j, at.lane).get(d);
+            if (with_dout && j < left) {
+                dout.get(j, at.lane).get(d);
                 return;
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) d[e] = 0.f;
         };
-        float2 own[VEC];
-        float sum[VEC], zero[VEC];
+        auto take = [&](auto whole) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[e] = zero[e] = 0.f;
+            for (int j = 0; j < kSteps; ++j) {
+                float xs[VEC], gs[VEC], ds[VEC], a[VEC], d[VEC], input[VEC], b[VEC];
+                x.get(j, at.lane).get(xs);
+                gate.get(j, at.lane).get(gs);
+                gradient(j, ds);
+                if (!whole.value && j >= left) {
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
-            float d[VEC], a[VEC];
-            gradient(j, d);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) a[e] = keeps(c[j][e]) ? 1.f + c[j][e] : c[j][e];
-            add_v(d, d, sum);
-            mul_v(sum, a, d);  // (a's rounding counts within these steps only)
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) own[e] = make_float2(product.decay(e), sum[e]);
-        float later[VEC];
-        join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, later);
-        if (!at.in || t >= k.length) continue;
-        char *const to_x = dx != nullptr ? dx + t * k.dx.step : nullptr, *const to_gate = dgate != nullptr ? dgate + t * k.dgate.step : nullptr;
-        const int rows = static_cast<int>(k.length - t < kSteps ? k.length - t : kSteps);
-        auto put = [&](auto whole) {
-#pragma unroll
-            for (int j = kSteps - 1; j >= 0; --j) {
-                float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC];
-                gradient(j, D);
-                add_v(D, D, later);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    later[e] = D[e];
-                    slopes<KIND>(c[j][e], slope[e], input[e]);
+                    for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
                 }
-                apply_v(later, c[j], zero);
-                mul_v(px, input, D);
-                mul_v(pg, slope, u[j]);
-                mul_v(pg, pg, D);
+                gates_of<KIND>(gs, c[j], a, d, input);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (!whole.value && j >= left) px[e] = pg[e] = 0.f;
-                }
-                if (whole.value || j < rows) {
-                    if (to_x != nullptr) Raw<T, VEC>::store(to_x + j * k.dx.step, px);
-                    if (to_gate != nullptr) Raw<G, VEC>::store(to_gate + j * k.dgate.step, pg);
-                }
+                for (int e = 0; e < VEC; ++e) u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
+                mul_v(b, input, xs);
+                own.decays(a, d);
+                fma_v(own.sum, own.a, ds, own.sum);  // what the steps' gradients make of the state in front of them: each times the a's up to it
+                apply_v(h, c[j], b);
             }
         };
-        if (left == kSteps) put(std::true_type{});
-        else put(std::false_type{});
+        if (left == kSteps) take(std::true_type{});
+        else take(std::false_type{});
+        float later[VEC], zero[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
+        join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, later);
+        if (at.in && t < length) {
+            const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
+            auto put = [&](auto whole) {
+                char *to_x = dx + (kSteps - 1) * k.dx.step, *to_gate = dgate + (kSteps - 1) * k.dgate.step;
+#pragma unroll
+                for (int j = kSteps - 1; j >= 0; --j, to_x -= k.dx.step, to_gate -= k.dgate.step) {
+                    float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC];
+                    gradient(j, D);
+                    add_v(D, D, later);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        later[e] = D[e];
+                        slopes<KIND>(c[j][e], slope[e], input[e]);
+                    }
+                    apply_v(later, c[j], zero);
+                    mul_v(px, input, D);
+                    mul_v(pg, slope, u[j]);
+                    mul_v(pg, pg, D);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        if (!whole.value && j >= left) px[e] = pg[e] = 0.f;
+                    }
+                    if (whole.value || j < rows) {
+                        if (with_dx) Raw<T, VEC>::store(to_x, px);
+                        if (with_dgate) Raw<G, VEC>::store(to_gate, pg);
+                    }
+                }
+            };
+            if (left == kSteps) put(std::true_type{});
+            else put(std::false_type{});
+        }
+        dx -= int64_t(span) * k.dx.step, dgate -= int64_t(span) * k.dgate.step;
     }
     if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
 #pragma unroll
@@ -843,8 +971,7 @@ struct Typed {
 Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams) {
     Walk w;
     if (s.length <= kSteps) return w;
-    // Copies of 16 or of 4 bytes where every row that is read lies on so many; two channels to a lane where every row of halves has them side by side on an address
-    // for both.
+    // Copies of 16 or of 4 bytes where every row that is read lies on so many; two channels to a lane where every row has them side by side on an address for both.
     bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
     int chunk = 16;
     for (const Typed& t : streams) {
@@ -868,16 +995,10 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
 // Calls go(VEC, CHUNK) with what a walk has.
 template <typename T, typename Fn>
 void by_walk(const Walk& w, Fn&& go) {
-    using One = std::integral_constant<int, 1>;
-    if constexpr (sizeof(T) == 2) {
-        using Two = std::integral_constant<int, 2>;
-        if (w.chunk == 16) go(Two{}, std::integral_constant<int, 16>{});
-        else if (w.chunk == 4) go(Two{}, std::integral_constant<int, 4>{});
-        else go(One{}, std::integral_constant<int, 2>{});
-    } else {
-        if (w.chunk == 16) go(One{}, std::integral_constant<int, 16>{});
-        else go(One{}, std::integral_constant<int, 4>{});
-    }
+    constexpr int kVec = sizeof(T) == 2 ? 2 : 1;
+    if (w.chunk == 16) go(std::integral_constant<int, kVec>{}, std::integral_constant<int, 16>{});
+    else if (w.chunk == 4) go(std::integral_constant<int, kVec>{}, std::integral_constant<int, 4>{});
+    else if constexpr (kVec == 2) go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
 }
 
 template <typename Kernel>
@@ -907,9 +1028,8 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
         } else {
             by_walk<T>(w, [&](auto vec, auto chunk) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
-                using X = Steps<T, VEC, CHUNK>;
-                using Y = Steps<G, VEC, CHUNK>;
-                launch_walk(ctx, walk_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * kStages * (X::kPlace + Y::kPlace), k);
+                constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>;
+                launch_walk(ctx, walk_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * stages_of(kBytes) * kBytes, k);
             });
         }
     });
@@ -938,9 +1058,8 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
         } else {
             by_walk<T>(w, [&](auto vec, auto chunk) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
-                using X = Steps<T, VEC, CHUNK>;
-                using Y = Steps<G, VEC, CHUNK>;
-                launch_walk(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * kBackStages * (2 * X::kPlace + Y::kPlace), k);
+                constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, true>;
+                launch_walk(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * stages_of(kBytes) * kBytes, k);
             });
         }
     });
