@@ -5,14 +5,15 @@
 //   log q_j = u_j - log s        H = log s - (sum e^u u) / s
 //   grad = k [ a (one at token - q) - w q (log q + H) ] / T,  a and w the gradients of the token's log q and of H
 //
-// Bound by memory: z read once, and backward as much written.  A block takes a row: each thread keeps the maximum of what it has read and the sums of e^u and
-// e^u u beside it, and the block joins these threes.
+// Bound by memory: z read once, and backward as much written.  A block takes a row after another: each thread keeps the maximum of what it has read and the sums of
+// e^u and e^u u beside it, and the block joins these threes.  What comes next, of this row or the next one, is on its way into shared memory all the while, so
+// that a row's end costs other rows' time only.  Few long rows are a cluster's each, whose blocks take a part of it.
 //
 // The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least
-// reach; it is found by halving the range between the maxima.  Only threads whose maximum reaches it (about K of them) read what they had again and put what reaches the
-// bound into shared memory, little more than K entries, where an entry's rank is the number of larger ones.  Where more entries reach it than there is room for (a
-// row of few different values: most of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in the order of
-// their columns.
+// reach; it is found by halving the range between the maxima.  Only what threads whose maximum reaches it (about K of them) had is read again, by the whole block, and
+// what reaches the bound goes into shared memory, little more than K entries, where an entry's rank is the number of larger ones.  Where more entries reach it than
+// there is room for (a row of few different values: most of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in
+// the order of their columns.
 #include "operators.cuh"
 
 #include <algorithm>
@@ -23,7 +24,11 @@ namespace {
 
 constexpr int kMostTop = B200_MOST_TOP;
 constexpr int kMostThreads = 512;
-constexpr int kRoom = 1280;  // entries: where fewer threads have elements than are wanted, all of a row's are (8 to each of 127, and the ends)
+constexpr int kBatch = 4;    // vectors that a thread takes at once
+constexpr int kStages = 3;   // batches on their way
+constexpr int kMostBlocks = 8;  // of a cluster
+// Entries that there is room for: where fewer threads have elements than are wanted, all of a row's are entries (8 to each of them, and the ends).
+__host__ __device__ constexpr int room_for(int top) { return top * 8 + 16; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -113,200 +118,368 @@ __device__ __forceinline__ Part warp_part(Part x, float c) {
     return x;
 }
 
-// Adds elements to a part; those of -inf count as far below (a power of two of -150 is 0).
-template <int N>
-__device__ __forceinline__ void take(Part& part, const float (&z)[N], float c) {
-    float top = z[0];
+template <typename T>
+constexpr uint32_t kNothing = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u;  // -inf
+
+// Adds vectors, or their powers beside a maximum that is there, to a part.  Elements of -inf count as far below, as powers of two of -150, which are 0.  Halves
+// are raised to the lowest finite one instead (CLAMP: two to an instruction), where that is as far below and the difference's power is a number.
+template <typename T, bool CLAMP, int N>
+__device__ __forceinline__ void take_powers(Part& part, uint4 (&raw)[N], float at, float c) {
+    constexpr int E = 16 / sizeof(T);
+    float sum[2] = {0.f, 0.f}, turned[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 1; e < N; ++e) top = max_nan(top, z[e]);
-    top = max_nan(top, part.top);
+    for (int i = 0; i < N; ++i) {
+        float z[E];
+        if constexpr (CLAMP) {
+            const __half2 lowest = __half2half2(__ushort_as_half(0xfbff));
+            __half2* h = reinterpret_cast<__half2*>(&raw[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = __hmax2_nan(h[e], lowest);
+        }
+        unpack<T>(raw[i], z);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            float v[2], p[2];
+            add_pair(v[0], v[1], z[e], z[e + 1], -at, -at);
+            mul_pair(v[0], v[1], v[0], v[1], c, c);
+            if constexpr (!CLAMP) v[0] = max_nan(v[0], -150.f), v[1] = max_nan(v[1], -150.f);
+            p[0] = fast_exp2(v[0]), p[1] = fast_exp2(v[1]);
+            add_pair(sum[0], sum[1], sum[0], sum[1], p[0], p[1]);
+            fma_pair(turned[0], turned[1], p[0], p[1], v[0], v[1], turned[0], turned[1]);
+        }
+    }
+    part.sum += sum[0] + sum[1];
+    part.turned += turned[0] + turned[1];
+}
+// The largest element of N vectors (halves compare as halves, two at a time); no number where one is none.
+template <typename T, int N>
+__device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
+    float top;
+    if constexpr (sizeof(T) == 2) {
+        const __half2* h = reinterpret_cast<const __half2*>(&raw[0]);
+        __half2 m[2] = {__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])};
+#pragma unroll
+        for (int i = 1; i < N; ++i) {
+            m[0] = __hmax2_nan(m[0], __hmax2_nan(h[4 * i], h[4 * i + 1]));
+            m[1] = __hmax2_nan(m[1], __hmax2_nan(h[4 * i + 2], h[4 * i + 3]));
+        }
+        m[0] = __hmax2_nan(m[0], m[1]);
+        top = max_nan(__low2float(m[0]), __high2float(m[0]));
+    } else {
+        const float* z = reinterpret_cast<const float*>(&raw[0]);
+        top = z[0];
+#pragma unroll
+        for (int i = 1; i < 4 * N; ++i) top = max_nan(top, z[i]);
+    }
+    return top;
+}
+template <typename T, int N>
+__device__ __forceinline__ void take(Part& part, uint4 (&raw)[N], float c) {
+    const float top = max_nan(largest<T>(raw), part.top);
     if (!(top == part.top)) shift_part(part, top, c);
     const float at = shift_of(top);
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const float v = max_nan((z[e] - at) * c, -150.f), p = fast_exp2(v);
-        part.sum += p;
-        part.turned = fmaf(p, v, part.turned);
-    }
+    if (sizeof(T) == 2 && (at + 65504.f) * c > 160.f && c < 1e30f) take_powers<T, sizeof(T) == 2>(part, raw, at, c);
+    else take_powers<T, false>(part, raw, at, c);
 }
 
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint32_t in_block(uint32_t address, uint32_t rank) {
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(address), "r"(rank));
+    return to;
+}
+
+__device__ __forceinline__ void copy_vector(uint32_t to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(__cvta_generic_to_global(from)) : "memory");
+}
+
+// A row, or the part of it that is a block's: its vectors [first, last), and the elements in front of its first vector and behind its last one.
 template <typename T>
-__global__ void __launch_bounds__(kMostThreads) logprobs_kernel(const Args k) {
-    constexpr int E = 16 / sizeof(T);
-    __shared__ Part parts[kMostThreads / 32];
-    __shared__ uint64_t entries[kRoom];
-    __shared__ int count;
-    __shared__ int before[kMostThreads / 32 + 1];
-    pdl_prologue();
-    const int tid = threadIdx.x, threads = blockDim.x, warps = threads / 32;
-    const uint32_t r = blockIdx.x;
-    const T* const z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
-    const int head = head_of(z, k.vocab);
-    const int vectors = static_cast<int>((k.vocab - head) / E), tail = head + vectors * E;
-    const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
-    const float c = k.inverse * kLog2e;
+struct Row {
+    const T* z;
+    int head, first, last, tail;
+    __device__ __forceinline__ Row(const Args& k, uint32_t r, uint32_t rank, uint32_t blocks) {
+        z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
+        head = head_of(z, k.vocab);
+        const int64_t vectors = (k.vocab - head) / int64_t(16 / sizeof(T));
+        tail = head + static_cast<int>(vectors) * int(16 / sizeof(T));
+        first = static_cast<int>(vectors * rank / blocks), last = static_cast<int>(vectors * (rank + 1) / blocks);
+    }
+    __device__ __forceinline__ const uint4* vectors() const { return reinterpret_cast<const uint4*>(z + head); }
+};
 
-    // an element of the row's ends for some threads
-    int end = -1;
-    if (tid < head) end = tid;
-    else if (tid >= 8 && tail + (tid - 8) < k.vocab) end = tail + (tid - 8);
-    Part part{-INFINITY, 0.f, 0.f};
-    if (end >= 0) {
-        const float one[1] = {to_float(z[end])};
-        take(part, one, c);
+// A row's log sum of exponentials and entropy, from its part.
+struct Totals {
+    float at, log_sum, entropy;
+    __device__ __forceinline__ explicit Totals(const Part& all) {
+        const bool some = all.sum != 0.f;  // (or no number)
+        at = shift_of(all.top);
+        log_sum = some ? logf(all.sum) : 0.f;
+        entropy = some ? log_sum - all.turned / all.sum * kLn2 : 0.f;
     }
-    float token_z = 0.f;
-    bool token = false;
-    if (tid == 0 && k.tokens.base != nullptr) {
-        const int64_t id = load_index(row_at(k.tokens, k.inner, r), k.wide_tokens);
-        if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
-        token = id >= 0 && id < k.vocab;
-        if (token) token_z = to_float(z[id]);
-    }
-    int v = tid;
-    for (; v + 3 * threads < vectors; v += 4 * threads) {
-        uint4 raw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = zv[v + i * threads];
-        float x[4 * E];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float y[E];
-            unpack<T>(raw[i], y);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[i * E + e] = y[e];
-        }
-        take(part, x, c);
-    }
-    for (; v < vectors; v += threads) {
-        float x[E];
-        unpack<T>(zv[v], x);
-        take(part, x, c);
-    }
-    const float own_top = part.top;
-    const Part mine = warp_part(part, c);
-    if (tid % 32 == 0) parts[tid / 32] = mine;
-    if (tid == 0) count = 0;
-    __syncthreads();
-    Part all = tid % 32 < warps ? parts[tid % 32] : Part{-INFINITY, 0.f, 0.f};
-    all = warp_part(all, c);
-    const bool some = all.sum != 0.f;  // (or no number)
-    const float at = shift_of(all.top);
-    const float log_sum = some ? logf(all.sum) : 0.f;
-    const float entropy = some ? log_sum - all.turned / all.sum * kLn2 : 0.f;
-    if (tid == 0) {
-        if (k.logprobs != nullptr) k.logprobs[r] = token ? (token_z - at) * k.inverse - log_sum : 0.f;
-        if (k.entropies != nullptr) k.entropies[r] = entropy;
-        if (k.stats != nullptr) k.stats[r] = make_float4(all.top, log_sum, entropy, 0.f);
-    }
+};
+__device__ __forceinline__ void write_row(const Args& k, uint32_t r, const Part& all, bool token, float token_z) {
+    const Totals x(all);
+    if (k.logprobs != nullptr) k.logprobs[r] = token ? (token_z - x.at) * k.inverse - x.log_sum : 0.f;
+    if (k.entropies != nullptr) k.entropies[r] = x.entropy;
+    if (k.stats != nullptr) k.stats[r] = make_float4(all.top, x.log_sum, x.entropy, 0.f);
+}
+// Each of n entries to the place of its rank, if it is one of the first: as a result, or, where `to` is given, as an entry in another block's shared memory.
+__device__ __forceinline__ void rank_entries(const Args& k, uint32_t r, const Part& all, const uint64_t* entries, int n, const uint32_t* to) {
     if (k.top == 0) return;
-
-    // a bound that at least `top` elements reach
-    const bool owner = end >= 0 || tid < vectors;
-    const uint32_t own = owner ? order_of(own_top) : 0u;
-    uint32_t lo = 0, hi = order_of(all.top);
-    if (__syncthreads_count(own >= hi) >= k.top) lo = hi;
-    else {
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            const int n = __syncthreads_count(own >= mid);
-            if (n >= k.top) lo = mid;
-            else hi = mid;
-            if (n == k.top) break;
-        }
-    }
-    auto each = [&](auto&& visit) {  // of this thread's elements: (order, column)
-        if (end >= 0) visit(order_of(to_float(z[end])), static_cast<uint32_t>(end));
-        for (int i = tid; i < vectors; i += threads) {
-            float x[E];
-            unpack<T>(zv[i], x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) visit(order_of(x[e]), static_cast<uint32_t>(head + i * E + e));
-        }
-    };
-    auto counted = [&](uint32_t bound) {  // how many of the row's elements reach a bound
-        int n = 0;
-        if (own >= bound) each([&](uint32_t o, uint32_t) { n += o >= bound; });
-        n = __reduce_add_sync(0xffffffffu, n);
-        __syncthreads();
-        if (tid % 32 == 0) before[tid / 32] = n;
-        __syncthreads();
-        n = tid % 32 < warps ? before[tid % 32] : 0;
-        return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
-    };
-    auto collect = [&](uint32_t bound) {
-        if (own >= bound && owner) {
-            each([&](uint32_t o, uint32_t column) {
-                if (o < bound) return;
-                const int i = atomicAdd(&count, 1);
-                if (i < kRoom) entries[i] = uint64_t(o) << 32 | (0xffffffffu - column);
-            });
-        }
-        __syncthreads();
-    };
-    collect(lo);
-    int n = count;
-    if (n > kRoom) {
-        uint32_t top = 0xffffffffu;  // the largest number that K elements reach, or one whose entries there is room for
-        if (counted(0xffffffffu) >= k.top) lo = 0xffffffffu;
-        else {
-            while (top - lo > 1) {
-                const uint32_t mid = lo + (top - lo) / 2;
-                const int reach = counted(mid);
-                if (reach >= k.top) {
-                    lo = mid;
-                    if (reach <= kRoom) break;
-                } else {
-                    top = mid;
-                }
-            }
-        }
-        const int equal_too = counted(lo);
-        __syncthreads();
-        if (tid == 0) count = 0;
-        __syncthreads();
-        if (equal_too <= kRoom) {
-            collect(lo);
-        } else {
-            // fewer than K are larger; of the equal ones those of the lowest columns
-            if (lo != 0xffffffffu) collect(lo + 1);
-            int have = count;
-            for (int64_t from = 0; from < k.vocab && have < k.top; from += threads) {
-                const int64_t column = from + tid;
-                const bool hit = column < k.vocab && order_of(to_float(z[column])) == lo;
-                const uint32_t ballot = __ballot_sync(0xffffffffu, hit);
-                __syncthreads();
-                if (tid % 32 == 0) before[tid / 32] = __popc(ballot);
-                __syncthreads();
-                int at_most = have, in_front = have;
-                for (int w = 0; w < warps; ++w) {
-                    if (w < tid / 32) in_front += before[w];
-                    at_most += before[w];
-                }
-                const int i = in_front + __popc(ballot & ((1u << tid % 32) - 1));
-                if (hit && i < k.top) entries[i] = uint64_t(lo) << 32 | (0xffffffffu - static_cast<uint32_t>(column));
-                have = min(at_most, k.top);
-            }
-            __syncthreads();
-            if (tid == 0) count = have;
-            __syncthreads();
-        }
-        n = count;
-    }
     char* const ids = k.ids.base != nullptr ? row_at(k.ids, k.inner, r) : nullptr;
     float* const tops = k.tops.base != nullptr ? reinterpret_cast<float*>(row_at(k.tops, k.inner, r)) : nullptr;
-    for (int i = tid; i < n; i += threads) {
+    const Totals x(all);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const uint64_t entry = entries[i];
         int rank = 0;
         for (int j = 0; j < n; ++j) rank += entries[j] > entry;
-        if (rank >= k.top) continue;
+        if (rank >= k.top || entry == 0) continue;
+        if (to != nullptr) {
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(*to + rank * 8), "l"(entry) : "memory");
+            continue;
+        }
         const uint32_t column = 0xffffffffu - static_cast<uint32_t>(entry);
         if (ids != nullptr) {
             if (k.wide_ids) reinterpret_cast<int64_t*>(ids)[rank] = column;
             else reinterpret_cast<int32_t*>(ids)[rank] = static_cast<int32_t>(column);
         }
-        if (tops != nullptr) tops[rank] = (value_of(static_cast<uint32_t>(entry >> 32)) - at) * k.inverse - log_sum;
+        if (tops != nullptr) tops[rank] = (value_of(static_cast<uint32_t>(entry >> 32)) - x.at) * k.inverse - x.log_sum;
     }
+}
+
+// `blocks`: of a row's cluster (1: the blocks take row after row).  Dynamic shared memory: the batches on their way, then the entries.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const Args k, uint32_t blocks) {
+    constexpr int E = 16 / sizeof(T), kWarps = THREADS / 32, kChunk = THREADS * kBatch;  // (vectors of a chunk)
+    extern __shared__ __align__(16) char shared[];
+    __shared__ Part parts[2][kWarps];
+    __shared__ Part cluster_parts[kMostBlocks];
+    __shared__ int count, owners;
+    __shared__ int before[kWarps];
+    __shared__ uint16_t owner_list[THREADS];
+    pdl_prologue();
+    const int tid = threadIdx.x, room = room_for(k.top);
+    const uint32_t rank = blockIdx.x % blocks, stride = gridDim.x / blocks;
+    uint4* const ring = reinterpret_cast<uint4*>(shared) + tid;
+    uint64_t* const entries = reinterpret_cast<uint64_t*>(shared + kStages * kChunk * 16);
+    uint64_t* const merged = entries + room;  // (of a cluster's first block)
+    const float c = k.inverse * kLog2e;
+    if (blocks > 1) cluster_sync();  // (every block is there before another writes to it)
+
+    // What is asked for next: this thread's first vector of a chunk, the vectors from that chunk on, and where they go.
+    uint32_t row_next = blockIdx.x / blocks;
+    const uint4* from;
+    int left;
+    auto begin = [&]() {
+        const Row<T> row(k, row_next, rank, blocks);
+        from = row.vectors() + row.first + tid;
+        left = row.last - row.first;
+    };
+    begin();
+    const uint32_t ring_begin = shared_address(ring), ring_end = ring_begin + kStages * kChunk * 16;
+    uint32_t to = ring_begin;
+    auto ask = [&]() {
+        while (left <= 0 && row_next < k.rows) {
+            row_next += stride;
+            if (row_next < k.rows) begin();
+        }
+        if (left >= kChunk) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) copy_vector(to + i * THREADS * 16, from + i * THREADS);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (i * THREADS + tid < left) copy_vector(to + i * THREADS * 16, from + i * THREADS);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        from += kChunk;
+        left -= kChunk;
+        to += kChunk * 16;
+        if (to == ring_end) to = ring_begin;
+    };
+    for (int i = 0; i < kStages; ++i) ask();
+
+    const uint4* place = ring;
+    uint32_t parity = 0;
+    for (uint32_t r = blockIdx.x / blocks; r < k.rows; r += stride, parity ^= 1) {
+        const Row<T> row(k, r, rank, blocks);
+        // an element of the row's ends for some threads
+        int end = -1;
+        if (rank == 0 && tid < row.head) end = tid;
+        else if (rank + 1 == blocks && tid >= 8 && row.tail + (tid - 8) < k.vocab) end = row.tail + (tid - 8);
+        Part part{-INFINITY, 0.f, 0.f};
+        float end_z = 0.f;
+        if (end >= 0) {
+            end_z = to_float(row.z[end]);
+            uint4 one[1] = {make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>)};
+            if constexpr (sizeof(T) == 2) one[0].x = 0xfc000000u | __half_as_ushort(row.z[end]);
+            else one[0].x = __float_as_uint(end_z);
+            take<T>(part, one, c);
+        }
+        float token_z = 0.f;
+        bool token = false;
+        if (tid == 0 && rank == 0 && k.tokens.base != nullptr) {
+            const int64_t id = load_index(row_at(k.tokens, k.inner, r), k.wide_tokens);
+            if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
+            token = id >= 0 && id < k.vocab;
+            if (token) token_z = to_float(row.z[id]);
+        }
+        for (int rest = row.last - row.first; rest > 0; rest -= kChunk) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+            uint4 raw[kBatch];
+            if (rest >= kChunk) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) raw[i] = place[i * THREADS];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    raw[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+                    if (i * THREADS + tid < rest) raw[i] = place[i * THREADS];
+                }
+            }
+            place += kChunk;
+            if (place == ring + kStages * kChunk) place = ring;
+            ask();  // (into the place that was just read)
+            take<T>(part, raw, c);
+        }
+        const float own_top = part.top;
+        const Part mine = warp_part(part, c);
+        if (tid % 32 == 0) parts[parity][tid / 32] = mine;
+        __syncthreads();
+        Part all = tid % 32 < kWarps ? parts[parity][tid % 32] : Part{-INFINITY, 0.f, 0.f};
+        all = warp_part(all, c);
+        const float block_top = all.top;
+        if (k.top == 0 && blocks == 1) {
+            if (tid == 0) write_row(k, r, all, token, token_z);
+            continue;
+        }
+        int n = 0;
+        if (k.top > 0) {
+            if (tid == 0) count = 0, owners = 0;
+            // a bound that at least `top` elements reach, if there are as many threads that have any
+            const bool owner = end >= 0 || row.first + tid < row.last;
+            const uint32_t own = owner ? order_of(own_top) : 0u;
+            uint32_t lo = 0, hi = order_of(block_top);
+            if (__syncthreads_count(own >= hi) >= k.top) lo = hi;
+            else {
+                while (hi - lo > (sizeof(T) == 2 ? 8192u : 1u)) {
+                    const uint32_t mid = lo + (hi - lo) / 2;
+                    const int reach = __syncthreads_count(own >= mid);
+                    if (reach >= k.top) lo = mid;
+                    else hi = mid;
+                    if (reach == k.top) break;
+                }
+            }
+            // Of vectors of a thread's from its `begin`-th on, every `step`-th: (order, column) of the elements, where one of a vector's reaches the bound.
+            auto each = [&](int of, int begin, int step, uint32_t bound, auto&& visit) {
+                for (int i = row.first + of + begin * THREADS; i < row.last; i += step * THREADS) {
+                    const uint4 raw[1] = {row.vectors()[i]};
+                    if (order_of(largest<T>(raw)) < bound) continue;
+                    float x[E];
+                    unpack<T>(raw[0], x);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) visit(order_of(x[e]), static_cast<uint32_t>(row.head + i * E + e));
+                }
+            };
+            auto counted = [&](uint32_t bound) {  // how many of the elements reach a bound
+                int some = 0;
+                if (own >= bound) each(tid, 0, 1, bound, [&](uint32_t o, uint32_t) { some += o >= bound; });
+                if (end >= 0) some += order_of(end_z) >= bound;
+                some = __reduce_add_sync(0xffffffffu, some);
+                __syncthreads();
+                if (tid % 32 == 0) before[tid / 32] = some;
+                __syncthreads();
+                some = tid % 32 < kWarps ? before[tid % 32] : 0;
+                return static_cast<int>(__reduce_add_sync(0xffffffffu, some));
+            };
+            auto collect = [&](uint32_t bound) {
+                auto put = [&](uint32_t o, uint32_t column) {
+                    if (o < bound) return;
+                    const int i = atomicAdd(&count, 1);
+                    if (i < room) entries[i] = uint64_t(o) << 32 | (0xffffffffu - column);
+                };
+                if (own >= bound && row.first + tid < row.last) owner_list[atomicAdd(&owners, 1)] = static_cast<uint16_t>(tid);
+                if (end >= 0) put(order_of(end_z), static_cast<uint32_t>(end));
+                __syncthreads();
+                for (int o = tid / 32; o < owners; o += kWarps) each(owner_list[o], tid % 32, 32, bound, put);
+                __syncthreads();
+            };
+            collect(lo);
+            n = count;
+            if (n > room) {
+                uint32_t top = 0xffffffffu;
+                if (counted(top) >= k.top) lo = top;
+                else {
+                    while (top - lo > 1) {
+                        const uint32_t mid = lo + (top - lo) / 2;
+                        const int reach = counted(mid);
+                        if (reach >= k.top) {
+                            lo = mid;
+                            if (reach <= room) break;
+                        } else {
+                            top = mid;
+                        }
+                    }
+                }
+                const int equal_too = counted(lo);
+                __syncthreads();
+                if (tid == 0) count = 0, owners = 0;
+                __syncthreads();
+                if (equal_too <= room) {
+                    collect(lo);
+                    n = count;
+                } else {
+                    // fewer than K are larger; of the equal ones those of the lowest columns
+                    if (lo != 0xffffffffu) collect(lo + 1);
+                    int have = count;
+                    const int64_t from_column = rank == 0 ? 0 : row.head + int64_t(row.first) * E, to_column = rank + 1 == blocks ? k.vocab : row.head + int64_t(row.last) * E;
+                    for (int64_t at = from_column; at < to_column && have < k.top; at += THREADS) {
+                        const int64_t column = at + tid;
+                        const bool hit = column < to_column && order_of(to_float(row.z[column])) == lo;
+                        const uint32_t ballot = __ballot_sync(0xffffffffu, hit);
+                        __syncthreads();
+                        if (tid % 32 == 0) before[tid / 32] = __popc(ballot);
+                        __syncthreads();
+                        int at_most = have, in_front = have;
+                        for (int w = 0; w < kWarps; ++w) {
+                            if (w < tid / 32) in_front += before[w];
+                            at_most += before[w];
+                        }
+                        const int i = in_front + __popc(ballot & ((1u << tid % 32) - 1));
+                        if (hit && i < k.top) entries[i] = uint64_t(lo) << 32 | (0xffffffffu - static_cast<uint32_t>(column));
+                        have = min(at_most, k.top);
+                    }
+                    __syncthreads();
+                    n = have;
+                }
+            }
+        }
+        if (blocks == 1) {
+            if (tid == 0) write_row(k, r, all, token, token_z);
+            rank_entries(k, r, all, entries, n, nullptr);
+        } else {
+            // the first block takes what the others found: their parts, and as many entries as are wanted of each
+            if (tid == 0) {
+                const uint32_t to = in_block(shared_address(&cluster_parts[rank]), 0);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(all.top) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(all.sum) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(all.turned) : "memory");
+            }
+            const uint32_t to = in_block(shared_address(merged + rank * k.top), 0);
+            for (int i = tid + n; i < k.top; i += THREADS) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + i * 8), "l"(uint64_t(0)) : "memory");
+            rank_entries(k, r, all, entries, n, &to);
+            cluster_sync();
+            if (rank == 0) {
+                all = tid % 32 < static_cast<int>(blocks) ? cluster_parts[tid % 32] : Part{-INFINITY, 0.f, 0.f};
+                all = warp_part(all, c);
+                if (tid == 0) write_row(k, r, all, token, token_z);
+                rank_entries(k, r, all, merged, static_cast<int>(blocks) * k.top, nullptr);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- the gradient -----------------------------------------------------------
@@ -516,8 +689,41 @@ void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
     k.wide_ids = a.top_ids.dtype == B200_I64;
     ProfScope scope(ctx, "token_logprobs");
     const bool half = a.logits.dtype == B200_F16;
-    const int threads = plan.vocab * (half ? 2 : 4) > 16384 ? kMostThreads : 128;
-    launch_kernel(ctx, half ? logprobs_kernel<__half> : logprobs_kernel<float>, dim3(k.rows), dim3(threads), 0, k);
+    const int64_t vectors = ceil_div(plan.vocab, half ? 8 : 4);
+    // Threads of a block: 32 vectors to each, as a row's end costs a thread as much as 4 of them or more; and more threads than entries that are wanted.  Few rows: up
+    // to 512 threads of four vectors, and long ones a cluster of blocks each.
+    const bool few = plan.s.rows <= sm_count();
+    int threads = 32, blocks = 1;
+    while (threads < kMostThreads && (vectors > int64_t(threads) * (few ? 4 : 32) || plan.top * 2 > threads)) threads *= 2;
+    while (blocks < kMostBlocks && plan.s.rows * blocks * 2 <= sm_count() && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
+    auto go = [&](auto kernel) {
+        const size_t shared = size_t(kStages) * kBatch * 16 * static_cast<size_t>(threads) + (k.top > 0 ? (static_cast<size_t>(room_for(k.top)) + (blocks > 1 ? static_cast<size_t>(blocks) * k.top : 0)) * 8 : 0);
+        const int most = blocks_at_once(reinterpret_cast<const void*>(kernel), threads, shared);
+        if (blocks > 1) {
+            launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(plan.s.rows * blocks)), dim3(threads), shared, blocks, false, k, static_cast<uint32_t>(blocks));
+            return;
+        }
+        // Blocks that stay: as many on an SM as leave the fewest without a last row, down to half.
+        const int64_t sms = sm_count();
+        auto rounds = [&](int on_sm) { return ceil_div(plan.s.rows, sms * on_sm) * on_sm; };
+        int on_sm = most;
+        for (int n = most - 1; n >= std::max(1, most / 2); --n) {
+            if (rounds(n) < rounds(on_sm)) on_sm = n;
+        }
+        launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(std::min<int64_t>(plan.s.rows, sms * on_sm))), dim3(threads), shared, k, 1u);
+    };
+    auto with = [&](auto element) {
+        using T = decltype(element);
+        switch (threads) {
+            case 32: go(logprobs_kernel<T, 32>); break;
+            case 64: go(logprobs_kernel<T, 64>); break;
+            case 128: go(logprobs_kernel<T, 128>); break;
+            case 256: go(logprobs_kernel<T, 256>); break;
+            default: go(logprobs_kernel<T, 512>); break;
+        }
+    };
+    if (half) with(__half{});
+    else with(float{});
     check_last_launch("token_logprobs");
     ctx->count_launch();
 }
