@@ -10,8 +10,8 @@
 // that a row's end costs other rows' time only.  Few long rows are a cluster's each, whose blocks take a part of it.
 //
 // The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least
-// reach; it is found by halving the range between the maxima.  Only what threads whose maximum reaches it (about K of them) had is read again, by the whole block, and
-// what reaches the bound goes into shared memory, little more than K entries, where an entry's rank is the number of larger ones.  Where more entries reach it than
+// reach; it is found by halving the range between the maxima, by one warp.  Each thread has kept the maxima of up to four stretches of what it had, too: only
+// stretches whose maximum reaches the bound (little more than K) are read again, and what reaches it goes into shared memory, where an entry's rank is the number of larger ones.  Where more entries reach it than
 // there is room for (a row of few different values: most of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in
 // the order of their columns.
 #include "operators.cuh"
@@ -27,6 +27,7 @@ constexpr int kMostThreads = 512;
 constexpr int kBatch = 4;    // vectors that a thread takes at once
 constexpr int kStages = 3;   // batches on their way
 constexpr int kMostBlocks = 8;  // of a cluster
+constexpr int kStretches = 4;   // of a thread's batches
 // Entries that there is room for: where fewer threads have elements than are wanted, all of a row's are entries (8 to each of them, and the ends).
 __host__ __device__ constexpr int room_for(int top) { return top * 8 + 16; }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -173,9 +174,10 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
     }
     return top;
 }
+// Vectors whose largest element is `most`.
 template <typename T, int N>
-__device__ __forceinline__ void take(Part& part, uint4 (&raw)[N], float c) {
-    const float top = max_nan(largest<T>(raw), part.top);
+__device__ __forceinline__ void take(Part& part, uint4 (&raw)[N], float most, float c) {
+    const float top = max_nan(most, part.top);
     if (!(top == part.top)) shift_part(part, top, c);
     const float at = shift_of(top);
     if (sizeof(T) == 2 && (at + 65504.f) * c > 160.f && c < 1e30f) take_powers<T, sizeof(T) == 2>(part, raw, at, c);
@@ -233,6 +235,7 @@ __device__ __forceinline__ void rank_entries(const Args& k, uint32_t r, const Pa
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const uint64_t entry = entries[i];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) rank += entries[j] > entry;
         if (rank >= k.top || entry == 0) continue;
         if (to != nullptr) {
@@ -255,15 +258,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     extern __shared__ __align__(16) char shared[];
     __shared__ Part parts[2][kWarps];
     __shared__ Part cluster_parts[kMostBlocks];
-    __shared__ int count, owners;
+    __shared__ int count, found;
+    __shared__ uint32_t least;  // what an entry has to reach
     __shared__ int before[kWarps];
-    __shared__ uint16_t owner_list[THREADS];
     pdl_prologue();
     const int tid = threadIdx.x, room = room_for(k.top);
     const uint32_t rank = blockIdx.x % blocks, stride = gridDim.x / blocks;
     uint4* const ring = reinterpret_cast<uint4*>(shared) + tid;
     uint64_t* const entries = reinterpret_cast<uint64_t*>(shared + kStages * kChunk * 16);
     uint64_t* const merged = entries + room;  // (of a cluster's first block)
+    // where entries are wanted: every thread's maximum, its stretches', and the stretches that are read again
+    uint32_t* const tops = reinterpret_cast<uint32_t*>(merged + (blocks > 1 ? blocks * k.top : 0));
+    uint32_t* const stretch_tops = tops + THREADS;
+    uint16_t* const stretch_list = reinterpret_cast<uint16_t*>(stretch_tops + kStretches * THREADS);
     const float c = k.inverse * kLog2e;
     if (blocks > 1) cluster_sync();  // (every block is there before another writes to it)
 
@@ -301,6 +308,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     };
     for (int i = 0; i < kStages; ++i) ask();
 
+    auto token_of = [&](uint32_t r) { return tid == 0 && rank == 0 && r < k.rows && k.tokens.base != nullptr ? load_index(row_at(k.tokens, k.inner, r), k.wide_tokens) : int64_t(-1); };
+    int64_t id = token_of(blockIdx.x / blocks);  // (asked for a row ahead)
     const uint4* place = ring;
     uint32_t parity = 0;
     for (uint32_t r = blockIdx.x / blocks; r < k.rows; r += stride, parity ^= 1) {
@@ -309,23 +318,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         int end = -1;
         if (rank == 0 && tid < row.head) end = tid;
         else if (rank + 1 == blocks && tid >= 8 && row.tail + (tid - 8) < k.vocab) end = row.tail + (tid - 8);
-        Part part{-INFINITY, 0.f, 0.f};
-        float end_z = 0.f;
-        if (end >= 0) {
-            end_z = to_float(row.z[end]);
-            uint4 one[1] = {make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>)};
-            if constexpr (sizeof(T) == 2) one[0].x = 0xfc000000u | __half_as_ushort(row.z[end]);
-            else one[0].x = __float_as_uint(end_z);
-            take<T>(part, one, c);
-        }
+        const T end_element = end >= 0 ? row.z[end] : from_float<T>(0.f);
         float token_z = 0.f;
         bool token = false;
-        if (tid == 0 && rank == 0 && k.tokens.base != nullptr) {
-            const int64_t id = load_index(row_at(k.tokens, k.inner, r), k.wide_tokens);
+        if (tid == 0) {
             if (id >= k.vocab) atomicOr(k.status, kStatusIndexOutOfRange);
             token = id >= 0 && id < k.vocab;
             if (token) token_z = to_float(row.z[id]);
+            id = token_of(r + stride);
         }
+        Part part{-INFINITY, 0.f, 0.f};
+        // (two to the power of `shift` batches make a stretch)
+        int shift = 0, batch = 0, stretch = 0;
+        while ((row.last - row.first + kChunk - 1) / kChunk > kStretches << shift) ++shift;
+        float stretch_top = -INFINITY;
         for (int rest = row.last - row.first; rest > 0; rest -= kChunk) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             uint4 raw[kBatch];
@@ -342,7 +348,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
             place += kChunk;
             if (place == ring + kStages * kChunk) place = ring;
             ask();  // (into the place that was just read)
-            take<T>(part, raw, c);
+            const float top = largest<T>(raw);
+            take<T>(part, raw, top, c);
+            if (k.top > 0) {
+                stretch_top = max_nan(stretch_top, top);
+                if ((++batch & ((1 << shift) - 1)) == 0 || rest <= kChunk) {
+                    stretch_tops[stretch++ * THREADS + tid] = order_of(stretch_top);
+                    stretch_top = -INFINITY;
+                }
+            }
+        }
+        const float end_z = to_float(end_element);
+        if (end >= 0) {
+            uint4 one[1] = {make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>)};
+            if constexpr (sizeof(T) == 2) one[0].x = 0xfc000000u | __half_as_ushort(end_element);
+            else one[0].x = __float_as_uint(end_element);
+            take<T>(part, one, end_z, c);
         }
         const float own_top = part.top;
         const Part mine = warp_part(part, c);
@@ -357,35 +378,46 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         }
         int n = 0;
         if (k.top > 0) {
-            if (tid == 0) count = 0, owners = 0;
-            // a bound that at least `top` elements reach, if there are as many threads that have any
             const bool owner = end >= 0 || row.first + tid < row.last;
             const uint32_t own = owner ? order_of(own_top) : 0u;
-            uint32_t lo = 0, hi = order_of(block_top);
-            if (__syncthreads_count(own >= hi) >= k.top) lo = hi;
-            else {
-                while (hi - lo > (sizeof(T) == 2 ? 8192u : 1u)) {
-                    const uint32_t mid = lo + (hi - lo) / 2;
-                    const int reach = __syncthreads_count(own >= mid);
-                    if (reach >= k.top) lo = mid;
-                    else hi = mid;
-                    if (reach == k.top) break;
-                }
-            }
-            // Of vectors of a thread's from its `begin`-th on, every `step`-th: (order, column) of the elements, where one of a vector's reaches the bound.
-            auto each = [&](int of, int begin, int step, uint32_t bound, auto&& visit) {
-                for (int i = row.first + of + begin * THREADS; i < row.last; i += step * THREADS) {
-                    const uint4 raw[1] = {row.vectors()[i]};
-                    if (order_of(largest<T>(raw)) < bound) continue;
-                    float x[E];
-                    unpack<T>(raw[0], x);
+            tops[tid] = own;
+            if (tid == 0) count = 0, found = 0;
+            __syncthreads();
+            if (tid < 32) {  // a bound that at least `top` elements reach, if there are as many threads that have any
+                uint32_t x[kWarps];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) visit(order_of(x[e]), static_cast<uint32_t>(row.head + i * E + e));
+                for (int i = 0; i < kWarps; ++i) x[i] = tops[i * 32 + tid];
+                auto reaching = [&](uint32_t bound) {
+                    int some = 0;
+#pragma unroll
+                    for (int i = 0; i < kWarps; ++i) some += x[i] >= bound;
+                    return static_cast<int>(__reduce_add_sync(0xffffffffu, some));
+                };
+                uint32_t low = 0, high = order_of(block_top);
+                if (reaching(high) >= k.top) low = high;
+                while (high - low > (sizeof(T) == 2 ? 8192u : 1u)) {
+                    const uint32_t mid = low + (high - low) / 2;
+                    const int reach = reaching(mid);
+                    if (reach >= k.top) low = mid;
+                    else high = mid;
+                    if (reach >= k.top && reach <= k.top + k.top / 4) break;
                 }
+                if (tid == 0) least = low;
+            }
+            __syncthreads();
+            uint32_t lo = least;
+            // (order, column) of a vector's elements, where one of them reaches the bound.
+            auto each = [&](int v, uint32_t bound, auto&& visit) {
+                const uint4 raw[1] = {row.vectors()[v]};
+                if (order_of(largest<T>(raw)) < bound) return;
+                float x[E];
+                unpack<T>(raw[0], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) visit(order_of(x[e]), static_cast<uint32_t>(row.head + v * E + e));
             };
             auto counted = [&](uint32_t bound) {  // how many of the elements reach a bound
                 int some = 0;
-                if (own >= bound) each(tid, 0, 1, bound, [&](uint32_t o, uint32_t) { some += o >= bound; });
+                for (int v = row.first + tid; v < row.last && own >= bound; v += THREADS) each(v, bound, [&](uint32_t o, uint32_t) { some += o >= bound; });
                 if (end >= 0) some += order_of(end_z) >= bound;
                 some = __reduce_add_sync(0xffffffffu, some);
                 __syncthreads();
@@ -400,10 +432,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
                     const int i = atomicAdd(&count, 1);
                     if (i < room) entries[i] = uint64_t(o) << 32 | (0xffffffffu - column);
                 };
-                if (own >= bound && row.first + tid < row.last) owner_list[atomicAdd(&owners, 1)] = static_cast<uint16_t>(tid);
+                for (int s = 0; s < stretch && own >= bound; ++s) {
+                    if (stretch_tops[s * THREADS + tid] >= bound) stretch_list[atomicAdd(&found, 1)] = static_cast<uint16_t>(s * THREADS + tid);
+                }
                 if (end >= 0) put(order_of(end_z), static_cast<uint32_t>(end));
                 __syncthreads();
-                for (int o = tid / 32; o < owners; o += kWarps) each(owner_list[o], tid % 32, 32, bound, put);
+                const int all_found = found, bits = shift + 2;  // (a stretch's vectors)
+                static_assert(kBatch == 4);
+                for (int m = tid; m < all_found << bits; m += THREADS) {
+                    const int at = stretch_list[m >> bits], v = row.first + ((at / THREADS << bits) + (m & ((1 << bits) - 1))) * THREADS + at % THREADS;
+                    if (v < row.last) each(v, bound, put);
+                }
                 __syncthreads();
             };
             collect(lo);
@@ -425,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
                 }
                 const int equal_too = counted(lo);
                 __syncthreads();
-                if (tid == 0) count = 0, owners = 0;
+                if (tid == 0) count = 0, found = 0;
                 __syncthreads();
                 if (equal_too <= room) {
                     collect(lo);
@@ -690,24 +729,26 @@ void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
     ProfScope scope(ctx, "token_logprobs");
     const bool half = a.logits.dtype == B200_F16;
     const int64_t vectors = ceil_div(plan.vocab, half ? 8 : 4);
-    // Threads of a block: 32 vectors to each, as a row's end costs a thread as much as 4 of them or more; and more threads than entries that are wanted.  Few rows: up
-    // to 512 threads of four vectors, and long ones a cluster of blocks each.
+    // Threads of a block: 32 vectors to each, as a row's end costs a thread as much as 4 of them or more, up to 128, whose warps wait together (2047 x 128000 F32: 171 us with
+    // blocks of 64, 174 with 128, 199 with 256); and more threads than entries that are wanted.  Few rows: up to 512 threads of four vectors, and long ones a
+    // cluster of blocks each.
     const bool few = plan.s.rows <= sm_count();
     int threads = 32, blocks = 1;
-    while (threads < kMostThreads && (vectors > int64_t(threads) * (few ? 4 : 32) || plan.top * 2 > threads)) threads *= 2;
+    while (threads < kMostThreads && ((vectors > int64_t(threads) * (few ? 4 : 32) && (few || threads < 128)) || plan.top * 2 > threads)) threads *= 2;
     while (blocks < kMostBlocks && plan.s.rows * blocks * 2 <= sm_count() && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
     auto go = [&](auto kernel) {
-        const size_t shared = size_t(kStages) * kBatch * 16 * static_cast<size_t>(threads) + (k.top > 0 ? (static_cast<size_t>(room_for(k.top)) + (blocks > 1 ? static_cast<size_t>(blocks) * k.top : 0)) * 8 : 0);
+        size_t shared = size_t(kStages) * kBatch * 16 * static_cast<size_t>(threads);
+        if (k.top > 0) shared += (static_cast<size_t>(room_for(k.top)) + (blocks > 1 ? static_cast<size_t>(blocks) * k.top : 0)) * 8 + static_cast<size_t>(threads) * (4 + 6 * kStretches);
         const int most = blocks_at_once(reinterpret_cast<const void*>(kernel), threads, shared);
         if (blocks > 1) {
             launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(plan.s.rows * blocks)), dim3(threads), shared, blocks, false, k, static_cast<uint32_t>(blocks));
             return;
         }
-        // Blocks that stay: as many on an SM as leave the fewest without a last row, down to half.
+        // Blocks that stay: as many on an SM as leave the fewest without a last row, down to three quarters.
         const int64_t sms = sm_count();
         auto rounds = [&](int on_sm) { return ceil_div(plan.s.rows, sms * on_sm) * on_sm; };
         int on_sm = most;
-        for (int n = most - 1; n >= std::max(1, most / 2); --n) {
+        for (int n = most - 1; n * 4 >= most * 3; --n) {
             if (rounds(n) < rounds(on_sm)) on_sm = n;
         }
         launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(std::min<int64_t>(plan.s.rows, sms * on_sm))), dim3(threads), shared, k, 1u);
