@@ -25,7 +25,6 @@ namespace {
 constexpr int kMostTop = B200_MOST_TOP;
 constexpr int kMostThreads = 512;
 constexpr int kBatch = 4;    // vectors that a thread takes at once
-constexpr int kStages = 3;   // batches on their way
 constexpr int kMostBlocks = 8;  // of a cluster
 constexpr int kStretches = 4;   // of a thread's batches
 // Entries that there is room for: where fewer threads have elements than are wanted, all of a row's are entries (8 to each of them, and the ends).
@@ -63,7 +62,7 @@ __device__ __forceinline__ float shift_of(float top) { return top == -INFINITY ?
 // Elements of a row that lie before its first 16-byte boundary.
 template <typename T>
 __device__ __forceinline__ int head_of(const T* row, int64_t n) {
-    const int64_t head = (16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / int64_t(sizeof(T));
+    const uint32_t head = (0u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row))) % 16 / uint32_t(sizeof(T));
     return static_cast<int>(head < n ? head : n);
 }
 
@@ -191,10 +190,6 @@ __device__ __forceinline__ uint32_t in_block(uint32_t address, uint32_t rank) {
     return to;
 }
 
-__device__ __forceinline__ void copy_vector(uint32_t to, const uint4* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(__cvta_generic_to_global(from)) : "memory");
-}
-
 // A row, or the part of it that is a block's: its vectors [first, last), and the elements in front of its first vector and behind its last one.
 template <typename T>
 struct Row {
@@ -203,9 +198,10 @@ struct Row {
     __device__ __forceinline__ Row(const Args& k, uint32_t r, uint32_t rank, uint32_t blocks) {
         z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
         head = head_of(z, k.vocab);
-        const int64_t vectors = (k.vocab - head) / int64_t(16 / sizeof(T));
+        const uint32_t vectors = static_cast<uint32_t>(k.vocab - head) / uint32_t(16 / sizeof(T));
         tail = head + static_cast<int>(vectors) * int(16 / sizeof(T));
-        first = static_cast<int>(vectors * rank / blocks), last = static_cast<int>(vectors * (rank + 1) / blocks);
+        const int bits = 31 - __clz(blocks);  // (a power of two)
+        first = static_cast<int>(uint64_t(vectors) * rank >> bits), last = static_cast<int>(uint64_t(vectors) * (rank + 1) >> bits);
     }
     __device__ __forceinline__ const uint4* vectors() const { return reinterpret_cast<const uint4*>(z + head); }
 };
@@ -251,9 +247,9 @@ __device__ __forceinline__ void rank_entries(const Args& k, uint32_t r, const Pa
     }
 }
 
-// `blocks`: of a row's cluster (1: the blocks take row after row).  Dynamic shared memory: the batches on their way, then the entries.
+// `blocks`: of a row's cluster (1: the blocks take row after row).
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const Args k, uint32_t blocks) {
+__global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 / THREADS) logprobs_kernel(const Args k, uint32_t blocks) {
     constexpr int E = 16 / sizeof(T), kWarps = THREADS / 32, kChunk = THREADS * kBatch;  // (vectors of a chunk)
     extern __shared__ __align__(16) char shared[];
     __shared__ Part parts[2][kWarps];
@@ -264,8 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     pdl_prologue();
     const int tid = threadIdx.x, room = room_for(k.top);
     const uint32_t rank = blockIdx.x % blocks, stride = gridDim.x / blocks;
-    uint4* const ring = reinterpret_cast<uint4*>(shared) + tid;
-    uint64_t* const entries = reinterpret_cast<uint64_t*>(shared + kStages * kChunk * 16);
+    uint64_t* const entries = reinterpret_cast<uint64_t*>(shared);
     uint64_t* const merged = entries + room;  // (of a cluster's first block)
     // where entries are wanted: every thread's maximum, its stretches', and the stretches that are read again
     uint32_t* const tops = reinterpret_cast<uint32_t*>(merged + (blocks > 1 ? blocks * k.top : 0));
@@ -274,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     const float c = k.inverse * kLog2e;
     if (blocks > 1) cluster_sync();  // (every block is there before another writes to it)
 
-    // What is asked for next: this thread's first vector of a chunk, the vectors from that chunk on, and where they go.
+    // What is on its way: this thread's vectors of the next chunk, of this row or of the one behind it; what is asked for after it, and the vectors left from there on.
     uint32_t row_next = blockIdx.x / blocks;
     const uint4* from;
     int left;
@@ -284,8 +279,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         left = row.last - row.first;
     };
     begin();
-    const uint32_t ring_begin = shared_address(ring), ring_end = ring_begin + kStages * kChunk * 16;
-    uint32_t to = ring_begin;
+    uint4 next[kBatch];
     auto ask = [&]() {
         while (left <= 0 && row_next < k.rows) {
             row_next += stride;
@@ -293,24 +287,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         }
         if (left >= kChunk) {
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) copy_vector(to + i * THREADS * 16, from + i * THREADS);
+            for (int i = 0; i < kBatch; ++i) next[i] = __ldcs(from + i * THREADS);
         } else {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                if (i * THREADS + tid < left) copy_vector(to + i * THREADS * 16, from + i * THREADS);
+                next[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
+                if (i * THREADS + tid < left) next[i] = __ldcs(from + i * THREADS);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
         from += kChunk;
         left -= kChunk;
-        to += kChunk * 16;
-        if (to == ring_end) to = ring_begin;
     };
-    for (int i = 0; i < kStages; ++i) ask();
+    ask();
 
     auto token_of = [&](uint32_t r) { return tid == 0 && rank == 0 && r < k.rows && k.tokens.base != nullptr ? load_index(row_at(k.tokens, k.inner, r), k.wide_tokens) : int64_t(-1); };
     int64_t id = token_of(blockIdx.x / blocks);  // (asked for a row ahead)
-    const uint4* place = ring;
     uint32_t parity = 0;
     for (uint32_t r = blockIdx.x / blocks; r < k.rows; r += stride, parity ^= 1) {
         const Row<T> row(k, r, rank, blocks);
@@ -333,21 +324,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
         while ((row.last - row.first + kChunk - 1) / kChunk > kStretches << shift) ++shift;
         float stretch_top = -INFINITY;
         for (int rest = row.last - row.first; rest > 0; rest -= kChunk) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
             uint4 raw[kBatch];
-            if (rest >= kChunk) {
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) raw[i] = place[i * THREADS];
-            } else {
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    raw[i] = make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>);
-                    if (i * THREADS + tid < rest) raw[i] = place[i * THREADS];
-                }
-            }
-            place += kChunk;
-            if (place == ring + kStages * kChunk) place = ring;
-            ask();  // (into the place that was just read)
+            for (int i = 0; i < kBatch; ++i) raw[i] = next[i];
+            ask();
             const float top = largest<T>(raw);
             take<T>(part, raw, top, c);
             if (k.top > 0) {
@@ -366,11 +346,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
             take<T>(part, one, end_z, c);
         }
         const float own_top = part.top;
-        const Part mine = warp_part(part, c);
-        if (tid % 32 == 0) parts[parity][tid / 32] = mine;
-        __syncthreads();
-        Part all = tid % 32 < kWarps ? parts[parity][tid % 32] : Part{-INFINITY, 0.f, 0.f};
-        all = warp_part(all, c);
+        Part all = warp_part(part, c);
+        if constexpr (kWarps > 1) {
+            if (tid % 32 == 0) parts[parity][tid / 32] = all;
+            __syncthreads();
+            all = tid % 32 < kWarps ? parts[parity][tid % 32] : Part{-INFINITY, 0.f, 0.f};
+            all = warp_part(all, c);
+        } else {
+            __syncwarp();
+        }
         const float block_top = all.top;
         if (k.top == 0 && blocks == 1) {
             if (tid == 0) write_row(k, r, all, token, token_z);
@@ -394,6 +378,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
                     return static_cast<int>(__reduce_add_sync(0xffffffffu, some));
                 };
                 uint32_t low = 0, high = order_of(block_top);
+                if (k.top <= 32) {  // (what every lane's largest reaches, 32 do)
+                    uint32_t lane_top = x[0];
+#pragma unroll
+                    for (int i = 1; i < kWarps; ++i) lane_top = max(lane_top, x[i]);
+                    low = __reduce_min_sync(0xffffffffu, lane_top);
+                }
                 if (reaching(high) >= k.top) low = high;
                 while (high - low > (sizeof(T) == 2 ? 8192u : 1u)) {
                     const uint32_t mid = low + (high - low) / 2;
@@ -518,7 +508,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
             }
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- the gradient -----------------------------------------------------------
@@ -737,7 +726,7 @@ void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
     while (threads < kMostThreads && ((vectors > int64_t(threads) * (few ? 4 : 32) && (few || threads < 128)) || plan.top * 2 > threads)) threads *= 2;
     while (blocks < kMostBlocks && plan.s.rows * blocks * 2 <= sm_count() && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
     auto go = [&](auto kernel) {
-        size_t shared = size_t(kStages) * kBatch * 16 * static_cast<size_t>(threads);
+        size_t shared = 0;
         if (k.top > 0) shared += (static_cast<size_t>(room_for(k.top)) + (blocks > 1 ? static_cast<size_t>(blocks) * k.top : 0)) * 8 + static_cast<size_t>(threads) * (4 + 6 * kStretches);
         const int most = blocks_at_once(reinterpret_cast<const void*>(kernel), threads, shared);
         if (blocks > 1) {
