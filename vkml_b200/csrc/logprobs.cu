@@ -10,7 +10,7 @@
 // that a row's end costs other rows' time only.  Few long rows are a cluster's each, whose blocks take a part of it.
 //
 // The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least
-// reach; it is found by halving the range between the maxima, by one warp.  Each thread has kept the maxima of up to four stretches of what it had, too: only
+// reach; it is found by halving the range between the maxima, by one warp.  Each thread has kept the maxima of up to sixteen stretches of what it had, too: only
 // stretches whose maximum reaches the bound (little more than K) are read again, and what reaches it goes into shared memory, where an entry's rank is the number of larger ones.  Where more entries reach it than
 // there is room for (a row of few different values: most of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in
 // the order of their columns.
@@ -26,7 +26,7 @@ constexpr int kMostTop = B200_MOST_TOP;
 constexpr int kMostThreads = 512;
 constexpr int kBatch = 4;    // vectors that a thread takes at once
 constexpr int kMostBlocks = 8;  // of a cluster
-constexpr int kStretches = 4;   // of a thread's batches
+constexpr int kStretches = 16;   // of a thread's batches
 // Entries that there is room for: where fewer threads have elements than are wanted, all of a row's are entries (8 to each of them, and the ends).
 __host__ __device__ constexpr int room_for(int top) { return top * 8 + 16; }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
                     const int reach = reaching(mid);
                     if (reach >= k.top) low = mid;
                     else high = mid;
-                    if (reach >= k.top && reach <= k.top + k.top / 4) break;
+                    if (reach >= k.top && reach <= k.top + k.top / 8) break;
                 }
                 if (tid == 0) least = low;
             }
