@@ -501,7 +501,7 @@ typedef struct b200_adamw_args {
     b200_tensor scale_on_device;      /* one F32, times grad_scale (clipping; an unscaled loss); absent: 1.  Where the product is not finite nothing changes */
     int64_t step;                     /* from 1 on */
     double beta1, beta2;              /* in [0, 1) */
-    float lr, eps, grad_scale;        /* eps above 0 */
+    float lr, eps, grad_scale;        /* eps: a normal number above 0 */
     uint32_t seed;                    /* 8 bits only */
 } b200_adamw_args;
 int b200_adamw(b200_ctx* ctx, const b200_adamw_args* args);

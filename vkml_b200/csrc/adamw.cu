@@ -44,7 +44,7 @@ struct Numbers {
     const int64_t* step_at;
     const float* scale_at;
     int64_t step;
-    float lr, b1, rest1, b2, rest2, eps, scale;
+    float lr, b1, rest1, b2, rest2, eps, scale, one;
     float log_b1, log_b2;                  // natural logarithms
     float inverse1, root_inverse2;         // 1 / (1 - b1^step), 1 / sqrt(1 - b2^step)
     uint32_t seed;
@@ -72,11 +72,19 @@ __device__ __forceinline__ float2 byte_values(uint32_t pair) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// The byte of a size that is at most 448, up or down by 16 random bits.  Times 2^-120 a float's exponent field is the byte's, and so are the leading bits of its
-// fraction, subnormal ones too: adding below them carries into them.
-__device__ __forceinline__ uint32_t byte_of(float x, uint32_t bits) {
-    const uint32_t whole = __float_as_uint(x * 0x1p-120f);
-    return min((whole + (bits << 4 | 8u)) >> 20, 126u);
+// The byte of a size that is at most 448, in the upper 8 bits, up or down by 16 random bits, which lie in `noise` as 0x00rrrr80.  Times 2^-120 a float's exponent field is
+// the byte's, and so are the leading bits of its fraction, subnormal ones too: adding below them carries into them.  `size`: that product, its sign aside.
+__device__ __forceinline__ uint32_t byte_of(float size, uint32_t noise) { return min((__float_as_uint(size) << 4) + noise, 0x7effffffu); }
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // What a block's sizes are divided by, and its inverse; of a block that is zero, or not finite.
@@ -98,12 +106,31 @@ __device__ __forceinline__ Scale scale_of(uint32_t most_bits) {
 
 struct Step {
     float b1, rest1, b2, rest2, eps, scale, root_inverse2, keep, rate;
-    __device__ __forceinline__ void moments(float g, float& m, float& v) const {
-        g = g * scale;
-        m = m * b1 + g * rest1;
-        v = v * b2 + g * g * rest2;
+    // 1, as the launch's parameters have it: a + b is a multiply-add by it.  Products and sums of pairs are joined into multiply-adds by the assembler, whatever the
+    // compiler is told (and so are those by a 1 that it sees), and the bytes would not be those of the formulas.
+    float one;
+    __device__ __forceinline__ void moments(const float (&grad)[8], float (&m)[8], float (&v)[8]) const {
+        float g[8], t[8];
+        mul8(g, grad, scale);
+        mul8(t, g, rest1);
+        mul8(m, m, b1);
+        fma8(m, m, one, t);
+        mul8(t, g, g);
+        mul8(t, t, rest2);
+        mul8(v, v, b2);
+        fma8(v, v, one, t);
     }
-    __device__ __forceinline__ float param(float p, float m, float root) const { return p * keep - __fdividef(m, root * root_inverse2 + eps) * rate; }
+    __device__ __forceinline__ void update(float (&p)[8], const float (&m)[8], const float (&root)[8]) const {
+        float t[8];
+        mul8(t, root, root_inverse2);
+        add8(t, t, eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = fast_reciprocal(t[e]);
+        mul8(t, t, m);
+        mul8(t, t, -rate);
+        mul8(p, p, keep);
+        add8(p, p, t);
+    }
 };
 
 // Eight elements of a lane: neighbours where the tensor's addresses allow it, else 32 apart.
@@ -157,9 +184,10 @@ __device__ __forceinline__ void bytes_values(float (&x)[8], const uint32_t (&c)[
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = byte_values(c[i / 2] >> (i % 2 * 16));
-        x[2 * i] = f.x * scale;
-        x[2 * i + 1] = f.y * scale;
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
     }
+    mul8(x, x, scale);
 }
 
 // 256 elements from element `from` on, or what is left of them.
@@ -179,45 +207,51 @@ __device__ __forceinline__ void step_block(const Tensor& t, const Step& s, uint3
         scales = t.scales[from / kBlock];
         bytes_values(m, a, scales.x);
         bytes_values(v, b, scales.y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * v[e];
+        mul8(v, v, v);
     } else {
         load_values<WIDE>(m, static_cast<const float*>(t.first) + from, left, lane);
         load_values<WIDE>(v, static_cast<const float*>(t.second) + from, left, lane);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s.moments(g[e], m[e], v[e]);
+    s.moments(g, m, v);
     if (!bytes) {
         store_values<WIDE>(static_cast<float*>(t.first) + from, m, left, lane);
         store_values<WIDE>(static_cast<float*>(t.second) + from, v, left, lane);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = sqrtf(v[e]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = s.param(p[e], m[e], v[e]);
+    s.update(p, m, v);
     store_values<WIDE>(t.param + from, p, left, lane);
     if (t.copy != nullptr) store_values<WIDE>(t.copy + from, p, left, lane);
     if (!bytes) return;
-    uint32_t most_m = 0, most_v = 0;
+    float most_m = fabsf(m[0]), most_v = v[0];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        most_m = max(most_m, __float_as_uint(m[e]) & 0x7fffffffu);
-        most_v = max(most_v, __float_as_uint(v[e]) & 0x7fffffffu);
+    for (int e = 1; e < 8; ++e) most_m = max_nan(most_m, fabsf(m[e])), most_v = max_nan(most_v, v[e]);
+    const Scale sm = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(most_m))), sv = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(most_v)));
+    // over the scale, times 2^-120: one product, where that factor is not subnormal (values up to 14336), else two
+    float x[8], y[8];
+    if (min(sm.inverse, sv.inverse) >= 0x1p-5f) {
+        mul8(x, m, sm.inverse * 0x1p-120f);
+        mul8(y, v, sv.inverse * 0x1p-120f);
+    } else {
+        mul8(x, m, sm.inverse);
+        mul8(x, x, 0x1p-120f);
+        mul8(y, v, sv.inverse);
+        mul8(y, y, 0x1p-120f);
     }
-    const Scale sm = scale_of(__reduce_max_sync(0xffffffffu, most_m)), sv = scale_of(__reduce_max_sync(0xffffffffu, most_v));
-    a[0] = a[1] = b[0] = b[1] = 0;
+    const uint32_t least = sv.inverse > 0.f ? 0x01000000u : 0u;
+    uint32_t first[8], second[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const uint32_t i = static_cast<uint32_t>(from) + static_cast<uint32_t>(WIDE ? lane * 8 + e : e * 32 + lane);
         const uint32_t bits = mix(key + i * 0x9e3779b9u);
-        uint32_t first = byte_of(fabsf(m[e]) * sm.inverse, bits & 0xffffu) | (__float_as_uint(m[e]) >> 31 << 7);
-        uint32_t second = byte_of(v[e] * sv.inverse, bits >> 16);
-        if (v[e] > 0.f && sv.inverse > 0.f) second = max(second, 1u);
-        if (sm.broken) first = 127u;
-        if (sv.broken) second = 127u;
-        a[e / 4] |= first << (e % 4 * 8);
-        b[e / 4] |= second << (e % 4 * 8);
+        first[e] = byte_of(x[e], __byte_perm(bits, 0x80u, 0x7104)) | (__float_as_uint(m[e]) & 0x80000000u);
+        second[e] = byte_of(y[e], __byte_perm(bits, 0x80u, 0x7324));
+        if (v[e] > 0.f) second[e] = max(second[e], least);
     }
+    a[0] = upper_bytes(first[0], first[1], first[2], first[3]), a[1] = upper_bytes(first[4], first[5], first[6], first[7]);
+    b[0] = upper_bytes(second[0], second[1], second[2], second[3]), b[1] = upper_bytes(second[4], second[5], second[6], second[7]);
+    if (sm.broken) a[0] = a[1] = 0x7f7f7f7fu;
+    if (sv.broken) b[0] = b[1] = 0x7f7f7f7fu;
     store_bytes<WIDE>(static_cast<uint8_t*>(t.first) + from, a, left, lane);
     store_bytes<WIDE>(static_cast<uint8_t*>(t.second) + from, b, left, lane);
     if (lane == 0) t.scales[from / kBlock] = make_float2(sm.scale, sv.scale);
@@ -235,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     const Tensor& t = k.t[lo];
     const Numbers& n = k.numbers;
     Step s;
-    s.b1 = n.b1, s.rest1 = n.rest1, s.b2 = n.b2, s.rest2 = n.rest2, s.eps = n.eps, s.scale = n.scale;
+    s.b1 = n.b1, s.rest1 = n.rest1, s.b2 = n.b2, s.rest2 = n.rest2, s.eps = n.eps, s.scale = n.scale, s.one = n.one;
     float inverse1 = n.inverse1, lr = n.lr;
     int64_t step = n.step;
     s.root_inverse2 = n.root_inverse2;
@@ -289,7 +323,7 @@ void check_numbers(const b200_adamw_args& a) {
     check_one(a.step_on_device, "step_on_device", B200_I64);
     check_one(a.scale_on_device, "scale_on_device", B200_F32);
     if (!(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1)) fail(B200_INVALID_ARGUMENT, "adamw: a beta is not in [0, 1)");
-    if (!(a.eps > 0.f) || std::isinf(a.eps)) fail(B200_INVALID_ARGUMENT, "adamw: eps is not above 0 and finite");
+    if (!(a.eps >= 0x1p-126f) || std::isinf(a.eps)) fail(B200_INVALID_ARGUMENT, "adamw: eps is not a normal number above 0");
     if (!std::isfinite(a.lr) || !std::isfinite(a.grad_scale)) fail(B200_INVALID_ARGUMENT, "adamw: lr or grad_scale is not finite");
     if (a.step < 1) fail(B200_INVALID_ARGUMENT, "adamw: the step is below 1");
 }
@@ -377,7 +411,7 @@ void launch_adamw(b200_ctx* ctx, const b200_adamw_args& a) {
     k.step_at = static_cast<const int64_t*>(a.step_on_device.data);
     k.scale_at = static_cast<const float*>(a.scale_on_device.data);
     k.step = a.step;
-    k.lr = a.lr, k.eps = a.eps, k.scale = a.grad_scale, k.seed = a.seed;
+    k.lr = a.lr, k.eps = a.eps, k.scale = a.grad_scale, k.seed = a.seed, k.one = 1.f;
     k.b1 = static_cast<float>(a.beta1), k.rest1 = static_cast<float>(1 - a.beta1), k.log_b1 = static_cast<float>(std::log(a.beta1));
     k.b2 = static_cast<float>(a.beta2), k.rest2 = static_cast<float>(1 - a.beta2), k.log_b2 = static_cast<float>(std::log(a.beta2));
     k.inverse1 = static_cast<float>(1 / (1 - std::pow(a.beta1, static_cast<double>(a.step))));
