@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <vector>
 
 namespace b200 {
@@ -21,9 +22,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;                // elements that share a scale: a warp's
-constexpr int kRounds = 4;                 // blocks of 256 that a warp takes one after another
-constexpr int kItem = kThreads / 32 * kRounds * kBlock;  // elements of a block of threads
+constexpr int kRound = kThreads / 32 * kBlock;  // elements that a block of threads takes at once
+constexpr int kMostRounds = 8;             // ... and how often, with 8-bit states: the next round's elements are on their way (8 a thread: 328 us in place of 369); half as often with F32
 constexpr int kMostTensors = 384;          // of a launch: 32,764 bytes of parameters
+constexpr int kFewTensors = 24;            // (fewer bytes go with a launch of few)
 
 struct Tensor {
     float* param;
@@ -48,6 +50,7 @@ struct Numbers {
     float log_b1, log_b2;                  // natural logarithms
     float inverse1, root_inverse2;         // 1 / (1 - b1^step), 1 / sqrt(1 - b2^step)
     uint32_t seed;
+    int rounds;
 };
 
 template <int N>
@@ -190,39 +193,38 @@ __device__ __forceinline__ void bytes_values(float (&x)[8], const uint32_t (&c)[
     mul8(x, x, scale);
 }
 
-// 256 elements from element `from` on, or what is left of them.
-template <bool WIDE>
-__device__ __forceinline__ void step_block(const Tensor& t, const Step& s, uint32_t key, int64_t from, int lane) {
-    const int64_t left = t.n - from;
-    float p[8], g[8], m[8], v[8];
-    uint32_t a[2], b[2];
-    float2 scales = make_float2(0.f, 0.f);
-    load_values<WIDE>(p, t.param + from, left, lane);
-    if (t.half_grad) load_values<WIDE>(g, static_cast<const __half*>(t.grad) + from, left, lane);
-    else load_values<WIDE>(g, static_cast<const float*>(t.grad) + from, left, lane);
-    const bool bytes = t.scales != nullptr;
-    if (bytes) {
-        load_bytes<WIDE>(a, static_cast<const uint8_t*>(t.first) + from, left, lane);
-        load_bytes<WIDE>(b, static_cast<const uint8_t*>(t.second) + from, left, lane);
+// What a lane has of 256 elements with 8-bit states, as it lies in memory.
+struct RawBytes {
+    Raw8<float> param, grad32;
+    Raw8<__half> grad16;
+    uint2 first, second;
+    float2 scales;
+    __device__ __forceinline__ void load(const Tensor& t, int64_t from, int lane) {
+        const int64_t at = from + lane * 8;
+        load8(param, t.param + at);
+        if (t.half_grad) load8(grad16, static_cast<const __half*>(t.grad) + at);
+        else load8(grad32, static_cast<const float*>(t.grad) + at);
+        first = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.first) + at);
+        second = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.second) + at);
         scales = t.scales[from / kBlock];
-        bytes_values(m, a, scales.x);
-        bytes_values(v, b, scales.y);
-        mul8(v, v, v);
-    } else {
-        load_values<WIDE>(m, static_cast<const float*>(t.first) + from, left, lane);
-        load_values<WIDE>(v, static_cast<const float*>(t.second) + from, left, lane);
     }
+};
+
+// The step of 256 elements with 8-bit states: p, g and the bytes as they were.
+template <bool WIDE>
+__device__ __forceinline__ void step_bytes(const Tensor& t, const Step& s, uint32_t key, int64_t from, int lane, float (&p)[8], const float (&g)[8], uint32_t (&a)[2], uint32_t (&b)[2],
+                                           float2 scales) {
+    const int64_t left = t.n - from;
+    float m[8], v[8];
+    bytes_values(m, a, scales.x);
+    bytes_values(v, b, scales.y);
+    mul8(v, v, v);
     s.moments(g, m, v);
-    if (!bytes) {
-        store_values<WIDE>(static_cast<float*>(t.first) + from, m, left, lane);
-        store_values<WIDE>(static_cast<float*>(t.second) + from, v, left, lane);
-    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = sqrtf(v[e]);
     s.update(p, m, v);
     store_values<WIDE>(t.param + from, p, left, lane);
     if (t.copy != nullptr) store_values<WIDE>(t.copy + from, p, left, lane);
-    if (!bytes) return;
     float most_m = fabsf(m[0]), most_v = v[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) most_m = max_nan(most_m, fabsf(m[e])), most_v = max_nan(most_v, v[e]);
@@ -256,9 +258,45 @@ __device__ __forceinline__ void step_block(const Tensor& t, const Step& s, uint3
     store_bytes<WIDE>(static_cast<uint8_t*>(t.second) + from, b, left, lane);
     if (lane == 0) t.scales[from / kBlock] = make_float2(sm.scale, sv.scale);
 }
+__device__ __forceinline__ void step_bytes(const Tensor& t, const Step& s, uint32_t key, int64_t from, int lane, const RawBytes& raw) {
+    float p[8], g[8];
+    unpack8(raw.param, p);
+    if (t.half_grad) unpack8(raw.grad16, g);
+    else unpack8(raw.grad32, g);
+    uint32_t a[2] = {raw.first.x, raw.first.y}, b[2] = {raw.second.x, raw.second.y};
+    step_bytes<true>(t, s, key, from, lane, p, g, a, b, raw.scales);
+}
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> k) {
+// 256 elements from element `from` on, or what is left of them.
+template <bool WIDE, bool BYTES>
+__device__ __forceinline__ void step_block(const Tensor& t, const Step& s, uint32_t key, int64_t from, int lane) {
+    const int64_t left = t.n - from;
+    float p[8], g[8], m[8], v[8];
+    load_values<WIDE>(p, t.param + from, left, lane);
+    if (t.half_grad) load_values<WIDE>(g, static_cast<const __half*>(t.grad) + from, left, lane);
+    else load_values<WIDE>(g, static_cast<const float*>(t.grad) + from, left, lane);
+    if (BYTES && t.scales != nullptr) {
+        uint32_t a[2], b[2];
+        load_bytes<WIDE>(a, static_cast<const uint8_t*>(t.first) + from, left, lane);
+        load_bytes<WIDE>(b, static_cast<const uint8_t*>(t.second) + from, left, lane);
+        step_bytes<WIDE>(t, s, key, from, lane, p, g, a, b, t.scales[from / kBlock]);
+        return;
+    }
+    load_values<WIDE>(m, static_cast<const float*>(t.first) + from, left, lane);
+    load_values<WIDE>(v, static_cast<const float*>(t.second) + from, left, lane);
+    s.moments(g, m, v);
+    store_values<WIDE>(static_cast<float*>(t.first) + from, m, left, lane);
+    store_values<WIDE>(static_cast<float*>(t.second) + from, v, left, lane);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sqrtf(v[e]);
+    s.update(p, m, v);
+    store_values<WIDE>(t.param + from, p, left, lane);
+    if (t.copy != nullptr) store_values<WIDE>(t.copy + from, p, left, lane);
+}
+
+// BYTES: whether a tensor has 8-bit states.  (Without them four blocks fit on an SM: 176 M parameters 720 us, 730 with three.)
+template <int N, bool BYTES>
+__global__ void __launch_bounds__(kThreads, BYTES ? 3 : 4) adamw_kernel(const __grid_constant__ Table<N> k) {
     pdl_prologue();
     int lo = 0, hi = k.count;  // the tensor whose items this block's is one of
     while (hi - lo > 1) {
@@ -289,13 +327,25 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     s.rate = lr * inverse1;
     const uint32_t key = t.scales != nullptr ? mix(mix(mix(n.seed) + static_cast<uint32_t>(step)) + t.number) : 0u;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t base = int64_t(blockIdx.x - t.item) * kItem;
+    int64_t from = int64_t(blockIdx.x - t.item) * (n.rounds * kRound) + warp * kBlock;
+    const int64_t whole = t.n / kBlock * kBlock, end = min(t.n, from - warp * kBlock + n.rounds * kRound);
+    if (BYTES && t.wide && t.scales != nullptr) {  // whole blocks, the next one on its way
+        const int64_t end_whole = min(whole, end);
+        if (from < end_whole) {
+            RawBytes raw;
+            raw.load(t, from, lane);
 #pragma unroll 1
-    for (int r = 0; r < kRounds; ++r) {
-        const int64_t from = base + (r * (kThreads / 32) + warp) * kBlock;
-        if (from >= t.n) return;
-        if (t.wide && t.n - from >= kBlock) step_block<true>(t, s, key, from, lane);
-        else step_block<false>(t, s, key, from, lane);
+            for (; from < end_whole; from += kRound) {
+                const RawBytes now = raw;
+                if (from + kRound < end_whole) raw.load(t, from + kRound, lane);
+                step_bytes(t, s, key, from, lane, now);
+            }
+        }
+    }
+#pragma unroll 1
+    for (; from < end; from += kRound) {
+        if (t.wide && (!BYTES || t.scales == nullptr) && from < whole) step_block<true, false>(t, s, key, from, lane);
+        else step_block<false, BYTES>(t, s, key, from, lane);
     }
 }
 
@@ -330,29 +380,40 @@ void check_numbers(const b200_adamw_args& a) {
 
 // The tensors' checks; what is written lies on nothing else of the call (sorted addresses: a neighbour shows it).
 void check_tensors(const b200_adamw_args& a) {
-    std::vector<Range> ranges;
-    ranges.reserve(static_cast<size_t>(a.count) * 6 + 3);
-    auto add = [&](const b200_tensor& t, bool written) {
+    // Addresses are sorted kind by kind (each kind of a model's mostly lies in order) and then merged.
+    std::vector<Range> kinds[7];
+    auto add = [&](int kind, const b200_tensor& t, bool written) {
         const int64_t bytes = numel_of(t) * static_cast<int64_t>(dtype_size(t.dtype));
-        if (present(t) && bytes != 0) ranges.push_back({static_cast<const char*>(t.data), static_cast<const char*>(t.data) + bytes, written});
+        if (present(t) && bytes != 0) kinds[kind].push_back({static_cast<const char*>(t.data), static_cast<const char*>(t.data) + bytes, written});
+    };
+    for (std::vector<Range>& k : kinds) k.reserve(static_cast<size_t>(a.count) + 3);
+    // A tensor that is one of param's extents and strides, of its type, needs no other check than that of its address.
+    auto alike = [](const b200_tensor& x, const b200_tensor& y) {
+        return x.ndim == y.ndim && x.dtype == y.dtype && std::memcmp(x.dims, y.dims, sizeof(int64_t) * static_cast<size_t>(x.ndim)) == 0 &&
+               std::memcmp(x.strides, y.strides, sizeof(int64_t) * static_cast<size_t>(x.ndim)) == 0 && reinterpret_cast<uintptr_t>(x.data) % 4 == 0;
     };
     for (int64_t i = 0; i < a.count; ++i) {
         const b200_adamw_tensor& t = a.tensors[i];
         auto refuse = [&](int status, const char* why) { fail(status, "adamw: tensor " + std::to_string(i) + ": " + why); };
         check_tensor(t.param, "param");
-        check_tensor(t.grad, "grad");
-        check_tensor(t.first, "first");
-        check_tensor(t.second, "second");
+        if (t.param.dtype != B200_F32) refuse(B200_DTYPE_ERROR, "param is F32");
         const int64_t n = numel_of(t.param);
         const bool bytes = t.first.dtype == B200_I32;
-        if (t.param.dtype != B200_F32) refuse(B200_DTYPE_ERROR, "param is F32");
-        if (!is_float(t.grad.dtype)) refuse(B200_DTYPE_ERROR, "grad is F32 or F16");
+        if (!is_dense(t.param)) refuse(B200_NOT_IMPLEMENTED, "a tensor is not dense");
+        if (!alike(t.grad, t.param)) {
+            check_tensor(t.grad, "grad");
+            if (!is_float(t.grad.dtype)) refuse(B200_DTYPE_ERROR, "grad is F32 or F16");
+            if (t.grad.ndim != t.param.ndim || !same_extents(t.grad, t.param, t.param.ndim)) refuse(B200_SHAPE_ERROR, "grad has not param's extents");
+            if (!is_dense(t.grad)) refuse(B200_NOT_IMPLEMENTED, "a tensor is not dense");
+        }
         if (t.first.dtype != t.second.dtype || (!bytes && t.first.dtype != B200_F32)) refuse(B200_DTYPE_ERROR, "first and second are both F32, or both I32 words of bytes");
-        if (t.grad.ndim != t.param.ndim || !same_extents(t.grad, t.param, t.param.ndim)) refuse(B200_SHAPE_ERROR, "grad has not param's extents");
         for (const b200_tensor* s : {&t.first, &t.second}) {
+            if (alike(*s, t.param)) continue;
+            check_tensor(*s, s == &t.first ? "first" : "second");
             if (bytes ? s->ndim != 1 || s->dims[0] != ceil_div(n, 4) : s->ndim != t.param.ndim || !same_extents(*s, t.param, t.param.ndim)) {
                 refuse(B200_SHAPE_ERROR, "a state has not param's extents, or its number of bytes");
             }
+            if (!is_dense(*s)) refuse(B200_NOT_IMPLEMENTED, "a tensor is not dense");
         }
         if (bytes ? n != 0 && !present(t.scales) : present(t.scales)) refuse(B200_INVALID_ARGUMENT, "scales go with 8-bit states, and only with them");
         if (present(t.scales)) {
@@ -369,21 +430,26 @@ void check_tensors(const b200_adamw_args& a) {
             if (!is_dense(t.copy)) refuse(B200_NOT_IMPLEMENTED, "copy is not dense");
         }
         for (const b200_tensor* s : {&t.param, &t.grad, &t.first, &t.second}) {
-            if (!is_dense(*s)) refuse(B200_NOT_IMPLEMENTED, "a tensor is not dense");
             if (n != 0 && !present(*s)) refuse(B200_INVALID_ARGUMENT, "a tensor has no storage");
         }
         if (!(t.weight_decay >= 0.f) || std::isinf(t.weight_decay) || !std::isfinite(t.lr_scale)) refuse(B200_INVALID_ARGUMENT, "weight_decay or lr_scale is not finite, or weight_decay below 0");
-        add(t.param, true);
-        add(t.grad, false);
-        add(t.first, true);
-        add(t.second, true);
-        if (present(t.scales)) add(t.scales, true);
-        if (present(t.copy)) add(t.copy, true);
+        add(0, t.param, true);
+        add(1, t.grad, false);
+        add(2, t.first, true);
+        add(3, t.second, true);
+        if (present(t.scales)) add(4, t.scales, true);
+        if (present(t.copy)) add(5, t.copy, true);
     }
-    add(a.lr_on_device, false);
-    add(a.step_on_device, false);
-    add(a.scale_on_device, false);
-    std::sort(ranges.begin(), ranges.end());
+    add(6, a.lr_on_device, false);
+    add(6, a.step_on_device, false);
+    add(6, a.scale_on_device, false);
+    std::vector<Range> ranges, merged;
+    for (std::vector<Range>& k : kinds) {
+        if (!std::is_sorted(k.begin(), k.end())) std::sort(k.begin(), k.end());
+        merged.resize(ranges.size() + k.size());
+        std::merge(ranges.begin(), ranges.end(), k.begin(), k.end(), merged.begin());
+        ranges.swap(merged);
+    }
     const char* reach[2] = {nullptr, nullptr};  // the farthest end so far, of what is read and of what is written
     for (const Range& r : ranges) {
         if (r.lo < reach[1] || (r.written && r.lo < reach[0])) fail(B200_INVALID_ARGUMENT, "adamw: a tensor that is written overlaps another");
@@ -391,14 +457,14 @@ void check_tensors(const b200_adamw_args& a) {
     }
 }
 
-template <int N>
+template <int N, bool BYTES>
 void launch_table(b200_ctx* ctx, const Numbers& numbers, const std::vector<Tensor>& tensors, size_t first, size_t count, uint32_t items) {
     static_assert(sizeof(Table<N>) <= 32764, "the launch's parameters");
     Table<N> table;
     table.numbers = numbers;
     table.count = static_cast<int>(count);
     std::copy_n(tensors.begin() + static_cast<std::ptrdiff_t>(first), count, table.t);
-    launch_kernel(ctx, adamw_kernel<N>, dim3(items), dim3(kThreads), 0, table);
+    launch_kernel(ctx, adamw_kernel<N, BYTES>, dim3(items), dim3(kThreads), 0, table);
     check_last_launch("adamw");
     ctx->count_launch();
 }
@@ -441,19 +507,27 @@ void launch_adamw(b200_ctx* ctx, const b200_adamw_args& a) {
     }
     wait_for_tensors(ctx, {&a.lr_on_device, &a.step_on_device, &a.scale_on_device});
     ProfScope scope(ctx, "adamw");
+    // As many rounds to a block as leave two waves of blocks; one where there is little to do.
+    int64_t all = 0;
+    for (const Tensor& t : tensors) all += ceil_div(t.n, kRound);
+    const bool any_bytes = std::any_of(tensors.begin(), tensors.end(), [](const Tensor& t) { return t.scales != nullptr; });
+    k.rounds = static_cast<int>(std::clamp<int64_t>(all / (int64_t(sm_count()) * 6), 1, any_bytes ? kMostRounds : kMostRounds / 2));
     size_t done = 0;
     while (done < tensors.size()) {
         size_t count = 0;
         int64_t items = 0;
         while (done + count < tensors.size() && count < kMostTensors) {
-            const int64_t more = ceil_div(tensors[done + count].n, kItem);
+            const int64_t more = ceil_div(tensors[done + count].n, int64_t(kRound) * k.rounds);
             if (items + more >= (int64_t(1) << 31)) break;
             tensors[done + count].item = static_cast<uint32_t>(items);
             items += more;
             ++count;
         }
         if (count == 0) fail(B200_SHAPE_ERROR, "adamw: a tensor is too large");
-        launch_table<kMostTensors>(ctx, k, tensors, done, count, static_cast<uint32_t>(items));
+        const bool bytes = std::any_of(tensors.begin() + static_cast<std::ptrdiff_t>(done), tensors.begin() + static_cast<std::ptrdiff_t>(done + count), [](const Tensor& t) { return t.scales != nullptr; });
+        auto go = [&](auto launch) { launch(ctx, k, tensors, done, count, static_cast<uint32_t>(items)); };
+        if (count <= kFewTensors) go(bytes ? launch_table<kFewTensors, true> : launch_table<kFewTensors, false>);
+        else go(bytes ? launch_table<kMostTensors, true> : launch_table<kMostTensors, false>);
         done += count;
     }
 }

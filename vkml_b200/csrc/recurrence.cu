@@ -129,15 +129,16 @@ __device__ __forceinline__ float gate_of(float gate, float& input) {
     input = i[0];
     return c[0];
 }
-// What dgate is (h_{t-1} - x) D times, or h_{t-1} D times; and dx is D times.
+// What dgate is (h_{t-1} - x) D times, or h_{t-1} D times; what dx is D times; and a.
 template <int KIND>
-__device__ __forceinline__ void slopes(float c, float& gate, float& input) {
+__device__ __forceinline__ void slopes(float c, float& gate, float& input, float& a) {
     if constexpr (KIND == B200_GATES_SIGMOID) {
         const float s = fabsf(c), r = 1.f - s;
         gate = s * r;
         input = keeps(c) ? s : r;
+        a = keeps(c) ? r : s;
     } else {
-        gate = keeps(c) ? 1.f + c : c;
+        gate = a = keeps(c) ? 1.f + c : c;
         input = 1.f;
     }
 }
@@ -271,8 +272,8 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
             const bool in = t0 + j < n;
             const float D = d[j] + e;
             e = apply(c[j], D, 0.f);
-            float gate, input;
-            slopes<KIND>(c[j], gate, input);
+            float gate, input, a;
+            slopes<KIND>(c[j], gate, input, a);
             if (t0 + j < k.length) {
                 if (k.dx.base != nullptr) *at<T>(k.dx, b, t0 + j, ch) = from_float<T>(in ? input * D : 0.f);
                 if (k.dgate.base != nullptr) *at<G>(k.dgate, b, t0 + j, ch) = from_float<G>(in ? gate * w[j] * D : 0.f);
@@ -551,6 +552,33 @@ struct Steps {
         }
     }
     __device__ __forceinline__ void next() { from += jump; }
+
+    // What a step's channels became, in the place that they came by; and (store) from there to `to`, this lane's first piece of the window: whole pieces of rows.  Pieces
+    // of 4 bytes and less go to memory one by one, at `one`.
+    static constexpr bool kPieced = CHUNK == 16;
+    __device__ __forceinline__ void put(int j, int lane, char* one, const float (&y)[VEC], bool in) const {
+        if constexpr (kPieced) Raw<T, VEC>::store(const_cast<char*>(place) + j * kBytes + lane * VEC * int(sizeof(T)), y);
+        else if (in) Raw<T, VEC>::store(one, y);
+    }
+    __device__ __forceinline__ void store(char* to, int64_t bytes, int rows, int lane) const {
+        if constexpr (kPieced) {
+            __syncwarp();
+            constexpr int kRows = 32 / kPieces;
+            const int row = lane / kPieces;
+            if (lane % kPieces * kCopy >= valid) return;
+            const uint4* mine = reinterpret_cast<const uint4*>(place) + lane;
+            char* p = to;
+#pragma unroll
+            for (int i = 0; i < kSteps / kRows; ++i, p += bytes * kRows) {
+                if (i * kRows + row < rows) *reinterpret_cast<uint4*>(p) = mine[i * 32];
+            }
+        }
+    }
+    // This lane's first piece of a result's window, or (other pieces) its channels at the window's first step.
+    static __device__ __forceinline__ char* first_piece(char* strip, int64_t bytes, uint32_t t, int lane) {
+        if constexpr (kPieced) return strip + (t + lane / kPieces) * bytes + lane % kPieces * kCopy;
+        else return strip + t * bytes + lane * VEC * int(sizeof(T));
+    }
     // The window that begins at `base` lies at `at`.
     __device__ __forceinline__ void look(const char* at, const char* base) {
         place = at;
@@ -596,7 +624,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     Y gate;
     x.begin(at.template strip<T>(k.x), k.x.step, at.first(), span, at.valid(k.width, sizeof(T)), at.lane);
     gate.begin(at.template strip<G>(k.gate), k.gate.step, at.first(), span, at.valid(k.width, sizeof(G)), at.lane);
-    char* out = at.template base<T>(k.out) + at.first() * k.out.step;
+    char* out = X::first_piece(const_cast<char*>(at.template strip<T>(k.out)), k.out.step, at.first(), at.lane);
     const int64_t out_jump = span * k.out.step;
     const char* x_at = at.template strip<T>(k.x) + at.first() * k.x.step;  // (of the window that is computed: X::kAround asks)
     const char* gate_at = at.template strip<G>(k.gate) + at.first() * k.gate.step;
@@ -628,7 +656,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         read += apart;
         if (read == end) read = places;
         load();  // (where the window before lay)
-        float c[kSteps][VEC], b[kSteps][VEC];
+        float a[kSteps][VEC], b[kSteps][VEC];
         Run<VEC> own;
         own.begin();
         float gate_sum[VEC];
@@ -638,18 +666,18 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         auto take = [&](auto whole) {
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
-                float xs[VEC], gs[VEC], a[VEC], d[VEC], input[VEC];
+                float xs[VEC], gs[VEC], c[VEC], d[VEC], input[VEC];
                 x.get(j, at.lane).get(xs);
                 gate.get(j, at.lane).get(gs);
                 if (!whole.value && j >= left) {  // the state stays
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
                 }
-                gates_of<KIND>(gs, c[j], a, d, input);
+                gates_of<KIND>(gs, c, a[j], d, input);
                 mul_v(b[j], input, xs);
-                if constexpr (KIND == B200_GATES_SIGMOID) own.decays(a, d);
+                if constexpr (KIND == B200_GATES_SIGMOID) own.decays(a[j], d);
                 else add_v(gate_sum, gate_sum, gs);
-                own.adds(a, b[j]);
+                own.adds(a[j], b[j]);
             }
         };
         if (left == kSteps) take(std::true_type{});
@@ -660,22 +688,23 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         }
         float h[VEC];
         join<VEC, false>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, h);
-        if (!at.in || t >= length) continue;
-        if (k.states != nullptr) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
+        if (t >= length) continue;
+        if (k.states != nullptr && at.in) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
         auto put = [&](auto whole) {
             char* p = out;
 #pragma unroll
             for (int j = 0; j < kSteps; ++j, p += k.out.step) {
-                apply_v(h, c[j], b[j]);
+                fma_v(h, a[j], h, b[j]);  // (a's rounding counts within these steps only)
                 float y[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) y[e] = whole.value || j < left ? h[e] : 0.f;
-                if (whole.value || j < rows) Raw<T, VEC>::store(p, y);
+                x.put(j, at.lane, p, y, at.in && (whole.value || j < rows));
             }
         };
         if (left == kSteps) put(std::true_type{});
         else put(std::false_type{});
+        x.store(out, k.out.step, rows, at.lane);
     }
     if (k.final_state.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
 #pragma unroll
@@ -704,10 +733,9 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     x.begin(at.template strip<T>(k.x), k.x.step, t, -int64_t(span), at.valid(k.width, sizeof(T)), at.lane);
     gate.begin(at.template strip<G>(k.gate), k.gate.step, t, -int64_t(span), at.valid(k.width, sizeof(G)), at.lane);
     if (with_dout) dout.begin(at.template strip<T>(k.dout), k.dout.step, t, -int64_t(span), at.valid(k.width, sizeof(T)), at.lane);
-    char *dx = at.template base<T>(k.dx), *dgate = at.template base<G>(k.dgate);
-    const bool with_dx = dx != nullptr, with_dgate = dgate != nullptr;
-    if (with_dx) dx += t * k.dx.step;
-    if (with_dgate) dgate += t * k.dgate.step;
+    const bool with_dx = k.dx.base != nullptr, with_dgate = k.dgate.base != nullptr;
+    char* dx = with_dx ? X::first_piece(const_cast<char*>(at.template strip<T>(k.dx)), k.dx.step, t, at.lane) : nullptr;
+    char* dgate = with_dgate ? Y::first_piece(const_cast<char*>(at.template strip<G>(k.dgate)), k.dgate.step, t, at.lane) : nullptr;
     const char *x_at = at.template strip<T>(k.x) + t * k.x.step, *gate_at = at.template strip<G>(k.gate) + t * k.gate.step, *dout_at = nullptr;
     if (with_dout) dout_at = at.template strip<T>(k.dout) + t * k.dout.step;
     char *const places = ring + at.warp * kBytes, *const end = places + kStages * at.warps * kBytes, *read = places, *write = places;
@@ -781,30 +809,25 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
                 mul_v(b, input, xs);
                 own.decays(a, d);
                 fma_v(own.sum, own.a, ds, own.sum);  // what the steps' gradients make of the state in front of them: each times the a's up to it
-                apply_v(h, c[j], b);
+                fma_v(h, a, h, b);  // (a's rounding counts within these steps only, here and below)
             }
         };
         if (left == kSteps) take(std::true_type{});
         else take(std::false_type{});
-        float later[VEC], zero[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
+        float later[VEC];
         join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, later);
-        if (at.in && t < length) {
+        if (t < length) {
             const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
             auto put = [&](auto whole) {
                 char *to_x = dx + (kSteps - 1) * k.dx.step, *to_gate = dgate + (kSteps - 1) * k.dgate.step;
 #pragma unroll
                 for (int j = kSteps - 1; j >= 0; --j, to_x -= k.dx.step, to_gate -= k.dgate.step) {
-                    float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC];
+                    float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC], a[VEC];
                     gradient(j, D);
                     add_v(D, D, later);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        later[e] = D[e];
-                        slopes<KIND>(c[j][e], slope[e], input[e]);
-                    }
-                    apply_v(later, c[j], zero);
+                    for (int e = 0; e < VEC; ++e) slopes<KIND>(c[j][e], slope[e], input[e], a[e]);
+                    mul_v(later, a, D);
                     mul_v(px, input, D);
                     mul_v(pg, slope, u[j]);
                     mul_v(pg, pg, D);
@@ -812,14 +835,15 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
                     for (int e = 0; e < VEC; ++e) {
                         if (!whole.value && j >= left) px[e] = pg[e] = 0.f;
                     }
-                    if (whole.value || j < rows) {
-                        if (with_dx) Raw<T, VEC>::store(to_x, px);
-                        if (with_dgate) Raw<G, VEC>::store(to_gate, pg);
-                    }
+                    const bool in = at.in && (whole.value || j < rows);
+                    if (with_dx) x.put(j, at.lane, to_x, px, in);
+                    if (with_dgate) gate.put(j, at.lane, to_gate, pg, in);
                 }
             };
             if (left == kSteps) put(std::true_type{});
             else put(std::false_type{});
+            if (with_dx) x.store(dx, k.dx.step, rows, at.lane);
+            if (with_dgate) gate.store(dgate, k.dgate.step, rows, at.lane);
         }
         dx -= int64_t(span) * k.dx.step, dgate -= int64_t(span) * k.dgate.step;
     }
@@ -966,12 +990,11 @@ struct Walk {
 struct Typed {
     Stream s;
     int dtype;
-    bool read;
 };
 Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams) {
     Walk w;
     if (s.length <= kSteps) return w;
-    // Copies of 16 or of 4 bytes where every row that is read lies on so many; two channels to a lane where every row has them side by side on an address for both.
+    // Copies of 16 or of 4 bytes where every row lies on so many; two channels to a lane where every row has them side by side on an address for both.
     bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
     int chunk = 16;
     for (const Typed& t : streams) {
@@ -980,8 +1003,8 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
         auto on = [&](int64_t bytes) { return reinterpret_cast<uintptr_t>(t.s.base) % static_cast<uintptr_t>(bytes) == 0 && t.s.step % bytes == 0 && t.s.batch % bytes == 0; };
         halves |= t.dtype == B200_F16;
         pairs = pairs && on(2 * size);
-        if (t.read && chunk == 16 && !(on(16) && s.width * size % 16 == 0)) chunk = 4;
-        if (t.read && chunk == 4 && !(on(4) && s.width * size % 4 == 0)) chunk = 2;
+        if (chunk == 16 && !(on(16) && s.width * size % 16 == 0)) chunk = 4;
+        if (chunk == 4 && !(on(4) && s.width * size % 4 == 0)) chunk = 2;
     }
     w.vec = pairs && halves ? 2 : 1;
     w.chunk = halves && !pairs ? 2 : chunk;
@@ -1018,7 +1041,7 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
     k.initial = end_of(a.initial);
     k.final_state = end_of(a.final_state);
     ProfScope scope(ctx, "gated_recurrence");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype, true}, {k.gate, a.gate.dtype, true}, {k.out, a.out.dtype, false}});
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}});
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
@@ -1048,7 +1071,7 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
     k.initial = end_of(a.initial_grad);
     k.final_state = end_of(a.final_grad);
     ProfScope scope(ctx, "gated_recurrence_backward");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype, true}, {k.gate, a.gate.dtype, true}, {k.dout, a.x.dtype, true}, {k.dx, a.x.dtype, false}, {k.dgate, a.gate.dtype, false}});
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}});
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
