@@ -423,7 +423,7 @@ int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
 #define B200_GATES_EXP 1
 #define B200_RECURRENCE_CHUNK 16
 typedef struct b200_recurrence_args {
-    b200_tensor x;         /* rows [L, D] or [B, L, D]: the axis in front of the rows' own is time */
+    b200_tensor x;         /* rows [L, D] or [B, L, D], D below 2^30: the axis in front of the rows' own is time */
     b200_tensor gate;      /* x's extents.  (x, gate): (F32, F32), (F16, F16) or (F16, F32) */
     b200_tensor initial;   /* h in front of the first step, rows [D] or [B, D], F32; absent: zeros */
     b200_tensor lengths;   /* steps of each sequence: [B], or one without an axis; I32 or I64, any stride; absent: L.  Steps behind a sequence's end are

@@ -129,6 +129,38 @@ def test_a_step(backend, bits, grad, copy):
         compare(t, got, i, 1e-2, 7, scale=0.5, seed=99)
 
 
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e6])
+def test_bytes_are_what_the_formulas_give_in_32_bits(backend, size):
+    """Operation by operation in F32, each rounded by itself: the same bytes and scales, not only near ones.  (Sizes of the second form of the scaling too.)"""
+    rng = np.random.default_rng(12)
+    t = tensor_of(rng, (70, 1001), F32, 8)
+    t["grad"] *= F32(size)
+    t["scales"] *= F32(size)
+    got = steps(backend, [t], lr=0.01, step=4, seed=77, grad_scale=0.75)[0]
+    n, f = t["param"].size, F32
+    values = byte_values().astype(f)
+    of = lambda k, i: values[t[k].view(np.uint8)[:n]] * np.repeat(t["scales"][:, i], 256)[:n]  # noqa: E731
+    g = t["grad"].reshape(-1) * f(0.75)
+    m, r = of("first", 0), of("second", 1)
+    m = m * f(0.9) + g * f(1 - 0.9)
+    r = np.sqrt(r * r * f(0.999) + g * g * f(1 - 0.999))
+    bits = random_bits(77, 4, 0, n).astype(np.uint32)
+    for k, i, x, draw in (("first", 0, m, bits & 0xFFFF), ("second", 1, r, bits >> 16)):
+        assert x.dtype == f
+        most = np.pad(np.abs(x), (0, -n % 256)).reshape(-1, 256).max(1)
+        assert np.array_equal(got["scales"][:, i], most * f(1 / 448))
+        y = np.abs(x) * np.repeat(f(1) / most * f(448), 256)[:n]
+        whole = (y * f(2.0 ** -120)).view(np.uint32)
+        code = np.minimum((whole + (draw << 4 | 8)) >> 20, 126)
+        if k == "second":
+            code = np.where(x > 0, np.maximum(code, 1), code)
+        else:
+            code = np.where(np.signbit(x), code + 128, code)
+        wrong = got[k].view(np.uint8)[:n] != code
+        # (a value below 2^-6 of the scale's unit is rounded twice here, to a float and to a subnormal one, and once by the kernel where one product scales it)
+        assert wrong.sum() <= (0 if size > 1e5 else 2), (k, wrong.sum())
+
+
 @pytest.mark.parametrize("step,beta1,beta2,eps", [(1, 0.9, 0.999, 1e-8), (2, 0.0, 0.95, 1e-6), (100000, 0.9, 0.999, 1e-3), (1 << 40, 0.99, 0.0, 1e-8), (3, 0.9, 0.9999999, 1e-12)])
 @pytest.mark.parametrize("bits", [32, 8])
 def test_steps_and_betas(backend, step, beta1, beta2, eps, bits):

@@ -34,11 +34,6 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
 // A step's decay: -d where a = 1 - d is above a half (never 0: the sign tells), else a.
 constexpr float kHold = -0x1p-126f;  // h stays
 __device__ __forceinline__ bool keeps(float c) { return c < 0.f; }
-__device__ __forceinline__ float apply(float c, float h, float b) {
-    const float t = fmaf(c, h, b);
-    return keeps(c) ? h + t : t;
-}
-
 // Arithmetic on a lane's channels, two to an instruction.
 template <int V>
 __device__ __forceinline__ void fma_v(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
@@ -122,13 +117,6 @@ __device__ __forceinline__ void gates_of(const float (&gate)[V], float (&c)[V], 
         }
     }
 }
-template <int KIND>
-__device__ __forceinline__ float gate_of(float gate, float& input) {
-    float g[1] = {gate}, c[1], a[1], d[1], i[1];
-    gates_of<KIND>(g, c, a, d, i);
-    input = i[0];
-    return c[0];
-}
 // What dgate is (h_{t-1} - x) D times, or h_{t-1} D times; what dx is D times; and a.
 template <int KIND>
 __device__ __forceinline__ void slopes(float c, float& gate, float& input, float& a) {
@@ -188,11 +176,6 @@ struct Args {
     uint32_t* status;
 };
 
-template <typename T>
-__device__ __forceinline__ T* at(const Stream& s, int b, int64_t t, int ch) {
-    return reinterpret_cast<T*>(s.base + b * s.batch + t * s.step) + ch;
-}
-
 // Steps of sequence b.
 __device__ __forceinline__ int64_t steps_of(const Args& k, int b) {
     if (k.lengths == nullptr) return k.length;
@@ -200,98 +183,6 @@ __device__ __forceinline__ int64_t steps_of(const Args& k, int b) {
     if (n < 0 || n > k.length) atomicOr(k.status, kStatusIndexOutOfRange);
     return n < 0 ? 0 : n > k.length ? k.length : n;
 }
-
-// ---- a thread to a channel, step by step ------------------------------------
-
-constexpr int kThreads = 128;
-
-template <typename T, typename G, int KIND>
-__global__ void __launch_bounds__(kThreads) serial_kernel(const Args k) {
-    pdl_prologue();
-    const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= int64_t(k.batch) * k.width) return;
-    const int b = static_cast<int>(i / k.width), ch = static_cast<int>(i % k.width);
-    const int64_t n = steps_of(k, b);
-    float h = k.initial.base != nullptr ? reinterpret_cast<const float*>(k.initial.base + b * k.initial.step)[ch] : 0.f;
-    float* state = k.states != nullptr ? k.states + int64_t(b) * k.chunks * k.width + ch : nullptr;
-    for (int64_t t0 = 0; t0 < k.length; t0 += kSteps) {
-        if (state != nullptr) {
-            *state = h;
-            state += k.width;
-        }
-        float x[kSteps], g[kSteps];
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const bool in = t0 + j < n;
-            x[j] = in ? to_float(*at<const T>(k.x, b, t0 + j, ch)) : 0.f;
-            g[j] = in ? to_float(*at<const G>(k.gate, b, t0 + j, ch)) : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            float input;
-            const float c = gate_of<KIND>(g[j], input);
-            const bool in = t0 + j < n;
-            if (in) h = apply(c, h, input * x[j]);
-            if (t0 + j < k.length) *at<T>(k.out, b, t0 + j, ch) = from_float<T>(in ? h : 0.f);
-        }
-    }
-    if (k.final_state.base != nullptr) reinterpret_cast<float*>(k.final_state.base + b * k.final_state.step)[ch] = h;
-}
-
-template <typename T, typename G, int KIND>
-__global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k) {
-    pdl_prologue();
-    const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= int64_t(k.batch) * k.width) return;
-    const int b = static_cast<int>(i / k.width), ch = static_cast<int>(i % k.width);
-    const int64_t n = steps_of(k, b);
-    float e = k.final_state.base != nullptr ? reinterpret_cast<const float*>(k.final_state.base + b * k.final_state.step)[ch] : 0.f;
-    for (int chunk = k.chunks - 1; chunk >= 0; --chunk) {
-        const int64_t t0 = int64_t(chunk) * kSteps;
-        float h = k.states[(int64_t(b) * k.chunks + chunk) * k.width + ch];
-        float c[kSteps], w[kSteps], d[kSteps];
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const bool in = t0 + j < n;
-            w[j] = in ? to_float(*at<const T>(k.x, b, t0 + j, ch)) : 0.f;
-            c[j] = in ? to_float(*at<const G>(k.gate, b, t0 + j, ch)) : 0.f;
-            d[j] = in && k.dout.base != nullptr ? to_float(*at<const T>(k.dout, b, t0 + j, ch)) : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const bool in = t0 + j < n;
-            const float x = w[j];
-            float input;
-            const float decay = gate_of<KIND>(c[j], input);
-            c[j] = in ? decay : kHold;
-            w[j] = KIND == B200_GATES_SIGMOID ? h - x : h;
-            if (in) h = apply(decay, h, input * x);
-        }
-#pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
-            const bool in = t0 + j < n;
-            const float D = d[j] + e;
-            e = apply(c[j], D, 0.f);
-            float gate, input, a;
-            slopes<KIND>(c[j], gate, input, a);
-            if (t0 + j < k.length) {
-                if (k.dx.base != nullptr) *at<T>(k.dx, b, t0 + j, ch) = from_float<T>(in ? input * D : 0.f);
-                if (k.dgate.base != nullptr) *at<G>(k.dgate, b, t0 + j, ch) = from_float<G>(in ? gate * w[j] * D : 0.f);
-            }
-        }
-    }
-    if (k.initial.base != nullptr) reinterpret_cast<float*>(k.initial.base + b * k.initial.step)[ch] = e;
-}
-
-// ---- blocks that walk along a sequence --------------------------------------
-//
-// A block, or a cluster of blocks, has 32 lanes' channels of a sequence and walks along it window by window; a warp has 16 steps of a window.  A thread computes what
-// its steps do to a state that comes in (a decay and a sum: a step like any other), the warps tell each other by shared memory, the cluster's blocks by each
-// other's, and every thread goes through its steps again from the state that does come in.  All of it stays in registers: gates and inputs are read once, and the
-// next window's are under way while this one is computed.
-
-constexpr int kMostWarps = 8;
-constexpr int kMostCluster = 8;
 
 // VEC neighbouring channels of a lane as they lie in memory, and as floats.
 template <typename T, int VEC>
@@ -321,6 +212,145 @@ struct Raw<float, 2> {
     __device__ __forceinline__ void get(float (&x)[2]) const { x[0] = a.x, x[1] = a.y; }
     static __device__ __forceinline__ void store(char* p, const float (&x)[2]) { *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]); }
 };
+
+template <int VEC>
+__device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, int b, int ch, bool in) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] = end.base != nullptr && in ? reinterpret_cast<const float*>(end.base + b * end.step)[ch + e] : 0.f;
+}
+template <int VEC>
+__device__ __forceinline__ void store_end(const RowsArg& end, int b, int ch, const float (&h)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(end.base + b * end.step)[ch + e] = h[e];
+}
+
+// ---- a thread to its channels, step by step ----------------------------------
+//
+// Few steps: the next token of many sequences, say, where the launch is what takes the time.  Every step is exact to its own rounding, so that a state that is carried on
+// a token at a time drifts no more than one that a long call carries.
+
+constexpr int kThreads = 128;
+
+// The steps of one sequence and VEC channels, N at a time.
+template <typename T, typename G, int KIND, int VEC, int N>
+__global__ void __launch_bounds__(kThreads) serial_kernel(const Args k) {
+    pdl_prologue();
+    const int ch = (blockIdx.x * kThreads + threadIdx.x) * VEC;
+    if (ch >= k.width) return;
+    const int length = static_cast<int>(k.length);
+    for (int b = blockIdx.y; b < k.batch; b += gridDim.y) {
+        const int n = static_cast<int>(steps_of(k, b));
+        const char *x = k.x.base + b * k.x.batch + ch * int64_t(sizeof(T)), *gate = k.gate.base + b * k.gate.batch + ch * int64_t(sizeof(G));
+        char* out = k.out.base + b * k.out.batch + ch * int64_t(sizeof(T));
+        float* state = k.states != nullptr ? k.states + int64_t(b) * k.chunks * k.width + ch : nullptr;
+        float h[VEC];
+        load_end<VEC>(h, k.initial, b, ch, true);
+        for (int t = 0; t < length; t += N) {
+            if (state != nullptr && t % kSteps == 0) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) state[e] = h[e];
+                state += k.width;
+            }
+            Raw<T, VEC> rx[N];
+            Raw<G, VEC> rg[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                rx[j].clear(), rg[j].clear();
+                if (t + j < n) rx[j].load(x + (t + j) * k.x.step), rg[j].load(gate + (t + j) * k.gate.step);
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (t + j >= length) break;
+                float y[VEC] = {};
+                if (t + j < n) {
+                    float xs[VEC], gs[VEC], c[VEC], a[VEC], d[VEC], input[VEC], add[VEC];
+                    rx[j].get(xs);
+                    rg[j].get(gs);
+                    gates_of<KIND>(gs, c, a, d, input);
+                    mul_v(add, input, xs);
+                    apply_v(h, c, add);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) y[e] = h[e];
+                }
+                Raw<T, VEC>::store(out + (t + j) * k.out.step, y);
+            }
+        }
+        if (k.final_state.base != nullptr) store_end<VEC>(k.final_state, b, ch, h);
+    }
+}
+
+// One chunk of steps at most.
+template <typename T, typename G, int KIND, int VEC, int N>
+__global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k) {
+    pdl_prologue();
+    const int ch = (blockIdx.x * kThreads + threadIdx.x) * VEC;
+    if (ch >= k.width) return;
+    const int length = static_cast<int>(k.length);
+    for (int b = blockIdx.y; b < k.batch; b += gridDim.y) {
+        const int n = static_cast<int>(steps_of(k, b));
+        const char *x = k.x.base + b * k.x.batch + ch * int64_t(sizeof(T)), *gate = k.gate.base + b * k.gate.batch + ch * int64_t(sizeof(G));
+        const char* dout = k.dout.base != nullptr ? k.dout.base + b * k.dout.batch + ch * int64_t(sizeof(T)) : nullptr;
+        char* dx = k.dx.base != nullptr ? k.dx.base + b * k.dx.batch + ch * int64_t(sizeof(T)) : nullptr;
+        char* dgate = k.dgate.base != nullptr ? k.dgate.base + b * k.dgate.batch + ch * int64_t(sizeof(G)) : nullptr;
+        float later[VEC], h[VEC];
+        load_end<VEC>(later, k.final_state, b, ch, true);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[e] = length > 0 ? k.states[int64_t(b) * k.width + ch + e] : 0.f;
+        Raw<T, VEC> rx[N], rd[N];
+        Raw<G, VEC> rg[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            rx[j].clear(), rg[j].clear(), rd[j].clear();
+            if (j < n) {
+                rx[j].load(x + j * k.x.step), rg[j].load(gate + j * k.gate.step);
+                if (dout != nullptr) rd[j].load(dout + j * k.dout.step);
+            }
+        }
+        float c[N][VEC], u[N][VEC];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float xs[VEC], gs[VEC], a[VEC], d[VEC], input[VEC], add[VEC];
+            rx[j].get(xs);
+            rg[j].get(gs);
+            gates_of<KIND>(gs, c[j], a, d, input);
+            mul_v(add, input, xs);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (j >= n) c[j][e] = kHold, add[e] = 0.f;
+                u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
+            }
+            apply_v(h, c[j], add);
+        }
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j) {
+            if (j >= length) continue;
+            float D[VEC], px[VEC] = {}, pg[VEC] = {}, zero[VEC] = {};
+            rd[j].get(D);
+            add_v(D, D, later);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                later[e] = D[e];
+                float slope, input, a;
+                slopes<KIND>(c[j][e], slope, input, a);
+                if (j < n) px[e] = input * D[e], pg[e] = slope * u[j][e] * D[e];
+            }
+            apply_v(later, c[j], zero);
+            if (dx != nullptr) Raw<T, VEC>::store(dx + j * k.dx.step, px);
+            if (dgate != nullptr) Raw<G, VEC>::store(dgate + j * k.dgate.step, pg);
+        }
+        if (k.initial.base != nullptr) store_end<VEC>(k.initial, b, ch, later);
+    }
+}
+
+// ---- blocks that walk along a sequence --------------------------------------
+//
+// A block, or a cluster of blocks, has 32 lanes' channels of a sequence and walks along it window by window; a warp has 16 steps of a window.  A thread computes what
+// its steps do to a state that comes in (a decay and a sum: a step like any other), the warps tell each other by shared memory, the cluster's blocks by each
+// other's, and every thread goes through its steps again from the state that does come in.  All of it stays in registers: gates and inputs are read once, and the
+// next window's are under way while this one is computed.
+
+constexpr int kMostWarps = 8;
+constexpr int kMostCluster = 8;
 
 // What the segments of a block, and the blocks of a cluster (as a decay and a sum), do to a state.  Two of the latter: a window's are read while the next one's are
 // written.  (A block that is told of the window after next has told the next one itself, behind its reading of this one.)
@@ -602,12 +632,6 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int PENDING>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
-template <int VEC>
-__device__ __forceinline__ void load_end(float (&h)[VEC], const RowsArg& end, int b, int ch, bool in) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) h[e] = end.base != nullptr && in ? reinterpret_cast<const float*>(end.base + b * end.step)[ch + e] : 0.f;
-}
-
 template <typename T, typename G, int KIND, int VEC, int CHUNK>
 __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, VEC, CHUNK, false>)) walk_kernel(const Args k, uint32_t strips, uint32_t cluster) {
     constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>, kStages = stages_of(kBytes);
@@ -706,10 +730,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         else put(std::false_type{});
         x.store(out, k.out.step, rows, at.lane);
     }
-    if (k.final_state.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(k.final_state.base + at.b * k.final_state.step)[at.ch + e] = carry[e];
-    }
+    if (k.final_state.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) store_end<VEC>(k.final_state, at.b, at.ch, carry);
     if (cluster > 1) end_cluster();
 }
 
@@ -847,10 +868,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         }
         dx -= int64_t(span) * k.dx.step, dgate -= int64_t(span) * k.dgate.step;
     }
-    if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) reinterpret_cast<float*>(k.initial.base + at.b * k.initial.step)[at.ch + e] = carry[e];
-    }
+    if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) store_end<VEC>(k.initial, at.b, at.ch, carry);
     if (cluster > 1) end_cluster();
 }
 
@@ -879,7 +897,7 @@ Shape check_streams(const b200_tensor& x, const b200_tensor& gate, const b200_te
     s.length = x.dims[s.axes - 1];
     s.batch = x.ndim == 3 ? x.dims[0] : 1;
     s.chunks = ceil_div(s.length, kSteps);
-    if (s.width >= (int64_t(1) << 31) || s.batch >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "x: 2^31 or more channels or sequences");
+    if (s.width >= (int64_t(1) << 30) || s.batch >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "x: 2^30 or more channels, or 2^31 or more sequences");
     if (present(lengths)) {
         check_tensor(lengths, "lengths");
         if (!is_index(lengths.dtype)) fail(B200_DTYPE_ERROR, "lengths are I32 or I64");
@@ -993,7 +1011,6 @@ struct Typed {
 };
 Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams) {
     Walk w;
-    if (s.length <= kSteps) return w;
     // Copies of 16 or of 4 bytes where every row lies on so many; two channels to a lane where every row has them side by side on an address for both.
     bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
     int chunk = 16;
@@ -1008,6 +1025,7 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
     }
     w.vec = pairs && halves ? 2 : 1;
     w.chunk = halves && !pairs ? 2 : chunk;
+    if (s.length <= kSteps) return w;
     w.strips = ceil_div(s.width, 32 * w.vec);
     w.warps = static_cast<int>(std::min<int64_t>(kMostWarps, ceil_div(s.length, kSteps)));
     while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
@@ -1047,7 +1065,11 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
         using G = decltype(g);
         constexpr int KIND = decltype(kind)::value;
         if (w.warps == 0) {
-            launch_kernel(ctx, serial_kernel<T, G, KIND>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
+            auto go = [&](auto kernel, int vec) {
+                launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(ceil_div(s.width, kThreads * vec)), static_cast<unsigned>(std::min<int64_t>(s.batch, 65535))), dim3(kThreads), 0, k);
+            };
+            if (w.vec == 1) go(s.length <= 1 ? serial_kernel<T, G, KIND, 1, 1> : serial_kernel<T, G, KIND, 1, kSteps>, 1);
+            else go(s.length <= 1 ? serial_kernel<T, G, KIND, 2, 1> : serial_kernel<T, G, KIND, 2, kSteps>, 2);
         } else {
             by_walk<T>(w, [&](auto vec, auto chunk) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
@@ -1077,7 +1099,11 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
         using G = decltype(g);
         constexpr int KIND = decltype(kind)::value;
         if (w.warps == 0) {
-            launch_kernel(ctx, serial_backward_kernel<T, G, KIND>, dim3(static_cast<unsigned>(ceil_div(s.batch * s.width, kThreads))), dim3(kThreads), 0, k);
+            auto go = [&](auto kernel, int vec) {
+                launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(ceil_div(s.width, kThreads * vec)), static_cast<unsigned>(std::min<int64_t>(s.batch, 65535))), dim3(kThreads), 0, k);
+            };
+            if (w.vec == 1) go(s.length <= 1 ? serial_backward_kernel<T, G, KIND, 1, 1> : serial_backward_kernel<T, G, KIND, 1, kSteps>, 1);
+            else go(s.length <= 1 ? serial_backward_kernel<T, G, KIND, 2, 1> : serial_backward_kernel<T, G, KIND, 2, kSteps>, 2);
         } else {
             by_walk<T>(w, [&](auto vec, auto chunk) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
