@@ -68,9 +68,14 @@ __device__ __forceinline__ void gates_of(const float (&gate)[V], float (&c)[V], 
         float z[V], one[V], tiny[V], least[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            asm("min.NaN.f32 %0, %1, %2;" : "=f"(z[e]) : "f"(gate[e] * -kLog2e), "f"(126.f));
+            one[e] = -kLog2e, tiny[e] = 0x1p-126f, least[e] = -0x1p-126f;
+        }
+        mul_v(z, gate, one);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            asm("min.NaN.f32 %0, %1, %2;" : "=f"(z[e]) : "f"(z[e]), "f"(126.f));
             z[e] = fast_exp2(z[e]);
-            one[e] = 1.f, tiny[e] = 0x1p-126f, least[e] = -0x1p-126f;
+            one[e] = 1.f;
         }
         add_v(one, one, z);
 #pragma unroll
@@ -140,24 +145,20 @@ struct Run {
 #pragma unroll
         for (int e = 0; e < V; ++e) a[e] = 1.f, d[e] = 0.f, sum[e] = 0.f;
     }
-    // A step, or another run, behind this one.  (a's rounding counts within the run only.)
+    // A step behind this one.  (a's rounding counts within the run only.)
     __device__ __forceinline__ void decays(const float (&a1)[V], const float (&d1)[V]) {
         mul_v(a, a, a1);
         fma_v(d, a1, d, d1);
     }
     __device__ __forceinline__ void adds(const float (&a1)[V], const float (&b)[V]) { fma_v(sum, a1, sum, b); }
-    __device__ __forceinline__ void then(const Run& r) {
-        adds(r.a, r.sum);
-        decays(r.a, r.d);
-    }
     __device__ __forceinline__ float decay(int e) const { return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : a[e]; }
-    __device__ __forceinline__ void apply_to(float (&h)[V]) const {
-        float c[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) c[e] = decay(e);
-        apply_v(h, c, sum);
-    }
 };
+// The decay of two runs, one behind the other.
+__device__ __forceinline__ float both(float c, float d) {
+    const float less = fmaf(c, d, c) + d;
+    const float product = (keeps(c) ? 1.f + c : c) * (keeps(d) ? 1.f + d : d);
+    return keeps(c) && keeps(d) ? (less > -0.5f ? fminf(less, kHold) : 1.f + less) : product;
+}
 
 struct Stream {
     char* base;
@@ -352,32 +353,32 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
 constexpr int kMostWarps = 8;
 constexpr int kMostCluster = 8;
 
-// What the segments of a block, and the blocks of a cluster (as a decay and a sum), do to a state.  Two of the latter: a window's are read while the next one's are
-// written.  (A block that is told of the window after next has told the next one itself, behind its reading of this one.)
+// What the segments of a block, and the blocks of a cluster, do to a state: a decay and a sum, for every channel; and the state in front of the window.  Two of each: a
+// window's are read while the next one's are written.  (A block that is told of the window after next has told the next one itself, behind its reading of
+// this one.)
 template <int VEC>
 struct Told {
-    float segments[kMostWarps][3][32 * VEC];
+    float segments[2][kMostWarps][2][32 * VEC];
     float blocks[2][kMostCluster][2][32 * VEC];
+    float front[2][32 * VEC];
     uint64_t bars[2];  // count the bytes that the cluster's blocks tell this one
     int given_up;
 };
 template <int VEC>
-__device__ __forceinline__ Run<VEC> read_run(const float (&from)[3][32 * VEC], int lane) {
-    Run<VEC> r;
-    Raw<float, VEC> x;
-    x.load(reinterpret_cast<const char*>(&from[0][lane * VEC]));
-    x.get(r.a);
-    x.load(reinterpret_cast<const char*>(&from[1][lane * VEC]));
-    x.get(r.d);
-    x.load(reinterpret_cast<const char*>(&from[2][lane * VEC]));
-    x.get(r.sum);
-    return r;
+__device__ __forceinline__ void get_row(float (&x)[VEC], const float* from, int lane) {
+    Raw<float, VEC> r;
+    r.load(reinterpret_cast<const char*>(from + lane * VEC));
+    r.get(x);
 }
 template <int VEC>
-__device__ __forceinline__ void write_run(float (&to)[3][32 * VEC], int lane, const Run<VEC>& r) {
-    Raw<float, VEC>::store(reinterpret_cast<char*>(&to[0][lane * VEC]), r.a);
-    Raw<float, VEC>::store(reinterpret_cast<char*>(&to[1][lane * VEC]), r.d);
-    Raw<float, VEC>::store(reinterpret_cast<char*>(&to[2][lane * VEC]), r.sum);
+__device__ __forceinline__ void put_row(float* to, int lane, const float (&x)[VEC]) { Raw<float, VEC>::store(reinterpret_cast<char*>(to + lane * VEC), x); }
+// h behind a segment or a block.
+template <int VEC>
+__device__ __forceinline__ void pass(float (&h)[VEC], const float (&run)[2][32 * VEC], int lane) {
+    float c[VEC], sum[VEC];
+    get_row<VEC>(c, run[0], lane);
+    get_row<VEC>(sum, run[1], lane);
+    apply_v(h, c, sum);
 }
 
 // Stores to another block of the cluster that its barrier counts.  (A cluster barrier would order them too, but waits for every store of the block before it.)
@@ -431,58 +432,57 @@ __device__ __forceinline__ void end_cluster() {
     asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
-// The state that comes into this warp's steps, from `carry` in front of the window (which becomes that behind it), by what every segment does.  Segments
-// come one after another, in the order of their warps and blocks, or (BACK) the other way round.  `window` counts from 0.
+// The state that comes into this warp's steps.  Segments come one after another, in the order of their warps and blocks, or (BACK) the other way round.  `window` counts from 0.
+// In front of window 0 the first warp has put the state to told.front[0]; behind the last one the last warp's `next` is the state there (of a cluster: everyone's).
 template <int VEC, bool BACK>
-__device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<VEC>& own,
-                                     float (&carry)[VEC], float (&in)[VEC]) {
+__device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<VEC>& own, float (&in)[VEC],
+                                     float (&next)[VEC]) {
     const uint32_t parity = window & 1;
-    write_run<VEC>(told.segments[warp], lane, own);
+    float decay[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) decay[e] = own.decay(e);
+    put_row<VEC>(told.segments[parity][warp][0], lane, decay);
+    put_row<VEC>(told.segments[parity][warp][1], lane, own.sum);
     __syncthreads();
-    Run<VEC> before, all;
-    before.begin();
-    all.begin();
-    const int mine = BACK ? warps - 1 - warp : warp;
-#pragma unroll
-    for (int i = 0; i < kMostWarps; ++i) {
-        if (i == mine) before = all;
-        if (i < warps) all.then(read_run<VEC>(told.segments[BACK ? warps - 1 - i : i], lane));
-    }
-    __syncthreads();  // (the next window's are written where these lie)
-    if (cluster > 1) {
+    const int mine = BACK ? warps - 1 - warp : warp;  // segments in front of this one
+    if (cluster == 1) {
+        get_row<VEC>(in, told.front[parity], lane);
+    } else {
         const uint32_t bar = shared_address(&told.bars[parity]);
-        if (warp == 0 && lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
-        float decay[VEC];
+        if (mine == 0) {  // (it has no segment in front to go through)
+            if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
+            float c[VEC], sum[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) decay[e] = all.decay(e);
-        for (uint32_t to = warp; to < cluster; to += warps) {
-            const uint32_t there = in_block(shared_address(&told.blocks[parity][rank][0][lane * VEC]), to), bar_there = in_block(bar, to);
-            tell<VEC>(there, bar_there, decay);
-            tell<VEC>(there + 128 * VEC, bar_there, all.sum);
+            for (int e = 0; e < VEC; ++e) c[e] = decay[e], sum[e] = own.sum[e];
+            for (int i = 1; i < warps; ++i) {
+                const auto& segment = told.segments[parity][BACK ? warps - 1 - i : i];
+                float c1[VEC];
+                get_row<VEC>(c1, segment[0], lane);
+                pass<VEC>(sum, segment, lane);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) c[e] = both(c[e], c1[e]);
+            }
+            for (uint32_t to = 0; to < cluster; ++to) {
+                const uint32_t there = in_block(shared_address(&told.blocks[parity][rank][0][lane * VEC]), to), bar_there = in_block(bar, to);
+                tell<VEC>(there, bar_there, c);
+                tell<VEC>(there + 128 * VEC, bar_there, sum);
+            }
         }
         wait_for(bar, window >> 1 & 1, &told.given_up, status);
         const uint32_t ahead = BACK ? cluster - 1 - rank : rank;
-        auto pass = [&](uint32_t j) {
-            const auto& block = told.blocks[parity][BACK ? cluster - 1 - j : j];
-            float c[VEC], sum[VEC];
-            Raw<float, VEC> x;
-            x.load(reinterpret_cast<const char*>(&block[0][lane * VEC]));
-            x.get(c);
-            x.load(reinterpret_cast<const char*>(&block[1][lane * VEC]));
-            x.get(sum);
-            apply_v(carry, c, sum);
-        };
         uint32_t j = 0;
-        for (; j < ahead; ++j) pass(j);
+        for (; j < ahead; ++j) pass<VEC>(next, told.blocks[parity][BACK ? cluster - 1 - j : j], lane);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) in[e] = carry[e];
-        for (; j < cluster; ++j) pass(j);
-    } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) in[e] = carry[e];
-        all.apply_to(carry);
+        for (int e = 0; e < VEC; ++e) in[e] = next[e];
+        for (; j < cluster; ++j) pass<VEC>(next, told.blocks[parity][BACK ? cluster - 1 - j : j], lane);
     }
-    before.apply_to(in);
+    for (int i = 0; i < mine; ++i) pass<VEC>(in, told.segments[parity][BACK ? warps - 1 - i : i], lane);
+    if (cluster == 1 && mine == warps - 1) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) next[e] = in[e];
+        apply_v(next, decay, own.sum);
+        put_row<VEC>(told.front[parity ^ 1], lane, next);
+    }
 }
 
 // Where a thread works: its sequence, channels, and place in a window.
@@ -670,6 +670,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     for (int i = 0; i < kStages - 1; ++i) load();
     float carry[VEC];
     load_end<VEC>(carry, k.initial, at.b, at.ch, at.in);
+    if (at.warp == 0) put_row<VEC>(told.front[0], at.lane, carry);
     for (uint32_t w = 0; w < windows; ++w, t += span, out += out_jump) {
         copies_wait<kStages - 2>();
         __syncwarp();
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
             gates_of<KIND>(gate_sum, unused[0], own.a, own.d, unused[1]);
         }
         float h[VEC];
-        join<VEC, false>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, h);
+        join<VEC, false>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, h, carry);
         if (t >= length) continue;
         if (k.states != nullptr && at.in) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
@@ -730,7 +731,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         else put(std::false_type{});
         x.store(out, k.out.step, rows, at.lane);
     }
-    if (k.final_state.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) store_end<VEC>(k.final_state, at.b, at.ch, carry);
+    if (k.final_state.base != nullptr && at.rank == 0 && at.warp == at.warps - 1 && at.in) store_end<VEC>(k.final_state, at.b, at.ch, carry);
     if (cluster > 1) end_cluster();
 }
 
@@ -785,6 +786,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     load_state(t);
     float carry[VEC];
     load_end<VEC>(carry, k.final_state, at.b, at.ch, at.in);
+    if (at.warp == 0) put_row<VEC>(told.front[0], at.lane, carry);
     for (uint32_t w = 0; w < windows; ++w, t -= span) {
         float c[kSteps][VEC], u[kSteps][VEC], h[VEC];
         rh.get(h);
@@ -836,7 +838,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         if (left == kSteps) take(std::true_type{});
         else take(std::false_type{});
         float later[VEC];
-        join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, carry, later);
+        join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, later, carry);
         if (t < length) {
             const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
             auto put = [&](auto whole) {
