@@ -151,15 +151,19 @@ struct Run {
         fma_v(d, a1, d, d1);
     }
     __device__ __forceinline__ void adds(const float (&a1)[V], const float (&b)[V]) { fma_v(sum, a1, sum, b); }
+    // Another run behind this one, by its decay and sum.
+    __device__ __forceinline__ void then(const float (&c)[V], const float (&s)[V]) {
+        float a1[V], d1[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            a1[e] = keeps(c[e]) ? 1.f + c[e] : c[e];
+            d1[e] = keeps(c[e]) ? -c[e] : 1.f - c[e];
+        }
+        adds(a1, s);
+        decays(a1, d1);
+    }
     __device__ __forceinline__ float decay(int e) const { return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : a[e]; }
 };
-// The decay of two runs, one behind the other.
-__device__ __forceinline__ float both(float c, float d) {
-    const float less = fmaf(c, d, c) + d;
-    const float product = (keeps(c) ? 1.f + c : c) * (keeps(d) ? 1.f + d : d);
-    return keeps(c) && keeps(d) ? (less > -0.5f ? fminf(less, kHold) : 1.f + less) : product;
-}
-
 struct Stream {
     char* base;
     int64_t batch, step;  // bytes
@@ -449,35 +453,50 @@ __device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp,
         get_row<VEC>(in, told.front[parity], lane);
     } else {
         const uint32_t bar = shared_address(&told.bars[parity]);
-        if (mine == 0) {  // (it has no segment in front to go through)
-            if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
-            float c[VEC], sum[VEC];
+        // What the segments in front of this one do, while the cluster's blocks tell each other; and what all do, by the last one.
+        Run<VEC> before;
+        before.begin();
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) c[e] = decay[e], sum[e] = own.sum[e];
-            for (int i = 1; i < warps; ++i) {
+        for (int i = 0; i < kMostWarps - 1; ++i) {
+            if (i < mine) {
                 const auto& segment = told.segments[parity][BACK ? warps - 1 - i : i];
-                float c1[VEC];
-                get_row<VEC>(c1, segment[0], lane);
-                pass<VEC>(sum, segment, lane);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) c[e] = both(c[e], c1[e]);
+                float c[VEC], sum[VEC];
+                get_row<VEC>(c, segment[0], lane);
+                get_row<VEC>(sum, segment[1], lane);
+                before.then(c, sum);
             }
+        }
+        if (mine == warps - 1) {
+            if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
+            Run<VEC> all = before;
+            all.then(decay, own.sum);
+            float c[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) c[e] = all.decay(e);
             for (uint32_t to = 0; to < cluster; ++to) {
                 const uint32_t there = in_block(shared_address(&told.blocks[parity][rank][0][lane * VEC]), to), bar_there = in_block(bar, to);
                 tell<VEC>(there, bar_there, c);
-                tell<VEC>(there + 128 * VEC, bar_there, sum);
+                tell<VEC>(there + 128 * VEC, bar_there, all.sum);
             }
         }
         wait_for(bar, window >> 1 & 1, &told.given_up, status);
         const uint32_t ahead = BACK ? cluster - 1 - rank : rank;
-        uint32_t j = 0;
-        for (; j < ahead; ++j) pass<VEC>(next, told.blocks[parity][BACK ? cluster - 1 - j : j], lane);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) in[e] = next[e];
-        for (; j < cluster; ++j) pass<VEC>(next, told.blocks[parity][BACK ? cluster - 1 - j : j], lane);
+        for (uint32_t j = 0; j < kMostCluster; ++j) {
+            if (j == ahead) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) in[e] = next[e];
+            }
+            if (j < cluster) pass<VEC>(next, told.blocks[parity][BACK ? cluster - 1 - j : j], lane);
+        }
+        float c[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) c[e] = before.decay(e);
+        apply_v(in, c, before.sum);
+        return;
     }
     for (int i = 0; i < mine; ++i) pass<VEC>(in, told.segments[parity][BACK ? warps - 1 - i : i], lane);
-    if (cluster == 1 && mine == warps - 1) {
+    if (mine == warps - 1) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) next[e] = in[e];
         apply_v(next, decay, own.sum);
