@@ -258,6 +258,36 @@ def test_a_sequence_in_parts_and_token_by_token(backend, types):
         check(state, *want["final"], F32, cuts)
 
 
+@pytest.mark.parametrize("length", [5, 100, 3000])
+def test_growing_states(backend, length):
+    """Gates above 0 of the kind exp: growth within F32's range is followed, and a channel without state and input stays at zero however its gates would have it grow."""
+    rng = np.random.default_rng(7)
+    shape = (2, length, 40)
+    x, gate = rng.standard_normal(shape).astype(F32), (rng.standard_normal(shape) * 0.3).astype(F32)
+    gate[:, : min(length, 60), ::4] = 0.4
+    x[0, :, 1::4], gate[0, :, 1::4] = 0, 30
+    initial, dout, dfinal = np.zeros((2, 40), F32), rng.standard_normal(shape).astype(F32), rng.standard_normal((2, 40)).astype(F32)
+    dout[0, :, 1::4], dfinal[0, 1::4] = 0, 0
+    run(backend, x, gate, initial, None, "exp", "dense", dout, dfinal)
+
+
+def test_many_short_sequences(backend):
+    rng = np.random.default_rng(8)
+    for length in (1, 3, 20):
+        x, gate, initial = problem(rng, (70001, length, 6), (F16, F16), "sigmoid")
+        out, final, states = forward(backend, x, gate, initial, None, "sigmoid")
+        some = np.array([0, 1, 65534, 65535, 65536, 70000])
+        want = recurrence(x[some], gate[some], initial[some], None, "sigmoid")
+        check(out[some], *want["out"], F16, "out")
+        check(final[some], *want["final"], F32, "final")
+        space = Space(backend)
+        dx, dinitial = nan(x.shape, F16), nan(initial.shape)
+        backend.gated_recurrence_backward(space.put(x), space.put(gate), space.put(states), out_grad=space.put(out), x_grad=space.put(dx), initial_grad=space.put(dinitial))
+        want = recurrence_backward(x[some], gate[some], initial[some], None, "sigmoid", out[some], None)
+        check(space.get(dx)[0][some], *want["x"], F16, "x")
+        check(space.get(dinitial)[0][some], *want["initial"], F32, "initial")
+
+
 @pytest.mark.parametrize("shape", [(2, 0, 8), (0, 5, 8), (2, 5, 0)])
 def test_nothing_to_do(backend, shape):
     """No step: the state passes through; no sequence or no channel: nothing."""

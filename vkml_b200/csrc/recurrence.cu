@@ -161,6 +161,12 @@ struct Run {
         }
         adds(a1, s);
         decays(a1, d1);
+        stay_finite();
+    }
+    // (Sixteen growing steps may have a product beyond F32's range, and no state to grow: not a number would come of it.)
+    __device__ __forceinline__ void stay_finite() {
+#pragma unroll
+        for (int e = 0; e < V; ++e) asm("min.NaN.f32 %0, %1, %2;" : "=f"(a[e]) : "f"(a[e]), "f"(3.4e38f));
     }
     __device__ __forceinline__ float decay(int e) const { return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : a[e]; }
 };
@@ -354,7 +360,8 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
 // other's, and every thread goes through its steps again from the state that does come in.  All of it stays in registers: gates and inputs are read once, and the
 // next window's are under way while this one is computed.
 
-constexpr int kMostWarps = 8;
+constexpr int kWarps = 8;        // of a block, two of which an SM holds
+constexpr int kMostWarps = 16;   // of one that has an SM to itself
 constexpr int kMostCluster = 8;
 
 // What the segments of a block, and the blocks of a cluster, do to a state: a decay and a sum, for every channel; and the state in front of the window.  Two of each: a
@@ -362,11 +369,15 @@ constexpr int kMostCluster = 8;
 // this one.)
 template <int VEC>
 struct Told {
-    float segments[2][kMostWarps][2][32 * VEC];
-    float blocks[2][kMostCluster][2][32 * VEC];
-    float front[2][32 * VEC];
-    uint64_t bars[2];  // count the bytes that the cluster's blocks tell this one
-    int given_up;
+    static constexpr int kRow = 32 * VEC;
+    float* at;  // in dynamic shared memory, behind the windows
+    int warps;
+    uint64_t* bars;  // [2]: count the bytes that the cluster's blocks tell this one
+    int* given_up;
+    static __host__ __device__ constexpr size_t bytes(int warps, bool cluster) { return size_t(2 * (2 * warps + 1) + (cluster ? 4 * kMostCluster : 0)) * kRow * 4; }
+    __device__ __forceinline__ float* front(uint32_t parity) const { return at + parity * kRow; }
+    __device__ __forceinline__ float* segment(uint32_t parity, int i) const { return at + (2 + (parity * warps + i) * 2) * kRow; }
+    __device__ __forceinline__ float* block(uint32_t parity, uint32_t i) const { return at + (2 + 4 * warps + (parity * kMostCluster + i) * 2) * kRow; }
 };
 template <int VEC>
 __device__ __forceinline__ void get_row(float (&x)[VEC], const float* from, int lane) {
@@ -378,10 +389,10 @@ template <int VEC>
 __device__ __forceinline__ void put_row(float* to, int lane, const float (&x)[VEC]) { Raw<float, VEC>::store(reinterpret_cast<char*>(to + lane * VEC), x); }
 // h behind a segment or a block.
 template <int VEC>
-__device__ __forceinline__ void pass(float (&h)[VEC], const float (&run)[2][32 * VEC], int lane) {
+__device__ __forceinline__ void pass(float (&h)[VEC], const float* run, int lane) {
     float c[VEC], sum[VEC];
-    get_row<VEC>(c, run[0], lane);
-    get_row<VEC>(sum, run[1], lane);
+    get_row<VEC>(c, run, lane);
+    get_row<VEC>(sum, run + 32 * VEC, lane);
     apply_v(h, c, sum);
 }
 
@@ -423,9 +434,9 @@ __device__ __noinline__ void wait_for(uint32_t bar, uint32_t phase, int* given_u
 
 // Before a cluster's blocks tell each other anything, and before one of them ends.
 template <int VEC>
-__device__ __forceinline__ void begin_cluster(Told<VEC>& told) {
+__device__ __forceinline__ void begin_cluster(const Told<VEC>& told) {
     if (threadIdx.x == 0) {
-        told.given_up = 0;
+        *told.given_up = 0;
         for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&told.bars[i])) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -439,33 +450,36 @@ __device__ __forceinline__ void end_cluster() {
 // The state that comes into this warp's steps.  Segments come one after another, in the order of their warps and blocks, or (BACK) the other way round.  `window` counts from 0.
 // In front of window 0 the first warp has put the state to told.front[0]; behind the last one the last warp's `next` is the state there (of a cluster: everyone's).
 template <int VEC, bool BACK>
-__device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp, int lane, int warps, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<VEC>& own, float (&in)[VEC],
+__device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int warp, int lane, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<VEC>& own, float (&in)[VEC],
                                      float (&next)[VEC]) {
     const uint32_t parity = window & 1;
+    const int warps = told.warps;
     float decay[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) decay[e] = own.decay(e);
-    put_row<VEC>(told.segments[parity][warp][0], lane, decay);
-    put_row<VEC>(told.segments[parity][warp][1], lane, own.sum);
+    put_row<VEC>(told.segment(parity, warp), lane, decay);
+    put_row<VEC>(told.segment(parity, warp) + 32 * VEC, lane, own.sum);
     __syncthreads();
     const int mine = BACK ? warps - 1 - warp : warp;  // segments in front of this one
     if (cluster == 1) {
-        get_row<VEC>(in, told.front[parity], lane);
+        get_row<VEC>(in, told.front(parity), lane);
     } else {
         const uint32_t bar = shared_address(&told.bars[parity]);
         // What the segments in front of this one do, while the cluster's blocks tell each other; and what all do, by the last one.
         Run<VEC> before;
         before.begin();
+        auto take = [&](int i) {
+            const float* const segment = told.segment(parity, BACK ? warps - 1 - i : i);
+            float c[VEC], sum[VEC];
+            get_row<VEC>(c, segment, lane);
+            get_row<VEC>(sum, segment + 32 * VEC, lane);
+            before.then(c, sum);
+        };
 #pragma unroll
-        for (int i = 0; i < kMostWarps - 1; ++i) {
-            if (i < mine) {
-                const auto& segment = told.segments[parity][BACK ? warps - 1 - i : i];
-                float c[VEC], sum[VEC];
-                get_row<VEC>(c, segment[0], lane);
-                get_row<VEC>(sum, segment[1], lane);
-                before.then(c, sum);
-            }
+        for (int i = 0; i < kWarps - 1; ++i) {
+            if (i < mine) take(i);
         }
+        for (int i = kWarps - 1; i < mine; ++i) take(i);
         if (mine == warps - 1) {
             if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
             Run<VEC> all = before;
@@ -474,12 +488,12 @@ __device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp,
 #pragma unroll
             for (int e = 0; e < VEC; ++e) c[e] = all.decay(e);
             for (uint32_t to = 0; to < cluster; ++to) {
-                const uint32_t there = in_block(shared_address(&told.blocks[parity][rank][0][lane * VEC]), to), bar_there = in_block(bar, to);
+                const uint32_t there = in_block(shared_address(told.block(parity, rank) + lane * VEC), to), bar_there = in_block(bar, to);
                 tell<VEC>(there, bar_there, c);
                 tell<VEC>(there + 128 * VEC, bar_there, all.sum);
             }
         }
-        wait_for(bar, window >> 1 & 1, &told.given_up, status);
+        wait_for(bar, window >> 1 & 1, told.given_up, status);
         const uint32_t ahead = BACK ? cluster - 1 - rank : rank;
 #pragma unroll
         for (uint32_t j = 0; j < kMostCluster; ++j) {
@@ -487,7 +501,7 @@ __device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp,
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) in[e] = next[e];
             }
-            if (j < cluster) pass<VEC>(next, told.blocks[parity][BACK ? cluster - 1 - j : j], lane);
+            if (j < cluster) pass<VEC>(next, told.block(parity, BACK ? cluster - 1 - j : j), lane);
         }
         float c[VEC];
 #pragma unroll
@@ -495,12 +509,12 @@ __device__ __forceinline__ void join(Told<VEC>& told, uint32_t window, int warp,
         apply_v(in, c, before.sum);
         return;
     }
-    for (int i = 0; i < mine; ++i) pass<VEC>(in, told.segments[parity][BACK ? warps - 1 - i : i], lane);
+    for (int i = 0; i < mine; ++i) pass<VEC>(in, told.segment(parity, BACK ? warps - 1 - i : i), lane);
     if (mine == warps - 1) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) next[e] = in[e];
         apply_v(next, decay, own.sum);
-        put_row<VEC>(told.front[parity ^ 1], lane, next);
+        put_row<VEC>(told.front(parity ^ 1), lane, next);
     }
 }
 
@@ -641,23 +655,27 @@ struct Steps {
         return x;
     }
 };
-// Windows in shared memory of a warp's `bytes` each: two or three, and two blocks on an SM where they fit.
+// Windows in shared memory of a warp's `bytes` each: two or three, and two blocks of 8 warps on an SM (or one of 16) where they fit.
 constexpr int kFewBytes = 98304;
-__host__ __device__ constexpr int stages_of(int bytes) { return kMostWarps * bytes * 3 <= kFewBytes ? 3 : kMostWarps * bytes * 2 <= kFewBytes ? 2 : kMostWarps * bytes * 3 <= 2 * kFewBytes ? 3 : 2; }
-__host__ __device__ constexpr int blocks_of(int bytes) { return kMostWarps * bytes * stages_of(bytes) <= kFewBytes ? 2 : 1; }
+__host__ __device__ constexpr int stages_of(int bytes) { return kWarps * bytes * 3 <= kFewBytes ? 3 : kWarps * bytes * 2 <= kFewBytes ? 2 : kWarps * bytes * 3 <= 2 * kFewBytes ? 3 : 2; }
+__host__ __device__ constexpr int blocks_of(int bytes) { return kWarps * bytes * stages_of(bytes) <= kFewBytes ? 2 : 1; }
 template <typename T, typename G, int VEC, int CHUNK, bool BACK>
 constexpr int kWindowBytes = (BACK ? 2 : 1) * Steps<T, VEC, CHUNK>::kPlace + Steps<G, VEC, CHUNK>::kPlace;
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
-template <typename T, typename G, int KIND, int VEC, int CHUNK>
-__global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, VEC, CHUNK, false>)) walk_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+// CLUSTER: whether `blocks` of them may be a cluster.
+template <typename T, typename G, int KIND, int VEC, int CHUNK, bool CLUSTER>
+__global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK, false>) == 2 ? kMostWarps : kWarps), 1) walk_kernel(const Args k, uint32_t strips, uint32_t blocks) {
+    const uint32_t cluster = CLUSTER ? blocks : 1;
     constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>, kStages = stages_of(kBytes);
     using X = Steps<T, VEC, CHUNK>;
     using Y = Steps<G, VEC, CHUNK>;
     extern __shared__ __align__(16) char ring[];
-    __shared__ Told<VEC> told;
+    __shared__ uint64_t bars[2];
+    __shared__ int given_up;
+    const Told<VEC> told{reinterpret_cast<float*>(ring + blockDim.x / 32 * kStages * kBytes), static_cast<int>(blockDim.x / 32), bars, &given_up};
     pdl_prologue();
     if (cluster > 1) begin_cluster(told);
     const Place<VEC> at(k, strips, cluster);
@@ -689,7 +707,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     for (int i = 0; i < kStages - 1; ++i) load();
     float carry[VEC];
     load_end<VEC>(carry, k.initial, at.b, at.ch, at.in);
-    if (at.warp == 0) put_row<VEC>(told.front[0], at.lane, carry);
+    if (at.warp == 0) put_row<VEC>(told.front(0), at.lane, carry);
     for (uint32_t w = 0; w < windows; ++w, t += span, out += out_jump) {
         copies_wait<kStages - 2>();
         __syncwarp();
@@ -729,9 +747,10 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         if constexpr (KIND == B200_GATES_EXP) {  // the product of the a's is that of one step whose gate is the sum
             float unused[2][VEC];
             gates_of<KIND>(gate_sum, unused[0], own.a, own.d, unused[1]);
+            own.stay_finite();
         }
         float h[VEC];
-        join<VEC, false>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, h, carry);
+        join<VEC, false>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, h, carry);
         if (t >= length) continue;
         if (k.states != nullptr && at.in) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
@@ -754,13 +773,17 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     if (cluster > 1) end_cluster();
 }
 
-template <typename T, typename G, int KIND, int VEC, int CHUNK>
-__global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, VEC, CHUNK, true>)) walk_backward_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+// CLUSTER: whether `blocks` of them may be a cluster.
+template <typename T, typename G, int KIND, int VEC, int CHUNK, bool CLUSTER>
+__global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK, true>) == 2 ? kMostWarps : kWarps), 1) walk_backward_kernel(const Args k, uint32_t strips, uint32_t blocks) {
+    const uint32_t cluster = CLUSTER ? blocks : 1;
     constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, true>, kStages = stages_of(kBytes);
     using X = Steps<T, VEC, CHUNK>;
     using Y = Steps<G, VEC, CHUNK>;
     extern __shared__ __align__(16) char ring[];
-    __shared__ Told<VEC> told;
+    __shared__ uint64_t bars[2];
+    __shared__ int given_up;
+    const Told<VEC> told{reinterpret_cast<float*>(ring + blockDim.x / 32 * kStages * kBytes), static_cast<int>(blockDim.x / 32), bars, &given_up};
     pdl_prologue();
     if (cluster > 1) begin_cluster(told);
     const Place<VEC> at(k, strips, cluster);
@@ -805,7 +828,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
     load_state(t);
     float carry[VEC];
     load_end<VEC>(carry, k.final_state, at.b, at.ch, at.in);
-    if (at.warp == 0) put_row<VEC>(told.front[0], at.lane, carry);
+    if (at.warp == 0) put_row<VEC>(told.front(0), at.lane, carry);
     for (uint32_t w = 0; w < windows; ++w, t -= span) {
         float c[kSteps][VEC], u[kSteps][VEC], h[VEC];
         rh.get(h);
@@ -850,6 +873,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
                 for (int e = 0; e < VEC; ++e) u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
                 mul_v(b, input, xs);
                 own.decays(a, d);
+                if constexpr (KIND == B200_GATES_EXP) own.stay_finite();
                 fma_v(own.sum, own.a, ds, own.sum);  // what the steps' gradients make of the state in front of them: each times the a's up to it
                 fma_v(h, a, h, b);  // (a's rounding counts within these steps only, here and below)
             }
@@ -857,7 +881,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, blocks_of(kWindowBytes<T, G, 
         if (left == kSteps) take(std::true_type{});
         else take(std::false_type{});
         float later[VEC];
-        join<VEC, true>(told, w, at.warp, at.lane, at.warps, at.rank, at.cluster, k.status, own, later, carry);
+        join<VEC, true>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, later, carry);
         if (t < length) {
             const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
             auto put = [&](auto whole) {
@@ -1024,6 +1048,7 @@ struct Walk {
     int vec = 1;     // channels of a lane
     int chunk = 2;   // of Steps
     int cluster = 1;
+    bool alone = false;  // a cluster's blocks have SMs to themselves, and there is room for them in every part of the device: twice the warps, where they fit
     int64_t strips = 0, blocks = 0;
 };
 struct Typed {
@@ -1048,8 +1073,9 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
     w.chunk = halves && !pairs ? 2 : chunk;
     if (s.length <= kSteps) return w;
     w.strips = ceil_div(s.width, 32 * w.vec);
-    w.warps = static_cast<int>(std::min<int64_t>(kMostWarps, ceil_div(s.length, kSteps)));
+    w.warps = static_cast<int>(std::min<int64_t>(kWarps, ceil_div(s.length, kSteps)));
     while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
+    w.alone = w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= sm_count() && s.length > int64_t(w.cluster) * w.warps * kSteps;
     w.blocks = s.batch * w.strips * w.cluster;
     return w;
 }
@@ -1063,10 +1089,12 @@ void by_walk(const Walk& w, Fn&& go) {
     else if constexpr (kVec == 2) go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
 }
 
-template <typename Kernel>
-void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, size_t shared, const Args& k) {
-    const dim3 grid(static_cast<unsigned>(w.blocks)), threads(static_cast<unsigned>(32 * w.warps));
-    (void)blocks_at_once(reinterpret_cast<const void*>(kernel), 32 * w.warps, shared);  // (allows that much shared memory)
+template <int BYTES, int VEC, typename Kernel>
+void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, const Args& k) {
+    const int warps = w.alone && blocks_of(BYTES) == 2 ? kMostWarps : w.warps;
+    const size_t shared = static_cast<size_t>(warps) * stages_of(BYTES) * BYTES + Told<VEC>::bytes(warps, w.cluster > 1);
+    const dim3 grid(static_cast<unsigned>(w.blocks)), threads(static_cast<unsigned>(32 * warps));
+    (void)blocks_at_once(reinterpret_cast<const void*>(kernel), 32 * warps, shared);  // (allows that much shared memory)
     if (w.cluster == 1) launch_kernel(ctx, kernel, grid, threads, shared, k, static_cast<uint32_t>(w.strips), 1u);
     else launch_kernel_clustered(ctx, kernel, grid, threads, shared, w.cluster, false, k, static_cast<uint32_t>(w.strips), static_cast<uint32_t>(w.cluster));
 }
@@ -1095,7 +1123,7 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
             by_walk<T>(w, [&](auto vec, auto chunk) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
                 constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>;
-                launch_walk(ctx, walk_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * stages_of(kBytes) * kBytes, k);
+                launch_walk<kBytes, VEC>(ctx, CHUNK == 16 && w.cluster == 1 ? walk_kernel<T, G, KIND, VEC, CHUNK, CHUNK != 16> : walk_kernel<T, G, KIND, VEC, CHUNK, true>, w, k);
             });
         }
     });
@@ -1129,7 +1157,7 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
             by_walk<T>(w, [&](auto vec, auto chunk) {
                 constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
                 constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, true>;
-                launch_walk(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK>, w, static_cast<size_t>(w.warps) * stages_of(kBytes) * kBytes, k);
+                launch_walk<kBytes, VEC>(ctx, CHUNK == 16 && w.cluster == 1 ? walk_backward_kernel<T, G, KIND, VEC, CHUNK, CHUNK != 16> : walk_backward_kernel<T, G, KIND, VEC, CHUNK, true>, w, k);
             });
         }
     });
