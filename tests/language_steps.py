@@ -46,9 +46,11 @@ def inside(lengths, shape):
 def recurrence(x, gate, initial, lengths, kind):
     """{out, final, states, before}: (values, bounds), of [B, L, D]."""
     batch, length, width = x.shape
+    valid = inside(lengths, x.shape)
+    gate = np.where(valid, gate, 0)  # (behind an end it may be anything)
     a, d, scale = gates(gate, kind)
-    b = scale * np.where(inside(lengths, x.shape), x, 0).astype(np.float64)
-    k, valid = spread(gate), inside(lengths, x.shape)
+    b = scale * np.where(valid, x, 0).astype(np.float64)
+    k = spread(gate)
     h = np.zeros((batch, width)) if initial is None else initial.astype(np.float64)
     e = np.zeros_like(h)
     out, error, before, before_error = (np.zeros(x.shape) for _ in range(4))
@@ -66,8 +68,10 @@ def recurrence(x, gate, initial, lengths, kind):
 def recurrence_backward(x, gate, initial, lengths, kind, dout, dfinal):
     """{x, gate, initial}: (gradients, bounds).  Everything is computed again from x, gate and initial: the states' errors are in the bounds."""
     batch, length, width = x.shape
+    valid = inside(lengths, x.shape)
+    gate = np.where(valid, gate, 0)
     a, d, scale = gates(gate, kind)
-    valid, k = inside(lengths, x.shape), spread(gate)
+    k = spread(gate)
     before, before_error = recurrence(x, gate, initial, lengths, kind)["before"]
     x = np.where(valid, x, 0).astype(np.float64)
     dout = np.zeros(x.shape) if dout is None else np.where(valid, dout, 0).astype(np.float64)
