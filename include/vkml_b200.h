@@ -418,7 +418,8 @@ int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
 
 /* A gated linear recurrence along a sequence, each channel by itself: h_t = a_t h_{t-1} + b_t, out_t = h_t, with
  *     B200_GATES_SIGMOID: a = sigmoid(gate), b = (1 - a) x        B200_GATES_EXP: a = exp(gate), b = x
- * A gate of -inf begins anew (a = 0).  Products of decays just below 1 keep their digits: 1 - a is carried where a is above a half. */
+ * A gate of -inf begins anew (a = 0).  Products of decays just below 1 keep their digits: 1 - a is carried where a is above a half.  A state that is infinite or no number
+ * leaves none that is finite behind it in its channel. */
 #define B200_GATES_SIGMOID 0
 #define B200_GATES_EXP 1
 #define B200_RECURRENCE_CHUNK 16

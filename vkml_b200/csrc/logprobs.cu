@@ -6,14 +6,16 @@
 //   grad = k [ a (one at token - q) - w q (log q + H) ] / T,  a and w the gradients of the token's log q and of H
 //
 // Bound by memory: z read once, and backward as much written.  A block takes a row after another: each thread keeps the maximum of what it has read and the sums of
-// e^u and e^u u beside it, and the block joins these threes.  What comes next, of this row or the next one, is on its way into shared memory all the while, so
-// that a row's end costs other rows' time only.  Few long rows are a cluster's each, whose blocks take a part of it.
+// e^u and e^u u beside it, and the block joins these threes.  What comes next, of this row or the next one, is on its way into registers all the while, so that a
+// row's end holds up nothing that is read.  (Through shared memory, by asynchronous copies, a row's end cost more than the registers do: 4096 x 32000 F16 95 us in place
+// of 55.)  Few long rows are a cluster's each, whose blocks take a part of it.  2047 x 128000 F32: 156 us, 6.7 TB/s; 4096 x 32000 F16: 54 us, 4.9 TB/s, bound by the
+// exponential, the two sums and the conversion of each element.
 //
 // The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least
-// reach; it is found by halving the range between the maxima, by one warp.  Each thread has kept the maxima of up to sixteen stretches of what it had, too: only
-// stretches whose maximum reaches the bound (little more than K) are read again, and what reaches it goes into shared memory, where an entry's rank is the number of larger ones.  Where more entries reach it than
-// there is room for (a row of few different values: most of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in
-// the order of their columns.
+// reach; it is found by halving the range between the maxima, by one warp.  Each thread has kept the maxima of up to sixteen stretches of what it had, too (with four,
+// the 20 largest of 2048 x 128000 F32 take 210 us in place of 179): only stretches whose maximum reaches the bound (little more than K) are read again, and what reaches
+// it goes into shared memory, where an entry's rank is the number of larger ones.  Where more entries reach it than there is room for (a row of few different values: most
+// of its columns forbidden, say) the bound is made exact by counting over the row, and equal ones are taken in the order of their columns.
 #include "operators.cuh"
 
 #include <algorithm>
@@ -511,6 +513,9 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
 }
 
 // ---- the gradient -----------------------------------------------------------
+//
+// A thread takes four vectors, all of them asked for before the first is worked on; a row is as many blocks' as that makes.  2048 x 50001 F16: 75 us (5.5 TB/s; one
+// exponential to an element); 4096 x 32000 F16 90 us (5.8 TB/s).
 
 constexpr int kGradThreads = 256;
 constexpr int kGradVectors = 4;
@@ -718,12 +723,13 @@ void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
     ProfScope scope(ctx, "token_logprobs");
     const bool half = a.logits.dtype == B200_F16;
     const int64_t vectors = ceil_div(plan.vocab, half ? 8 : 4);
-    // Threads of a block: 32 vectors to each, as a row's end costs a thread as much as 4 of them or more, up to 128, whose warps wait together (2047 x 128000 F32: 171 us with
-    // blocks of 64, 174 with 128, 199 with 256); and more threads than entries that are wanted.  Few rows: up to 512 threads of four vectors, and long ones a
-    // cluster of blocks each.
+    // Threads of a block: 32 vectors to each, as a row's end costs a thread as much as 4 of them or more, up to 64 (2047 x 128000 F32: 156 us, 161 with 128, 171 with 256), or
+    // 128 where entries are wanted, which are found by stretches of a thread each (the 20 largest of 2048 x 128000 F32: 188 us with 64, 179 with 128, 195 with 256); and
+    // more threads than entries.  Few rows: up to 512 threads of four vectors, and long ones a cluster of blocks each (1 x 128000 F32 6.2 us, 8.7 by one block; 16 x 128000
+    // F16 with the 20 largest 11.7 and 12.8).
     const bool few = plan.s.rows <= sm_count();
     int threads = 32, blocks = 1;
-    while (threads < kMostThreads && ((vectors > int64_t(threads) * (few ? 4 : 32) && (few || threads < 128)) || plan.top * 2 > threads)) threads *= 2;
+    while (threads < kMostThreads && ((vectors > int64_t(threads) * (few ? 4 : 32) && (few || threads < (plan.top > 0 ? 128 : 64))) || plan.top * 2 > threads)) threads *= 2;
     while (blocks < kMostBlocks && plan.s.rows * blocks * 2 <= sm_count() && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
     auto go = [&](auto kernel) {
         size_t shared = 0;
