@@ -91,7 +91,7 @@ __device__ __forceinline__ uint32_t order_of(float z) {
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order >> 31 ? order & 0x7fffffffu : ~order); }
 
-// The maximum, and beside it the sums of e^u and of e^u u in powers of two: 2^v and 2^v v, v = (z - max) log2 e / T.
+// A number that no element is far above, and beside it the sums of e^u and of e^u u in powers of two: 2^v and 2^v v, v = (z - top) log2 e / T.
 struct Part {
     float top, sum, turned;
 };
@@ -107,8 +107,8 @@ __device__ __forceinline__ void shift_part(Part& x, float top, float c) {
     x.top = top;
 }
 
-__device__ __forceinline__ Part warp_part(Part x, float c) {
-    float top = x.top;
+// The lanes' parts joined beside the largest element, of which `top` is each lane's own.
+__device__ __forceinline__ Part warp_part(Part x, float top, float c) {
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
     shift_part(x, top, c);
@@ -123,12 +123,15 @@ __device__ __forceinline__ Part warp_part(Part x, float c) {
 template <typename T>
 constexpr uint32_t kNothing = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u;  // -inf
 
-// Adds vectors, or their powers beside a maximum that is there, to a part.  Elements of -inf count as far below, as powers of two of -150, which are 0.  Halves
-// are raised to the lowest finite one instead (CLAMP: two to an instruction), where that is as far below and the difference's power is a number.
+// Adds vectors' powers to a part.  Elements of -inf count as far below, as powers of two of -150, which are 0.
+//
+// CLAMP: halves are raised to the lowest finite one instead, two to an instruction, where that is as far below.  v is one multiply-add then, z c - at c: at c's rounding
+// is the same for all and at most 2^-8, and what it made of the sums is given back at the end.
 template <typename T, bool CLAMP, int N>
 __device__ __forceinline__ void take_powers(Part& part, uint4 (&raw)[N], float at, float c) {
     constexpr int E = 16 / sizeof(T);
     float sum[2] = {0.f, 0.f}, turned[2] = {0.f, 0.f};
+    const float off = -at * c;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         float z[E];
@@ -142,16 +145,27 @@ __device__ __forceinline__ void take_powers(Part& part, uint4 (&raw)[N], float a
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             float v[2], p[2];
-            add_pair(v[0], v[1], z[e], z[e + 1], -at, -at);
-            mul_pair(v[0], v[1], v[0], v[1], c, c);
-            if constexpr (!CLAMP) v[0] = max_nan(v[0], -150.f), v[1] = max_nan(v[1], -150.f);
+            if constexpr (CLAMP) {
+                fma_pair(v[0], v[1], z[e], z[e + 1], c, c, off, off);
+            } else {
+                add_pair(v[0], v[1], z[e], z[e + 1], -at, -at);
+                mul_pair(v[0], v[1], v[0], v[1], c, c);
+                v[0] = max_nan(v[0], -150.f), v[1] = max_nan(v[1], -150.f);
+            }
             p[0] = fast_exp2(v[0]), p[1] = fast_exp2(v[1]);
             add_pair(sum[0], sum[1], sum[0], sum[1], p[0], p[1]);
             fma_pair(turned[0], turned[1], p[0], p[1], v[0], v[1], turned[0], turned[1]);
         }
     }
-    part.sum += sum[0] + sum[1];
-    part.turned += turned[0] + turned[1];
+    sum[0] += sum[1], turned[0] += turned[1];
+    if constexpr (CLAMP) {
+        const float less = fmaf(-at, c, -off);  // what every v lacks
+        const float f = fast_exp2(less);
+        sum[0] *= f;
+        turned[0] = fmaf(turned[0], f, less * sum[0]);
+    }
+    part.sum += sum[0];
+    part.turned += turned[0];
 }
 // The largest element of N vectors (halves compare as halves, two at a time); no number where one is none.
 template <typename T, int N>
@@ -175,13 +189,13 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
     }
     return top;
 }
-// Vectors whose largest element is `most`.
+// Vectors whose largest element is `most`.  The number that the sums are beside of moves when an element is above it, to two powers of two above that one: it moves a few
+// times in a row.
 template <typename T, int N>
-__device__ __forceinline__ void take(Part& part, uint4 (&raw)[N], float most, float c) {
-    const float top = max_nan(most, part.top);
-    if (!(top == part.top)) shift_part(part, top, c);
-    const float at = shift_of(top);
-    if (sizeof(T) == 2 && (at + 65504.f) * c > 160.f && c < 1e30f) take_powers<T, sizeof(T) == 2>(part, raw, at, c);
+__device__ __forceinline__ void take(Part& part, uint4 (&raw)[N], float most, float c, float above) {
+    if (!(most <= part.top)) shift_part(part, most + above, c);
+    const float at = shift_of(part.top);
+    if (sizeof(T) == 2 && (at + 65504.f) * c > 160.f && fabsf(at * c) < 0x1p17f) take_powers<T, sizeof(T) == 2>(part, raw, at, c);
     else take_powers<T, false>(part, raw, at, c);
 }
 
@@ -226,7 +240,7 @@ __device__ __forceinline__ void write_row(const Args& k, uint32_t r, const Part&
 }
 // Each of n entries to the place of its rank, if it is one of the first: as a result, or, where `to` is given, as an entry in another block's shared memory.
 __device__ __forceinline__ void rank_entries(const Args& k, uint32_t r, const Part& all, const uint64_t* entries, int n, const uint32_t* to) {
-    if (k.top == 0) return;
+    if (static_cast<int>(threadIdx.x) >= n) return;
     char* const ids = k.ids.base != nullptr ? row_at(k.ids, k.inner, r) : nullptr;
     float* const tops = k.tops.base != nullptr ? reinterpret_cast<float*>(row_at(k.tops, k.inner, r)) : nullptr;
     const Totals x(all);
@@ -266,9 +280,9 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
     uint64_t* const merged = entries + room;  // (of a cluster's first block)
     // where entries are wanted: every thread's maximum, its stretches', and the stretches that are read again
     uint32_t* const tops = reinterpret_cast<uint32_t*>(merged + (blocks > 1 ? blocks * k.top : 0));
-    uint32_t* const stretch_tops = tops + THREADS;
+    float* const stretch_tops = reinterpret_cast<float*>(tops + THREADS);
     uint16_t* const stretch_list = reinterpret_cast<uint16_t*>(stretch_tops + kStretches * THREADS);
-    const float c = k.inverse * kLog2e;
+    const float c = k.inverse * kLog2e, above = fminf(2.f / c, 1e30f);
     if (blocks > 1) cluster_sync();  // (every block is there before another writes to it)
 
     // What is on its way: this thread's vectors of the next chunk, of this row or of the one behind it; what is asked for after it, and the vectors left from there on.
@@ -324,18 +338,20 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
         // (two to the power of `shift` batches make a stretch)
         int shift = 0, batch = 0, stretch = 0;
         while ((row.last - row.first + kChunk - 1) / kChunk > kStretches << shift) ++shift;
-        float stretch_top = -INFINITY;
+        float most = -INFINITY, stretch_top = -INFINITY;
         for (int rest = row.last - row.first; rest > 0; rest -= kChunk) {
             uint4 raw[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) raw[i] = next[i];
             ask();
             const float top = largest<T>(raw);
-            take<T>(part, raw, top, c);
+            most = max_nan(most, top);
+            if (rest == row.last - row.first) part.top = value_of(__reduce_max_sync(0xffffffffu, order_of(top))) + above;  // (the warp's, so that few lanes meet a larger one)
+            take<T>(part, raw, top, c, above);
             if (k.top > 0) {
                 stretch_top = max_nan(stretch_top, top);
                 if ((++batch & ((1 << shift) - 1)) == 0 || rest <= kChunk) {
-                    stretch_tops[stretch++ * THREADS + tid] = order_of(stretch_top);
+                    stretch_tops[stretch++ * THREADS + tid] = stretch_top;
                     stretch_top = -INFINITY;
                 }
             }
@@ -345,15 +361,15 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
             uint4 one[1] = {make_uint4(kNothing<T>, kNothing<T>, kNothing<T>, kNothing<T>)};
             if constexpr (sizeof(T) == 2) one[0].x = 0xfc000000u | __half_as_ushort(end_element);
             else one[0].x = __float_as_uint(end_element);
-            take<T>(part, one, end_z, c);
+            take<T>(part, one, end_z, c, above);
+            most = max_nan(most, end_z);
         }
-        const float own_top = part.top;
-        Part all = warp_part(part, c);
+        Part all = warp_part(part, most, c);
         if constexpr (kWarps > 1) {
             if (tid % 32 == 0) parts[parity][tid / 32] = all;
             __syncthreads();
             all = tid % 32 < kWarps ? parts[parity][tid % 32] : Part{-INFINITY, 0.f, 0.f};
-            all = warp_part(all, c);
+            all = warp_part(all, all.top, c);
         } else {
             __syncwarp();
         }
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
         int n = 0;
         if (k.top > 0) {
             const bool owner = end >= 0 || row.first + tid < row.last;
-            const uint32_t own = owner ? order_of(own_top) : 0u;
+            const uint32_t own = owner ? order_of(most) : 0u;
             tops[tid] = own;
             if (tid == 0) count = 0, found = 0;
             __syncthreads();
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
                     if (i < room) entries[i] = uint64_t(o) << 32 | (0xffffffffu - column);
                 };
                 for (int s = 0; s < stretch && own >= bound; ++s) {
-                    if (stretch_tops[s * THREADS + tid] >= bound) stretch_list[atomicAdd(&found, 1)] = static_cast<uint16_t>(s * THREADS + tid);
+                    if (order_of(stretch_tops[s * THREADS + tid]) >= bound) stretch_list[atomicAdd(&found, 1)] = static_cast<uint16_t>(s * THREADS + tid);
                 }
                 if (end >= 0) put(order_of(end_z), static_cast<uint32_t>(end));
                 __syncthreads();
@@ -504,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 /
             cluster_sync();
             if (rank == 0) {
                 all = tid % 32 < static_cast<int>(blocks) ? cluster_parts[tid % 32] : Part{-INFINITY, 0.f, 0.f};
-                all = warp_part(all, c);
+                all = warp_part(all, all.top, c);
                 if (tid == 0) write_row(k, r, all, token, token_z);
                 rank_entries(k, r, all, merged, static_cast<int>(blocks) * k.top, nullptr);
             }

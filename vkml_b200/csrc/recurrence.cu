@@ -367,6 +367,7 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
 constexpr int kWarps = 8;        // of a block, two of which an SM holds
 constexpr int kMostWarps = 16;   // of one that has an SM to itself
 constexpr int kMostCluster = 8;
+constexpr int kAheadSlots = 4;   // (walk_ahead_kernel)
 
 // What the segments of a block, and the blocks of a cluster, do to a state: a decay and a sum, for every channel; and the state in front of the window.  Two of each: a
 // window's are read while the next one's are written.  (A block that is told of the window after next has told the next one itself, behind its reading of
@@ -376,12 +377,12 @@ struct Told {
     static constexpr int kRow = 32 * VEC;
     float* at;  // in dynamic shared memory, behind the windows
     int warps;
-    uint64_t* bars;  // [2]: count the bytes that the cluster's blocks tell this one
+    uint64_t* bars;  // one for each place to be told at: counts the bytes that the cluster's blocks tell this one
     int* given_up;
-    static __host__ __device__ constexpr size_t bytes(int warps, bool cluster) { return size_t(2 * (2 * warps + 1) + (cluster ? 4 * kMostCluster : 0)) * kRow * 4; }
+    static __host__ __device__ constexpr size_t bytes(int warps, int slots) { return size_t(2 * (2 * warps + 1) + 2 * slots * kMostCluster) * kRow * 4; }
     __device__ __forceinline__ float* front(uint32_t parity) const { return at + parity * kRow; }
     __device__ __forceinline__ float* segment(uint32_t parity, int i) const { return at + (2 + (parity * warps + i) * 2) * kRow; }
-    __device__ __forceinline__ float* block(uint32_t parity, uint32_t i) const { return at + (2 + 4 * warps + (parity * kMostCluster + i) * 2) * kRow; }
+    __device__ __forceinline__ float* block(uint32_t slot, uint32_t i) const { return at + (2 + 4 * warps + (slot * kMostCluster + i) * 2) * kRow; }
 };
 template <int VEC>
 __device__ __forceinline__ void get_row(float (&x)[VEC], const float* from, int lane) {
@@ -438,10 +439,10 @@ __device__ __noinline__ void wait_for(uint32_t bar, uint32_t phase, int* given_u
 
 // Before a cluster's blocks tell each other anything, and before one of them ends.
 template <int VEC>
-__device__ __forceinline__ void begin_cluster(const Told<VEC>& told) {
+__device__ __forceinline__ void begin_cluster(const Told<VEC>& told, int slots) {
     if (threadIdx.x == 0) {
         *told.given_up = 0;
-        for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&told.bars[i])) : "memory");
+        for (int i = 0; i < slots; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&told.bars[i])) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     cluster_sync();
@@ -669,6 +670,57 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int PENDING>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
+// The first walk through a window's steps, of which `left` are the sequence's: what they do to a state, by themselves and all together.
+template <int KIND, int VEC, typename X, typename Y>
+__device__ __forceinline__ void take_steps(const X& x, const Y& gate, int lane, int left, float (&a)[kSteps][VEC], float (&b)[kSteps][VEC], Run<VEC>& own) {
+    own.begin();
+    float gate_sum[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) gate_sum[e] = 0.f;
+    auto take = [&](auto whole) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            float xs[VEC], gs[VEC], c[VEC], d[VEC], input[VEC];
+            x.get(j, lane).get(xs);
+            gate.get(j, lane).get(gs);
+            if (!whole.value && j >= left) {  // the state stays
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
+            }
+            gates_of<KIND>(gs, c, a[j], d, input);
+            mul_v(b[j], input, xs);
+            if constexpr (KIND == B200_GATES_SIGMOID) own.decays(a[j], d);
+            else add_v(gate_sum, gate_sum, gs);
+            own.adds(a[j], b[j]);
+        }
+    };
+    if (left == kSteps) take(std::true_type{});
+    else take(std::false_type{});
+    if constexpr (KIND == B200_GATES_EXP) {  // the product of the a's is that of one step whose gate is the sum
+        float unused[2][VEC];
+        gates_of<KIND>(gate_sum, unused[0], own.a, own.d, unused[1]);
+        own.stay_finite();
+    }
+}
+// The second one, from the state h in front of them, to `rows` rows of the result.
+template <int VEC, typename X>
+__device__ __forceinline__ void put_steps(const X& x, int lane, bool in, int left, int rows, char* out, int64_t step, const float (&a)[kSteps][VEC], const float (&b)[kSteps][VEC], float (&h)[VEC]) {
+    auto put = [&](auto whole) {
+        char* p = out;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j, p += step) {
+            fma_v(h, a[j], h, b[j]);  // (a's rounding counts within these steps only)
+            float y[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[e] = whole.value || j < left ? h[e] : 0.f;
+            x.put(j, lane, p, y, in && (whole.value || j < rows));
+        }
+    };
+    if (left == kSteps) put(std::true_type{});
+    else put(std::false_type{});
+    x.store(out, step, rows, lane);
+}
+
 // CLUSTER: whether `blocks` of them may be a cluster.
 template <typename T, typename G, int KIND, int VEC, int CHUNK, bool CLUSTER>
 __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK, false>) == 2 ? kMostWarps : kWarps), 1) walk_kernel(const Args k, uint32_t strips, uint32_t blocks) {
@@ -681,7 +733,7 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
     __shared__ int given_up;
     const Told<VEC> told{reinterpret_cast<float*>(ring + blockDim.x / 32 * kStages * kBytes), static_cast<int>(blockDim.x / 32), bars, &given_up};
     pdl_prologue();
-    if (cluster > 1) begin_cluster(told);
+    if (cluster > 1) begin_cluster(told, 2);
     const Place<VEC> at(k, strips, cluster);
     const uint32_t length = static_cast<uint32_t>(k.length), n = static_cast<uint32_t>(steps_of(k, at.b)), span = at.span();
     const uint32_t windows = (length + span - 1) / span;
@@ -724,57 +776,138 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
         load();  // (where the window before lay)
         float a[kSteps][VEC], b[kSteps][VEC];
         Run<VEC> own;
-        own.begin();
-        float gate_sum[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) gate_sum[e] = 0.f;
         const int left = t < n ? static_cast<int>(min(n - t, uint32_t(kSteps))) : 0;  // steps of the sequence
-        auto take = [&](auto whole) {
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                float xs[VEC], gs[VEC], c[VEC], d[VEC], input[VEC];
-                x.get(j, at.lane).get(xs);
-                gate.get(j, at.lane).get(gs);
-                if (!whole.value && j >= left) {  // the state stays
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
-                }
-                gates_of<KIND>(gs, c, a[j], d, input);
-                mul_v(b[j], input, xs);
-                if constexpr (KIND == B200_GATES_SIGMOID) own.decays(a[j], d);
-                else add_v(gate_sum, gate_sum, gs);
-                own.adds(a[j], b[j]);
-            }
-        };
-        if (left == kSteps) take(std::true_type{});
-        else take(std::false_type{});
-        if constexpr (KIND == B200_GATES_EXP) {  // the product of the a's is that of one step whose gate is the sum
-            float unused[2][VEC];
-            gates_of<KIND>(gate_sum, unused[0], own.a, own.d, unused[1]);
-            own.stay_finite();
-        }
+        take_steps<KIND, VEC>(x, gate, at.lane, left, a, b, own);
         float h[VEC];
         join<VEC, false>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, h, carry);
         if (t >= length) continue;
         if (k.states != nullptr && at.in) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
-        auto put = [&](auto whole) {
-            char* p = out;
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j, p += k.out.step) {
-                fma_v(h, a[j], h, b[j]);  // (a's rounding counts within these steps only)
-                float y[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) y[e] = whole.value || j < left ? h[e] : 0.f;
-                x.put(j, at.lane, p, y, at.in && (whole.value || j < rows));
-            }
-        };
-        if (left == kSteps) put(std::true_type{});
-        else put(std::false_type{});
-        x.store(out, k.out.step, rows, at.lane);
+        put_steps<VEC>(x, at.lane, at.in, left, rows, out, k.out.step, a, b, h);
     }
     if (k.final_state.base != nullptr && at.rank == 0 && at.warp == at.warps - 1 && at.in) store_end<VEC>(k.final_state, at.b, at.ch, carry);
     if (cluster > 1) end_cluster();
+}
+
+// Clusters whose lanes have a channel each: what a window's segments do to a state is told a window ahead, so that the wait for the other blocks is one for what was sent
+// while this window was gone through the first time.  (Two windows' steps in registers, and four places to be told at: a block that is told of the fourth window from here has
+// told this one's cluster of the second, behind its reading of this one.)
+template <typename T, typename G, int KIND, int CHUNK>
+__global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, false>) == 2 ? kMostWarps : kWarps), 1) walk_ahead_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    constexpr int kBytes = kWindowBytes<T, G, 1, CHUNK, false>, kStages = stages_of(kBytes);
+    static_assert(kStages == 3);  // (one is loaded, one gone through the first time, one the second time)
+    using X = Steps<T, 1, CHUNK>;
+    using Y = Steps<G, 1, CHUNK>;
+    extern __shared__ __align__(16) char ring[];
+    __shared__ uint64_t bars[kAheadSlots];
+    __shared__ int given_up;
+    const Told<1> told{reinterpret_cast<float*>(ring + blockDim.x / 32 * kStages * kBytes), static_cast<int>(blockDim.x / 32), bars, &given_up};
+    pdl_prologue();
+    begin_cluster(told, kAheadSlots);
+    const Place<1> at(k, strips, cluster);
+    const uint32_t length = static_cast<uint32_t>(k.length), n = static_cast<uint32_t>(steps_of(k, at.b)), span = at.span();
+    const uint32_t windows = (length + span - 1) / span;
+    X x;
+    Y gate;
+    x.begin(at.template strip<T>(k.x), k.x.step, at.first(), span, at.valid(k.width, sizeof(T)), at.lane);
+    gate.begin(at.template strip<G>(k.gate), k.gate.step, at.first(), span, at.valid(k.width, sizeof(G)), at.lane);
+    char* out = X::first_piece(const_cast<char*>(at.template strip<T>(k.out)), k.out.step, at.first(), at.lane);
+    const int64_t out_jump = span * k.out.step;
+    const char* x_at = at.template strip<T>(k.x) + at.first() * k.x.step;  // (of the window that is gone through the first time: X::kAround asks)
+    const char* gate_at = at.template strip<G>(k.gate) + at.first() * k.gate.step;
+    char *const places = ring + at.warp * kBytes, *const end = places + kStages * at.warps * kBytes, *read = places, *write = places;
+    const int apart = at.warps * kBytes;
+    uint32_t t_load = at.first(), w_load = 0;
+    auto load = [&]() {
+        if (w_load < windows && t_load < length) {
+            const int rows = t_load < n ? static_cast<int>(min(n - t_load, uint32_t(kSteps))) : 0;
+            x.load(write, rows, at.lane);
+            gate.load(write + X::kPlace, rows, at.lane);
+        }
+        copies_commit();
+        x.next(), gate.next();
+        ++w_load, t_load += span;
+        write += apart;
+        if (write == end) write = places;
+    };
+    load();
+    float carry[1];
+    load_end<1>(carry, k.initial, at.b, at.ch, at.in);
+    struct Window {
+        float a[kSteps][1], b[kSteps][1], decay[1], sum[1];  // (decay, sum: of the segments in front of this one, in this block)
+        int left;
+        const char* place;
+    } next;
+    uint32_t t_first = at.first();
+    auto first = [&](uint32_t w) {
+        __syncwarp();
+        load();  // (where the window before the last one lay)
+        copies_wait<1>();
+        __syncwarp();
+        x.look(read, x_at);
+        gate.look(read + X::kPlace, gate_at);
+        if constexpr (X::kAround) x_at += x.jump;
+        if constexpr (Y::kAround) gate_at += gate.jump;
+        next.place = read;
+        read += apart;
+        if (read == end) read = places;
+        next.left = t_first < n ? static_cast<int>(min(n - t_first, uint32_t(kSteps))) : 0;
+        t_first += span;
+        Run<1> own;
+        take_steps<KIND, 1>(x, gate, at.lane, next.left, next.a, next.b, own);
+        const uint32_t parity = w & 1, slot = w % kAheadSlots;
+        float decay[1] = {own.decay(0)};
+        put_row<1>(told.segment(parity, at.warp), at.lane, decay);
+        put_row<1>(told.segment(parity, at.warp) + 32, at.lane, own.sum);
+        __syncthreads();
+        Run<1> before;
+        before.begin();
+        auto take = [&](int i) {
+            const float* const segment = told.segment(parity, i);
+            float c[1], sum[1];
+            get_row<1>(c, segment, at.lane);
+            get_row<1>(sum, segment + 32, at.lane);
+            before.then(c, sum);
+        };
+#pragma unroll
+        for (int i = 0; i < kWarps - 1; ++i) {
+            if (i < at.warp) take(i);
+        }
+        for (int i = kWarps - 1; i < at.warp; ++i) take(i);
+        next.decay[0] = before.decay(0), next.sum[0] = before.sum[0];
+        if (at.warp == at.warps - 1) {
+            const uint32_t bar = shared_address(&told.bars[slot]);
+            if (at.lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * 8u) : "memory");
+            before.then(decay, own.sum);
+            const float c[1] = {before.decay(0)};
+            for (uint32_t to = 0; to < cluster; ++to) {
+                const uint32_t there = in_block(shared_address(told.block(slot, at.rank) + at.lane), to), bar_there = in_block(bar, to);
+                tell<1>(there, bar_there, c);
+                tell<1>(there + 128, bar_there, before.sum);
+            }
+        }
+    };
+    first(0);
+    uint32_t t = at.first();
+    for (uint32_t w = 0; w < windows; ++w, t += span, out += out_jump) {
+        const Window now = next;
+        if (w + 1 < windows) first(w + 1);
+        const uint32_t slot = w % kAheadSlots;
+        wait_for(shared_address(&told.bars[slot]), w / kAheadSlots & 1, told.given_up, k.status);
+        float h[1];
+#pragma unroll
+        for (uint32_t j = 0; j < kMostCluster; ++j) {
+            if (j == at.rank) h[0] = carry[0];
+            if (j < cluster) pass<1>(carry, told.block(slot, j), at.lane);
+        }
+        apply_v(h, now.decay, now.sum);
+        if (t >= length) continue;
+        if (k.states != nullptr && at.in) Raw<float, 1>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
+        x.place = now.place;
+        put_steps<1>(x, at.lane, at.in, now.left, static_cast<int>(min(length - t, uint32_t(kSteps))), out, k.out.step, now.a, now.b, h);
+    }
+    if (k.final_state.base != nullptr && at.rank == 0 && at.warp == at.warps - 1 && at.in) store_end<1>(k.final_state, at.b, at.ch, carry);
+    end_cluster();
 }
 
 // CLUSTER: whether `blocks` of them may be a cluster.
@@ -789,7 +922,7 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
     __shared__ int given_up;
     const Told<VEC> told{reinterpret_cast<float*>(ring + blockDim.x / 32 * kStages * kBytes), static_cast<int>(blockDim.x / 32), bars, &given_up};
     pdl_prologue();
-    if (cluster > 1) begin_cluster(told);
+    if (cluster > 1) begin_cluster(told, 2);
     const Place<VEC> at(k, strips, cluster);
     const uint32_t length = static_cast<uint32_t>(k.length), n = static_cast<uint32_t>(steps_of(k, at.b)), span = at.span();
     const uint32_t windows = (length + span - 1) / span;
@@ -1059,7 +1192,7 @@ struct Typed {
     Stream s;
     int dtype;
 };
-Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams) {
+Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams, bool ahead) {
     Walk w;
     // Copies of 16 or of 4 bytes where every row lies on so many; two channels to a lane where every row has them side by side on an address for both.
     bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
@@ -1076,12 +1209,20 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
     w.vec = pairs && halves ? 2 : 1;
     w.chunk = halves && !pairs ? 2 : chunk;
     if (s.length <= kSteps) return w;
-    w.strips = ceil_div(s.width, 32 * w.vec);
     w.warps = static_cast<int>(std::min<int64_t>(kWarps, ceil_div(s.length, kSteps)));
     // Blocks that leave half of the device's places (two to an SM) empty share their sequences' windows with another one each: 50000 steps of 1000 channels, F32, 423 us with
     // blocks by themselves, 313, 188 and 151 by clusters of 2, 4 and 8; 4 sequences of 4096 steps, 2048 channels, F16, 74 and, by two, 56.  Further apart than that a
     // cluster costs more than it gives: 8 such sequences 84 us by themselves, 106 by two, 111 by four.
-    while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
+    auto spread = [&]() {
+        w.strips = ceil_div(s.width, 32 * w.vec);
+        w.cluster = 1;
+        while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
+    };
+    spread();
+    if (ahead && w.vec == 2 && w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2) {
+        w.vec = 1;
+        spread();
+    }
     w.alone = w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= sm_count() && s.length > int64_t(w.cluster) * w.warps * kSteps;
     w.blocks = s.batch * w.strips * w.cluster;
     return w;
@@ -1097,9 +1238,9 @@ void by_walk(const Walk& w, Fn&& go) {
 }
 
 template <int BYTES, int VEC, typename Kernel>
-void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, const Args& k) {
+void launch_walk(b200_ctx* ctx, Kernel kernel, const Walk& w, const Args& k, int slots = 2) {
     const int warps = w.alone && blocks_of(BYTES) == 2 ? kMostWarps : w.warps;
-    const size_t shared = static_cast<size_t>(warps) * stages_of(BYTES) * BYTES + Told<VEC>::bytes(warps, w.cluster > 1);
+    const size_t shared = static_cast<size_t>(warps) * stages_of(BYTES) * BYTES + Told<VEC>::bytes(warps, w.cluster > 1 ? slots : 0);
     const dim3 grid(static_cast<unsigned>(w.blocks)), threads(static_cast<unsigned>(32 * warps));
     (void)blocks_at_once(reinterpret_cast<const void*>(kernel), 32 * warps, shared);  // (allows that much shared memory)
     if (w.cluster == 1) launch_kernel(ctx, kernel, grid, threads, shared, k, static_cast<uint32_t>(w.strips), 1u);
@@ -1115,7 +1256,7 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
     k.initial = end_of(a.initial);
     k.final_state = end_of(a.final_state);
     ProfScope scope(ctx, "gated_recurrence");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}});
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}}, true);
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
@@ -1126,13 +1267,26 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
             };
             if (w.vec == 1) go(s.length <= 1 ? serial_kernel<T, G, KIND, 1, 1> : serial_kernel<T, G, KIND, 1, kSteps>, 1);
             else go(s.length <= 1 ? serial_kernel<T, G, KIND, 2, 1> : serial_kernel<T, G, KIND, 2, kSteps>, 2);
-        } else {
-            by_walk<T>(w, [&](auto vec, auto chunk) {
-                constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
-                constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>;
-                launch_walk<kBytes, VEC>(ctx, CHUNK == 16 && w.cluster == 1 ? walk_kernel<T, G, KIND, VEC, CHUNK, CHUNK != 16> : walk_kernel<T, G, KIND, VEC, CHUNK, true>, w, k);
-            });
+            return;
         }
+        if constexpr (sizeof(T) == 2) {
+            if (w.cluster > 1 && w.vec == 1) {
+                auto go = [&](auto chunk) {
+                    constexpr int CHUNK = decltype(chunk)::value;
+                    launch_walk<kWindowBytes<T, G, 1, CHUNK, false>, 1>(ctx, walk_ahead_kernel<T, G, KIND, CHUNK>, w, k, kAheadSlots);
+                };
+                if (w.chunk == 16) go(std::integral_constant<int, 16>{});
+                else if (w.chunk == 4) go(std::integral_constant<int, 4>{});
+                else go(std::integral_constant<int, 2>{});
+                return;
+            }
+        }
+        by_walk<T>(w, [&](auto vec, auto chunk) {
+            constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
+            constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, false>;
+            if constexpr (sizeof(T) == 2 && VEC == 1) launch_walk<kBytes, VEC>(ctx, walk_kernel<T, G, KIND, VEC, CHUNK, false>, w, k);
+            else launch_walk<kBytes, VEC>(ctx, CHUNK == 16 && w.cluster == 1 ? walk_kernel<T, G, KIND, VEC, CHUNK, CHUNK != 16> : walk_kernel<T, G, KIND, VEC, CHUNK, true>, w, k);
+        });
     });
     check_last_launch("gated_recurrence");
     ctx->count_launch();
@@ -1149,7 +1303,7 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
     k.initial = end_of(a.initial_grad);
     k.final_state = end_of(a.final_grad);
     ProfScope scope(ctx, "gated_recurrence_backward");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}});
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}}, false);
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
