@@ -523,6 +523,56 @@ __device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int
     }
 }
 
+// What a block's segments do to a state, told to the cluster: this warp's, and beside it (decay, sum) what those in front of it do.  Segments come in the order of their
+// warps and blocks, or (BACK) the other way round.
+template <bool BACK>
+__device__ __forceinline__ void tell_ahead(const Told<1>& told, uint32_t parity, uint32_t slot, int warp, int lane, uint32_t rank, uint32_t cluster, const Run<1>& own, float (&decay)[1], float (&sum)[1]) {
+    const int warps = told.warps;
+    const float mine[1] = {own.decay(0)};
+    put_row<1>(told.segment(parity, warp), lane, mine);
+    put_row<1>(told.segment(parity, warp) + 32, lane, own.sum);
+    __syncthreads();
+    const int in_front = BACK ? warps - 1 - warp : warp;
+    Run<1> before;
+    before.begin();
+    auto take = [&](int i) {
+        const float* const segment = told.segment(parity, BACK ? warps - 1 - i : i);
+        float c[1], s[1];
+        get_row<1>(c, segment, lane);
+        get_row<1>(s, segment + 32, lane);
+        before.then(c, s);
+    };
+#pragma unroll
+    for (int i = 0; i < kWarps - 1; ++i) {
+        if (i < in_front) take(i);
+    }
+    for (int i = kWarps - 1; i < in_front; ++i) take(i);
+    decay[0] = before.decay(0), sum[0] = before.sum[0];
+    if (in_front != warps - 1) return;
+    const uint32_t bar = shared_address(&told.bars[slot]);
+    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * 8u) : "memory");
+    before.then(mine, own.sum);
+    const float c[1] = {before.decay(0)};
+    for (uint32_t to = 0; to < cluster; ++to) {
+        const uint32_t there = in_block(shared_address(told.block(slot, rank) + lane), to), bar_there = in_block(bar, to);
+        tell<1>(there, bar_there, c);
+        tell<1>(there + 128, bar_there, before.sum);
+    }
+}
+// The state that comes into this warp's steps of window w, and `carry`, the state behind the window before it and then behind this one.
+template <bool BACK>
+__device__ __forceinline__ void hear_ahead(const Told<1>& told, uint32_t w, int lane, uint32_t rank, uint32_t cluster, uint32_t* status, const float (&decay)[1], const float (&sum)[1], float (&carry)[1],
+                                           float (&in)[1]) {
+    const uint32_t slot = w % kAheadSlots, ahead = BACK ? cluster - 1 - rank : rank;
+    wait_for(shared_address(&told.bars[slot]), w / kAheadSlots & 1, told.given_up, status);
+#pragma unroll
+    for (uint32_t j = 0; j < kMostCluster; ++j) {
+        if (j == ahead) in[0] = carry[0];
+        if (j < cluster) pass<1>(carry, told.block(slot, BACK ? cluster - 1 - j : j), lane);
+    }
+    apply_v(in, decay, sum);
+}
+
 // Where a thread works: its sequence, channels, and place in a window.
 template <int VEC>
 struct Place {
@@ -579,14 +629,19 @@ struct Steps {
     __device__ __forceinline__ void load(char* to, int rows, int lane) {
         const uint32_t place = shared_address(to);
         if constexpr (kAround) {
+            static_assert(kPieces < 32 && 2 * kPieces > 32);
+            asm volatile("" : "+r"(lane));  // (nine pieces' rows and offsets are counted for every window: kept, they would leave the steps too few registers)
+            int row = lane >= kPieces, off = (lane - row * kPieces) * kCopy;
+            const char *p = from + row * step, *const none = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3));
 #pragma unroll
             for (int i = 0; i < (kSteps * kPieces + 31) / 32; ++i) {
-                const int at = i * 32 + lane, row = at / kPieces, off = at % kPieces * kCopy;
-                if (row >= kSteps) break;
-                const char* p = from + row * step;
-                const int behind = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 2);  // bytes in front of the row's in its first word
-                const bool in = row < rows && off < valid + behind;
-                copy(place + at * kCopy, in ? p - behind + off : reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3)), in ? kCopy : 0);
+                if (row < kSteps) {
+                    const int behind = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 2);  // bytes in front of the row's in its first word
+                    const bool in = row < rows && off < valid + behind;
+                    copy(place + (i * 32 + lane) * kCopy, in ? p - behind + off : none, in ? kCopy : 0);
+                }
+                off += (32 - kPieces) * kCopy, ++row, p += step;
+                if (off >= kPieces * kCopy) off -= kPieces * kCopy, ++row, p += step;
             }
         } else if constexpr (kPieces <= 32) {
             constexpr int kRows = 32 / kPieces;  // of one copy of the warp's
@@ -661,7 +716,7 @@ struct Steps {
     }
 };
 // Windows in shared memory of a warp's `bytes` each: two or three, and two blocks of 8 warps on an SM (or one of 16) where they fit.
-constexpr int kFewBytes = 98304;
+constexpr int kFewBytes = 101376;
 __host__ __device__ constexpr int stages_of(int bytes) { return kWarps * bytes * 3 <= kFewBytes ? 3 : kWarps * bytes * 2 <= kFewBytes ? 2 : kWarps * bytes * 3 <= 2 * kFewBytes ? 3 : 2; }
 __host__ __device__ constexpr int blocks_of(int bytes) { return kWarps * bytes * stages_of(bytes) <= kFewBytes ? 2 : 1; }
 template <typename T, typename G, int VEC, int CHUNK, bool BACK>
@@ -813,8 +868,8 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, f
     gate.begin(at.template strip<G>(k.gate), k.gate.step, at.first(), span, at.valid(k.width, sizeof(G)), at.lane);
     char* out = X::first_piece(const_cast<char*>(at.template strip<T>(k.out)), k.out.step, at.first(), at.lane);
     const int64_t out_jump = span * k.out.step;
-    const char* x_at = at.template strip<T>(k.x) + at.first() * k.x.step;  // (of the window that is gone through the first time: X::kAround asks)
-    const char* gate_at = at.template strip<G>(k.gate) + at.first() * k.gate.step;
+    // (a window is 32 steps or more: what X::kAround asks of its address is the same for all)
+    const char *const x_at = at.template strip<T>(k.x) + at.first() * k.x.step, *const gate_at = at.template strip<G>(k.gate) + at.first() * k.gate.step;
     char *const places = ring + at.warp * kBytes, *const end = places + kStages * at.warps * kBytes, *read = places, *write = places;
     const int apart = at.warps * kBytes;
     uint32_t t_load = at.first(), w_load = 0;
@@ -846,8 +901,6 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, f
         __syncwarp();
         x.look(read, x_at);
         gate.look(read + X::kPlace, gate_at);
-        if constexpr (X::kAround) x_at += x.jump;
-        if constexpr (Y::kAround) gate_at += gate.jump;
         next.place = read;
         read += apart;
         if (read == end) read = places;
@@ -855,52 +908,15 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, f
         t_first += span;
         Run<1> own;
         take_steps<KIND, 1>(x, gate, at.lane, next.left, next.a, next.b, own);
-        const uint32_t parity = w & 1, slot = w % kAheadSlots;
-        float decay[1] = {own.decay(0)};
-        put_row<1>(told.segment(parity, at.warp), at.lane, decay);
-        put_row<1>(told.segment(parity, at.warp) + 32, at.lane, own.sum);
-        __syncthreads();
-        Run<1> before;
-        before.begin();
-        auto take = [&](int i) {
-            const float* const segment = told.segment(parity, i);
-            float c[1], sum[1];
-            get_row<1>(c, segment, at.lane);
-            get_row<1>(sum, segment + 32, at.lane);
-            before.then(c, sum);
-        };
-#pragma unroll
-        for (int i = 0; i < kWarps - 1; ++i) {
-            if (i < at.warp) take(i);
-        }
-        for (int i = kWarps - 1; i < at.warp; ++i) take(i);
-        next.decay[0] = before.decay(0), next.sum[0] = before.sum[0];
-        if (at.warp == at.warps - 1) {
-            const uint32_t bar = shared_address(&told.bars[slot]);
-            if (at.lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * 8u) : "memory");
-            before.then(decay, own.sum);
-            const float c[1] = {before.decay(0)};
-            for (uint32_t to = 0; to < cluster; ++to) {
-                const uint32_t there = in_block(shared_address(told.block(slot, at.rank) + at.lane), to), bar_there = in_block(bar, to);
-                tell<1>(there, bar_there, c);
-                tell<1>(there + 128, bar_there, before.sum);
-            }
-        }
+        tell_ahead<false>(told, w & 1, w % kAheadSlots, at.warp, at.lane, at.rank, cluster, own, next.decay, next.sum);
     };
     first(0);
     uint32_t t = at.first();
     for (uint32_t w = 0; w < windows; ++w, t += span, out += out_jump) {
         const Window now = next;
         if (w + 1 < windows) first(w + 1);
-        const uint32_t slot = w % kAheadSlots;
-        wait_for(shared_address(&told.bars[slot]), w / kAheadSlots & 1, told.given_up, k.status);
         float h[1];
-#pragma unroll
-        for (uint32_t j = 0; j < kMostCluster; ++j) {
-            if (j == at.rank) h[0] = carry[0];
-            if (j < cluster) pass<1>(carry, told.block(slot, j), at.lane);
-        }
-        apply_v(h, now.decay, now.sum);
+        hear_ahead<false>(told, w, at.lane, at.rank, cluster, k.status, now.decay, now.sum, carry, h);
         if (t >= length) continue;
         if (k.states != nullptr && at.in) Raw<float, 1>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         x.place = now.place;
@@ -908,6 +924,77 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, f
     }
     if (k.final_state.base != nullptr && at.rank == 0 && at.warp == at.warps - 1 && at.in) store_end<1>(k.final_state, at.b, at.ch, carry);
     end_cluster();
+}
+
+// The gradient of a step's result, of `left` steps that are the sequence's.
+template <int VEC, typename X>
+__device__ __forceinline__ void step_gradient(const X& dout, bool with_dout, int lane, int left, int j, float (&d)[VEC]) {
+    if (with_dout && j < left) {
+        dout.get(j, lane).get(d);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) d[e] = 0.f;
+}
+// The first walk through a window's steps, from the state h in front of them: their decays, what dgate takes of them, and what they do to a gradient that comes from behind.
+template <int KIND, int VEC, typename X, typename Y>
+__device__ __forceinline__ void take_back_steps(const X& x, const Y& gate, const X& dout, bool with_dout, int lane, int left, float (&h)[VEC], float (&c)[kSteps][VEC], float (&u)[kSteps][VEC],
+                                                Run<VEC>& own) {
+    own.begin();
+    auto take = [&](auto whole) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            float xs[VEC], gs[VEC], ds[VEC], a[VEC], d[VEC], input[VEC], b[VEC];
+            x.get(j, lane).get(xs);
+            gate.get(j, lane).get(gs);
+            step_gradient<VEC>(dout, with_dout, lane, left, j, ds);
+            if (!whole.value && j >= left) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
+            }
+            gates_of<KIND>(gs, c[j], a, d, input);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
+            mul_v(b, input, xs);
+            own.decays(a, d);
+            if constexpr (KIND == B200_GATES_EXP) own.stay_finite();
+            fma_v(own.sum, own.a, ds, own.sum);  // what the steps' gradients make of the state in front of them: each times the a's up to it
+            fma_v(h, a, h, b);  // (a's rounding counts within these steps only, here and below)
+        }
+    };
+    if (left == kSteps) take(std::true_type{});
+    else take(std::false_type{});
+}
+// The second one, from the gradient `later` behind them, to `rows` rows of the results.
+template <int KIND, int VEC, typename X, typename Y>
+__device__ __forceinline__ void put_back_steps(const X& x, const Y& gate, const X& dout, bool with_dout, int lane, bool there, int left, int rows, char* dx, char* dgate, int64_t dx_step, int64_t dgate_step, bool with_dx, bool with_dgate,
+                                               const float (&c)[kSteps][VEC], const float (&u)[kSteps][VEC], float (&later)[VEC]) {
+    auto put = [&](auto whole) {
+        char *to_x = dx + (kSteps - 1) * dx_step, *to_gate = dgate + (kSteps - 1) * dgate_step;
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j, to_x -= dx_step, to_gate -= dgate_step) {
+            float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC], a[VEC];
+            step_gradient<VEC>(dout, with_dout, lane, left, j, D);
+            add_v(D, D, later);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) slopes<KIND>(c[j][e], slope[e], input[e], a[e]);
+            mul_v(later, a, D);
+            mul_v(px, input, D);
+            mul_v(pg, slope, u[j]);
+            mul_v(pg, pg, D);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (!whole.value && j >= left) px[e] = pg[e] = 0.f;
+            }
+            const bool in = there && (whole.value || j < rows);
+            if (with_dx) x.put(j, lane, to_x, px, in);
+            if (with_dgate) gate.put(j, lane, to_gate, pg, in);
+        }
+    };
+    if (left == kSteps) put(std::true_type{});
+    else put(std::false_type{});
+    if (with_dx) x.store(dx, dx_step, rows, lane);
+    if (with_dgate) gate.store(dgate, dgate_step, rows, lane);
 }
 
 // CLUSTER: whether `blocks` of them may be a cluster.
@@ -984,74 +1071,119 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
         load();  // (where the window before lay)
         if (w + 1 < windows) load_state(t - span);
         Run<VEC> own;
-        own.begin();
         const int left = t < n ? static_cast<int>(min(n - t, uint32_t(kSteps))) : 0;  // steps of the sequence
-        auto gradient = [&](int j, float (&d)[VEC]) {
-            if (with_dout && j < left) {
-                dout.get(j, at.lane).get(d);
-                return;
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d[e] = 0.f;
-        };
-        auto take = [&](auto whole) {
-#pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                float xs[VEC], gs[VEC], ds[VEC], a[VEC], d[VEC], input[VEC], b[VEC];
-                x.get(j, at.lane).get(xs);
-                gate.get(j, at.lane).get(gs);
-                gradient(j, ds);
-                if (!whole.value && j >= left) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
-                }
-                gates_of<KIND>(gs, c[j], a, d, input);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
-                mul_v(b, input, xs);
-                own.decays(a, d);
-                if constexpr (KIND == B200_GATES_EXP) own.stay_finite();
-                fma_v(own.sum, own.a, ds, own.sum);  // what the steps' gradients make of the state in front of them: each times the a's up to it
-                fma_v(h, a, h, b);  // (a's rounding counts within these steps only, here and below)
-            }
-        };
-        if (left == kSteps) take(std::true_type{});
-        else take(std::false_type{});
+        take_back_steps<KIND, VEC>(x, gate, dout, with_dout, at.lane, left, h, c, u, own);
         float later[VEC];
         join<VEC, true>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, later, carry);
         if (t < length) {
             const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
-            auto put = [&](auto whole) {
-                char *to_x = dx + (kSteps - 1) * k.dx.step, *to_gate = dgate + (kSteps - 1) * k.dgate.step;
-#pragma unroll
-                for (int j = kSteps - 1; j >= 0; --j, to_x -= k.dx.step, to_gate -= k.dgate.step) {
-                    float D[VEC], px[VEC], pg[VEC], slope[VEC], input[VEC], a[VEC];
-                    gradient(j, D);
-                    add_v(D, D, later);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) slopes<KIND>(c[j][e], slope[e], input[e], a[e]);
-                    mul_v(later, a, D);
-                    mul_v(px, input, D);
-                    mul_v(pg, slope, u[j]);
-                    mul_v(pg, pg, D);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        if (!whole.value && j >= left) px[e] = pg[e] = 0.f;
-                    }
-                    const bool in = at.in && (whole.value || j < rows);
-                    if (with_dx) x.put(j, at.lane, to_x, px, in);
-                    if (with_dgate) gate.put(j, at.lane, to_gate, pg, in);
-                }
-            };
-            if (left == kSteps) put(std::true_type{});
-            else put(std::false_type{});
-            if (with_dx) x.store(dx, k.dx.step, rows, at.lane);
-            if (with_dgate) gate.store(dgate, k.dgate.step, rows, at.lane);
+            put_back_steps<KIND, VEC>(x, gate, dout, with_dout, at.lane, at.in, left, rows, dx, dgate, k.dx.step, k.dgate.step, with_dx, with_dgate, c, u, later);
         }
         dx -= int64_t(span) * k.dx.step, dgate -= int64_t(span) * k.dgate.step;
     }
     if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) store_end<VEC>(k.initial, at.b, at.ch, carry);
     if (cluster > 1) end_cluster();
+}
+
+// As walk_ahead_kernel.
+template <typename T, typename G, int KIND, int CHUNK>
+__global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, true>) == 2 ? kMostWarps : kWarps), 1) walk_backward_ahead_kernel(const Args k, uint32_t strips, uint32_t cluster) {
+    constexpr int kBytes = kWindowBytes<T, G, 1, CHUNK, true>, kStages = stages_of(kBytes);
+    static_assert(kStages == 3);
+    using X = Steps<T, 1, CHUNK>;
+    using Y = Steps<G, 1, CHUNK>;
+    extern __shared__ __align__(16) char ring[];
+    __shared__ uint64_t bars[kAheadSlots];
+    __shared__ int given_up;
+    const Told<1> told{reinterpret_cast<float*>(ring + blockDim.x / 32 * kStages * kBytes), static_cast<int>(blockDim.x / 32), bars, &given_up};
+    pdl_prologue();
+    begin_cluster(told, kAheadSlots);
+    const Place<1> at(k, strips, cluster);
+    const uint32_t length = static_cast<uint32_t>(k.length), n = static_cast<uint32_t>(steps_of(k, at.b)), span = at.span();
+    const uint32_t windows = (length + span - 1) / span;
+    // windows from the last on
+    uint32_t t = (windows - 1) * span + at.first(), t_load = t, t_first = t, w_load = 0;
+    X x, dout;
+    Y gate;
+    const bool with_dout = k.dout.base != nullptr;
+    x.begin(at.template strip<T>(k.x), k.x.step, t, -int64_t(span), at.valid(k.width, sizeof(T)), at.lane);
+    gate.begin(at.template strip<G>(k.gate), k.gate.step, t, -int64_t(span), at.valid(k.width, sizeof(G)), at.lane);
+    if (with_dout) dout.begin(at.template strip<T>(k.dout), k.dout.step, t, -int64_t(span), at.valid(k.width, sizeof(T)), at.lane);
+    const bool with_dx = k.dx.base != nullptr, with_dgate = k.dgate.base != nullptr;
+    char* dx = with_dx ? X::first_piece(const_cast<char*>(at.template strip<T>(k.dx)), k.dx.step, t, at.lane) : nullptr;
+    char* dgate = with_dgate ? Y::first_piece(const_cast<char*>(at.template strip<G>(k.dgate)), k.dgate.step, t, at.lane) : nullptr;
+    // (a window is 32 steps or more: what X::kAround asks of its address is the same for all)
+    const char *const x_at = at.template strip<T>(k.x) + t * k.x.step, *const gate_at = at.template strip<G>(k.gate) + t * k.gate.step;
+    const char* const dout_at = with_dout ? at.template strip<T>(k.dout) + t * k.dout.step : nullptr;
+    char *const places = ring + at.warp * kBytes, *const end = places + kStages * at.warps * kBytes, *read = places, *write = places;
+    const int apart = at.warps * kBytes;
+    auto look = [&](const char* place) {
+        x.look(place, x_at);
+        gate.look(place + X::kPlace, gate_at);
+        dout.look(place + X::kPlace + Y::kPlace, dout_at);
+    };
+    auto load = [&]() {
+        if (w_load < windows && t_load < length) {
+            const int rows = t_load < n ? static_cast<int>(min(n - t_load, uint32_t(kSteps))) : 0;
+            x.load(write, rows, at.lane);
+            gate.load(write + X::kPlace, rows, at.lane);
+            if (with_dout) dout.load(write + X::kPlace + Y::kPlace, rows, at.lane);
+        }
+        copies_commit();
+        x.next(), gate.next();
+        if (with_dout) dout.next();
+        ++w_load, t_load -= span;
+        write += apart;
+        if (write == end) write = places;
+    };
+    load();
+    const float* const states = k.states + int64_t(at.b) * k.chunks * k.width + at.ch;
+    Raw<float, 1> rh;  // the state in front of the next window's steps
+    auto load_state = [&](uint32_t t) {
+        rh.clear();
+        if (at.in && t < n) rh.load(reinterpret_cast<const char*>(states + int64_t(t / kSteps) * k.width));
+    };
+    load_state(t);
+    float carry[1];
+    load_end<1>(carry, k.final_state, at.b, at.ch, at.in);
+    struct Window {
+        float c[kSteps][1], u[kSteps][1], decay[1], sum[1];  // (decay, sum: of the segments behind this one, in this block)
+        int left;
+        const char* place;
+    } next;
+    auto first = [&](uint32_t w) {
+        float h[1];
+        rh.get(h);
+        __syncwarp();
+        load();  // (where the window before the last one lay)
+        copies_wait<1>();
+        __syncwarp();
+        look(read);
+        next.place = read;
+        read += apart;
+        if (read == end) read = places;
+        next.left = t_first < n ? static_cast<int>(min(n - t_first, uint32_t(kSteps))) : 0;
+        t_first -= span;
+        if (w + 1 < windows) load_state(t_first);
+        Run<1> own;
+        take_back_steps<KIND, 1>(x, gate, dout, with_dout, at.lane, next.left, h, next.c, next.u, own);
+        tell_ahead<true>(told, w & 1, w % kAheadSlots, at.warp, at.lane, at.rank, cluster, own, next.decay, next.sum);
+    };
+    first(0);
+    for (uint32_t w = 0; w < windows; ++w, t -= span) {
+        const Window now = next;
+        if (w + 1 < windows) first(w + 1);
+        float later[1];
+        hear_ahead<true>(told, w, at.lane, at.rank, cluster, k.status, now.decay, now.sum, carry, later);
+        if (t < length) {
+            look(now.place);
+            put_back_steps<KIND, 1>(x, gate, dout, with_dout, at.lane, at.in, now.left, static_cast<int>(min(length - t, uint32_t(kSteps))), dx, dgate, k.dx.step, k.dgate.step, with_dx, with_dgate, now.c,
+                                    now.u, later);
+        }
+        dx -= int64_t(span) * k.dx.step, dgate -= int64_t(span) * k.dgate.step;
+    }
+    if (k.initial.base != nullptr && at.rank == 0 && at.warp == 0 && at.in) store_end<1>(k.initial, at.b, at.ch, carry);
+    end_cluster();
 }
 
 // ---- arguments --------------------------------------------------------------
@@ -1192,7 +1324,7 @@ struct Typed {
     Stream s;
     int dtype;
 };
-Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams, bool ahead) {
+Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams) {
     Walk w;
     // Copies of 16 or of 4 bytes where every row lies on so many; two channels to a lane where every row has them side by side on an address for both.
     bool pairs = s.width % 2 == 0 && reinterpret_cast<uintptr_t>(k.states) % 8 == 0, halves = false;
@@ -1219,7 +1351,7 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
         while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
     };
     spread();
-    if (ahead && w.vec == 2 && w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2) {
+    if (w.vec == 2 && w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2) {
         w.vec = 1;
         spread();
     }
@@ -1235,6 +1367,14 @@ void by_walk(const Walk& w, Fn&& go) {
     if (w.chunk == 16) go(std::integral_constant<int, kVec>{}, std::integral_constant<int, 16>{});
     else if (w.chunk == 4) go(std::integral_constant<int, kVec>{}, std::integral_constant<int, 4>{});
     else if constexpr (kVec == 2) go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+}
+
+// ... and go(CHUNK), of halves.
+template <typename Fn>
+void by_chunk(const Walk& w, Fn&& go) {
+    if (w.chunk == 16) go(std::integral_constant<int, 16>{});
+    else if (w.chunk == 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 2>{});
 }
 
 template <int BYTES, int VEC, typename Kernel>
@@ -1256,7 +1396,7 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
     k.initial = end_of(a.initial);
     k.final_state = end_of(a.final_state);
     ProfScope scope(ctx, "gated_recurrence");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}}, true);
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.out, a.out.dtype}});
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
@@ -1271,13 +1411,10 @@ void launch_forward(b200_ctx* ctx, const b200_recurrence_args& a) {
         }
         if constexpr (sizeof(T) == 2) {
             if (w.cluster > 1 && w.vec == 1) {
-                auto go = [&](auto chunk) {
+                by_chunk(w, [&](auto chunk) {
                     constexpr int CHUNK = decltype(chunk)::value;
                     launch_walk<kWindowBytes<T, G, 1, CHUNK, false>, 1>(ctx, walk_ahead_kernel<T, G, KIND, CHUNK>, w, k, kAheadSlots);
-                };
-                if (w.chunk == 16) go(std::integral_constant<int, 16>{});
-                else if (w.chunk == 4) go(std::integral_constant<int, 4>{});
-                else go(std::integral_constant<int, 2>{});
+                });
                 return;
             }
         }
@@ -1303,7 +1440,7 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
     k.initial = end_of(a.initial_grad);
     k.final_state = end_of(a.final_grad);
     ProfScope scope(ctx, "gated_recurrence_backward");
-    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}}, false);
+    const Walk w = walk_of(s, k, {{k.x, a.x.dtype}, {k.gate, a.gate.dtype}, {k.dout, a.x.dtype}, {k.dx, a.x.dtype}, {k.dgate, a.gate.dtype}});
     by_type(a.x, a.gate, a.kind, [&](auto t, auto g, auto kind) {
         using T = decltype(t);
         using G = decltype(g);
@@ -1314,13 +1451,23 @@ void launch_backward(b200_ctx* ctx, const b200_recurrence_grad_args& a) {
             };
             if (w.vec == 1) go(s.length <= 1 ? serial_backward_kernel<T, G, KIND, 1, 1> : serial_backward_kernel<T, G, KIND, 1, kSteps>, 1);
             else go(s.length <= 1 ? serial_backward_kernel<T, G, KIND, 2, 1> : serial_backward_kernel<T, G, KIND, 2, kSteps>, 2);
-        } else {
-            by_walk<T>(w, [&](auto vec, auto chunk) {
-                constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
-                constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, true>;
-                launch_walk<kBytes, VEC>(ctx, CHUNK == 16 && w.cluster == 1 ? walk_backward_kernel<T, G, KIND, VEC, CHUNK, CHUNK != 16> : walk_backward_kernel<T, G, KIND, VEC, CHUNK, true>, w, k);
-            });
+            return;
         }
+        if constexpr (sizeof(T) == 2) {
+            if (w.cluster > 1 && w.vec == 1) {
+                by_chunk(w, [&](auto chunk) {
+                    constexpr int CHUNK = decltype(chunk)::value;
+                    launch_walk<kWindowBytes<T, G, 1, CHUNK, true>, 1>(ctx, walk_backward_ahead_kernel<T, G, KIND, CHUNK>, w, k, kAheadSlots);
+                });
+                return;
+            }
+        }
+        by_walk<T>(w, [&](auto vec, auto chunk) {
+            constexpr int VEC = decltype(vec)::value, CHUNK = decltype(chunk)::value;
+            constexpr int kBytes = kWindowBytes<T, G, VEC, CHUNK, true>;
+            if constexpr (sizeof(T) == 2 && VEC == 1) launch_walk<kBytes, VEC>(ctx, walk_backward_kernel<T, G, KIND, VEC, CHUNK, false>, w, k);
+            else launch_walk<kBytes, VEC>(ctx, CHUNK == 16 && w.cluster == 1 ? walk_backward_kernel<T, G, KIND, VEC, CHUNK, CHUNK != 16> : walk_backward_kernel<T, G, KIND, VEC, CHUNK, true>, w, k);
+        });
     });
     check_last_launch("gated_recurrence_backward");
     ctx->count_launch();
