@@ -8,7 +8,7 @@
 // Bound by memory: z read once, and backward as much written.  A block takes a row after another: each thread keeps the maximum of what it has read and the sums of
 // e^u and e^u u beside it, and the block joins these threes.  What comes next, of this row or the next one, is on its way into registers all the while, so that a
 // row's end holds up nothing that is read.  (Through shared memory, by asynchronous copies, a row's end cost more than the registers do: 4096 x 32000 F16 95 us in place
-// of 55.)  Few long rows are a cluster's each, whose blocks take a part of it.  2047 x 128000 F32: 156 us, 6.7 TB/s; 4096 x 32000 F16: 54 us, 4.9 TB/s, bound by the
+// of 53.)  Few long rows are a cluster's each, whose blocks take a part of it.  2047 x 128000 F32: 154 us, 6.8 TB/s; 4096 x 32000 F16: 53 us, 4.9 TB/s, bound by the
 // exponential, the two sums and the conversion of each element.
 //
 // The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least
@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kMostTop = B200_MOST_TOP;
 constexpr int kMostThreads = 512;
+__host__ __device__ constexpr int threads_on_sm(int threads) { return threads < 256 ? 896 : 768; }  // by their registers, in blocks of so many
 constexpr int kBatch = 4;    // vectors that a thread takes at once
 constexpr int kMostBlocks = 8;  // of a cluster
 constexpr int kStretches = 16;   // of a thread's batches
@@ -265,7 +266,7 @@ __device__ __forceinline__ void rank_entries(const Args& k, uint32_t r, const Pa
 
 // `blocks`: of a row's cluster (1: the blocks take row after row).
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS < 256 ? 896 / THREADS : 768 / THREADS) logprobs_kernel(const Args k, uint32_t blocks) {
+__global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) logprobs_kernel(const Args k, uint32_t blocks) {
     constexpr int E = 16 / sizeof(T), kWarps = THREADS / 32, kChunk = THREADS * kBatch;  // (vectors of a chunk)
     extern __shared__ __align__(16) char shared[];
     __shared__ Part parts[2][kWarps];
@@ -739,30 +740,31 @@ void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
     ProfScope scope(ctx, "token_logprobs");
     const bool half = a.logits.dtype == B200_F16;
     const int64_t vectors = ceil_div(plan.vocab, half ? 8 : 4);
-    // Threads of a block: 32 vectors to each, as a row's end costs a thread as much as 4 of them or more, up to 64 (2047 x 128000 F32: 156 us, 161 with 128, 171 with 256), or
-    // 128 where entries are wanted, which are found by stretches of a thread each (the 20 largest of 2048 x 128000 F32: 188 us with 64, 179 with 128, 195 with 256); and
-    // more threads than entries.  Few rows: up to 512 threads of four vectors, and long ones a cluster of blocks each (1 x 128000 F32 6.2 us, 8.7 by one block; 16 x 128000
-    // F16 with the 20 largest 11.7 and 12.8).
-    const bool few = plan.s.rows <= sm_count();
+    // Threads of a block: as many as the rows leave room for on the device, of four vectors or more, up to 256 (300 x 128000 F32: 31 us, 98 with 64; 1024 x 128000 83 and
+    // 95), or 512 where each row has an SM.  Many rows: 32 vectors to a thread, as a row's end costs it as much as 4 of them or more, up to 64 threads (2047 x 128000 F32:
+    // 156 us, 161 with 128, 171 with 256), or 128 where entries are wanted, which are found by stretches of a thread each (the 20 largest of 2048 x 128000 F32: 188 us with
+    // 64, 179 with 128, 195 with 256).  And more threads than entries.  Few long rows are a cluster's each (1 x 128000 F32 6.2 us, 8.7 by one block; 16 x 128000 F16 with
+    // the 20 largest 11.7 and 12.8).
+    const int64_t rows = plan.s.rows, sms = sm_count();
     int threads = 32, blocks = 1;
-    while (threads < kMostThreads && ((vectors > int64_t(threads) * (few ? 4 : 32) && (few || threads < (plan.top > 0 ? 128 : 64))) || plan.top * 2 > threads)) threads *= 2;
-    while (blocks < kMostBlocks && plan.s.rows * blocks * 2 <= sm_count() && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
+    while (threads < (rows <= sms ? kMostThreads : kMostThreads / 2) && vectors > int64_t(threads) * 4 && rows * threads * 2 <= sms * threads_on_sm(threads * 2)) threads *= 2;
+    while ((threads < (plan.top > 0 ? 128 : 64) && vectors > int64_t(threads) * 32) || plan.top * 2 > threads) threads *= 2;
+    while (blocks < kMostBlocks && rows * blocks * 2 <= sms && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
     auto go = [&](auto kernel) {
         size_t shared = 0;
         if (k.top > 0) shared += (static_cast<size_t>(room_for(k.top)) + (blocks > 1 ? static_cast<size_t>(blocks) * k.top : 0)) * 8 + static_cast<size_t>(threads) * (4 + 6 * kStretches);
         const int most = blocks_at_once(reinterpret_cast<const void*>(kernel), threads, shared);
         if (blocks > 1) {
-            launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(plan.s.rows * blocks)), dim3(threads), shared, blocks, false, k, static_cast<uint32_t>(blocks));
+            launch_kernel_clustered(ctx, kernel, dim3(static_cast<unsigned>(rows * blocks)), dim3(threads), shared, blocks, false, k, static_cast<uint32_t>(blocks));
             return;
         }
         // Blocks that stay: as many on an SM as leave the fewest without a last row, down to three quarters.
-        const int64_t sms = sm_count();
-        auto rounds = [&](int on_sm) { return ceil_div(plan.s.rows, sms * on_sm) * on_sm; };
+        auto rounds = [&](int on_sm) { return ceil_div(rows, sms * on_sm) * on_sm; };
         int on_sm = most;
         for (int n = most - 1; n * 4 >= most * 3; --n) {
             if (rounds(n) < rounds(on_sm)) on_sm = n;
         }
-        launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(std::min<int64_t>(plan.s.rows, sms * on_sm))), dim3(threads), shared, k, 1u);
+        launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(std::min<int64_t>(rows, sms * on_sm))), dim3(threads), shared, k, 1u);
     };
     auto with = [&](auto element) {
         using T = decltype(element);

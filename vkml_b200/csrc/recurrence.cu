@@ -846,7 +846,8 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
 
 // Clusters whose lanes have a channel each: what a window's segments do to a state is told a window ahead, so that the wait for the other blocks is one for what was sent
 // while this window was gone through the first time.  (Two windows' steps in registers, and four places to be told at: a block that is told of the fourth window from here has
-// told this one's cluster of the second, behind its reading of this one.)
+// told this one's cluster of the second, behind its reading of this one.)  For halves: 32768 steps of 1024 channels 80 us, 103 with a wait in every window.  In F32 its
+// second window in registers costs what it saves (50000 steps of 1000 channels 160 us, 150 without).
 template <typename T, typename G, int KIND, int CHUNK>
 __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, false>) == 2 ? kMostWarps : kWarps), 1) walk_ahead_kernel(const Args k, uint32_t strips, uint32_t cluster) {
     constexpr int kBytes = kWindowBytes<T, G, 1, CHUNK, false>, kStages = stages_of(kBytes);
@@ -1351,6 +1352,8 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
         while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
     };
     spread();
+    // Half empty still: a channel to a lane, twice the blocks (1 sequence of 32768 steps, 1024 channels, F16: 80 us, 113 with two; its gradient 128 and 184).  Where two to a lane
+    // leave less empty they are the faster ones (1 and 2 of 4096 steps, 2048 channels: 20.6 and 33 us, 22.6 and 41 with one).
     if (w.vec == 2 && w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2) {
         w.vec = 1;
         spread();
