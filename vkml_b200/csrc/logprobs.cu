@@ -531,8 +531,8 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
 
 // ---- the gradient -----------------------------------------------------------
 //
-// A thread takes four vectors, all of them asked for before the first is worked on; a row is as many blocks' as that makes.  2048 x 50001 F16: 75 us (5.5 TB/s; one
-// exponential to an element); 4096 x 32000 F16 90 us (5.8 TB/s).
+// A thread takes four vectors, all of them asked for before the first is worked on; a row is as many threads' of a block, or blocks', as that makes.  2048 x 50001 F16:
+// 75 us (5.5 TB/s; one exponential to an element); 4096 x 32000 F16 88 us (6.0 TB/s); 100000 x 256 F16 46 us, 226 by a block for each row.
 
 constexpr int kGradThreads = 256;
 constexpr int kGradVectors = 4;
@@ -548,12 +548,14 @@ __device__ __forceinline__ float grad_of(const RowGrad& g, float inverse, float 
     return fast_exp2(log_q * kLog2e) * fmaf(g.turned, log_q, g.plain);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const Args k, uint32_t pieces) {
+// SHORT: a block is several rows', 2^bits threads each.
+template <typename T, bool SHORT>
+__global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const Args k, uint32_t pieces, int bits) {
     constexpr int E = 16 / sizeof(T);
     pdl_prologue();
-    const int tid = threadIdx.x;
-    const uint32_t r = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+    const int threads = SHORT ? 1 << bits : kGradThreads, tid = static_cast<int>(threadIdx.x) & (threads - 1);
+    const uint32_t r = SHORT ? blockIdx.x * (kGradThreads >> bits) + (threadIdx.x >> bits) : blockIdx.x / pieces, piece = SHORT ? 0 : blockIdx.x % pieces;
+    if (SHORT && r >= k.rows) return;
     const T* const z = reinterpret_cast<const T*>(row_at(k.logits, k.inner, r));
     T* const to = reinterpret_cast<T*>(row_at(k.grad, k.inner, r));
     const int head = head_of(z, k.vocab);
@@ -586,16 +588,16 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_kernel(const Args 
         if (tid >= 8 && column < k.vocab) to[column] = from_float<T>(value(zero ? 0.f : to_float(z[column]), column));
     }
     const uint4* const zv = reinterpret_cast<const uint4*>(z + head);
-    const int64_t first = int64_t(piece) * (kGradThreads * kGradVectors) + tid;
+    const int64_t first = int64_t(piece) * (threads * kGradVectors) + tid;
     uint4 raw[kGradVectors];
 #pragma unroll
     for (int i = 0; i < kGradVectors; ++i) {
-        const int64_t v = first + i * kGradThreads;
+        const int64_t v = first + i * threads;
         raw[i] = !zero && v < vectors ? zv[v] : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < kGradVectors; ++i) {
-        const int64_t v = first + i * kGradThreads;
+        const int64_t v = first + i * threads;
         if (v >= vectors) break;
         float x[E];
         unpack<T>(raw[i], x);
@@ -706,10 +708,16 @@ Plan check_logprobs(const b200_token_logprobs_args& a, bool forward) {
     return plan;
 }
 
-// Blocks that a row's gradient takes.
+// Pieces of a row's gradient, and the threads of one: a warp's at least, a block's at most.
 int64_t grad_pieces(int64_t vocab, bool half) {
     const int64_t vectors = vocab / (half ? 8 : 4);
     return std::max<int64_t>(1, ceil_div(vectors, kGradThreads * kGradVectors));
+}
+int grad_bits(int64_t vocab, bool half) {
+    const int64_t vectors = vocab / (half ? 8 : 4);
+    int bits = 5;
+    while (1 << bits < kGradThreads && vectors > int64_t(kGradVectors) << bits) ++bits;
+    return bits;
 }
 
 Args common_args(b200_ctx* ctx, const b200_token_logprobs_args& a, const Plan& plan) {
@@ -787,6 +795,7 @@ void launch_logprobs_backward(b200_ctx* ctx, const b200_token_logprobs_args& a) 
     if (plan.s.rows == 0) return;
     const bool half = a.logits.dtype == B200_F16;
     const int64_t pieces = grad_pieces(plan.vocab, half);
+    const int bits = grad_bits(plan.vocab, half);
     if (plan.s.rows * pieces >= (int64_t(1) << 31)) fail(B200_SHAPE_ERROR, "token_logprobs_backward: too many rows of this length");
     wait_for_tensors(ctx, {&a.logits, &a.tokens, &a.stats, &a.logprobs_grad, &a.entropies_grad, &a.grad});
     Args k = common_args(ctx, a, plan);
@@ -795,7 +804,12 @@ void launch_logprobs_backward(b200_ctx* ctx, const b200_token_logprobs_args& a) 
     k.grad = rows_arg(a.grad, plan.axes);
     k.scale = a.grad_scale / a.temperature;
     ProfScope scope(ctx, "token_logprobs_backward");
-    launch_kernel(ctx, half ? logprobs_grad_kernel<__half> : logprobs_grad_kernel<float>, dim3(static_cast<unsigned>(plan.s.rows * pieces)), dim3(kGradThreads), 0, k, static_cast<uint32_t>(pieces));
+    auto go = [&](auto kernel) {
+        launch_kernel(ctx, kernel, dim3(static_cast<unsigned>(ceil_div(plan.s.rows * pieces, kGradThreads >> bits))), dim3(kGradThreads), 0, k, static_cast<uint32_t>(pieces), bits);
+    };
+    const bool shorts = 1 << bits < kGradThreads;
+    if (half) go(shorts ? logprobs_grad_kernel<__half, true> : logprobs_grad_kernel<__half, false>);
+    else go(shorts ? logprobs_grad_kernel<float, true> : logprobs_grad_kernel<float, false>);
     check_last_launch("token_logprobs_backward");
     ctx->count_launch();
 }
