@@ -119,6 +119,34 @@ def test_forbidden_and_equal_logits(backend, dtype, vocab, top):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("size,temperature", [(30, 1.0), (30, 0.02), (30000, 0.2), (30000, 400.0), (0.01, 1e-3), (5, 1e30)])
+def test_rows_that_rise(backend, dtype, size, temperature):
+    """Each stretch's largest logit above the last one's, from far below or far above zero; and the other way round."""
+    vocab = 40003
+    rng = np.random.default_rng(3)
+    z = np.linspace(-size, size, vocab) + rng.standard_normal((6, vocab)) * size / 50
+    z[1::2] = z[1::2, ::-1]
+    z[2:4] += size
+    z[4:] -= size
+    z = z.astype(dtype)
+    tokens = z.astype(F32).argmax(1)
+    tokens[0] = 17
+    got = forward(backend, z, tokens, temperature, 5)
+    compare(got, z, tokens, temperature, 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rows,vocab,top,layout", [(160, 9001, 0, "offset"), (160, 9001, 20, "dense"), (400, 5000, 128, "dense"), (700, 2600, 7, "odd"), (149, 70000, 3, "dense")])
+def test_rows_that_leave_room(backend, dtype, rows, vocab, top, layout):
+    """More rows than SMs and fewer than the device holds blocks of a few warps."""
+    rng = np.random.default_rng(rows + top)
+    z = placed((rng.standard_normal((rows, vocab), dtype=F32) * 2.5).astype(dtype), layout)
+    tokens = rng.integers(0, vocab, rows)
+    some = np.unique(np.concatenate([[0, 147, 148, rows - 1], rng.integers(0, rows, 8)]))
+    compare(forward(backend, z, tokens, 1.0, top, layout=layout), z, tokens, 1.0, top, some)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("vocab", [9, 3000, 70001])
 def test_rows_that_hold_no_numbers(backend, dtype, vocab):
     """+inf and not-a-number: no numbers where the formulas have none, the neighbours untouched, the top in order."""

@@ -100,6 +100,18 @@ def test_lengths_outside(backend):
     check(space.get(final)[0], *want["final"], F32, "final")
 
 
+@pytest.mark.parametrize("types", [(F16, F16), (F16, F32)])
+@pytest.mark.parametrize("kind", ["sigmoid", "exp"])
+@pytest.mark.parametrize("shape,layout", [((1, 9300, 64), "dense"), ((2, 5300, 34), "dense"), ((1, 6200, 33), "odd"), ((2, 10500, 72), "pitch")])
+def test_few_channels_of_long_sequences(backend, types, kind, shape, layout):
+    """Clusters that tell each other of window after window; sequences that end in an early one, for whose later blocks nothing is left."""
+    rng = np.random.default_rng(shape[1])
+    x, gate, initial = problem(rng, shape, types, kind)
+    dout, dfinal = rng.standard_normal(shape).astype(types[0]), rng.standard_normal(initial.shape).astype(F32)
+    lengths = np.array([shape[1] - 5, 1100][: shape[0]], np.int64)
+    run(backend, placed(x, layout), placed(gate, layout), initial, lengths, kind, layout, placed(dout, layout), dfinal)
+
+
 @pytest.mark.parametrize("shape", [(2, 1, 64), (2, 70, 64), (1, 1500, 33)])
 @pytest.mark.parametrize("dtype", [F32, F16])
 def test_results_over_inputs(backend, shape, dtype):
