@@ -415,14 +415,17 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
             }
             __syncthreads();
             uint32_t lo = least;
-            // (order, column) of a vector's elements, where one of them reaches the bound.
+            // (order, column) of a vector's elements that reach the bound, and, of one that is no number, others.
             auto each = [&](int v, uint32_t bound, auto&& visit) {
                 const uint4 raw[1] = {row.vectors()[v]};
-                if (order_of(largest<T>(raw)) < bound) return;
+                const float at_least = value_of(bound);
+                if (largest<T>(raw) < at_least) return;
                 float x[E];
                 unpack<T>(raw[0], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) visit(order_of(x[e]), static_cast<uint32_t>(row.head + v * E + e));
+                for (int e = 0; e < E; ++e) {
+                    if (!(x[e] < at_least)) visit(order_of(x[e]), static_cast<uint32_t>(row.head + v * E + e));
+                }
             };
             auto counted = [&](uint32_t bound) {  // how many of the elements reach a bound
                 int some = 0;
@@ -442,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
                     if (i < room) entries[i] = uint64_t(o) << 32 | (0xffffffffu - column);
                 };
                 for (int s = 0; s < stretch && own >= bound; ++s) {
-                    if (order_of(stretch_tops[s * THREADS + tid]) >= bound) stretch_list[atomicAdd(&found, 1)] = static_cast<uint16_t>(s * THREADS + tid);
+                    if (!(stretch_tops[s * THREADS + tid] < value_of(bound))) stretch_list[atomicAdd(&found, 1)] = static_cast<uint16_t>(s * THREADS + tid);
                 }
                 if (end >= 0) put(order_of(end_z), static_cast<uint32_t>(end));
                 __syncthreads();
@@ -750,13 +753,15 @@ void launch_logprobs(b200_ctx* ctx, const b200_token_logprobs_args& a) {
     const int64_t vectors = ceil_div(plan.vocab, half ? 8 : 4);
     // Threads of a block: as many as the rows leave room for on the device, of four vectors or more, up to 256 (300 x 128000 F32: 31 us, 98 with 64; 1024 x 128000 83 and
     // 95), or 512 where each row has an SM.  Many rows: 32 vectors to a thread, as a row's end costs it as much as 4 of them or more, up to 64 threads (2047 x 128000 F32:
-    // 156 us, 161 with 128, 171 with 256), or 128 where entries are wanted, which are found by stretches of a thread each (the 20 largest of 2048 x 128000 F32: 188 us with
-    // 64, 179 with 128, 195 with 256).  And more threads than entries.  Few long rows are a cluster's each (1 x 128000 F32 6.2 us, 8.7 by one block; 16 x 128000 F16 with
+    // 156 us, 161 with 128, 171 with 256), or 128 where entries are wanted and a thread's stretch would be more than one batch (the 20 largest of 2048 x 128000 F32: 188 us
+    // with 64, 179 with 128, 195 with 256; of 4096 x 32000 F16 68 and 72).  And more threads than entries.  Few long rows are a cluster's each (1 x 128000 F32 6.2 us, 8.7 by one block; 16 x 128000 F16 with
     // the 20 largest 11.7 and 12.8).
     const int64_t rows = plan.s.rows, sms = sm_count();
     int threads = 32, blocks = 1;
     while (threads < (rows <= sms ? kMostThreads : kMostThreads / 2) && vectors > int64_t(threads) * 4 && rows * threads * 2 <= sms * threads_on_sm(threads * 2)) threads *= 2;
-    while ((threads < (plan.top > 0 ? 128 : 64) && vectors > int64_t(threads) * 32) || plan.top * 2 > threads) threads *= 2;
+    while (threads < 64 && vectors > int64_t(threads) * 32) threads *= 2;
+    if (plan.top > 0 && threads == 64 && vectors > int64_t(threads) * kBatch * kStretches) threads = 128;
+    while (plan.top * 2 > threads) threads *= 2;
     while (blocks < kMostBlocks && rows * blocks * 2 <= sms && vectors >= int64_t(threads) * blocks * 8) blocks *= 2;
     auto go = [&](auto kernel) {
         size_t shared = 0;
