@@ -365,6 +365,8 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
             take<T>(part, one, end_z, c, above);
             most = max_nan(most, end_z);
         }
+        const uint32_t own = end >= 0 || row.first + tid < row.last ? order_of(most) : 0u;  // (0: this thread has no element)
+        if (k.top > 0) tops[tid] = own;
         Part all = warp_part(part, most, c);
         if constexpr (kWarps > 1) {
             if (tid % 32 == 0) parts[parity][tid / 32] = all;
@@ -381,15 +383,14 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
         }
         int n = 0;
         if (k.top > 0) {
-            const bool owner = end >= 0 || row.first + tid < row.last;
-            const uint32_t own = owner ? order_of(most) : 0u;
-            tops[tid] = own;
-            if (tid == 0) count = 0, found = 0;
-            __syncthreads();
-            if (tid < 32) {  // a bound that at least `top` elements reach, if there are as many threads that have any
+            if (tid == 0) {
+                count = 0, found = 0;
+                if (blocks == 1) write_row(k, r, all, token, token_z);
+            }
+            if (tid >= THREADS - 32) {  // (the last warp:) a bound that at least `top` elements reach, if there are as many threads that have any
                 uint32_t x[kWarps];
 #pragma unroll
-                for (int i = 0; i < kWarps; ++i) x[i] = tops[i * 32 + tid];
+                for (int i = 0; i < kWarps; ++i) x[i] = tops[i * 32 + tid % 32];
                 auto reaching = [&](uint32_t bound) {
                     int some = 0;
 #pragma unroll
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
                     else high = mid;
                     if (reach >= k.top && reach <= k.top + k.top / 8) break;
                 }
-                if (tid == 0) least = low;
+                if (tid == THREADS - 1) least = low;
             }
             __syncthreads();
             uint32_t lo = least;
@@ -508,7 +509,6 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
             }
         }
         if (blocks == 1) {
-            if (tid == 0) write_row(k, r, all, token, token_z);
             rank_entries(k, r, all, entries, n, nullptr);
         } else {
             // the first block takes what the others found: their parts, and as many entries as are wanted of each
