@@ -206,6 +206,50 @@ def test_captured_and_replayed(backend):
         rt("cudaStreamDestroy", stream)
 
 
+def test_long_sequences_beside_each_other(backend):
+    """Clusters of several graphs on the device at once, many windows each, a state that is carried on from replay to replay: the eager calls' bits."""
+    rt = runtime()
+
+    def prepared(seed):
+        rng = np.random.default_rng(seed)
+        length, width = (9300, 64) if seed % 2 else (7001, 33)
+        s = {k: tensor(backend, rng.standard_normal((1, length, width)).astype(F16)) for k in ("x", "gate", "dout")}
+        s["state"] = tensor(backend, rng.standard_normal((1, width)).astype(F32))
+        for k, dims, dtype in (("out", (1, length, width), DType.F16), ("states", (1, -(-length // 16), width), DType.F32), ("dx", (1, length, width), DType.F16),
+                               ("dgate", (1, length, width), DType.F16), ("dstate", (1, width), DType.F32)):
+            s[k] = DeviceTensor.empty(backend, dims, dtype)
+        return s
+
+    def calls(s):
+        backend.gated_recurrence(s["x"], s["gate"], s["out"], initial=s["state"], final=s["state"], states=s["states"])
+        backend.gated_recurrence_backward(s["x"], s["gate"], s["states"], out_grad=s["dout"], x_grad=s["dx"], gate_grad=s["dgate"], initial_grad=s["dstate"])
+
+    seeds, rounds = (0, 1, 2, 3), 4
+    problems, same = [prepared(i) for i in seeds], [prepared(i) for i in seeds]
+    for s in same:
+        for _ in range(rounds):
+            calls(s)
+    backend.synchronize()
+    graphs, streams = [], []
+    for s in problems:
+        graphs.append(capture(rt, backend.stream, lambda: calls(s)))
+        stream = C.c_void_p()
+        rt("cudaStreamCreateWithFlags", C.byref(stream), 1)
+        streams.append(stream)
+    for _ in range(rounds):
+        for graph, stream in zip(graphs, streams):
+            rt("cudaGraphLaunch", graph, stream)
+    for stream in streams:
+        rt("cudaStreamSynchronize", stream)
+    for s, w in zip(problems, same):
+        for k in ("out", "state", "states", "dx", "dgate", "dstate"):
+            assert np.array_equal(s[k].numpy(), w[k].numpy()), k
+    backend.synchronize()
+    for graph, stream in zip(graphs, streams):
+        rt("cudaGraphExecDestroy", graph)
+        rt("cudaStreamDestroy", stream)
+
+
 def test_two_threads_with_a_context_each():
     """Both begin at the same time; the bits are those of one after the other."""
     contexts = [B.Backend(0) for _ in range(2)]
