@@ -418,8 +418,10 @@ int b200_distill_loss_backward(b200_ctx* ctx, const b200_distill_args* args);
 
 /* A gated linear recurrence along a sequence, each channel by itself: h_t = a_t h_{t-1} + b_t, out_t = h_t, with
  *     B200_GATES_SIGMOID: a = sigmoid(gate), b = (1 - a) x        B200_GATES_EXP: a = exp(gate), b = x
- * A gate of -inf begins anew (a = 0).  Products of decays just below 1 keep their digits: 1 - a is carried where a is above a half.  A state that is infinite or no number
- * leaves none that is finite behind it in its channel. */
+ * A gate of -inf begins anew (a = 0).  Products of decays just below 1 keep their digits: 1 - a is carried where a is above a half.  A state in front, an input or an a (a gate
+ * of the kind exp above 88.7) that is infinite or no number leaves no state that is finite behind it in its channel; of a state that passes F32's range by itself and comes back
+ * nothing is said.  Kind exp: decays may multiply far beyond F32's range in either direction, as long as states and gradients stay within that of its normal numbers.  Kind
+ * sigmoid: where decays multiply to less than 2^-126, what they multiply may count as 0. */
 #define B200_GATES_SIGMOID 0
 #define B200_GATES_EXP 1
 #define B200_RECURRENCE_CHUNK 16

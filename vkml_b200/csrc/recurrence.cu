@@ -31,6 +31,12 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
     return y;
 }
 
+__device__ __forceinline__ float fast_root(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // A step's decay: -d where a = 1 - d is above a half (never 0: the sign tells), else a.
 constexpr float kHold = -0x1p-126f;  // h stays
 __device__ __forceinline__ bool keeps(float c) { return c < 0.f; }
@@ -57,6 +63,34 @@ __device__ __forceinline__ void apply_v(float (&h)[V], const float (&c)[V], cons
     add_v(more, h, t);
 #pragma unroll
     for (int e = 0; e < V; ++e) h[e] = keeps(c[e]) ? more[e] : t[e];
+}
+
+// e^x - 1 by its series, for x of (-0.69, 0] (the term left out is 2e-8 of it at its lower end); never 0.
+__device__ __forceinline__ bool in_series(float x) { return x <= 0.f && x > -0.6931f; }
+template <int V>
+__device__ __forceinline__ void series_of(const float (&x)[V], float (&s)[V]) {
+    float q[V], k[V];
+    auto constant = [&](float value) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) k[e] = value;
+    };
+    auto next = [&](float value) {
+        constant(value);
+        fma_v(s, x, s, k);
+    };
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 1.f / 362880.f;
+    next(1.f / 40320.f);
+    next(1.f / 5040.f);
+    next(1.f / 720.f);
+    next(1.f / 120.f);
+    next(1.f / 24.f);
+    next(1.f / 6.f);
+    next(0.5f);
+    mul_v(q, x, x);
+    constant(-0x1p-126f);
+    add_v(k, x, k);
+    fma_v(s, q, s, k);
 }
 
 // What gates do to a step: its decay c (as above), a, d = 1 - a, and b / x.
@@ -88,32 +122,11 @@ __device__ __forceinline__ void gates_of(const float (&gate)[V], float (&c)[V], 
             input[e] = d[e];
         }
     } else {
-        // e^x - 1 by its series down to -0.69 (the term left out is 2e-8 of it there), e^x itself beyond
-        float s[V], q[V], k[V];
-        auto constant = [&](float value) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) k[e] = value;
-        };
-        auto next = [&](float value) {
-            constant(value);
-            fma_v(s, gate, s, k);
-        };
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[e] = 1.f / 362880.f;
-        next(1.f / 40320.f);
-        next(1.f / 5040.f);
-        next(1.f / 720.f);
-        next(1.f / 120.f);
-        next(1.f / 24.f);
-        next(1.f / 6.f);
-        next(0.5f);
-        mul_v(q, gate, gate);
-        constant(-0x1p-126f);
-        add_v(k, gate, k);  // (never 0)
-        fma_v(s, q, s, k);
+        float s[V];
+        series_of(gate, s);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const bool near = gate[e] <= 0.f && gate[e] > -0.6931f;
+            const bool near = in_series(gate[e]);
             const float far = fast_exp2(gate[e] * kLog2e);
             c[e] = near ? s[e] : far;  // (a growing state: a itself, as below a half)
             a[e] = near ? 1.f + s[e] : far;
@@ -138,12 +151,17 @@ __device__ __forceinline__ void slopes(float c, float& gate, float& input, float
 
 // What a run of steps does to the state in front of it: h becomes a h + sum, as h + (sum - d h) where a is above a half.  The product of the a's is kept as such and as
 // d = 1 - a: either has digits that the other loses.
-template <int V>
+//
+// Kind exp: states may grow, and a product of growing decays leaves F32's range long before the state that it multiplies has to (128 steps of gates of 0.8 make 1e-30
+// to 3e14 by a product of 3e44).  Its root is kept in the product's place, which is in F32's range for every product that takes one number of normal size to another.
+template <int KIND, int V>
 struct Run {
-    float a[V], d[V], sum[V];
+    static constexpr bool kRoot = KIND == B200_GATES_EXP;
+    float a[V], d[V], sum[V];  // (kRoot: a is the root, but for its part `above`, the product of runs whose own is above a half)
+    float above[kRoot ? V : 1];
     __device__ __forceinline__ void begin() {
 #pragma unroll
-        for (int e = 0; e < V; ++e) a[e] = 1.f, d[e] = 0.f, sum[e] = 0.f;
+        for (int e = 0; e < V; ++e) a[e] = 1.f, d[e] = 0.f, sum[e] = 0.f, above[kRoot ? e : 0] = 1.f;
     }
     // A step behind this one.  (a's rounding counts within the run only.)
     __device__ __forceinline__ void decays(const float (&a1)[V], const float (&d1)[V]) {
@@ -151,25 +169,76 @@ struct Run {
         fma_v(d, a1, d, d1);
     }
     __device__ __forceinline__ void adds(const float (&a1)[V], const float (&b)[V]) { fma_v(sum, a1, sum, b); }
+    // Steps of the kind exp have the product of their a's by the sum of their gates: that of one step.
+    __device__ __forceinline__ void decays_of_sum(const float (&gate)[V]) {
+        float s[V];
+        series_of(gate, s);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            d[e] = in_series(gate[e]) ? -s[e] : NAN;  // (of no use where a is below a half)
+            a[e] = fast_exp2(gate[e] * (0.5f * kLog2e));
+        }
+        stay_finite();
+    }
     // Another run behind this one, by its decay and sum.
     __device__ __forceinline__ void then(const float (&c)[V], const float (&s)[V]) {
         float a1[V], d1[V];
+        if constexpr (kRoot) {
+            // (d is for runs that keep: one of them that does not leaves the product below a half, or it may rise and fall, and 1 less that has no digits)
+            // (What does not depend on what is in front comes first: of the sums a product and a multiply-add follow one another.)
+            float first[V], second[V], kept[V], half[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            a1[e] = keeps(c[e]) ? 1.f + c[e] : c[e];
-            d1[e] = keeps(c[e]) ? -c[e] : 1.f - c[e];
+            for (int e = 0; e < V; ++e) {
+                const bool near = keeps(c[e]);
+                a1[e] = 1.f + c[e], d1[e] = -c[e];
+                first[e] = near ? 1.f : c[e];
+                second[e] = near ? a1[e] : c[e];
+                half[e] = near ? a1[e] : 1.f;
+                kept[e] = near ? a1[e] : NAN;
+            }
+            mul_v(a, a, first);
+            mul_v(first, first, sum);
+            fma_v(sum, second, first, s);
+            mul_v(above, above, half);
+            fma_v(d, kept, d, d1);
+            stay_finite();
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                a1[e] = keeps(c[e]) ? 1.f + c[e] : c[e];
+                d1[e] = keeps(c[e]) ? -c[e] : 1.f - c[e];
+            }
+            adds(a1, s);
+            decays(a1, d1);
         }
-        adds(a1, s);
-        decays(a1, d1);
-        stay_finite();
     }
-    // (Sixteen growing steps may have a product beyond F32's range, and no state to grow: not a number would come of it.)
+    // (A product beyond even that has no state to grow but zero: not a number would come of an infinite one.)
     __device__ __forceinline__ void stay_finite() {
 #pragma unroll
         for (int e = 0; e < V; ++e) asm("min.NaN.f32 %0, %1, %2;" : "=f"(a[e]) : "f"(a[e]), "f"(3.4e38f));
     }
-    __device__ __forceinline__ float decay(int e) const { return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : a[e]; }
+    // As keeps() has it, but for a root where kRoot.
+    __device__ __forceinline__ float decay(int e) const {
+        float rest = a[e];
+        if constexpr (kRoot) rest *= fast_root(above[e]);
+        return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : rest;
+    }
 };
+// h behind a run, by its decay and sum.
+template <int KIND, int V>
+__device__ __forceinline__ void apply_run(float (&h)[V], const float (&c)[V], const float (&sum)[V]) {
+    if constexpr (KIND == B200_GATES_EXP) {
+        float t[V], less[V], grown[V], more[V];
+        mul_v(t, c, h);
+        fma_v(grown, t, c, sum);
+        fma_v(less, c, h, sum);
+        add_v(more, h, less);
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[e] = keeps(c[e]) ? more[e] : grown[e];
+    } else {
+        apply_v(h, c, sum);
+    }
+}
 struct Stream {
     char* base;
     int64_t batch, step;  // bytes
@@ -393,12 +462,12 @@ __device__ __forceinline__ void get_row(float (&x)[VEC], const float* from, int 
 template <int VEC>
 __device__ __forceinline__ void put_row(float* to, int lane, const float (&x)[VEC]) { Raw<float, VEC>::store(reinterpret_cast<char*>(to + lane * VEC), x); }
 // h behind a segment or a block.
-template <int VEC>
+template <int KIND, int VEC>
 __device__ __forceinline__ void pass(float (&h)[VEC], const float* run, int lane) {
     float c[VEC], sum[VEC];
     get_row<VEC>(c, run, lane);
     get_row<VEC>(sum, run + 32 * VEC, lane);
-    apply_v(h, c, sum);
+    apply_run<KIND>(h, c, sum);
 }
 
 // Stores to another block of the cluster that its barrier counts.  (A cluster barrier would order them too, but waits for every store of the block before it.)
@@ -454,8 +523,8 @@ __device__ __forceinline__ void end_cluster() {
 
 // The state that comes into this warp's steps.  Segments come one after another, in the order of their warps and blocks, or (BACK) the other way round.  `window` counts from 0.
 // In front of window 0 the first warp has put the state to told.front[0]; behind the last one the last warp's `next` is the state there (of a cluster: everyone's).
-template <int VEC, bool BACK>
-__device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int warp, int lane, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<VEC>& own, float (&in)[VEC],
+template <int KIND, int VEC, bool BACK>
+__device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int warp, int lane, uint32_t rank, uint32_t cluster, uint32_t* status, const Run<KIND, VEC>& own, float (&in)[VEC],
                                      float (&next)[VEC]) {
     const uint32_t parity = window & 1;
     const int warps = told.warps;
@@ -471,7 +540,7 @@ __device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int
     } else {
         const uint32_t bar = shared_address(&told.bars[parity]);
         // What the segments in front of this one do, while the cluster's blocks tell each other; and what all do, by the last one.
-        Run<VEC> before;
+        Run<KIND, VEC> before;
         before.begin();
         auto take = [&](int i) {
             const float* const segment = told.segment(parity, BACK ? warps - 1 - i : i);
@@ -487,7 +556,7 @@ __device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int
         for (int i = kWarps - 1; i < mine; ++i) take(i);
         if (mine == warps - 1) {
             if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
-            Run<VEC> all = before;
+            Run<KIND, VEC> all = before;
             all.then(decay, own.sum);
             float c[VEC];
 #pragma unroll
@@ -506,34 +575,34 @@ __device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) in[e] = next[e];
             }
-            if (j < cluster) pass<VEC>(next, told.block(parity, BACK ? cluster - 1 - j : j), lane);
+            if (j < cluster) pass<KIND, VEC>(next, told.block(parity, BACK ? cluster - 1 - j : j), lane);
         }
         float c[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) c[e] = before.decay(e);
-        apply_v(in, c, before.sum);
+        apply_run<KIND>(in, c, before.sum);
         return;
     }
-    for (int i = 0; i < mine; ++i) pass<VEC>(in, told.segment(parity, BACK ? warps - 1 - i : i), lane);
+    for (int i = 0; i < mine; ++i) pass<KIND, VEC>(in, told.segment(parity, BACK ? warps - 1 - i : i), lane);
     if (mine == warps - 1) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) next[e] = in[e];
-        apply_v(next, decay, own.sum);
+        apply_run<KIND>(next, decay, own.sum);
         put_row<VEC>(told.front(parity ^ 1), lane, next);
     }
 }
 
 // What a block's segments do to a state, told to the cluster: this warp's, and beside it (decay, sum) what those in front of it do.  Segments come in the order of their
 // warps and blocks, or (BACK) the other way round.
-template <bool BACK>
-__device__ __forceinline__ void tell_ahead(const Told<1>& told, uint32_t parity, uint32_t slot, int warp, int lane, uint32_t rank, uint32_t cluster, const Run<1>& own, float (&decay)[1], float (&sum)[1]) {
+template <int KIND, bool BACK>
+__device__ __forceinline__ void tell_ahead(const Told<1>& told, uint32_t parity, uint32_t slot, int warp, int lane, uint32_t rank, uint32_t cluster, const Run<KIND, 1>& own, float (&decay)[1], float (&sum)[1]) {
     const int warps = told.warps;
     const float mine[1] = {own.decay(0)};
     put_row<1>(told.segment(parity, warp), lane, mine);
     put_row<1>(told.segment(parity, warp) + 32, lane, own.sum);
     __syncthreads();
     const int in_front = BACK ? warps - 1 - warp : warp;
-    Run<1> before;
+    Run<KIND, 1> before;
     before.begin();
     auto take = [&](int i) {
         const float* const segment = told.segment(parity, BACK ? warps - 1 - i : i);
@@ -560,7 +629,7 @@ __device__ __forceinline__ void tell_ahead(const Told<1>& told, uint32_t parity,
     }
 }
 // The state that comes into this warp's steps of window w, and `carry`, the state behind the window before it and then behind this one.
-template <bool BACK>
+template <int KIND, bool BACK>
 __device__ __forceinline__ void hear_ahead(const Told<1>& told, uint32_t w, int lane, uint32_t rank, uint32_t cluster, uint32_t* status, const float (&decay)[1], const float (&sum)[1], float (&carry)[1],
                                            float (&in)[1]) {
     const uint32_t slot = w % kAheadSlots, ahead = BACK ? cluster - 1 - rank : rank;
@@ -568,9 +637,9 @@ __device__ __forceinline__ void hear_ahead(const Told<1>& told, uint32_t w, int 
 #pragma unroll
     for (uint32_t j = 0; j < kMostCluster; ++j) {
         if (j == ahead) in[0] = carry[0];
-        if (j < cluster) pass<1>(carry, told.block(slot, BACK ? cluster - 1 - j : j), lane);
+        if (j < cluster) pass<KIND, 1>(carry, told.block(slot, BACK ? cluster - 1 - j : j), lane);
     }
-    apply_v(in, decay, sum);
+    apply_run<KIND>(in, decay, sum);
 }
 
 // Where a thread works: its sequence, channels, and place in a window.
@@ -727,7 +796,7 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 
 // The first walk through a window's steps, of which `left` are the sequence's: what they do to a state, by themselves and all together.
 template <int KIND, int VEC, typename X, typename Y>
-__device__ __forceinline__ void take_steps(const X& x, const Y& gate, int lane, int left, float (&a)[kSteps][VEC], float (&b)[kSteps][VEC], Run<VEC>& own) {
+__device__ __forceinline__ void take_steps(const X& x, const Y& gate, int lane, int left, float (&a)[kSteps][VEC], float (&b)[kSteps][VEC], Run<KIND, VEC>& own) {
     own.begin();
     float gate_sum[VEC];
 #pragma unroll
@@ -751,11 +820,7 @@ __device__ __forceinline__ void take_steps(const X& x, const Y& gate, int lane, 
     };
     if (left == kSteps) take(std::true_type{});
     else take(std::false_type{});
-    if constexpr (KIND == B200_GATES_EXP) {  // the product of the a's is that of one step whose gate is the sum
-        float unused[2][VEC];
-        gates_of<KIND>(gate_sum, unused[0], own.a, own.d, unused[1]);
-        own.stay_finite();
-    }
+    if constexpr (KIND == B200_GATES_EXP) own.decays_of_sum(gate_sum);
 }
 // The second one, from the state h in front of them, to `rows` rows of the result.
 template <int VEC, typename X>
@@ -830,11 +895,11 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
         if (read == end) read = places;
         load();  // (where the window before lay)
         float a[kSteps][VEC], b[kSteps][VEC];
-        Run<VEC> own;
+        Run<KIND, VEC> own;
         const int left = t < n ? static_cast<int>(min(n - t, uint32_t(kSteps))) : 0;  // steps of the sequence
         take_steps<KIND, VEC>(x, gate, at.lane, left, a, b, own);
         float h[VEC];
-        join<VEC, false>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, h, carry);
+        join<KIND, VEC, false>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, h, carry);
         if (t >= length) continue;
         if (k.states != nullptr && at.in) Raw<float, VEC>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
@@ -907,9 +972,9 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, f
         if (read == end) read = places;
         next.left = t_first < n ? static_cast<int>(min(n - t_first, uint32_t(kSteps))) : 0;
         t_first += span;
-        Run<1> own;
+        Run<KIND, 1> own;
         take_steps<KIND, 1>(x, gate, at.lane, next.left, next.a, next.b, own);
-        tell_ahead<false>(told, w & 1, w % kAheadSlots, at.warp, at.lane, at.rank, cluster, own, next.decay, next.sum);
+        tell_ahead<KIND, false>(told, w & 1, w % kAheadSlots, at.warp, at.lane, at.rank, cluster, own, next.decay, next.sum);
     };
     first(0);
     uint32_t t = at.first();
@@ -917,7 +982,7 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, f
         const Window now = next;
         if (w + 1 < windows) first(w + 1);
         float h[1];
-        hear_ahead<false>(told, w, at.lane, at.rank, cluster, k.status, now.decay, now.sum, carry, h);
+        hear_ahead<KIND, false>(told, w, at.lane, at.rank, cluster, k.status, now.decay, now.sum, carry, h);
         if (t >= length) continue;
         if (k.states != nullptr && at.in) Raw<float, 1>::store(reinterpret_cast<char*>(k.states + (int64_t(at.b) * k.chunks + t / kSteps) * k.width + at.ch), h);
         x.place = now.place;
@@ -940,15 +1005,17 @@ __device__ __forceinline__ void step_gradient(const X& dout, bool with_dout, int
 // The first walk through a window's steps, from the state h in front of them: their decays, what dgate takes of them, and what they do to a gradient that comes from behind.
 template <int KIND, int VEC, typename X, typename Y>
 __device__ __forceinline__ void take_back_steps(const X& x, const Y& gate, const X& dout, bool with_dout, int lane, int left, float (&h)[VEC], float (&c)[kSteps][VEC], float (&u)[kSteps][VEC],
-                                                Run<VEC>& own) {
+                                                Run<KIND, VEC>& own) {
     own.begin();
+    float gate_sum[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) gate_sum[e] = 0.f;
     auto take = [&](auto whole) {
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-            float xs[VEC], gs[VEC], ds[VEC], a[VEC], d[VEC], input[VEC], b[VEC];
+            float xs[VEC], gs[VEC], a[VEC], d[VEC], input[VEC], b[VEC];
             x.get(j, lane).get(xs);
             gate.get(j, lane).get(gs);
-            step_gradient<VEC>(dout, with_dout, lane, left, j, ds);
             if (!whole.value && j >= left) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) gs[e] = KIND == B200_GATES_SIGMOID ? INFINITY : 0.f, xs[e] = 0.f;
@@ -957,14 +1024,31 @@ __device__ __forceinline__ void take_back_steps(const X& x, const Y& gate, const
 #pragma unroll
             for (int e = 0; e < VEC; ++e) u[j][e] = KIND == B200_GATES_SIGMOID ? h[e] - xs[e] : h[e];
             mul_v(b, input, xs);
-            own.decays(a, d);
-            if constexpr (KIND == B200_GATES_EXP) own.stay_finite();
-            fma_v(own.sum, own.a, ds, own.sum);  // what the steps' gradients make of the state in front of them: each times the a's up to it
+            if constexpr (KIND == B200_GATES_SIGMOID) {  // what the steps' gradients make of the state in front of them: each times the a's up to it
+                float ds[VEC];
+                own.decays(a, d);
+                step_gradient<VEC>(dout, with_dout, lane, left, j, ds);
+                fma_v(own.sum, own.a, ds, own.sum);
+            } else {
+                add_v(gate_sum, gate_sum, gs);
+            }
             fma_v(h, a, h, b);  // (a's rounding counts within these steps only, here and below)
         }
     };
     if (left == kSteps) take(std::true_type{});
     else take(std::false_type{});
+    if constexpr (KIND == B200_GATES_EXP) {  // (a product of the a's up to a step may be beyond F32, that step's gradient times it not)
+        own.decays_of_sum(gate_sum);
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            float ds[VEC], a[VEC], unused[2];
+            step_gradient<VEC>(dout, with_dout, lane, left, j, ds);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) slopes<KIND>(c[j][e], unused[0], unused[1], a[e]);
+            add_v(own.sum, own.sum, ds);
+            mul_v(own.sum, a, own.sum);
+        }
+    }
 }
 // The second one, from the gradient `later` behind them, to `rows` rows of the results.
 template <int KIND, int VEC, typename X, typename Y>
@@ -1071,11 +1155,11 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
         if (read == end) read = places;
         load();  // (where the window before lay)
         if (w + 1 < windows) load_state(t - span);
-        Run<VEC> own;
+        Run<KIND, VEC> own;
         const int left = t < n ? static_cast<int>(min(n - t, uint32_t(kSteps))) : 0;  // steps of the sequence
         take_back_steps<KIND, VEC>(x, gate, dout, with_dout, at.lane, left, h, c, u, own);
         float later[VEC];
-        join<VEC, true>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, later, carry);
+        join<KIND, VEC, true>(told, w, at.warp, at.lane, at.rank, at.cluster, k.status, own, later, carry);
         if (t < length) {
             const int rows = static_cast<int>(min(length - t, uint32_t(kSteps)));
             put_back_steps<KIND, VEC>(x, gate, dout, with_dout, at.lane, at.in, left, rows, dx, dgate, k.dx.step, k.dgate.step, with_dx, with_dgate, c, u, later);
@@ -1166,16 +1250,16 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, t
         next.left = t_first < n ? static_cast<int>(min(n - t_first, uint32_t(kSteps))) : 0;
         t_first -= span;
         if (w + 1 < windows) load_state(t_first);
-        Run<1> own;
+        Run<KIND, 1> own;
         take_back_steps<KIND, 1>(x, gate, dout, with_dout, at.lane, next.left, h, next.c, next.u, own);
-        tell_ahead<true>(told, w & 1, w % kAheadSlots, at.warp, at.lane, at.rank, cluster, own, next.decay, next.sum);
+        tell_ahead<KIND, true>(told, w & 1, w % kAheadSlots, at.warp, at.lane, at.rank, cluster, own, next.decay, next.sum);
     };
     first(0);
     for (uint32_t w = 0; w < windows; ++w, t -= span) {
         const Window now = next;
         if (w + 1 < windows) first(w + 1);
         float later[1];
-        hear_ahead<true>(told, w, at.lane, at.rank, cluster, k.status, now.decay, now.sum, carry, later);
+        hear_ahead<KIND, true>(told, w, at.lane, at.rank, cluster, k.status, now.decay, now.sum, carry, later);
         if (t < length) {
             look(now.place);
             put_back_steps<KIND, 1>(x, gate, dout, with_dout, at.lane, at.in, now.left, static_cast<int>(min(length - t, uint32_t(kSteps))), dx, dgate, k.dx.step, k.dgate.step, with_dx, with_dgate, now.c,
