@@ -319,7 +319,8 @@ __global__ void __launch_bounds__(kThreads) serial_kernel(const Args k) {
     const int ch = (blockIdx.x * kThreads + threadIdx.x) * VEC;
     if (ch >= k.width) return;
     const int length = static_cast<int>(k.length);
-    for (int b = blockIdx.y; b < k.batch; b += gridDim.y) {
+    for (uint32_t i = blockIdx.y; i < static_cast<uint32_t>(k.batch); i += gridDim.y) {  // (what is behind the last of 2^31 - 1 sequences has 32 bits)
+        const int b = static_cast<int>(i);
         const int n = static_cast<int>(steps_of(k, b));
         const char *x = k.x.base + b * k.x.batch + ch * int64_t(sizeof(T)), *gate = k.gate.base + b * k.gate.batch + ch * int64_t(sizeof(G));
         char* out = k.out.base + b * k.out.batch + ch * int64_t(sizeof(T));
@@ -367,7 +368,8 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
     const int ch = (blockIdx.x * kThreads + threadIdx.x) * VEC;
     if (ch >= k.width) return;
     const int length = static_cast<int>(k.length);
-    for (int b = blockIdx.y; b < k.batch; b += gridDim.y) {
+    for (uint32_t i = blockIdx.y; i < static_cast<uint32_t>(k.batch); i += gridDim.y) {  // (what is behind the last of 2^31 - 1 sequences has 32 bits)
+        const int b = static_cast<int>(i);
         const int n = static_cast<int>(steps_of(k, b));
         const char *x = k.x.base + b * k.x.batch + ch * int64_t(sizeof(T)), *gate = k.gate.base + b * k.gate.batch + ch * int64_t(sizeof(G));
         const char* dout = k.dout.base != nullptr ? k.dout.base + b * k.dout.batch + ch * int64_t(sizeof(T)) : nullptr;
