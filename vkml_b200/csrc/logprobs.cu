@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, threads_on_sm(THREADS) / THREADS) log
         // an element of the row's ends for some threads
         int end = -1;
         if (rank == 0 && tid < row.head) end = tid;
-        else if (rank + 1 == blocks && tid >= 8 && row.tail + (tid - 8) < k.vocab) end = row.tail + (tid - 8);
+        else if (rank + 1 == blocks && tid >= 8 && tid - 8 < k.vocab - row.tail) end = row.tail + (tid - 8);
         const T end_element = end >= 0 ? row.z[end] : from_float<T>(0.f);
         float token_z = 0.f;
         bool token = false;
