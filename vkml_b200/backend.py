@@ -270,7 +270,8 @@ class Backend:
 
     def adamw(self, tensors, *, lr, step, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale=1.0,
               seed: int = 0) -> None:
-        """One AdamW step over all tensors: a sequence of AdamWTensor, or what adamw_table() made of one, once for all steps.  States in
+        """One AdamW step over all tensors: a sequence of AdamWTensor, or what adamw_table() made of one, once for all steps (a sequence is
+        described anew in every call, some 3 us a tensor, which for a small model is more than the step itself).  States in
         F32, or in 8 bits with a scale to 256 elements, rounded up or down by bits of seed and step.  lr, step (from 1 on) and grad_scale are
         numbers, or one-element tensors on the device (F32, I64, F32) for a step that is captured once: where grad_scale is not finite there,
         or step below 1, nothing changes."""

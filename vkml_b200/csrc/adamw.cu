@@ -5,7 +5,7 @@
 // Bound by memory: 28 bytes to an element with everything in F32, 14 to 18 with 8-bit states.  The tensors' addresses travel in the launch's parameters, some
 // hundreds at a time, so that a step over all of a model's tensors is one launch and uploads nothing.  A warp takes 256 elements, which are a block of 8-bit
 // states: their largest is a reduction in the warp, and a state is read, updated, scaled and written without leaving its registers.  176 M parameters in F32: 720 us, 6.8
-// TB/s; 118 M with 8-bit states, F16 gradients and F16 copies: 330 us, 5.8 TB/s, where the instructions of a state's rounding are what is left.
+// TB/s; 118 M with 8-bit states, F16 gradients and F16 copies: 328 to 347 us, 5.5 to 5.8 TB/s, where the instructions of a state's rounding are what is left.
 //
 // An 8-bit state's change in a step is mostly smaller than half a step of its byte (v moves by a thousandth, a byte's step is 6 to 12 %): rounded to the nearest,
 // it would stay where it is.  Each is rounded up or down by random bits instead, whose mean is what was computed.  The root of v is what is kept: it has half
@@ -508,7 +508,8 @@ void launch_adamw(b200_ctx* ctx, const b200_adamw_args& a) {
     }
     wait_for_tensors(ctx, {&a.lr_on_device, &a.step_on_device, &a.scale_on_device});
     ProfScope scope(ctx, "adamw");
-    // As many rounds to a block as leave two waves of blocks; one where there is little to do.
+    // As many rounds to a block as leave 6 blocks for each SM: two waves of the three with 8-bit states that an SM holds, one and a half of the four without (until the most
+    // rounds are reached: a large model has more of them); one round where there is little to do.
     int64_t all = 0;
     for (const Tensor& t : tensors) all += ceil_div(t.n, kRound);
     const bool any_bytes = std::any_of(tensors.begin(), tensors.end(), [](const Tensor& t) { return t.scales != nullptr; });

@@ -8,7 +8,7 @@
 // Bound by memory: z read once, and backward as much written.  A block takes a row after another: each thread keeps the maximum of what it has read and the sums of
 // e^u and e^u u beside it, and the block joins these threes.  What comes next, of this row or the next one, is on its way into registers all the while, so that a
 // row's end holds up nothing that is read.  (Through shared memory, by asynchronous copies, a row's end cost more than the registers do: 4096 x 32000 F16 95 us in place
-// of 53.)  Few long rows are a cluster's each, whose blocks take a part of it.  2047 x 128000 F32: 154 us, 6.8 TB/s; 4096 x 32000 F16: 53 us, 4.9 TB/s, bound by the
+// of 53.)  Few long rows are a cluster's each, whose blocks take a part of it.  2047 x 128000 F32: 151 to 159 us, 6.6 to 6.9 TB/s; 4096 x 32000 F16: 53 to 55 us, 4.8 to 4.9 TB/s, bound by the
 // exponential, the two sums and the conversion of each element.
 //
 // The K largest cost no second pass.  Some K threads' maxima are K elements, so that the K-th largest of all threads' maxima is a bound that K elements at least

@@ -432,8 +432,10 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
 // other's, and every thread goes through its steps again from the state that does come in.  All of it stays in registers: gates and inputs are read once, and the
 // next window's are under way while this one is computed.
 //
-// 8 sequences of 4096 steps, 2048 channels, F16: 84 us (5.0 TB/s), gradient 142 us (4.8 TB/s); instructions bound it (two gates, two walks through the steps and the
-// conversions of F16: 74 us with the loads left out), and 256 blocks on 296 places.  50000 steps of 1000 channels, F32: 151 us (4.1 TB/s), a cluster's meeting in each of 49 windows.
+// 8 sequences of 4096 steps, 2048 channels, F16: 82 to 86 us (5.0 TB/s), gradient 141 to 147 us (4.8 TB/s).  Neither memory nor the issue slots are full (56 and 65 % of them where an SM has
+// work, at the 16 warps that its registers hold): steps follow one another in both walks, results wait for gates' functions, warps for the block's meeting in each window; and 256 blocks on 296 places
+// leave 40 SMs with one block where the others have two.  The same in F32: 143 to 146 us (5.7 TB/s), gradient 240 to 257.  50000 steps of 1000 channels, F32, kind exp: 155 us (3.9 TB/s), a cluster's
+// meeting in each of 49 windows.
 
 constexpr int kWarps = 8;        // of a block, two of which an SM holds
 constexpr int kMostWarps = 16;   // of one that has an SM to itself
@@ -914,7 +916,7 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
 // Clusters whose lanes have a channel each: what a window's segments do to a state is told a window ahead, so that the wait for the other blocks is one for what was sent
 // while this window was gone through the first time.  (Two windows' steps in registers, and four places to be told at: a block that is told of the fourth window from here has
 // told this one's cluster of the second, behind its reading of this one.)  For halves: 32768 steps of 1024 channels 80 us, 103 with a wait in every window.  In F32 its
-// second window in registers costs what it saves (50000 steps of 1000 channels 160 us, 150 without).
+// second window in registers costs what it saves (50000 steps of 1000 channels 160 us where it was 150 without).
 template <typename T, typename G, int KIND, int CHUNK>
 __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, false>) == 2 ? kMostWarps : kWarps), 1) walk_ahead_kernel(const Args k, uint32_t strips, uint32_t cluster) {
     constexpr int kBytes = kWindowBytes<T, G, 1, CHUNK, false>, kStages = stages_of(kBytes);
@@ -1430,7 +1432,7 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
     if (s.length <= kSteps) return w;
     w.warps = static_cast<int>(std::min<int64_t>(kWarps, ceil_div(s.length, kSteps)));
     // Blocks that leave half of the device's places (two to an SM) empty share their sequences' windows with another one each: 50000 steps of 1000 channels, F32, 423 us with
-    // blocks by themselves, 313, 188 and 151 by clusters of 2, 4 and 8; 4 sequences of 4096 steps, 2048 channels, F16, 74 and, by two, 56.  Further apart than that a
+    // blocks by themselves, 313, 188 and 151 by clusters of 2, 4 and 8 (155 since products are kept as roots); 4 sequences of 4096 steps, 2048 channels, F16, 74 and, by two, 56.  Further apart than that a
     // cluster costs more than it gives: 8 such sequences 84 us by themselves, 106 by two, 111 by four.
     auto spread = [&]() {
         w.strips = ceil_div(s.width, 32 * w.vec);
