@@ -59,9 +59,9 @@ def waves(shape, period, swing, rng):
 
 
 @pytest.mark.parametrize("shape", SHAPES)
-@pytest.mark.parametrize("period,swing", [(32, 150.0), (300, 150.0), (512, 120.0)])
+@pytest.mark.parametrize("period,swing", [(32, 150.0), (300, 150.0), (512, 120.0), (64, 40.0), (700, 6.0)])
 def test_states_that_rise_and_fall(backend, shape, period, swing):
-    """States from 1e-33 to 1e32 and back, gradients the other way round: inputs and gradients of a step are a part of what it has."""
+    """States from 1e-33 to 1e32 and back (or less far), gradients the other way round: inputs and gradients of a step are a part of what it has."""
     rng = np.random.default_rng(period + shape[1])
     gate, level = waves(shape, period, swing, rng)
     size = np.exp(level - swing / 2)

@@ -65,7 +65,7 @@ __device__ __forceinline__ void apply_v(float (&h)[V], const float (&c)[V], cons
     for (int e = 0; e < V; ++e) h[e] = keeps(c[e]) ? more[e] : t[e];
 }
 
-// e^x - 1 by its series, for x of (-0.69, 0] (the term left out is 2e-8 of it at its lower end); never 0.
+// e^x - 1 by its series, for x of (-0.69, 0.17) (the term left out is 2e-8 of it at the lower end); never 0 where x is not above 0, which is where steps use it.
 __device__ __forceinline__ bool in_series(float x) { return x <= 0.f && x > -0.6931f; }
 template <int V>
 __device__ __forceinline__ void series_of(const float (&x)[V], float (&s)[V]) {
@@ -150,18 +150,22 @@ __device__ __forceinline__ void slopes(float c, float& gate, float& input, float
 }
 
 // What a run of steps does to the state in front of it: h becomes a h + sum, as h + (sum - d h) where a is above a half.  The product of the a's is kept as such and as
-// d = 1 - a: either has digits that the other loses.
+// d = 1 - a: either has digits that the other loses.  A run tells its decay as a step does.
 //
 // Kind exp: states may grow, and a product of growing decays leaves F32's range long before the state that it multiplies has to (128 steps of gates of 0.8 make 1e-30
-// to 3e14 by a product of 3e44).  Its root is kept in the product's place, which is in F32's range for every product that takes one number of normal size to another.
+// to 3e14 by a product of 3e44).  What a run tells is -d where a is above a half and not above 1, -a up to 1.19, and beyond these a's root, which is in F32's range for every
+// product that takes one number of normal size to another.  (Where decays fall and then rise d has no digits left: sixteen runs that grow by 1.19 at most multiply its rounding by 16 at most.)
+constexpr float kMild = 0.19f;
+__device__ __forceinline__ bool is_root(float c) { return !(c < 0.f); }
+__device__ __forceinline__ bool grows(float c) { return c < -0.75f; }
 template <int KIND, int V>
 struct Run {
     static constexpr bool kRoot = KIND == B200_GATES_EXP;
-    float a[V], d[V], sum[V];  // (kRoot: a is the root, but for its part `above`, the product of runs whose own is above a half)
-    float above[kRoot ? V : 1];
+    float a[V], d[V], sum[V];   // (kRoot: a is the root, but for `near`; d is no number where a part tells a root)
+    float near[kRoot ? V : 1];  // the product of the parts that do not
     __device__ __forceinline__ void begin() {
 #pragma unroll
-        for (int e = 0; e < V; ++e) a[e] = 1.f, d[e] = 0.f, sum[e] = 0.f, above[kRoot ? e : 0] = 1.f;
+        for (int e = 0; e < V; ++e) a[e] = 1.f, d[e] = 0.f, sum[e] = 0.f, near[kRoot ? e : 0] = 1.f;
     }
     // A step behind this one.  (a's rounding counts within the run only.)
     __device__ __forceinline__ void decays(const float (&a1)[V], const float (&d1)[V]) {
@@ -175,7 +179,7 @@ struct Run {
         series_of(gate, s);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            d[e] = in_series(gate[e]) ? -s[e] : NAN;  // (of no use where a is below a half)
+            d[e] = gate[e] < 0.17f && gate[e] > -0.6931f ? -s[e] : NAN;  // (up to kMild)
             a[e] = fast_exp2(gate[e] * (0.5f * kLog2e));
         }
         stay_finite();
@@ -184,22 +188,22 @@ struct Run {
     __device__ __forceinline__ void then(const float (&c)[V], const float (&s)[V]) {
         float a1[V], d1[V];
         if constexpr (kRoot) {
-            // (d is for runs that keep: one of them that does not leaves the product below a half, or it may rise and fall, and 1 less that has no digits)
             // (What does not depend on what is in front comes first: of the sums a product and a multiply-add follow one another.)
-            float first[V], second[V], kept[V], half[V];
+            float first[V], second[V], factor[V], kept[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const bool near = keeps(c[e]);
-                a1[e] = 1.f + c[e], d1[e] = -c[e];
-                first[e] = near ? 1.f : c[e];
-                second[e] = near ? a1[e] : c[e];
-                half[e] = near ? a1[e] : 1.f;
-                kept[e] = near ? a1[e] : NAN;
+                const bool root = is_root(c[e]);
+                a1[e] = grows(c[e]) ? -c[e] : 1.f + c[e];
+                d1[e] = grows(c[e]) ? 1.f + c[e] : -c[e];
+                first[e] = root ? c[e] : 1.f;
+                second[e] = root ? c[e] : a1[e];
+                factor[e] = root ? 1.f : a1[e];
+                kept[e] = root ? NAN : a1[e];
             }
             mul_v(a, a, first);
             mul_v(first, first, sum);
             fma_v(sum, second, first, s);
-            mul_v(above, above, half);
+            mul_v(near, near, factor);
             fma_v(d, kept, d, d1);
             stay_finite();
         } else {
@@ -217,24 +221,29 @@ struct Run {
 #pragma unroll
         for (int e = 0; e < V; ++e) asm("min.NaN.f32 %0, %1, %2;" : "=f"(a[e]) : "f"(a[e]), "f"(3.4e38f));
     }
-    // As keeps() has it, but for a root where kRoot.
+    // What the run tells.
     __device__ __forceinline__ float decay(int e) const {
-        float rest = a[e];
-        if constexpr (kRoot) rest *= fast_root(above[e]);
-        return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : rest;
+        if constexpr (kRoot) {
+            const float mild = d[e] >= 0.f ? fminf(-d[e], kHold) : d[e] - 1.f;
+            return d[e] > -kMild && d[e] < 0.5f ? mild : a[e] * fast_root(near[e]);
+        } else {
+            return d[e] >= 0.f && d[e] < 0.5f ? fminf(-d[e], kHold) : a[e];
+        }
     }
 };
-// h behind a run, by its decay and sum.
+// h behind a run, by what it tells and its sum.
 template <int KIND, int V>
 __device__ __forceinline__ void apply_run(float (&h)[V], const float (&c)[V], const float (&sum)[V]) {
     if constexpr (KIND == B200_GATES_EXP) {
-        float t[V], less[V], grown[V], more[V];
+        float t[V], less[V], far[V], more[V];
         mul_v(t, c, h);
-        fma_v(grown, t, c, sum);
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[e] = is_root(c[e]) ? t[e] : -h[e];
+        fma_v(far, t, c, sum);
         fma_v(less, c, h, sum);
         add_v(more, h, less);
 #pragma unroll
-        for (int e = 0; e < V; ++e) h[e] = keeps(c[e]) ? more[e] : grown[e];
+        for (int e = 0; e < V; ++e) h[e] = is_root(c[e]) || grows(c[e]) ? far[e] : more[e];
     } else {
         apply_v(h, c, sum);
     }
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(kThreads) serial_backward_kernel(const Args k)
 //
 // 8 sequences of 4096 steps, 2048 channels, F16: 82 to 86 us (5.0 TB/s), gradient 141 to 147 us (4.8 TB/s).  Neither memory nor the issue slots are full (56 and 65 % of them where an SM has
 // work, at the 16 warps that its registers hold): steps follow one another in both walks, results wait for gates' functions, warps for the block's meeting in each window; and 256 blocks on 296 places
-// leave 40 SMs with one block where the others have two.  The same in F32: 143 to 146 us (5.7 TB/s), gradient 240 to 257.  50000 steps of 1000 channels, F32, kind exp: 155 us (3.9 TB/s), a cluster's
+// leave 40 SMs with one block where the others have two.  The same in F32: 143 to 146 us (5.7 TB/s), gradient 240 to 257.  50000 steps of 1000 channels, F32, kind exp: 152 to 154 us (4.0 TB/s), a cluster's
 // meeting in each of 49 windows.
 
 constexpr int kWarps = 8;        // of a block, two of which an SM holds
@@ -472,6 +481,33 @@ __device__ __forceinline__ void pass(float (&h)[VEC], const float* run, int lane
     get_row<VEC>(c, run, lane);
     get_row<VEC>(sum, run + 32 * VEC, lane);
     apply_run<KIND>(h, c, sum);
+}
+
+// h behind a cluster's blocks, and the state in front of the one that has `ahead` of them in front of it.  Kind exp: each is asked for while the one before it is passed, which takes longer
+// there (gradient of 4 sequences of 4096 steps, 2048 channels, F16: 92 us, 98 without; kind sigmoid, 50000 steps of 1000 channels, F32: 143 and 137).
+template <int KIND, int VEC, bool BACK>
+__device__ __forceinline__ void pass_blocks(const Told<VEC>& told, uint32_t slot, int lane, uint32_t cluster, uint32_t ahead, float (&h)[VEC], float (&in)[VEC]) {
+    constexpr bool kAsk = KIND == B200_GATES_EXP;
+    float c[2][VEC], sum[2][VEC];
+    auto ask = [&](uint32_t j) {
+        const float* const run = told.block(slot, BACK ? cluster - 1 - j : j);
+        get_row<VEC>(c[j % 2], run, lane);
+        get_row<VEC>(sum[j % 2], run + 32 * VEC, lane);
+    };
+    if (kAsk) ask(0);
+#pragma unroll
+    for (uint32_t j = 0; j < kMostCluster; ++j) {
+        if (kAsk && j >= cluster) break;
+        if (j == ahead) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) in[e] = h[e];
+        }
+        if (j < cluster) {
+            if (!kAsk) ask(j);
+            else if (j + 1 < cluster) ask(j + 1);
+            apply_run<KIND>(h, c[j % 2], sum[j % 2]);
+        }
+    }
 }
 
 // Stores to another block of the cluster that its barrier counts.  (A cluster barrier would order them too, but waits for every store of the block before it.)
@@ -546,18 +582,20 @@ __device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int
         // What the segments in front of this one do, while the cluster's blocks tell each other; and what all do, by the last one.
         Run<KIND, VEC> before;
         before.begin();
-        auto take = [&](int i) {
+        float c_next[VEC], sum_next[VEC];  // (asked for one segment ahead)
+        auto ask = [&](int i) {
             const float* const segment = told.segment(parity, BACK ? warps - 1 - i : i);
-            float c[VEC], sum[VEC];
-            get_row<VEC>(c, segment, lane);
-            get_row<VEC>(sum, segment + 32 * VEC, lane);
-            before.then(c, sum);
+            get_row<VEC>(c_next, segment, lane);
+            get_row<VEC>(sum_next, segment + 32 * VEC, lane);
         };
+        ask(0);
+        for (int i = 0; i < mine; ++i) {
+            float c[VEC], sum[VEC];
 #pragma unroll
-        for (int i = 0; i < kWarps - 1; ++i) {
-            if (i < mine) take(i);
+            for (int e = 0; e < VEC; ++e) c[e] = c_next[e], sum[e] = sum_next[e];
+            ask(i + 1);
+            before.then(c, sum);
         }
-        for (int i = kWarps - 1; i < mine; ++i) take(i);
         if (mine == warps - 1) {
             if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(cluster * 32u * VEC * 8u) : "memory");
             Run<KIND, VEC> all = before;
@@ -573,14 +611,7 @@ __device__ __forceinline__ void join(const Told<VEC>& told, uint32_t window, int
         }
         wait_for(bar, window >> 1 & 1, told.given_up, status);
         const uint32_t ahead = BACK ? cluster - 1 - rank : rank;
-#pragma unroll
-        for (uint32_t j = 0; j < kMostCluster; ++j) {
-            if (j == ahead) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) in[e] = next[e];
-            }
-            if (j < cluster) pass<KIND, VEC>(next, told.block(parity, BACK ? cluster - 1 - j : j), lane);
-        }
+        pass_blocks<KIND, VEC, BACK>(told, parity, lane, cluster, ahead, next, in);
         float c[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) c[e] = before.decay(e);
@@ -608,18 +639,18 @@ __device__ __forceinline__ void tell_ahead(const Told<1>& told, uint32_t parity,
     const int in_front = BACK ? warps - 1 - warp : warp;
     Run<KIND, 1> before;
     before.begin();
-    auto take = [&](int i) {
+    float c_next[1], sum_next[1];  // (asked for one segment ahead)
+    auto ask = [&](int i) {
         const float* const segment = told.segment(parity, BACK ? warps - 1 - i : i);
-        float c[1], s[1];
-        get_row<1>(c, segment, lane);
-        get_row<1>(s, segment + 32, lane);
-        before.then(c, s);
+        get_row<1>(c_next, segment, lane);
+        get_row<1>(sum_next, segment + 32, lane);
     };
-#pragma unroll
-    for (int i = 0; i < kWarps - 1; ++i) {
-        if (i < in_front) take(i);
+    ask(0);
+    for (int i = 0; i < in_front; ++i) {
+        const float c[1] = {c_next[0]}, s[1] = {sum_next[0]};
+        ask(i + 1);
+        before.then(c, s);
     }
-    for (int i = kWarps - 1; i < in_front; ++i) take(i);
     decay[0] = before.decay(0), sum[0] = before.sum[0];
     if (in_front != warps - 1) return;
     const uint32_t bar = shared_address(&told.bars[slot]);
@@ -638,11 +669,7 @@ __device__ __forceinline__ void hear_ahead(const Told<1>& told, uint32_t w, int 
                                            float (&in)[1]) {
     const uint32_t slot = w % kAheadSlots, ahead = BACK ? cluster - 1 - rank : rank;
     wait_for(shared_address(&told.bars[slot]), w / kAheadSlots & 1, told.given_up, status);
-#pragma unroll
-    for (uint32_t j = 0; j < kMostCluster; ++j) {
-        if (j == ahead) in[0] = carry[0];
-        if (j < cluster) pass<KIND, 1>(carry, told.block(slot, BACK ? cluster - 1 - j : j), lane);
-    }
+    pass_blocks<KIND, 1, BACK>(told, slot, lane, cluster, ahead, carry, in);
     apply_run<KIND>(in, decay, sum);
 }
 
@@ -915,7 +942,7 @@ __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, VEC, CHUNK,
 
 // Clusters whose lanes have a channel each: what a window's segments do to a state is told a window ahead, so that the wait for the other blocks is one for what was sent
 // while this window was gone through the first time.  (Two windows' steps in registers, and four places to be told at: a block that is told of the fourth window from here has
-// told this one's cluster of the second, behind its reading of this one.)  For halves: 32768 steps of 1024 channels 80 us, 103 with a wait in every window.  In F32 its
+// told this one's cluster of the second, behind its reading of this one.)  For halves: 32768 steps of 1024 channels 78 us (kind exp 92 to 94), 103 with a wait in every window.  In F32 its
 // second window in registers costs what it saves (50000 steps of 1000 channels 160 us where it was 150 without).
 template <typename T, typename G, int KIND, int CHUNK>
 __global__ void __launch_bounds__(32 * (blocks_of(kWindowBytes<T, G, 1, CHUNK, false>) == 2 ? kMostWarps : kWarps), 1) walk_ahead_kernel(const Args k, uint32_t strips, uint32_t cluster) {
@@ -1432,7 +1459,7 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
     if (s.length <= kSteps) return w;
     w.warps = static_cast<int>(std::min<int64_t>(kWarps, ceil_div(s.length, kSteps)));
     // Blocks that leave half of the device's places (two to an SM) empty share their sequences' windows with another one each: 50000 steps of 1000 channels, F32, 423 us with
-    // blocks by themselves, 313, 188 and 151 by clusters of 2, 4 and 8 (155 since products are kept as roots); 4 sequences of 4096 steps, 2048 channels, F16, 74 and, by two, 56.  Further apart than that a
+    // blocks by themselves, 313, 188 and 151 by clusters of 2, 4 and 8 (152 to 154 since products of growing decays are kept); 4 sequences of 4096 steps, 2048 channels, F16, 74 and, by two, 56.  Further apart than that a
     // cluster costs more than it gives: 8 such sequences 84 us by themselves, 106 by two, 111 by four.
     auto spread = [&]() {
         w.strips = ceil_div(s.width, 32 * w.vec);
@@ -1440,7 +1467,7 @@ Walk walk_of(const Shape& s, const Args& k, std::initializer_list<Typed> streams
         while (w.cluster < kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2 && s.length > int64_t(w.cluster) * w.warps * kSteps) w.cluster *= 2;
     };
     spread();
-    // Half empty still: a channel to a lane, twice the blocks (1 sequence of 32768 steps, 1024 channels, F16: 80 us, 113 with two; its gradient 128 and 184).  Where two to a lane
+    // Half empty still: a channel to a lane, twice the blocks (1 sequence of 32768 steps, 1024 channels, F16: 78 us, 113 with two; its gradient 124 and 184).  Where two to a lane
     // leave less empty they are the faster ones (1 and 2 of 4096 steps, 2048 channels: 20.6 and 33 us, 22.6 and 41 with one).
     if (w.vec == 2 && w.cluster == kMostCluster && s.batch * w.strips * w.cluster * 2 <= int64_t(sm_count()) * 2) {
         w.vec = 1;
